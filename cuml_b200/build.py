@@ -22,9 +22,14 @@ SOURCES = ["api.cu", "kernels.cu", "kernels_q_top6.cu", "kernels_q_plain6.cu", "
            "kernels_q_cat.cu", "kernels_q_generic.cu", "kernels_q_narrow.cu", "kernels_q_pair.cu",
            "kernels_q_leafg.cu", "kernels_q_vec.cu", "kernels_q_top_vec.cu", "kernels_q_top_out.cu",
            "kernels_sparse_c.cu",
-           "pack.cpp", "blocks.cpp"]
+           "pack.cpp", "blocks.cpp",
+           "distill_api.cu", "distill_top.cu", "distill_loss.cu"]
 HEADERS = ["each_tree.hpp", "forest.hpp", "host_pool.hpp", "kernels.hpp", "kernels_q.hpp", "device_common.cuh", "dense_q.cuh",
-           os.path.join("..", "..", "include", "b2fil.h")]
+           os.path.join("..", "..", "include", "b2fil.h"), "distill.hpp", "distill_common.cuh"]
+# sources that include none of the others' headers: they are compiled again for these alone
+OWN_HEADERS = {"distill_api.cu": ["distill.hpp", os.path.join("..", "..", "include", "b2fil.h")],
+               "distill_top.cu": ["distill.hpp", "distill_common.cuh"],
+               "distill_loss.cu": ["distill.hpp", "distill_common.cuh"]}
 
 
 # Native call path for torch tensors: a CPython module compiled against the installed torch, whose
@@ -63,6 +68,12 @@ def _newer(target: str, deps: list) -> bool:
         return False
     t = os.path.getmtime(target)
     return all((not os.path.exists(d)) or os.path.getmtime(d) <= t for d in deps)
+
+
+def _object_deps(src: str) -> list:
+    """Files that an object is older than when it has to be compiled again."""
+    headers = OWN_HEADERS.get(src, [h for h in HEADERS if h not in ("distill_common.cuh", "distill_linear.cuh")])
+    return [os.path.join(SRC, f) for f in [src] + headers] + [os.path.abspath(__file__)]
 
 
 def _lib_up_to_date() -> bool:
@@ -125,9 +136,12 @@ def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(obj_dir, exist_ok=True)
     base = [_nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
             "-Xcompiler", "-fPIC,-Wall", "-Xptxas", "-v"]
-    jobs = []
+    jobs, objects = [], []
     for src in SOURCES:
         obj = os.path.join(obj_dir, os.path.splitext(src)[0] + ".o")
+        objects.append(obj)
+        if not force and _newer(obj, _object_deps(src)):
+            continue
         cmd = base + ["-c", os.path.join(SRC, src), "-o", obj]
         out = open(obj + ".log", "w+")  # a file, not a pipe: nothing blocks while others run
         jobs.append((cmd, obj, subprocess.Popen(cmd, stdout=out, stderr=subprocess.STDOUT), out))
@@ -138,9 +152,11 @@ def build(force: bool = False, verbose: bool = False) -> str:
         log.append(" ".join(cmd) + "\n" + out.read())
         out.close()
         failed |= proc.returncode != 0
+        if proc.returncode != 0 and os.path.exists(obj):
+            os.remove(obj)  # of an earlier build
     if not failed:
         cmd = [_nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", LIB]
-        cmd += [obj for _, obj, _, _ in jobs]
+        cmd += objects
         proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
         log.append(" ".join(cmd) + "\n" + proc.stdout)
         failed = proc.returncode != 0

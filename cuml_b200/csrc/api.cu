@@ -17,6 +17,7 @@
 
 #include "forest.hpp"
 #include "host_pool.hpp"
+#include "distill.hpp"
 #include "kernels.hpp"
 #include "kernels_q.hpp"
 
@@ -870,6 +871,16 @@ class HostPrediction {
 };
 
 }  // namespace
+
+namespace b2fil {
+
+int report_error(int code, const char* text)
+{
+  return set_error(code, text);
+}
+void count_launches(int n) { g_launches += n; }
+
+}  // namespace b2fil
 
 extern "C" {
 

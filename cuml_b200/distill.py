@@ -1,0 +1,233 @@
+"""Distillation: a teacher's best scores, and losses that train a small network on them.
+
+A large forest can be compressed into a small network by training that on the forest's answers.
+These operators take a teacher's scores over classes (a forest's probabilities, or the logits of any other
+model), keep the `k` best classes of each row, and compute the loss of a student and its gradient:
+
+    top_scores                 the k best scores of each row, their classes, the row's log-sum-exp
+    distillation_loss          T^2 KL(teacher || student) from the student's logits
+    linear_cross_entropy       softmax cross entropy from the last linear layer, logits not kept
+    linear_distillation_loss   distillation_loss from the last linear layer, logits not kept
+
+`ForestInference.predict_top`, `.teach` and `.distillation_loss` call them with a forest as the teacher.
+All tensors are CUDA tensors of one device; work is enqueued on torch's current stream of that device and
+nothing waits.  The losses have first derivatives by the logits, or by the layer's input and weight; the
+teacher's values are constants.  All computation happens in libb2fil.so.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .fil import _lib
+
+MOST_TOP = 256  # largest k
+_TYPES = {torch.float32: 0, torch.float64: 1, torch.bfloat16: 2, torch.float16: 3}
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+_TAILS = ("renormalise", "bucket")
+_NO_CLASS = -(1 << 62)
+
+
+class TopScores(NamedTuple):
+    """The best scores of each row (see `top_scores`); `logsumexp` may be None."""
+    values: torch.Tensor
+    index: torch.Tensor
+    logsumexp: Optional[torch.Tensor]
+
+
+class CTeacher(C.Structure):
+    """`b2fil_teacher`."""
+    _fields_ = [("values", C.c_void_p), ("index", C.c_void_p), ("logsumexp", C.c_void_p),
+                ("values_stride", C.c_int64), ("index_stride", C.c_int64), ("ignore", C.c_int64),
+                ("k", C.c_int32), ("index64", C.c_int32)]
+
+
+def _cuda(name, x, dtypes, ndim=None):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor, got {type(x).__name__}")
+    if not x.is_cuda:
+        raise ValueError(f"{name} must be on a CUDA device, it is on {x.device}")
+    if x.dtype not in dtypes:
+        raise ValueError(f"{name} must be one of {', '.join(str(d) for d in dtypes)}, got {x.dtype}")
+    if ndim is not None and x.ndim != ndim:
+        raise ValueError(f"{name} must have {ndim} dimensions, got shape {tuple(x.shape)}")
+
+
+def _rows(x):
+    """`x` with unit stride within its rows and rows that do not overlap."""
+    if x.stride(1) != 1 and x.shape[1] > 1 or x.stride(0) < x.shape[1] and x.shape[0] > 1:
+        x = x.contiguous()
+    return x
+
+
+def _temperature(t):
+    t = float(t)
+    if not 1e-6 <= t <= 1e6:
+        raise ValueError(f"temperature must be between 1e-6 and 1e6, got {t}")
+    return t
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _workspace(n_bytes, device):
+    if n_bytes < 0:
+        _lib.check(int(n_bytes))
+    return torch.empty(n_bytes, dtype=torch.uint8, device=device)
+
+
+def top_scores(scores, k: int, *, temperature: float = 1.0, probabilities: bool = False) -> TopScores:
+    """The `k` largest of each row of `scores` (..., n_classes), fp32, fp64, bf16 or fp16.
+
+    Returns `TopScores`: `values` (..., k) of the scores' type in descending order, equal ones in the
+    order of their classes, NaN above everything; their classes as `index` (..., k) int32; and
+    `logsumexp` (...), log sum exp(score / temperature) over the whole row (fp32, of fp64 scores fp64).
+    With `probabilities` the logarithms of the scores take the scores' place in `values` and
+    `logsumexp`: what a distillation loss takes as a forest's logits.  1 <= k <= min(n_classes, 256).
+    The outputs are constants to autograd."""
+    _cuda("scores", scores, _TYPES)
+    if scores.ndim < 1:
+        raise ValueError("scores must have at least one dimension")
+    shape, n_cols, k = scores.shape[:-1], scores.shape[-1], int(k)
+    if not 1 <= k <= min(n_cols, MOST_TOP):
+        raise ValueError(f"k must be between 1 and min(n_classes, {MOST_TOP}) = {min(n_cols, MOST_TOP)}, got {k}")
+    temperature = _temperature(temperature)
+    x = scores.detach()
+    x = _rows(x if x.ndim == 2 else x.reshape(-1, n_cols))
+    n, dev = x.shape[0], x.device
+    values = torch.empty((n, k), dtype=x.dtype, device=dev)
+    index = torch.empty((n, k), dtype=torch.int32, device=dev)
+    lse = torch.empty((n,), dtype=torch.float64 if x.dtype == torch.float64 else torch.float32, device=dev)
+    if n:
+        lib, kind = _lib.load(), _TYPES[x.dtype]
+        ws = _workspace(lib.b2fil_top_scores_workspace(kind, n, n_cols, k, dev.index), dev)
+        _lib.check(lib.b2fil_top_scores(kind, x.data_ptr(), n, n_cols, x.stride(0), k, bool(probabilities),
+                                        temperature, values.data_ptr(), index.data_ptr(), lse.data_ptr(),
+                                        ws.data_ptr(), ws.numel(), dev.index, _stream(dev)))
+    if len(shape) != 1:
+        values, index, lse = values.view(*shape, k), index.view(*shape, k), lse.view(shape)
+    return TopScores(values, index, lse)
+
+
+class _Teacher:
+    """The teacher's tensors of one call, checked, and the structure that points at them."""
+
+    def __init__(self, n, dev, values, index, lse, ignore=_NO_CLASS):
+        self.tensors = (values, index, lse)  # kept while the structure is in use
+        self.c = CTeacher(values.data_ptr() if values is not None else None, index.data_ptr(),
+                          lse.data_ptr() if lse is not None else None,
+                          values.stride(0) if values is not None else 0, index.stride(0), ignore, index.shape[1],
+                          index.dtype == torch.int64)
+
+
+def _top(top, n, dev, tail):
+    """(values fp32, index, logsumexp fp32 or None) of `top` for n rows, checked."""
+    if tail not in _TAILS:
+        raise ValueError(f"tail must be one of {_TAILS}, got {tail!r}")
+    if not isinstance(top, (tuple, list)) or len(top) not in (2, 3):
+        raise TypeError("the teacher must be a TopScores, or (values, index[, logsumexp])")
+    values, index, lse = (*top, None) if len(top) == 2 else top
+    _cuda("the teacher's values", values, _TYPES)
+    _cuda("the teacher's index", index, (torch.int32, torch.int64))
+    if values.ndim < 1 or values.shape != index.shape:
+        raise ValueError(f"the teacher's values and index differ in shape: {tuple(values.shape)}, {tuple(index.shape)}")
+    k = values.shape[-1]
+    if not 1 <= k <= MOST_TOP:
+        raise ValueError(f"the teacher's k must be between 1 and {MOST_TOP}, got {k}")
+    values, index = values.detach().reshape(-1, k), index.reshape(-1, k)
+    if values.shape[0] != n:
+        raise ValueError(f"the teacher has {values.shape[0]} rows, the student {n}")
+    if tail == "bucket":
+        if lse is None:
+            raise ValueError("tail='bucket' needs the teacher's logsumexp")
+        _cuda("the teacher's logsumexp", lse, _TYPES)
+        if lse.numel() != n:
+            raise ValueError(f"the teacher's logsumexp has {lse.numel()} rows, the student {n}")
+        lse = lse.detach().reshape(-1).float().contiguous()
+    else:
+        lse = None
+    for t in (values, index, lse):
+        if t is not None and t.device != dev:
+            raise ValueError(f"the teacher is on {t.device}, the student on {dev}")
+    return _rows(values.float()), _rows(index), lse
+
+
+def _upstream(g):
+    """(fp32 gradient by the loss, elements from one row's to the next)."""
+    g = g if g.dtype == torch.float32 else g.float()
+    return g, (g.stride(0) if g.ndim else 0)
+
+
+def _reduction(reduction):
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {tuple(_REDUCTIONS)}, got {reduction!r}")
+    return _REDUCTIONS[reduction]
+
+
+class _Loss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, values, index, lse, temperature, ignore, reduction):
+        lib, kind, dev = _lib.load(), _TYPES[logits.dtype], logits.device
+        x = _rows(logits)
+        n, n_cols = x.shape
+        t = _Teacher(n, dev, values, index, lse, ignore)
+        ws = _workspace(lib.b2fil_distill_loss_workspace(kind, n, n_cols, t.c.k, dev.index), dev)
+        stats = torch.empty((4 * n + 4,), dtype=torch.float32, device=dev)  # and the factor
+        rows = torch.empty((n,), dtype=torch.float32, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev) if reduction else rows
+        factor = stats.data_ptr() + 16 * n if reduction else None
+        _lib.check(lib.b2fil_distill_loss(kind, x.data_ptr(), n, n_cols, x.stride(0), C.byref(t.c), temperature,
+                                          reduction, rows.data_ptr(), stats.data_ptr(), loss.data_ptr(), factor,
+                                          ws.data_ptr(), ws.numel(), dev.index, _stream(dev)))
+        ctx.save_for_backward(logits, values, index, lse)
+        ctx.stats, ctx.options = stats, (temperature, ignore, reduction)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        logits, values, index, lse = ctx.saved_tensors
+        temperature, ignore, reduction = ctx.options
+        lib, kind, dev = _lib.load(), _TYPES[logits.dtype], logits.device
+        x = _rows(logits)
+        n, n_cols = x.shape
+        grad = torch.empty((n, n_cols), dtype=x.dtype, device=dev)
+        t = _Teacher(n, dev, values, index, lse, ignore)
+        g, stride = _upstream(g)
+        _lib.check(lib.b2fil_distill_loss_grad(
+            kind, x.data_ptr(), n, n_cols, x.stride(0), C.byref(t.c), temperature, ctx.stats.data_ptr(), g.data_ptr(),
+            stride, ctx.stats.data_ptr() + 16 * n if reduction else None, grad.data_ptr(), n_cols, dev.index,
+            _stream(dev)))
+        return grad, None, None, None, None, None, None
+
+
+_STUDENT = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def distillation_loss(logits, top, *, temperature: float = 1.0, tail: str = "renormalise", reduction: str = "mean"):
+    """T^2 KL(teacher || softmax(logits / T)) over the classes that the teacher names.
+
+    logits : (..., n_classes) fp32, bf16 or fp16; rows whose logits are all -inf do not count.
+    top : `TopScores`, or (values, index[, logsumexp]) with values and index of shape (..., k), k <= 256.
+        Entries whose class is outside [0, n_classes) do not count, a class that is named twice has the sum of its
+        probabilities; rows without an entry do not count.
+    tail : what becomes of the classes that the teacher does not name.  'renormalise': nothing, the named ones'
+        probabilities are scaled to a sum of 1.  'bucket': together they are one more class on both sides;
+        this takes the teacher's `logsumexp` over all its classes at the same temperature, and at most 2^20 classes.
+    reduction : 'mean' over the rows that count (0 where none does), 'sum', or 'none': (...), 0 for others.
+
+    The loss is fp32, the gradient by the logits has their type."""
+    _cuda("logits", logits, _STUDENT)
+    if logits.ndim < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must have shape (..., n_classes), got {tuple(logits.shape)}")
+    shape, n_cols = logits.shape[:-1], logits.shape[-1]
+    x = logits if logits.ndim == 2 else logits.reshape(-1, n_cols)
+    values, index, lse = _top(top, x.shape[0], x.device, tail)
+    if lse is not None and n_cols > 1 << 20:
+        raise ValueError(f"tail='bucket' takes at most 2^20 classes, got {n_cols}")
+    loss = _Loss.apply(x, values, index, lse, _temperature(temperature), _NO_CLASS, _reduction(reduction))
+    return loss.view(shape) if reduction == "none" and len(shape) != 1 else loss

@@ -82,6 +82,17 @@ def load() -> C.CDLL:
     lib.b2fil_predict_sharded.restype = i32
     lib.b2fil_predict_sharded.argtypes = [C.POINTER(vp), i32, i32, C.POINTER(vp),
                                           C.POINTER(i64), i64, vp, i32, C.c_double]
+    f64 = C.c_double
+    lib.b2fil_top_scores_workspace.restype = i64
+    lib.b2fil_top_scores_workspace.argtypes = [i32, i64, i64, i32, i32]
+    lib.b2fil_top_scores.restype = i32
+    lib.b2fil_top_scores.argtypes = [i32, vp, i64, i64, i64, i32, i32, f64, vp, vp, vp, vp, i64, i32, vp]
+    lib.b2fil_distill_loss_workspace.restype = i64
+    lib.b2fil_distill_loss_workspace.argtypes = [i32, i64, i64, i32, i32]
+    lib.b2fil_distill_loss.restype = i32
+    lib.b2fil_distill_loss.argtypes = [i32, vp, i64, i64, i64, vp, f64, i32, vp, vp, vp, vp, vp, i64, i32, vp]
+    lib.b2fil_distill_loss_grad.restype = i32
+    lib.b2fil_distill_loss_grad.argtypes = [i32, vp, i64, i64, i64, vp, f64, vp, vp, i64, vp, vp, i64, i32, vp]
     _lib = lib
     return lib
 

@@ -338,6 +338,78 @@ int b2fil_predict_sharded(b2fil_forest* const* forests, int n_devices, int infer
 int b2fil_last_sharded_timing(double* compute_ms, double* gather_ms, double* wall_ms,
                               int* gather_direct);
 
+/* ---- distillation ---------------------------------------------------------------------------- */
+/*
+ * What a forest (or any other teacher) answers is cut down to the k best classes of each row, and a
+ * student network is trained on those.  None of these calls has a counterpart in the reference.  All
+ * of them are stream ordered on cuda_stream of device_id, allocate nothing and keep nothing: the
+ * caller passes a workspace of the size that the *_workspace call gives (a negative code on bad
+ * arguments), 256-byte aligned, which may be used for something else once the call's work on the
+ * stream is done; two calls that may run at the same time need one each.
+ */
+
+/* element types of scores, logits and the parts of a linear layer */
+#define B2FIL_TYPE_F32 0
+#define B2FIL_TYPE_F64 1   /* b2fil_top_scores only */
+#define B2FIL_TYPE_BF16 2
+#define B2FIL_TYPE_F16 3
+
+/* reductions of a loss over the rows */
+#define B2FIL_REDUCE_NONE 0
+#define B2FIL_REDUCE_SUM 1
+#define B2FIL_REDUCE_MEAN 2 /* over the rows that count; 0 where none does */
+
+#define B2FIL_MOST_TOP 256 /* largest k */
+
+/* The k largest scores of each row of (n_rows, n_cols), row_stride elements between rows, in
+ * descending order, equal ones in the order of their classes (NaN above everything), to values
+ * (n_rows, k) of the scores' type, their classes to index (n_rows, k), and log sum exp(score /
+ * temperature) of the whole row to logsumexp ((n_rows) double for B2FIL_TYPE_F64, else float; may be
+ * NULL).  With `probabilities` the scores' logarithms stand for the scores in values and logsumexp.
+ * 1 <= k <= min(n_cols, B2FIL_MOST_TOP), n_cols < 2^31. */
+int64_t b2fil_top_scores_workspace(int dtype, int64_t n_rows, int64_t n_cols, int k, int device_id);
+int b2fil_top_scores(int dtype, const void* scores, int64_t n_rows, int64_t n_cols, int64_t row_stride,
+                     int k, int probabilities, double temperature, void* values, int32_t* index,
+                     void* logsumexp, void* workspace, int64_t workspace_bytes, int device_id,
+                     void* cuda_stream);
+
+/* What a teacher says of each row: k classes and their scores.  Entries whose class is outside
+ * [0, n_cols) or equals `ignore` do not count; a class named twice has the sum of its
+ * probabilities.  A row counts where some entry with a score above -inf is left (with logsumexp: where
+ * that is above -inf) and some logit is above -inf; the loss and the gradient of other rows are 0. */
+typedef struct b2fil_teacher {
+  const float* values;     /* (n_rows, k) scores, or NULL: all entries of a row weigh the same */
+  const void* index;       /* (n_rows, k) classes, int32 or int64                               */
+  const float* logsumexp;  /* (n_rows) log sum exp(score / temperature) over ALL the teacher's classes:
+                              the classes that are not named become one more, with what is left
+                              of 1 (less than 2^-20 counts as nothing).  NULL: the named classes'
+                              probabilities are scaled to a sum of 1                              */
+  int64_t values_stride;   /* elements between rows */
+  int64_t index_stride;
+  int64_t ignore;          /* class that does not count, e.g. -100 */
+  int32_t k;
+  int32_t index64;         /* 1: int64 classes */
+} b2fil_teacher;
+
+/* temperature^2 * KL(teacher || softmax(logits / temperature)) of each row to row_loss (n_rows), what the
+ * gradient needs to row_stats (n_rows, 4), 16-byte aligned, and the sum or mean to loss[0] and its
+ * factor to factor[0] (not used with B2FIL_REDUCE_NONE).  One entry per row with values = NULL and
+ * temperature 1 is softmax cross entropy.  The teacher's logsumexp needs n_cols <= 2^20. */
+int64_t b2fil_distill_loss_workspace(int dtype, int64_t n_rows, int64_t n_cols, int k, int device_id);
+int b2fil_distill_loss(int dtype, const void* logits, int64_t n_rows, int64_t n_cols, int64_t row_stride,
+                       const b2fil_teacher* teacher, double temperature, int reduction, float* row_loss,
+                       float* row_stats, float* loss, float* factor, void* workspace,
+                       int64_t workspace_bytes, int device_id, void* cuda_stream);
+
+/* The gradient of that loss by the logits to grad (n_rows, n_cols), grad_stride elements between rows.
+ * upstream: the gradient by the loss, one value per row upstream_stride apart (0: one value);
+ * factor: what b2fil_distill_loss wrote, or NULL for B2FIL_REDUCE_NONE. */
+int b2fil_distill_loss_grad(int dtype, const void* logits, int64_t n_rows, int64_t n_cols,
+                            int64_t row_stride, const b2fil_teacher* teacher, double temperature,
+                            const float* row_stats, const float* upstream, int64_t upstream_stride,
+                            const float* factor, void* grad, int64_t grad_stride, int device_id,
+                            void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif
