@@ -23,13 +23,14 @@ SOURCES = ["api.cu", "kernels.cu", "kernels_q_top6.cu", "kernels_q_plain6.cu", "
            "kernels_q_leafg.cu", "kernels_q_vec.cu", "kernels_q_top_vec.cu", "kernels_q_top_out.cu",
            "kernels_sparse_c.cu",
            "pack.cpp", "blocks.cpp",
-           "distill_api.cu", "distill_top.cu", "distill_loss.cu"]
+           "distill_api.cu", "distill_top.cu", "distill_loss.cu", "distill_linear.cu"]
 HEADERS = ["each_tree.hpp", "forest.hpp", "host_pool.hpp", "kernels.hpp", "kernels_q.hpp", "device_common.cuh", "dense_q.cuh",
            os.path.join("..", "..", "include", "b2fil.h"), "distill.hpp", "distill_common.cuh"]
 # sources that include none of the others' headers: they are compiled again for these alone
 OWN_HEADERS = {"distill_api.cu": ["distill.hpp", os.path.join("..", "..", "include", "b2fil.h")],
                "distill_top.cu": ["distill.hpp", "distill_common.cuh"],
-               "distill_loss.cu": ["distill.hpp", "distill_common.cuh"]}
+               "distill_loss.cu": ["distill.hpp", "distill_common.cuh"],
+               "distill_linear.cu": ["distill.hpp", "distill_common.cuh"]}
 
 
 # Native call path for torch tensors: a CPython module compiled against the installed torch, whose
@@ -72,7 +73,7 @@ def _newer(target: str, deps: list) -> bool:
 
 def _object_deps(src: str) -> list:
     """Files that an object is older than when it has to be compiled again."""
-    headers = OWN_HEADERS.get(src, [h for h in HEADERS if h not in ("distill_common.cuh", "distill_linear.cuh")])
+    headers = OWN_HEADERS.get(src, [h for h in HEADERS if h != "distill_common.cuh"])
     return [os.path.join(SRC, f) for f in [src] + headers] + [os.path.abspath(__file__)]
 
 

@@ -71,5 +71,41 @@ struct LossGradArgs {
 };
 cudaError_t launch_loss_grad(int dtype, const LossGradArgs& a, int n_sms, cudaStream_t s);
 
+// ---- loss on a linear layer's output (distill_linear.cu) -------------------------------------
+// What the teacher names in each row, kept for the gradient: (n_rows, k) each.
+struct Named {
+  float* logit;  // h . w of the class
+  float* p;      // the teacher's probability
+  int32_t* at;   // the class, below 0: none
+};
+struct LinearArgs {
+  const void* hidden;  // (n_rows, width), 16-byte aligned rows, width a multiple of 8
+  const void* weight;  // (n_cols, width), likewise
+  int64_t n_rows, n_cols, width, hidden_stride, weight_stride;
+  Teacher teacher;     // no logsumexp
+  float temperature;
+  float* row_loss;
+  float4* row_stats;   // as in LossArgs; the factor is 1
+  Named named;
+};
+size_t linear_workspace(const LinearArgs& a, int n_sms);
+cudaError_t launch_linear(int dtype, const LinearArgs& a, const Reduced& out, void* workspace, int n_sms, cudaStream_t s);
+
+struct LinearGradArgs {
+  LinearArgs fwd;
+  const float* upstream;
+  int64_t upstream_stride;
+  const float* factor;  // null: upstream has one value per row
+  void* grad_hidden;    // (n_rows, width) contiguous, or null
+  void* grad_weight;    // (n_cols, width) contiguous, or null
+};
+size_t linear_grad_workspace(const LinearGradArgs& g, int n_sms);
+cudaError_t launch_linear_grad(int dtype, const LinearGradArgs& g, void* workspace, int n_sms, cudaStream_t s);
+
+// Waits for the current device, reads its status word and clears it: not 0 where a bounded wait ran out.
+cudaError_t linear_status(int* status);
+// A kernel whose only work is such a wait, which nothing ends and which gives up after a millisecond.
+cudaError_t launch_linear_timeout(cudaStream_t s);
+
 }  // namespace distill
 }  // namespace b2fil

@@ -102,6 +102,26 @@ int check_loss(int dtype, int64_t n_rows, int64_t n_cols, int k)
   return B2FIL_OK;
 }
 
+int check_linear(int dtype, int64_t n_rows, int64_t n_cols, int64_t width, int k)
+{
+  if (dtype != B2FIL_TYPE_BF16 && dtype != B2FIL_TYPE_F16) return invalid("a linear layer must be bf16 or fp16");
+  if (n_rows < 0 || n_rows >= INT32_MAX - 256 || n_cols < 1 || n_cols >= INT32_MAX - 256)
+    return invalid("n_rows is not in 0 to 2^31 - 257, or n_cols not in 1 to 2^31 - 257");
+  if (width < 8 || width % 8 || width > (1 << 20)) return invalid("width must be a multiple of 8, 8 to 2^20");
+  if (k < 1 || k > B2FIL_MOST_TOP) return invalid("the teacher's k must be 1 to 256");
+  return B2FIL_OK;
+}
+
+int check_layer(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride, int64_t n_rows, int64_t width)
+{
+  if ((!hidden && n_rows > 0) || !weight) return invalid("NULL buffer");
+  if (!aligned(hidden, 16) || !aligned(weight, 16) || hidden_stride % 8 || weight_stride % 8)
+    return invalid("rows of hidden and weight must start on 16 bytes");
+  if (hidden_stride < width || weight_stride < width || hidden_stride > (1ll << 32) || weight_stride > (1ll << 32))
+    return invalid("a row stride is smaller than width, or above 2^32");
+  return B2FIL_OK;
+}
+
 int64_t rounded(size_t bytes) { return static_cast<int64_t>((bytes + 255) / 256 * 256); }
 
 int finish(const char* what, cudaError_t e) { return e == cudaSuccess ? B2FIL_OK : cuda_failed(what, e); }
@@ -222,6 +242,145 @@ int b2fil_distill_loss_grad(int dtype, const void* logits, int64_t n_rows, int64
   g.grad            = grad;
   g.grad_stride     = grad_stride;
   return finish("b2fil_distill_loss_grad", launch_loss_grad(dtype, g, sms, static_cast<cudaStream_t>(cuda_stream)));
+}
+
+int64_t b2fil_linear_loss_workspace(int dtype, int64_t n_rows, int64_t n_cols, int64_t width, int k, int device_id)
+{
+  int rc = check_linear(dtype, n_rows, n_cols, width, k);
+  if (rc != B2FIL_OK) return rc;
+  const int sms = sms_of(device_id);
+  if (sms < 0) return sms;
+  LinearArgs a{};
+  a.n_rows    = n_rows;
+  a.n_cols    = n_cols;
+  a.width     = width;
+  a.teacher.k = k;
+  return rounded(linear_workspace(a, sms));
+}
+
+int b2fil_linear_loss(int dtype, const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride,
+                      int64_t n_rows, int64_t n_cols, int64_t width, const b2fil_teacher* teacher, double temperature,
+                      int reduction, float* row_loss, float* row_stats, float* named_logit, float* named_p, int32_t* named_at,
+                      float* loss, float* factor, void* workspace, int64_t workspace_bytes, int device_id, void* cuda_stream)
+{
+  LinearArgs a{};
+  int rc = check_teacher(teacher, n_rows, a.teacher);
+  if (rc == B2FIL_OK) rc = check_linear(dtype, n_rows, n_cols, width, a.teacher.k);
+  if (rc == B2FIL_OK) rc = check_temperature(temperature);
+  if (rc == B2FIL_OK) rc = check_layer(hidden, hidden_stride, weight, weight_stride, n_rows, width);
+  if (rc != B2FIL_OK) return rc;
+  if (a.teacher.logsumexp) return invalid("the loss of a linear layer takes no logsumexp of the teacher");
+  if (reduction < B2FIL_REDUCE_NONE || reduction > B2FIL_REDUCE_MEAN) return invalid("unknown reduction");
+  if (reduction != B2FIL_REDUCE_NONE && (!loss || !factor)) return invalid("a reduced loss needs loss and factor");
+  if (n_rows > 0 && (!row_loss || !row_stats || !named_logit || !named_p || !named_at)) return invalid("NULL buffer");
+  if (!aligned(row_stats, 16) || !aligned(row_loss, 4) || !aligned(named_logit, 4) || !aligned(named_p, 4) || !aligned(named_at, 4))
+    return invalid("a buffer is not aligned");
+  rc = check_workspace(workspace, workspace_bytes, b2fil_linear_loss_workspace(dtype, n_rows, n_cols, width, a.teacher.k, device_id));
+  if (rc != B2FIL_OK) return rc;
+  OnDevice on(device_id);
+  if (!on.ok) return invalid("device_id cannot be made current");
+  a.hidden        = hidden;
+  a.weight        = weight;
+  a.n_rows        = n_rows;
+  a.n_cols        = n_cols;
+  a.width         = width;
+  a.hidden_stride = hidden_stride;
+  a.weight_stride = weight_stride;
+  a.temperature   = static_cast<float>(temperature);
+  a.row_loss      = row_loss;
+  a.row_stats     = reinterpret_cast<float4*>(row_stats);
+  a.named         = Named{named_logit, named_p, named_at};
+  return finish("b2fil_linear_loss", launch_linear(dtype, a, Reduced{reduction, loss, factor}, workspace,
+                                                   sms_of(device_id), static_cast<cudaStream_t>(cuda_stream)));
+}
+
+int64_t b2fil_linear_loss_grad_workspace(int dtype, int64_t n_rows, int64_t n_cols, int64_t width, int k, int wants_hidden,
+                                         int wants_weight, int device_id)
+{
+  int rc = check_linear(dtype, n_rows, n_cols, width, k);
+  if (rc != B2FIL_OK) return rc;
+  const int sms = sms_of(device_id);
+  if (sms < 0) return sms;
+  LinearGradArgs g{};
+  g.fwd.n_rows    = n_rows;
+  g.fwd.n_cols    = n_cols;
+  g.fwd.width     = width;
+  g.fwd.teacher.k = k;
+  char some;
+  g.grad_hidden = wants_hidden ? &some : nullptr;
+  g.grad_weight = wants_weight ? &some : nullptr;
+  return n_rows && (wants_hidden || wants_weight) ? rounded(linear_grad_workspace(g, sms)) : 0;
+}
+
+int b2fil_linear_loss_grad(int dtype, const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride,
+                           int64_t n_rows, int64_t n_cols, int64_t width, int k, double temperature, const float* row_stats,
+                           const float* named_logit, const float* named_p, const int32_t* named_at, const float* upstream,
+                           int64_t upstream_stride, const float* factor, void* grad_hidden, void* grad_weight,
+                           void* workspace, int64_t workspace_bytes, int device_id, void* cuda_stream)
+{
+  LinearGradArgs g{};
+  LinearArgs& a = g.fwd;
+  int rc        = check_linear(dtype, n_rows, n_cols, width, k);
+  if (rc == B2FIL_OK) rc = check_temperature(temperature);
+  if (rc == B2FIL_OK) rc = check_layer(hidden, hidden_stride, weight, weight_stride, n_rows, width);
+  if (rc != B2FIL_OK) return rc;
+  if (!grad_hidden && !grad_weight) return B2FIL_OK;
+  if (n_rows > 0 && (!row_stats || !named_logit || !named_p || !named_at || !upstream)) return invalid("NULL buffer");
+  if (!aligned(row_stats, 16) || !aligned(named_logit, 4) || !aligned(named_p, 4) || !aligned(named_at, 4) ||
+      !aligned(upstream, 4) || !aligned(factor, 4) || !aligned(grad_hidden, 16) || !aligned(grad_weight, 16))
+    return invalid("a buffer is not aligned");
+  rc = check_workspace(workspace, workspace_bytes,
+                       b2fil_linear_loss_grad_workspace(dtype, n_rows, n_cols, width, k, grad_hidden != nullptr,
+                                                        grad_weight != nullptr, device_id));
+  if (rc != B2FIL_OK) return rc;
+  const int sms = sms_of(device_id);
+  if (sms < 0) return sms;
+  OnDevice on(device_id);
+  if (!on.ok) return invalid("device_id cannot be made current");
+  const cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+  if (n_rows == 0)
+    return finish("b2fil_linear_loss_grad", grad_weight ? cudaMemsetAsync(grad_weight, 0, n_cols * width * 2, s) : cudaSuccess);
+  a.hidden          = hidden;
+  a.weight          = weight;
+  a.n_rows          = n_rows;
+  a.n_cols          = n_cols;
+  a.width           = width;
+  a.hidden_stride   = hidden_stride;
+  a.weight_stride   = weight_stride;
+  a.teacher.k       = k;
+  a.temperature     = static_cast<float>(temperature);
+  a.row_stats       = const_cast<float4*>(reinterpret_cast<const float4*>(row_stats));
+  a.named           = Named{const_cast<float*>(named_logit), const_cast<float*>(named_p), const_cast<int32_t*>(named_at)};
+  g.upstream        = upstream;
+  g.upstream_stride = upstream_stride;
+  g.factor          = factor;
+  g.grad_hidden     = grad_hidden;
+  g.grad_weight     = grad_weight;
+  return finish("b2fil_linear_loss_grad", launch_linear_grad(dtype, g, workspace, sms, s));
+}
+
+int b2fil_distill_status(int device_id, int32_t* status)
+{
+  if (!status) return invalid("status is NULL");
+  *status       = 0;
+  const int sms = sms_of(device_id);
+  if (sms < 0) return sms;
+  OnDevice on(device_id);
+  if (!on.ok) return invalid("device_id cannot be made current");
+  int word            = 0;
+  const cudaError_t e = linear_status(&word);
+  if (e != cudaSuccess) return cuda_failed("b2fil_distill_status", e);
+  *status = word;
+  return word ? report_error(B2FIL_ERR_TIMEOUT, "a bounded wait inside a kernel of the linear loss ran out") : B2FIL_OK;
+}
+
+int b2fil_distill_selftest_timeout(int device_id, void* cuda_stream)
+{
+  const int sms = sms_of(device_id);
+  if (sms < 0) return sms;
+  OnDevice on(device_id);
+  if (!on.ok) return invalid("device_id cannot be made current");
+  return finish("b2fil_distill_selftest_timeout", launch_linear_timeout(static_cast<cudaStream_t>(cuda_stream)));
 }
 
 }  // extern "C"

@@ -1,0 +1,879 @@
+// Loss of a linear layer's output z = H W^T and its gradients without keeping z.
+//
+//   forward   z tile by tile on the tensor cores; of a tile only each row's maximum and sum of
+//             exp((z - max) / T) are kept, then joined per row with the logits of the classes that the
+//             teacher names (dot products of their own: k per row)
+//   backward  piece by piece of the classes: z again, d = q - p to a buffer of 16-bit values that
+//             stays in L2, then dH += d W and dW = d^T H from it
+//
+// Bound by the tensor cores: 8 N D V operations for a training step, of which the second z (2 N D V) is the
+// price of not keeping it; kept in 16 bits it would be written once and read twice, and its rounding would
+// be in q.  d is rounded to the layer's own 16 bits because both operands of a matrix instruction have
+// one type: half a step of each d, independent of each other, where the gradient's own rounding
+// is as much again.  For fp16 d is scaled by 2^14, so that probabilities down to 4e-9 are normal
+// numbers.  Sums over classes and rows are in 32 bits; a sum over several pieces stays in 32 bits.
+//
+// One kernel does all products: a cluster of two CTAs takes 256 x 256 of the output
+// (tcgen05.mma.cta_group::2; each CTA holds 128 rows of A, half of B and 128 rows of the result), since
+// one CTA alone with 128 x 256 would have to read 96 bytes per cycle from L2 where 64 pass.  Warp 0 brings the
+// tiles (TMA, 128-byte swizzle, ring of 6 x 32 KB), warp 1 of the first CTA issues the products, warps 4 to
+// 7 work on the finished tile while the next one is summed in the other half of TMEM.  All waits are
+// bounded: after two seconds a role gives up, sets the status word and leaves by the common exit.
+#include <cuda.h>
+
+#include "distill_common.cuh"
+
+namespace b2fil {
+namespace distill {
+namespace {
+
+constexpr int kTile    = 256;              // rows and columns of a cluster's tile
+constexpr int kHalf    = 128;              // of one CTA
+constexpr int kDepth   = 64;               // of the inner dimension per stage: 128 bytes
+constexpr int kStages  = 6;
+constexpr int kStageA  = kHalf * kDepth * 2;
+constexpr int kStage   = 2 * kStageA;      // A and B of one CTA
+constexpr int kThreads = 256;
+constexpr int kSmem    = kStages * kStage + 1024 + 256;
+constexpr long long kPatience = 2000000000ll;  // ns
+constexpr int64_t kPieceBytes = 64ll << 20;    // of d: fits L2 beside what is read
+constexpr int kMostSplits     = 16;
+constexpr float kHalfScale    = 16384.f;       // of d in fp16
+
+__device__ int g_status;
+
+// ---- PTX -------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t shared_of(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ uint32_t rank_in_cluster()
+{
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t shared, uint32_t rank)
+{
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(shared), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void bar_init(uint32_t bar, int count)
+{
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, int bytes)
+{
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t bar)  // shared::cluster address
+{
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity)
+{
+  uint32_t ok;
+  asm volatile(
+    "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+    : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok;
+}
+__device__ __forceinline__ long long now_ns()
+{
+  long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+// False: the wait ran out (status word set), or another role of the CTA had given up.
+__device__ __noinline__ bool bar_wait_long(uint32_t bar, uint32_t parity, volatile int* gave_up, long long patience)
+{
+  const long long until = now_ns() + patience;
+  while (!bar_try(bar, parity)) {
+    if (*gave_up) return false;
+    if (now_ns() > until) {
+      *gave_up = 1;
+      atomicExch(&g_status, 1);
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up)
+{
+  return bar_try(bar, parity) || bar_wait_long(bar, parity, gave_up, kPatience);
+}
+// 2-dimensional box to this CTA's shared memory; the bytes are counted at `bar`, which may be the other CTA's
+__device__ __forceinline__ void load_box(uint32_t to, const CUtensorMap* map, uint32_t bar, int x, int y)
+{
+  asm volatile(
+    "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];"
+    ::"r"(to), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
+{
+  asm volatile(
+    "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}"
+    ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add)) : "memory");
+}
+// Arrives at `bar` of both CTAs when the products issued so far are done.
+__device__ __forceinline__ void commit(uint32_t bar)
+{
+  asm volatile(
+    "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+    ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+__device__ __forceinline__ void load_columns(uint32_t from, float (&x)[32])
+{
+  uint32_t r[32];
+  asm volatile(
+    "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+    "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+    "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+    : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+      "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+      "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+      "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+    : "r"(from));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
+}
+
+// Shared-memory descriptor of a tile with 128-byte swizzle (version 1).  Inner dimension contiguous: rows of
+// 128 bytes, 1024 bytes from 8 rows to the next.  Outer dimension contiguous: 64 outer by 64 inner elements
+// are 64 rows of 128 bytes; 1024 bytes from 8 of the inner dimension to the next, 8192 from one such block to
+// that of the next 64 outer elements.
+__device__ __forceinline__ uint64_t descriptor(uint32_t at, bool outer)
+{
+  const uint64_t leading = outer ? 8192 >> 4 : 1, stride = 1024 >> 4;
+  return (at >> 4 & 0x3fff) | leading << 16 | stride << 32 | 1ull << 46 | 2ull << 61;
+}
+// Instruction descriptor: 32-bit sums, A and B of one 16-bit type, 256 x 256.
+__device__ __forceinline__ uint32_t instruction(bool bf16, bool a_outer, bool b_outer)
+{
+  return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | static_cast<uint32_t>(a_outer) << 15 |
+         static_cast<uint32_t>(b_outer) << 16 | (kTile >> 3) << 17 | (kTile >> 4) << 24;
+}
+
+// ---- products --------------------------------------------------------------------------------
+enum Result { kStats, kDiff, kSumHidden, kHidden, kWeight };
+
+// out (m x n) = A (m x depth) B (n x depth)^T.  *_outer: the matrix lies with its depth outermost.
+struct Product {
+  CUtensorMap a, b;
+  int m, n, depth;
+  int m_tiles, n_tiles, splits;  // splits: parts of the depth, each with a result of its own (kSumHidden)
+  int a_outer, b_outer;
+  int result;
+};
+struct Work {
+  Product product[2];
+  int products;
+  int bf16;
+  // kStats: (row, tile of columns) -> maximum and sum
+  float2* parts;
+  // kStats, kDiff
+  float c;                // log2(e) / T
+  // kDiff: d = scale q of the classes from `first` on, columns up to a whole tile
+  const float4* stats;
+  const float* row_scale; // or null: 1
+  void* diff;
+  int64_t diff_stride;
+  float diff_scale;
+  // kSumHidden: 32-bit sums, one matrix per split; kHidden, kWeight: 16-bit results times *scale
+  float* sums;
+  int add;
+  void *grad_hidden, *grad_weight;
+  int64_t width;
+  const float* scale;
+};
+
+struct Tile {
+  int which, m, n, split, begin, end;  // begin, end: stages of the depth
+};
+__device__ __forceinline__ bool tile_of(const Work& w, int t, Tile& r)
+{
+  for (int i = 0; i < w.products; ++i) {
+    const Product& p = w.product[i];
+    const int tiles  = p.m_tiles * p.n_tiles * p.splits;
+    if (t < tiles) {
+      r.which         = i;
+      r.m             = t % p.m_tiles;
+      r.n             = t / p.m_tiles % p.n_tiles;
+      r.split         = t / (p.m_tiles * p.n_tiles);
+      const int steps = (p.depth + kDepth - 1) / kDepth;
+      r.begin         = static_cast<int>(static_cast<int64_t>(steps) * r.split / p.splits);
+      r.end           = static_cast<int>(static_cast<int64_t>(steps) * (r.split + 1) / p.splits);
+      return true;
+    }
+    t -= tiles;
+  }
+  return false;
+}
+
+__device__ __forceinline__ void store32(void* to, const uint32_t (&x)[8])
+{
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]),
+               "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]) : "memory");
+}
+__device__ __forceinline__ uint32_t two(float lo, float hi, bool bf16)
+{
+  uint32_t r;
+  if (bf16)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Part of a row (32 columns from `col` on) of a finished tile.  n: columns of the result.
+template <int KIND>
+__device__ __forceinline__ void take_columns(const Work& w, const Product& p, int split, int64_t row, int col, float (&x)[32],
+                                             Running<float>& r, float base, float factor)
+{
+  if (KIND == kStats) {
+    if (col + 32 > p.n) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (col + i >= p.n) x[i] = lowest<float>();
+    }
+    float most = x[0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) most = fmaxf(most, x[i]);
+    if (most > r.m) r.raise(most, w.c);
+    const float b = base_of(r.m);
+    float s[4]    = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s[i & 3] += power((x[i] - b) * w.c);
+    r.s += (s[0] + s[1]) + (s[2] + s[3]);
+    return;
+  }
+  if (KIND == kDiff) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = col + i < p.n ? power((x[i] - base) * w.c) * factor : 0.f;
+    if (factor == 0.f) {  // a row that does not count, whatever its logits are
+#pragma unroll
+      for (int i = 0; i < 32; ++i) x[i] = 0.f;
+    }
+    char* to = static_cast<char*>(w.diff) + (row * w.diff_stride + col) * 2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = two(x[16 * h + 2 * i], x[16 * h + 2 * i + 1], w.bf16);
+      store32(to + 32 * h, v);
+    }
+    return;
+  }
+  if (p.result == kSumHidden) {
+    float* to = w.sums + (split * static_cast<int64_t>(p.m) + row) * w.width + col;
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      if (col + i >= p.n) break;
+      float4 v = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+      if (w.add) {
+        const float4 o = *reinterpret_cast<const float4*>(to + i);
+        v              = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+      }
+      *reinterpret_cast<float4*>(to + i) = v;
+    }
+    return;
+  }
+  char* to = static_cast<char*>(p.result == kWeight ? w.grad_weight : w.grad_hidden) + (row * w.width + col) * 2;
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    if (col + i >= p.n) break;
+    uint4 v;
+    v.x = two(x[i] * factor, x[i + 1] * factor, w.bf16);
+    v.y = two(x[i + 2] * factor, x[i + 3] * factor, w.bf16);
+    v.z = two(x[i + 4] * factor, x[i + 5] * factor, w.bf16);
+    v.w = two(x[i + 6] * factor, x[i + 7] * factor, w.bf16);
+    *reinterpret_cast<uint4*>(to + 2 * i) = v;
+  }
+}
+
+// KIND: kStats, kDiff, or kWeight for the products of the gradients.
+template <int KIND>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) products(const __grid_constant__ Work w)
+{
+  extern __shared__ char raw[];
+  __shared__ __align__(8) uint64_t bars[2 * kStages + 5];
+  __shared__ uint32_t tmem_at;
+  __shared__ volatile int gave_up;
+  const uint32_t ring = (shared_of(raw) + 1023) & ~1023u;
+  const uint32_t full = shared_of(bars), empty = full + 8 * kStages, done = empty + 8 * kStages, freed = done + 16,
+                 last = freed + 16;
+  const uint32_t rank = rank_in_cluster();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int cluster = blockIdx.x / 2, clusters = gridDim.x / 2;
+  if (threadIdx.x == 0) {
+    gave_up = 0;
+    for (int i = 0; i < kStages; ++i) {
+      bar_init(full + 8 * i, 1);
+      bar_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      bar_init(done + 8 * i, 1);
+      bar_init(freed + 8 * i, 8);  // the four warps of both CTAs
+    }
+    bar_init(last, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(shared_of(&tmem_at)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_at;
+
+  if (warp == 0 && lane == 0) {
+    // tiles to the ring; the bytes of both CTAs are counted at the first one's barrier
+    const uint32_t count_at = in_cta(full, 0);
+    int stage = 0, phase = 0;
+    bool ok = true;
+    int issued = 0;
+    Tile t;
+    for (int i = cluster; ok && tile_of(w, i, t); i += clusters) {
+      const Product& p = w.product[t.which];
+      const int m0 = t.m * kTile + rank * kHalf, n0 = t.n * kTile + rank * kHalf;
+      for (int k = t.begin; k < t.end; ++k) {
+        if (!bar_wait(empty + 8 * stage, phase ^ 1, &gave_up)) {
+          ok = false;
+          break;
+        }
+        if (rank == 0) bar_expect(full + 8 * stage, 2 * kStage);
+        const uint32_t a = ring + stage * kStage, b = a + kStageA, bar = count_at + 8 * stage;
+        if (p.a_outer) {
+          load_box(a, &p.a, bar, m0, k * kDepth);
+          load_box(a + 8192, &p.a, bar, m0 + 64, k * kDepth);
+        } else {
+          load_box(a, &p.a, bar, k * kDepth, m0);
+        }
+        if (p.b_outer) {
+          load_box(b, &p.b, bar, n0, k * kDepth);
+          load_box(b + 8192, &p.b, bar, n0 + 64, k * kDepth);
+        } else {
+          load_box(b, &p.b, bar, k * kDepth, n0);
+        }
+        ++issued;
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    if (!ok && rank == 0) {
+      // copies in flight have to land before the CTA ends: the last phase of every stage that was filled
+      for (int i = 0; i < kStages && i < issued; ++i) {
+        const int n     = issued - 1 - i;
+        const long long until = now_ns() + kPatience;
+        while (!bar_try(full + 8 * (n % kStages), (n / kStages) & 1) && now_ns() < until) {}
+      }
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    int stage = 0, phase = 0, half = 0, turn = 0;
+    bool ok = true;
+    Tile t;
+    for (int i = cluster; ok && tile_of(w, i, t); i += clusters) {
+      const Product& p     = w.product[t.which];
+      const uint32_t idesc = instruction(w.bf16, p.a_outer, p.b_outer);
+      const uint64_t step_a = (p.a_outer ? 2048 : 32) >> 4, step_b = (p.b_outer ? 2048 : 32) >> 4;
+      if (!bar_wait(freed + 8 * half, turn ^ 1, &gave_up)) {
+        ok = false;
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      for (int k = t.begin; k < t.end; ++k) {
+        if (!bar_wait(full + 8 * stage, phase, &gave_up)) {
+          ok = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t a = descriptor(ring + stage * kStage, p.a_outer);
+        const uint64_t b = descriptor(ring + stage * kStage + kStageA, p.b_outer);
+#pragma unroll
+        for (int j = 0; j < kDepth / 16; ++j)
+          mma(tmem + half * kTile, a + j * step_a, b + j * step_b, idesc, k > t.begin || j > 0);
+        commit(empty + 8 * stage);
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (!ok) break;
+      commit(done + 8 * half);
+      half ^= 1;
+      turn ^= half == 0;
+    }
+    if (!ok) {  // products in flight have to end before TMEM is given back
+      commit(last);
+      const long long until = now_ns() + kPatience;
+      while (!bar_try(last, 0) && now_ns() < until) {}
+    }
+  } else if (warp >= 4) {
+    const int quarter     = warp - 4;
+    const uint32_t freed0 = in_cta(freed, 0);
+    int half = 0, turn = 0;
+    Tile t;
+    for (int i = cluster; tile_of(w, i, t); i += clusters) {
+      const Product& p  = w.product[t.which];
+      const int64_t row = static_cast<int64_t>(t.m) * kTile + rank * kHalf + quarter * 32 + lane;
+      const bool in     = row < p.m;
+      float base = 0.f, factor = 1.f;
+      if (KIND == kDiff && in) {
+        const float4 s = w.stats[row];
+        base           = base_of(s.x);
+        factor         = s.w == 0.f ? 0.f : s.y * w.diff_scale * (w.row_scale ? w.row_scale[row] : 1.f);
+      }
+      if (KIND == kWeight && p.result != kSumHidden) factor = *w.scale;
+      if (!__all_sync(~0u, bar_wait(done + 8 * half, turn, &gave_up))) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      Running<float> r;
+#pragma unroll 1
+      for (int c = 0; c < kTile; c += 32) {
+        const int col = t.n * kTile + c;
+        if (KIND != kDiff && col >= p.n) break;
+        float x[32];
+        load_columns(tmem + half * kTile + c + (static_cast<uint32_t>(quarter * 32) << 16), x);
+        if (in) take_columns<KIND>(w, p, t.split, row, col, x, r, base, factor);
+        __syncwarp();
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive_cluster(freed0 + 8 * half);
+      if (KIND == kStats && in) w.parts[row * p.n_tiles + t.n] = make_float2(r.m, r.s);
+      half ^= 1;
+      turn ^= half == 0;
+    }
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();
+  if (warp == 2) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// ---- rows ------------------------------------------------------------------------------------
+template <class T>
+__device__ __forceinline__ float dot_piece(const Piece<T>& a, const Piece<T>& b, float s)
+{
+#pragma unroll
+  for (int i = 0; i < Piece<T>::N; ++i) s = fmaf(widen(a.v[i]), widen(b.v[i]), s);
+  return s;
+}
+
+// Loss of a row from the maxima and sums of its tiles; the named classes' logits are dot products of
+// their own, a warp each.
+template <class T, int THREADS>
+__global__ void __launch_bounds__(kThreads) linear_rows(LinearArgs a, const float2* parts, int tiles, double2* block_sums)
+{
+  constexpr int ROWS = kThreads / THREADS, N = Piece<T>::N;
+  extern __shared__ __align__(16) char smem[];
+  const int slot = threadIdx.x / THREADS, tid = threadIdx.x % THREADS, lane = threadIdx.x % 32;
+  const int k        = a.teacher.k;
+  char* mine         = smem + slot * static_cast<size_t>(256 + (k + 1) / 2 * 2 * 12);
+  double* room       = reinterpret_cast<double*>(mine);
+  float* p           = reinterpret_cast<float*>(mine + 256);
+  int* at            = reinterpret_cast<int*>(p + k);
+  float* logit       = reinterpret_cast<float*>(at + k);
+  const float c      = 1.4426950408889634f / a.temperature;
+  const double inv_t = 1.0 / a.temperature;
+  double sum = 0, count = 0;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + slot; row < a.n_rows;
+       row += static_cast<int64_t>(gridDim.x) * ROWS) {
+    const TeacherRow t = read_teacher<THREADS>(a.teacher, row, a.n_cols, inv_t, tid, p, at, room);
+    const T* h         = static_cast<const T*>(a.hidden) + row * a.hidden_stride;
+    for (int j = tid / 32; j < k; j += THREADS / 32) {
+      const int cls = at[j];
+      float s       = 0.f;
+      if (cls >= 0) {
+        const T* v = static_cast<const T*>(a.weight) + cls * a.weight_stride;
+        for (int i = lane * N; i < a.width; i += 32 * N) s = dot_piece(load_piece(h + i), load_piece(v + i), s);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+      }
+      if (lane == 0) logit[j] = s;
+    }
+    Running<float> r;
+    for (int i = tid; i < tiles; i += THREADS) r.join(parts[row * tiles + i].x, parts[row * tiles + i].y, c);
+    join_row<THREADS>(r, c, reinterpret_cast<float*>(room));
+    sync_row<THREADS>();
+    const double log_s = log(static_cast<double>(r.s));
+    const bool counts  = t.counts && !(r.s == 0.f);
+    double loss        = 0;
+    for (int j = tid; j < k; j += THREADS) {
+      const int64_t to  = row * k + j;
+      a.named.logit[to] = logit[j];
+      a.named.p[to]     = p[j];
+      a.named.at[to]    = at[j];
+      if (at[j] < 0 || p[j] == 0.f) continue;
+      const double log_p = t.merged ? log(static_cast<double>(p[j]))
+                                    : (a.teacher.values ? a.teacher.values[row * a.teacher.values_stride + j] * inv_t : 0.0) - t.log_norm;
+      loss += p[j] * (log_p - ((static_cast<double>(logit[j]) - r.m) * inv_t - log_s));
+    }
+    loss = sum_row<THREADS>(loss, room);
+    if (!counts) loss = 0;
+    loss *= static_cast<double>(a.temperature) * a.temperature;
+    if (tid == 0) {
+      a.row_loss[row]  = static_cast<float>(loss);
+      a.row_stats[row] = make_float4(r.m, 1.f / r.s, 1.f, counts ? 1.f : 0.f);
+      sum += loss;
+      count += counts;
+    }
+  }
+  __shared__ double2 sums[ROWS];
+  if (tid == 0) sums[slot] = make_double2(sum, count);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double2 all = sums[0];
+    for (int i = 1; i < ROWS; ++i) {
+      all.x += sums[i].x;
+      all.y += sums[i].y;
+    }
+    block_sums[blockIdx.x] = all;
+  }
+}
+
+// Scales of the gradient.  One upstream value: *scale takes it all.  One per row: the rows' are brought below
+// 1 by a power of two, which *scale takes back, so that d stays in fp16's range.
+__global__ void __launch_bounds__(1024) grad_scales(LinearGradArgs g, float diff_scale, float* scale, float* row_scale)
+{
+  __shared__ float room[32];
+  const float t = g.fwd.temperature / diff_scale;
+  if (!row_scale) {
+    if (threadIdx.x == 0) *scale = *g.upstream * (g.factor ? *g.factor : 1.f) * t;
+    return;
+  }
+  float most = 0.f;
+  for (int64_t i = threadIdx.x; i < g.fwd.n_rows; i += 1024) most = fmaxf(most, fabsf(g.upstream[i * g.upstream_stride]));
+#pragma unroll
+  for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+  if (threadIdx.x % 32 == 0) room[threadIdx.x / 32] = most;
+  __syncthreads();
+  most = room[threadIdx.x % 32];
+#pragma unroll
+  for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+  int e = 0;
+  if (most > 0.f && most < INFINITY) frexpf(most, &e);
+  e              = max(-100, min(100, e));
+  const float up = ldexpf(1.f, e), down = ldexpf(1.f, -e);
+  if (threadIdx.x == 0) *scale = up * t;
+  for (int64_t i = threadIdx.x; i < g.fwd.n_rows; i += 1024) row_scale[i] = g.upstream[i * g.upstream_stride] * down;
+}
+
+// d of the classes that the teacher names, in a piece of the classes.
+template <class T>
+__global__ void __launch_bounds__(kThreads) named_diff(LinearArgs a, int64_t first, int64_t n, T* diff, int64_t stride,
+                                                       const float* row_scale, float diff_scale, float c)
+{
+  const int64_t all = a.n_rows * a.teacher.k;
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < all; i += gridDim.x * static_cast<int64_t>(kThreads)) {
+    const int cls = a.named.at[i];
+    if (cls < first || cls >= first + n) continue;
+    const int64_t row = i / a.teacher.k;
+    const float4 s    = a.row_stats[row];
+    if (s.w == 0.f) continue;
+    const float q = power((a.named.logit[i] - base_of(s.x)) * c) * s.y;
+    diff[row * stride + cls - first] = narrow<T>((q - a.named.p[i]) * diff_scale * (row_scale ? row_scale[row] : 1.f));
+  }
+}
+
+// dH from the sums of its parts.
+template <class T>
+__global__ void __launch_bounds__(kThreads) finish_hidden(const float* sums, int splits, int64_t n, const float* scale, T* out)
+{
+  const float f = *scale;
+  for (int64_t i = 4 * (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x); i < n; i += 4 * gridDim.x * static_cast<int64_t>(kThreads)) {
+    float4 v = *reinterpret_cast<const float4*>(sums + i);
+    for (int s = 1; s < splits; ++s) {
+      const float4 o = *reinterpret_cast<const float4*>(sums + s * n + i);
+      v              = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+    }
+    T r[4] = {narrow<T>(v.x * f), narrow<T>(v.y * f), narrow<T>(v.z * f), narrow<T>(v.w * f)};
+    *reinterpret_cast<uint2*>(out + i) = *reinterpret_cast<const uint2*>(r);
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) reduce_rows(const double2* block_sums, int n, Reduced out)
+{
+  __shared__ double room[32];
+  double sum = 0, count = 0;
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    sum += block_sums[i].x;
+    count += block_sums[i].y;
+  }
+  sum   = sum_row<kThreads>(sum, room);
+  count = sum_row<kThreads>(count, room);
+  if (threadIdx.x == 0) {
+    const double f = out.reduction == 1 ? 1.0 : count > 0 ? 1.0 / count : 0.0;
+    *out.loss      = static_cast<float>(count > 0 ? sum * f : 0.0);
+    *out.factor    = static_cast<float>(f);
+  }
+}
+
+__global__ void wait_for_nothing()
+{
+  __shared__ __align__(8) uint64_t bar;
+  __shared__ volatile int gave_up;
+  gave_up = 0;
+  bar_init(shared_of(&bar), 1);
+  bar_wait_long(shared_of(&bar), 0, &gave_up, 1000000ll);
+}
+
+// ---- host ------------------------------------------------------------------------------------
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder()
+{
+  static EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+// A matrix of `rows` rows of `cols` 16-bit elements, in boxes of 64 columns by box_rows rows.
+bool make_map(CUtensorMap* map, bool bf16, const void* base, int64_t rows, int64_t cols, int64_t stride, int box_rows)
+{
+  const EncodeFn encode    = encoder();
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t step[1] = {static_cast<cuuint64_t>(stride) * 2};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)}, one[2] = {1, 1};
+  return encode && encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                          const_cast<void*>(base), dims, step, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+int tiles_of(int64_t n) { return static_cast<int>((n + kTile - 1) / kTile); }
+
+template <int KIND>
+cudaError_t run_products(const Work& w, int n_sms, cudaStream_t s)
+{
+  const cudaError_t e = cudaFuncSetAttribute(products<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) return e;
+  int tiles = 0;
+  for (int i = 0; i < w.products; ++i) tiles += w.product[i].m_tiles * w.product[i].n_tiles * w.product[i].splits;
+  const int clusters = tiles < n_sms / 2 ? tiles : n_sms / 2;
+  products<KIND><<<2 * clusters, kThreads, kSmem, s>>>(w);
+  return cudaGetLastError();
+}
+
+// z = H W^T of the classes from `first` on
+bool logits_product(Product& p, bool bf16, const LinearArgs& a, int64_t first, int64_t n, int result)
+{
+  p.m       = static_cast<int>(a.n_rows);
+  p.n       = static_cast<int>(n);
+  p.depth   = static_cast<int>(a.width);
+  p.m_tiles = tiles_of(p.m);
+  p.n_tiles = tiles_of(p.n);
+  p.splits  = 1;
+  p.a_outer = p.b_outer = 0;
+  p.result  = result;
+  return make_map(&p.a, bf16, a.hidden, a.n_rows, a.width, a.hidden_stride, kHalf) &&
+         make_map(&p.b, bf16, static_cast<const char*>(a.weight) + first * a.weight_stride * 2, n, a.width, a.weight_stride, kHalf);
+}
+
+template <class T>
+cudaError_t run_linear(bool bf16, const LinearArgs& a, const Reduced& out, void* workspace, int n_sms, cudaStream_t s)
+{
+  double2* sums = static_cast<double2*>(workspace);
+  int launched = 0, blocks = 0;
+  if (a.n_rows > 0) {
+    Work w{};
+    w.products = 1;
+    w.bf16     = bf16;
+    w.c        = 1.4426950408889634f / a.temperature;
+    w.parts    = reinterpret_cast<float2*>(sums + 8 * n_sms);
+    if (!logits_product(w.product[0], bf16, a, 0, a.n_cols, kStats)) return cudaErrorInvalidValue;
+    cudaError_t e = run_products<kStats>(w, n_sms, s);
+    if (e != cudaSuccess) return e;
+    const bool warp    = a.teacher.k == 1;
+    const int per      = warp ? kThreads / 32 : 1;
+    const int64_t need = (a.n_rows + per - 1) / per;
+    blocks             = static_cast<int>(need < 8 * n_sms ? need : 8 * n_sms);
+    const size_t bytes = per * (256 + static_cast<size_t>(a.teacher.k + 1) / 2 * 2 * 12);
+    if (warp)
+      linear_rows<T, 32><<<blocks, kThreads, bytes, s>>>(a, w.parts, w.product[0].n_tiles, sums);
+    else
+      linear_rows<T, kThreads><<<blocks, kThreads, bytes, s>>>(a, w.parts, w.product[0].n_tiles, sums);
+    launched = 2;
+  }
+  if (out.reduction != 0) {
+    reduce_rows<<<1, kThreads, 0, s>>>(sums, blocks, out);
+    ++launched;
+  }
+  count_launches(launched);
+  return cudaGetLastError();
+}
+
+// How the classes are cut into pieces and the sums over them split.
+struct Plan {
+  int pieces;
+  int64_t cols;  // of a piece, a multiple of a tile
+  int splits;    // of dH's sum over a piece's classes
+  bool direct;   // dH needs no sums in memory
+};
+Plan plan_of(const LinearGradArgs& g, int n_sms)
+{
+  const LinearArgs& a = g.fwd;
+  Plan p;
+  int64_t most = kPieceBytes / 2 / (a.n_rows > 0 ? a.n_rows : 1) / kTile * kTile;
+  if (most < 2 * kTile) most = 2 * kTile;
+  p.pieces = static_cast<int>((a.n_cols + most - 1) / most);
+  p.cols   = static_cast<int64_t>(tiles_of((a.n_cols + p.pieces - 1) / p.pieces)) * kTile;
+  p.pieces = static_cast<int>((a.n_cols + p.cols - 1) / p.cols);
+  // as many parts as bring a part of dH down to an even share of the machine, 16 stages at least
+  const int64_t wide = tiles_of(a.width), dh_tiles = tiles_of(a.n_rows) * wide, dh_steps = p.cols / kDepth;
+  int64_t all = dh_tiles * dh_steps;
+  if (g.grad_weight) all += tiles_of(p.cols) * wide * ((a.n_rows + kDepth - 1) / kDepth);
+  int64_t share = all / (n_sms / 2);
+  if (share < 16) share = 16;
+  const int64_t splits = (dh_steps + share - 1) / share;
+  p.splits             = static_cast<int>(splits < 1 ? 1 : splits > kMostSplits ? kMostSplits : splits);
+  p.direct             = p.pieces == 1 && p.splits == 1;
+  return p;
+}
+int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+template <class T>
+cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace, int n_sms, cudaStream_t s)
+{
+  const LinearArgs& a  = g.fwd;
+  const Plan plan      = plan_of(g, n_sms);
+  char* at             = static_cast<char*>(workspace);
+  float* scale         = reinterpret_cast<float*>(at);
+  float* row_scale     = reinterpret_cast<float*>(at += 256);
+  T* diff              = reinterpret_cast<T*>(at += padded(a.n_rows * 4));
+  float* sums          = reinterpret_cast<float*>(at += padded(a.n_rows * plan.cols * 2));
+  const float d_scale  = bf16 ? 1.f : kHalfScale;
+  const bool per_row   = g.factor == nullptr;
+  int launched         = 1;
+  cudaError_t e        = cudaSuccess;
+  grad_scales<<<1, 1024, 0, s>>>(g, d_scale, scale, per_row ? row_scale : nullptr);
+  Work w{};
+  w.bf16        = bf16;
+  w.c           = 1.4426950408889634f / a.temperature;
+  w.stats       = a.row_stats;
+  w.row_scale   = per_row ? row_scale : nullptr;
+  w.diff        = diff;
+  w.diff_stride = plan.cols;
+  w.diff_scale  = d_scale;
+  w.sums        = sums;
+  w.grad_hidden = g.grad_hidden;
+  w.width       = a.width;
+  w.scale       = scale;
+  for (int i = 0; i < plan.pieces; ++i) {
+    const int64_t first = i * plan.cols, n = a.n_cols - first < plan.cols ? a.n_cols - first : plan.cols;
+    w.products = 1;
+    if (!logits_product(w.product[0], bf16, a, first, n, kDiff)) return cudaErrorInvalidValue;
+    if ((e = run_products<kDiff>(w, n_sms, s)) != cudaSuccess) return e;
+    const int64_t entries = a.n_rows * a.teacher.k;
+    const int64_t need    = (entries + kThreads - 1) / kThreads;
+    named_diff<T><<<static_cast<unsigned>(need < 8 * n_sms ? need : 8 * n_sms), kThreads, 0, s>>>(
+      a, first, n, diff, plan.cols, w.row_scale, d_scale, w.c);
+    // d ends with the tile that holds its last class: what is behind has not been written
+    const int64_t made = static_cast<int64_t>(tiles_of(n)) * kTile;
+    w.products         = 0;
+    const char* weight = static_cast<const char*>(a.weight) + first * a.weight_stride * 2;
+    if (g.grad_weight) {
+      Product& p = w.product[w.products++];
+      p.m        = static_cast<int>(n);
+      p.n        = static_cast<int>(a.width);
+      p.depth    = static_cast<int>(a.n_rows);
+      p.splits   = 1;
+      p.a_outer = p.b_outer = 1;
+      p.result  = kWeight;
+      if (!make_map(&p.a, bf16, diff, a.n_rows, made, plan.cols, 64) ||
+          !make_map(&p.b, bf16, a.hidden, a.n_rows, a.width, a.hidden_stride, 64))
+        return cudaErrorInvalidValue;
+    }
+    if (g.grad_hidden) {
+      Product& p = w.product[w.products++];
+      p.m        = static_cast<int>(a.n_rows);
+      p.n        = static_cast<int>(a.width);
+      p.depth    = static_cast<int>(made);
+      p.splits   = plan.splits;
+      p.a_outer  = 0;
+      p.b_outer  = 1;
+      p.result   = plan.direct ? kHidden : kSumHidden;
+      if (!make_map(&p.a, bf16, diff, a.n_rows, made, plan.cols, kHalf) ||
+          !make_map(&p.b, bf16, weight, n, a.width, a.weight_stride, 64))
+        return cudaErrorInvalidValue;
+    }
+    for (int j = 0; j < w.products; ++j) {
+      w.product[j].m_tiles = tiles_of(w.product[j].m);
+      w.product[j].n_tiles = tiles_of(w.product[j].n);
+    }
+    w.add         = i > 0;
+    w.grad_weight = g.grad_weight ? static_cast<T*>(g.grad_weight) + first * a.width : nullptr;
+    if (w.products && (e = run_products<kWeight>(w, n_sms, s)) != cudaSuccess) return e;
+    launched += 3;
+  }
+  if (g.grad_hidden && !plan.direct) {
+    const int64_t n = a.n_rows * a.width, need = (n / 4 + kThreads - 1) / kThreads;
+    finish_hidden<T><<<static_cast<unsigned>(need < 8 * n_sms ? need : 8 * n_sms), kThreads, 0, s>>>(
+      sums, plan.splits, n, scale, static_cast<T*>(g.grad_hidden));
+    ++launched;
+  }
+  count_launches(launched);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+size_t linear_workspace(const LinearArgs& a, int n_sms)
+{
+  return 8 * n_sms * sizeof(double2) + a.n_rows * static_cast<size_t>(tiles_of(a.n_cols)) * sizeof(float2);
+}
+
+size_t linear_grad_workspace(const LinearGradArgs& g, int n_sms)
+{
+  const LinearArgs& a = g.fwd;
+  const Plan p        = plan_of(g, n_sms);
+  return 256 + padded(a.n_rows * 4) + padded(a.n_rows * p.cols * 2) +
+         (g.grad_hidden && !p.direct ? p.splits * a.n_rows * a.width * sizeof(float) : 0);
+}
+
+cudaError_t launch_linear(int dtype, const LinearArgs& a, const Reduced& out, void* workspace, int n_sms, cudaStream_t s)
+{
+  return dtype == kBF16 ? run_linear<__nv_bfloat16>(true, a, out, workspace, n_sms, s)
+                        : run_linear<__half>(false, a, out, workspace, n_sms, s);
+}
+
+cudaError_t launch_linear_grad(int dtype, const LinearGradArgs& g, void* workspace, int n_sms, cudaStream_t s)
+{
+  return dtype == kBF16 ? run_linear_grad<__nv_bfloat16>(true, g, workspace, n_sms, s)
+                        : run_linear_grad<__half>(false, g, workspace, n_sms, s);
+}
+
+cudaError_t linear_status(int* status)
+{
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(status, g_status, sizeof(int));
+  if (e == cudaSuccess && *status != 0) {
+    const int zero = 0;
+    e              = cudaMemcpyToSymbol(g_status, &zero, sizeof(int));
+  }
+  return e;
+}
+
+cudaError_t launch_linear_timeout(cudaStream_t s)
+{
+  wait_for_nothing<<<1, 1, 0, s>>>();
+  return cudaGetLastError();
+}
+
+}  // namespace distill
+}  // namespace b2fil

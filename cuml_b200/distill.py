@@ -231,3 +231,124 @@ def distillation_loss(logits, top, *, temperature: float = 1.0, tail: str = "ren
         raise ValueError(f"tail='bucket' takes at most 2^20 classes, got {n_cols}")
     loss = _Loss.apply(x, values, index, lse, _temperature(temperature), _NO_CLASS, _reduction(reduction))
     return loss.view(shape) if reduction == "none" and len(shape) != 1 else loss
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, values, index, temperature, ignore, reduction):
+        lib, kind, dev = _lib.load(), _TYPES[hidden.dtype], hidden.device
+        (n, width), n_cols = hidden.shape, weight.shape[0]
+        t = _Teacher(n, dev, values, index, None, ignore)
+        k = t.c.k
+        ws = _workspace(lib.b2fil_linear_loss_workspace(kind, n, n_cols, width, k, dev.index), dev)
+        # kept for the gradient: statistics and the factor; the named classes' logits, probabilities and places
+        kept = torch.empty((4 * n + 4 + 3 * n * k,), dtype=torch.float32, device=dev)
+        rows = torch.empty((n,), dtype=torch.float32, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev) if reduction else rows
+        stats, factor, named = _kept(kept, n)
+        _lib.check(lib.b2fil_linear_loss(
+            kind, hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0), n, n_cols, width,
+            C.byref(t.c), temperature, reduction, rows.data_ptr(), stats, named, named + 4 * n * k, named + 8 * n * k,
+            loss.data_ptr(), factor if reduction else None, ws.data_ptr(), ws.numel(), dev.index, _stream(dev)))
+        ctx.save_for_backward(hidden, weight)
+        ctx.kept, ctx.options = kept, (temperature, reduction, k)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        hidden, weight = ctx.saved_tensors
+        temperature, reduction, k = ctx.options
+        lib, kind, dev = _lib.load(), _TYPES[hidden.dtype], hidden.device
+        (n, width), n_cols = hidden.shape, weight.shape[0]
+        of_hidden, of_weight = ctx.needs_input_grad[:2]
+        dh = torch.empty((n, width), dtype=hidden.dtype, device=dev) if of_hidden else None
+        dw = torch.empty((n_cols, width), dtype=hidden.dtype, device=dev) if of_weight else None
+        ws = _workspace(lib.b2fil_linear_loss_grad_workspace(kind, n, n_cols, width, k, of_hidden, of_weight, dev.index), dev)
+        g, stride = _upstream(g)
+        stats, factor, named = _kept(ctx.kept, n)
+        _lib.check(lib.b2fil_linear_loss_grad(
+            kind, hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0), n, n_cols, width, k,
+            temperature, stats, named, named + 4 * n * k, named + 8 * n * k, g.data_ptr(), stride,
+            factor if reduction else None, dh.data_ptr() if of_hidden else None, dw.data_ptr() if of_weight else None,
+            ws.data_ptr(), ws.numel(), dev.index, _stream(dev)))
+        return dh, dw, None, None, None, None, None
+
+
+def _kept(kept, n):
+    """Addresses of the statistics, the factor and the named classes' arrays in what a forward pass keeps."""
+    at = kept.data_ptr()
+    return at, at + 16 * n, at + 16 * n + 16
+
+
+_LAYER = (torch.bfloat16, torch.float16)
+
+
+def _layer(hidden, weight):
+    """(hidden (n, width), weight (n_classes, width), leading shape), checked, in rows that start on 16 bytes."""
+    if torch.is_autocast_enabled("cuda"):
+        t = torch.get_autocast_dtype("cuda")
+        hidden, weight = (x.to(t) if isinstance(x, torch.Tensor) and x.is_floating_point() else x for x in (hidden, weight))
+    _cuda("hidden", hidden, _LAYER)
+    _cuda("weight", weight, _LAYER, 2)
+    if hidden.dtype != weight.dtype or hidden.device != weight.device:
+        raise ValueError(f"hidden and weight differ in type or device: {hidden.dtype} on {hidden.device}, "
+                         f"{weight.dtype} on {weight.device}")
+    if hidden.ndim < 1 or hidden.shape[-1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"hidden must be (..., width) and weight (n_classes, width), got {tuple(hidden.shape)} and "
+                         f"{tuple(weight.shape)}")
+    shape, width = hidden.shape[:-1], weight.shape[1]
+    if hidden.ndim != 2:
+        hidden = hidden.reshape(-1, width)
+    if width % 8:  # zeros behind each row change no product
+        hidden, weight = (torch.nn.functional.pad(x, (0, 8 - width % 8)) for x in (hidden, weight))
+    return _tiled(hidden), _tiled(weight), shape
+
+
+def _tiled(x):
+    x = _rows(x)
+    if x.stride(0) % 8 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def linear_cross_entropy(hidden, weight, target, *, ignore_index: int = -100, reduction: str = "mean"):
+    """Softmax cross entropy of the logits `hidden @ weight.T` and `target`, without keeping the logits.
+
+    hidden : (..., width), weight : (n_classes, width), both bf16 or both fp16 (under autocast they are cast).
+    target : (...) int32 or int64 classes; rows whose target is `ignore_index` or outside [0, n_classes) do
+        not count (their hidden values must be finite: they take part in weight's gradient with zeros).
+    reduction : 'mean' over the rows that count (0 where none does), 'sum', or 'none': (...), 0 for others.
+
+    The loss is fp32; products are summed in fp32.  The gradients have the layer's type; the
+    differences softmax - target are rounded to it before they are multiplied."""
+    hidden, weight, shape = _layer(hidden, weight)
+    _cuda("target", target, (torch.int32, torch.int64))
+    if target.shape != shape:
+        raise ValueError(f"target must have shape {tuple(shape)}, got {tuple(target.shape)}")
+    if target.device != hidden.device:
+        raise ValueError(f"target is on {target.device}, hidden on {hidden.device}")
+    target = target.reshape(-1, 1)
+    loss = _Linear.apply(hidden, weight, None, target, 1.0, int(ignore_index), _reduction(reduction))
+    return loss.view(shape) if reduction == "none" and len(shape) != 1 else loss
+
+
+def linear_distillation_loss(hidden, weight, top, *, temperature: float = 1.0, reduction: str = "mean"):
+    """`distillation_loss` (with tail='renormalise') of the logits `hidden @ weight.T`, without keeping them.
+
+    hidden : (..., width), weight : (n_classes, width), both bf16 or both fp16 (under autocast they are cast).
+    top, temperature, reduction : as in `distillation_loss`; types and rounding as in
+    `linear_cross_entropy`."""
+    hidden, weight, shape = _layer(hidden, weight)
+    values, index, _ = _top(top, hidden.shape[0], hidden.device, "renormalise")
+    loss = _Linear.apply(hidden, weight, values, index, _temperature(temperature), _NO_CLASS, _reduction(reduction))
+    return loss.view(shape) if reduction == "none" and len(shape) != 1 else loss
+
+
+def check_status(device=None) -> None:
+    """Wait for all work on `device` and raise `B2FilError` (code -7) if a bounded wait inside a kernel of the
+    linear losses ran out since the last check."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    word = C.c_int32(0)
+    index = torch.cuda.current_device() if device.index is None else device.index
+    _lib.check(_lib.load().b2fil_distill_status(index, C.byref(word)))

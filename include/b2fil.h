@@ -410,6 +410,40 @@ int b2fil_distill_loss_grad(int dtype, const void* logits, int64_t n_rows, int64
                             const float* factor, void* grad, int64_t grad_stride, int device_id,
                             void* cuda_stream);
 
+/* The same loss of logits = hidden * weight^T that are not kept: hidden (n_rows, width), weight (n_cols,
+ * width), both B2FIL_TYPE_BF16 or both B2FIL_TYPE_F16, sums in 32 bits.  width is a multiple of 8; rows
+ * start on 16 bytes (both strides are multiples of 8).  teacher->logsumexp must be NULL.  named_logit,
+ * named_p (float) and named_at (int32), (n_rows, k) each, keep what the gradient needs of the named
+ * classes.  n_rows < 2^31 - 256, n_cols < 2^31 - 256, width <= 2^20. */
+int64_t b2fil_linear_loss_workspace(int dtype, int64_t n_rows, int64_t n_cols, int64_t width, int k, int device_id);
+int b2fil_linear_loss(int dtype, const void* hidden, int64_t hidden_stride, const void* weight,
+                      int64_t weight_stride, int64_t n_rows, int64_t n_cols, int64_t width,
+                      const b2fil_teacher* teacher, double temperature, int reduction, float* row_loss,
+                      float* row_stats, float* named_logit, float* named_p, int32_t* named_at, float* loss,
+                      float* factor, void* workspace, int64_t workspace_bytes, int device_id,
+                      void* cuda_stream);
+
+/* Its gradients by hidden, to grad_hidden (n_rows, width), and by weight, to grad_weight (n_cols, width),
+ * both contiguous, 16-byte aligned and of the layer's type; either may be NULL (in both calls).  The
+ * differences softmax - teacher are rounded to the layer's type before they are multiplied. */
+int64_t b2fil_linear_loss_grad_workspace(int dtype, int64_t n_rows, int64_t n_cols, int64_t width, int k,
+                                         int wants_hidden, int wants_weight, int device_id);
+int b2fil_linear_loss_grad(int dtype, const void* hidden, int64_t hidden_stride, const void* weight,
+                           int64_t weight_stride, int64_t n_rows, int64_t n_cols, int64_t width,
+                           int k, double temperature, const float* row_stats,
+                           const float* named_logit, const float* named_p, const int32_t* named_at,
+                           const float* upstream, int64_t upstream_stride, const float* factor,
+                           void* grad_hidden, void* grad_weight, void* workspace,
+                           int64_t workspace_bytes, int device_id, void* cuda_stream);
+
+/* Waits for all work on device_id, reads the status word of the linear loss's kernels there and returns
+ * B2FIL_ERR_TIMEOUT when a bounded wait inside one ran out (its outputs are then incomplete); the
+ * word is cleared by the read. */
+int b2fil_distill_status(int device_id, int32_t* status);
+
+/* Self test of that report: enqueues a kernel whose only work is a bounded wait that nothing ends. */
+int b2fil_distill_selftest_timeout(int device_id, void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif
