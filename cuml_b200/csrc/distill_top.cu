@@ -2,25 +2,36 @@
 // log-sum-exp.
 //
 // Every score gets a key that no other of its row has: its value as an ordered integer, then the
-// complement of its class.  NaN is above everything, -0 equals +0.  The thread t of a block sees the
-// elements of its own group; the k-th largest of the groups' best keys is a bound tau that at least k
-// elements reach, and all that reach it lie in the k groups whose best does: only these are read
-// again (from L1 or L2).  Random rows leave little more than k candidates, which are sorted; where there
-// are more than the list holds, the k-th key itself is found bit by bit.
+// complement of its class.  NaN is above everything, -0 equals +0.
+//
+// A row is taken by a block, or where it is short by a warp, whose threads see one group of its elements
+// each.  A bound tau that at least k, and hardly more, of the groups' best keys reach is found bit by bit
+// (a vote per bit, until few too many are left); at least k elements reach it, and all that do lie in
+// those groups: only these are read again, from L1 or L2, dealt out anew to all threads.  Random rows
+// leave little more than k candidates whatever the row's length; each finds its place by counting the larger
+// ones.  Where there are more than the list holds, the k-th key itself is found bit by bit.  Rows of a
+// few classes are taken by one thread each, from a tile in shared memory, which keeps its best sorted in
+// registers.
 //
 // Bound by memory: one pass over the scores, which also takes the running maximum and sum of the
 // log-sum-exp (the maximum is the thread's best score, so that both cost one comparison per 16 bytes).
-// A block takes a segment of a row; the lists of several segments are joined by a second kernel.
+// Where rows are few, several blocks share one and a second kernel joins their lists.
 #include "distill_common.cuh"
 
 namespace b2fil {
 namespace distill {
 namespace {
 
-constexpr int kThreads  = 256;   // groups: at least the largest k
-constexpr int kSegment  = 16384; // largest part of a row that one block takes
-constexpr int kList     = 2048;  // candidates that a block sorts
+constexpr int kThreads  = 256;   // groups of a block: at least the largest k
+constexpr int kList     = 2048;  // candidates of a block
+constexpr int kWarpList = 256;   // candidates of a warp
+constexpr int kWarpCols = 1024;  // longest rows and largest k that a warp takes
+constexpr int kWarpTop  = 24;
+constexpr int kSlack    = 8;     // groups more than k that end the search of the bound
 constexpr int kInFlight = 4;
+constexpr int kTileRows = 128;   // rows of a tile for one thread each, their most classes and k
+constexpr int kTileCols = 48;
+constexpr int kTileTop  = 8;
 static_assert(kThreads >= kMostTop, "a group per entry");
 
 // ---- keys ----------------------------------------------------------------------------------
@@ -56,7 +67,6 @@ struct Key32 {
   __device__ __forceinline__ bool above(const Key32& o) const { return w > o.w; }
   __device__ __forceinline__ float value() const { return from_ordered(static_cast<uint32_t>(w >> 32)); }
   __device__ __forceinline__ uint32_t index() const { return ~static_cast<uint32_t>(w); }
-  __device__ __forceinline__ Key32 lane_xor(int d) const { return {__shfl_xor_sync(~0u, w, d)}; }
   static constexpr int kBits = 64;
   __device__ __forceinline__ Key32 with(int bit) const { return {w | 1ull << bit}; }
 };
@@ -68,7 +78,6 @@ struct Key64 {
   __device__ __forceinline__ bool above(const Key64& o) const { return v > o.v || (v == o.v && i > o.i); }
   __device__ __forceinline__ double value() const { return from_ordered(v); }
   __device__ __forceinline__ uint32_t index() const { return ~i; }
-  __device__ __forceinline__ Key64 lane_xor(int d) const { return {__shfl_xor_sync(~0u, v, d), __shfl_xor_sync(~0u, i, d)}; }
   static constexpr int kBits = 96;
   __device__ __forceinline__ Key64 with(int bit) const
   {
@@ -102,29 +111,6 @@ __device__ void sort_list(K* list, int n)
     }
   }
 }
-// One key per thread of the block, descending by thread; `room`: kThreads keys.
-template <class K>
-__device__ K sort_threads(K x, K* room)
-{
-  const int t = threadIdx.x;
-  for (int size = 2; size <= kThreads; size <<= 1) {
-    const bool down = (t & size) == 0;
-    for (int d = size >> 1; d; d >>= 1) {
-      K y;
-      if (d >= 32) {
-        __syncthreads();
-        room[t] = x;
-        __syncthreads();
-        y = room[t ^ d];
-      } else {
-        y = x.lane_xor(d);
-      }
-      const bool first = (t & d) == 0;
-      if ((first == down) == y.above(x)) x = y;
-    }
-  }
-  return x;
-}
 
 template <class V>
 __device__ __forceinline__ V log_of(V x);
@@ -133,16 +119,7 @@ __device__ __forceinline__ float log_of(float x) { return logf(x); }
 template <>
 __device__ __forceinline__ double log_of(double x) { return log(x); }
 
-// What a score adds to the sum: exp((x - m) / T), or x^(1/T) for a probability.
-template <class V>
-__device__ __forceinline__ V term(V x, V m, V c, bool prob, bool plain)
-{
-  if (!prob) return power((x - base_of(m)) * c);
-  // (the exponent of a probability is taken from its logarithm; T = 1 needs neither)
-  return plain ? x : x == V(0) ? V(0) : power(log_of(x) * c);
-}
-
-// Writes the sorted keys of a row.
+// Writes entry j of a row.
 template <class T, class K>
 __device__ __forceinline__ void write_top(const TopArgs& a, int64_t row, int j, const K& key)
 {
@@ -152,9 +129,30 @@ __device__ __forceinline__ void write_top(const TopArgs& a, int64_t row, int j, 
   static_cast<T*>(a.values)[row * a.k + j] = narrow<T>(v);
   a.index[row * a.k + j]                   = static_cast<int32_t>(key.index());
 }
-// m, s: of exp((x - m) / T), or of x^(1/T) (m unused); best: the row's largest key.
+
+// The sum over a row: of exp((x - m) / T) beside the maximum m, or of the probabilities' x^(1/T).  Probabilities
+// add up to nearly 1, whose logarithm is a difference: at T = 1 their sum keeps what each addition drops.
+template <class V, bool PROB>
+struct Sum {
+  Running<V> r;  // PROB: m is the largest, s the sum
+  V dropped = V(0);
+  __device__ __forceinline__ void add(V x, V c, bool plain)
+  {
+    if (!PROB) {
+      r.s += power((x - base_of(r.m)) * c);
+    } else if (plain) {
+      const V t = r.s + x, b = t - r.s;
+      dropped += (r.s - (t - b)) + (x - b);
+      r.s = t;
+    } else {
+      r.s += x == V(0) ? V(0) : power(log_of(x) * c);
+    }
+  }
+};
+
+// log-sum-exp of a row from its sum; best: the row's largest key.
 template <class V, class K>
-__device__ __forceinline__ void write_lse(const TopArgs& a, int64_t row, V m, V s, const K& best)
+__device__ __forceinline__ void write_lse(const TopArgs& a, int64_t row, V s, double dropped, const K& best)
 {
   if (!a.logsumexp) return;
   const V top = best.value();
@@ -162,122 +160,160 @@ __device__ __forceinline__ void write_lse(const TopArgs& a, int64_t row, V m, V 
   if (top != top)
     r = top;
   else if (a.probabilities)
-    r = log_of(s);
+    r = static_cast<V>(log(static_cast<double>(s) + dropped));
   else
     r = top == lowest<V>() || top == -lowest<V>() ? top : static_cast<V>(top * a.inv_temperature) + log_of(s);
   static_cast<V*>(a.logsumexp)[row] = r;
 }
 
-// A segment of a row per block.  segs == 1: the row's answer; else its k best keys and its sum.
-template <class T>
-__global__ void __launch_bounds__(kThreads) top_segments(TopArgs a, int64_t seg_cols, typename KeyOf<T>::type* keys,
-                                                         typename ValueOf<T>::type* sums)
+// How many of the row's threads say yes.
+template <int THREADS>
+__device__ __forceinline__ int count_row(bool yes)
+{
+  if (THREADS == 32) return __popc(__ballot_sync(~0u, yes));
+  return __syncthreads_count(yes);
+}
+
+// What a row's threads share.
+template <class K, int LIST, int GROUPS>
+struct RowShared {
+  K list[LIST];
+  int16_t groups[GROUPS];
+  int found, chosen;
+};
+
+// A segment of a row per block or warp.  segs == 1: the row's answer; else its k best keys and its sum.
+template <class T, int THREADS, bool PROB>
+__global__ void __launch_bounds__(kThreads) top_segments(TopArgs a, int segs, int64_t seg_cols,
+                                                         typename KeyOf<T>::type* keys, double* sums)
 {
   using V = typename ValueOf<T>::type;
   using K = typename KeyOf<T>::type;
-  __shared__ K list[kList];
-  __shared__ V room[64];
-  __shared__ int found;
-  const int segs      = gridDim.x;
-  const int64_t begin = blockIdx.x * seg_cols;
+  constexpr int ROWS = kThreads / THREADS, N = Piece<T>::N;
+  constexpr int LIST = THREADS == 32 ? kWarpList : kList;
+  __shared__ RowShared<K, LIST, THREADS> shared[ROWS];
+  __shared__ double room[64];
+  const int slot = threadIdx.x / THREADS, tid = threadIdx.x % THREADS;
+  RowShared<K, LIST, THREADS>& mine = shared[slot];
+  const int seg       = blockIdx.x % segs;
+  const int64_t begin = seg * seg_cols;
   const int64_t n     = min(seg_cols, a.n_cols - begin);
   const int k         = static_cast<int>(min(static_cast<int64_t>(a.k), n));
   const V c           = static_cast<V>(1.4426950408889634 * a.inv_temperature);
   const bool plain    = a.inv_temperature == 1.0;
-  const bool prob     = a.probabilities;
-  for (int64_t row = blockIdx.y; row < a.n_rows; row += gridDim.y) {
-    const T* x = static_cast<const T*>(a.scores) + row * a.row_stride + begin;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x / segs) * ROWS + slot; row < a.n_rows;
+       row += static_cast<int64_t>(gridDim.x / segs) * ROWS) {
+    const T* x       = static_cast<const T*>(a.scores) + row * a.row_stride + begin;
+    const int lead   = lead_of(x, n);
+    const int pieces = static_cast<int>((n - lead) / N);
+    const T* body    = x + lead;
     // the thread's best score and its place, and the sum
-    Running<V> r;
-    uint32_t at  = ~0u;  // none yet
-    bool nan     = false;
+    Sum<V, PROB> sum;
+    uint32_t at = ~0u;  // none yet
+    auto raise  = [&](V v) {
+      if (PROB)
+        sum.r.m = v;
+      else
+        sum.r.raise(v, c);
+    };
     visit_row<kInFlight>(
-      x, n, threadIdx.x, kThreads,
+      x, n, tid, THREADS,
       [&](int64_t i, T e) {
         const V v = widen(e);
-        nan |= v != v;
-        if (v > r.m || at == ~0u) {
-          if (!prob && v > r.m) r.raise(v, c);
-          r.m = larger(r.m, v);
-          at  = static_cast<uint32_t>(i);
+        if (v > sum.r.m || at == ~0u) {
+          if (v > sum.r.m) raise(v);
+          at = static_cast<uint32_t>(i);
         }
-        r.s += term(v, r.m, c, prob, plain);
+        sum.add(v, c, plain);
       },
       [&](int64_t i, const Piece<T>& p) {
-        constexpr int N = Piece<T>::N;
         V v[N], most;
 #pragma unroll
         for (int e = 0; e < N; ++e) v[e] = widen(p.v[e]);
         most = v[0];
 #pragma unroll
         for (int e = 1; e < N; ++e) most = larger(most, v[e]);
-        if (most > r.m || at == ~0u) {
-          if (!prob && most > r.m) r.raise(most, c);
-          r.m = larger(r.m, most);
-          at  = static_cast<uint32_t>(i);
+        if (most > sum.r.m || at == ~0u) {
+          if (most > sum.r.m) raise(most);
+          at = static_cast<uint32_t>(i);
 #pragma unroll
           for (int e = N - 1; e >= 0; --e)
             if (v[e] == most) at = static_cast<uint32_t>(i + e);
         }
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          nan |= v[e] != v[e];
-          r.s += term(v[e], r.m, c, prob, plain);
-        }
+        for (int e = 0; e < N; ++e) sum.add(v[e], c, plain);
       });
     K best = K::none();
-    if (nan) {  // the first NaN of the group is its best
+    if (at != ~0u) best = K::of(sum.r.m, static_cast<uint32_t>(begin) + at);
+    if (sum.r.s != sum.r.s) {  // a NaN, or infinities: the first NaN of the group is its best
       uint32_t first = ~0u;
       visit_row<1>(
-        x, n, threadIdx.x, kThreads,
+        x, n, tid, THREADS,
         [&](int64_t i, T e) {
           if (widen(e) != widen(e)) first = min(first, static_cast<uint32_t>(i));
         },
         [&](int64_t i, const Piece<T>& p) {
 #pragma unroll
-          for (int e = 0; e < Piece<T>::N; ++e)
+          for (int e = 0; e < N; ++e)
             if (widen(p.v[e]) != widen(p.v[e])) first = min(first, static_cast<uint32_t>(i + e));
         });
-      best = K::of(static_cast<V>(NAN), static_cast<uint32_t>(begin) + first);
-    } else if (at != ~0u) {
-      best = K::of(r.m, static_cast<uint32_t>(begin) + at);
+      if (first != ~0u) best = K::of(static_cast<V>(NAN), static_cast<uint32_t>(begin) + first);
     }
-    if (prob) {
-      r.s = sum_row<kThreads>(r.s, room);
-      r.m = V(0);
+    double dropped = 0;
+    if (PROB) {
+      // (in 64 bits: see Sum)
+      dropped = sum_row<THREADS>(static_cast<double>(sum.r.s) + sum.dropped, room);
+      sum.r.s = V(0);
     } else {
-      join_row<kThreads>(r, c, room);
+      join_row<THREADS>(sum.r, c, reinterpret_cast<V*>(room));
     }
-    // tau: the k-th largest of the groups' best keys (no key where there are fewer groups)
-    const K mine = sort_threads(best, list);
-    __syncthreads();
-    if (threadIdx.x == k - 1) list[0] = mine;
-    if (threadIdx.x == 0) found = 0;
-    __syncthreads();
-    const K tau = list[0];
-    __syncthreads();
-    auto collect = [&](const K& bound, bool store) {
+    // tau: a bound that k groups reach, and at most kSlack more unless its last bit is reached
+    K tau = K::none();
+    const int seen = count_row<THREADS>(at != ~0u);
+    if (seen > k + kSlack || (seen > k && n > LIST)) {
+      for (int bit = K::kBits - 1; bit >= 0; --bit) {
+        const K next  = tau.with(bit);
+        const int got = count_row<THREADS>(!next.above(best));
+        if (got < k) continue;
+        tau = next;
+        if (got <= k + kSlack) break;
+      }
+    }
+    if (tid == 0) mine.found = mine.chosen = 0;
+    sync_row<THREADS>();
+    const bool reaches = at != ~0u && !tau.above(best);
+    if (reaches) mine.groups[atomicAdd(&mine.chosen, 1)] = static_cast<int16_t>(tid);
+    sync_row<THREADS>();
+    const int chosen = mine.chosen;
+    // pieces of a group: the same number of all, those behind the last are left out below
+    const int per = (pieces + THREADS - 1) / THREADS;
+    auto collect  = [&](const K& bound, bool store) {
       auto take = [&](int64_t i, T e) {
         const K key = K::of(widen(e), static_cast<uint32_t>(begin + i));
-        if (!bound.above(key)) {
-          const int to = atomicAdd(&found, 1);
-          if (store && to < kList) list[to] = key;
-        }
+        if (bound.above(key)) return;
+        const int to = atomicAdd(&mine.found, 1);
+        if (store && to < LIST) mine.list[to] = key;
       };
-      if (!bound.above(best))
-        visit_row<1>(x, n, threadIdx.x, kThreads, take, [&](int64_t i, const Piece<T>& p) {
+      for (int i = tid; i < chosen * per; i += THREADS) {
+        const int p = mine.groups[i / per] + i % per * THREADS;
+        if (p >= pieces) continue;
+        const Piece<T> v = load_piece(body + static_cast<int64_t>(p) * N);
 #pragma unroll
-          for (int e = 0; e < Piece<T>::N; ++e) take(i + e, p.v[e]);
-        });
-      __syncthreads();
-      const int got = found;
-      __syncthreads();
-      if (threadIdx.x == 0) found = 0;
-      __syncthreads();
+        for (int e = 0; e < N; ++e) take(lead + static_cast<int64_t>(p) * N + e, v.v[e]);
+      }
+      // the elements before the first and behind the last boundary
+      if (tid < lead) take(tid, x[tid]);
+      const int64_t end = lead + static_cast<int64_t>(pieces) * N + tid;
+      if (end < n) take(end, x[end]);
+      sync_row<THREADS>();
+      const int got = mine.found;
+      sync_row<THREADS>();
+      if (tid == 0) mine.found = 0;
+      sync_row<THREADS>();
       return got;
     };
     int got = collect(tau, true);
-    if (got > kList) {
+    if (got > LIST) {
       // the largest bound that k keys reach, bit by bit: keys differ, so exactly k do
       K bound = K::none();
       for (int bit = K::kBits - 1; bit >= 0; --bit) {
@@ -286,36 +322,42 @@ __global__ void __launch_bounds__(kThreads) top_segments(TopArgs a, int64_t seg_
       }
       got = collect(bound, true);
     }
-    int size = 1;
-    while (size < got) size <<= 1;
-    for (int i = got + threadIdx.x; i < size; i += kThreads) list[i] = K::none();
-    __syncthreads();
-    sort_list(list, size);
-    if (segs == 1) {
-      for (int j = threadIdx.x; j < a.k; j += kThreads) write_top<T>(a, row, j, list[j]);
-      if (threadIdx.x == 0) write_lse(a, row, r.m, r.s, list[0]);
-    } else {
-      const int64_t part = row * segs + blockIdx.x;
-      for (int j = threadIdx.x; j < a.k; j += kThreads) keys[part * a.k + j] = j < k ? list[j] : K::none();
-      if (threadIdx.x == 0) {
-        sums[2 * part]     = r.m;
-        sums[2 * part + 1] = r.s;
+    // a candidate's place is the number of larger ones
+    const int64_t part = row * segs + seg;
+    for (int i = tid; i < got; i += THREADS) {
+      const K key = mine.list[i];
+      int place   = 0;
+#pragma unroll 4
+      for (int j = 0; j < got; ++j) place += mine.list[j].above(key);
+      if (place >= k) continue;
+      if (segs == 1) {
+        write_top<T>(a, row, place, key);
+        if (place == 0) write_lse(a, row, sum.r.s, dropped, key);
+      } else {
+        keys[part * a.k + place] = key;
       }
     }
-    __syncthreads();
+    if (segs > 1) {
+      for (int j = k + tid; j < a.k; j += THREADS) keys[part * a.k + j] = K::none();
+      if (tid == 0) {
+        sums[2 * part]     = PROB ? dropped : static_cast<double>(sum.r.s);
+        sums[2 * part + 1] = sum.r.m;
+      }
+    }
+    sync_row<THREADS>();
   }
 }
 
 // Joins the segments' lists of a row: as many as fit are sorted with the best so far.
 template <class T>
 __global__ void __launch_bounds__(kThreads) top_join(TopArgs a, int segs, const typename KeyOf<T>::type* keys,
-                                                     const typename ValueOf<T>::type* sums)
+                                                     const double* sums)
 {
   using V = typename ValueOf<T>::type;
   using K = typename KeyOf<T>::type;
   __shared__ K list[kList];
-  __shared__ V room[64];
-  const V c = static_cast<V>(1.4426950408889634 * a.inv_temperature);
+  __shared__ double room[64];
+  const double c = 1.4426950408889634 * a.inv_temperature;
   for (int64_t row = blockIdx.x; row < a.n_rows; row += gridDim.x) {
     const K* from = keys + row * segs * a.k;
     const int all = segs * a.k;
@@ -331,9 +373,9 @@ __global__ void __launch_bounds__(kThreads) top_join(TopArgs a, int segs, const 
       have = min(a.k, have + more);
     }
     for (int j = threadIdx.x; j < a.k; j += kThreads) write_top<T>(a, row, j, list[j]);
-    Running<V> r;
+    Running<double> r;
     for (int i = threadIdx.x; i < segs; i += kThreads) {
-      const V m = sums[2 * (row * segs + i)], s = sums[2 * (row * segs + i) + 1];
+      const double s = sums[2 * (row * segs + i)], m = sums[2 * (row * segs + i) + 1];
       if (a.probabilities)
         r.s += s;
       else
@@ -343,41 +385,149 @@ __global__ void __launch_bounds__(kThreads) top_join(TopArgs a, int segs, const 
       r.s = sum_row<kThreads>(r.s, room);
     else
       join_row<kThreads>(r, c, room);
-    if (threadIdx.x == 0) write_lse(a, row, r.m, r.s, list[0]);
+    if (threadIdx.x == 0) write_lse(a, row, static_cast<V>(a.probabilities ? 0.0 : r.s), a.probabilities ? r.s : 0.0, list[0]);
     __syncthreads();
   }
 }
 
-// Parts of a row: enough blocks to fill the machine, none below 2048 elements or above kSegment.
+// Ordered integers of one thread's best scores.
+template <class V>
+struct Ordered {
+  using type = uint32_t;
+};
+template <>
+struct Ordered<double> {
+  using type = uint64_t;
+};
+
+// A row per thread: n_cols <= kTileCols, k <= TOP.
+template <class T, int TOP, bool PROB>
+__global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
+{
+  using V = typename ValueOf<T>::type;
+  using K = typename KeyOf<T>::type;
+  using O = typename Ordered<V>::type;
+  extern __shared__ __align__(16) char smem[];
+  T* tile       = reinterpret_cast<T*>(smem);
+  const int c_n = static_cast<int>(a.n_cols);
+  // rows an odd number of words apart fall into different banks
+  const int pitch = sizeof(T) >= 4 ? c_n | 1 : (c_n + 1) / 2 * 2 + ((c_n + 1) / 2 % 2 ? 0 : 2);
+  const V c       = static_cast<V>(1.4426950408889634 * a.inv_temperature);
+  const bool plain = a.inv_temperature == 1.0;
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kTileRows; first < a.n_rows;
+       first += static_cast<int64_t>(gridDim.x) * kTileRows) {
+    const int rows = static_cast<int>(min(static_cast<int64_t>(kTileRows), a.n_rows - first));
+    const T* from  = static_cast<const T*>(a.scores) + first * a.row_stride;
+    __syncthreads();  // the last tile has been used
+    {
+      int r = threadIdx.x / c_n, i = threadIdx.x % c_n;
+      const int dr = kTileRows / c_n, di = kTileRows % c_n;
+      while (r < rows) {
+        tile[r * pitch + i] = from[r * a.row_stride + i];
+        r += dr;
+        i += di;
+        if (i >= c_n) {
+          i -= c_n;
+          ++r;
+        }
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x >= rows) continue;
+    const T* x = tile + threadIdx.x * pitch;
+    O key[TOP];
+    int at[TOP];
+#pragma unroll
+    for (int j = 0; j < TOP; ++j) {
+      key[j] = 0;
+      at[j]  = 0;
+    }
+    for (int i = 0; i < c_n; ++i) {
+      O o = ordered(widen(x[i]));
+      if (o <= key[TOP - 1]) continue;  // (equal ones: the earlier class stays)
+      int p   = i;
+      bool up = false;  // all entries behind the new one move down
+#pragma unroll
+      for (int j = 0; j < TOP; ++j) {
+        up |= o > key[j];
+        const O ko    = key[j];
+        const int ka  = at[j];
+        key[j]        = up ? o : ko;
+        at[j]         = up ? p : ka;
+        o             = up ? ko : o;
+        p             = up ? ka : p;
+      }
+    }
+    Sum<V, PROB> sum;
+    sum.r.m        = from_ordered(key[0]);
+    double dropped = 0;
+    if (PROB && plain) {
+      for (int i = 0; i < c_n; ++i) dropped += static_cast<double>(widen(x[i]));
+    } else {
+      for (int i = 0; i < c_n; ++i) sum.add(widen(x[i]), c, plain);
+    }
+    const int64_t row = first + threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < TOP; ++j)
+      if (j < a.k) write_top<T>(a, row, j, K::of(from_ordered(key[j]), static_cast<uint32_t>(at[j])));
+    write_lse(a, row, sum.r.s, dropped, K::of(from_ordered(key[0]), 0u));
+  }
+}
+
+// Parts of a row: enough blocks to fill the machine, none below 2048 elements.
 int segments(int64_t n_rows, int64_t n_cols, int n_sms)
 {
-  const int64_t least = (n_cols + kSegment - 1) / kSegment;
-  const int64_t fill  = (4 * n_sms + n_rows - 1) / (n_rows ? n_rows : 1);
-  const int64_t most  = (n_cols + 2047) / 2048;
-  const int64_t segs  = fill < most ? fill : most;
-  return static_cast<int>(segs < least ? least : segs);
+  if (n_rows == 0) return 1;
+  const int64_t fill = (4 * n_sms + n_rows - 1) / n_rows;
+  const int64_t most = (n_cols + 2047) / 2048;
+  const int64_t segs = fill < most ? fill : most;
+  return static_cast<int>(n_rows >= 2 * n_sms || segs < 1 ? 1 : segs);
 }
 int64_t part_cols(int64_t n_cols, int segs)
 {
   return segs == 1 ? n_cols : ((n_cols + segs - 1) / segs + 63) / 64 * 64;
 }
 
+template <class T, int TOP>
+cudaError_t run_tiles(const TopArgs& a, int n_sms, cudaStream_t s)
+{
+  const size_t bytes   = (a.n_cols + 3) * kTileRows * sizeof(T);
+  const int64_t blocks = (a.n_rows + kTileRows - 1) / kTileRows, most = 16ll * n_sms;
+  const auto kernel    = a.probabilities ? top_tiles<T, TOP, true> : top_tiles<T, TOP, false>;
+  if (bytes > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (e != cudaSuccess) return e;
+  }
+  kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), kTileRows, bytes, s>>>(a);
+  count_launches(1);
+  return cudaGetLastError();
+}
+
 template <class T>
 cudaError_t run_top(const TopArgs& a, void* workspace, int n_sms, cudaStream_t s)
 {
   using K = typename KeyOf<T>::type;
-  using V = typename ValueOf<T>::type;
+  if (a.n_cols <= kTileCols && a.k <= kTileTop) {
+    if (a.k == 1) return run_tiles<T, 1>(a, n_sms, s);
+    if (a.k <= 4) return run_tiles<T, 4>(a, n_sms, s);
+    return run_tiles<T, kTileTop>(a, n_sms, s);
+  }
+  if (a.n_cols <= kWarpCols && a.k <= kWarpTop) {
+    const int64_t need = (a.n_rows + kThreads / 32 - 1) / (kThreads / 32), most = 16ll * n_sms;
+    const auto kernel  = a.probabilities ? top_segments<T, 32, true> : top_segments<T, 32, false>;
+    kernel<<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(a, 1, a.n_cols, nullptr, nullptr);
+    count_launches(1);
+    return cudaGetLastError();
+  }
   int segs           = segments(a.n_rows, a.n_cols, n_sms);
   const int64_t cols = part_cols(a.n_cols, segs);
   segs               = static_cast<int>((a.n_cols + cols - 1) / cols);
-  K* keys            = static_cast<K*>(workspace);
-  V* sums            = reinterpret_cast<V*>(keys + (segs > 1 ? a.n_rows * segs * a.k : 0));
-  const unsigned rows = static_cast<unsigned>(a.n_rows < 65535 ? a.n_rows : 65535);
-  top_segments<T><<<dim3(segs, rows), kThreads, 0, s>>>(a, cols, keys, sums);
-  if (segs > 1) {
-    const int64_t most = 16ll * n_sms;
-    top_join<T><<<static_cast<unsigned>(a.n_rows < most ? a.n_rows : most), kThreads, 0, s>>>(a, segs, keys, sums);
-  }
+  double* sums       = static_cast<double*>(workspace);
+  K* keys            = reinterpret_cast<K*>(sums + (segs > 1 ? 2 * a.n_rows * segs : 0));
+  const int64_t most = 16ll * n_sms;
+  const auto kernel  = a.probabilities ? top_segments<T, kThreads, true> : top_segments<T, kThreads, false>;
+  kernel<<<static_cast<unsigned>((a.n_rows < most ? a.n_rows : most) * segs), kThreads, 0, s>>>(a, segs, cols, keys, sums);
+  if (segs > 1) top_join<T><<<static_cast<unsigned>(a.n_rows < most ? a.n_rows : most), kThreads, 0, s>>>(a, segs, keys, sums);
   count_launches(segs > 1 ? 2 : 1);
   return cudaGetLastError();
 }
@@ -388,8 +538,7 @@ size_t top_workspace(int dtype, const TopArgs& a, int n_sms)
 {
   const int64_t segs = segments(a.n_rows, a.n_cols, n_sms);
   if (segs <= 1) return 0;
-  const size_t key = dtype == kF64 ? sizeof(Key64) : sizeof(Key32);
-  return a.n_rows * segs * (a.k * key + 2 * (dtype == kF64 ? 8 : 4)) + 16;
+  return a.n_rows * segs * (a.k * (dtype == kF64 ? sizeof(Key64) : sizeof(Key32)) + 2 * sizeof(double));
 }
 
 cudaError_t launch_top(int dtype, const TopArgs& a, void* workspace, int n_sms, cudaStream_t s)
