@@ -17,6 +17,7 @@ teacher's values are constants.  All computation happens in libb2fil.so.
 from __future__ import annotations
 
 import ctypes as C
+import warnings
 from typing import NamedTuple, Optional
 
 import torch
@@ -43,6 +44,36 @@ class CTeacher(C.Structure):
     _fields_ = [("values", C.c_void_p), ("index", C.c_void_p), ("logsumexp", C.c_void_p),
                 ("values_stride", C.c_int64), ("index_stride", C.c_int64), ("ignore", C.c_int64),
                 ("k", C.c_int32), ("index64", C.c_int32)]
+
+
+_call = None  # the compiled call path; False: not available
+
+
+def _native():
+    """The compiled call path (csrc/torch_call.cpp), or False where it was not built for the installed
+    torch: the same calls then go through ctypes, slower by tens of microseconds."""
+    global _call
+    if _call is None:
+        try:
+            module = _lib.torch_module()
+        except (ImportError, OSError) as e:
+            warnings.warn(f"distillation calls take longer than they need: {e}", RuntimeWarning, stacklevel=3)
+            _call = False
+            return _call
+        lib = _lib.load()
+        module.bind(*(C.cast(getattr(lib, "b2fil_" + name), C.c_void_p).value for name in (
+            "last_error", "top_scores_workspace", "top_scores", "distill_loss_workspace", "distill_loss",
+            "distill_loss_grad", "linear_loss_workspace", "linear_loss", "linear_loss_grad_workspace",
+            "linear_loss_grad")))
+        _call = module
+    return _call
+
+
+def _answer(out):
+    """What the compiled path returned, an error code raised."""
+    if type(out) is int:
+        _lib.check(out)
+    return out
 
 
 def _cuda(name, x, dtypes, ndim=None):
@@ -89,13 +120,16 @@ def top_scores(scores, k: int, *, temperature: float = 1.0, probabilities: bool 
     With `probabilities` the logarithms of the scores take the scores' place in `values` and
     `logsumexp`: what a distillation loss takes as a forest's logits.  1 <= k <= min(n_classes, 256).
     The outputs are constants to autograd."""
+    temperature = _temperature(temperature)
+    call = _native() if isinstance(scores, torch.Tensor) and scores.is_cuda else False
+    if call and (out := _answer(call.top_scores(scores, int(k), temperature, probabilities))) is not None:
+        return TopScores(*out)
     _cuda("scores", scores, _TYPES)
     if scores.ndim < 1:
         raise ValueError("scores must have at least one dimension")
     shape, n_cols, k = scores.shape[:-1], scores.shape[-1], int(k)
     if not 1 <= k <= min(n_cols, MOST_TOP):
         raise ValueError(f"k must be between 1 and min(n_classes, {MOST_TOP}) = {min(n_cols, MOST_TOP)}, got {k}")
-    temperature = _temperature(temperature)
     x = scores.detach()
     x = _rows(x if x.ndim == 2 else x.reshape(-1, n_cols))
     n, dev = x.shape[0], x.device
@@ -208,6 +242,15 @@ class _Loss(torch.autograd.Function):
 _STUDENT = (torch.float32, torch.bfloat16, torch.float16)
 
 
+def _loss(x, values, index, lse, temperature, reduction, compiled_only=False):
+    call = _native() if isinstance(x, torch.Tensor) and x.is_cuda else False
+    if call:
+        out = _answer(call.distill_loss(x, values, index, lse, temperature, _NO_CLASS, reduction))
+        if out is not None:
+            return out
+    return None if compiled_only else _Loss.apply(x, values, index, lse, temperature, _NO_CLASS, reduction)
+
+
 def distillation_loss(logits, top, *, temperature: float = 1.0, tail: str = "renormalise", reduction: str = "mean"):
     """T^2 KL(teacher || softmax(logits / T)) over the classes that the teacher names.
 
@@ -221,6 +264,12 @@ def distillation_loss(logits, top, *, temperature: float = 1.0, tail: str = "ren
     reduction : 'mean' over the rows that count (0 where none does), 'sum', or 'none': (...), 0 for others.
 
     The loss is fp32, the gradient by the logits has their type."""
+    if reduction in _REDUCTIONS and tail in _TAILS and type(top) is TopScores and (tail != "bucket" or
+                                                                                   top.logsumexp is not None):
+        loss = _loss(logits, top.values, top.index, top.logsumexp if tail == "bucket" else None, _temperature(temperature),
+                     _REDUCTIONS[reduction], compiled_only=True)
+        if loss is not None:
+            return loss
     _cuda("logits", logits, _STUDENT)
     if logits.ndim < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits must have shape (..., n_classes), got {tuple(logits.shape)}")
@@ -229,7 +278,7 @@ def distillation_loss(logits, top, *, temperature: float = 1.0, tail: str = "ren
     values, index, lse = _top(top, x.shape[0], x.device, tail)
     if lse is not None and n_cols > 1 << 20:
         raise ValueError(f"tail='bucket' takes at most 2^20 classes, got {n_cols}")
-    loss = _Loss.apply(x, values, index, lse, _temperature(temperature), _NO_CLASS, _reduction(reduction))
+    loss = _loss(x, values, index, lse, _temperature(temperature), _reduction(reduction))
     return loss.view(shape) if reduction == "none" and len(shape) != 1 else loss
 
 
@@ -312,6 +361,15 @@ def _tiled(x):
     return x
 
 
+def _linear(hidden, weight, values, index, temperature, ignore, reduction):
+    call = _native()
+    if call:
+        out = _answer(call.linear_loss(hidden, weight, values, index, temperature, ignore, reduction))
+        if out is not None:
+            return out
+    return _Linear.apply(hidden, weight, values, index, temperature, ignore, reduction)
+
+
 def linear_cross_entropy(hidden, weight, target, *, ignore_index: int = -100, reduction: str = "mean"):
     """Softmax cross entropy of the logits `hidden @ weight.T` and `target`, without keeping the logits.
 
@@ -329,7 +387,7 @@ def linear_cross_entropy(hidden, weight, target, *, ignore_index: int = -100, re
     if target.device != hidden.device:
         raise ValueError(f"target is on {target.device}, hidden on {hidden.device}")
     target = target.reshape(-1, 1)
-    loss = _Linear.apply(hidden, weight, None, target, 1.0, int(ignore_index), _reduction(reduction))
+    loss = _linear(hidden, weight, None, target, 1.0, int(ignore_index), _reduction(reduction))
     return loss.view(shape) if reduction == "none" and len(shape) != 1 else loss
 
 
@@ -341,7 +399,7 @@ def linear_distillation_loss(hidden, weight, top, *, temperature: float = 1.0, r
     `linear_cross_entropy`."""
     hidden, weight, shape = _layer(hidden, weight)
     values, index, _ = _top(top, hidden.shape[0], hidden.device, "renormalise")
-    loss = _Linear.apply(hidden, weight, values, index, _temperature(temperature), _NO_CLASS, _reduction(reduction))
+    loss = _linear(hidden, weight, values, index, _temperature(temperature), _NO_CLASS, _reduction(reduction))
     return loss.view(shape) if reduction == "none" and len(shape) != 1 else loss
 
 

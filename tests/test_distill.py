@@ -366,3 +366,72 @@ def test_gradient_against_differences():
                 d[r, c] = h
                 slope = (f(z.detach() + d) - f(z.detach() - d)) / (2 * h)
                 assert abs(slope.item() - g[r, c].item()) < h * h / 6 + 3 * 4 * 3 * S / h
+
+
+@gpu
+def test_without_the_compiled_call_path(monkeypatch):
+    """The same numbers, gradients and errors through ctypes."""
+    from cuml_b200 import distill
+
+    z, v, i, lse = make(50, 300, 7, "bf16", 9)
+    h = torch.randn((50, 64), generator=gen(1), device="cuda").bfloat16()
+    w = torch.randn((300, 64), generator=gen(2), device="cuda").bfloat16()
+
+    def everything():
+        out = list(distill.top_scores(z, 5))
+        for reduction in ("mean", "none"):
+            x = z.detach().requires_grad_()
+            loss = distill.distillation_loss(x, distill.TopScores(v, i, lse), tail="bucket", reduction=reduction)
+            a, b = h.detach().requires_grad_(), w.detach().requires_grad_()
+            of_layer = distill.linear_distillation_loss(a, b, (v, i), reduction=reduction, temperature=2.0)
+            out += [loss, *torch.autograd.grad(loss.sum(), x), of_layer, *torch.autograd.grad(of_layer.sum(), (a, b))]
+        return out
+
+    assert distill._native()
+    compiled = everything()
+    monkeypatch.setattr(distill, "_call", False)
+    for x, y in zip(compiled, everything()):
+        assert x.dtype == y.dtype and torch.equal(x, y)
+
+
+@gpu
+@pytest.mark.parametrize("compiled", [True, False])
+def test_autograd_rules(monkeypatch, compiled):
+    """A graph is used once unless it is retained, inputs are not changed in between, there is no second derivative."""
+    from cuml_b200 import distill
+
+    if not compiled:
+        monkeypatch.setattr(distill, "_call", False)
+    z, v, i, lse = make(5, 30, 4, "fp32", 9)
+    h = torch.randn((5, 16), generator=gen(1), device="cuda").bfloat16()
+    w = torch.randn((30, 16), generator=gen(2), device="cuda").bfloat16()
+    top = distill.TopScores(v, i, lse)
+    for leaves, f in (([z], lambda a: distill.distillation_loss(a, top)),
+                      ([h, w], lambda a, b: distill.linear_distillation_loss(a, b, top))):
+        leaves = [x.detach().requires_grad_() for x in leaves]
+        loss = f(*leaves)
+        first = torch.autograd.grad(loss, leaves, retain_graph=True)
+        again = torch.autograd.grad(loss, leaves)
+        assert all(torch.equal(x, y) for x, y in zip(first, again))
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(loss, leaves)
+        loss = f(*leaves)
+        with torch.no_grad():
+            leaves[0].mul_(2)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(loss, leaves)
+        grads = torch.autograd.grad(f(*leaves), leaves, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(grads[0].sum(), leaves)
+        with torch.no_grad():
+            assert not f(*leaves).requires_grad
+        assert not f(*[x.detach() for x in leaves]).requires_grad
+        (2 * f(*leaves)).backward()
+        assert all(x.grad is not None and x.grad.shape == x.shape for x in leaves)
+        # an upstream gradient of another type and stride
+        rows = distill.distillation_loss(leaves[0], top, reduction="none") if len(leaves) == 1 else \
+            distill.linear_distillation_loss(*leaves, top, reduction="none")
+        up = torch.arange(10, device="cuda", dtype=torch.float32)[::2]
+        a = torch.autograd.grad(rows, leaves, up, retain_graph=True)
+        b = torch.autograd.grad(rows, leaves, up.contiguous())
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
