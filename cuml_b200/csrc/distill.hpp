@@ -43,6 +43,13 @@ struct Teacher {
   int64_t ignore;          // an index that does not count (besides those outside the classes)
 };
 
+// What the teacher names in each row, kept for the gradient: (n_rows, k) each.
+struct Named {
+  float* logit;  // of the class; not used by the loss on logits
+  float* p;      // the teacher's probability
+  int32_t* at;   // the class, below 0: none
+};
+
 // ---- loss on logits (distill_loss.cu) --------------------------------------------------------
 struct LossArgs {
   const void* logits;
@@ -51,6 +58,7 @@ struct LossArgs {
   float temperature;
   float* row_loss;   // (n_rows)
   float4* row_stats; // (n_rows) max, 1 / sum, factor of the classes outside the teacher's, 1: the row counts
+  Named named;
 };
 // reduction: 0 none, 1 sum, 2 mean over the rows that count.
 struct Reduced {
@@ -72,12 +80,6 @@ struct LossGradArgs {
 cudaError_t launch_loss_grad(int dtype, const LossGradArgs& a, int n_sms, cudaStream_t s);
 
 // ---- loss on a linear layer's output (distill_linear.cu) -------------------------------------
-// What the teacher names in each row, kept for the gradient: (n_rows, k) each.
-struct Named {
-  float* logit;  // h . w of the class
-  float* p;      // the teacher's probability
-  int32_t* at;   // the class, below 0: none
-};
 struct LinearArgs {
   const void* hidden;  // (n_rows, width), 16-byte aligned rows, width a multiple of 8
   const void* weight;  // (n_cols, width), likewise

@@ -180,8 +180,8 @@ int64_t b2fil_distill_loss_workspace(int dtype, int64_t n_rows, int64_t n_cols, 
 
 int b2fil_distill_loss(int dtype, const void* logits, int64_t n_rows, int64_t n_cols, int64_t row_stride,
                        const b2fil_teacher* teacher, double temperature, int reduction, float* row_loss, float* row_stats,
-                       float* loss, float* factor, void* workspace, int64_t workspace_bytes, int device_id,
-                       void* cuda_stream)
+                       float* named_p, int32_t* named_at, float* loss, float* factor, void* workspace,
+                       int64_t workspace_bytes, int device_id, void* cuda_stream)
 {
   LossArgs a{};
   int rc = check_teacher(teacher, n_rows, a.teacher);
@@ -190,8 +190,9 @@ int b2fil_distill_loss(int dtype, const void* logits, int64_t n_rows, int64_t n_
   if (rc != B2FIL_OK) return rc;
   if (reduction < B2FIL_REDUCE_NONE || reduction > B2FIL_REDUCE_MEAN) return invalid("unknown reduction");
   if (reduction != B2FIL_REDUCE_NONE && (!loss || !factor)) return invalid("a reduced loss needs loss and factor");
-  if (n_rows > 0 && (!logits || !row_loss || !row_stats)) return invalid("NULL buffer");
-  if (!aligned(logits, type_bytes(dtype)) || !aligned(row_stats, 16) || !aligned(row_loss, 4))
+  if (n_rows > 0 && (!logits || !row_loss || !row_stats || !named_p || !named_at)) return invalid("NULL buffer");
+  if (!aligned(logits, type_bytes(dtype)) || !aligned(row_stats, 16) || !aligned(row_loss, 4) || !aligned(named_p, 4) ||
+      !aligned(named_at, 4))
     return invalid("a buffer is not aligned");
   if (row_stride < n_cols && n_rows > 1) return invalid("row_stride is smaller than n_cols");
   if (a.teacher.logsumexp && n_cols > (1 << 20)) return invalid("the teacher's logsumexp needs n_cols <= 2^20");
@@ -206,24 +207,25 @@ int b2fil_distill_loss(int dtype, const void* logits, int64_t n_rows, int64_t n_
   a.temperature = static_cast<float>(temperature);
   a.row_loss    = row_loss;
   a.row_stats   = reinterpret_cast<float4*>(row_stats);
+  a.named       = Named{nullptr, named_p, named_at};
   return finish("b2fil_distill_loss", launch_loss(dtype, a, Reduced{reduction, loss, factor}, workspace,
                                                   sms_of(device_id), static_cast<cudaStream_t>(cuda_stream)));
 }
 
 int b2fil_distill_loss_grad(int dtype, const void* logits, int64_t n_rows, int64_t n_cols, int64_t row_stride,
-                            const b2fil_teacher* teacher, double temperature, const float* row_stats, const float* upstream,
-                            int64_t upstream_stride, const float* factor, void* grad, int64_t grad_stride, int device_id,
-                            void* cuda_stream)
+                            int k, double temperature, const float* row_stats, const float* named_p,
+                            const int32_t* named_at, const float* upstream, int64_t upstream_stride, const float* factor,
+                            void* grad, int64_t grad_stride, int device_id, void* cuda_stream)
 {
   LossGradArgs g{};
   LossArgs& a = g.fwd;
-  int rc      = check_teacher(teacher, n_rows, a.teacher);
-  if (rc == B2FIL_OK) rc = check_loss(dtype, n_rows, n_cols, a.teacher.k);
+  int rc      = check_loss(dtype, n_rows, n_cols, k);
   if (rc == B2FIL_OK) rc = check_temperature(temperature);
   if (rc != B2FIL_OK) return rc;
   if (n_rows == 0) return B2FIL_OK;
-  if (!logits || !row_stats || !upstream || !grad) return invalid("NULL buffer");
-  if (!aligned(logits, type_bytes(dtype)) || !aligned(grad, type_bytes(dtype)) || !aligned(row_stats, 16))
+  if (!logits || !row_stats || !named_p || !named_at || !upstream || !grad) return invalid("NULL buffer");
+  if (!aligned(logits, type_bytes(dtype)) || !aligned(grad, type_bytes(dtype)) || !aligned(row_stats, 16) ||
+      !aligned(named_p, 4) || !aligned(named_at, 4) || !aligned(upstream, 4) || !aligned(factor, 4))
     return invalid("a buffer is not aligned");
   if ((row_stride < n_cols || grad_stride < n_cols) && n_rows > 1) return invalid("a row stride is smaller than n_cols");
   const int sms = sms_of(device_id);
@@ -236,6 +238,8 @@ int b2fil_distill_loss_grad(int dtype, const void* logits, int64_t n_rows, int64
   a.row_stride      = row_stride;
   a.temperature     = static_cast<float>(temperature);
   a.row_stats       = const_cast<float4*>(reinterpret_cast<const float4*>(row_stats));
+  a.teacher.k       = k;
+  a.named           = Named{nullptr, const_cast<float*>(named_p), const_cast<int32_t*>(named_at)};
   g.upstream        = upstream;
   g.upstream_stride = upstream_stride;
   g.factor          = factor;

@@ -127,10 +127,15 @@ struct Running {
     s          = (m == lowest<V>() ? s : s * power((m - b) * c)) + (m2 == lowest<V>() ? s2 : s2 * power((m2 - b) * c));
     m          = to;
   }
-  __device__ __forceinline__ void join_lanes(V c)
+  __device__ __forceinline__ void join_lanes(V c)  // the maximum first: one power for all steps
   {
+    V to = m;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) join(__shfl_xor_sync(~0u, m, d), __shfl_xor_sync(~0u, s, d), c);
+    for (int d = 16; d; d >>= 1) to = larger(to, __shfl_xor_sync(~0u, to, d));
+    if (m != lowest<V>()) s *= power((m - to) * c);
+    m = to;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
   }
 };
 
@@ -183,33 +188,53 @@ __device__ __forceinline__ V sum_row(V x, V* room)
   return x;
 }
 
-template <int THREADS>
-__device__ __forceinline__ double max_row(double x, double* room)
+// ---- the teacher's side of a row -------------------------------------------------------------
+// ln of a sum of 32-bit numbers, off by 2^-24 of less than 1 whatever its size: the exponent's part is exact.
+__device__ __forceinline__ double log_sum(float s)
+{
+  if (!(s > 0.f) || s == INFINITY) return log(static_cast<double>(s));
+  int e;
+  float f = frexpf(s, &e);
+  if (f < 0.70710678f) {
+    f *= 2.f;
+    --e;
+  }
+  return fma(static_cast<double>(e), 0.69314718055994530942, static_cast<double>(logf(f)));
+}
+
+template <class V>
+__device__ __forceinline__ V sum_lanes(V x)
 {
 #pragma unroll
-  for (int d = 16; d; d >>= 1) x = fmax(x, __shfl_xor_sync(~0u, x, d));
-  if (THREADS == 32) return x;
-  constexpr int W = THREADS / 32;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  __syncthreads();
-  if (lane == 0) room[warp] = x;
-  __syncthreads();
-  x = lane < W ? room[lane] : -INFINITY;
+  for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(~0u, x, d);
+  return x;
+}
+__device__ __forceinline__ float max_lanes(float x)
+{
 #pragma unroll
-  for (int d = 16; d; d >>= 1) x = fmax(x, __shfl_xor_sync(~0u, x, d));
+  for (int d = 16; d; d >>= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
   return x;
 }
 
-// ---- the teacher's side of a row -------------------------------------------------------------
-// Entry j names class at[j] (-1: none) with the probability p[j]; a class that is named again adds
-// to its first entry and the later one has at -2 - first.  In 64 bits: the two sides' logarithms nearly
-// cancel, and what is left of the teacher is a difference from 1.
+// What a teacher names in a row.  Entry j is the class at[j] (-1: none) with the score v[j] and the
+// probability p[j]; a class that is named again adds to its first entry and the later one has at -1.
+struct Entries {
+  float *v, *p;
+  int* at;
+};
+__host__ __device__ __forceinline__ size_t entry_bytes(int k) { return static_cast<size_t>(k) * 12; }
+__device__ __forceinline__ Entries entries_at(void* base, int k)
+{
+  float* v = static_cast<float*>(base);
+  return {v, v + k, reinterpret_cast<int*>(v + 2 * k)};
+}
+
+// log p[j] = v[j] / T - log_norm is taken in 64 bits, as it nearly cancels with the student's logarithm.
 struct TeacherRow {
-  double log_norm;  // log p[j] = values[j] / T - log_norm
-  double rest;      // probability of all classes that are not named
-  int named;        // different classes named
+  double log_norm;
+  float rest;    // probability of all classes that are not named
   bool counts;
-  bool merged;      // a class was named twice: log p[j] is that of p[j]
+  bool merged;   // a class was named twice: log p[j] is that of p[j]
 };
 
 __device__ __forceinline__ int64_t teacher_index(const Teacher& t, int64_t row, int j)
@@ -218,79 +243,130 @@ __device__ __forceinline__ int64_t teacher_index(const Teacher& t, int64_t row, 
                    : static_cast<int64_t>(static_cast<const int32_t*>(t.index)[row * t.index_stride + j]);
 }
 
-// p, at: shared, k entries of this row; room: shared, at least 32 doubles of this row.
-template <int THREADS>
-__device__ __forceinline__ TeacherRow read_teacher(const Teacher& t, int64_t row, int64_t n_cols, double inv_t, int tid,
-                                                   float* p, int* at, double* room)
+// By one warp; e: shared memory.  REST: the teacher has a logsumexp.
+template <bool REST>
+__device__ __forceinline__ TeacherRow read_teacher(const Teacher& t, int64_t row, int64_t n_cols, double inv_t, const Entries& e)
 {
   TeacherRow r;
-  sync_row<THREADS>();  // the last row's entries have been used
-  double top = -INFINITY;
-  for (int j = tid; j < t.k; j += THREADS) {
+  const int lane = threadIdx.x % 32, k = t.k;
+  float top      = lowest<float>();
+  for (int j = lane; j < k; j += 32) {
     const int64_t c = teacher_index(t, row, j);
+    const float v   = t.values ? t.values[row * t.values_stride + j] : 0.f;
     const bool is   = c >= 0 && c < n_cols && c != t.ignore;
-    at[j]           = is ? static_cast<int>(c) : -1;
-    if (is) top = fmax(top, t.values ? t.values[row * t.values_stride + j] * inv_t : 0.0);
+    e.at[j]         = is ? static_cast<int>(c) : -1;
+    e.v[j]          = v;
+    if (is) top = fmaxf(top, v);
   }
-  sync_row<THREADS>();
-  if (t.logsumexp) {
-    r.log_norm = t.logsumexp[row];
+  __syncwarp();
+  if (REST) {
+    // what is left of 1 is a difference: in 64 bits
+    r.log_norm  = t.logsumexp[row];
+    r.counts    = !(r.log_norm == -INFINITY);
+    double mass = 0;
+    for (int j = lane; j < k; j += 32) {
+      const double q = e.at[j] >= 0 && r.counts ? exp(e.v[j] * inv_t - r.log_norm) : 0.0;
+      e.p[j]         = static_cast<float>(q);
+      mass += q;
+    }
+    mass = sum_lanes(mass);
+    // (a log-sum-exp in 32 bits leaves about 2^-20 where nothing is left)
+    r.rest = 1.0 - mass < 0x1p-20 ? 0.f : static_cast<float>(1.0 - mass);
   } else {
-    const double most = max_row<THREADS>(top, room);
-    double sum        = 0;
-    for (int j = tid; j < t.k; j += THREADS)
-      if (at[j] >= 0) sum += t.values ? exp(t.values[row * t.values_stride + j] * inv_t - (most == -INFINITY ? 0.0 : most)) : 1.0;
-    sum        = sum_row<THREADS>(sum, room);
-    r.log_norm = most + log(sum);
+    const float most = base_of(max_lanes(top));
+    const float ti   = static_cast<float>(inv_t);
+    float sum        = 0.f;
+    for (int j = lane; j < k; j += 32) {
+      const float x = e.at[j] >= 0 ? expf((e.v[j] - most) * ti) : 0.f;
+      e.p[j]        = x;
+      sum += x;
+    }
+    sum        = sum_lanes(sum);
+    r.log_norm = most * inv_t + log_sum(sum);
+    r.counts   = !(sum == 0.f);
+    r.rest     = 0.f;
+    if (r.counts)
+      for (int j = lane; j < k; j += 32) e.p[j] = e.p[j] / sum;
   }
-  r.counts = !(r.log_norm == -INFINITY);
-  // (a NaN among the values is not seen by fmax: it is in the sum)
-  double mass = 0;
-  int named   = 0;
-  for (int j = tid; j < t.k; j += THREADS) {
-    double q = 0;
-    if (at[j] >= 0 && r.counts) q = exp((t.values ? t.values[row * t.values_stride + j] * inv_t : 0.0) - r.log_norm);
-    p[j] = static_cast<float>(q);
-    mass += q;
-  }
+  __syncwarp();
   // classes named twice (top scores name none twice; a caller's list may)
-  sync_row<THREADS>();
   bool again = false;
-  for (int j = tid; j < t.k; j += THREADS) {
-    const int c = at[j];
-    if (c < 0) continue;
-    bool dup = false;
-    for (int i = 0; i < j; ++i) dup |= at[i] == c;
-    named += !dup;
-    again |= dup;
+  int named  = 0;
+  if (k <= 32) {
+    const int c        = lane < k ? e.at[lane] : -1;
+    const unsigned all = __match_any_sync(~0u, c < 0 ? -1 - lane : c);
+    again              = __ffs(all) - 1 < lane;
+    named              = c >= 0 && !again;
+  } else {
+    for (int j = lane; j < k; j += 32) {
+      const int c = e.at[j];
+      bool dup    = false;
+      for (int i = 0; i < j; ++i) dup |= e.at[i] == c;
+      named += c >= 0 && !dup;
+      again |= c >= 0 && dup;
+    }
   }
-  double both = sum_row<THREADS>(named + (again ? 65536.0 : 0.0), room);
-  r.merged    = both >= 65536.0;
+  r.merged = __any_sync(~0u, again);
   if (r.merged) {
-    sync_row<THREADS>();
-    if (tid == 0) {
-      for (int j = 1; j < t.k; ++j) {
-        if (at[j] < 0) continue;
+    if (lane == 0) {
+      for (int j = 1; j < k; ++j) {
+        if (e.at[j] < 0) continue;
         for (int i = 0; i < j; ++i)
-          if (at[i] == at[j]) {
-            p[i] += p[j];
-            p[j]  = 0;
-            at[j] = -2 - i;
+          if (e.at[i] == e.at[j]) {
+            e.p[i] += e.p[j];
+            e.at[j] = -1;
             break;
           }
       }
     }
-    sync_row<THREADS>();
-    both = both - 65536.0 * floor(both / 65536.0);
+    __syncwarp();
   }
-  r.named = static_cast<int>(both);
-  r.rest  = 0;
-  if (t.logsumexp) {
-    mass   = sum_row<THREADS>(mass, room);
-    // (a log-sum-exp in 32 bits leaves about that much where nothing is left)
-    r.rest = r.named < n_cols && !(1.0 - mass < 0x1p-20) ? 1.0 - mass : 0.0;
-  }
+  if (REST && __reduce_add_sync(~0u, named) >= n_cols) r.rest = 0.f;  // no class is left
   return r;
+}
+
+// Sum over a row's entries of p (log p - log q), q the softmax with the maximum m and the logarithm of the sum
+// log_s; logit(j, class).  By one warp.
+template <class F>
+__device__ __forceinline__ double named_loss(const Entries& e, int k, const TeacherRow& t, double inv_t, float m, double log_s,
+                                             F logit)
+{
+  double loss = 0;
+  for (int j = threadIdx.x % 32; j < k; j += 32) {
+    const int at  = e.at[j];
+    const float p = e.p[j];
+    if (at < 0 || p == 0.f) continue;
+    const double log_p = t.merged ? log(static_cast<double>(p)) : e.v[j] * inv_t - t.log_norm;
+    loss += p * (log_p - ((static_cast<double>(logit(j, at)) - m) * inv_t - log_s));
+  }
+  return sum_lanes(loss);
+}
+
+// ---- sums over the rows ----------------------------------------------------------------------
+// {sum of the losses, rows that count} of the rows of a block's threads that have any, in a fixed order;
+// for thread 0.
+template <int THREADS>
+__device__ __forceinline__ double2 sum_block(double loss, double count, double2* room)
+{
+  loss  = sum_lanes(loss);
+  count = sum_lanes(count);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) room[threadIdx.x / 32] = make_double2(loss, count);
+  __syncthreads();
+  double2 all = make_double2(0, 0);
+  if (threadIdx.x == 0)
+    for (int i = 0; i < THREADS / 32; ++i) {
+      all.x += room[i].x;
+      all.y += room[i].y;
+    }
+  return all;
+}
+// Sum, or mean over the rows that count (0 if none does).
+__device__ __forceinline__ void write_reduced(const Reduced& out, double2 all)
+{
+  const double f = out.reduction == 1 ? 1.0 : all.y > 0 ? 1.0 / all.y : 0.0;
+  *out.loss      = static_cast<float>(all.y > 0 ? all.x * f : 0.0);
+  *out.factor    = static_cast<float>(f);
 }
 
 }  // namespace distill

@@ -39,6 +39,10 @@ constexpr long long kPatience = 2000000000ll;  // ns
 constexpr int64_t kPieceBytes = 64ll << 20;    // of d: fits L2 beside what is read
 constexpr int kMostSplits     = 16;
 constexpr float kHalfScale    = 16384.f;       // of d in fp16
+// Named classes of a row that the epilogue looks through for each tile; more are put into d by a kernel of their
+// own (4096 x 1024 x 50,001, seven pieces: 32 per row cost 290 us in the epilogue and 28 us in the kernel,
+// one per row nothing in the epilogue and 3.6 us per piece in the kernel).
+constexpr int kFewNamed = 4;
 
 __device__ int g_status;
 
@@ -168,6 +172,12 @@ struct Product {
   int a_outer, b_outer;
   int result;
 };
+// A factor on the device: a b T, or a T.
+struct Scale {
+  const float *a, *b;
+  float t;
+  __device__ __forceinline__ float operator()() const { return *a * (b ? *b : 1.f) * t; }
+};
 struct Work {
   Product product[2];
   int products;
@@ -182,12 +192,15 @@ struct Work {
   void* diff;
   int64_t diff_stride;
   float diff_scale;
-  // kSumHidden: 32-bit sums, one matrix per split; kHidden, kWeight: 16-bit results times *scale
+  Named named;
+  int k, first;
+  // kSumHidden: 32-bit sums, one matrix per split; kHidden, kWeight: 16-bit results times `scale`
   float* sums;
   int add;
   void *grad_hidden, *grad_weight;
   int64_t width;
-  const float* scale;
+  Scale scale;
+  int* ticket;            // kStats: set to 0 for linear_rows
 };
 
 struct Tile {
@@ -308,6 +321,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
   const uint32_t rank = rank_in_cluster();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int cluster = blockIdx.x / 2, clusters = gridDim.x / 2;
+  if (KIND == kStats && blockIdx.x == 0 && threadIdx.x == 0) *w.ticket = 0;
   if (threadIdx.x == 0) {
     gave_up = 0;
     for (int i = 0; i < kStages; ++i) {
@@ -430,7 +444,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
         base           = base_of(s.x);
         factor         = s.w == 0.f ? 0.f : s.y * w.diff_scale * (w.row_scale ? w.row_scale[row] : 1.f);
       }
-      if (KIND == kWeight && p.result != kSumHidden) factor = *w.scale;
+      if (KIND == kWeight && p.result != kSumHidden) factor = w.scale();
       if (!__all_sync(~0u, bar_wait(done + 8 * half, turn, &gave_up))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       Running<float> r;
@@ -446,6 +460,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) bar_arrive_cluster(freed0 + 8 * half);
+      if (KIND == kDiff && in && factor != 0.f && w.k <= kFewNamed) {  // over what has just been written
+        const float per = w.diff_scale * (w.row_scale ? w.row_scale[row] : 1.f), inv = w.stats[row].y;
+        const int low = t.n * kTile, high = min(low + kTile, p.n);
+        for (int j = 0; j < w.k; ++j) {
+          const int64_t e = row * w.k + j;
+          const int at    = w.named.at[e] - w.first;
+          if (at < low || at >= high) continue;
+          const float d = (power((w.named.logit[e] - base) * w.c) * inv - w.named.p[e]) * per;
+          char* to      = static_cast<char*>(w.diff) + (row * w.diff_stride + at) * 2;
+          *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(two(d, 0.f, w.bf16));
+        }
+      }
       if (KIND == kStats && in) w.parts[row * p.n_tiles + t.n] = make_float2(r.m, r.s);
       half ^= 1;
       turn ^= half == 0;
@@ -470,127 +496,134 @@ __device__ __forceinline__ float dot_piece(const Piece<T>& a, const Piece<T>& b,
   return s;
 }
 
-// Loss of a row from the maxima and sums of its tiles; the named classes' logits are dot products of
-// their own, a warp each.
+// Loss of a row from the maxima and sums of its tiles, by THREADS threads, of which the first warp does what
+// concerns the teacher; the named classes' logits are dot products of their own, a warp each, four at a time.
+// The block that is last to finish adds up all blocks' losses.
 template <class T, int THREADS>
-__global__ void __launch_bounds__(kThreads) linear_rows(LinearArgs a, const float2* parts, int tiles, double2* block_sums)
+__global__ void __launch_bounds__(kThreads) linear_rows(LinearArgs a, const float2* parts, int tiles, Reduced out,
+                                                        double2* block_sums, int* ticket)
 {
-  constexpr int ROWS = kThreads / THREADS, N = Piece<T>::N;
+  constexpr int ROWS = kThreads / THREADS, N = Piece<T>::N, WARPS = THREADS / 32;
   extern __shared__ __align__(16) char smem[];
+  __shared__ double2 room[kThreads / 32];
+  __shared__ float joins[2 * kThreads / 32];
+  __shared__ bool is_last;
   const int slot = threadIdx.x / THREADS, tid = threadIdx.x % THREADS, lane = threadIdx.x % 32;
   const int k        = a.teacher.k;
-  char* mine         = smem + slot * static_cast<size_t>(256 + (k + 1) / 2 * 2 * 12);
-  double* room       = reinterpret_cast<double*>(mine);
-  float* p           = reinterpret_cast<float*>(mine + 256);
-  int* at            = reinterpret_cast<int*>(p + k);
-  float* logit       = reinterpret_cast<float*>(at + k);
+  char* mine         = smem + slot * (entry_bytes(k) + static_cast<size_t>(k) * 4);
+  const Entries e    = entries_at(mine, k);
+  float* logit       = reinterpret_cast<float*>(e.at + k);
   const float c      = 1.4426950408889634f / a.temperature;
   const double inv_t = 1.0 / a.temperature;
   double sum = 0, count = 0;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + slot; row < a.n_rows;
        row += static_cast<int64_t>(gridDim.x) * ROWS) {
-    const TeacherRow t = read_teacher<THREADS>(a.teacher, row, a.n_cols, inv_t, tid, p, at, room);
-    const T* h         = static_cast<const T*>(a.hidden) + row * a.hidden_stride;
-    for (int j = tid / 32; j < k; j += THREADS / 32) {
-      const int cls = at[j];
-      float s       = 0.f;
-      if (cls >= 0) {
-        const T* v = static_cast<const T*>(a.weight) + cls * a.weight_stride;
-        for (int i = lane * N; i < a.width; i += 32 * N) s = dot_piece(load_piece(h + i), load_piece(v + i), s);
+    TeacherRow t{};
+    sync_row<THREADS>();
+    if (tid < 32) t = read_teacher<false>(a.teacher, row, a.n_cols, inv_t, e);
+    sync_row<THREADS>();
+    const T* h = static_cast<const T*>(a.hidden) + row * a.hidden_stride;
+    for (int j = 4 * (tid / 32); j < k; j += 4 * WARPS) {
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+      const T* v[4];
 #pragma unroll
-        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+      for (int u = 0; u < 4; ++u) {
+        const int cls = j + u < k ? e.at[j + u] : -1;
+        v[u]          = static_cast<const T*>(a.weight) + (cls < 0 ? 0 : cls) * a.weight_stride;
       }
-      if (lane == 0) logit[j] = s;
+      const int most = min(4, k - j);
+      for (int i = lane * N; i < a.width; i += 32 * N) {
+        const Piece<T> x = load_piece(h + i);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (u < most) s[u] = dot_piece(x, load_piece(v[u] + i), s[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (u < most) s[u] = sum_lanes(s[u]);
+      if (lane < most) logit[j + lane] = lane == 0 ? s[0] : lane == 1 ? s[1] : lane == 2 ? s[2] : s[3];
     }
     Running<float> r;
     for (int i = tid; i < tiles; i += THREADS) r.join(parts[row * tiles + i].x, parts[row * tiles + i].y, c);
-    join_row<THREADS>(r, c, reinterpret_cast<float*>(room));
+    join_row<THREADS>(r, c, joins);
     sync_row<THREADS>();
-    const double log_s = log(static_cast<double>(r.s));
-    const bool counts  = t.counts && !(r.s == 0.f);
-    double loss        = 0;
-    for (int j = tid; j < k; j += THREADS) {
-      const int64_t to  = row * k + j;
-      a.named.logit[to] = logit[j];
-      a.named.p[to]     = p[j];
-      a.named.at[to]    = at[j];
-      if (at[j] < 0 || p[j] == 0.f) continue;
-      const double log_p = t.merged ? log(static_cast<double>(p[j]))
-                                    : (a.teacher.values ? a.teacher.values[row * a.teacher.values_stride + j] * inv_t : 0.0) - t.log_norm;
-      loss += p[j] * (log_p - ((static_cast<double>(logit[j]) - r.m) * inv_t - log_s));
-    }
-    loss = sum_row<THREADS>(loss, room);
-    if (!counts) loss = 0;
-    loss *= static_cast<double>(a.temperature) * a.temperature;
-    if (tid == 0) {
-      a.row_loss[row]  = static_cast<float>(loss);
-      a.row_stats[row] = make_float4(r.m, 1.f / r.s, 1.f, counts ? 1.f : 0.f);
-      sum += loss;
-      count += counts;
+    if (tid < 32) {
+      const bool counts = t.counts && !(r.s == 0.f);
+      double loss = named_loss(e, k, t, inv_t, r.m, log_sum(r.s), [&](int j, int) { return logit[j]; });
+      if (!counts) loss = 0;
+      loss *= static_cast<double>(a.temperature) * a.temperature;
+      for (int j = lane; j < k; j += 32) {
+        a.named.logit[row * k + j] = logit[j];
+        a.named.p[row * k + j]     = e.p[j];
+        a.named.at[row * k + j]    = e.at[j];
+      }
+      if (lane == 0) {
+        a.row_loss[row]  = static_cast<float>(loss);
+        a.row_stats[row] = make_float4(r.m, 1.f / r.s, 1.f, counts ? 1.f : 0.f);
+        sum += loss;
+        count += counts;
+      }
     }
   }
-  __shared__ double2 sums[ROWS];
-  if (tid == 0) sums[slot] = make_double2(sum, count);
-  __syncthreads();
+  if (out.reduction == 0) return;
+  const double2 all = sum_block<kThreads>(sum, count, room);
   if (threadIdx.x == 0) {
-    double2 all = sums[0];
-    for (int i = 1; i < ROWS; ++i) {
-      all.x += sums[i].x;
-      all.y += sums[i].y;
-    }
     block_sums[blockIdx.x] = all;
+    __threadfence();
+    is_last = atomicAdd(ticket, 1) == static_cast<int>(gridDim.x) - 1;
   }
+  __syncthreads();
+  if (!is_last) return;
+  __threadfence();
+  sum = count = 0;
+  for (int i = threadIdx.x; i < static_cast<int>(gridDim.x); i += kThreads) {  // in a fixed order
+    sum += __ldcg(&block_sums[i].x);
+    count += __ldcg(&block_sums[i].y);
+  }
+  const double2 total = sum_block<kThreads>(sum, count, room);
+  if (threadIdx.x == 0) write_reduced(out, total);
 }
 
-// Scales of the gradient.  One upstream value: *scale takes it all.  One per row: the rows' are brought below
-// 1 by a power of two, which *scale takes back, so that d stays in fp16's range.
-__global__ void __launch_bounds__(1024) grad_scales(LinearGradArgs g, float diff_scale, float* scale, float* row_scale)
+// One upstream value per row: the rows' are brought below 1 by a power of two, which *scale takes back, so
+// that d stays in fp16's range.
+__global__ void __launch_bounds__(1024) grad_scales(LinearGradArgs g, float* scale, float* row_scale)
 {
   __shared__ float room[32];
-  const float t = g.fwd.temperature / diff_scale;
-  if (!row_scale) {
-    if (threadIdx.x == 0) *scale = *g.upstream * (g.factor ? *g.factor : 1.f) * t;
-    return;
-  }
   float most = 0.f;
   for (int64_t i = threadIdx.x; i < g.fwd.n_rows; i += 1024) most = fmaxf(most, fabsf(g.upstream[i * g.upstream_stride]));
-#pragma unroll
-  for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+  most = max_lanes(most);
   if (threadIdx.x % 32 == 0) room[threadIdx.x / 32] = most;
   __syncthreads();
-  most = room[threadIdx.x % 32];
-#pragma unroll
-  for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+  most  = max_lanes(room[threadIdx.x % 32]);
   int e = 0;
   if (most > 0.f && most < INFINITY) frexpf(most, &e);
-  e              = max(-100, min(100, e));
-  const float up = ldexpf(1.f, e), down = ldexpf(1.f, -e);
-  if (threadIdx.x == 0) *scale = up * t;
+  e                = max(-100, min(100, e));
+  const float down = ldexpf(1.f, -e);
+  if (threadIdx.x == 0) *scale = ldexpf(1.f, e);
   for (int64_t i = threadIdx.x; i < g.fwd.n_rows; i += 1024) row_scale[i] = g.upstream[i * g.upstream_stride] * down;
 }
 
 // d of the classes that the teacher names, in a piece of the classes.
 template <class T>
-__global__ void __launch_bounds__(kThreads) named_diff(LinearArgs a, int64_t first, int64_t n, T* diff, int64_t stride,
-                                                       const float* row_scale, float diff_scale, float c)
+__global__ void __launch_bounds__(kThreads) named_diff(Work w, int64_t entries, int n)
 {
-  const int64_t all = a.n_rows * a.teacher.k;
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < all; i += gridDim.x * static_cast<int64_t>(kThreads)) {
-    const int cls = a.named.at[i];
-    if (cls < first || cls >= first + n) continue;
-    const int64_t row = i / a.teacher.k;
-    const float4 s    = a.row_stats[row];
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < entries; i += gridDim.x * static_cast<int64_t>(kThreads)) {
+    const int at = w.named.at[i] - w.first;
+    if (at < 0 || at >= n) continue;
+    const int64_t row = i / w.k;
+    const float4 s    = w.stats[row];
     if (s.w == 0.f) continue;
-    const float q = power((a.named.logit[i] - base_of(s.x)) * c) * s.y;
-    diff[row * stride + cls - first] = narrow<T>((q - a.named.p[i]) * diff_scale * (row_scale ? row_scale[row] : 1.f));
+    const float q = power((w.named.logit[i] - base_of(s.x)) * w.c) * s.y;
+    static_cast<T*>(w.diff)[row * w.diff_stride + at] =
+      narrow<T>((q - w.named.p[i]) * w.diff_scale * (w.row_scale ? w.row_scale[row] : 1.f));
   }
 }
 
 // dH from the sums of its parts.
 template <class T>
-__global__ void __launch_bounds__(kThreads) finish_hidden(const float* sums, int splits, int64_t n, const float* scale, T* out)
+__global__ void __launch_bounds__(kThreads) finish_hidden(const float* sums, int splits, int64_t n, Scale scale, T* out)
 {
-  const float f = *scale;
+  const float f = scale();
   for (int64_t i = 4 * (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x); i < n; i += 4 * gridDim.x * static_cast<int64_t>(kThreads)) {
     float4 v = *reinterpret_cast<const float4*>(sums + i);
     for (int s = 1; s < splits; ++s) {
@@ -602,22 +635,7 @@ __global__ void __launch_bounds__(kThreads) finish_hidden(const float* sums, int
   }
 }
 
-__global__ void __launch_bounds__(kThreads) reduce_rows(const double2* block_sums, int n, Reduced out)
-{
-  __shared__ double room[32];
-  double sum = 0, count = 0;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    sum += block_sums[i].x;
-    count += block_sums[i].y;
-  }
-  sum   = sum_row<kThreads>(sum, room);
-  count = sum_row<kThreads>(count, room);
-  if (threadIdx.x == 0) {
-    const double f = out.reduction == 1 ? 1.0 : count > 0 ? 1.0 / count : 0.0;
-    *out.loss      = static_cast<float>(count > 0 ? sum * f : 0.0);
-    *out.factor    = static_cast<float>(f);
-  }
-}
+__global__ void no_rows(Reduced out) { write_reduced(out, make_double2(0, 0)); }
 
 __global__ void wait_for_nothing()
 {
@@ -688,33 +706,32 @@ bool logits_product(Product& p, bool bf16, const LinearArgs& a, int64_t first, i
 template <class T>
 cudaError_t run_linear(bool bf16, const LinearArgs& a, const Reduced& out, void* workspace, int n_sms, cudaStream_t s)
 {
+  if (a.n_rows == 0) {
+    if (out.reduction != 0) no_rows<<<1, 1, 0, s>>>(out);
+    count_launches(out.reduction != 0);
+    return cudaGetLastError();
+  }
   double2* sums = static_cast<double2*>(workspace);
-  int launched = 0, blocks = 0;
-  if (a.n_rows > 0) {
-    Work w{};
-    w.products = 1;
-    w.bf16     = bf16;
-    w.c        = 1.4426950408889634f / a.temperature;
-    w.parts    = reinterpret_cast<float2*>(sums + 8 * n_sms);
-    if (!logits_product(w.product[0], bf16, a, 0, a.n_cols, kStats)) return cudaErrorInvalidValue;
-    cudaError_t e = run_products<kStats>(w, n_sms, s);
-    if (e != cudaSuccess) return e;
-    const bool warp    = a.teacher.k == 1;
-    const int per      = warp ? kThreads / 32 : 1;
-    const int64_t need = (a.n_rows + per - 1) / per;
-    blocks             = static_cast<int>(need < 8 * n_sms ? need : 8 * n_sms);
-    const size_t bytes = per * (256 + static_cast<size_t>(a.teacher.k + 1) / 2 * 2 * 12);
-    if (warp)
-      linear_rows<T, 32><<<blocks, kThreads, bytes, s>>>(a, w.parts, w.product[0].n_tiles, sums);
-    else
-      linear_rows<T, kThreads><<<blocks, kThreads, bytes, s>>>(a, w.parts, w.product[0].n_tiles, sums);
-    launched = 2;
-  }
-  if (out.reduction != 0) {
-    reduce_rows<<<1, kThreads, 0, s>>>(sums, blocks, out);
-    ++launched;
-  }
-  count_launches(launched);
+  Work w{};
+  w.products = 1;
+  w.bf16     = bf16;
+  w.c        = 1.4426950408889634f / a.temperature;
+  w.ticket   = reinterpret_cast<int*>(sums + 8 * n_sms);
+  w.parts    = reinterpret_cast<float2*>(sums + 8 * n_sms + 1);
+  if (!logits_product(w.product[0], bf16, a, 0, a.n_cols, kStats)) return cudaErrorInvalidValue;
+  cudaError_t e = run_products<kStats>(w, n_sms, s);
+  if (e != cudaSuccess) return e;
+  // a warp per row where there are enough rows (or nothing to share), else a block
+  const bool warp    = a.teacher.k <= 4 || a.n_rows >= 8 * n_sms;
+  const int per      = warp ? kThreads / 32 : 1;
+  const int64_t need = (a.n_rows + per - 1) / per;
+  const int blocks   = static_cast<int>(need < 8 * n_sms ? need : 8 * n_sms);
+  const size_t bytes = per * (entry_bytes(a.teacher.k) + static_cast<size_t>(a.teacher.k) * 4);
+  if (warp)
+    linear_rows<T, 32><<<blocks, kThreads, bytes, s>>>(a, w.parts, w.product[0].n_tiles, out, sums, w.ticket);
+  else
+    linear_rows<T, kThreads><<<blocks, kThreads, bytes, s>>>(a, w.parts, w.product[0].n_tiles, out, sums, w.ticket);
+  count_launches(2);
   return cudaGetLastError();
 }
 
@@ -759,9 +776,9 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
   float* sums          = reinterpret_cast<float*>(at += padded(a.n_rows * plan.cols * 2));
   const float d_scale  = bf16 ? 1.f : kHalfScale;
   const bool per_row   = g.factor == nullptr;
-  int launched         = 1;
+  int launched         = per_row;
   cudaError_t e        = cudaSuccess;
-  grad_scales<<<1, 1024, 0, s>>>(g, d_scale, scale, per_row ? row_scale : nullptr);
+  if (per_row) grad_scales<<<1, 1024, 0, s>>>(g, scale, row_scale);
   Work w{};
   w.bf16        = bf16;
   w.c           = 1.4426950408889634f / a.temperature;
@@ -773,16 +790,20 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
   w.sums        = sums;
   w.grad_hidden = g.grad_hidden;
   w.width       = a.width;
-  w.scale       = scale;
+  w.scale       = Scale{per_row ? scale : g.upstream, g.factor, a.temperature / d_scale};
+  w.named       = a.named;
+  w.k           = a.teacher.k;
   for (int i = 0; i < plan.pieces; ++i) {
     const int64_t first = i * plan.cols, n = a.n_cols - first < plan.cols ? a.n_cols - first : plan.cols;
     w.products = 1;
+    w.first    = static_cast<int>(first);
     if (!logits_product(w.product[0], bf16, a, first, n, kDiff)) return cudaErrorInvalidValue;
     if ((e = run_products<kDiff>(w, n_sms, s)) != cudaSuccess) return e;
-    const int64_t entries = a.n_rows * a.teacher.k;
-    const int64_t need    = (entries + kThreads - 1) / kThreads;
-    named_diff<T><<<static_cast<unsigned>(need < 8 * n_sms ? need : 8 * n_sms), kThreads, 0, s>>>(
-      a, first, n, diff, plan.cols, w.row_scale, d_scale, w.c);
+    if (w.k > kFewNamed) {
+      const int64_t entries = a.n_rows * w.k, need = (entries + kThreads - 1) / kThreads;
+      named_diff<T><<<static_cast<unsigned>(need < 8 * n_sms ? need : 8 * n_sms), kThreads, 0, s>>>(w, entries, static_cast<int>(n));
+      ++launched;
+    }
     // d ends with the tile that holds its last class: what is behind has not been written
     const int64_t made = static_cast<int64_t>(tiles_of(n)) * kTile;
     w.products         = 0;
@@ -819,12 +840,12 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
     w.add         = i > 0;
     w.grad_weight = g.grad_weight ? static_cast<T*>(g.grad_weight) + first * a.width : nullptr;
     if (w.products && (e = run_products<kWeight>(w, n_sms, s)) != cudaSuccess) return e;
-    launched += 3;
+    launched += 2;
   }
   if (g.grad_hidden && !plan.direct) {
     const int64_t n = a.n_rows * a.width, need = (n / 4 + kThreads - 1) / kThreads;
     finish_hidden<T><<<static_cast<unsigned>(need < 8 * n_sms ? need : 8 * n_sms), kThreads, 0, s>>>(
-      sums, plan.splits, n, scale, static_cast<T*>(g.grad_hidden));
+      sums, plan.splits, n, w.scale, static_cast<T*>(g.grad_hidden));
     ++launched;
   }
   count_launches(launched);
@@ -835,7 +856,7 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
 
 size_t linear_workspace(const LinearArgs& a, int n_sms)
 {
-  return 8 * n_sms * sizeof(double2) + a.n_rows * static_cast<size_t>(tiles_of(a.n_cols)) * sizeof(float2);
+  return (8 * n_sms + 1) * sizeof(double2) + a.n_rows * static_cast<size_t>(tiles_of(a.n_cols)) * sizeof(float2);
 }
 
 size_t linear_grad_workspace(const LinearGradArgs& g, int n_sms)

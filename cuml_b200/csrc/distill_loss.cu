@@ -7,9 +7,13 @@
 // Softmax cross entropy is the case of one named class of probability 1 and T = 1.
 //
 // Bound by memory: the forward pass reads the logits once (running maximum and sum), the backward pass
-// reads them again and writes as much.  A row is visited by a warp (up to kWarpCols classes; eight rows
-// per block, so that narrow rows fill the machine) or by a block; where rows are few, by several blocks
-// whose maxima and sums are joined by the kernel that reads the teacher.
+// reads them again and writes as much.  What a teacher names in a row is the work of one warp, whose chain of
+// dependent loads, votes and logarithms takes as long as reading some 32 KB.  Rows of up to kWarpCols
+// classes therefore belong to one warp altogether, and many warps hide it; longer ones to a block of eight
+// warps that read, while a ninth prepares the next row and a tenth finishes the last.  Where rows are few,
+// several blocks read parts of one and a warp joins their maxima and sums.
+#include <cooperative_groups.h>
+
 #include "distill_common.cuh"
 
 namespace b2fil {
@@ -17,32 +21,17 @@ namespace distill {
 namespace {
 
 constexpr int kThreads  = 256;
-constexpr int kWarpCols = 2048;   // widest rows that one warp visits
-constexpr int kSegment  = 8192;   // fewest elements of a row that are worth a block of their own
+constexpr int kWide     = kThreads + 64;  // eight warps that read, two for the teacher
+constexpr int kWideRows = 4;              // blocks of an SM
+constexpr int kWarpCols = 2048;           // longest rows of one warp
+constexpr int kSegment  = 8192;           // fewest elements of a row that are worth a block of their own
+constexpr int kMostBits = 1 << 17;        // classes that a block marks (three rows of it: 48 KB)
 constexpr int kMostSegs = 64;
 constexpr int kInFlight = 4;
+constexpr int kCluster  = 8;              // blocks that add up their losses without another kernel
 
-// Shared memory of one row: room for reductions, p, at and (REST) the bits of the named classes.
-struct RowRoom {
-  double* room;
-  float* p;
-  int* at;
-  uint32_t* bits;
-};
-__host__ __device__ __forceinline__ size_t row_bytes(int k, int64_t bit_cols)
-{
-  const size_t bits = bit_cols ? ((bit_cols + 32) / 32 + 2) * 4 : 0;
-  return (32 * 8 + static_cast<size_t>(k) * 8 + bits + 7) / 8 * 8;
-}
-__device__ __forceinline__ RowRoom room_of(char* base, int k)
-{
-  RowRoom r;
-  r.room = reinterpret_cast<double*>(base);
-  r.p    = reinterpret_cast<float*>(base + 256);
-  r.at   = reinterpret_cast<int*>(r.p + k);
-  r.bits = reinterpret_cast<uint32_t*>(r.at + k);
-  return r;
-}
+// Bits of the named classes: bit 32 stands for the first element on a 16-byte boundary.
+__host__ __device__ __forceinline__ size_t bit_bytes(int64_t cols) { return cols ? ((cols + 32) / 32 + 2) * 4 : 0; }
 
 // Running maximum and sum of n elements; with REST those whose bit is set are left out.  Bit 32 stands for
 // the first element on a 16-byte boundary, so that a piece's bits lie in one word.
@@ -63,19 +52,18 @@ __device__ __forceinline__ Running<float> visit_logits(const T* row, int64_t n, 
       r.take(widen(x), c);
     },
     [&](int64_t i, const Piece<T>& v) {
+      float x[N], most;
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[e] = widen(v.v[e]);
       if (REST) {
         const uint32_t at  = static_cast<uint32_t>(i - lead + 32);
         const uint32_t set = bits[at >> 5] >> (at & 31) & ((1u << N) - 1);
         if (set) {
 #pragma unroll
           for (int e = 0; e < N; ++e)
-            if (!(set >> e & 1)) r.take(widen(v.v[e]), c);
-          return;
+            if (set >> e & 1) x[e] = lowest<float>();
         }
       }
-      float x[N], most;
-#pragma unroll
-      for (int e = 0; e < N; ++e) x[e] = widen(v.v[e]);
       most = x[0];
 #pragma unroll
       for (int e = 1; e < N; ++e) most = fmaxf(most, x[e]);
@@ -87,19 +75,19 @@ __device__ __forceinline__ Running<float> visit_logits(const T* row, int64_t n, 
   return r;
 }
 
-template <int THREADS>
-__device__ __forceinline__ void mark_named(const Teacher& t, int64_t row, int64_t n_cols, int64_t begin, int64_t n,
-                                           int lead, int tid, uint32_t* bits)
+// Marks (or unmarks) the entries that lie in n columns from `begin` on.  By one warp.
+template <bool SET>
+__device__ __forceinline__ void mark(const Entries& e, int k, int64_t begin, int64_t n, int lead, uint32_t* bits)
 {
-  for (int w = tid; w < (n - lead + 32) / 32 + 1; w += THREADS) bits[w] = 0;
-  sync_row<THREADS>();
-  for (int j = tid; j < t.k; j += THREADS) {
-    const int64_t c = teacher_index(t, row, j);
-    if (c < begin || c >= begin + n || c >= n_cols || c == t.ignore) continue;
-    const uint32_t at = static_cast<uint32_t>(c - begin - lead + 32);
-    atomicOr(&bits[at >> 5], 1u << (at & 31));
+  for (int j = threadIdx.x % 32; j < k; j += 32) {
+    const int64_t c = e.at[j] - begin;
+    if (e.at[j] < 0 || c < 0 || c >= n) continue;
+    const uint32_t at = static_cast<uint32_t>(c - lead + 32);
+    if (SET)
+      atomicOr(&bits[at >> 5], 1u << (at & 31));
+    else
+      atomicAnd(&bits[at >> 5], ~(1u << (at & 31)));
   }
-  sync_row<THREADS>();
 }
 
 // One part of a row per block: (row, segment) -> its maximum and sum.
@@ -107,126 +95,213 @@ template <class T, bool REST>
 __global__ void __launch_bounds__(kThreads) loss_parts(LossArgs a, int64_t seg_cols, float2* parts)
 {
   extern __shared__ __align__(16) char smem[];
-  const RowRoom room  = room_of(smem, a.teacher.k);
+  __shared__ float room[2 * kThreads / 32];
+  uint32_t* bits      = reinterpret_cast<uint32_t*>(smem);
   const int64_t begin = blockIdx.x * seg_cols;
   const int64_t n     = min(seg_cols, a.n_cols - begin);
   const float c       = 1.4426950408889634f / a.temperature;
   for (int64_t row = blockIdx.y; row < a.n_rows; row += gridDim.y) {
     const T* x = static_cast<const T*>(a.logits) + row * a.row_stride + begin;
     if (REST) {
+      const int lead = lead_of(x, n);
       __syncthreads();
-      mark_named<kThreads>(a.teacher, row, a.n_cols, begin, n, lead_of(x, n), threadIdx.x, room.bits);
+      for (int w = threadIdx.x; w < bit_bytes(n) / 4; w += kThreads) bits[w] = 0;
+      __syncthreads();
+      for (int j = threadIdx.x; j < a.teacher.k; j += kThreads) {
+        const int64_t at = teacher_index(a.teacher, row, j);
+        if (at < begin || at >= begin + n || at == a.teacher.ignore) continue;
+        const uint32_t bit = static_cast<uint32_t>(at - begin - lead + 32);
+        atomicOr(&bits[bit >> 5], 1u << (bit & 31));
+      }
+      __syncthreads();
     }
-    Running<float> r = visit_logits<T, REST>(x, n, threadIdx.x, kThreads, c, room.bits);
-    join_row<kThreads>(r, c, reinterpret_cast<float*>(room.room));
+    Running<float> r = visit_logits<T, REST>(x, n, threadIdx.x, kThreads, c, bits);
+    join_row<kThreads>(r, c, room);
     if (threadIdx.x == 0) parts[row * gridDim.x + blockIdx.x] = make_float2(r.m, r.s);
   }
 }
 
-// Losses of rows; THREADS threads per row.  segs > 0: maxima and sums come from `parts`.
-template <class T, int THREADS, bool REST>
-__global__ void __launch_bounds__(kThreads) loss_rows(LossArgs a, int segs, const float2* parts, size_t row_room,
-                                                      double2* block_sums)
+// A row's loss, by one warp.  r: maximum and sum of the logits (REST: of those that are not named).
+template <class T, bool REST>
+__device__ __forceinline__ void finish_row(const LossArgs& a, int64_t row, const T* x, const Entries& e, const TeacherRow& t,
+                                           double inv_t, float c, Running<float> r, double& sum, double& count)
 {
-  extern __shared__ __align__(16) char smem[];
-  constexpr int ROWS = kThreads / THREADS;
-  const int slot = threadIdx.x / THREADS, tid = threadIdx.x % THREADS;
-  const RowRoom room = room_of(smem + slot * row_room, a.teacher.k);
-  const float c      = 1.4426950408889634f / a.temperature;
-  const double inv_t = 1.0 / a.temperature;
-  double sum = 0, count = 0;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + slot; row < a.n_rows;
-       row += static_cast<int64_t>(gridDim.x) * ROWS) {
-    const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
-    const TeacherRow t =
-      read_teacher<THREADS>(a.teacher, row, a.n_cols, inv_t, tid, room.p, room.at, room.room);
-    Running<float> r;
-    if (segs > 0) {
-      for (int i = tid; i < segs; i += THREADS) r.join(parts[row * segs + i].x, parts[row * segs + i].y, c);
-    } else {
-      if (REST) mark_named<THREADS>(a.teacher, row, a.n_cols, 0, a.n_cols, lead_of(x, a.n_cols), tid, room.bits);
-      r = visit_logits<T, REST>(x, a.n_cols, tid, THREADS, c, room.bits);
-    }
-    join_row<THREADS>(r, c, reinterpret_cast<float*>(room.room));
-    const Running<float> others = r;
-    if (REST) {
-      Running<float> mine;
-      for (int j = tid; j < a.teacher.k; j += THREADS)
-        if (room.at[j] >= 0) mine.take(widen(x[room.at[j]]), c);
-      join_row<THREADS>(mine, c, reinterpret_cast<float*>(room.room));
-      r.join(mine.m, mine.s, c);
-    }
-    const double log_s = log(static_cast<double>(r.s));
-    const bool counts  = t.counts && !(r.s == 0.f);  // (no class has a finite logit: no softmax)
-    double loss        = 0;
-    for (int j = tid; j < a.teacher.k; j += THREADS) {
-      const int at  = room.at[j];
-      const float p = room.p[j];
-      if (at < 0 || p == 0.f) continue;
-      const double log_p = t.merged ? log(static_cast<double>(p))
-                                    : (a.teacher.values ? a.teacher.values[row * a.teacher.values_stride + j] * inv_t : 0.0) - t.log_norm;
-      const double log_q = (static_cast<double>(widen(x[at])) - r.m) * inv_t - log_s;
-      loss += p * (log_p - log_q);
-    }
-    loss         = sum_row<THREADS>(loss, room.room);
-    float factor = 1.f;
-    if (REST && t.rest != 0.0) {
-      const double log_rest = (static_cast<double>(others.m) - r.m) * inv_t + log(static_cast<double>(others.s)) - log_s;
-      loss += t.rest * (log(t.rest) - log_rest);
-      factor = static_cast<float>(1.0 - t.rest / exp(log_rest));
-    }
-    if (!counts) loss = 0;
-    loss *= static_cast<double>(a.temperature) * a.temperature;
-    if (tid == 0) {
-      a.row_loss[row]  = static_cast<float>(loss);
-      a.row_stats[row] = make_float4(r.m, 1.f / r.s, factor, counts ? 1.f : 0.f);
-      sum += loss;
-      count += counts;
-    }
+  const int lane = threadIdx.x % 32, k = a.teacher.k;
+  const Running<float> others = r;
+  if (REST) {
+    Running<float> mine;
+    for (int j = lane; j < k; j += 32)
+      if (e.at[j] >= 0) mine.take(widen(x[e.at[j]]), c);
+    mine.join_lanes(c);
+    r.join(mine.m, mine.s, c);
   }
-  // sums of the block's rows, in a fixed order
-  __shared__ double2 sums[ROWS];
-  if (tid == 0) sums[slot] = make_double2(sum, count);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double2 all = sums[0];
-    for (int i = 1; i < ROWS; ++i) {
-      all.x += sums[i].x;
-      all.y += sums[i].y;
-    }
-    block_sums[blockIdx.x] = all;
+  const double log_s = log_sum(r.s);
+  const bool counts  = t.counts && !(r.s == 0.f);  // (no class has a finite logit: no softmax)
+  double loss        = named_loss(e, k, t, inv_t, r.m, log_s, [&](int, int at) { return widen(x[at]); });
+  float factor       = 1.f;
+  if (REST && t.rest != 0.f) {
+    const double log_rest = (static_cast<double>(others.m) - r.m) * inv_t + log_sum(others.s) - log_s;
+    loss += t.rest * (log_sum(t.rest) - log_rest);
+    factor = 1.f - t.rest / (others.s * power((others.m - base_of(r.m)) * c) / r.s);
+  }
+  if (!counts) loss = 0;
+  loss *= static_cast<double>(a.temperature) * a.temperature;
+  for (int j = lane; j < k; j += 32) {
+    a.named.p[row * k + j]  = e.p[j];
+    a.named.at[row * k + j] = e.at[j];
+  }
+  if (lane == 0) {
+    a.row_loss[row]  = static_cast<float>(loss);
+    a.row_stats[row] = make_float4(r.m, 1.f / r.s, factor, counts ? 1.f : 0.f);
+    sum += loss;
+    count += counts;
   }
 }
 
-// Sum, or mean over the rows that count (0 if none does).
+// Adds up the losses of a launch of one cluster, or leaves the block's for reduce_loss.
+template <int THREADS>
+__device__ __forceinline__ void finish_block(double sum, double count, bool one_cluster, const Reduced& out, double2* block_sums)
+{
+  __shared__ double2 room[THREADS / 32];
+  __shared__ double2 mine;
+  if (out.reduction == 0) return;
+  const double2 all = sum_block<THREADS>(sum, count, room);
+  if (!one_cluster) {
+    if (threadIdx.x == 0) block_sums[blockIdx.x] = all;
+    return;
+  }
+  namespace cg = cooperative_groups;
+  if (threadIdx.x == 0) mine = all;
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    double2 total = make_double2(0, 0);
+    for (int i = 0; i < static_cast<int>(gridDim.x); ++i) {
+      const double2 o = *cluster.map_shared_rank(&mine, i);
+      total.x += o.x;
+      total.y += o.y;
+    }
+    write_reduced(out, total);
+  }
+  cluster.sync();  // the others' shared memory has been read
+}
+
+// A row per warp.  segs > 0: maxima and sums come from `parts`.
+template <class T, bool REST>
+__global__ void __launch_bounds__(kThreads, 5) loss_narrow(LossArgs a, int segs, const float2* parts, size_t warp_room,
+                                                        bool one_cluster, Reduced out, double2* block_sums)
+{
+  extern __shared__ __align__(16) char smem[];
+  constexpr int ROWS = kThreads / 32;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, k = a.teacher.k;
+  const Entries e    = entries_at(smem + warp * warp_room, k);
+  uint32_t* bits     = reinterpret_cast<uint32_t*>(e.at + k);
+  const float c      = 1.4426950408889634f / a.temperature;
+  const double inv_t = 1.0 / a.temperature;
+  double sum = 0, count = 0;
+  if (REST && segs == 0) {
+    for (int w = lane; w < bit_bytes(a.n_cols) / 4; w += 32) bits[w] = 0;
+    __syncwarp();
+  }
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + warp; row < a.n_rows; row += static_cast<int64_t>(gridDim.x) * ROWS) {
+    const T* x         = static_cast<const T*>(a.logits) + row * a.row_stride;
+    const int lead     = lead_of(x, a.n_cols);
+    const TeacherRow t = read_teacher<REST>(a.teacher, row, a.n_cols, inv_t, e);
+    Running<float> r;
+    if (segs > 0) {
+      for (int i = lane; i < segs; i += 32) r.join(parts[row * segs + i].x, parts[row * segs + i].y, c);
+    } else {
+      if (REST) {
+        mark<true>(e, k, 0, a.n_cols, lead, bits);
+        __syncwarp();
+      }
+      r = visit_logits<T, REST>(x, a.n_cols, lane, 32, c, bits);
+    }
+    r.join_lanes(c);
+    finish_row<T, REST>(a, row, x, e, t, inv_t, c, r, sum, count);
+    if (REST && segs == 0) mark<false>(e, k, 0, a.n_cols, lead, bits);
+    __syncwarp();
+  }
+  finish_block<kThreads>(sum, count, one_cluster, out, block_sums);
+}
+
+// A row per block: while eight warps read row i, one prepares row i + 1 and one finishes row i - 1.
+template <class T, bool REST>
+__global__ void __launch_bounds__(kWide, kWideRows) loss_wide(LossArgs a, size_t bits_room, bool one_cluster, Reduced out,
+                                                              double2* block_sums)
+{
+  extern __shared__ __align__(16) char smem[];
+  constexpr int W = kThreads / 32;
+  __shared__ float2 parts[2][W];
+  __shared__ TeacherRow teachers[3];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, k = a.teacher.k;
+  const float c      = 1.4426950408889634f / a.temperature;
+  const double inv_t = 1.0 / a.temperature;
+  auto entries       = [&](int i) { return entries_at(smem + 3 * bits_room + i * entry_bytes(k), k); };
+  auto bits          = [&](int i) { return reinterpret_cast<uint32_t*>(smem + i * bits_room); };
+  auto logits        = [&](int64_t row) { return static_cast<const T*>(a.logits) + row * a.row_stride; };
+  double sum = 0, count = 0;
+  if (REST)
+    for (int w = threadIdx.x; w < 3 * bits_room / 4; w += kWide) reinterpret_cast<uint32_t*>(smem)[w] = 0;
+  // (bits and entries of rows i - 1, i and i + 1 are in use at a time)
+  auto prepare = [&](int64_t row, int at) {
+    const TeacherRow t = read_teacher<REST>(a.teacher, row, a.n_cols, inv_t, entries(at));
+    if (lane == 0) teachers[at] = t;
+    if (REST) mark<true>(entries(at), k, 0, a.n_cols, lead_of(logits(row), a.n_cols), bits(at));
+  };
+  __syncthreads();
+  if (warp == W && blockIdx.x < a.n_rows) prepare(blockIdx.x, 0);
+  int last = 2, now = 0, next = 1, half = 0;
+  for (int64_t row = blockIdx.x; row - gridDim.x < a.n_rows; row += gridDim.x) {
+    __syncthreads();  // this row is marked, the last one has been read
+    if (warp < W) {
+      if (row < a.n_rows) {
+        Running<float> r = visit_logits<T, REST>(logits(row), a.n_cols, threadIdx.x, kThreads, c, bits(now));
+        r.join_lanes(c);
+        if (lane == 0) parts[half][warp] = make_float2(r.m, r.s);
+      }
+    } else if (warp == W) {
+      if (row + gridDim.x < a.n_rows) prepare(row + gridDim.x, next);
+    } else if (row != blockIdx.x) {
+      const int64_t done = row - gridDim.x;
+      Running<float> r;
+      if (lane < W) {
+        r.m = parts[half ^ 1][lane].x;
+        r.s = parts[half ^ 1][lane].y;
+      }
+      r.join_lanes(c);
+      finish_row<T, REST>(a, done, logits(done), entries(last), teachers[last], inv_t, c, r, sum, count);
+      if (REST) mark<false>(entries(last), k, 0, a.n_cols, lead_of(logits(done), a.n_cols), bits(last));
+    }
+    const int first = last;
+    last = now;
+    now  = next;
+    next = first;
+    half ^= 1;
+  }
+  finish_block<kWide>(sum, count, one_cluster, out, block_sums);
+}
+
 __global__ void __launch_bounds__(kThreads) reduce_loss(const double2* block_sums, int n, Reduced out)
 {
-  __shared__ double room[32];
+  __shared__ double2 room[kThreads / 32];
   double sum = 0, count = 0;
   for (int i = threadIdx.x; i < n; i += kThreads) {
     sum += block_sums[i].x;
     count += block_sums[i].y;
   }
-  sum   = sum_row<kThreads>(sum, room);
-  count = sum_row<kThreads>(count, room);
-  if (threadIdx.x == 0) {
-    const double f = out.reduction == 1 ? 1.0 : count > 0 ? 1.0 / count : 0.0;
-    *out.loss      = static_cast<float>(count > 0 ? sum * f : 0.0);
-    *out.factor    = static_cast<float>(f);
-  }
+  const double2 all = sum_block<kThreads>(sum, count, room);
+  if (threadIdx.x == 0) write_reduced(out, all);
 }
 
-// Gradient of a part of a row; blockIdx.y: the part.
-template <class T, int THREADS, bool REST>
-__global__ void __launch_bounds__(kThreads) loss_grad(LossGradArgs g, int64_t seg_cols, size_t row_room)
+// Gradient of a part of a row by THREADS threads; blockIdx.y: the part.
+template <class T, int THREADS>
+__global__ void __launch_bounds__(kThreads) loss_grad(LossGradArgs g, int64_t seg_cols)
 {
-  extern __shared__ __align__(16) char smem[];
   constexpr int ROWS = kThreads / THREADS, N = Piece<T>::N;
   const LossArgs& a = g.fwd;
-  const int slot = threadIdx.x / THREADS, tid = threadIdx.x % THREADS;
-  const RowRoom room  = room_of(smem + slot * row_room, a.teacher.k);
+  const int slot = threadIdx.x / THREADS, tid = threadIdx.x % THREADS, k = a.teacher.k;
   const float c       = 1.4426950408889634f / a.temperature;
-  const double inv_t  = 1.0 / a.temperature;
   const int64_t begin = blockIdx.y * seg_cols;
   const int64_t n     = min(seg_cols, a.n_cols - begin);
   const float scale   = (g.factor ? *g.factor : 1.f) * a.temperature;
@@ -237,10 +312,8 @@ __global__ void __launch_bounds__(kThreads) loss_grad(LossGradArgs g, int64_t se
     const float4 s = a.row_stats[row];
     const float up = g.upstream[row * g.upstream_stride] * scale;
     const bool counts = s.w != 0.f;
-    const TeacherRow t = read_teacher<THREADS>(a.teacher, row, a.n_cols, inv_t, tid, room.p, room.at, room.room);
-    (void)t;
     // zero for rows that do not count, whatever their logits are
-    const float base = base_of(s.x), f = s.y * up * (REST ? s.z : 1.f);
+    const float base = base_of(s.x), f = s.y * up * s.z;
     auto one = [&](int64_t i, T v) { d[i] = narrow<T>(counts ? power((widen(v) - base) * c) * f : 0.f); };
     if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0) {
       visit_row<kInFlight>(x, n, tid, THREADS, one, [&](int64_t i, const Piece<T>& v) {
@@ -254,22 +327,25 @@ __global__ void __launch_bounds__(kThreads) loss_grad(LossGradArgs g, int64_t se
     }
     sync_row<THREADS>();
     if (counts) {
-      for (int j = tid; j < a.teacher.k; j += THREADS) {
-        const int64_t at = room.at[j] - begin;
-        if (room.at[j] < 0 || at < 0 || at >= n) continue;
-        d[at] = narrow<T>((power((widen(x[at]) - base) * c) * s.y - room.p[j]) * up);
+      for (int j = tid; j < k; j += THREADS) {
+        const int cls    = a.named.at[row * k + j];
+        const int64_t at = cls - begin;
+        if (cls < 0 || at < 0 || at >= n) continue;
+        d[at] = narrow<T>((power((widen(x[at]) - base) * c) * s.y - a.named.p[row * k + j]) * up);
       }
     }
   }
 }
 
-int segments(int64_t n_rows, int64_t n_cols, int n_sms)
+int segments(int64_t n_rows, int64_t n_cols, int n_sms, bool rest)
 {
-  if (n_rows == 0 || n_cols <= kWarpCols || n_rows >= 2 * n_sms) return 1;
+  const int64_t least = rest ? (n_cols + kMostBits - 1) / kMostBits : 1;
+  if (n_rows == 0 || n_cols <= kWarpCols || n_rows >= 2 * n_sms) return static_cast<int>(least);
   const int64_t want = (4 * n_sms + n_rows - 1) / n_rows;
   const int64_t most = (n_cols + kSegment - 1) / kSegment;
-  const int64_t segs = want < most ? want : most;
-  return static_cast<int>(segs < 1 ? 1 : segs > kMostSegs ? kMostSegs : segs);
+  int64_t segs       = want < most ? want : most;
+  segs               = segs < 1 ? 1 : segs > kMostSegs ? kMostSegs : segs;
+  return static_cast<int>(segs < least ? least : segs);
 }
 // length of a part: whole 128-byte lines of every type
 int64_t part_cols(int64_t n_cols, int segs)
@@ -284,37 +360,63 @@ cudaError_t allow(K kernel, size_t bytes)
                             : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
 }
 
+// Launches a kernel whose blocks, up to kCluster of them, are one cluster and add up their losses.
+template <class... P, class... A>
+cudaError_t launch_rows(void (*kernel)(P...), int blocks, bool one_cluster, int threads, size_t bytes, cudaStream_t s, A... args)
+{
+  cudaError_t e = allow(kernel, bytes);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t config{};
+  config.gridDim          = dim3(blocks);
+  config.blockDim         = dim3(threads);
+  config.dynamicSmemBytes = bytes;
+  config.stream           = s;
+  cudaLaunchAttribute attribute{};
+  attribute.id               = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = blocks;
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs    = &attribute;
+  config.numAttrs = one_cluster ? 1 : 0;
+  return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
+}
+
 template <class T, bool REST>
 cudaError_t run_loss(const LossArgs& a, const Reduced& out, void* workspace, int n_sms, cudaStream_t s)
 {
-  int segs           = segments(a.n_rows, a.n_cols, n_sms);
+  int segs           = segments(a.n_rows, a.n_cols, n_sms, REST);
   const int64_t cols = part_cols(a.n_cols, segs);
   segs               = segs == 1 ? 1 : static_cast<int>((a.n_cols + cols - 1) / cols);
-  const bool warp    = a.n_cols <= kWarpCols;
-  const int per      = warp ? kThreads / 32 : 1;
-  const int64_t need = (a.n_rows + per - 1) / per;
-  const int blocks   = static_cast<int>(need < 8 * n_sms ? need : 8 * n_sms);
+  const bool narrow  = a.n_cols <= kWarpCols || segs > 1;
+  const int per      = narrow ? kThreads / 32 : 1;
+  const int64_t need = (a.n_rows + per - 1) / per, most = (narrow ? 8ll : kWideRows) * n_sms;
+  int blocks         = static_cast<int>(need < most ? need : most);
   double2* sums      = static_cast<double2*>(workspace);
   float2* parts      = reinterpret_cast<float2*>(sums + 8 * n_sms);
-  int launched       = 1;
-  cudaError_t e      = cudaSuccess;
-  if (segs > 1) {
-    const size_t bytes = row_bytes(a.teacher.k, REST ? cols : 0);
+  const bool cluster = out.reduction != 0 && blocks >= 1 && blocks <= kCluster;
+  while (cluster && (blocks & (blocks - 1))) ++blocks;
+  int launched  = 0;
+  cudaError_t e = cudaSuccess;
+  if (segs > 1 && a.n_rows > 0) {
+    const size_t bytes = REST ? bit_bytes(cols) : 0;
+    const unsigned rows = static_cast<unsigned>(a.n_rows < 65535 ? a.n_rows : 65535);
     if ((e = allow(loss_parts<T, REST>, bytes)) != cudaSuccess) return e;
-    loss_parts<T, REST><<<dim3(segs, static_cast<unsigned>(a.n_rows)), kThreads, bytes, s>>>(a, cols, parts);
+    loss_parts<T, REST><<<dim3(segs, rows), kThreads, bytes, s>>>(a, cols, parts);
     ++launched;
   }
-  const size_t bytes = row_bytes(a.teacher.k, REST && segs == 1 ? a.n_cols : 0);
-  if (a.n_rows == 0) {
-    launched = 0;
-  } else if (warp) {
-    if ((e = allow(loss_rows<T, 32, REST>, per * bytes)) != cudaSuccess) return e;
-    loss_rows<T, 32, REST><<<blocks, kThreads, per * bytes, s>>>(a, 0, nullptr, bytes, sums);
-  } else {
-    if ((e = allow(loss_rows<T, kThreads, REST>, bytes)) != cudaSuccess) return e;
-    loss_rows<T, kThreads, REST><<<blocks, kThreads, bytes, s>>>(a, segs > 1 ? segs : 0, parts, bytes, sums);
+  if (blocks > 0) {
+    const size_t bits = REST && segs == 1 ? (bit_bytes(a.n_cols) + 15) / 16 * 16 : 0;
+    if (narrow) {
+      const size_t room = (entry_bytes(a.teacher.k) + bits + 15) / 16 * 16;
+      e = launch_rows(loss_narrow<T, REST>, blocks, cluster, kThreads, room * per, s, a, segs > 1 ? segs : 0, parts, room,
+                      cluster, out, sums);
+    } else {
+      e = launch_rows(loss_wide<T, REST>, blocks, cluster, kWide, 3 * (bits + entry_bytes(a.teacher.k)), s, a, bits, cluster,
+                      out, sums);
+    }
+    if (e != cudaSuccess) return e;
+    ++launched;
   }
-  if (out.reduction != 0) {
+  if (out.reduction != 0 && !cluster) {
     reduce_loss<<<1, kThreads, 0, s>>>(sums, blocks, out);
     ++launched;
   }
@@ -322,25 +424,21 @@ cudaError_t run_loss(const LossArgs& a, const Reduced& out, void* workspace, int
   return cudaGetLastError();
 }
 
-template <class T, bool REST>
+template <class T>
 cudaError_t run_grad(const LossGradArgs& g, int n_sms, cudaStream_t s)
 {
   const LossArgs& a  = g.fwd;
   const bool warp    = a.n_cols <= kWarpCols;
   const int per      = warp ? kThreads / 32 : 1;
-  int segs           = warp ? 1 : segments(a.n_rows, a.n_cols, n_sms);
+  int segs           = warp ? 1 : segments(a.n_rows, a.n_cols, n_sms, false);
   const int64_t cols = part_cols(a.n_cols, segs);
   segs               = segs == 1 ? 1 : static_cast<int>((a.n_cols + cols - 1) / cols);
   const int64_t need = (a.n_rows + per - 1) / per;
   const int blocks   = static_cast<int>(need < 8 * n_sms ? need : 8 * n_sms);
-  const size_t bytes = row_bytes(a.teacher.k, 0);
-  cudaError_t e;
-  if (warp) {
-    if ((e = allow(loss_grad<T, 32, REST>, per * bytes)) != cudaSuccess) return e;
-    loss_grad<T, 32, REST><<<dim3(blocks, 1), kThreads, per * bytes, s>>>(g, cols, bytes);
-  } else {
-    loss_grad<T, kThreads, REST><<<dim3(blocks, segs), kThreads, bytes, s>>>(g, cols, bytes);
-  }
+  if (warp)
+    loss_grad<T, 32><<<dim3(blocks, 1), kThreads, 0, s>>>(g, cols);
+  else
+    loss_grad<T, kThreads><<<dim3(blocks, segs), kThreads, 0, s>>>(g, cols);
   count_launches(1);
   return cudaGetLastError();
 }
@@ -349,7 +447,7 @@ cudaError_t run_grad(const LossGradArgs& g, int n_sms, cudaStream_t s)
 
 size_t loss_workspace(const LossArgs& a, int n_sms)
 {
-  const int segs = segments(a.n_rows, a.n_cols, n_sms);
+  const int segs = segments(a.n_rows, a.n_cols, n_sms, true);  // (as many as either kind of tail takes)
   return 8 * n_sms * sizeof(double2) + (segs > 1 ? a.n_rows * segs * sizeof(float2) : 0);
 }
 
@@ -369,15 +467,11 @@ cudaError_t launch_loss(int dtype, const LossArgs& a, const Reduced& out, void* 
 
 cudaError_t launch_loss_grad(int dtype, const LossGradArgs& g, int n_sms, cudaStream_t s)
 {
-  const bool rest = g.fwd.teacher.logsumexp != nullptr;
-#define B2FIL_CASE(id, T) \
-  case id: return rest ? run_grad<T, true>(g, n_sms, s) : run_grad<T, false>(g, n_sms, s);
   switch (dtype) {
-    B2FIL_CASE(kF32, float)
-    B2FIL_CASE(kBF16, __nv_bfloat16)
-    B2FIL_CASE(kF16, __half)
+    case kF32: return run_grad<float>(g, n_sms, s);
+    case kBF16: return run_grad<__nv_bfloat16>(g, n_sms, s);
+    case kF16: return run_grad<__half>(g, n_sms, s);
   }
-#undef B2FIL_CASE
   return cudaErrorInvalidValue;
 }
 

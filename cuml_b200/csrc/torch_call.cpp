@@ -294,9 +294,10 @@ void no_second_derivative(Tensor& grad, const ag::variable_list& of)
 }
 
 struct LossNode : ag::Node {
-  ag::SavedVariable logits, values, index, logsumexp;
+  ag::SavedVariable logits;
   Tensor kept;
   Options o;
+  int k;
   bool gone = false;
 
   ag::variable_list apply(ag::variable_list&& grads) override
@@ -308,18 +309,17 @@ struct LossNode : ag::Node {
       at::AutoDispatchBelowADInplaceOrView below;
       at::NoGradGuard no_grad;
       x = logits.unpack();
-      const TeacherOf t{values.unpack(), index.unpack(), logsumexp.unpack(), o.ignore};
       const int64_t n = x.size(0), c = x.size(1);
       grad = make({n, c}, x.scalar_type(), x);
       int64_t stride;
-      const Tensor g           = upstream_of(grads[0], stride);
-      const b2fil_teacher tc   = t.c();
-      const float* stats       = kept.const_data_ptr<float>();
-      const int device         = x.get_device();
+      const Tensor g     = upstream_of(grads[0], stride);
+      const float* at    = kept.const_data_ptr<float>();
+      const float* named = at + 4 * n + 4;
+      const int device   = x.get_device();
       try {
-        ok(library.loss_grad(type_of(x), x.const_data_ptr(), n, c, x.stride(0), &tc, o.temperature, stats,
-                             g.const_data_ptr<float>(), stride, o.reduction ? stats + 4 * n : nullptr,
-                             grad.mutable_data_ptr(), c, device, stream_of(device)));
+        ok(library.loss_grad(type_of(x), x.const_data_ptr(), n, c, x.stride(0), k, o.temperature, at, named,
+                             reinterpret_cast<const int32_t*>(named + n * k), g.const_data_ptr<float>(), stride,
+                             o.reduction ? at + 4 * n : nullptr, grad.mutable_data_ptr(), c, device, stream_of(device)));
       } catch (const LibraryError& e) {
         raise_library_error(e);
       }
@@ -330,9 +330,6 @@ struct LossNode : ag::Node {
   void release_variables() override
   {
     logits.reset_data();
-    values.reset_data();
-    index.reset_data();
-    logsumexp.reset_data();
     kept = Tensor();
     gone = true;
   }
@@ -353,32 +350,34 @@ PyObject* distill_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   if (type < 0 || type == B2FIL_TYPE_F64 || !teacher_of(args[1], args[2], args[3], x, t)) Py_RETURN_NONE;
   t.ignore        = o.ignore;
   const int64_t n = x.size(0), c = x.size(1);
+  const int k     = static_cast<int>(t.index.size(1));
   Tensor kept, loss;
   try {
     at::AutoDispatchBelowADInplaceOrView below;
     const int device   = x.get_device();
-    const int64_t room = ok(library.loss_workspace(type, n, c, static_cast<int>(t.index.size(1)), device));
-    // statistics, factor, losses of the rows where they are not what is returned, workspace
-    const int64_t rows_at = 4 * n + 4, work_at = (rows_at + (o.reduction ? n : 0) + 63) / 64 * 64;
-    kept           = make({work_at + room / 4}, at::kFloat, x);
-    loss           = o.reduction ? make({}, at::kFloat, x) : make({n}, at::kFloat, x);
-    float* at      = kept.mutable_data_ptr<float>();
-    float* to      = loss.mutable_data_ptr<float>();
-    const auto tc  = t.c();
+    const int64_t room = ok(library.loss_workspace(type, n, c, k, device));
+    // statistics, factor, the named classes' arrays, losses of the rows where they are not what is
+    // returned, workspace
+    const int64_t named_at = 4 * n + 4, rows_at = named_at + 2 * n * k,
+                  work_at = (rows_at + (o.reduction ? n : 0) + 63) / 64 * 64;
+    kept          = make({work_at + room / 4}, at::kFloat, x);
+    loss          = o.reduction ? make({}, at::kFloat, x) : make({n}, at::kFloat, x);
+    float* at     = kept.mutable_data_ptr<float>();
+    float* to     = loss.mutable_data_ptr<float>();
+    const auto tc = t.c();
     ok(library.loss(type, x.const_data_ptr(), n, c, x.stride(0), &tc, o.temperature, o.reduction,
-                    o.reduction ? at + rows_at : to, at, to, at + 4 * n, at + work_at, room, device, stream_of(device)));
+                    o.reduction ? at + rows_at : to, at, at + named_at, reinterpret_cast<int32_t*>(at + named_at + n * k), to,
+                    at + 4 * n, at + work_at, room, device, stream_of(device)));
   } catch (const LibraryError& e) {
     return PyLong_FromLong(e.code);
   }
   if (at::GradMode::is_enabled() && x.requires_grad()) {
     auto node = std::shared_ptr<LossNode>(new LossNode(), ag::deleteNode);
     node->set_next_edges(ag::collect_next_edges(x));
-    node->logits    = ag::SavedVariable(x, false);
-    node->values    = ag::SavedVariable(t.values, false);
-    node->index     = ag::SavedVariable(t.index, false);
-    node->logsumexp = ag::SavedVariable(t.logsumexp, false);
-    node->kept      = std::move(kept);
-    node->o         = o;
+    node->logits = ag::SavedVariable(x, false);
+    node->kept   = std::move(kept);
+    node->o      = o;
+    node->k      = k;
     ag::set_history(loss, node);
   }
   return THPVariable_Wrap(std::move(loss));

@@ -209,34 +209,42 @@ class _Loss(torch.autograd.Function):
         x = _rows(logits)
         n, n_cols = x.shape
         t = _Teacher(n, dev, values, index, lse, ignore)
-        ws = _workspace(lib.b2fil_distill_loss_workspace(kind, n, n_cols, t.c.k, dev.index), dev)
-        stats = torch.empty((4 * n + 4,), dtype=torch.float32, device=dev)  # and the factor
+        k = t.c.k
+        ws = _workspace(lib.b2fil_distill_loss_workspace(kind, n, n_cols, k, dev.index), dev)
+        # kept for the gradient: statistics and the factor; the named classes' probabilities and places
+        kept = torch.empty((4 * n + 4 + 2 * n * k,), dtype=torch.float32, device=dev)
         rows = torch.empty((n,), dtype=torch.float32, device=dev)
         loss = torch.empty((), dtype=torch.float32, device=dev) if reduction else rows
-        factor = stats.data_ptr() + 16 * n if reduction else None
-        _lib.check(lib.b2fil_distill_loss(kind, x.data_ptr(), n, n_cols, x.stride(0), C.byref(t.c), temperature,
-                                          reduction, rows.data_ptr(), stats.data_ptr(), loss.data_ptr(), factor,
-                                          ws.data_ptr(), ws.numel(), dev.index, _stream(dev)))
-        ctx.save_for_backward(logits, values, index, lse)
-        ctx.stats, ctx.options = stats, (temperature, ignore, reduction)
+        stats, factor, named = _kept(kept, n)
+        _lib.check(lib.b2fil_distill_loss(
+            kind, x.data_ptr(), n, n_cols, x.stride(0), C.byref(t.c), temperature, reduction, rows.data_ptr(), stats, named,
+            named + 4 * n * k, loss.data_ptr(), factor if reduction else None, ws.data_ptr(), ws.numel(), dev.index,
+            _stream(dev)))
+        ctx.save_for_backward(logits)
+        ctx.kept, ctx.options = kept, (temperature, reduction, k)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        logits, values, index, lse = ctx.saved_tensors
-        temperature, ignore, reduction = ctx.options
+        (logits,) = ctx.saved_tensors
+        temperature, reduction, k = ctx.options
         lib, kind, dev = _lib.load(), _TYPES[logits.dtype], logits.device
         x = _rows(logits)
         n, n_cols = x.shape
         grad = torch.empty((n, n_cols), dtype=x.dtype, device=dev)
-        t = _Teacher(n, dev, values, index, lse, ignore)
         g, stride = _upstream(g)
+        stats, factor, named = _kept(ctx.kept, n)
         _lib.check(lib.b2fil_distill_loss_grad(
-            kind, x.data_ptr(), n, n_cols, x.stride(0), C.byref(t.c), temperature, ctx.stats.data_ptr(), g.data_ptr(),
-            stride, ctx.stats.data_ptr() + 16 * n if reduction else None, grad.data_ptr(), n_cols, dev.index,
-            _stream(dev)))
+            kind, x.data_ptr(), n, n_cols, x.stride(0), k, temperature, stats, named, named + 4 * n * k, g.data_ptr(), stride,
+            factor if reduction else None, grad.data_ptr(), n_cols, dev.index, _stream(dev)))
         return grad, None, None, None, None, None, None
+
+
+def _kept(kept, n):
+    """Addresses of the statistics, the factor and the named classes' arrays in what a forward pass keeps."""
+    at = kept.data_ptr()
+    return at, at + 16 * n, at + 16 * n + 16
 
 
 _STUDENT = (torch.float32, torch.bfloat16, torch.float16)
@@ -322,12 +330,6 @@ class _Linear(torch.autograd.Function):
             factor if reduction else None, dh.data_ptr() if of_hidden else None, dw.data_ptr() if of_weight else None,
             ws.data_ptr(), ws.numel(), dev.index, _stream(dev)))
         return dh, dw, None, None, None, None, None
-
-
-def _kept(kept, n):
-    """Addresses of the statistics, the factor and the named classes' arrays in what a forward pass keeps."""
-    at = kept.data_ptr()
-    return at, at + 16 * n, at + 16 * n + 16
 
 
 _LAYER = (torch.bfloat16, torch.float16)

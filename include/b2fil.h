@@ -392,23 +392,23 @@ typedef struct b2fil_teacher {
 } b2fil_teacher;
 
 /* temperature^2 * KL(teacher || softmax(logits / temperature)) of each row to row_loss (n_rows), what the
- * gradient needs to row_stats (n_rows, 4), 16-byte aligned, and the sum or mean to loss[0] and its
- * factor to factor[0] (not used with B2FIL_REDUCE_NONE).  One entry per row with values = NULL and
+ * gradient needs to row_stats (n_rows, 4), 16-byte aligned, named_p (float) and named_at (int32), (n_rows, k)
+ * each, and the sum or mean to loss[0] and its factor to factor[0] (not used with B2FIL_REDUCE_NONE).  One entry per row with values = NULL and
  * temperature 1 is softmax cross entropy.  The teacher's logsumexp needs n_cols <= 2^20. */
 int64_t b2fil_distill_loss_workspace(int dtype, int64_t n_rows, int64_t n_cols, int k, int device_id);
 int b2fil_distill_loss(int dtype, const void* logits, int64_t n_rows, int64_t n_cols, int64_t row_stride,
                        const b2fil_teacher* teacher, double temperature, int reduction, float* row_loss,
-                       float* row_stats, float* loss, float* factor, void* workspace,
-                       int64_t workspace_bytes, int device_id, void* cuda_stream);
+                       float* row_stats, float* named_p, int32_t* named_at, float* loss, float* factor,
+                       void* workspace, int64_t workspace_bytes, int device_id, void* cuda_stream);
 
 /* The gradient of that loss by the logits to grad (n_rows, n_cols), grad_stride elements between rows.
  * upstream: the gradient by the loss, one value per row upstream_stride apart (0: one value);
  * factor: what b2fil_distill_loss wrote, or NULL for B2FIL_REDUCE_NONE. */
 int b2fil_distill_loss_grad(int dtype, const void* logits, int64_t n_rows, int64_t n_cols,
-                            int64_t row_stride, const b2fil_teacher* teacher, double temperature,
-                            const float* row_stats, const float* upstream, int64_t upstream_stride,
-                            const float* factor, void* grad, int64_t grad_stride, int device_id,
-                            void* cuda_stream);
+                            int64_t row_stride, int k, double temperature, const float* row_stats,
+                            const float* named_p, const int32_t* named_at, const float* upstream,
+                            int64_t upstream_stride, const float* factor, void* grad, int64_t grad_stride,
+                            int device_id, void* cuda_stream);
 
 /* The same loss of logits = hidden * weight^T that are not kept: hidden (n_rows, width), weight (n_cols,
  * width), both B2FIL_TYPE_BF16 or both B2FIL_TYPE_F16, sums in 32 bits.  width is a multiple of 8; rows

@@ -65,18 +65,20 @@ def test_c_refusals_without_a_gpu(lib):
 
     def loss(dtype=2, n=4, c=8, stride=8, k=2, index=64, t=1.0, reduction=2, stats=64, out=64, lse=None):
         teacher = CTeacher(64, index, lse, k, k, -100, k, 0)
-        return lib.b2fil_distill_loss(dtype, 64, n, c, stride, C.byref(teacher), t, reduction, 64, stats, out, 64, None, 0,
-                                      0, None)
+        return lib.b2fil_distill_loss(dtype, 64, n, c, stride, C.byref(teacher), t, reduction, 64, stats, 64, 64, out, 64,
+                                      None, 0, 0, None)
 
     for bad in (dict(dtype=1), dict(n=-1), dict(c=0), dict(stride=3), dict(k=0), dict(k=257), dict(index=None),
                 dict(index=66), dict(t=0.0), dict(t=1e9), dict(reduction=3), dict(stats=72), dict(out=None),
                 dict(c=(1 << 20) + 1, stride=1 << 21, lse=64)):
         assert loss(**bad) == -1, bad
-    assert lib.b2fil_distill_loss(2, 64, 4, 8, 8, None, 1.0, 0, 64, 64, None, None, None, 0, 0, None) == -1
-    teacher = CTeacher(64, 64, None, 2, 2, -100, 2, 0)
-    grad = lambda g, stride: lib.b2fil_distill_loss_grad(2, 64, 4, 8, 8, C.byref(teacher), 1.0, 64, 64, 0, None, g,  # noqa: E731
-                                                         stride, 0, None)
-    assert grad(None, 8) == -1 and grad(65, 8) == -1 and grad(64, 7) == -1
+    assert lib.b2fil_distill_loss(2, 64, 4, 8, 8, None, 1.0, 0, 64, 64, 64, 64, None, None, None, 0, 0, None) == -1
+
+    def grad(g=64, stride=8, k=2, at=64):
+        return lib.b2fil_distill_loss_grad(2, 64, 4, 8, 8, k, 1.0, 64, 64, at, 64, 0, None, g, stride, 0, None)
+
+    for bad in (dict(g=None), dict(g=65), dict(stride=7), dict(k=0), dict(at=None), dict(at=66)):
+        assert grad(**bad) == -1, bad
 
 
 @pytest.mark.skipif(has_gpu(), reason="checks the behaviour on a box without a GPU")
