@@ -38,17 +38,16 @@ int sms_of(int device)
   return n;
 }
 
-// Makes a device current and puts the previous one back.
+// Makes a device current and puts the previous one back.  Also where it is current already: only this call
+// gives a thread that has not used the device yet (autograd's, in a process's first backward pass) the
+// context that encoding a tensor map needs.
 struct OnDevice {
   int prev = -1;
   bool ok  = true;
   explicit OnDevice(int device)
   {
-    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-    if (prev == device)
-      prev = -1;
-    else
-      ok = cudaSetDevice(device) == cudaSuccess;
+    if (cudaGetDevice(&prev) != cudaSuccess || prev == device) prev = -1;
+    ok = cudaSetDevice(device) == cudaSuccess;
   }
   ~OnDevice()
   {

@@ -36,8 +36,9 @@ constexpr int kStage   = 2 * kStageA;      // A and B of one CTA
 constexpr int kThreads = 256;
 constexpr int kSmem    = kStages * kStage + 1024 + 256;
 constexpr long long kPatience = 2000000000ll;  // ns
-constexpr int64_t kPieceBytes = 64ll << 20;    // of d: fits L2 beside what is read
+constexpr int64_t kPieceBytes = 256ll << 20;   // of d (8192 x 2048 x 131,072, gradient: 12.8 ms with 64 MB, 10.7 with 256)
 constexpr int kMostSplits     = 16;
+constexpr int kGroup          = 32;            // tiles of rows whose part of H stays in L2 while all of W passes
 constexpr float kHalfScale    = 16384.f;       // of d in fp16
 // Named classes of a row that the epilogue looks through for each tile; more are put into d by a kernel of their
 // own (4096 x 1024 x 50,001, seven pieces: 32 per row cost 290 us in the epilogue and 28 us in the kernel,
@@ -162,15 +163,19 @@ __device__ __forceinline__ uint32_t instruction(bool bf16, bool a_outer, bool b_
 }
 
 // ---- products --------------------------------------------------------------------------------
-enum Result { kStats, kDiff, kSumHidden, kHidden, kWeight };
+enum Result { kStats, kDiff, kGrad };
 
 // out (m x n) = A (m x depth) B (n x depth)^T.  *_outer: the matrix lies with its depth outermost.
 struct Product {
   CUtensorMap a, b;
   int m, n, depth;
-  int m_tiles, n_tiles, splits;  // splits: parts of the depth, each with a result of its own (kSumHidden)
+  int m_tiles, n_tiles, splits;  // splits: parts of the depth, each with sums of its own
   int a_outer, b_outer;
-  int result;
+  int n_first;  // order of the tiles: all of a row of tiles, else kGroup of a column
+  // kGrad: rows of n elements; 32-bit sums, one matrix per split, to which `add` adds, or 16-bit results
+  float* sums;
+  int add;
+  void* out;    // times `scale`
 };
 // A factor on the device: a b T, or a T.
 struct Scale {
@@ -194,13 +199,8 @@ struct Work {
   float diff_scale;
   Named named;
   int k, first;
-  // kSumHidden: 32-bit sums, one matrix per split; kHidden, kWeight: 16-bit results times `scale`
-  float* sums;
-  int add;
-  void *grad_hidden, *grad_weight;
-  int64_t width;
-  Scale scale;
-  int* ticket;            // kStats: set to 0 for linear_rows
+  Scale scale;            // kGrad
+  int* ticket;            // kStats: set to 0 for linear_rows; kDiff: for the next kernel, which takes its tiles by it
 };
 
 struct Tile {
@@ -212,10 +212,18 @@ __device__ __forceinline__ bool tile_of(const Work& w, int t, Tile& r)
     const Product& p = w.product[i];
     const int tiles  = p.m_tiles * p.n_tiles * p.splits;
     if (t < tiles) {
-      r.which         = i;
-      r.m             = t % p.m_tiles;
-      r.n             = t / p.m_tiles % p.n_tiles;
-      r.split         = t / (p.m_tiles * p.n_tiles);
+      r.which = i;
+      r.split = t / (p.m_tiles * p.n_tiles);
+      t %= p.m_tiles * p.n_tiles;
+      if (p.n_first) {
+        r.m = t / p.n_tiles;
+        r.n = t % p.n_tiles;
+      } else {
+        const int first = t / (kGroup * p.n_tiles) * kGroup, rows = min(kGroup, p.m_tiles - first);
+        t -= first * p.n_tiles;
+        r.m = first + t % rows;
+        r.n = t / rows;
+      }
       const int steps = (p.depth + kDepth - 1) / kDepth;
       r.begin         = static_cast<int>(static_cast<int64_t>(steps) * r.split / p.splits);
       r.end           = static_cast<int>(static_cast<int64_t>(steps) * (r.split + 1) / p.splits);
@@ -280,13 +288,13 @@ __device__ __forceinline__ void take_columns(const Work& w, const Product& p, in
     }
     return;
   }
-  if (p.result == kSumHidden) {
-    float* to = w.sums + (split * static_cast<int64_t>(p.m) + row) * w.width + col;
+  if (p.sums) {
+    float* to = p.sums + (split * static_cast<int64_t>(p.m) + row) * p.n + col;
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
       if (col + i >= p.n) break;
       float4 v = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-      if (w.add) {
+      if (p.add) {
         const float4 o = *reinterpret_cast<const float4*>(to + i);
         v              = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
       }
@@ -294,7 +302,7 @@ __device__ __forceinline__ void take_columns(const Work& w, const Product& p, in
     }
     return;
   }
-  char* to = static_cast<char*>(p.result == kWeight ? w.grad_weight : w.grad_hidden) + (row * w.width + col) * 2;
+  char* to = static_cast<char*>(p.out) + (row * p.n + col) * 2;
 #pragma unroll
   for (int i = 0; i < 32; i += 8) {
     if (col + i >= p.n) break;
@@ -307,21 +315,23 @@ __device__ __forceinline__ void take_columns(const Work& w, const Product& p, in
   }
 }
 
-// KIND: kStats, kDiff, or kWeight for the products of the gradients.
 template <int KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) products(const __grid_constant__ Work w)
 {
   extern __shared__ char raw[];
-  __shared__ __align__(8) uint64_t bars[2 * kStages + 5];
+  constexpr bool kByTicket = KIND == kGrad;
+  constexpr int kReaders   = 11;  // of a ticket: 2 producers, the issuer, 8 warps of the two epilogues
+  __shared__ __align__(8) uint64_t bars[2 * kStages + 9];
+  __shared__ volatile int tickets[2];
   __shared__ uint32_t tmem_at;
   __shared__ volatile int gave_up;
   const uint32_t ring = (shared_of(raw) + 1023) & ~1023u;
   const uint32_t full = shared_of(bars), empty = full + 8 * kStages, done = empty + 8 * kStages, freed = done + 16,
-                 last = freed + 16;
+                 last = freed + 16, told = last + 8, heard = told + 16;
   const uint32_t rank = rank_in_cluster();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int cluster = blockIdx.x / 2, clusters = gridDim.x / 2;
-  if (KIND == kStats && blockIdx.x == 0 && threadIdx.x == 0) *w.ticket = 0;
+  if (!kByTicket && blockIdx.x == 0 && threadIdx.x == 0) *w.ticket = 0;
   if (threadIdx.x == 0) {
     gave_up = 0;
     for (int i = 0; i < kStages; ++i) {
@@ -331,6 +341,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
     for (int i = 0; i < 2; ++i) {
       bar_init(done + 8 * i, 1);
       bar_init(freed + 8 * i, 8);  // the four warps of both CTAs
+      bar_init(told + 8 * i, 1);
+      bar_init(heard + 8 * i, kReaders);
     }
     bar_init(last, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -345,6 +357,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_at;
 
+  // The tile after tile i: the next in turn, or what the first CTA's fourth warp has drawn for the cluster.
+  int drawn       = 0;
+  auto next_tile = [&](int& i, bool whole_warp) {
+    if (!kByTicket) {
+      i += clusters;
+      return true;
+    }
+    const int slot = drawn & 1;
+    bool ok        = bar_wait(told + 8 * slot, drawn >> 1 & 1, &gave_up);
+    if (whole_warp) ok = __all_sync(~0u, ok);
+    if (!ok) return false;
+    i = tickets[slot];
+    if (whole_warp) __syncwarp();
+    if (!whole_warp || lane == 0) bar_arrive_cluster(in_cta(heard + 8 * slot, 0));
+    ++drawn;
+    return true;
+  };
+
   if (warp == 0 && lane == 0) {
     // tiles to the ring; the bytes of both CTAs are counted at the first one's barrier
     const uint32_t count_at = in_cta(full, 0);
@@ -352,7 +382,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
     bool ok = true;
     int issued = 0;
     Tile t;
-    for (int i = cluster; ok && tile_of(w, i, t); i += clusters) {
+    for (int i = cluster; ok && tile_of(w, i, t); ok = ok && next_tile(i, false)) {
       const Product& p = w.product[t.which];
       const int m0 = t.m * kTile + rank * kHalf, n0 = t.n * kTile + rank * kHalf;
       for (int k = t.begin; k < t.end; ++k) {
@@ -393,7 +423,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
     int stage = 0, phase = 0, half = 0, turn = 0;
     bool ok = true;
     Tile t;
-    for (int i = cluster; ok && tile_of(w, i, t); i += clusters) {
+    for (int i = cluster; ok && tile_of(w, i, t); ok = ok && next_tile(i, false)) {
       const Product& p     = w.product[t.which];
       const uint32_t idesc = instruction(w.bf16, p.a_outer, p.b_outer);
       const uint64_t step_a = (p.a_outer ? 2048 : 32) >> 4, step_b = (p.b_outer ? 2048 : 32) >> 4;
@@ -429,12 +459,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
       const long long until = now_ns() + kPatience;
       while (!bar_try(last, 0) && now_ns() < until) {}
     }
+  } else if (kByTicket && warp == 3 && lane == 0 && rank == 0) {
+    // draws tiles, one ahead, and tells both CTAs
+    Tile t;
+    int i = 0;
+    for (int n = 0; tile_of(w, i, t); ++n) {
+      const int slot = n & 1;
+      if (!bar_wait(heard + 8 * slot, (n >> 1 & 1) ^ 1, &gave_up)) break;
+      i = clusters + atomicAdd(w.ticket, 1);
+      for (int cta = 0; cta < 2; ++cta) {
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(in_cta(shared_of(const_cast<int*>(tickets) + slot), cta)), "r"(i) : "memory");
+        bar_arrive_cluster(in_cta(told + 8 * slot, cta));
+      }
+    }
   } else if (warp >= 4) {
     const int quarter     = warp - 4;
     const uint32_t freed0 = in_cta(freed, 0);
     int half = 0, turn = 0;
     Tile t;
-    for (int i = cluster; tile_of(w, i, t); i += clusters) {
+    bool ok = true;
+    for (int i = cluster; ok && tile_of(w, i, t); ok = next_tile(i, true)) {
       const Product& p  = w.product[t.which];
       const int64_t row = static_cast<int64_t>(t.m) * kTile + rank * kHalf + quarter * 32 + lane;
       const bool in     = row < p.m;
@@ -444,7 +488,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
         base           = base_of(s.x);
         factor         = s.w == 0.f ? 0.f : s.y * w.diff_scale * (w.row_scale ? w.row_scale[row] : 1.f);
       }
-      if (KIND == kWeight && p.result != kSumHidden) factor = w.scale();
+      if (KIND == kGrad && !p.sums) factor = w.scale();
       if (!__all_sync(~0u, bar_wait(done + 8 * half, turn, &gave_up))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       Running<float> r;
@@ -619,9 +663,9 @@ __global__ void __launch_bounds__(kThreads) named_diff(Work w, int64_t entries, 
   }
 }
 
-// dH from the sums of its parts.
+// A gradient from the sums of its parts.
 template <class T>
-__global__ void __launch_bounds__(kThreads) finish_hidden(const float* sums, int splits, int64_t n, Scale scale, T* out)
+__global__ void __launch_bounds__(kThreads) finish_sums(const float* sums, int splits, int64_t n, Scale scale, T* out)
 {
   const float f = scale();
   for (int64_t i = 4 * (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x); i < n; i += 4 * gridDim.x * static_cast<int64_t>(kThreads)) {
@@ -689,7 +733,7 @@ cudaError_t run_products(const Work& w, int n_sms, cudaStream_t s)
 }
 
 // z = H W^T of the classes from `first` on
-bool logits_product(Product& p, bool bf16, const LinearArgs& a, int64_t first, int64_t n, int result)
+bool logits_product(Product& p, bool bf16, const LinearArgs& a, int64_t first, int64_t n)
 {
   p.m       = static_cast<int>(a.n_rows);
   p.n       = static_cast<int>(n);
@@ -698,7 +742,7 @@ bool logits_product(Product& p, bool bf16, const LinearArgs& a, int64_t first, i
   p.n_tiles = tiles_of(p.n);
   p.splits  = 1;
   p.a_outer = p.b_outer = 0;
-  p.result  = result;
+  p.n_first = 0;
   return make_map(&p.a, bf16, a.hidden, a.n_rows, a.width, a.hidden_stride, kHalf) &&
          make_map(&p.b, bf16, static_cast<const char*>(a.weight) + first * a.weight_stride * 2, n, a.width, a.weight_stride, kHalf);
 }
@@ -718,7 +762,7 @@ cudaError_t run_linear(bool bf16, const LinearArgs& a, const Reduced& out, void*
   w.c        = 1.4426950408889634f / a.temperature;
   w.ticket   = reinterpret_cast<int*>(sums + 8 * n_sms);
   w.parts    = reinterpret_cast<float2*>(sums + 8 * n_sms + 1);
-  if (!logits_product(w.product[0], bf16, a, 0, a.n_cols, kStats)) return cudaErrorInvalidValue;
+  if (!logits_product(w.product[0], bf16, a, 0, a.n_cols)) return cudaErrorInvalidValue;
   cudaError_t e = run_products<kStats>(w, n_sms, s);
   if (e != cudaSuccess) return e;
   // a warp per row where there are enough rows (or nothing to share), else a block
@@ -735,12 +779,12 @@ cudaError_t run_linear(bool bf16, const LinearArgs& a, const Reduced& out, void*
   return cudaGetLastError();
 }
 
-// How the classes are cut into pieces and the sums over them split.
+// How the classes are cut into pieces and the sums over classes and rows into parts.
 struct Plan {
   int pieces;
-  int64_t cols;  // of a piece, a multiple of a tile
-  int splits;    // of dH's sum over a piece's classes
-  bool direct;   // dH needs no sums in memory
+  int64_t cols;                 // of a piece, a multiple of a tile
+  int splits_hidden, splits_weight;
+  bool sums_hidden, sums_weight;  // in memory
 };
 Plan plan_of(const LinearGradArgs& g, int n_sms)
 {
@@ -751,18 +795,31 @@ Plan plan_of(const LinearGradArgs& g, int n_sms)
   p.pieces = static_cast<int>((a.n_cols + most - 1) / most);
   p.cols   = static_cast<int64_t>(tiles_of((a.n_cols + p.pieces - 1) / p.pieces)) * kTile;
   p.pieces = static_cast<int>((a.n_cols + p.cols - 1) / p.cols);
-  // as many parts as bring a part of dH down to an even share of the machine, 16 stages at least
-  const int64_t wide = tiles_of(a.width), dh_tiles = tiles_of(a.n_rows) * wide, dh_steps = p.cols / kDepth;
-  int64_t all = dh_tiles * dh_steps;
-  if (g.grad_weight) all += tiles_of(p.cols) * wide * ((a.n_rows + kDepth - 1) / kDepth);
-  int64_t share = all / (n_sms / 2);
+  // as many parts as bring a part down to an even share of the machine, 16 stages at least
+  const int64_t wide = tiles_of(a.width), dh_tiles = tiles_of(a.n_rows) * wide, dw_tiles = tiles_of(p.cols) * wide;
+  const int64_t dh_steps = p.cols / kDepth, dw_steps = (a.n_rows + kDepth - 1) / kDepth;
+  int64_t share = ((g.grad_hidden ? dh_tiles * dh_steps : 0) + (g.grad_weight ? dw_tiles * dw_steps : 0)) / (n_sms / 2);
   if (share < 16) share = 16;
-  const int64_t splits = (dh_steps + share - 1) / share;
-  p.splits             = static_cast<int>(splits < 1 ? 1 : splits > kMostSplits ? kMostSplits : splits);
-  p.direct             = p.pieces == 1 && p.splits == 1;
+  auto parts = [&](int64_t steps) {
+    const int64_t n = (steps + share - 1) / share;
+    return static_cast<int>(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
+  };
+  p.splits_hidden = parts(dh_steps);
+  p.splits_weight = parts(dw_steps);
+  p.sums_hidden   = g.grad_hidden && (p.pieces > 1 || p.splits_hidden > 1);
+  p.sums_weight   = g.grad_weight && p.splits_weight > 1;
   return p;
 }
 int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+template <class T>
+cudaError_t finish(const float* sums, int splits, int64_t n, const Scale& scale, void* out, int n_sms, cudaStream_t s)
+{
+  const int64_t need = (n / 4 + kThreads - 1) / kThreads;
+  finish_sums<T><<<static_cast<unsigned>(need < 8 * n_sms ? need : 8 * n_sms), kThreads, 0, s>>>(sums, splits, n, scale,
+                                                                                              static_cast<T*>(out));
+  return cudaGetLastError();
+}
 
 template <class T>
 cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace, int n_sms, cudaStream_t s)
@@ -771,9 +828,11 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
   const Plan plan      = plan_of(g, n_sms);
   char* at             = static_cast<char*>(workspace);
   float* scale         = reinterpret_cast<float*>(at);
+  int* ticket          = reinterpret_cast<int*>(at + 16);
   float* row_scale     = reinterpret_cast<float*>(at += 256);
   T* diff              = reinterpret_cast<T*>(at += padded(a.n_rows * 4));
-  float* sums          = reinterpret_cast<float*>(at += padded(a.n_rows * plan.cols * 2));
+  float* sums_hidden   = reinterpret_cast<float*>(at += padded(a.n_rows * plan.cols * 2));
+  float* sums_weight   = reinterpret_cast<float*>(at + (plan.sums_hidden ? plan.splits_hidden * a.n_rows * a.width * 4 : 0));
   const float d_scale  = bf16 ? 1.f : kHalfScale;
   const bool per_row   = g.factor == nullptr;
   int launched         = per_row;
@@ -787,17 +846,15 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
   w.diff        = diff;
   w.diff_stride = plan.cols;
   w.diff_scale  = d_scale;
-  w.sums        = sums;
-  w.grad_hidden = g.grad_hidden;
-  w.width       = a.width;
   w.scale       = Scale{per_row ? scale : g.upstream, g.factor, a.temperature / d_scale};
   w.named       = a.named;
   w.k           = a.teacher.k;
+  w.ticket      = ticket;
   for (int i = 0; i < plan.pieces; ++i) {
     const int64_t first = i * plan.cols, n = a.n_cols - first < plan.cols ? a.n_cols - first : plan.cols;
     w.products = 1;
     w.first    = static_cast<int>(first);
-    if (!logits_product(w.product[0], bf16, a, first, n, kDiff)) return cudaErrorInvalidValue;
+    if (!logits_product(w.product[0], bf16, a, first, n)) return cudaErrorInvalidValue;
     if ((e = run_products<kDiff>(w, n_sms, s)) != cudaSuccess) return e;
     if (w.k > kFewNamed) {
       const int64_t entries = a.n_rows * w.k, need = (entries + kThreads - 1) / kThreads;
@@ -806,50 +863,59 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
     }
     // d ends with the tile that holds its last class: what is behind has not been written
     const int64_t made = static_cast<int64_t>(tiles_of(n)) * kTile;
-    w.products         = 0;
     const char* weight = static_cast<const char*>(a.weight) + first * a.weight_stride * 2;
-    if (g.grad_weight) {
-      Product& p = w.product[w.products++];
-      p.m        = static_cast<int>(n);
-      p.n        = static_cast<int>(a.width);
-      p.depth    = static_cast<int>(a.n_rows);
-      p.splits   = 1;
-      p.a_outer = p.b_outer = 1;
-      p.result  = kWeight;
-      if (!make_map(&p.a, bf16, diff, a.n_rows, made, plan.cols, 64) ||
-          !make_map(&p.b, bf16, a.hidden, a.n_rows, a.width, a.hidden_stride, 64))
-        return cudaErrorInvalidValue;
-    }
-    if (g.grad_hidden) {
+    T* grad_weight     = g.grad_weight ? static_cast<T*>(g.grad_weight) + first * a.width : nullptr;
+    w.products         = 0;
+    auto hidden = [&] {
+      if (!g.grad_hidden) return true;
       Product& p = w.product[w.products++];
       p.m        = static_cast<int>(a.n_rows);
-      p.n        = static_cast<int>(a.width);
       p.depth    = static_cast<int>(made);
-      p.splits   = plan.splits;
+      p.splits   = plan.splits_hidden;
       p.a_outer  = 0;
-      p.b_outer  = 1;
-      p.result   = plan.direct ? kHidden : kSumHidden;
-      if (!make_map(&p.a, bf16, diff, a.n_rows, made, plan.cols, kHalf) ||
-          !make_map(&p.b, bf16, weight, n, a.width, a.weight_stride, 64))
-        return cudaErrorInvalidValue;
-    }
+      p.sums     = plan.sums_hidden ? sums_hidden : nullptr;
+      p.add      = i > 0;
+      p.out      = g.grad_hidden;
+      return make_map(&p.a, bf16, diff, a.n_rows, made, plan.cols, kHalf) &&
+             make_map(&p.b, bf16, weight, n, a.width, a.weight_stride, 64);
+    };
+    auto of_weight = [&] {
+      if (!g.grad_weight) return true;
+      Product& p = w.product[w.products++];
+      p.m        = static_cast<int>(n);
+      p.depth    = static_cast<int>(a.n_rows);
+      p.splits   = plan.splits_weight;
+      p.a_outer  = 1;
+      p.sums     = plan.sums_weight ? sums_weight : nullptr;
+      p.add      = 0;
+      p.out      = grad_weight;
+      return make_map(&p.a, bf16, diff, a.n_rows, made, plan.cols, 64) &&
+             make_map(&p.b, bf16, a.hidden, a.n_rows, a.width, a.hidden_stride, 64);
+    };
+    // the longer sums first: what is left at the end is short
+    const bool hidden_first = made / plan.splits_hidden >= a.n_rows / plan.splits_weight;
+    if (!(hidden_first ? hidden() && of_weight() : of_weight() && hidden())) return cudaErrorInvalidValue;
     for (int j = 0; j < w.products; ++j) {
-      w.product[j].m_tiles = tiles_of(w.product[j].m);
-      w.product[j].n_tiles = tiles_of(w.product[j].n);
+      Product& p = w.product[j];
+      p.n        = static_cast<int>(a.width);
+      p.b_outer  = 1;
+      p.m_tiles  = tiles_of(p.m);
+      p.n_tiles  = tiles_of(p.n);
+      p.n_first  = 1;  // d is read once, by all the tiles of a row of them at the same time
     }
-    w.add         = i > 0;
-    w.grad_weight = g.grad_weight ? static_cast<T*>(g.grad_weight) + first * a.width : nullptr;
-    if (w.products && (e = run_products<kWeight>(w, n_sms, s)) != cudaSuccess) return e;
+    if ((e = run_products<kGrad>(w, n_sms, s)) != cudaSuccess) return e;
     launched += 2;
+    if (plan.sums_weight) {
+      if ((e = finish<T>(sums_weight, plan.splits_weight, n * a.width, w.scale, grad_weight, n_sms, s)) != cudaSuccess) return e;
+      ++launched;
+    }
   }
-  if (g.grad_hidden && !plan.direct) {
-    const int64_t n = a.n_rows * a.width, need = (n / 4 + kThreads - 1) / kThreads;
-    finish_hidden<T><<<static_cast<unsigned>(need < 8 * n_sms ? need : 8 * n_sms), kThreads, 0, s>>>(
-      sums, plan.splits, n, w.scale, static_cast<T*>(g.grad_hidden));
+  if (plan.sums_hidden) {
+    e = finish<T>(sums_hidden, plan.splits_hidden, a.n_rows * a.width, w.scale, g.grad_hidden, n_sms, s);
     ++launched;
   }
   count_launches(launched);
-  return cudaGetLastError();
+  return e;
 }
 
 }  // namespace
@@ -864,7 +930,8 @@ size_t linear_grad_workspace(const LinearGradArgs& g, int n_sms)
   const LinearArgs& a = g.fwd;
   const Plan p        = plan_of(g, n_sms);
   return 256 + padded(a.n_rows * 4) + padded(a.n_rows * p.cols * 2) +
-         (g.grad_hidden && !p.direct ? p.splits * a.n_rows * a.width * sizeof(float) : 0);
+         (p.sums_hidden ? p.splits_hidden * a.n_rows * a.width * sizeof(float) : 0) +
+         (p.sums_weight ? p.splits_weight * p.cols * a.width * sizeof(float) : 0);
 }
 
 cudaError_t launch_linear(int dtype, const LinearArgs& a, const Reduced& out, void* workspace, int n_sms, cudaStream_t s)

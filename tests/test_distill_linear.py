@@ -77,9 +77,11 @@ def entries(n, c, k, seed=0, index64=False):
     return v, i if index64 else i.int()
 
 
-# rows, width, classes: one tile and less, its borders, several tiles, several splits of the sum over classes, odd widths
+# rows, width, classes: one tile and less, its borders, several tiles, sums over classes and over rows in several
+# parts, odd widths
 SIZES = [(1, 8, 1), (1, 64, 2), (3, 16, 7), (128, 64, 256), (129, 72, 257), (256, 256, 256), (257, 264, 300),
-         (64, 128, 1000), (200, 520, 1003), (513, 200, 2050), (40, 96, 20_011), (300, 33, 130), (70, 1001, 515)]
+         (64, 128, 1000), (200, 520, 1003), (513, 200, 2050), (40, 96, 20_011), (300, 33, 130), (70, 1001, 515),
+         (5000, 64, 40), (9000, 264, 513)]
 
 
 @gpu
@@ -122,10 +124,11 @@ def test_linear_cross_entropy(n, width, c, dtype):
 
 
 @gpu
-def test_several_pieces_of_the_classes():
-    """(17,000 x 6,000 differences are more than one piece holds; few enough for the CPU to check.)"""
-    h, w = layer(17_000, 16, 6000, "bf16")
-    v, i = entries(17_000, 6000, 3)
+@pytest.mark.parametrize("k", [2, 5])
+def test_several_pieces_of_the_classes(k):
+    """(20,000 x 7,000 differences are more than one piece holds; few enough for the CPU to check.)"""
+    h, w = layer(20_000, 16, 7000, "bf16")
+    v, i = entries(20_000, 7000, k)
     check(h, w, v, i, 1.0, "mean")
 
 
@@ -225,3 +228,27 @@ def test_a_wait_that_runs_out_is_reported_once():
         distill.check_status()
     assert e.value.code == -7
     distill.check_status()
+
+
+_FIRST_BACKWARD = """
+import torch
+from cuml_b200 import distill
+h = torch.ones(256, 128, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+w = torch.ones(1000, 128, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+loss = distill.linear_cross_entropy(h, w, torch.zeros(256, dtype=torch.int64, device="cuda"))
+torch.autograd.grad(loss, (h, w))
+distill.check_status()
+print("first", loss.item())
+"""
+
+
+@gpu
+def test_the_first_thing_that_autograds_thread_does():
+    """The thread of a process's first backward pass has no CUDA context yet."""
+    import subprocess
+    import sys
+
+    from tests.conftest import ROOT
+
+    r = subprocess.run([sys.executable, "-c", _FIRST_BACKWARD], cwd=ROOT, capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout.startswith("first 6.9"), r.stderr[-800:]
