@@ -85,6 +85,14 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity)
     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok;
 }
+// One lane of a converged warp: what it alone executes stays free of per-lane loops around instructions that
+// take uniform registers (a TMA load issued by `lane == 0` takes 260 cycles, by the elected lane a tenth).
+__device__ __forceinline__ bool elected()
+{
+  uint32_t yes;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(yes));
+  return yes;
+}
 __device__ __forceinline__ long long now_ns()
 {
   long long t;
@@ -108,6 +116,10 @@ __device__ __noinline__ bool bar_wait_long(uint32_t bar, uint32_t parity, volati
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up)
 {
   return bar_try(bar, parity) || bar_wait_long(bar, parity, gave_up, kPatience);
+}
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* gave_up)
+{
+  return __all_sync(~0u, bar_wait(bar, parity, gave_up));
 }
 // 2-dimensional box to this CTA's shared memory; the bytes are counted at `bar`, which may be the other CTA's
 __device__ __forceinline__ void load_box(uint32_t to, const CUtensorMap* map, uint32_t bar, int x, int y)
@@ -329,7 +341,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
   const uint32_t full = shared_of(bars), empty = full + 8 * kStages, done = empty + 8 * kStages, freed = done + 16,
                  last = freed + 16, told = last + 8, heard = told + 16;
   const uint32_t rank = rank_in_cluster();
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const int cluster = blockIdx.x / 2, clusters = gridDim.x / 2;
   if (!kByTicket && blockIdx.x == 0 && threadIdx.x == 0) *w.ticket = 0;
   if (threadIdx.x == 0) {
@@ -359,51 +371,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
 
   // The tile after tile i: the next in turn, or what the first CTA's fourth warp has drawn for the cluster.
   int drawn       = 0;
-  auto next_tile = [&](int& i, bool whole_warp) {
+  auto next_tile = [&](int& i) {
     if (!kByTicket) {
       i += clusters;
       return true;
     }
     const int slot = drawn & 1;
-    bool ok        = bar_wait(told + 8 * slot, drawn >> 1 & 1, &gave_up);
-    if (whole_warp) ok = __all_sync(~0u, ok);
-    if (!ok) return false;
-    i = tickets[slot];
-    if (whole_warp) __syncwarp();
-    if (!whole_warp || lane == 0) bar_arrive_cluster(in_cta(heard + 8 * slot, 0));
+    if (!warp_wait(told + 8 * slot, drawn >> 1 & 1, &gave_up)) return false;
+    i = __shfl_sync(~0u, tickets[slot], 0);
+    if (elected()) bar_arrive_cluster(in_cta(heard + 8 * slot, 0));
     ++drawn;
     return true;
   };
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     // tiles to the ring; the bytes of both CTAs are counted at the first one's barrier
     const uint32_t count_at = in_cta(full, 0);
-    int stage = 0, phase = 0;
+    int stage = 0, phase = 0, issued = 0;
     bool ok = true;
-    int issued = 0;
     Tile t;
-    for (int i = cluster; ok && tile_of(w, i, t); ok = ok && next_tile(i, false)) {
+    for (int i = cluster; ok && tile_of(w, i, t); ok = ok && next_tile(i)) {
       const Product& p = w.product[t.which];
       const int m0 = t.m * kTile + rank * kHalf, n0 = t.n * kTile + rank * kHalf;
       for (int k = t.begin; k < t.end; ++k) {
-        if (!bar_wait(empty + 8 * stage, phase ^ 1, &gave_up)) {
+        if (!warp_wait(empty + 8 * stage, phase ^ 1, &gave_up)) {
           ok = false;
           break;
         }
-        if (rank == 0) bar_expect(full + 8 * stage, 2 * kStage);
         const uint32_t a = ring + stage * kStage, b = a + kStageA, bar = count_at + 8 * stage;
-        if (p.a_outer) {
-          load_box(a, &p.a, bar, m0, k * kDepth);
-          load_box(a + 8192, &p.a, bar, m0 + 64, k * kDepth);
-        } else {
-          load_box(a, &p.a, bar, k * kDepth, m0);
+        if (elected()) {
+          if (rank == 0) bar_expect(full + 8 * stage, 2 * kStage);
+          if (p.a_outer) {
+            load_box(a, &p.a, bar, m0, k * kDepth);
+            load_box(a + 8192, &p.a, bar, m0 + 64, k * kDepth);
+          } else {
+            load_box(a, &p.a, bar, k * kDepth, m0);
+          }
+          if (p.b_outer) {
+            load_box(b, &p.b, bar, n0, k * kDepth);
+            load_box(b + 8192, &p.b, bar, n0 + 64, k * kDepth);
+          } else {
+            load_box(b, &p.b, bar, k * kDepth, n0);
+          }
         }
-        if (p.b_outer) {
-          load_box(b, &p.b, bar, n0, k * kDepth);
-          load_box(b + 8192, &p.b, bar, n0 + 64, k * kDepth);
-        } else {
-          load_box(b, &p.b, bar, k * kDepth, n0);
-        }
+        __syncwarp();
         ++issued;
         if (++stage == kStages) {
           stage = 0;
@@ -414,48 +425,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
     if (!ok && rank == 0) {
       // copies in flight have to land before the CTA ends: the last phase of every stage that was filled
       for (int i = 0; i < kStages && i < issued; ++i) {
-        const int n     = issued - 1 - i;
+        const int n           = issued - 1 - i;
         const long long until = now_ns() + kPatience;
         while (!bar_try(full + 8 * (n % kStages), (n / kStages) & 1) && now_ns() < until) {}
       }
     }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+  } else if (warp == 1 && rank == 0) {
     int stage = 0, phase = 0, half = 0, turn = 0;
     bool ok = true;
     Tile t;
-    for (int i = cluster; ok && tile_of(w, i, t); ok = ok && next_tile(i, false)) {
-      const Product& p     = w.product[t.which];
-      const uint32_t idesc = instruction(w.bf16, p.a_outer, p.b_outer);
+    for (int i = cluster; ok && tile_of(w, i, t); ok = ok && next_tile(i)) {
+      const Product& p      = w.product[t.which];
+      const uint32_t idesc  = instruction(w.bf16, p.a_outer, p.b_outer);
       const uint64_t step_a = (p.a_outer ? 2048 : 32) >> 4, step_b = (p.b_outer ? 2048 : 32) >> 4;
-      if (!bar_wait(freed + 8 * half, turn ^ 1, &gave_up)) {
+      const uint64_t a0     = descriptor(ring, p.a_outer), b0 = descriptor(ring + kStageA, p.b_outer);
+      if (!warp_wait(freed + 8 * half, turn ^ 1, &gave_up)) {
         ok = false;
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       for (int k = t.begin; k < t.end; ++k) {
-        if (!bar_wait(full + 8 * stage, phase, &gave_up)) {
+        if (!warp_wait(full + 8 * stage, phase, &gave_up)) {
           ok = false;
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t a = descriptor(ring + stage * kStage, p.a_outer);
-        const uint64_t b = descriptor(ring + stage * kStage + kStageA, p.b_outer);
+        const uint64_t a = a0 + stage * (kStage >> 4), b = b0 + stage * (kStage >> 4);
+        if (elected()) {
 #pragma unroll
-        for (int j = 0; j < kDepth / 16; ++j)
-          mma(tmem + half * kTile, a + j * step_a, b + j * step_b, idesc, k > t.begin || j > 0);
-        commit(empty + 8 * stage);
+          for (int j = 0; j < kDepth / 16; ++j)
+            mma(tmem + half * kTile, a + j * step_a, b + j * step_b, idesc, k > t.begin || j > 0);
+          commit(empty + 8 * stage);
+          if (k + 1 == t.end) commit(done + 8 * half);
+        }
+        __syncwarp();
         if (++stage == kStages) {
           stage = 0;
           phase ^= 1;
         }
       }
       if (!ok) break;
-      commit(done + 8 * half);
       half ^= 1;
       turn ^= half == 0;
     }
     if (!ok) {  // products in flight have to end before TMEM is given back
-      commit(last);
+      if (elected()) commit(last);
       const long long until = now_ns() + kPatience;
       while (!bar_try(last, 0) && now_ns() < until) {}
     }
@@ -478,7 +492,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
     int half = 0, turn = 0;
     Tile t;
     bool ok = true;
-    for (int i = cluster; ok && tile_of(w, i, t); ok = next_tile(i, true)) {
+    for (int i = cluster; ok && tile_of(w, i, t); ok = next_tile(i)) {
       const Product& p  = w.product[t.which];
       const int64_t row = static_cast<int64_t>(t.m) * kTile + rank * kHalf + quarter * 32 + lane;
       const bool in     = row < p.m;
@@ -489,7 +503,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
         factor         = s.w == 0.f ? 0.f : s.y * w.diff_scale * (w.row_scale ? w.row_scale[row] : 1.f);
       }
       if (KIND == kGrad && !p.sums) factor = w.scale();
-      if (!__all_sync(~0u, bar_wait(done + 8 * half, turn, &gave_up))) break;
+      if (!warp_wait(done + 8 * half, turn, &gave_up)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       Running<float> r;
 #pragma unroll 1
