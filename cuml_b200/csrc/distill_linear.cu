@@ -16,8 +16,8 @@
 // One kernel does all products: a cluster of two CTAs takes 256 x 256 of the output
 // (tcgen05.mma.cta_group::2; each CTA holds 128 rows of A, half of B and 128 rows of the result), since
 // one CTA alone with 128 x 256 would have to read 96 bytes per cycle from L2 where 64 pass.  Warp 0 brings the
-// tiles (TMA, 128-byte swizzle, ring of 6 x 32 KB), warp 1 of the first CTA issues the products, warps 4 to
-// 7 work on the finished tile while the next one is summed in the other half of TMEM.  All waits are
+// tiles (TMA, 128-byte swizzle, ring of 6 x 32 KB), warp 1 of the first CTA issues the products, the others
+// work on the finished tile while the next one is summed in the other half of TMEM.  All waits are
 // bounded: after two seconds a role gives up, sets the status word and leaves by the common exit.
 #include <cuda.h>
 
@@ -34,6 +34,8 @@ constexpr int kStages  = 6;
 constexpr int kStageA  = kHalf * kDepth * 2;
 constexpr int kStage   = 2 * kStageA;      // A and B of one CTA
 constexpr int kThreads = 256;
+constexpr int kEpilogue = 8;               // warps that work on finished tiles: a quarter of the rows and half of the columns each
+constexpr int kProductThreads = (4 + kEpilogue) * 32;
 constexpr int kSmem    = kStages * kStage + 1024 + 256;
 constexpr long long kPatience = 2000000000ll;  // ns
 constexpr int64_t kPieceBytes = 256ll << 20;   // of d (8192 x 2048 x 131,072, gradient: 12.8 ms with 64 MB, 10.7 with 256)
@@ -199,7 +201,7 @@ struct Work {
   Product product[2];
   int products;
   int bf16;
-  // kStats: (row, tile of columns) -> maximum and sum
+  // kStats: (row, half a tile of columns) -> maximum and sum
   float2* parts;
   // kStats, kDiff
   float c;                // log2(e) / T
@@ -328,11 +330,11 @@ __device__ __forceinline__ void take_columns(const Work& w, const Product& p, in
 }
 
 template <int KIND>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) products(const __grid_constant__ Work w)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) products(const __grid_constant__ Work w)
 {
   extern __shared__ char raw[];
   constexpr bool kByTicket = KIND == kGrad;
-  constexpr int kReaders   = 11;  // of a ticket: 2 producers, the issuer, 8 warps of the two epilogues
+  constexpr int kReaders   = 3 + 2 * kEpilogue;  // of a ticket: two producers, the issuer, both CTAs' epilogues
   __shared__ __align__(8) uint64_t bars[2 * kStages + 9];
   __shared__ volatile int tickets[2];
   __shared__ uint32_t tmem_at;
@@ -352,7 +354,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
     }
     for (int i = 0; i < 2; ++i) {
       bar_init(done + 8 * i, 1);
-      bar_init(freed + 8 * i, 8);  // the four warps of both CTAs
+      bar_init(freed + 8 * i, 2 * kEpilogue);
       bar_init(told + 8 * i, 1);
       bar_init(heard + 8 * i, kReaders);
     }
@@ -487,7 +489,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
       }
     }
   } else if (warp >= 4) {
-    const int quarter     = warp - 4;
+    const int quarter = warp % 4, from = (warp - 4) / 4 * (kTile / 2);
     const uint32_t freed0 = in_cta(freed, 0);
     int half = 0, turn = 0;
     Tile t;
@@ -507,7 +509,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       Running<float> r;
 #pragma unroll 1
-      for (int c = 0; c < kTile; c += 32) {
+      for (int c = from; c < from + kTile / 2; c += 32) {
         const int col = t.n * kTile + c;
         if (KIND != kDiff && col >= p.n) break;
         float x[32];
@@ -520,7 +522,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
       if (lane == 0) bar_arrive_cluster(freed0 + 8 * half);
       if (KIND == kDiff && in && factor != 0.f && w.k <= kFewNamed) {  // over what has just been written
         const float per = w.diff_scale * (w.row_scale ? w.row_scale[row] : 1.f), inv = w.stats[row].y;
-        const int low = t.n * kTile, high = min(low + kTile, p.n);
+        const int low = t.n * kTile + from, high = min(low + kTile / 2, p.n);
         for (int j = 0; j < w.k; ++j) {
           const int64_t e = row * w.k + j;
           const int at    = w.named.at[e] - w.first;
@@ -530,7 +532,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
           *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(two(d, 0.f, w.bf16));
         }
       }
-      if (KIND == kStats && in) w.parts[row * p.n_tiles + t.n] = make_float2(r.m, r.s);
+      if (KIND == kStats && in) w.parts[(row * p.n_tiles + t.n) * 2 + (from != 0)] = make_float2(r.m, r.s);
       half ^= 1;
       turn ^= half == 0;
     }
@@ -742,7 +744,7 @@ cudaError_t run_products(const Work& w, int n_sms, cudaStream_t s)
   int tiles = 0;
   for (int i = 0; i < w.products; ++i) tiles += w.product[i].m_tiles * w.product[i].n_tiles * w.product[i].splits;
   const int clusters = tiles < n_sms / 2 ? tiles : n_sms / 2;
-  products<KIND><<<2 * clusters, kThreads, kSmem, s>>>(w);
+  products<KIND><<<2 * clusters, kProductThreads, kSmem, s>>>(w);
   return cudaGetLastError();
 }
 
@@ -786,9 +788,9 @@ cudaError_t run_linear(bool bf16, const LinearArgs& a, const Reduced& out, void*
   const int blocks   = static_cast<int>(need < 8 * n_sms ? need : 8 * n_sms);
   const size_t bytes = per * (entry_bytes(a.teacher.k) + static_cast<size_t>(a.teacher.k) * 4);
   if (warp)
-    linear_rows<T, 32><<<blocks, kThreads, bytes, s>>>(a, w.parts, w.product[0].n_tiles, out, sums, w.ticket);
+    linear_rows<T, 32><<<blocks, kThreads, bytes, s>>>(a, w.parts, 2 * w.product[0].n_tiles, out, sums, w.ticket);
   else
-    linear_rows<T, kThreads><<<blocks, kThreads, bytes, s>>>(a, w.parts, w.product[0].n_tiles, out, sums, w.ticket);
+    linear_rows<T, kThreads><<<blocks, kThreads, bytes, s>>>(a, w.parts, 2 * w.product[0].n_tiles, out, sums, w.ticket);
   count_launches(2);
   return cudaGetLastError();
 }
@@ -936,7 +938,7 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
 
 size_t linear_workspace(const LinearArgs& a, int n_sms)
 {
-  return (8 * n_sms + 1) * sizeof(double2) + a.n_rows * static_cast<size_t>(tiles_of(a.n_cols)) * sizeof(float2);
+  return (8 * n_sms + 1) * sizeof(double2) + a.n_rows * static_cast<size_t>(2 * tiles_of(a.n_cols)) * sizeof(float2);
 }
 
 size_t linear_grad_workspace(const LinearGradArgs& g, int n_sms)

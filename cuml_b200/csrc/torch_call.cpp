@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/TensorSubclassLikeUtils.h>
+#include <ATen/autocast_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -239,8 +240,14 @@ struct TeacherOf {
 bool teacher_of(PyObject* values, PyObject* index, PyObject* lse, const Tensor& like, TeacherOf& t)
 {
   const int64_t n = like.size(0);
-  if (!plain_rows(index)) return false;
-  t.index = THPVariable_Unpack(index);
+  if (values == Py_None && THPVariable_Check(index) && THPVariable_Unpack(index).dim() == 1) {
+    t.index = THPVariable_Unpack(index);  // one class per row
+    if (!t.index.is_cuda() || t.index.layout() != at::kStrided || at::isTensorSubclassLike(t.index)) return false;
+    t.index = t.index.unsqueeze(1);
+  } else {
+    if (!plain_rows(index)) return false;
+    t.index = THPVariable_Unpack(index);
+  }
   if ((t.index.scalar_type() != at::kInt && t.index.scalar_type() != at::kLong) || t.index.size(0) != n ||
       t.index.size(1) > B2FIL_MOST_TOP || !on(t.index, like))
     return false;
@@ -443,7 +450,8 @@ PyObject* linear_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   if (nargs != 7) return PyErr_Format(PyExc_TypeError, "linear_loss takes 7 arguments");
   Options o;
   if (!options_of(args + 4, o)) return nullptr;
-  if (!library.linear || !plain_rows(args[0]) || !plain_rows(args[1])) Py_RETURN_NONE;
+  if (!library.linear || at::autocast::is_autocast_enabled(at::kCUDA) || !plain_rows(args[0]) || !plain_rows(args[1]))
+    Py_RETURN_NONE;
   const Tensor& h = THPVariable_Unpack(args[0]);
   const Tensor& w = THPVariable_Unpack(args[1]);
   const int type  = type_of(h);
@@ -453,7 +461,8 @@ PyObject* linear_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   };
   TeacherOf t;
   if ((type != B2FIL_TYPE_BF16 && type != B2FIL_TYPE_F16) || w.scalar_type() != h.scalar_type() || !on(w, h) ||
-      w.size(1) != width || width % 8 || !tiled(h) || !tiled(w) || !teacher_of(args[2], args[3], Py_None, h, t))
+      w.size(1) != width || width % 8 || (width % 16 && n * c >= (int64_t(1) << 36) / width) || !tiled(h) || !tiled(w) ||
+      !teacher_of(args[2], args[3], Py_None, h, t))
     Py_RETURN_NONE;
   t.ignore    = o.ignore;
   const int k = static_cast<int>(t.index.size(1));

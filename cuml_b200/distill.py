@@ -351,8 +351,10 @@ def _layer(hidden, weight):
     shape, width = hidden.shape[:-1], weight.shape[1]
     if hidden.ndim != 2:
         hidden = hidden.reshape(-1, width)
-    if width % 8:  # zeros behind each row change no product
-        hidden, weight = (torch.nn.functional.pad(x, (0, 8 - width % 8)) for x in (hidden, weight))
+    # Zeros behind each row change no product.  Rows that start within a 32-byte sector are read a quarter slower
+    # (4096 x 1032 x 16,384: 501 us, with 1040 or 1024 columns 380), which pays for four copies in large products.
+    if width % 8 or (width % 16 and hidden.shape[0] * weight.shape[0] >= (1 << 36) // width):
+        hidden, weight = (torch.nn.functional.pad(x, (0, -width % 16)) for x in (hidden, weight))
     return _tiled(hidden), _tiled(weight), shape
 
 
@@ -363,13 +365,13 @@ def _tiled(x):
     return x
 
 
-def _linear(hidden, weight, values, index, temperature, ignore, reduction):
-    call = _native()
+def _linear(hidden, weight, values, index, temperature, ignore, reduction, compiled_only=False):
+    call = _native() if isinstance(hidden, torch.Tensor) and hidden.is_cuda else False
     if call:
         out = _answer(call.linear_loss(hidden, weight, values, index, temperature, ignore, reduction))
         if out is not None:
             return out
-    return _Linear.apply(hidden, weight, values, index, temperature, ignore, reduction)
+    return None if compiled_only else _Linear.apply(hidden, weight, values, index, temperature, ignore, reduction)
 
 
 def linear_cross_entropy(hidden, weight, target, *, ignore_index: int = -100, reduction: str = "mean"):
@@ -382,6 +384,10 @@ def linear_cross_entropy(hidden, weight, target, *, ignore_index: int = -100, re
 
     The loss is fp32; products are summed in fp32.  The gradients have the layer's type; the
     differences softmax - target are rounded to it before they are multiplied."""
+    if reduction in _REDUCTIONS:
+        loss = _linear(hidden, weight, None, target, 1.0, int(ignore_index), _REDUCTIONS[reduction], compiled_only=True)
+        if loss is not None:
+            return loss
     hidden, weight, shape = _layer(hidden, weight)
     _cuda("target", target, (torch.int32, torch.int64))
     if target.shape != shape:
@@ -399,6 +405,11 @@ def linear_distillation_loss(hidden, weight, top, *, temperature: float = 1.0, r
     hidden : (..., width), weight : (n_classes, width), both bf16 or both fp16 (under autocast they are cast).
     top, temperature, reduction : as in `distillation_loss`; types and rounding as in
     `linear_cross_entropy`."""
+    if reduction in _REDUCTIONS and type(top) is TopScores:
+        loss = _linear(hidden, weight, top.values, top.index, _temperature(temperature), _NO_CLASS, _REDUCTIONS[reduction],
+                       compiled_only=True)
+        if loss is not None:
+            return loss
     hidden, weight, shape = _layer(hidden, weight)
     values, index, _ = _top(top, hidden.shape[0], hidden.device, "renormalise")
     loss = _linear(hidden, weight, values, index, _temperature(temperature), _NO_CLASS, _reduction(reduction))
