@@ -89,7 +89,8 @@ __device__ __forceinline__ void visit_row(const T* row, int64_t n, int tid, int 
   if (at < n) one(at, row[at]);
 }
 
-// ---- running maximum m and sum s of exp((x - m) / T), c = log2(e) / T ------------------------
+// ---- reference m and sum s of exp((x - m) / T), c = log2(e) / T -------------------------------
+// m is the largest value, or one hardly below it.
 // The difference is taken before the scale: the scaled lowest value of a type would be -inf.
 __device__ __forceinline__ float power(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ double power(double x) { return exp2(x); }
@@ -136,6 +137,34 @@ struct Running {
     m = to;
 #pragma unroll
     for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+  }
+};
+
+// The same for a stream of values: the sum's reference is raised only when a value exceeds it by kSlack powers of
+// two.  (A warp of 32 maxima is raised for most of a short row's pieces; an exponent of up to kSlack
+// is rounded by 2^-22.)
+constexpr float kSlack = 6.f;
+template <class V>
+struct Stream {
+  V m = lowest<V>(), s = V(0), b = V(0), limit = lowest<V>();  // b: what is subtracted, limit: m + slack
+  __device__ __forceinline__ void raise(V to, V c, V slack)
+  {
+    s     = m == lowest<V>() ? s : s * power((m - to) * c);
+    m = b = to;
+    limit = to + slack;
+  }
+  __device__ __forceinline__ void add(V x, V c) { s += power((x - b) * c); }
+  __device__ __forceinline__ void take(V x, V c, V slack)
+  {
+    if (x > limit) raise(x, c, slack);
+    add(x, c);
+  }
+  __device__ __forceinline__ Running<V> running() const
+  {
+    Running<V> r;
+    r.m = m;
+    r.s = s;
+    return r;
   }
 };
 

@@ -40,8 +40,9 @@ __device__ __forceinline__ Running<float> visit_logits(const T* row, int64_t n, 
                                                        const uint32_t* bits)
 {
   constexpr int N = Piece<T>::N;
-  Running<float> r;
-  const int lead = lead_of(row, n);
+  Stream<float> r;
+  const int lead    = lead_of(row, n);
+  const float slack = kSlack / c;
   visit_row<kInFlight>(
     row, n, tid, threads,
     [&](int64_t i, T x) {
@@ -49,7 +50,7 @@ __device__ __forceinline__ Running<float> visit_logits(const T* row, int64_t n, 
         const uint32_t at = static_cast<uint32_t>(i - lead + 32);
         if (bits[at >> 5] >> (at & 31) & 1) return;
       }
-      r.take(widen(x), c);
+      r.take(widen(x), c, slack);
     },
     [&](int64_t i, const Piece<T>& v) {
       float x[N], most;
@@ -67,12 +68,11 @@ __device__ __forceinline__ Running<float> visit_logits(const T* row, int64_t n, 
       most = x[0];
 #pragma unroll
       for (int e = 1; e < N; ++e) most = fmaxf(most, x[e]);
-      if (most > r.m) r.raise(most, c);
-      const float b = base_of(r.m);
+      if (most > r.limit) r.raise(most, c, slack);
 #pragma unroll
-      for (int e = 0; e < N; ++e) r.s += power((x[e] - b) * c);
+      for (int e = 0; e < N; ++e) r.add(x[e], c);
     });
-  return r;
+  return r.running();
 }
 
 // Marks (or unmarks) the entries that lie in n columns from `begin` on.  By one warp.

@@ -14,7 +14,8 @@
 // registers.
 //
 // Bound by memory: one pass over the scores, which also takes the running maximum and sum of the
-// log-sum-exp (the maximum is the thread's best score, so that both cost one comparison per 16 bytes).
+// log-sum-exp.  Of a thread's best score that pass keeps the value and the 16 bytes that hold it; the keys of
+// their first and last element stand for its own above and below.
 // Where rows are few, several blocks share one and a second kernel joins their lists.
 #include "distill_common.cuh"
 
@@ -27,11 +28,12 @@ constexpr int kList     = 2048;  // candidates of a block
 constexpr int kWarpList = 256;   // candidates of a warp
 constexpr int kWarpCols = 1024;  // longest rows and largest k that a warp takes
 constexpr int kWarpTop  = 24;
-constexpr int kSlack    = 8;     // groups more than k that end the search of the bound
+constexpr int kMore     = 8;     // groups more than k that end the search of the bound
 constexpr int kInFlight = 4;
 constexpr int kTileRows = 128;   // rows of a tile for one thread each, their most classes and k
 constexpr int kTileCols = 48;
 constexpr int kTileTop  = 8;
+constexpr int kTileFlight = 4;
 static_assert(kThreads >= kMostTop, "a group per entry");
 
 // ---- keys ----------------------------------------------------------------------------------
@@ -130,16 +132,20 @@ __device__ __forceinline__ void write_top(const TopArgs& a, int64_t row, int j, 
   a.index[row * a.k + j]                   = static_cast<int32_t>(key.index());
 }
 
-// The sum over a row: of exp((x - m) / T) beside the maximum m, or of the probabilities' x^(1/T).  Probabilities
+// The sum over a row: of exp((x - m) / T) beside the reference m, or of the probabilities' x^(1/T).  Probabilities
 // add up to nearly 1, whose logarithm is a difference: at T = 1 their sum keeps what each addition drops.
 template <class V, bool PROB>
 struct Sum {
-  Running<V> r;  // PROB: m is the largest, s the sum
+  Stream<V> r;  // PROB: the sum alone
   V dropped = V(0);
+  __device__ __forceinline__ void reach(V most, V c, V slack)
+  {
+    if (!PROB && most > r.limit) r.raise(most, c, slack);
+  }
   __device__ __forceinline__ void add(V x, V c, bool plain)
   {
     if (!PROB) {
-      r.s += power((x - base_of(r.m)) * c);
+      r.add(x, c);
     } else if (plain) {
       const V t = r.s + x, b = t - r.s;
       dropped += (r.s - (t - b)) + (x - b);
@@ -150,9 +156,22 @@ struct Sum {
   }
 };
 
+// The logarithm of s + dropped, which may be nearly 1: of its 32-bit part, and what that leaves.
+__device__ __forceinline__ float log_of_sum(float s, double dropped)
+{
+  const double all = s + dropped;
+  const float high = static_cast<float>(all);
+  return high > 0.f && high < INFINITY ? logf(high) + static_cast<float>(all - high) / high : logf(high);
+}
+__device__ __forceinline__ double log_of_sum(double s, double dropped) { return log(s + dropped); }
+
+__device__ __forceinline__ double log_of_terms(float s) { return log_sum(s); }
+__device__ __forceinline__ double log_of_terms(double s) { return log(s); }
+
 // log-sum-exp of a row from its sum; best: the row's largest key.
+// m: what its terms are relative to.
 template <class V, class K>
-__device__ __forceinline__ void write_lse(const TopArgs& a, int64_t row, V s, double dropped, const K& best)
+__device__ __forceinline__ void write_lse(const TopArgs& a, int64_t row, V m, V s, double dropped, const K& best)
 {
   if (!a.logsumexp) return;
   const V top = best.value();
@@ -160,9 +179,9 @@ __device__ __forceinline__ void write_lse(const TopArgs& a, int64_t row, V s, do
   if (top != top)
     r = top;
   else if (a.probabilities)
-    r = static_cast<V>(log(static_cast<double>(s) + dropped));
+    r = log_of_sum(s, dropped);
   else
-    r = top == lowest<V>() || top == -lowest<V>() ? top : static_cast<V>(top * a.inv_temperature) + log_of(s);
+    r = top == lowest<V>() || top == -lowest<V>() ? top : static_cast<V>(m * a.inv_temperature + log_of_terms(s));
   static_cast<V*>(a.logsumexp)[row] = r;
 }
 
@@ -184,7 +203,7 @@ struct RowShared {
 
 // A segment of a row per block or warp.  segs == 1: the row's answer; else its k best keys and its sum.
 template <class T, int THREADS, bool PROB>
-__global__ void __launch_bounds__(kThreads) top_segments(TopArgs a, int segs, int64_t seg_cols,
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments(TopArgs a, int segs, int64_t seg_cols,
                                                          typename KeyOf<T>::type* keys, double* sums)
 {
   using V = typename ValueOf<T>::type;
@@ -201,29 +220,24 @@ __global__ void __launch_bounds__(kThreads) top_segments(TopArgs a, int segs, in
   const int k         = static_cast<int>(min(static_cast<int64_t>(a.k), n));
   const V c           = static_cast<V>(1.4426950408889634 * a.inv_temperature);
   const bool plain    = a.inv_temperature == 1.0;
+  const V slack       = V(kSlack) / c;
   for (int64_t row = static_cast<int64_t>(blockIdx.x / segs) * ROWS + slot; row < a.n_rows;
        row += static_cast<int64_t>(gridDim.x / segs) * ROWS) {
     const T* x       = static_cast<const T*>(a.scores) + row * a.row_stride + begin;
     const int lead   = lead_of(x, n);
     const int pieces = static_cast<int>((n - lead) / N);
     const T* body    = x + lead;
-    // the thread's best score and its place, and the sum
+    // the thread's best score, the first element of the piece that holds it, and the sum
     Sum<V, PROB> sum;
+    V top       = lowest<V>();
     uint32_t at = ~0u;  // none yet
-    auto raise  = [&](V v) {
-      if (PROB)
-        sum.r.m = v;
-      else
-        sum.r.raise(v, c);
-    };
     visit_row<kInFlight>(
       x, n, tid, THREADS,
       [&](int64_t i, T e) {
         const V v = widen(e);
-        if (v > sum.r.m || at == ~0u) {
-          if (v > sum.r.m) raise(v);
-          at = static_cast<uint32_t>(i);
-        }
+        if (v > top || at == ~0u) at = static_cast<uint32_t>(i);
+        top = larger(top, v);
+        sum.reach(v, c, slack);
         sum.add(v, c, plain);
       },
       [&](int64_t i, const Piece<T>& p) {
@@ -233,18 +247,12 @@ __global__ void __launch_bounds__(kThreads) top_segments(TopArgs a, int segs, in
         most = v[0];
 #pragma unroll
         for (int e = 1; e < N; ++e) most = larger(most, v[e]);
-        if (most > sum.r.m || at == ~0u) {
-          if (most > sum.r.m) raise(most);
-          at = static_cast<uint32_t>(i);
-#pragma unroll
-          for (int e = N - 1; e >= 0; --e)
-            if (v[e] == most) at = static_cast<uint32_t>(i + e);
-        }
+        if (most > top || at == ~0u) at = static_cast<uint32_t>(i);
+        top = larger(top, most);
+        sum.reach(most, c, slack);
 #pragma unroll
         for (int e = 0; e < N; ++e) sum.add(v[e], c, plain);
       });
-    K best = K::none();
-    if (at != ~0u) best = K::of(sum.r.m, static_cast<uint32_t>(begin) + at);
     if (sum.r.s != sum.r.s) {  // a NaN, or infinities: the first NaN of the group is its best
       uint32_t first = ~0u;
       visit_row<1>(
@@ -257,54 +265,69 @@ __global__ void __launch_bounds__(kThreads) top_segments(TopArgs a, int segs, in
           for (int e = 0; e < N; ++e)
             if (widen(p.v[e]) != widen(p.v[e])) first = min(first, static_cast<uint32_t>(i + e));
         });
-      if (first != ~0u) best = K::of(static_cast<V>(NAN), static_cast<uint32_t>(begin) + first);
+      if (first != ~0u) {
+        top = static_cast<V>(NAN);
+        at  = first;
+      }
     }
+    // bounds of the best element's key
+    const bool any = at != ~0u;
+    const K below  = any ? K::of(top, static_cast<uint32_t>(begin) + at + N - 1) : K::none();
+    const K above  = any ? K::of(top, static_cast<uint32_t>(begin) + at) : K::none();
     double dropped = 0;
+    Running<V> all;
+    all.m = V(0);
     if (PROB) {
       // (in 64 bits: see Sum)
       dropped = sum_row<THREADS>(static_cast<double>(sum.r.s) + sum.dropped, room);
-      sum.r.s = V(0);
     } else {
-      join_row<THREADS>(sum.r, c, reinterpret_cast<V*>(room));
+      all = sum.r.running();
+      join_row<THREADS>(all, c, reinterpret_cast<V*>(room));
     }
-    // tau: a bound that k groups reach, and at most kSlack more unless its last bit is reached
-    K tau = K::none();
-    const int seen = count_row<THREADS>(at != ~0u);
-    if (seen > k + kSlack || (seen > k && n > LIST)) {
+    // tau: a bound that k groups reach, and at most kMore more unless its last bit is reached
+    K tau          = K::none();
+    const int seen = count_row<THREADS>(any);
+    if (seen > k + kMore || (seen > k && n > LIST)) {
       for (int bit = K::kBits - 1; bit >= 0; --bit) {
         const K next  = tau.with(bit);
-        const int got = count_row<THREADS>(!next.above(best));
+        const int got = count_row<THREADS>(!next.above(below));
         if (got < k) continue;
         tau = next;
-        if (got <= k + kSlack) break;
+        if (got <= k + kMore) break;
       }
     }
     if (tid == 0) mine.found = mine.chosen = 0;
     sync_row<THREADS>();
-    const bool reaches = at != ~0u && !tau.above(best);
+    const bool reaches = any && !tau.above(above);
     if (reaches) mine.groups[atomicAdd(&mine.chosen, 1)] = static_cast<int16_t>(tid);
     sync_row<THREADS>();
     const int chosen = mine.chosen;
-    // pieces of a group: the same number of all, those behind the last are left out below
-    const int per = (pieces + THREADS - 1) / THREADS;
-    auto collect  = [&](const K& bound, bool store) {
-      auto take = [&](int64_t i, T e) {
-        const K key = K::of(widen(e), static_cast<uint32_t>(begin + i));
+    // A group's pieces, to the next power of two: those behind the last are left out below.
+    const int per   = (pieces + THREADS - 1) / THREADS;
+    const int shift = per <= 1 ? 0 : 32 - __clz(per - 1);
+    auto collect    = [&](const K& bound) {
+      auto take = [&](int64_t i) {
+        const K key = K::of(widen(x[i]), static_cast<uint32_t>(begin + i));
         if (bound.above(key)) return;
         const int to = atomicAdd(&mine.found, 1);
-        if (store && to < LIST) mine.list[to] = key;
+        if (to < LIST) mine.list[to] = key;
       };
-      for (int i = tid; i < chosen * per; i += THREADS) {
-        const int p = mine.groups[i / per] + i % per * THREADS;
+      // (values below the bound's are left out at once; NaN is not below)
+      const V least = bound.value();
+#pragma unroll 4
+      for (int i = tid; i < chosen << shift; i += THREADS) {
+        const int p = mine.groups[i >> shift] + (i & ((1 << shift) - 1)) * THREADS;
         if (p >= pieces) continue;
         const Piece<T> v = load_piece(body + static_cast<int64_t>(p) * N);
+        uint32_t some = 0;
 #pragma unroll
-        for (int e = 0; e < N; ++e) take(lead + static_cast<int64_t>(p) * N + e, v.v[e]);
+        for (int e = 0; e < N; ++e) some |= !(widen(v.v[e]) < least) ? 1u << e : 0u;
+        for (; some; some &= some - 1) take(lead + static_cast<int64_t>(p) * N + (__ffs(some) - 1));
       }
       // the elements before the first and behind the last boundary
-      if (tid < lead) take(tid, x[tid]);
+      if (tid < lead) take(tid);
       const int64_t end = lead + static_cast<int64_t>(pieces) * N + tid;
-      if (end < n) take(end, x[end]);
+      if (end < n) take(end);
       sync_row<THREADS>();
       const int got = mine.found;
       sync_row<THREADS>();
@@ -312,15 +335,19 @@ __global__ void __launch_bounds__(kThreads) top_segments(TopArgs a, int segs, in
       sync_row<THREADS>();
       return got;
     };
-    int got = collect(tau, true);
-    if (got > LIST) {
-      // the largest bound that k keys reach, bit by bit: keys differ, so exactly k do
-      K bound = K::none();
-      for (int bit = K::kBits - 1; bit >= 0; --bit) {
-        const K next = bound.with(bit);
-        if (collect(next, false) >= k) bound = next;
+    // Where the list is too short, the largest bound that k keys reach is found bit by bit: keys differ, so
+    // exactly k do.
+    int got = 0;
+    K bound = K::none(), next = tau;
+    for (int bit = -1;;) {
+      got = collect(next);
+      if (bit < 0) {
+        if (got <= LIST) break;
+        bit = K::kBits;
+      } else if (got >= k) {
+        bound = next;
       }
-      got = collect(bound, true);
+      next = --bit < 0 ? bound : bound.with(bit);
     }
     // a candidate's place is the number of larger ones
     const int64_t part = row * segs + seg;
@@ -332,7 +359,7 @@ __global__ void __launch_bounds__(kThreads) top_segments(TopArgs a, int segs, in
       if (place >= k) continue;
       if (segs == 1) {
         write_top<T>(a, row, place, key);
-        if (place == 0) write_lse(a, row, sum.r.s, dropped, key);
+        if (place == 0) write_lse(a, row, all.m, all.s, dropped, key);
       } else {
         keys[part * a.k + place] = key;
       }
@@ -340,8 +367,8 @@ __global__ void __launch_bounds__(kThreads) top_segments(TopArgs a, int segs, in
     if (segs > 1) {
       for (int j = k + tid; j < a.k; j += THREADS) keys[part * a.k + j] = K::none();
       if (tid == 0) {
-        sums[2 * part]     = PROB ? dropped : static_cast<double>(sum.r.s);
-        sums[2 * part + 1] = sum.r.m;
+        sums[2 * part]     = PROB ? dropped : static_cast<double>(all.s);
+        sums[2 * part + 1] = all.m;
       }
     }
     sync_row<THREADS>();
@@ -385,7 +412,7 @@ __global__ void __launch_bounds__(kThreads) top_join(TopArgs a, int segs, const 
       r.s = sum_row<kThreads>(r.s, room);
     else
       join_row<kThreads>(r, c, room);
-    if (threadIdx.x == 0) write_lse(a, row, static_cast<V>(a.probabilities ? 0.0 : r.s), a.probabilities ? r.s : 0.0, list[0]);
+    if (threadIdx.x == 0) write_lse(a, row, static_cast<V>(r.m), static_cast<V>(a.probabilities ? 0.0 : r.s), a.probabilities ? r.s : 0.0, list[0]);
     __syncthreads();
   }
 }
@@ -414,12 +441,33 @@ __global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
   const int pitch = sizeof(T) >= 4 ? c_n | 1 : (c_n + 1) / 2 * 2 + ((c_n + 1) / 2 % 2 ? 0 : 2);
   const V c       = static_cast<V>(1.4426950408889634 * a.inv_temperature);
   const bool plain = a.inv_temperature == 1.0;
+  const bool whole = a.row_stride == a.n_cols && (reinterpret_cast<uintptr_t>(a.scores) & 15) == 0 && c_n > 1;
+  // i / c_n = i * inverse / 2^32 for i < 128 x 48 (exact: i * c_n < 2^32)
+  const uint32_t inverse = 0xffffffffu / c_n + 1;
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * kTileRows; first < a.n_rows;
        first += static_cast<int64_t>(gridDim.x) * kTileRows) {
     const int rows = static_cast<int>(min(static_cast<int64_t>(kTileRows), a.n_rows - first));
     const T* from  = static_cast<const T*>(a.scores) + first * a.row_stride;
     __syncthreads();  // the last tile has been used
-    {
+    if (whole) {
+      // rows without gaps: 16 bytes at a time, kTileFlight of them in flight
+      constexpr int N     = Piece<T>::N;
+      const int all       = rows * c_n, pieces = all / N, pad = pitch - c_n;
+      for (int p = threadIdx.x; p < pieces; p += kTileFlight * kTileRows) {
+        Piece<T> v[kTileFlight];
+#pragma unroll
+        for (int u = 0; u < kTileFlight; ++u)
+          if (p + u * kTileRows < pieces) v[u] = load_piece(from + (p + u * kTileRows) * N);
+#pragma unroll
+        for (int u = 0; u < kTileFlight; ++u) {
+          const uint32_t at = (p + u * kTileRows) * N;
+          if (p + u * kTileRows >= pieces) break;
+#pragma unroll
+          for (int e = 0; e < N; ++e) tile[at + e + __umulhi(at + e, inverse) * pad] = v[u].v[e];
+        }
+      }
+      for (int i = pieces * N + threadIdx.x; i < all; i += kTileRows) tile[i + __umulhi(i, inverse) * pad] = from[i];
+    } else {
       int r = threadIdx.x / c_n, i = threadIdx.x % c_n;
       const int dr = kTileRows / c_n, di = kTileRows % c_n;
       while (r < rows) {
@@ -459,18 +507,14 @@ __global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
       }
     }
     Sum<V, PROB> sum;
-    sum.r.m        = from_ordered(key[0]);
-    double dropped = 0;
-    if (PROB && plain) {
-      for (int i = 0; i < c_n; ++i) dropped += static_cast<double>(widen(x[i]));
-    } else {
-      for (int i = 0; i < c_n; ++i) sum.add(widen(x[i]), c, plain);
-    }
+    const V top = from_ordered(key[0]);
+    sum.reach(top, c, V(0));
+    for (int i = 0; i < c_n; ++i) sum.add(widen(x[i]), c, plain);
     const int64_t row = first + threadIdx.x;
 #pragma unroll
     for (int j = 0; j < TOP; ++j)
       if (j < a.k) write_top<T>(a, row, j, K::of(from_ordered(key[j]), static_cast<uint32_t>(at[j])));
-    write_lse(a, row, sum.r.s, dropped, K::of(from_ordered(key[0]), 0u));
+    write_lse(a, row, sum.r.m, sum.r.s, static_cast<double>(sum.dropped), K::of(top, 0u));
   }
 }
 
