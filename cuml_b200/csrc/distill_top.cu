@@ -132,26 +132,33 @@ __device__ __forceinline__ void write_top(const TopArgs& a, int64_t row, int j, 
   a.index[row * a.k + j]                   = static_cast<int32_t>(key.index());
 }
 
-// The sum over a row: of exp((x - m) / T) beside the reference m, or of the probabilities' x^(1/T).  Probabilities
-// add up to nearly 1, whose logarithm is a difference: at T = 1 their sum keeps what each addition drops.
+// The sum over a row: of 2^(x c - r), c = log2(e) / T, or of the probabilities' x^(1/T).  r is m c of a score m that
+// no score exceeds by more than kSlack powers of two; it stays finite for the lowest values, whose terms
+// may all be 0 then: such a row's log-sum-exp is its largest score.  Probabilities add up to nearly 1, whose
+// logarithm is a difference: at T = 1 their sum keeps what each addition drops.
 template <class V, bool PROB>
 struct Sum {
-  Stream<V> r;  // PROB: the sum alone
-  V dropped = V(0);
-  __device__ __forceinline__ void reach(V most, V c, V slack)
+  V r = V(0), s = V(0), limit = lowest<V>(), dropped = V(0);
+  bool first = true;
+  __device__ __forceinline__ void reach(V most, V c)
   {
-    if (!PROB && most > r.limit) r.raise(most, c, slack);
+    if (PROB || !(most > limit)) return;
+    const V to = larger(larger(most, V(-1e36)) * c, V(-1e36));
+    s          = first ? s : s * power(r - to);
+    r          = to;
+    first      = false;
+    limit      = larger(most, V(-1e36)) + V(kSlack) / c;
   }
   __device__ __forceinline__ void add(V x, V c, bool plain)
   {
     if (!PROB) {
-      r.add(x, c);
+      s += power(fma(x, c, -r));
     } else if (plain) {
-      const V t = r.s + x, b = t - r.s;
-      dropped += (r.s - (t - b)) + (x - b);
-      r.s = t;
+      const V t = s + x, b = t - s;
+      dropped += (s - (t - b)) + (x - b);
+      s = t;
     } else {
-      r.s += x == V(0) ? V(0) : power(log_of(x) * c);
+      s += x == V(0) ? V(0) : power(log_of(x) * c);
     }
   }
 };
@@ -169,7 +176,7 @@ __device__ __forceinline__ double log_of_terms(float s) { return log_sum(s); }
 __device__ __forceinline__ double log_of_terms(double s) { return log(s); }
 
 // log-sum-exp of a row from its sum; best: the row's largest key.
-// m: what its terms are relative to.
+// m: the terms are relative to 2^m.
 template <class V, class K>
 __device__ __forceinline__ void write_lse(const TopArgs& a, int64_t row, V m, V s, double dropped, const K& best)
 {
@@ -181,22 +188,17 @@ __device__ __forceinline__ void write_lse(const TopArgs& a, int64_t row, V m, V 
   else if (a.probabilities)
     r = log_of_sum(s, dropped);
   else
-    r = top == lowest<V>() || top == -lowest<V>() ? top : static_cast<V>(m * a.inv_temperature + log_of_terms(s));
+    r = top == lowest<V>() || top == -lowest<V>() ? top
+        : s == V(0)                               ? static_cast<V>(top * a.inv_temperature)
+                                                  : static_cast<V>(m * 0.69314718055994530942 + log_of_terms(s));
   static_cast<V*>(a.logsumexp)[row] = r;
-}
-
-// How many of the row's threads say yes.
-template <int THREADS>
-__device__ __forceinline__ int count_row(bool yes)
-{
-  if (THREADS == 32) return __popc(__ballot_sync(~0u, yes));
-  return __syncthreads_count(yes);
 }
 
 // What a row's threads share.
 template <class K, int LIST, int GROUPS>
 struct RowShared {
   K list[LIST];
+  K tau;
   int16_t groups[GROUPS];
   int found, chosen;
 };
@@ -220,7 +222,6 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
   const int k         = static_cast<int>(min(static_cast<int64_t>(a.k), n));
   const V c           = static_cast<V>(1.4426950408889634 * a.inv_temperature);
   const bool plain    = a.inv_temperature == 1.0;
-  const V slack       = V(kSlack) / c;
   for (int64_t row = static_cast<int64_t>(blockIdx.x / segs) * ROWS + slot; row < a.n_rows;
        row += static_cast<int64_t>(gridDim.x / segs) * ROWS) {
     const T* x       = static_cast<const T*>(a.scores) + row * a.row_stride + begin;
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
         const V v = widen(e);
         if (v > top || at == ~0u) at = static_cast<uint32_t>(i);
         top = larger(top, v);
-        sum.reach(v, c, slack);
+        sum.reach(v, c);
         sum.add(v, c, plain);
       },
       [&](int64_t i, const Piece<T>& p) {
@@ -249,11 +250,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
         for (int e = 1; e < N; ++e) most = larger(most, v[e]);
         if (most > top || at == ~0u) at = static_cast<uint32_t>(i);
         top = larger(top, most);
-        sum.reach(most, c, slack);
+        sum.reach(most, c);
 #pragma unroll
         for (int e = 0; e < N; ++e) sum.add(v[e], c, plain);
       });
-    if (sum.r.s != sum.r.s) {  // a NaN, or infinities: the first NaN of the group is its best
+    if (sum.s != sum.s) {  // a NaN, or infinities: the first NaN of the group is its best
       uint32_t first = ~0u;
       visit_row<1>(
         x, n, tid, THREADS,
@@ -279,25 +280,45 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
     all.m = V(0);
     if (PROB) {
       // (in 64 bits: see Sum)
-      dropped = sum_row<THREADS>(static_cast<double>(sum.r.s) + sum.dropped, room);
+      dropped = sum_row<THREADS>(static_cast<double>(sum.s) + sum.dropped, room);
     } else {
-      all = sum.r.running();
-      join_row<THREADS>(all, c, reinterpret_cast<V*>(room));
+      all.m = sum.first ? lowest<V>() : sum.r;
+      all.s = sum.s;
+      join_row<THREADS>(all, V(1), reinterpret_cast<V*>(room));
     }
-    // tau: a bound that k groups reach, and at most kMore more unless its last bit is reached
-    K tau          = K::none();
-    const int seen = count_row<THREADS>(any);
-    if (seen > k + kMore || (seen > k && n > LIST)) {
-      for (int bit = K::kBits - 1; bit >= 0; --bit) {
-        const K next  = tau.with(bit);
-        const int got = count_row<THREADS>(!next.above(below));
-        if (got < k) continue;
-        tau = next;
-        if (got <= k + kMore) break;
+    // tau: a bound that k groups reach, and at most kMore more unless its last bit is reached; the first warp
+    // counts for all
+    K tau = K::none();
+    if (THREADS > 32) {
+      mine.list[tid] = below;
+      __syncthreads();
+    }
+    if (tid < 32) {
+      constexpr int G = THREADS / 32;
+      K group[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) group[g] = THREADS > 32 ? mine.list[tid + 32 * g] : below;
+      auto reached = [&](const K& by) {
+        int some = 0;
+#pragma unroll
+        for (int g = 0; g < G; ++g) some += !by.above(group[g]);
+        return static_cast<int>(__reduce_add_sync(~0u, some));
+      };
+      const int seen = reached(K::none().with(0));  // (a group without elements has no key)
+      if (seen > k + kMore || (seen >= k && n > LIST)) {
+        for (int bit = K::kBits - 1; bit >= 0; --bit) {
+          const K next  = tau.with(bit);
+          const int got = reached(next);
+          if (got < k) continue;
+          tau = next;
+          if (got <= k + kMore) break;
+        }
       }
+      if (tid == 0) mine.tau = tau;
     }
     if (tid == 0) mine.found = mine.chosen = 0;
     sync_row<THREADS>();
+    tau                = mine.tau;
     const bool reaches = any && !tau.above(above);
     if (reaches) mine.groups[atomicAdd(&mine.chosen, 1)] = static_cast<int16_t>(tid);
     sync_row<THREADS>();
@@ -384,7 +405,6 @@ __global__ void __launch_bounds__(kThreads) top_join(TopArgs a, int segs, const 
   using K = typename KeyOf<T>::type;
   __shared__ K list[kList];
   __shared__ double room[64];
-  const double c = 1.4426950408889634 * a.inv_temperature;
   for (int64_t row = blockIdx.x; row < a.n_rows; row += gridDim.x) {
     const K* from = keys + row * segs * a.k;
     const int all = segs * a.k;
@@ -406,12 +426,12 @@ __global__ void __launch_bounds__(kThreads) top_join(TopArgs a, int segs, const 
       if (a.probabilities)
         r.s += s;
       else
-        r.join(m, s, c);
+        r.join(m, s, 1.0);
     }
     if (a.probabilities)
       r.s = sum_row<kThreads>(r.s, room);
     else
-      join_row<kThreads>(r, c, room);
+      join_row<kThreads>(r, 1.0, room);
     if (threadIdx.x == 0) write_lse(a, row, static_cast<V>(r.m), static_cast<V>(a.probabilities ? 0.0 : r.s), a.probabilities ? r.s : 0.0, list[0]);
     __syncthreads();
   }
@@ -508,13 +528,13 @@ __global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
     }
     Sum<V, PROB> sum;
     const V top = from_ordered(key[0]);
-    sum.reach(top, c, V(0));
+    sum.reach(top, c);
     for (int i = 0; i < c_n; ++i) sum.add(widen(x[i]), c, plain);
     const int64_t row = first + threadIdx.x;
 #pragma unroll
     for (int j = 0; j < TOP; ++j)
       if (j < a.k) write_top<T>(a, row, j, K::of(from_ordered(key[j]), static_cast<uint32_t>(at[j])));
-    write_lse(a, row, sum.r.m, sum.r.s, static_cast<double>(sum.dropped), K::of(top, 0u));
+    write_lse(a, row, sum.r, sum.s, static_cast<double>(sum.dropped), K::of(top, 0u));
   }
 }
 
