@@ -96,6 +96,8 @@ __device__ __forceinline__ float power(float x) { float y; asm("ex2.approx.ftz.f
 __device__ __forceinline__ double power(double x) { return exp2(x); }
 __device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
+__device__ __forceinline__ float smaller(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ double smaller(double a, double b) { return fmin(a, b); }
 template <class V>
 __device__ __forceinline__ V lowest()
 {

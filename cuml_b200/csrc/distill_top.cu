@@ -503,38 +503,66 @@ __global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
     __syncthreads();
     if (threadIdx.x >= rows) continue;
     const T* x = tile + threadIdx.x * pitch;
-    O key[TOP];
+    // Sorted insertion without branches: of the entries that x exceeds the first becomes x, the others move down.
+    V top[TOP], odd = V(0);
     int at[TOP];
 #pragma unroll
     for (int j = 0; j < TOP; ++j) {
-      key[j] = 0;
-      at[j]  = 0;
+      top[j] = lowest<V>();
+      at[j]  = j < c_n ? j : 0;  // (a row of -inf)
     }
     for (int i = 0; i < c_n; ++i) {
-      O o = ordered(widen(x[i]));
-      if (o <= key[TOP - 1]) continue;  // (equal ones: the earlier class stays)
-      int p   = i;
-      bool up = false;  // all entries behind the new one move down
+      const V v = widen(x[i]);
+      odd       = fma(v, V(0), odd);  // NaN where one of the scores is infinite or no number
+      bool up[TOP];
+#pragma unroll
+      for (int j = 0; j < TOP; ++j) up[j] = v > top[j];
+#pragma unroll
+      for (int j = TOP - 1; j > 0; --j) {
+        top[j] = larger(top[j], smaller(top[j - 1], v));
+        at[j]  = up[j - 1] ? at[j - 1] : up[j] ? i : at[j];
+      }
+      top[0] = larger(top[0], v);
+      at[0]  = up[0] ? i : at[0];
+    }
+    if (odd != V(0)) {  // by ordered integers
+      O key[TOP];
 #pragma unroll
       for (int j = 0; j < TOP; ++j) {
-        up |= o > key[j];
-        const O ko    = key[j];
-        const int ka  = at[j];
-        key[j]        = up ? o : ko;
-        at[j]         = up ? p : ka;
-        o             = up ? ko : o;
-        p             = up ? ka : p;
+        key[j] = 0;
+        at[j]  = 0;
       }
+      for (int i = 0; i < c_n; ++i) {
+        O o     = ordered(widen(x[i]));
+        int p   = i;
+        bool up = false;  // all entries behind the new one move down (equal ones: the earlier class stays)
+#pragma unroll
+        for (int j = 0; j < TOP; ++j) {
+          up |= o > key[j];
+          const O ko   = key[j];
+          const int ka = at[j];
+          key[j]       = up ? o : ko;
+          at[j]        = up ? p : ka;
+          o            = up ? ko : o;
+          p            = up ? ka : p;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < TOP; ++j) top[j] = from_ordered(key[j]);
     }
     Sum<V, PROB> sum;
-    const V top = from_ordered(key[0]);
-    sum.reach(top, c);
+    sum.reach(top[0], c);
     for (int i = 0; i < c_n; ++i) sum.add(widen(x[i]), c, plain);
     const int64_t row = first + threadIdx.x;
+    T* values         = static_cast<T*>(a.values) + row * a.k;
+    int32_t* index    = a.index + row * a.k;
 #pragma unroll
-    for (int j = 0; j < TOP; ++j)
-      if (j < a.k) write_top<T>(a, row, j, K::of(from_ordered(key[j]), static_cast<uint32_t>(at[j])));
-    write_lse(a, row, sum.r, sum.s, static_cast<double>(sum.dropped), K::of(top, 0u));
+    for (int j = 0; j < TOP; ++j) {
+      if (j >= a.k) break;
+      values[j] = narrow<T>(PROB ? log_of(top[j]) : top[j]);
+      index[j]  = at[j];
+    }
+    write_lse(a, row, sum.r, sum.s, static_cast<double>(sum.dropped), K::of(top[0], 0u));
   }
 }
 
@@ -572,9 +600,13 @@ cudaError_t run_top(const TopArgs& a, void* workspace, int n_sms, cudaStream_t s
 {
   using K = typename KeyOf<T>::type;
   if (a.n_cols <= kTileCols && a.k <= kTileTop) {
-    if (a.k == 1) return run_tiles<T, 1>(a, n_sms, s);
-    if (a.k <= 4) return run_tiles<T, 4>(a, n_sms, s);
-    return run_tiles<T, kTileTop>(a, n_sms, s);
+    switch (a.k) {
+      case 1: return run_tiles<T, 1>(a, n_sms, s);
+      case 2: return run_tiles<T, 2>(a, n_sms, s);
+      case 3: return run_tiles<T, 3>(a, n_sms, s);
+      case 4: return run_tiles<T, 4>(a, n_sms, s);
+      default: return run_tiles<T, kTileTop>(a, n_sms, s);
+    }
   }
   if (a.n_cols <= kWarpCols && a.k <= kWarpTop) {
     const int64_t need = (a.n_rows + kThreads / 32 - 1) / (kThreads / 32), most = 16ll * n_sms;
