@@ -6,13 +6,16 @@ model), keep the `k` best classes of each row, and compute the loss of a student
 
     top_scores                 the k best scores of each row, their classes, the row's log-sum-exp
     distillation_loss          T^2 KL(teacher || student) from the student's logits
+    cross_entropy              softmax cross entropy from the student's logits
     linear_cross_entropy       softmax cross entropy from the last linear layer, logits not kept
     linear_distillation_loss   distillation_loss from the last linear layer, logits not kept
 
 `ForestInference.predict_top`, `.teach` and `.distillation_loss` call them with a forest as the teacher.
 All tensors are CUDA tensors of one device; work is enqueued on torch's current stream of that device and
 nothing waits.  The losses have first derivatives by the logits, or by the layer's input and weight; the
-teacher's values are constants.  All computation happens in libb2fil.so.
+teacher's values are constants.  Calls and their gradients can be captured into CUDA graphs once they have run on
+the device (as everywhere in torch, while no autograd graph of the same leaves from outside the capture is
+alive).  All computation happens in libb2fil.so.
 """
 from __future__ import annotations
 
@@ -250,13 +253,13 @@ def _kept(kept, n):
 _STUDENT = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _loss(x, values, index, lse, temperature, reduction, compiled_only=False):
+def _loss(x, values, index, lse, temperature, reduction, ignore=_NO_CLASS, compiled_only=False):
     call = _native() if isinstance(x, torch.Tensor) and x.is_cuda else False
     if call:
-        out = _answer(call.distill_loss(x, values, index, lse, temperature, _NO_CLASS, reduction))
+        out = _answer(call.distill_loss(x, values, index, lse, temperature, ignore, reduction))
         if out is not None:
             return out
-    return None if compiled_only else _Loss.apply(x, values, index, lse, temperature, _NO_CLASS, reduction)
+    return None if compiled_only else _Loss.apply(x, values, index, lse, temperature, ignore, reduction)
 
 
 def distillation_loss(logits, top, *, temperature: float = 1.0, tail: str = "renormalise", reduction: str = "mean"):
@@ -288,6 +291,34 @@ def distillation_loss(logits, top, *, temperature: float = 1.0, tail: str = "ren
         raise ValueError(f"tail='bucket' takes at most 2^20 classes, got {n_cols}")
     loss = _loss(x, values, index, lse, _temperature(temperature), _reduction(reduction))
     return loss.view(shape) if reduction == "none" and len(shape) != 1 else loss
+
+
+def cross_entropy(logits, target, *, ignore_index: int = -100, reduction: str = "mean"):
+    """Softmax cross entropy of `logits` (..., n_classes), fp32, bf16 or fp16, and the classes `target` (...), int32
+    or int64: `distillation_loss` of a teacher that is sure.  Rows whose target is `ignore_index` or outside
+    [0, n_classes), or whose logits are all -inf, do not count; reduction and types as there."""
+    if reduction in _REDUCTIONS:
+        loss = _loss(logits, None, target, None, 1.0, _REDUCTIONS[reduction], int(ignore_index), compiled_only=True)
+        if loss is not None:
+            return loss
+    _cuda("logits", logits, _STUDENT)
+    if logits.ndim < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must have shape (..., n_classes), got {tuple(logits.shape)}")
+    shape = logits.shape[:-1]
+    target = _target(target, shape, logits.device)
+    x = logits if logits.ndim == 2 else logits.reshape(-1, logits.shape[-1])
+    loss = _loss(x, None, target, None, 1.0, _reduction(reduction), int(ignore_index))
+    return loss.view(shape) if reduction == "none" and len(shape) != 1 else loss
+
+
+def _target(target, shape, dev):
+    """Classes of rows of that leading shape as (n, 1), checked."""
+    _cuda("target", target, (torch.int32, torch.int64))
+    if target.shape != shape:
+        raise ValueError(f"target must have shape {tuple(shape)}, got {tuple(target.shape)}")
+    if target.device != dev:
+        raise ValueError(f"target is on {target.device}, the student on {dev}")
+    return target.reshape(-1, 1)
 
 
 class _Linear(torch.autograd.Function):
@@ -389,12 +420,7 @@ def linear_cross_entropy(hidden, weight, target, *, ignore_index: int = -100, re
         if loss is not None:
             return loss
     hidden, weight, shape = _layer(hidden, weight)
-    _cuda("target", target, (torch.int32, torch.int64))
-    if target.shape != shape:
-        raise ValueError(f"target must have shape {tuple(shape)}, got {tuple(target.shape)}")
-    if target.device != hidden.device:
-        raise ValueError(f"target is on {target.device}, hidden on {hidden.device}")
-    target = target.reshape(-1, 1)
+    target = _target(target, shape, hidden.device)
     loss = _linear(hidden, weight, None, target, 1.0, int(ignore_index), _reduction(reduction))
     return loss.view(shape) if reduction == "none" and len(shape) != 1 else loss
 

@@ -82,6 +82,11 @@ class RandomForestClassifier(_ForestModel):
             X, threshold=threshold)
         return self.classes_[_to_numpy(idx).astype(np.int64)]
 
+    def predict_top(self, X, k):
+        """The k most probable labels of each row: (probabilities, labels), both (n_rows, k)."""
+        values, idx = self._inference_model().predict_top(X, k)
+        return values, self.classes_[_to_numpy(idx).astype(np.int64)]
+
     def score(self, X, y, **kw):
         return float(np.mean(self.predict(X, **kw) == np.asarray(y)))
 

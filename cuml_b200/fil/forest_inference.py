@@ -279,14 +279,16 @@ class ForestInference:
             return ((n, nt, k) if self._vec else (n, nt)), dt
         return (n, k), dt
 
-    def _run(self, X, kind: int, chunk_size: Optional[int], threshold: float = 0.5, preds=None):
+    def _run(self, X, kind: int, chunk_size: Optional[int], threshold: float = 0.5, preds=None,
+             output_type: Optional[str] = None):
         f = self.forest
+        want = output_type or self.output_type
         cs = int(chunk_size or self.default_chunk_size or 0)
         if cs and (cs < 1 or cs & (cs - 1)):
             raise ValueError("chunk_size must be a positive power of two")
         # CUDA tensors that need no conversion: one native call (None: not such a call)
         call = f._device_call
-        if call and self.output_type != "numpy":
+        if call and want != "numpy":
             out = call(X, preds, kind, cs, threshold)
             if out is not None:
                 if type(out) is int:
@@ -313,7 +315,6 @@ class ForestInference:
             raise ValueError(f"X must have shape (n_rows, {self._nf}), got {tuple(X.shape)}")
         n = int(X.shape[0])
         shape, odt = self._out_spec(kind, n)
-        want = self.output_type
         if is_torch and X.is_cuda:
             # device path: cast / make row-major like check_inputs(order="C") of the reference
             # (python/cuml/cuml/ensemble/randomforestclassifier.py:330-336)
@@ -384,6 +385,74 @@ class ForestInference:
             return res.astype(np.int32) if isinstance(res, np.ndarray) else res.to(_torch().int32)
         return self._run(X, INFER_CLASS, chunk_size,
                          threshold=0.5 if threshold is None else float(threshold), preds=preds)
+
+    def _proba_on_device(self, X, chunk_size: Optional[int]):
+        """Class probabilities as a CUDA tensor, whatever kind of array X is, and whether X was one."""
+        if not self.is_classifier:
+            raise RuntimeError("class probabilities are only available for classifiers")
+        torch = _torch()
+        kind = INFER_PROBA2 if self.n_outputs == 1 else INFER_DEFAULT
+        proba = self._run(X, kind, chunk_size, output_type="torch")
+        on_device = proba.is_cuda
+        return (proba if on_device else proba.to(f"cuda:{self._dev}")), on_device
+
+    def predict_top(self, X, k: int, *, chunk_size: Optional[int] = None):
+        """The `k` most probable classes of each row: (probabilities, classes), both (n_rows, k), in
+        descending order, equal ones in the order of their classes; 1 <= k <= min(n_classes, 256).
+        The arrays are of the kind that `predict_proba` returns; classes are int32."""
+        from .. import distill
+
+        proba, on_device = self._proba_on_device(X, chunk_size)
+        values, index, _ = distill.top_scores(proba, k)
+        if self.output_type == "numpy" or (self.output_type == "input" and not on_device and
+                                           not isinstance(X, _torch().Tensor)):
+            return values.cpu().numpy(), index.cpu().numpy()
+        return (values, index) if on_device else (values.cpu(), index.cpu())
+
+    def teach(self, X, k: int, *, temperature: float = 1.0, chunk_size: Optional[int] = None):
+        """What a student is trained on: the `k` most probable classes of each row as `TopScores`
+        (CUDA tensors) with the logarithms of their probabilities as scores, and log sum_c p_c^(1 / T)
+        over all classes as `logsumexp`.  `cuml_b200.distill`'s losses take it as it is."""
+        from .. import distill
+
+        return distill.top_scores(self._proba_on_device(X, chunk_size)[0], k, temperature=temperature,
+                                  probabilities=True)
+
+    def distillation_loss(self, X, logits=None, *, hidden=None, weight=None, k: int = 8,
+                          temperature: float = 1.0, tail: str = "renormalise", labels=None,
+                          label_weight: float = 0.5, reduction: str = "mean",
+                          chunk_size: Optional[int] = None):
+        """Loss of a student on the rows X with this forest as its teacher, and with `labels` (n_rows,)
+        (1 - label_weight) of it plus label_weight of the cross entropy.
+
+        The student's side is `logits` (n_rows, n_classes), or `hidden` (n_rows, width) and `weight`
+        (n_classes, width) of its last linear layer, whose logits are then not kept (bf16 or fp16).
+        k (at most n_classes are taken), temperature, tail, reduction : as in
+        `cuml_b200.distill.distillation_loss`; tail='bucket' needs `logits`.  The loss has gradients by
+        the student's tensors."""
+        from .. import distill
+
+        linear = hidden is not None or weight is not None
+        if linear == (logits is not None) or linear and (hidden is None or weight is None):
+            raise ValueError("give the student's logits, or hidden and weight of its last layer")
+        if linear and tail != "renormalise":
+            raise ValueError("tail='bucket' needs the student's logits")
+        n_classes = 2 if self.n_outputs == 1 else self.n_outputs
+        wide = weight.shape[0] if linear else logits.shape[-1]
+        if wide != n_classes:
+            raise ValueError(f"the student has {wide} classes, the forest {n_classes}")
+        top = self.teach(X, min(int(k), n_classes), temperature=temperature, chunk_size=chunk_size)
+        if linear:
+            loss = distill.linear_distillation_loss(hidden, weight, top, temperature=temperature, reduction=reduction)
+        else:
+            loss = distill.distillation_loss(logits, top, temperature=temperature, tail=tail, reduction=reduction)
+        if labels is None:
+            return loss
+        if linear:
+            hard = distill.linear_cross_entropy(hidden, weight, labels, reduction=reduction)
+        else:
+            hard = distill.cross_entropy(logits, labels, reduction=reduction)
+        return (1 - label_weight) * loss + label_weight * hard
 
     def predict_per_tree(self, X, *, preds=None, chunk_size: Optional[int] = None):
         """Raw output of every tree: (n_rows, n_trees) or (n_rows, n_trees, n_classes)

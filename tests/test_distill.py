@@ -437,3 +437,34 @@ def test_autograd_rules(monkeypatch, compiled):
         a = torch.autograd.grad(rows, leaves, up, retain_graph=True)
         b = torch.autograd.grad(rows, leaves, up.contiguous())
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@gpu
+@pytest.mark.parametrize("compiled", [True, False])
+@pytest.mark.parametrize("n,c", [(1, 2), (64, 10), (33, 1001), (5, 5000)])
+def test_cross_entropy(monkeypatch, compiled, n, c):
+    from cuml_b200 import distill
+
+    if not compiled:
+        monkeypatch.setattr(distill, "_call", False)
+    z = (torch.randn((n, c), generator=gen(c), device="cuda") * 2).requires_grad_()
+    target = torch.randint(0, c, (n,), generator=gen(n), device="cuda")
+    if n > 4:
+        target[1], target[2], target[3] = -100, c, -1
+    rows, grad, counts = ref.loss(z, None, target[:, None])
+    for reduction in ("mean", "sum", "none"):
+        want, factor = ref.reduced(rows, counts, reduction)
+        loss = distill.cross_entropy(z, target, reduction=reduction)
+        check_values(loss, want, 4 * U, 3 * S * (n if reduction == "sum" else 1), U)
+        (g,) = torch.autograd.grad(loss, z, torch.ones_like(loss))
+        check_values(g, grad * factor, 4 * S, 4 * S * factor, U)
+    assert torch.equal(distill.cross_entropy(z, target.int(), ignore_index=0, reduction="none"),
+                       distill.cross_entropy(z, torch.where(target == 0, -5, target), reduction="none"))
+    cube = z.detach().reshape(n, 1, c)
+    assert torch.equal(distill.cross_entropy(cube, target[:, None], reduction="none")[:, 0],
+                       distill.cross_entropy(z, target, reduction="none"))
+    for bad, text in ((target[:0], "target must have shape"), (target.float(), "target must be one of"), (target.cpu(), "CUDA")):
+        with pytest.raises(ValueError, match=text):
+            distill.cross_entropy(z, bad)
+    with pytest.raises(ValueError, match="reduction"):
+        distill.cross_entropy(z, target, reduction="max")
