@@ -10,7 +10,8 @@
 // price of not keeping it; kept in 16 bits it would be written once and read twice, and its rounding would
 // be in q.  d is rounded to the layer's own 16 bits because both operands of a matrix instruction have
 // one type: half a step of each d, independent of each other, where the gradient's own rounding
-// is as much again.  For fp16 d is scaled by 2^14, so that probabilities down to 4e-9 are normal
+// is as much again.  Where products are so small that they hardly count, d is kept as two numbers of 16 bits
+// (two planes), and the sums run over both.  For fp16 d is scaled by 2^14, so that probabilities down to 4e-9 are normal
 // numbers.  Sums over classes and rows are in 32 bits; a sum over several pieces stays in 32 bits.
 //
 // One kernel does all products: a cluster of two CTAs takes 256 x 256 of the output
@@ -40,6 +41,10 @@ constexpr int kSmem    = kStages * kStage + 1024 + 256;
 constexpr long long kPatience = 2000000000ll;  // ns
 constexpr int64_t kPieceBytes = 256ll << 20;   // of d (8192 x 2048 x 131,072, gradient: 12.8 ms with 64 MB, 10.7 with 256)
 constexpr int kMostSplits     = 16;
+// Rows x classes x width up to which d has two planes (2048 x 512 x 1000: the errors of the gradients against
+// 64 bits are 1.4 times those of their own rounding with one plane and 1.0 with two, which takes 5 us of
+// 31; with two classes one plane made them up to twice as large).
+constexpr int64_t kSmallProduct = 1ll << 32;
 constexpr int kGroup          = 32;            // tiles of rows whose part of H stays in L2 while all of W passes
 constexpr float kHalfScale    = 16384.f;       // of d in fp16
 // Named classes of a row that the epilogue looks through for each tile; more are put into d by a kernel of their
@@ -184,6 +189,7 @@ struct Product {
   CUtensorMap a, b;
   int m, n, depth;
   int m_tiles, n_tiles, splits;  // splits: parts of the depth, each with sums of its own
+  int planes, plane_rows;        // the depth is passed once for each plane of A, which are plane_rows rows apart
   int a_outer, b_outer;
   int n_first;  // order of the tiles: all of a row of tiles, else kGroup of a column
   // kGrad: rows of n elements; 32-bit sums, one matrix per split, to which `add` adds, or 16-bit results
@@ -211,6 +217,7 @@ struct Work {
   void* diff;
   int64_t diff_stride;
   float diff_scale;
+  int planes, plane_rows;
   Named named;
   int k, first;
   Scale scale;            // kGrad
@@ -238,7 +245,7 @@ __device__ __forceinline__ bool tile_of(const Work& w, int t, Tile& r)
         r.m = first + t % rows;
         r.n = t / rows;
       }
-      const int steps = (p.depth + kDepth - 1) / kDepth;
+      const int steps = (p.depth + kDepth - 1) / kDepth * p.planes;
       r.begin         = static_cast<int>(static_cast<int64_t>(steps) * r.split / p.splits);
       r.end           = static_cast<int>(static_cast<int64_t>(steps) * (r.split + 1) / p.splits);
       return true;
@@ -261,6 +268,12 @@ __device__ __forceinline__ uint32_t two(float lo, float hi, bool bf16)
   else
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// What rounding x to 16 bits leaves.
+__device__ __forceinline__ float left_of(float x, bool bf16)
+{
+  return bf16 ? x - __bfloat162float(__float2bfloat16_rn(x)) : x - __half2float(__float2half_rn(x));
 }
 
 // Part of a row (32 columns from `col` on) of a finished tile.  n: columns of the result.
@@ -292,13 +305,18 @@ __device__ __forceinline__ void take_columns(const Work& w, const Product& p, in
 #pragma unroll
       for (int i = 0; i < 32; ++i) x[i] = 0.f;
     }
-    char* to = static_cast<char*>(w.diff) + (row * w.diff_stride + col) * 2;
+    for (int plane = 0;;) {
+      char* to = static_cast<char*>(w.diff) + ((plane * static_cast<int64_t>(w.plane_rows) + row) * w.diff_stride + col) * 2;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t v[8];
+      for (int h = 0; h < 2; ++h) {
+        uint32_t v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = two(x[16 * h + 2 * i], x[16 * h + 2 * i + 1], w.bf16);
-      store32(to + 32 * h, v);
+        for (int i = 0; i < 8; ++i) v[i] = two(x[16 * h + 2 * i], x[16 * h + 2 * i + 1], w.bf16);
+        store32(to + 32 * h, v);
+      }
+      if (++plane == w.planes) break;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) x[i] = left_of(x[i], w.bf16);
     }
     return;
   }
@@ -395,6 +413,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
     for (int i = cluster; ok && tile_of(w, i, t); ok = ok && next_tile(i)) {
       const Product& p = w.product[t.which];
       const int m0 = t.m * kTile + rank * kHalf, n0 = t.n * kTile + rank * kHalf;
+      const int steps = (p.depth + kDepth - 1) / kDepth;
+      int plane = t.begin / steps, at = t.begin % steps;  // step of the plane
       for (int k = t.begin; k < t.end; ++k) {
         if (!warp_wait(empty + 8 * stage, phase ^ 1, &gave_up)) {
           ok = false;
@@ -403,20 +423,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
         const uint32_t a = ring + stage * kStage, b = a + kStageA, bar = count_at + 8 * stage;
         if (elected()) {
           if (rank == 0) bar_expect(full + 8 * stage, 2 * kStage);
+          const int x = at * kDepth, y = plane * p.plane_rows;
           if (p.a_outer) {
-            load_box(a, &p.a, bar, m0, k * kDepth);
-            load_box(a + 8192, &p.a, bar, m0 + 64, k * kDepth);
+            load_box(a, &p.a, bar, m0, y + x);
+            load_box(a + 8192, &p.a, bar, m0 + 64, y + x);
           } else {
-            load_box(a, &p.a, bar, k * kDepth, m0);
+            load_box(a, &p.a, bar, x, y + m0);
           }
           if (p.b_outer) {
-            load_box(b, &p.b, bar, n0, k * kDepth);
-            load_box(b + 8192, &p.b, bar, n0 + 64, k * kDepth);
+            load_box(b, &p.b, bar, n0, x);
+            load_box(b + 8192, &p.b, bar, n0 + 64, x);
           } else {
-            load_box(b, &p.b, bar, k * kDepth, n0);
+            load_box(b, &p.b, bar, x, n0);
           }
         }
         __syncwarp();
+        if (++at == steps) {
+          at = 0;
+          ++plane;
+        }
         ++issued;
         if (++stage == kStages) {
           stage = 0;
@@ -497,10 +522,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
     for (int i = cluster; ok && tile_of(w, i, t); ok = next_tile(i)) {
       const Product& p  = w.product[t.which];
       const int64_t row = static_cast<int64_t>(t.m) * kTile + rank * kHalf + quarter * 32 + lane;
-      const bool in     = row < p.m;
+      const bool in     = row < (KIND == kDiff ? w.plane_rows : p.m);
       float base = 0.f, factor = 1.f;
-      if (KIND == kDiff && in) {
-        const float4 s = w.stats[row];
+      if (KIND == kDiff && in) {  // (rows up to a plane's end are zeros: they meet zeros, but not as NaN)
+        const float4 s = row < p.m ? w.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
         base           = base_of(s.x);
         factor         = s.w == 0.f ? 0.f : s.y * w.diff_scale * (w.row_scale ? w.row_scale[row] : 1.f);
       }
@@ -527,9 +552,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
           const int64_t e = row * w.k + j;
           const int at    = w.named.at[e] - w.first;
           if (at < low || at >= high) continue;
-          const float d = (power((w.named.logit[e] - base) * w.c) * inv - w.named.p[e]) * per;
-          char* to      = static_cast<char*>(w.diff) + (row * w.diff_stride + at) * 2;
-          *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(two(d, 0.f, w.bf16));
+          float d  = (power((w.named.logit[e] - base) * w.c) * inv - w.named.p[e]) * per;
+          char* to = static_cast<char*>(w.diff) + (row * w.diff_stride + at) * 2;
+          for (int plane = 0; plane < w.planes; ++plane, d = left_of(d, w.bf16), to += w.plane_rows * w.diff_stride * 2)
+            *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(two(d, 0.f, w.bf16));
         }
       }
       if (KIND == kStats && in) w.parts[(row * p.n_tiles + t.n) * 2 + (from != 0)] = make_float2(r.m, r.s);
@@ -674,8 +700,9 @@ __global__ void __launch_bounds__(kThreads) named_diff(Work w, int64_t entries, 
     const float4 s    = w.stats[row];
     if (s.w == 0.f) continue;
     const float q = power((w.named.logit[i] - base_of(s.x)) * w.c) * s.y;
-    static_cast<T*>(w.diff)[row * w.diff_stride + at] =
-      narrow<T>((q - w.named.p[i]) * w.diff_scale * (w.row_scale ? w.row_scale[row] : 1.f));
+    float d       = (q - w.named.p[i]) * w.diff_scale * (w.row_scale ? w.row_scale[row] : 1.f);
+    for (int plane = 0; plane < w.planes; ++plane, d -= widen(narrow<T>(d)))
+      static_cast<T*>(w.diff)[(plane * static_cast<int64_t>(w.plane_rows) + row) * w.diff_stride + at] = narrow<T>(d);
   }
 }
 
@@ -756,7 +783,8 @@ bool logits_product(Product& p, bool bf16, const LinearArgs& a, int64_t first, i
   p.depth   = static_cast<int>(a.width);
   p.m_tiles = tiles_of(p.m);
   p.n_tiles = tiles_of(p.n);
-  p.splits  = 1;
+  p.splits = p.planes = 1;
+  p.plane_rows = 0;
   p.a_outer = p.b_outer = 0;
   p.n_first = 0;
   return make_map(&p.a, bf16, a.hidden, a.n_rows, a.width, a.hidden_stride, kHalf) &&
@@ -799,6 +827,8 @@ cudaError_t run_linear(bool bf16, const LinearArgs& a, const Reduced& out, void*
 struct Plan {
   int pieces;
   int64_t cols;                 // of a piece, a multiple of a tile
+  int planes;                   // of d
+  int64_t plane_rows;
   int splits_hidden, splits_weight;
   bool sums_hidden, sums_weight;  // in memory
 };
@@ -811,9 +841,11 @@ Plan plan_of(const LinearGradArgs& g, int n_sms)
   p.pieces = static_cast<int>((a.n_cols + most - 1) / most);
   p.cols   = static_cast<int64_t>(tiles_of((a.n_cols + p.pieces - 1) / p.pieces)) * kTile;
   p.pieces = static_cast<int>((a.n_cols + p.cols - 1) / p.cols);
+  p.planes     = a.n_rows * a.n_cols <= kSmallProduct / a.width ? 2 : 1;
+  p.plane_rows = (a.n_rows + kDepth - 1) / kDepth * kDepth;
   // as many parts as bring a part down to an even share of the machine, 16 stages at least
   const int64_t wide = tiles_of(a.width), dh_tiles = tiles_of(a.n_rows) * wide, dw_tiles = tiles_of(p.cols) * wide;
-  const int64_t dh_steps = p.cols / kDepth, dw_steps = (a.n_rows + kDepth - 1) / kDepth;
+  const int64_t dh_steps = p.planes * (p.cols / kDepth), dw_steps = p.planes * (p.plane_rows / kDepth);
   int64_t share = ((g.grad_hidden ? dh_tiles * dh_steps : 0) + (g.grad_weight ? dw_tiles * dw_steps : 0)) / (n_sms / 2);
   if (share < 16) share = 16;
   auto parts = [&](int64_t steps) {
@@ -847,7 +879,7 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
   int* ticket          = reinterpret_cast<int*>(at + 16);
   float* row_scale     = reinterpret_cast<float*>(at += 256);
   T* diff              = reinterpret_cast<T*>(at += padded(a.n_rows * 4));
-  float* sums_hidden   = reinterpret_cast<float*>(at += padded(a.n_rows * plan.cols * 2));
+  float* sums_hidden   = reinterpret_cast<float*>(at += padded(plan.planes * plan.plane_rows * plan.cols * 2));
   float* sums_weight   = reinterpret_cast<float*>(at + (plan.sums_hidden ? plan.splits_hidden * a.n_rows * a.width * 4 : 0));
   const float d_scale  = bf16 ? 1.f : kHalfScale;
   const bool per_row   = g.factor == nullptr;
@@ -862,6 +894,8 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
   w.diff        = diff;
   w.diff_stride = plan.cols;
   w.diff_scale  = d_scale;
+  w.planes      = plan.planes;
+  w.plane_rows  = static_cast<int>(plan.plane_rows);
   w.scale       = Scale{per_row ? scale : g.upstream, g.factor, a.temperature / d_scale};
   w.named       = a.named;
   w.k           = a.teacher.k;
@@ -892,7 +926,7 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
       p.sums     = plan.sums_hidden ? sums_hidden : nullptr;
       p.add      = i > 0;
       p.out      = g.grad_hidden;
-      return make_map(&p.a, bf16, diff, a.n_rows, made, plan.cols, kHalf) &&
+      return make_map(&p.a, bf16, diff, plan.planes * plan.plane_rows, made, plan.cols, kHalf) &&
              make_map(&p.b, bf16, weight, n, a.width, a.weight_stride, 64);
     };
     auto of_weight = [&] {
@@ -905,7 +939,7 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
       p.sums     = plan.sums_weight ? sums_weight : nullptr;
       p.add      = 0;
       p.out      = grad_weight;
-      return make_map(&p.a, bf16, diff, a.n_rows, made, plan.cols, 64) &&
+      return make_map(&p.a, bf16, diff, plan.planes * plan.plane_rows, made, plan.cols, 64) &&
              make_map(&p.b, bf16, a.hidden, a.n_rows, a.width, a.hidden_stride, 64);
     };
     // the longer sums first: what is left at the end is short
@@ -917,6 +951,8 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
       p.b_outer  = 1;
       p.m_tiles  = tiles_of(p.m);
       p.n_tiles  = tiles_of(p.n);
+      p.planes     = plan.planes;
+      p.plane_rows = static_cast<int>(plan.plane_rows);
       p.n_first  = 1;  // d is read once, by all the tiles of a row of them at the same time
     }
     if ((e = run_products<kGrad>(w, n_sms, s)) != cudaSuccess) return e;
@@ -945,7 +981,7 @@ size_t linear_grad_workspace(const LinearGradArgs& g, int n_sms)
 {
   const LinearArgs& a = g.fwd;
   const Plan p        = plan_of(g, n_sms);
-  return 256 + padded(a.n_rows * 4) + padded(a.n_rows * p.cols * 2) +
+  return 256 + padded(a.n_rows * 4) + padded(p.planes * p.plane_rows * p.cols * 2) +
          (p.sums_hidden ? p.splits_hidden * a.n_rows * a.width * sizeof(float) : 0) +
          (p.sums_weight ? p.splits_weight * p.cols * a.width * sizeof(float) : 0);
 }

@@ -4,14 +4,14 @@
 // Every score gets a key that no other of its row has: its value as an ordered integer, then the
 // complement of its class.  NaN is above everything, -0 equals +0.
 //
-// A row is taken by a block, or where it is short by a warp, whose threads see one group of its elements
-// each.  A bound tau that at least k, and hardly more, of the groups' best keys reach is found bit by bit
-// (a vote per bit, until few too many are left); at least k elements reach it, and all that do lie in
-// those groups: only these are read again, from L1 or L2, dealt out anew to all threads.  Random rows
-// leave little more than k candidates whatever the row's length; each finds its place by counting the larger
-// ones.  Where there are more than the list holds, the k-th key itself is found bit by bit.  Rows of a
-// few classes are taken by one thread each, from a tile in shared memory, which keeps its best sorted in
-// registers.
+// Rows above kWarpCols are taken by a block, whose threads see one group of elements each.  A bound tau that at
+// least k, and hardly more, of the groups' best keys reach is found bit by bit (one warp counts, until few
+// too many are left); at least k elements reach it, and all that do lie in those groups: only these are read
+// again, from L1 or L2, dealt out anew to all threads.  Random rows leave little more than k candidates whatever
+// the row's length; each finds its place by counting the larger ones.  Where there are more than the list
+// holds, the k-th key itself is found bit by bit.  Shorter rows stay in the registers of a warp, which
+// finds its bound by votes on all of them.  Rows of a few classes are taken by one thread each, from a tile in
+// shared memory, which keeps its best sorted in registers.
 //
 // Bound by memory: one pass over the scores, which also takes the running maximum and sum of the
 // log-sum-exp.  Of a thread's best score that pass keeps the value and the 16 bytes that hold it; the keys of
@@ -25,14 +25,20 @@ namespace {
 
 constexpr int kThreads  = 256;   // groups of a block: at least the largest k
 constexpr int kList     = 2048;  // candidates of a block
-constexpr int kWarpList = 256;   // candidates of a warp
-constexpr int kWarpCols = 1024;  // longest rows and largest k that a warp takes
-constexpr int kWarpTop  = 24;
+constexpr int kWarpList = 320;   // candidates of a warp: at least the largest k
+constexpr int kWarpCols = 1024;  // longest rows of a warp (fp64: 512)
+constexpr int kFew      = 32;    // candidates that a warp places in one go
+constexpr int kCount    = 160;   // candidates of a block that are placed by counting; more are sorted
 constexpr int kMore     = 8;     // groups more than k that end the search of the bound
 constexpr int kInFlight = 4;
-constexpr int kTileRows = 128;   // rows of a tile for one thread each, their most classes and k
-constexpr int kTileCols = 48;
-constexpr int kTileTop  = 8;
+// Rows for one thread each: tiles of kTileRows.  A thread takes some 5 k instructions per score, a warp with a row
+// 20 per score and lane and 300 more: many short rows are a thread's (200,000 x 64 fp32, k 4: 155 us by
+// warps), few or long ones a warp's, since a thread's steps follow one another.
+constexpr int kTileRows  = 128;
+constexpr int kTileBytes = 512;  // of a row
+constexpr int kTileTop   = 32;   // largest k, and most classes where k is above 8
+constexpr int kTileSteps = 160;  // classes x (k + 1) that a thread takes however few rows there are
+constexpr int kTileLeast = 32;   // rows per SM from which on threads take the others
 constexpr int kTileFlight = 4;
 static_assert(kThreads >= kMostTop, "a group per entry");
 
@@ -203,7 +209,7 @@ struct RowShared {
   int found, chosen;
 };
 
-// A segment of a row per block or warp.  segs == 1: the row's answer; else its k best keys and its sum.
+// A segment of a row per block.  segs == 1: the row's answer; else its k best keys and its sum.
 template <class T, int THREADS, bool PROB>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments(TopArgs a, int segs, int64_t seg_cols,
                                                          typename KeyOf<T>::type* keys, double* sums)
@@ -211,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
   using V = typename ValueOf<T>::type;
   using K = typename KeyOf<T>::type;
   constexpr int ROWS = kThreads / THREADS, N = Piece<T>::N;
-  constexpr int LIST = THREADS == 32 ? kWarpList : kList;
+  constexpr int LIST = kList;
   __shared__ RowShared<K, LIST, THREADS> shared[ROWS];
   __shared__ double room[64];
   const int slot = threadIdx.x / THREADS, tid = threadIdx.x % THREADS;
@@ -372,18 +378,30 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
     }
     // a candidate's place is the number of larger ones
     const int64_t part = row * segs + seg;
-    for (int i = tid; i < got; i += THREADS) {
-      const K key = mine.list[i];
-      int place   = 0;
-#pragma unroll 4
-      for (int j = 0; j < got; ++j) place += mine.list[j].above(key);
-      if (place >= k) continue;
+    auto put           = [&](int place, const K& key) {
+      if (place >= k) return;
       if (segs == 1) {
         write_top<T>(a, row, place, key);
         if (place == 0) write_lse(a, row, all.m, all.s, dropped, key);
       } else {
         keys[part * a.k + place] = key;
       }
+    };
+    if (got <= kCount) {
+      if (tid < got) {
+        const K key = mine.list[tid];
+        int place   = 0;
+#pragma unroll 4
+        for (int j = 0; j < got; ++j) place += mine.list[j].above(key);
+        put(place, key);
+      }
+    } else {
+      int size = 256;
+      while (size < got) size <<= 1;
+      for (int i = got + tid; i < size; i += THREADS) mine.list[i] = K::none();
+      __syncthreads();
+      sort_list(mine.list, size);
+      if (tid < k) put(tid, mine.list[tid]);
     }
     if (segs > 1) {
       for (int j = k + tid; j < a.k; j += THREADS) keys[part * a.k + j] = K::none();
@@ -396,7 +414,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
   }
 }
 
-// Joins the segments' lists of a row: as many as fit are sorted with the best so far.
+// Joins the segments' sorted lists of a row.  With r = k / segs rounded up, at least k keys reach the least of the
+// lists' r-th keys: these alone are sorted, where they fit; else as many as fit with the best so far.
 template <class T>
 __global__ void __launch_bounds__(kThreads) top_join(TopArgs a, int segs, const typename KeyOf<T>::type* keys,
                                                      const double* sums)
@@ -405,19 +424,43 @@ __global__ void __launch_bounds__(kThreads) top_join(TopArgs a, int segs, const 
   using K = typename KeyOf<T>::type;
   __shared__ K list[kList];
   __shared__ double room[64];
+  __shared__ int found;
   for (int64_t row = blockIdx.x; row < a.n_rows; row += gridDim.x) {
     const K* from = keys + row * segs * a.k;
-    const int all = segs * a.k;
-    int have      = 0;
-    for (int i = 0; i < all;) {
-      const int more = min(all - i, kList - have);
-      int size       = 1;
-      while (size < have + more) size <<= 1;
-      for (int j = threadIdx.x; j < size - have; j += kThreads) list[have + j] = j < more ? from[i + j] : K::none();
+    const int all = segs * a.k, r_th = (a.k + segs - 1) / segs - 1;
+    if (threadIdx.x == 0) found = 0;
+    __syncthreads();
+    K bound = K::of(static_cast<V>(NAN), 0u);  // nothing is above
+    for (int i = 0; i < segs; ++i) {
+      const K key = from[i * a.k + r_th];
+      if (bound.above(key)) bound = key;
+    }
+    for (int i = threadIdx.x; i < all; i += kThreads) {
+      const K key = from[i];
+      if (bound.above(key)) continue;
+      const int to = atomicAdd(&found, 1);
+      if (to < kList) list[to] = key;
+    }
+    __syncthreads();
+    const int got = found;
+    if (got <= kList) {
+      int size = 1;
+      while (size < got) size <<= 1;
+      for (int i = got + threadIdx.x; i < size; i += kThreads) list[i] = K::none();
       __syncthreads();
       sort_list(list, size);
-      i += more;
-      have = min(a.k, have + more);
+    } else {
+      int have = 0;
+      for (int i = 0; i < all;) {
+        const int more = min(all - i, kList - have);
+        int size       = 1;
+        while (size < have + more) size <<= 1;
+        for (int j = threadIdx.x; j < size - have; j += kThreads) list[have + j] = j < more ? from[i + j] : K::none();
+        __syncthreads();
+        sort_list(list, size);
+        i += more;
+        have = min(a.k, have + more);
+      }
     }
     for (int j = threadIdx.x; j < a.k; j += kThreads) write_top<T>(a, row, j, list[j]);
     Running<double> r;
@@ -447,7 +490,176 @@ struct Ordered<double> {
   using type = uint64_t;
 };
 
-// A row per thread: n_cols <= kTileCols, k <= TOP.
+__device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint64_t max_of(uint64_t a, uint64_t b) { return a > b ? a : b; }
+
+// A row per warp, in registers.  Short rows: every 32nd element is a lane's, S of them.  Longer ones: U pieces of
+// 16 bytes and at most one element from before the first or behind the last boundary per lane, and S is 0.
+template <class T, int U, int S, bool PROB>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 2 : 4) top_warps(TopArgs a)
+{
+  using V = typename ValueOf<T>::type;
+  using K = typename KeyOf<T>::type;
+  using O = typename Ordered<V>::type;
+  constexpr int N = Piece<T>::N, E = S ? S : U * N + 1, ROWS = kThreads / 32, kBits = sizeof(O) * 8;
+  __shared__ K lists[ROWS][kWarpList];
+  const int lane = threadIdx.x % 32, n = static_cast<int>(a.n_cols), k = a.k;
+  K* list          = lists[threadIdx.x / 32];
+  const V c        = static_cast<V>(1.4426950408889634 * a.inv_temperature);
+  const bool plain = a.inv_temperature == 1.0;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / 32; row < a.n_rows;
+       row += static_cast<int64_t>(gridDim.x) * ROWS) {
+    const T* x       = static_cast<const T*>(a.scores) + row * a.row_stride;
+    const int lead   = S ? 0 : lead_of(x, n), pieces = S ? 0 : (n - lead) / N;
+    // the odd element: the first lanes' before, the last lanes' behind the pieces
+    const int behind = lead + pieces * N + 31 - lane;
+    const int odd    = lane < lead ? lane : behind < n ? behind : -1;
+    auto place_of    = [&](int e) { return S ? lane + 32 * e : e == E - 1 ? odd : lead + (lane + 32 * (e / N)) * N + e % N; };
+    auto is_there    = [&](int e) { return S ? lane + 32 * e < n : e == E - 1 ? odd >= 0 : lane + 32 * (e / N) < pieces; };
+    V v[E], top = lowest<V>();
+    if constexpr (S > 0) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = lane + 32 * e < n ? widen(x[lane + 32 * e]) : lowest<V>();
+    } else {
+      const T* body = x + lead;
+      Piece<T> w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (lane + 32 * u < pieces) w[u] = load_piece(body + (lane + 32 * u) * N);
+      v[E - 1] = odd >= 0 ? widen(x[odd]) : lowest<V>();
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[u * N + e] = lane + 32 * u < pieces ? widen(w[u].v[e]) : lowest<V>();
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) top = larger(top, v[e]);
+    const V most = top;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = larger(top, __shfl_xor_sync(~0u, top, d));
+    // the sum (what is not there is -inf and adds nothing to a sum of powers)
+    Sum<V, PROB> sum;
+    sum.reach(top, c);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (!PROB || is_there(e)) sum.add(v[e], c, plain);
+    V s            = sum.s;
+    double dropped = 0;
+    if (PROB) {
+      dropped = sum_lanes(static_cast<double>(sum.s) + sum.dropped);
+      s       = V(0);
+    } else {
+      s = sum_lanes(s);
+    }
+    int got = 0;
+    const bool nan = PROB ? dropped != dropped : s != s;
+    // Few of many: a bound that at least k lanes' best reach, a ballot per bit.
+    bool done = false;
+    if (k <= kFew - 8 && (S ? E > 2 : pieces >= kFew) && !nan) {
+      const O best = ordered(most);
+      O tau        = 0;
+      for (int bit = kBits - 1; bit >= 0; --bit) {
+        const O next   = tau | O(1) << bit;
+        const int some = __popc(__ballot_sync(~0u, best >= next));
+        if (some < k) continue;
+        tau = next;
+        if (some <= k + 2) break;
+      }
+      const V least = tau > ordered(lowest<V>()) ? from_ordered(tau) : lowest<V>();
+      // the lane's hits, then its part of the list
+      uint64_t hits = 0;
+      if (least > lowest<V>()) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) hits |= v[e] >= least ? 1ull << e : 0ull;
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) hits |= is_there(e) ? 1ull << e : 0ull;
+      }
+      const int mine = __popcll(hits);
+      int to         = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(~0u, to, d);
+        if (lane >= d) to += o;
+      }
+      got  = __shfl_sync(~0u, to, 31);
+      done = got <= kWarpList;
+      if (done) {
+        to -= mine;
+        for (; hits; hits &= hits - 1) {
+          const int at = place_of(__ffsll(hits) - 1);
+          list[to++]   = K::of(widen(x[at]), static_cast<uint32_t>(at));
+        }
+      }
+    }
+    if (!done) {
+      // All elements as ordered integers (0: not there); tau: a value that k of them reach and, unless equal ones are
+      // among them, hardly more.
+      O o[E], tau = 1;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = is_there(e) ? ordered(v[e]) : O(0);
+      auto reached = [&](O by) {
+        int some = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) some += o[e] >= by;
+        return static_cast<int>(__reduce_add_sync(~0u, some));
+      };
+      int some = n;
+      if (n > k + kMore) {
+        O t = 0;
+        for (int bit = kBits - 1; bit >= 0; --bit) {
+          const O next = t | O(1) << bit;
+          const int up = reached(next);
+          if (up < k) continue;
+          t    = next;
+          some = up;
+          if (some <= k + kMore) break;
+        }
+        tau = max_of(t, O(1));
+      }
+      // equal ones at the bound beyond what the list holds: the first of them only
+      int last = n;
+      if (some > kWarpList) {
+        const int over = tau == ~O(0) ? 0 : reached(tau + 1);
+        int low = 0, high = n - 1;  // the least place up to which k - over of them lie
+        while (low < high) {
+          const int mid = (low + high) / 2;
+          int up        = 0;
+#pragma unroll
+          for (int e = 0; e < E; ++e) up += o[e] == tau && place_of(e) <= mid;
+          if (static_cast<int>(__reduce_add_sync(~0u, up)) >= k - over)
+            high = mid;
+          else
+            low = mid + 1;
+        }
+        last = low;
+      }
+      got = 0;
+      // puts an element of each lane that has one into the list
+      auto push = [&](bool is, int e) {
+        const unsigned all = __ballot_sync(~0u, is);
+        if (all == 0) return;
+        if (is) list[got + __popc(all & ((1u << lane) - 1))] = K::of(from_ordered(o[e]), static_cast<uint32_t>(place_of(e)));
+        got += __popc(all);
+      };
+#pragma unroll
+      for (int e = 0; e < E; ++e) push(o[e] > tau || (o[e] == tau && place_of(e) <= last), e);
+    }
+    __syncwarp();
+    for (int i = lane; i < got; i += 32) {
+      const K key = list[i];
+      int place   = 0;
+#pragma unroll 4
+      for (int j = 0; j < got; ++j) place += list[j].above(key);
+      if (place >= k) continue;
+      write_top<T>(a, row, place, key);
+      if (place == 0) write_lse(a, row, sum.r, s, dropped, key);
+    }
+    __syncwarp();
+  }
+}
+
+// A row per thread: n_cols x sizeof(T) <= kTileBytes, k <= TOP.
 template <class T, int TOP, bool PROB>
 __global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
 {
@@ -462,7 +674,7 @@ __global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
   const V c       = static_cast<V>(1.4426950408889634 * a.inv_temperature);
   const bool plain = a.inv_temperature == 1.0;
   const bool whole = a.row_stride == a.n_cols && (reinterpret_cast<uintptr_t>(a.scores) & 15) == 0 && c_n > 1;
-  // i / c_n = i * inverse / 2^32 for i < 128 x 48 (exact: i * c_n < 2^32)
+  // i / c_n = i * inverse / 2^32 for i < 128 x 512 (exact: i * c_n < 2^32)
   const uint32_t inverse = 0xffffffffu / c_n + 1;
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * kTileRows; first < a.n_rows;
        first += static_cast<int64_t>(gridDim.x) * kTileRows) {
@@ -595,26 +807,39 @@ cudaError_t run_tiles(const TopArgs& a, int n_sms, cudaStream_t s)
   return cudaGetLastError();
 }
 
+template <class T, int U, int S>
+cudaError_t run_warps(const TopArgs& a, int n_sms, cudaStream_t s)
+{
+  const int64_t need = (a.n_rows + kThreads / 32 - 1) / (kThreads / 32), most = 16ll * n_sms;
+  const auto kernel  = a.probabilities ? top_warps<T, U, S, true> : top_warps<T, U, S, false>;
+  kernel<<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(a);
+  count_launches(1);
+  return cudaGetLastError();
+}
+
 template <class T>
 cudaError_t run_top(const TopArgs& a, void* workspace, int n_sms, cudaStream_t s)
 {
   using K = typename KeyOf<T>::type;
-  if (a.n_cols <= kTileCols && a.k <= kTileTop) {
+  const int64_t bytes = a.n_cols * static_cast<int64_t>(sizeof(T));
+  if (a.n_cols <= kTileTop && a.k > 8 && a.n_rows >= kTileLeast * n_sms)
+    return a.k <= 16 ? run_tiles<T, 16>(a, n_sms, s) : run_tiles<T, kTileTop>(a, n_sms, s);
+  if (bytes <= kTileBytes && a.k <= 8 && (a.n_cols * (a.k + 1) <= kTileSteps || a.n_rows >= kTileLeast * n_sms)) {
     switch (a.k) {
       case 1: return run_tiles<T, 1>(a, n_sms, s);
       case 2: return run_tiles<T, 2>(a, n_sms, s);
       case 3: return run_tiles<T, 3>(a, n_sms, s);
       case 4: return run_tiles<T, 4>(a, n_sms, s);
-      default: return run_tiles<T, kTileTop>(a, n_sms, s);
+      default: return run_tiles<T, 8>(a, n_sms, s);
     }
   }
-  if (a.n_cols <= kWarpCols && a.k <= kWarpTop) {
-    const int64_t need = (a.n_rows + kThreads / 32 - 1) / (kThreads / 32), most = 16ll * n_sms;
-    const auto kernel  = a.probabilities ? top_segments<T, 32, true> : top_segments<T, 32, false>;
-    kernel<<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(a, 1, a.n_cols, nullptr, nullptr);
-    count_launches(1);
-    return cudaGetLastError();
-  }
+  if (a.n_cols <= 32) return run_warps<T, 0, 1>(a, n_sms, s);
+  if (a.n_cols <= 64) return run_warps<T, 0, 2>(a, n_sms, s);
+  if (a.n_cols <= 128) return run_warps<T, 0, 4>(a, n_sms, s);
+  if (a.n_cols <= 256) return run_warps<T, 0, 8>(a, n_sms, s);
+  constexpr int kPieces = sizeof(T) == 8 ? 8 : sizeof(T);  // 512 elements
+  if (a.n_cols <= 512) return run_warps<T, kPieces, 0>(a, n_sms, s);
+  if (a.n_cols <= kWarpCols && sizeof(T) < 8) return run_warps<T, 2 * kPieces, 0>(a, n_sms, s);
   int segs           = segments(a.n_rows, a.n_cols, n_sms);
   const int64_t cols = part_cols(a.n_cols, segs);
   segs               = static_cast<int>((a.n_cols + cols - 1) / cols);
