@@ -81,8 +81,8 @@ cudaError_t launch_loss_grad(int dtype, const LossGradArgs& a, int n_sms, cudaSt
 
 // ---- loss on a linear layer's output (distill_linear.cu) -------------------------------------
 struct LinearArgs {
-  const void* hidden;  // (n_rows, width), 16-byte aligned rows, width a multiple of 8
-  const void* weight;  // (n_cols, width), likewise
+  const void* hidden;  // (n_rows, width)
+  const void* weight;  // (n_cols, width)
   int64_t n_rows, n_cols, width, hidden_stride, weight_stride;
   Teacher teacher;     // no logsumexp
   float temperature;

@@ -106,7 +106,7 @@ int check_linear(int dtype, int64_t n_rows, int64_t n_cols, int64_t width, int k
   if (dtype != B2FIL_TYPE_BF16 && dtype != B2FIL_TYPE_F16) return invalid("a linear layer must be bf16 or fp16");
   if (n_rows < 0 || n_rows >= INT32_MAX - 256 || n_cols < 1 || n_cols >= INT32_MAX - 256)
     return invalid("n_rows is not in 0 to 2^31 - 257, or n_cols not in 1 to 2^31 - 257");
-  if (width < 8 || width % 8 || width > (1 << 20)) return invalid("width must be a multiple of 8, 8 to 2^20");
+  if (width < 1 || width > (1 << 20)) return invalid("width must be 1 to 2^20");
   if (k < 1 || k > B2FIL_MOST_TOP) return invalid("the teacher's k must be 1 to 256");
   return B2FIL_OK;
 }
@@ -114,8 +114,7 @@ int check_linear(int dtype, int64_t n_rows, int64_t n_cols, int64_t width, int k
 int check_layer(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride, int64_t n_rows, int64_t width)
 {
   if ((!hidden && n_rows > 0) || !weight) return invalid("NULL buffer");
-  if (!aligned(hidden, 16) || !aligned(weight, 16) || hidden_stride % 8 || weight_stride % 8)
-    return invalid("rows of hidden and weight must start on 16 bytes");
+  if (!aligned(hidden, 2) || !aligned(weight, 2)) return invalid("hidden or weight is not aligned to its elements");
   if (hidden_stride < width || weight_stride < width || hidden_stride > (1ll << 32) || weight_stride > (1ll << 32))
     return invalid("a row stride is smaller than width, or above 2^32");
   return B2FIL_OK;
@@ -247,17 +246,23 @@ int b2fil_distill_loss_grad(int dtype, const void* logits, int64_t n_rows, int64
   return finish("b2fil_distill_loss_grad", launch_loss_grad(dtype, g, sms, static_cast<cudaStream_t>(cuda_stream)));
 }
 
-int64_t b2fil_linear_loss_workspace(int dtype, int64_t n_rows, int64_t n_cols, int64_t width, int k, int device_id)
+int64_t b2fil_linear_loss_workspace(int dtype, const void* hidden, int64_t hidden_stride, const void* weight,
+                                    int64_t weight_stride, int64_t n_rows, int64_t n_cols, int64_t width, int k, int device_id)
 {
   int rc = check_linear(dtype, n_rows, n_cols, width, k);
+  if (rc == B2FIL_OK) rc = check_layer(hidden, hidden_stride, weight, weight_stride, n_rows, width);
   if (rc != B2FIL_OK) return rc;
   const int sms = sms_of(device_id);
   if (sms < 0) return sms;
   LinearArgs a{};
-  a.n_rows    = n_rows;
-  a.n_cols    = n_cols;
-  a.width     = width;
-  a.teacher.k = k;
+  a.hidden        = hidden;
+  a.weight        = weight;
+  a.hidden_stride = hidden_stride;
+  a.weight_stride = weight_stride;
+  a.n_rows        = n_rows;
+  a.n_cols        = n_cols;
+  a.width         = width;
+  a.teacher.k     = k;
   return rounded(linear_workspace(a, sms));
 }
 
@@ -278,7 +283,8 @@ int b2fil_linear_loss(int dtype, const void* hidden, int64_t hidden_stride, cons
   if (n_rows > 0 && (!row_loss || !row_stats || !named_logit || !named_p || !named_at)) return invalid("NULL buffer");
   if (!aligned(row_stats, 16) || !aligned(row_loss, 4) || !aligned(named_logit, 4) || !aligned(named_p, 4) || !aligned(named_at, 4))
     return invalid("a buffer is not aligned");
-  rc = check_workspace(workspace, workspace_bytes, b2fil_linear_loss_workspace(dtype, n_rows, n_cols, width, a.teacher.k, device_id));
+  rc = check_workspace(workspace, workspace_bytes, b2fil_linear_loss_workspace(dtype, hidden, hidden_stride, weight, weight_stride, n_rows, n_cols,
+                                                                             width, a.teacher.k, device_id));
   if (rc != B2FIL_OK) return rc;
   OnDevice on(device_id);
   if (!on.ok) return invalid("device_id cannot be made current");
@@ -297,18 +303,24 @@ int b2fil_linear_loss(int dtype, const void* hidden, int64_t hidden_stride, cons
                                                    sms_of(device_id), static_cast<cudaStream_t>(cuda_stream)));
 }
 
-int64_t b2fil_linear_loss_grad_workspace(int dtype, int64_t n_rows, int64_t n_cols, int64_t width, int k, int wants_hidden,
-                                         int wants_weight, int device_id)
+int64_t b2fil_linear_loss_grad_workspace(int dtype, const void* hidden, int64_t hidden_stride, const void* weight,
+                                         int64_t weight_stride, int64_t n_rows, int64_t n_cols, int64_t width, int k,
+                                         int wants_hidden, int wants_weight, int device_id)
 {
   int rc = check_linear(dtype, n_rows, n_cols, width, k);
+  if (rc == B2FIL_OK) rc = check_layer(hidden, hidden_stride, weight, weight_stride, n_rows, width);
   if (rc != B2FIL_OK) return rc;
   const int sms = sms_of(device_id);
   if (sms < 0) return sms;
   LinearGradArgs g{};
-  g.fwd.n_rows    = n_rows;
-  g.fwd.n_cols    = n_cols;
-  g.fwd.width     = width;
-  g.fwd.teacher.k = k;
+  g.fwd.hidden        = hidden;
+  g.fwd.weight        = weight;
+  g.fwd.hidden_stride = hidden_stride;
+  g.fwd.weight_stride = weight_stride;
+  g.fwd.n_rows        = n_rows;
+  g.fwd.n_cols        = n_cols;
+  g.fwd.width         = width;
+  g.fwd.teacher.k     = k;
   char some;
   g.grad_hidden = wants_hidden ? &some : nullptr;
   g.grad_weight = wants_weight ? &some : nullptr;
@@ -333,8 +345,8 @@ int b2fil_linear_loss_grad(int dtype, const void* hidden, int64_t hidden_stride,
       !aligned(upstream, 4) || !aligned(factor, 4) || !aligned(grad_hidden, 16) || !aligned(grad_weight, 16))
     return invalid("a buffer is not aligned");
   rc = check_workspace(workspace, workspace_bytes,
-                       b2fil_linear_loss_grad_workspace(dtype, n_rows, n_cols, width, k, grad_hidden != nullptr,
-                                                        grad_weight != nullptr, device_id));
+                       b2fil_linear_loss_grad_workspace(dtype, hidden, hidden_stride, weight, weight_stride, n_rows, n_cols,
+                                                        width, k, grad_hidden != nullptr, grad_weight != nullptr, device_id));
   if (rc != B2FIL_OK) return rc;
   const int sms = sms_of(device_id);
   if (sms < 0) return sms;

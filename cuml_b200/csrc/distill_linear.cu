@@ -45,6 +45,10 @@ constexpr int kMostSplits     = 16;
 // 64 bits are 1.4 times those of their own rounding with one plane and 1.0 with two, which takes 5 us of
 // 31; with two classes one plane made them up to twice as large).
 constexpr int64_t kSmallProduct = 1ll << 32;
+// ... and classes up to which the forward pass takes the logits as dot products in the kernel that reads the
+// teacher: a load's latency per 32 classes of a row, against a kernel of 8 us.
+constexpr int64_t kSmallLogits  = 1ll << 25;
+constexpr int kFewClasses       = 128;
 constexpr int kGroup          = 32;            // tiles of rows whose part of H stays in L2 while all of W passes
 constexpr float kHalfScale    = 16384.f;       // of d in fp16
 // Named classes of a row that the epilogue looks through for each tile; more are put into d by a kernel of their
@@ -582,14 +586,46 @@ __device__ __forceinline__ float dot_piece(const Piece<T>& a, const Piece<T>& b,
   return s;
 }
 
+// Dot products of h with n rows of w, those that class_of(j) names, by WARPS warps, four at a time: take(j, sum) for
+// lane 0 of the warp that has j.  (A class below 0 has none.)
+template <class T, int WARPS, class C, class F>
+__device__ __forceinline__ void dots(const LinearArgs& a, const T* h, int n, int warp, C class_of, F take)
+{
+  constexpr int N = Piece<T>::N;
+  const int lane  = threadIdx.x % 32;
+  for (int j = 4 * warp; j < n; j += 4 * WARPS) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    const T* v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int cls = j + u < n ? class_of(j + u) : -1;
+      v[u]          = static_cast<const T*>(a.weight) + (cls < 0 ? 0 : cls) * a.weight_stride;
+    }
+    const int most = min(4, n - j);
+    for (int i = lane * N; i < a.width; i += 32 * N) {
+      const Piece<T> x = load_piece(h + i);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (u < most) s[u] = dot_piece(x, load_piece(v[u] + i), s[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (u < most) {
+        s[u] = sum_lanes(s[u]);
+        if (lane == 0) take(j + u, s[u]);
+      }
+  }
+}
+
 // Loss of a row from the maxima and sums of its tiles, by THREADS threads, of which the first warp does what
-// concerns the teacher; the named classes' logits are dot products of their own, a warp each, four at a time.
-// The block that is last to finish adds up all blocks' losses.
+// concerns the teacher; the named classes' logits are dot products of their own.  Without tiles (small
+// problems: a launch less, and logits whose sums do not go through the tensor cores) all logits are.  The
+// block that is last to finish adds up all blocks' losses.
 template <class T, int THREADS>
 __global__ void __launch_bounds__(kThreads) linear_rows(LinearArgs a, const float2* parts, int tiles, Reduced out,
                                                         double2* block_sums, int* ticket)
 {
-  constexpr int ROWS = kThreads / THREADS, N = Piece<T>::N, WARPS = THREADS / 32;
+  constexpr int ROWS = kThreads / THREADS, WARPS = THREADS / 32;
   extern __shared__ __align__(16) char smem[];
   __shared__ double2 room[kThreads / 32];
   __shared__ float joins[2 * kThreads / 32];
@@ -609,28 +645,13 @@ __global__ void __launch_bounds__(kThreads) linear_rows(LinearArgs a, const floa
     if (tid < 32) t = read_teacher<false>(a.teacher, row, a.n_cols, inv_t, e);
     sync_row<THREADS>();
     const T* h = static_cast<const T*>(a.hidden) + row * a.hidden_stride;
-    for (int j = 4 * (tid / 32); j < k; j += 4 * WARPS) {
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
-      const T* v[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int cls = j + u < k ? e.at[j + u] : -1;
-        v[u]          = static_cast<const T*>(a.weight) + (cls < 0 ? 0 : cls) * a.weight_stride;
-      }
-      const int most = min(4, k - j);
-      for (int i = lane * N; i < a.width; i += 32 * N) {
-        const Piece<T> x = load_piece(h + i);
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (u < most) s[u] = dot_piece(x, load_piece(v[u] + i), s[u]);
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (u < most) s[u] = sum_lanes(s[u]);
-      if (lane < most) logit[j + lane] = lane == 0 ? s[0] : lane == 1 ? s[1] : lane == 2 ? s[2] : s[3];
-    }
+    dots<T, WARPS>(a, h, k, tid / 32, [&](int j) { return e.at[j]; }, [&](int j, float s) { logit[j] = s; });
     Running<float> r;
-    for (int i = tid; i < tiles; i += THREADS) r.join(parts[row * tiles + i].x, parts[row * tiles + i].y, c);
+    if (tiles > 0) {
+      for (int i = tid; i < tiles; i += THREADS) r.join(parts[row * tiles + i].x, parts[row * tiles + i].y, c);
+    } else {
+      dots<T, WARPS>(a, h, static_cast<int>(a.n_cols), tid / 32, [](int j) { return j; }, [&](int, float s) { r.take(s, c); });
+    }
     join_row<THREADS>(r, c, joins);
     sync_row<THREADS>();
     if (tid < 32) {
@@ -722,6 +743,52 @@ __global__ void __launch_bounds__(kThreads) finish_sums(const float* sums, int s
   }
 }
 
+// The same for rows of `width` of `pitch` columns: four results per thread, which may be in two rows (or more).
+template <class T>
+__global__ void __launch_bounds__(kThreads) finish_rows(const float* sums, int splits, int64_t rows, int pitch, int width,
+                                                        Scale scale, T* out)
+{
+  const float f     = scale();
+  const int64_t all = rows * width;
+  for (int64_t i = 4 * (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x); i < all; i += 4 * gridDim.x * static_cast<int64_t>(kThreads)) {
+    int64_t r = i / width;
+    int c     = static_cast<int>(i - r * width);
+    T v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float x = 0.f;
+      if (i + j < all)
+        for (int s = 0; s < splits; ++s) x += sums[(s * rows + r) * pitch + c];
+      v[j] = narrow<T>(x * f);
+      if (++c == width) {
+        c = 0;
+        ++r;
+      }
+    }
+    if (i + 3 < all) {
+      *reinterpret_cast<uint2*>(out + i) = *reinterpret_cast<const uint2*>(v);
+    } else {
+      for (int j = 0; i + j < all; ++j) out[i + j] = v[j];
+    }
+  }
+}
+
+// Rows of `width` elements to rows of `pitch` (a multiple of 8) with zeros behind: 16 bytes per thread.
+template <class T>
+__global__ void __launch_bounds__(kThreads) pad_rows(const T* from, int64_t stride, int64_t rows, int width, int pitch, T* to)
+{
+  const int per     = pitch / 8;
+  const int64_t all = rows * per;
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < all; i += gridDim.x * static_cast<int64_t>(kThreads)) {
+    const int64_t r = i / per;
+    const int c     = static_cast<int>(i - r * per) * 8;
+    Piece<T> v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v.v[j] = c + j < width ? from[r * stride + c + j] : narrow<T>(0.f);
+    *reinterpret_cast<uint4*>(to + i * 8) = *reinterpret_cast<const uint4*>(&v);
+  }
+}
+
 __global__ void no_rows(Reduced out) { write_reduced(out, make_double2(0, 0)); }
 
 __global__ void wait_for_nothing()
@@ -775,6 +842,47 @@ cudaError_t run_products(const Work& w, int n_sms, cudaStream_t s)
   return cudaGetLastError();
 }
 
+// The kernels read 16 bytes at a time, rows that start on them and end with whole pieces.  Others are copied, with
+// zeros behind each row, which change no product; so are large ones off the 32-byte sectors, which are read a
+// quarter slower (4096 x 1032 x 16,384, loss and gradient: 501 us, with 1040 or 1024 columns 380).
+struct Layer {
+  bool copied;
+  int64_t width;         // of a row as the kernels read it
+  int64_t bytes;         // of the copies
+};
+int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+Layer layer_of(const LinearArgs& a)
+{
+  Layer l;
+  l.copied = a.width % 8 || a.hidden_stride % 8 || a.weight_stride % 8 || reinterpret_cast<uintptr_t>(a.hidden) % 16 ||
+             reinterpret_cast<uintptr_t>(a.weight) % 16 ||
+             ((a.width % 16 || a.hidden_stride % 16 || a.weight_stride % 16) && a.n_rows * a.n_cols >= (1ll << 36) / a.width);
+  l.width = l.copied ? (a.width + 15) / 16 * 16 : a.width;
+  l.bytes = l.copied ? padded(a.n_rows * l.width * 2) + padded(a.n_cols * l.width * 2) : 0;
+  return l;
+}
+// `a` with the layer as the kernels read it; copies go to `at`, which is moved behind them.
+template <class T>
+cudaError_t give_layer(LinearArgs& a, const Layer& l, char*& at, int n_sms, cudaStream_t s)
+{
+  if (!l.copied) return cudaSuccess;
+  T* hidden = reinterpret_cast<T*>(at);
+  T* weight = reinterpret_cast<T*>(at + padded(a.n_rows * l.width * 2));
+  at += l.bytes;
+  auto pad = [&](const void* from, int64_t stride, int64_t rows, T* to) {
+    const int64_t need = (rows * l.width / 8 + kThreads - 1) / kThreads, most = 16ll * n_sms;
+    pad_rows<T><<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(
+      static_cast<const T*>(from), stride, rows, static_cast<int>(a.width), static_cast<int>(l.width), to);
+  };
+  pad(a.hidden, a.hidden_stride, a.n_rows, hidden);
+  pad(a.weight, a.weight_stride, a.n_cols, weight);
+  a.hidden = hidden;
+  a.weight = weight;
+  a.width = a.hidden_stride = a.weight_stride = l.width;
+  count_launches(2);
+  return cudaGetLastError();
+}
+
 // z = H W^T of the classes from `first` on
 bool logits_product(Product& p, bool bf16, const LinearArgs& a, int64_t first, int64_t n)
 {
@@ -792,33 +900,43 @@ bool logits_product(Product& p, bool bf16, const LinearArgs& a, int64_t first, i
 }
 
 template <class T>
-cudaError_t run_linear(bool bf16, const LinearArgs& a, const Reduced& out, void* workspace, int n_sms, cudaStream_t s)
+cudaError_t run_linear(bool bf16, const LinearArgs& given, const Reduced& out, void* workspace, int n_sms, cudaStream_t s)
 {
+  LinearArgs a = given;
   if (a.n_rows == 0) {
     if (out.reduction != 0) no_rows<<<1, 1, 0, s>>>(out);
     count_launches(out.reduction != 0);
     return cudaGetLastError();
   }
-  double2* sums = static_cast<double2*>(workspace);
+  char* at      = static_cast<char*>(workspace);
+  cudaError_t e = give_layer<T>(a, layer_of(given), at, n_sms, s);
+  if (e != cudaSuccess) return e;
+  double2* sums = reinterpret_cast<double2*>(at);
   Work w{};
   w.products = 1;
   w.bf16     = bf16;
   w.c        = 1.4426950408889634f / a.temperature;
   w.ticket   = reinterpret_cast<int*>(sums + 8 * n_sms);
   w.parts    = reinterpret_cast<float2*>(sums + 8 * n_sms + 1);
-  if (!logits_product(w.product[0], bf16, a, 0, a.n_cols)) return cudaErrorInvalidValue;
-  cudaError_t e = run_products<kStats>(w, n_sms, s);
+  const bool small = a.n_cols <= kFewClasses && a.n_rows * a.n_cols <= kSmallLogits / a.width;
+  if (small) {
+    if (out.reduction != 0) e = cudaMemsetAsync(w.ticket, 0, sizeof(int), s);
+  } else {
+    if (!logits_product(w.product[0], bf16, a, 0, a.n_cols)) return cudaErrorInvalidValue;
+    e = run_products<kStats>(w, n_sms, s);
+  }
   if (e != cudaSuccess) return e;
+  const int tiles = small ? 0 : 2 * w.product[0].n_tiles;
   // a warp per row where there are enough rows (or nothing to share), else a block
-  const bool warp    = a.teacher.k <= 4 || a.n_rows >= 8 * n_sms;
+  const bool warp    = (a.teacher.k <= 4 && !(small && a.n_cols > 8)) || a.n_rows >= 8 * n_sms;
   const int per      = warp ? kThreads / 32 : 1;
   const int64_t need = (a.n_rows + per - 1) / per;
   const int blocks   = static_cast<int>(need < 8 * n_sms ? need : 8 * n_sms);
   const size_t bytes = per * (entry_bytes(a.teacher.k) + static_cast<size_t>(a.teacher.k) * 4);
   if (warp)
-    linear_rows<T, 32><<<blocks, kThreads, bytes, s>>>(a, w.parts, 2 * w.product[0].n_tiles, out, sums, w.ticket);
+    linear_rows<T, 32><<<blocks, kThreads, bytes, s>>>(a, w.parts, tiles, out, sums, w.ticket);
   else
-    linear_rows<T, kThreads><<<blocks, kThreads, bytes, s>>>(a, w.parts, 2 * w.product[0].n_tiles, out, sums, w.ticket);
+    linear_rows<T, kThreads><<<blocks, kThreads, bytes, s>>>(a, w.parts, tiles, out, sums, w.ticket);
   count_launches(2);
   return cudaGetLastError();
 }
@@ -832,7 +950,7 @@ struct Plan {
   int splits_hidden, splits_weight;
   bool sums_hidden, sums_weight;  // in memory
 };
-Plan plan_of(const LinearGradArgs& g, int n_sms)
+Plan plan_of(const LinearGradArgs& g, const Layer& l, int n_sms)
 {
   const LinearArgs& a = g.fwd;
   Plan p;
@@ -841,10 +959,10 @@ Plan plan_of(const LinearGradArgs& g, int n_sms)
   p.pieces = static_cast<int>((a.n_cols + most - 1) / most);
   p.cols   = static_cast<int64_t>(tiles_of((a.n_cols + p.pieces - 1) / p.pieces)) * kTile;
   p.pieces = static_cast<int>((a.n_cols + p.cols - 1) / p.cols);
-  p.planes     = a.n_rows * a.n_cols <= kSmallProduct / a.width ? 2 : 1;
+  p.planes     = a.n_rows * a.n_cols <= kSmallProduct / l.width ? 2 : 1;
   p.plane_rows = (a.n_rows + kDepth - 1) / kDepth * kDepth;
   // as many parts as bring a part down to an even share of the machine, 16 stages at least
-  const int64_t wide = tiles_of(a.width), dh_tiles = tiles_of(a.n_rows) * wide, dw_tiles = tiles_of(p.cols) * wide;
+  const int64_t wide = tiles_of(l.width), dh_tiles = tiles_of(a.n_rows) * wide, dw_tiles = tiles_of(p.cols) * wide;
   const int64_t dh_steps = p.planes * (p.cols / kDepth), dw_steps = p.planes * (p.plane_rows / kDepth);
   int64_t share = ((g.grad_hidden ? dh_tiles * dh_steps : 0) + (g.grad_weight ? dw_tiles * dw_steps : 0)) / (n_sms / 2);
   if (share < 16) share = 16;
@@ -854,27 +972,37 @@ Plan plan_of(const LinearGradArgs& g, int n_sms)
   };
   p.splits_hidden = parts(dh_steps);
   p.splits_weight = parts(dw_steps);
-  p.sums_hidden   = g.grad_hidden && (p.pieces > 1 || p.splits_hidden > 1);
-  p.sums_weight   = g.grad_weight && p.splits_weight > 1;
+  p.sums_hidden   = g.grad_hidden && (p.pieces > 1 || p.splits_hidden > 1 || l.width != a.width);
+  p.sums_weight   = g.grad_weight && (p.splits_weight > 1 || l.width != a.width);
   return p;
 }
-int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 template <class T>
-cudaError_t finish(const float* sums, int splits, int64_t n, const Scale& scale, void* out, int n_sms, cudaStream_t s)
+cudaError_t finish(const float* sums, int splits, int64_t rows, int64_t pitch, int64_t width, const Scale& scale, void* out,
+                   int n_sms, cudaStream_t s)
 {
-  const int64_t need = (n / 4 + kThreads - 1) / kThreads;
-  finish_sums<T><<<static_cast<unsigned>(need < 8 * n_sms ? need : 8 * n_sms), kThreads, 0, s>>>(sums, splits, n, scale,
-                                                                                              static_cast<T*>(out));
+  const int64_t n = rows * width, most = 8ll * n_sms;
+  if (pitch == width) {
+    const int64_t need = (n / 4 + kThreads - 1) / kThreads;
+    finish_sums<T><<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(sums, splits, n, scale, static_cast<T*>(out));
+  } else {
+    const int64_t need = (n / 4 + kThreads) / kThreads;
+    finish_rows<T><<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(
+      sums, splits, rows, static_cast<int>(pitch), static_cast<int>(width), scale, static_cast<T*>(out));
+  }
   return cudaGetLastError();
 }
 
 template <class T>
 cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace, int n_sms, cudaStream_t s)
 {
-  const LinearArgs& a  = g.fwd;
-  const Plan plan      = plan_of(g, n_sms);
-  char* at             = static_cast<char*>(workspace);
+  LinearArgs a        = g.fwd;
+  const int64_t width = a.width;  // of the gradients' rows
+  const Layer layer   = layer_of(a);
+  const Plan plan     = plan_of(g, layer, n_sms);
+  char* at            = static_cast<char*>(workspace);
+  cudaError_t e       = give_layer<T>(a, layer, at, n_sms, s);
+  if (e != cudaSuccess) return e;
   float* scale         = reinterpret_cast<float*>(at);
   int* ticket          = reinterpret_cast<int*>(at + 16);
   float* row_scale     = reinterpret_cast<float*>(at += 256);
@@ -884,7 +1012,6 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
   const float d_scale  = bf16 ? 1.f : kHalfScale;
   const bool per_row   = g.factor == nullptr;
   int launched         = per_row;
-  cudaError_t e        = cudaSuccess;
   if (per_row) grad_scales<<<1, 1024, 0, s>>>(g, scale, row_scale);
   Work w{};
   w.bf16        = bf16;
@@ -914,7 +1041,7 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
     // d ends with the tile that holds its last class: what is behind has not been written
     const int64_t made = static_cast<int64_t>(tiles_of(n)) * kTile;
     const char* weight = static_cast<const char*>(a.weight) + first * a.weight_stride * 2;
-    T* grad_weight     = g.grad_weight ? static_cast<T*>(g.grad_weight) + first * a.width : nullptr;
+    T* grad_weight     = g.grad_weight ? static_cast<T*>(g.grad_weight) + first * width : nullptr;
     w.products         = 0;
     auto hidden = [&] {
       if (!g.grad_hidden) return true;
@@ -958,12 +1085,12 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
     if ((e = run_products<kGrad>(w, n_sms, s)) != cudaSuccess) return e;
     launched += 2;
     if (plan.sums_weight) {
-      if ((e = finish<T>(sums_weight, plan.splits_weight, n * a.width, w.scale, grad_weight, n_sms, s)) != cudaSuccess) return e;
+      if ((e = finish<T>(sums_weight, plan.splits_weight, n, a.width, width, w.scale, grad_weight, n_sms, s)) != cudaSuccess) return e;
       ++launched;
     }
   }
   if (plan.sums_hidden) {
-    e = finish<T>(sums_hidden, plan.splits_hidden, a.n_rows * a.width, w.scale, g.grad_hidden, n_sms, s);
+    e = finish<T>(sums_hidden, plan.splits_hidden, a.n_rows, a.width, width, w.scale, g.grad_hidden, n_sms, s);
     ++launched;
   }
   count_launches(launched);
@@ -974,16 +1101,18 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
 
 size_t linear_workspace(const LinearArgs& a, int n_sms)
 {
-  return (8 * n_sms + 1) * sizeof(double2) + a.n_rows * static_cast<size_t>(2 * tiles_of(a.n_cols)) * sizeof(float2);
+  return layer_of(a).bytes + (8 * n_sms + 1) * sizeof(double2) +
+         a.n_rows * static_cast<size_t>(2 * tiles_of(a.n_cols)) * sizeof(float2);
 }
 
 size_t linear_grad_workspace(const LinearGradArgs& g, int n_sms)
 {
   const LinearArgs& a = g.fwd;
-  const Plan p        = plan_of(g, n_sms);
-  return 256 + padded(a.n_rows * 4) + padded(p.planes * p.plane_rows * p.cols * 2) +
-         (p.sums_hidden ? p.splits_hidden * a.n_rows * a.width * sizeof(float) : 0) +
-         (p.sums_weight ? p.splits_weight * p.cols * a.width * sizeof(float) : 0);
+  const Layer l       = layer_of(a);
+  const Plan p        = plan_of(g, l, n_sms);
+  return l.bytes + 256 + padded(a.n_rows * 4) + padded(p.planes * p.plane_rows * p.cols * 2) +
+         (p.sums_hidden ? p.splits_hidden * a.n_rows * l.width * sizeof(float) : 0) +
+         (p.sums_weight ? p.splits_weight * p.cols * l.width * sizeof(float) : 0);
 }
 
 cudaError_t launch_linear(int dtype, const LinearArgs& a, const Reduced& out, void* workspace, int n_sms, cudaStream_t s)

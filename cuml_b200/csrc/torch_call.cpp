@@ -409,6 +409,7 @@ struct LinearNode : ag::Node {
       h = hidden.unpack();
       w = weight.unpack();
       const int64_t n = h.size(0), width = h.size(1), c = w.size(0);
+      auto step = [&](const Tensor& x) { return x.size(0) == 1 ? width : x.stride(0); };
       const bool wants_h = task_should_compute_output(0), wants_w = task_should_compute_output(1);
       if (wants_h) dh = make({n, width}, h.scalar_type(), h);
       if (wants_w) dw = make({c, width}, h.scalar_type(), h);
@@ -418,9 +419,10 @@ struct LinearNode : ag::Node {
       const float* named = at + 4 * n + 4;
       const int device = h.get_device(), type = type_of(h);
       try {
-        const int64_t room = ok(library.linear_grad_workspace(type, n, c, width, k, wants_h, wants_w, device));
+        const int64_t room = ok(library.linear_grad_workspace(type, h.const_data_ptr(), step(h), w.const_data_ptr(), step(w),
+                                                               n, c, width, k, wants_h, wants_w, device));
         const Tensor work  = make({room}, at::kByte, h);
-        ok(library.linear_grad(type, h.const_data_ptr(), h.stride(0), w.const_data_ptr(), w.stride(0), n, c, width, k,
+        ok(library.linear_grad(type, h.const_data_ptr(), step(h), w.const_data_ptr(), step(w), n, c, width, k,
                                o.temperature, at, named, named + n * k, reinterpret_cast<const int32_t*>(named + 2 * n * k),
                                g.const_data_ptr<float>(), stride, o.reduction ? at + 4 * n : nullptr,
                                wants_h ? dh.mutable_data_ptr() : nullptr, wants_w ? dw.mutable_data_ptr() : nullptr,
@@ -456,13 +458,11 @@ PyObject* linear_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   const Tensor& w = THPVariable_Unpack(args[1]);
   const int type  = type_of(h);
   const int64_t n = h.size(0), width = h.size(1), c = w.size(0);
-  auto tiled = [](const Tensor& t) {
-    return t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
-  };
+  // (a single row's stride says nothing)
+  auto step = [&](const Tensor& x) { return x.size(0) == 1 ? width : x.stride(0); };
   TeacherOf t;
   if ((type != B2FIL_TYPE_BF16 && type != B2FIL_TYPE_F16) || w.scalar_type() != h.scalar_type() || !on(w, h) ||
-      w.size(1) != width || width % 8 || (width % 16 && n * c >= (int64_t(1) << 36) / width) || !tiled(h) || !tiled(w) ||
-      !teacher_of(args[2], args[3], Py_None, h, t))
+      w.size(1) != width || !teacher_of(args[2], args[3], Py_None, h, t))
     Py_RETURN_NONE;
   t.ignore    = o.ignore;
   const int k = static_cast<int>(t.index.size(1));
@@ -470,7 +470,8 @@ PyObject* linear_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   try {
     at::AutoDispatchBelowADInplaceOrView below;
     const int device   = h.get_device();
-    const int64_t room = ok(library.linear_workspace(type, n, c, width, k, device));
+    const int64_t room = ok(library.linear_workspace(type, h.const_data_ptr(), step(h), w.const_data_ptr(), step(w), n, c, width,
+                                                      k, device));
     const Tensor work  = make({room}, at::kByte, h);
     // statistics, factor, the named classes' arrays, losses of the rows where they are not what is returned
     kept          = make({4 * n + 4 + 3 * n * k + (o.reduction ? n : 0)}, at::kFloat, h);
@@ -479,7 +480,7 @@ PyObject* linear_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     float* named  = at + 4 * n + 4;
     float* to     = loss.mutable_data_ptr<float>();
     const auto tc = t.c();
-    ok(library.linear(type, h.const_data_ptr(), h.stride(0), w.const_data_ptr(), w.stride(0), n, c, width, &tc,
+    ok(library.linear(type, h.const_data_ptr(), step(h), w.const_data_ptr(), step(w), n, c, width, &tc,
                       o.temperature, o.reduction, o.reduction ? named + 3 * n * k : to, at, named, named + n * k,
                       reinterpret_cast<int32_t*>(named + 2 * n * k), to, at + 4 * n, work.mutable_data_ptr(), room, device,
                       stream_of(device)));

@@ -97,6 +97,11 @@ def _rows(x):
     return x
 
 
+def _step(x):
+    """Elements from one row to the next (a single row's stride says nothing)."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
 def _temperature(t):
     t = float(t)
     if not 1e-6 <= t <= 1e6:
@@ -328,15 +333,15 @@ class _Linear(torch.autograd.Function):
         (n, width), n_cols = hidden.shape, weight.shape[0]
         t = _Teacher(n, dev, values, index, None, ignore)
         k = t.c.k
-        ws = _workspace(lib.b2fil_linear_loss_workspace(kind, n, n_cols, width, k, dev.index), dev)
+        layer = (hidden.data_ptr(), _step(hidden), weight.data_ptr(), _step(weight), n, n_cols, width)
+        ws = _workspace(lib.b2fil_linear_loss_workspace(kind, *layer, k, dev.index), dev)
         # kept for the gradient: statistics and the factor; the named classes' logits, probabilities and places
         kept = torch.empty((4 * n + 4 + 3 * n * k,), dtype=torch.float32, device=dev)
         rows = torch.empty((n,), dtype=torch.float32, device=dev)
         loss = torch.empty((), dtype=torch.float32, device=dev) if reduction else rows
         stats, factor, named = _kept(kept, n)
         _lib.check(lib.b2fil_linear_loss(
-            kind, hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0), n, n_cols, width,
-            C.byref(t.c), temperature, reduction, rows.data_ptr(), stats, named, named + 4 * n * k, named + 8 * n * k,
+            kind, *layer, C.byref(t.c), temperature, reduction, rows.data_ptr(), stats, named, named + 4 * n * k, named + 8 * n * k,
             loss.data_ptr(), factor if reduction else None, ws.data_ptr(), ws.numel(), dev.index, _stream(dev)))
         ctx.save_for_backward(hidden, weight)
         ctx.kept, ctx.options = kept, (temperature, reduction, k)
@@ -352,12 +357,12 @@ class _Linear(torch.autograd.Function):
         of_hidden, of_weight = ctx.needs_input_grad[:2]
         dh = torch.empty((n, width), dtype=hidden.dtype, device=dev) if of_hidden else None
         dw = torch.empty((n_cols, width), dtype=hidden.dtype, device=dev) if of_weight else None
-        ws = _workspace(lib.b2fil_linear_loss_grad_workspace(kind, n, n_cols, width, k, of_hidden, of_weight, dev.index), dev)
+        layer = (hidden.data_ptr(), _step(hidden), weight.data_ptr(), _step(weight), n, n_cols, width)
+        ws = _workspace(lib.b2fil_linear_loss_grad_workspace(kind, *layer, k, of_hidden, of_weight, dev.index), dev)
         g, stride = _upstream(g)
         stats, factor, named = _kept(ctx.kept, n)
         _lib.check(lib.b2fil_linear_loss_grad(
-            kind, hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0), n, n_cols, width, k,
-            temperature, stats, named, named + 4 * n * k, named + 8 * n * k, g.data_ptr(), stride,
+            kind, *layer, k, temperature, stats, named, named + 4 * n * k, named + 8 * n * k, g.data_ptr(), stride,
             factor if reduction else None, dh.data_ptr() if of_hidden else None, dw.data_ptr() if of_weight else None,
             ws.data_ptr(), ws.numel(), dev.index, _stream(dev)))
         return dh, dw, None, None, None, None, None
@@ -367,7 +372,7 @@ _LAYER = (torch.bfloat16, torch.float16)
 
 
 def _layer(hidden, weight):
-    """(hidden (n, width), weight (n_classes, width), leading shape), checked, in rows that start on 16 bytes."""
+    """(hidden (n, width), weight (n_classes, width), leading shape), checked."""
     if torch.is_autocast_enabled("cuda"):
         t = torch.get_autocast_dtype("cuda")
         hidden, weight = (x.to(t) if isinstance(x, torch.Tensor) and x.is_floating_point() else x for x in (hidden, weight))
@@ -382,18 +387,7 @@ def _layer(hidden, weight):
     shape, width = hidden.shape[:-1], weight.shape[1]
     if hidden.ndim != 2:
         hidden = hidden.reshape(-1, width)
-    # Zeros behind each row change no product.  Rows that start within a 32-byte sector are read a quarter slower
-    # (4096 x 1032 x 16,384: 501 us, with 1040 or 1024 columns 380), which pays for four copies in large products.
-    if width % 8 or (width % 16 and hidden.shape[0] * weight.shape[0] >= (1 << 36) // width):
-        hidden, weight = (torch.nn.functional.pad(x, (0, -width % 16)) for x in (hidden, weight))
-    return _tiled(hidden), _tiled(weight), shape
-
-
-def _tiled(x):
-    x = _rows(x)
-    if x.stride(0) % 8 or x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
+    return _rows(hidden), _rows(weight), shape
 
 
 def _linear(hidden, weight, values, index, temperature, ignore, reduction, compiled_only=False):

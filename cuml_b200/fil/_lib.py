@@ -96,12 +96,12 @@ def load() -> C.CDLL:
     lib.b2fil_distill_loss_grad.argtypes = [i32, vp, i64, i64, i64, i32, f64, vp, vp, vp, vp, i64, vp, vp, i64,
                                             i32, vp]
     lib.b2fil_linear_loss_workspace.restype = i64
-    lib.b2fil_linear_loss_workspace.argtypes = [i32, i64, i64, i64, i32, i32]
+    lib.b2fil_linear_loss_workspace.argtypes = [i32, vp, i64, vp, i64, i64, i64, i64, i32, i32]
     lib.b2fil_linear_loss.restype = i32
     lib.b2fil_linear_loss.argtypes = [i32, vp, i64, vp, i64, i64, i64, i64, vp, f64, i32, vp, vp, vp, vp, vp, vp, vp,
                                       vp, i64, i32, vp]
     lib.b2fil_linear_loss_grad_workspace.restype = i64
-    lib.b2fil_linear_loss_grad_workspace.argtypes = [i32, i64, i64, i64, i32, i32, i32, i32]
+    lib.b2fil_linear_loss_grad_workspace.argtypes = [i32, vp, i64, vp, i64, i64, i64, i64, i32, i32, i32, i32]
     lib.b2fil_linear_loss_grad.restype = i32
     lib.b2fil_linear_loss_grad.argtypes = [i32, vp, i64, vp, i64, i64, i64, i64, i32, f64, vp, vp, vp, vp, vp, i64, vp,
                                            vp, vp, vp, i64, i32, vp]

@@ -411,11 +411,13 @@ int b2fil_distill_loss_grad(int dtype, const void* logits, int64_t n_rows, int64
                             int device_id, void* cuda_stream);
 
 /* The same loss of logits = hidden * weight^T that are not kept: hidden (n_rows, width), weight (n_cols,
- * width), both B2FIL_TYPE_BF16 or both B2FIL_TYPE_F16, sums in 32 bits.  width is a multiple of 8; rows
- * start on 16 bytes (both strides are multiples of 8).  teacher->logsumexp must be NULL.  named_logit,
+ * width), both B2FIL_TYPE_BF16 or both B2FIL_TYPE_F16, sums in 32 bits.  Rows that start on 32 bytes (and
+ * whose width is a multiple of 8) are read as they are, others may be copied first.  teacher->logsumexp must be NULL.  named_logit,
  * named_p (float) and named_at (int32), (n_rows, k) each, keep what the gradient needs of the named
  * classes.  n_rows < 2^31 - 256, n_cols < 2^31 - 256, width <= 2^20. */
-int64_t b2fil_linear_loss_workspace(int dtype, int64_t n_rows, int64_t n_cols, int64_t width, int k, int device_id);
+int64_t b2fil_linear_loss_workspace(int dtype, const void* hidden, int64_t hidden_stride, const void* weight,
+                                    int64_t weight_stride, int64_t n_rows, int64_t n_cols, int64_t width,
+                                    int k, int device_id);
 int b2fil_linear_loss(int dtype, const void* hidden, int64_t hidden_stride, const void* weight,
                       int64_t weight_stride, int64_t n_rows, int64_t n_cols, int64_t width,
                       const b2fil_teacher* teacher, double temperature, int reduction, float* row_loss,
@@ -425,9 +427,12 @@ int b2fil_linear_loss(int dtype, const void* hidden, int64_t hidden_stride, cons
 
 /* Its gradients by hidden, to grad_hidden (n_rows, width), and by weight, to grad_weight (n_cols, width),
  * both contiguous, 16-byte aligned and of the layer's type; either may be NULL (in both calls).  The
- * differences softmax - teacher are rounded to the layer's type before they are multiplied. */
-int64_t b2fil_linear_loss_grad_workspace(int dtype, int64_t n_rows, int64_t n_cols, int64_t width, int k,
-                                         int wants_hidden, int wants_weight, int device_id);
+ * differences softmax - teacher are rounded to the layer's type before they are multiplied (small layers: to two
+ * numbers of that type). */
+int64_t b2fil_linear_loss_grad_workspace(int dtype, const void* hidden, int64_t hidden_stride,
+                                         const void* weight, int64_t weight_stride, int64_t n_rows,
+                                         int64_t n_cols, int64_t width, int k, int wants_hidden,
+                                         int wants_weight, int device_id);
 int b2fil_linear_loss_grad(int dtype, const void* hidden, int64_t hidden_stride, const void* weight,
                            int64_t weight_stride, int64_t n_rows, int64_t n_cols, int64_t width,
                            int k, double temperature, const float* row_stats,

@@ -295,14 +295,15 @@ def test_rows_behind_the_last_are_left_alone():
     stats, p = torch.full((64, 4), 7.0, device="cuda"), torch.full((64, k), 7.0, device="cuda")
     logit, at = p.clone(), torch.full((64, k), 7, device="cuda", dtype=torch.int32)
     h, w = s["h"].detach(), s["w"].detach()
-    ws = torch.empty(lib.b2fil_linear_loss_workspace(2, n, c, 64, k, 0), dtype=torch.uint8, device="cuda")
+    layer = (h.data_ptr(), 64, w.data_ptr(), 64, n, c, 64)
+    ws = torch.empty(lib.b2fil_linear_loss_workspace(2, *layer, k, 0), dtype=torch.uint8, device="cuda")
     assert lib.b2fil_linear_loss(2, h.data_ptr(), 64, w.data_ptr(), 64, n, c, 64, C.byref(teacher), 1.0, 0, rows.data_ptr(),
                                  stats.data_ptr(), logit.data_ptr(), p.data_ptr(), at.data_ptr(), None, None,
                                  ws.data_ptr(), ws.numel(), 0, stream) == 0
     up = torch.ones(n, device="cuda")
     dh = torch.full((64, 64), 7.0, device="cuda").bfloat16()
     dw = torch.full((c + 27, 64), 7.0, device="cuda").bfloat16()
-    ws = torch.empty(lib.b2fil_linear_loss_grad_workspace(2, n, c, 64, k, 1, 1, 0), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(lib.b2fil_linear_loss_grad_workspace(2, *layer, k, 1, 1, 0), dtype=torch.uint8, device="cuda")
     assert lib.b2fil_linear_loss_grad(2, h.data_ptr(), 64, w.data_ptr(), 64, n, c, 64, k, 1.0, stats.data_ptr(),
                                       logit.data_ptr(), p.data_ptr(), at.data_ptr(), up.data_ptr(), 1, None,
                                       dh.data_ptr(), dw.data_ptr(), ws.data_ptr(), ws.numel(), 0, stream) == 0

@@ -81,7 +81,7 @@ def entries(n, c, k, seed=0, index64=False):
 # parts, odd widths
 SIZES = [(1, 8, 1), (1, 64, 2), (3, 16, 7), (128, 64, 256), (129, 72, 257), (256, 256, 256), (257, 264, 300),
          (64, 128, 1000), (200, 520, 1003), (513, 200, 2050), (40, 96, 20_011), (300, 33, 130), (70, 1001, 515),
-         (5000, 64, 40), (9000, 264, 513)]
+         (5000, 64, 40), (9000, 264, 513), (3, 1, 5), (500, 1003, 2100)]
 
 
 @gpu
@@ -200,8 +200,8 @@ def test_c_refusals_without_a_gpu(lib):
         return lib.b2fil_linear_loss(dtype, hidden, hs, weight, ws, n, c, width, C.byref(teacher), t, reduction, 64, stats,
                                      64, 64, at, 64, 64, None, 0, 0, None)
 
-    for bad in (dict(dtype=0), dict(hidden=None), dict(weight=72), dict(hs=8), dict(hs=20), dict(n=-1), dict(n=(1 << 31) - 1),
-                dict(c=0), dict(width=12), dict(width=0), dict(k=0), dict(k=257), dict(lse=64), dict(reduction=5),
+    for bad in (dict(dtype=0), dict(hidden=None), dict(weight=65), dict(hs=8), dict(ws=15), dict(n=-1), dict(n=(1 << 31) - 1),
+                dict(c=0), dict(width=0), dict(width=(1 << 20) + 1), dict(k=0), dict(k=257), dict(lse=64), dict(reduction=5),
                 dict(stats=68), dict(at=None), dict(t=0.0)):
         assert call(**bad) == -1, bad
         assert lib.b2fil_last_error()
@@ -210,7 +210,7 @@ def test_c_refusals_without_a_gpu(lib):
         return lib.b2fil_linear_loss_grad(2, 64, 16, 64, 16, n, 10, width, k, t, 64, 64, 64, 64, up, 0, None, dh, dw, None,
                                           0, 0, None)
 
-    for bad in (dict(n=-1), dict(width=4), dict(k=0), dict(up=None), dict(dh=72), dict(dw=8), dict(t=-1.0)):
+    for bad in (dict(n=-1), dict(width=17), dict(k=0), dict(up=None), dict(dh=72), dict(dw=8), dict(t=-1.0)):
         assert grad(**bad) == -1, bad
     assert grad(dh=None, dw=None) == 0
     assert lib.b2fil_distill_status(0, None) == -1
