@@ -22,6 +22,8 @@
 // bounded: after two seconds a role gives up, sets the status word and leaves by the common exit.
 #include <cuda.h>
 
+#include <algorithm>
+
 #include "distill_common.cuh"
 
 namespace b2fil {
@@ -201,11 +203,11 @@ struct Product {
   int add;
   void* out;    // times `scale`
 };
-// A factor on the device: a b T, or a T.
+// A factor, of what is there of a, b and t.
 struct Scale {
   const float *a, *b;
   float t;
-  __device__ __forceinline__ float operator()() const { return *a * (b ? *b : 1.f) * t; }
+  __device__ __forceinline__ float operator()() const { return (a ? *a : 1.f) * (b ? *b : 1.f) * t; }
 };
 struct Work {
   Product product[2];
@@ -217,7 +219,8 @@ struct Work {
   float c;                // log2(e) / T
   // kDiff: d = scale q of the classes from `first` on, columns up to a whole tile
   const float4* stats;
-  const float* row_scale; // or null: 1
+  const float* row_scale; // row_step elements from one row's to the next, or null: 1
+  int64_t row_step;
   void* diff;
   int64_t diff_stride;
   float diff_scale;
@@ -531,7 +534,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
       if (KIND == kDiff && in) {  // (rows up to a plane's end are zeros: they meet zeros, but not as NaN)
         const float4 s = row < p.m ? w.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
         base           = base_of(s.x);
-        factor         = s.w == 0.f ? 0.f : s.y * w.diff_scale * (w.row_scale ? w.row_scale[row] : 1.f);
+        factor         = s.w == 0.f ? 0.f : s.y * w.diff_scale * (w.row_scale ? w.row_scale[row * w.row_step] : 1.f);
       }
       if (KIND == kGrad && !p.sums) factor = w.scale();
       if (!warp_wait(done + 8 * half, turn, &gave_up)) break;
@@ -550,7 +553,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
       __syncwarp();
       if (lane == 0) bar_arrive_cluster(freed0 + 8 * half);
       if (KIND == kDiff && in && factor != 0.f && w.k <= kFewNamed) {  // over what has just been written
-        const float per = w.diff_scale * (w.row_scale ? w.row_scale[row] : 1.f), inv = w.stats[row].y;
+        const float per = w.diff_scale * (w.row_scale ? w.row_scale[row * w.row_step] : 1.f), inv = w.stats[row].y;
         const int low = t.n * kTile + from, high = min(low + kTile / 2, p.n);
         for (int j = 0; j < w.k; ++j) {
           const int64_t e = row * w.k + j;
@@ -691,8 +694,8 @@ __global__ void __launch_bounds__(kThreads) linear_rows(LinearArgs a, const floa
   if (threadIdx.x == 0) write_reduced(out, total);
 }
 
-// One upstream value per row: the rows' are brought below 1 by a power of two, which *scale takes back, so
-// that d stays in fp16's range.
+// One upstream value per row of an fp16 layer: the rows' are brought below 1 by a power of two, which *scale takes
+// back, so that d stays in range.
 __global__ void __launch_bounds__(1024) grad_scales(LinearGradArgs g, float* scale, float* row_scale)
 {
   __shared__ float room[32];
@@ -721,7 +724,7 @@ __global__ void __launch_bounds__(kThreads) named_diff(Work w, int64_t entries, 
     const float4 s    = w.stats[row];
     if (s.w == 0.f) continue;
     const float q = power((w.named.logit[i] - base_of(s.x)) * w.c) * s.y;
-    float d       = (q - w.named.p[i]) * w.diff_scale * (w.row_scale ? w.row_scale[row] : 1.f);
+    float d       = (q - w.named.p[i]) * w.diff_scale * (w.row_scale ? w.row_scale[row * w.row_step] : 1.f);
     for (int plane = 0; plane < w.planes; ++plane, d -= widen(narrow<T>(d)))
       static_cast<T*>(w.diff)[(plane * static_cast<int64_t>(w.plane_rows) + row) * w.diff_stride + at] = narrow<T>(d);
   }
@@ -1011,19 +1014,21 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
   float* sums_weight   = reinterpret_cast<float*>(at + (plan.sums_hidden ? plan.splits_hidden * a.n_rows * a.width * 4 : 0));
   const float d_scale  = bf16 ? 1.f : kHalfScale;
   const bool per_row   = g.factor == nullptr;
-  int launched         = per_row;
-  if (per_row) grad_scales<<<1, 1024, 0, s>>>(g, scale, row_scale);
+  const bool scaled    = per_row && !bf16;  // (bf16 has the range of the upstream values itself)
+  int launched         = scaled;
+  if (scaled) grad_scales<<<1, 1024, 0, s>>>(g, scale, row_scale);
   Work w{};
   w.bf16        = bf16;
   w.c           = 1.4426950408889634f / a.temperature;
   w.stats       = a.row_stats;
-  w.row_scale   = per_row ? row_scale : nullptr;
+  w.row_scale   = scaled ? row_scale : per_row ? g.upstream : nullptr;
+  w.row_step    = scaled ? 1 : g.upstream_stride;
   w.diff        = diff;
   w.diff_stride = plan.cols;
   w.diff_scale  = d_scale;
   w.planes      = plan.planes;
   w.plane_rows  = static_cast<int>(plan.plane_rows);
-  w.scale       = Scale{per_row ? scale : g.upstream, g.factor, a.temperature / d_scale};
+  w.scale       = Scale{scaled ? scale : per_row ? nullptr : g.upstream, g.factor, a.temperature / d_scale};
   w.named       = a.named;
   w.k           = a.teacher.k;
   w.ticket      = ticket;
@@ -1048,7 +1053,8 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
       Product& p = w.product[w.products++];
       p.m        = static_cast<int>(a.n_rows);
       p.depth    = static_cast<int>(made);
-      p.splits   = plan.splits_hidden;
+      // (a short last piece adds to the first of them; the first piece has written all)
+      p.splits = static_cast<int>(std::min<int64_t>(plan.splits_hidden, plan.planes * (made / kDepth)));
       p.a_outer  = 0;
       p.sums     = plan.sums_hidden ? sums_hidden : nullptr;
       p.add      = i > 0;

@@ -16,7 +16,10 @@
 // Bound by memory: one pass over the scores, which also takes the running maximum and sum of the
 // log-sum-exp.  Of a thread's best score that pass keeps the value and the 16 bytes that hold it; the keys of
 // their first and last element stand for its own above and below.
-// Where rows are few, several blocks share one and a second kernel joins their lists.
+// Where rows are few, several blocks share one: up to eight as a cluster, whose first block joins the lists over
+// distributed shared memory; of longer rows a second kernel does.
+#include <cooperative_groups.h>
+
 #include "distill_common.cuh"
 
 namespace b2fil {
@@ -29,6 +32,8 @@ constexpr int kWarpList = 320;   // candidates of a warp: at least the largest k
 constexpr int kWarpCols = 1024;  // longest rows of a warp (fp64: 512)
 constexpr int kFew      = 32;    // candidates that a warp places in one go
 constexpr int kCount    = 160;   // candidates of a block that are placed by counting; more are sorted
+constexpr int kCluster  = 8;     // blocks that share a row of up to kJoinCols and join their lists themselves
+constexpr int64_t kJoinCols = 1 << 17;  // (1 x 50,001, k 20: 13.8 us by two kernels, 10.7 this way, 14.2 by 16 blocks)
 constexpr int kMore     = 8;     // groups more than k that end the search of the bound
 constexpr int kInFlight = 4;
 // Rows for one thread each: tiles of kTileRows.  A thread takes some 5 k instructions per score, a warp with a row
@@ -200,36 +205,52 @@ __device__ __forceinline__ void write_lse(const TopArgs& a, int64_t row, V m, V 
   static_cast<V*>(a.logsumexp)[row] = r;
 }
 
-// What a row's threads share.
-template <class K, int LIST, int GROUPS>
-struct RowShared {
-  K list[LIST];
-  K tau;
-  int16_t groups[GROUPS];
-  int found, chosen;
-};
+// Places `got` keys of `list` in descending order: put(place, key).  By a block; at most kList.
+template <class K, class F>
+__device__ __forceinline__ void arrange(K* list, int got, int k, F put)
+{
+  const int tid = threadIdx.x;
+  if (got <= kCount) {  // a key's place is the number of larger ones
+    if (tid < got) {
+      const K key = list[tid];
+      int place   = 0;
+#pragma unroll 4
+      for (int j = 0; j < got; ++j) place += list[j].above(key);
+      if (place < k) put(place, key);
+    }
+  } else {
+    int size = 256;
+    while (size < got) size <<= 1;
+    for (int i = got + tid; i < size; i += kThreads) list[i] = K::none();
+    __syncthreads();
+    sort_list(list, size);
+    if (tid < k) put(tid, list[tid]);
+  }
+}
 
-// A segment of a row per block.  segs == 1: the row's answer; else its k best keys and its sum.
-template <class T, int THREADS, bool PROB>
+// A segment of a row per block.  segs == 1: the row's answer; else its k best keys and its sum, which the first
+// block of a cluster of segs blocks joins, or top_join does.
+template <class T, bool PROB>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments(TopArgs a, int segs, int64_t seg_cols,
-                                                         typename KeyOf<T>::type* keys, double* sums)
+                                                                                 bool clustered,
+                                                                                 typename KeyOf<T>::type* keys, double* sums)
 {
   using V = typename ValueOf<T>::type;
   using K = typename KeyOf<T>::type;
-  constexpr int ROWS = kThreads / THREADS, N = Piece<T>::N;
-  constexpr int LIST = kList;
-  __shared__ RowShared<K, LIST, THREADS> shared[ROWS];
+  constexpr int N = Piece<T>::N;
+  __shared__ K list[kList], best[kMostTop], shared_tau;
+  __shared__ double best_sum[2];
+  __shared__ int16_t groups[kThreads];
+  __shared__ int found, chosen;
   __shared__ double room[64];
-  const int slot = threadIdx.x / THREADS, tid = threadIdx.x % THREADS;
-  RowShared<K, LIST, THREADS>& mine = shared[slot];
+  const int tid       = threadIdx.x;
   const int seg       = blockIdx.x % segs;
   const int64_t begin = seg * seg_cols;
   const int64_t n     = min(seg_cols, a.n_cols - begin);
   const int k         = static_cast<int>(min(static_cast<int64_t>(a.k), n));
   const V c           = static_cast<V>(1.4426950408889634 * a.inv_temperature);
   const bool plain    = a.inv_temperature == 1.0;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x / segs) * ROWS + slot; row < a.n_rows;
-       row += static_cast<int64_t>(gridDim.x / segs) * ROWS) {
+  for (int64_t row = blockIdx.x / segs; row < a.n_rows; row += gridDim.x / segs) {
     const T* x       = static_cast<const T*>(a.scores) + row * a.row_stride + begin;
     const int lead   = lead_of(x, n);
     const int pieces = static_cast<int>((n - lead) / N);
@@ -239,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
     V top       = lowest<V>();
     uint32_t at = ~0u;  // none yet
     visit_row<kInFlight>(
-      x, n, tid, THREADS,
+      x, n, tid, kThreads,
       [&](int64_t i, T e) {
         const V v = widen(e);
         if (v > top || at == ~0u) at = static_cast<uint32_t>(i);
@@ -263,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
     if (sum.s != sum.s) {  // a NaN, or infinities: the first NaN of the group is its best
       uint32_t first = ~0u;
       visit_row<1>(
-        x, n, tid, THREADS,
+        x, n, tid, kThreads,
         [&](int64_t i, T e) {
           if (widen(e) != widen(e)) first = min(first, static_cast<uint32_t>(i));
         },
@@ -286,24 +307,22 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
     all.m = V(0);
     if (PROB) {
       // (in 64 bits: see Sum)
-      dropped = sum_row<THREADS>(static_cast<double>(sum.s) + sum.dropped, room);
+      dropped = sum_row<kThreads>(static_cast<double>(sum.s) + sum.dropped, room);
     } else {
       all.m = sum.first ? lowest<V>() : sum.r;
       all.s = sum.s;
-      join_row<THREADS>(all, V(1), reinterpret_cast<V*>(room));
+      join_row<kThreads>(all, V(1), reinterpret_cast<V*>(room));
     }
     // tau: a bound that k groups reach, and at most kMore more unless its last bit is reached; the first warp
     // counts for all
     K tau = K::none();
-    if (THREADS > 32) {
-      mine.list[tid] = below;
-      __syncthreads();
-    }
+    list[tid] = below;
+    __syncthreads();
     if (tid < 32) {
-      constexpr int G = THREADS / 32;
+      constexpr int G = kThreads / 32;
       K group[G];
 #pragma unroll
-      for (int g = 0; g < G; ++g) group[g] = THREADS > 32 ? mine.list[tid + 32 * g] : below;
+      for (int g = 0; g < G; ++g) group[g] = list[tid + 32 * g];
       auto reached = [&](const K& by) {
         int some = 0;
 #pragma unroll
@@ -311,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
         return static_cast<int>(__reduce_add_sync(~0u, some));
       };
       const int seen = reached(K::none().with(0));  // (a group without elements has no key)
-      if (seen > k + kMore || (seen >= k && n > LIST)) {
+      if (seen > k + kMore || (seen >= k && n > kList)) {
         for (int bit = K::kBits - 1; bit >= 0; --bit) {
           const K next  = tau.with(bit);
           const int got = reached(next);
@@ -320,30 +339,30 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
           if (got <= k + kMore) break;
         }
       }
-      if (tid == 0) mine.tau = tau;
+      if (tid == 0) shared_tau = tau;
     }
-    if (tid == 0) mine.found = mine.chosen = 0;
-    sync_row<THREADS>();
-    tau                = mine.tau;
+    if (tid == 0) found = chosen = 0;
+    __syncthreads();
+    tau                = shared_tau;
     const bool reaches = any && !tau.above(above);
-    if (reaches) mine.groups[atomicAdd(&mine.chosen, 1)] = static_cast<int16_t>(tid);
-    sync_row<THREADS>();
-    const int chosen = mine.chosen;
+    if (reaches) groups[atomicAdd(&chosen, 1)] = static_cast<int16_t>(tid);
+    __syncthreads();
+    const int reached_by = chosen;
     // A group's pieces, to the next power of two: those behind the last are left out below.
-    const int per   = (pieces + THREADS - 1) / THREADS;
+    const int per   = (pieces + kThreads - 1) / kThreads;
     const int shift = per <= 1 ? 0 : 32 - __clz(per - 1);
     auto collect    = [&](const K& bound) {
       auto take = [&](int64_t i) {
         const K key = K::of(widen(x[i]), static_cast<uint32_t>(begin + i));
         if (bound.above(key)) return;
-        const int to = atomicAdd(&mine.found, 1);
-        if (to < LIST) mine.list[to] = key;
+        const int to = atomicAdd(&found, 1);
+        if (to < kList) list[to] = key;
       };
       // (values below the bound's are left out at once; NaN is not below)
       const V least = bound.value();
 #pragma unroll 4
-      for (int i = tid; i < chosen << shift; i += THREADS) {
-        const int p = mine.groups[i >> shift] + (i & ((1 << shift) - 1)) * THREADS;
+      for (int i = tid; i < reached_by << shift; i += kThreads) {
+        const int p = groups[i >> shift] + (i & ((1 << shift) - 1)) * kThreads;
         if (p >= pieces) continue;
         const Piece<T> v = load_piece(body + static_cast<int64_t>(p) * N);
         uint32_t some = 0;
@@ -355,11 +374,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
       if (tid < lead) take(tid);
       const int64_t end = lead + static_cast<int64_t>(pieces) * N + tid;
       if (end < n) take(end);
-      sync_row<THREADS>();
-      const int got = mine.found;
-      sync_row<THREADS>();
-      if (tid == 0) mine.found = 0;
-      sync_row<THREADS>();
+      __syncthreads();
+      const int got = found;
+      __syncthreads();
+      if (tid == 0) found = 0;
+      __syncthreads();
       return got;
     };
     // Where the list is too short, the largest bound that k keys reach is found bit by bit: keys differ, so
@@ -369,48 +388,64 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
     for (int bit = -1;;) {
       got = collect(next);
       if (bit < 0) {
-        if (got <= LIST) break;
+        if (got <= kList) break;
         bit = K::kBits;
       } else if (got >= k) {
         bound = next;
       }
       next = --bit < 0 ? bound : bound.with(bit);
     }
-    // a candidate's place is the number of larger ones
     const int64_t part = row * segs + seg;
-    auto put           = [&](int place, const K& key) {
-      if (place >= k) return;
-      if (segs == 1) {
+    if (segs == 1) {
+      arrange(list, got, k, [&](int place, const K& key) {
         write_top<T>(a, row, place, key);
         if (place == 0) write_lse(a, row, all.m, all.s, dropped, key);
-      } else {
-        keys[part * a.k + place] = key;
-      }
-    };
-    if (got <= kCount) {
-      if (tid < got) {
-        const K key = mine.list[tid];
-        int place   = 0;
-#pragma unroll 4
-        for (int j = 0; j < got; ++j) place += mine.list[j].above(key);
-        put(place, key);
-      }
-    } else {
-      int size = 256;
-      while (size < got) size <<= 1;
-      for (int i = got + tid; i < size; i += THREADS) mine.list[i] = K::none();
+      });
       __syncthreads();
-      sort_list(mine.list, size);
-      if (tid < k) put(tid, mine.list[tid]);
+      continue;
     }
-    if (segs > 1) {
-      for (int j = k + tid; j < a.k; j += THREADS) keys[part * a.k + j] = K::none();
-      if (tid == 0) {
-        sums[2 * part]     = PROB ? dropped : static_cast<double>(all.s);
-        sums[2 * part + 1] = all.m;
+    K* to = clustered ? best : keys + part * a.k;
+    arrange(list, got, k, [&](int place, const K& key) { to[place] = key; });
+    for (int j = k + tid; j < a.k; j += kThreads) to[j] = K::none();
+    if (tid == 0) {
+      double* sum_to = clustered ? best_sum : sums + 2 * part;
+      sum_to[0]      = PROB ? dropped : static_cast<double>(all.s);
+      sum_to[1]      = all.m;
+    }
+    if (clustered) {
+      // With r = k / segs rounded up, at least k keys reach the least of the lists' r-th keys.
+      namespace cg = cooperative_groups;
+      cg::cluster_group cluster = cg::this_cluster();
+      cluster.sync();
+      if (seg == 0) {
+        const int r_th = (a.k + segs - 1) / segs - 1;
+        K least        = K::of(static_cast<V>(NAN), 0u);  // nothing is above
+        for (int i = 0; i < segs; ++i) {
+          const K key = *cluster.map_shared_rank(best + r_th, i);
+          if (least.above(key)) least = key;
+        }
+        for (int i = tid; i < segs * a.k; i += kThreads) {
+          const K key = *cluster.map_shared_rank(best + i % a.k, i / a.k);
+          if (!least.above(key)) list[atomicAdd(&found, 1)] = key;
+        }
+        __syncthreads();
+        arrange(list, found, a.k, [&](int place, const K& key) {
+          write_top<T>(a, row, place, key);
+          if (place > 0) return;
+          Running<double> r;
+          for (int i = 0; i < segs; ++i) {
+            const double* from = cluster.map_shared_rank(best_sum, i);
+            if (PROB)
+              r.s += from[0];
+            else
+              r.join(from[1], from[0], 1.0);
+          }
+          write_lse(a, row, static_cast<V>(r.m), static_cast<V>(PROB ? 0.0 : r.s), PROB ? r.s : 0.0, key);
+        });
       }
+      cluster.sync();  // the others' lists have been read
     }
-    sync_row<THREADS>();
+    __syncthreads();
   }
 }
 
@@ -840,16 +875,36 @@ cudaError_t run_top(const TopArgs& a, void* workspace, int n_sms, cudaStream_t s
   constexpr int kPieces = sizeof(T) == 8 ? 8 : sizeof(T);  // 512 elements
   if (a.n_cols <= 512) return run_warps<T, kPieces, 0>(a, n_sms, s);
   if (a.n_cols <= kWarpCols && sizeof(T) < 8) return run_warps<T, 2 * kPieces, 0>(a, n_sms, s);
-  int segs           = segments(a.n_rows, a.n_cols, n_sms);
-  const int64_t cols = part_cols(a.n_cols, segs);
-  segs               = static_cast<int>((a.n_cols + cols - 1) / cols);
+  int segs             = segments(a.n_rows, a.n_cols, n_sms);
+  const bool clustered = segs > 1 && a.n_cols <= kJoinCols;
+  if (clustered) {
+    // (a part has more than 1024 elements: segs is at most one for 2048 of them)
+    int power = 2;
+    while (power < segs && power < kCluster) power *= 2;
+    segs = power;
+  }
+  int64_t cols = part_cols(a.n_cols, segs);
+  if (!clustered) segs = static_cast<int>((a.n_cols + cols - 1) / cols);
   double* sums       = static_cast<double*>(workspace);
   K* keys            = reinterpret_cast<K*>(sums + (segs > 1 ? 2 * a.n_rows * segs : 0));
   const int64_t most = 16ll * n_sms;
-  const auto kernel  = a.probabilities ? top_segments<T, kThreads, true> : top_segments<T, kThreads, false>;
-  kernel<<<static_cast<unsigned>((a.n_rows < most ? a.n_rows : most) * segs), kThreads, 0, s>>>(a, segs, cols, keys, sums);
-  if (segs > 1) top_join<T><<<static_cast<unsigned>(a.n_rows < most ? a.n_rows : most), kThreads, 0, s>>>(a, segs, keys, sums);
-  count_launches(segs > 1 ? 2 : 1);
+  const unsigned rows = static_cast<unsigned>(a.n_rows < most ? a.n_rows : most);
+  cudaLaunchConfig_t config{};
+  config.gridDim  = dim3(rows * segs);
+  config.blockDim = dim3(kThreads);
+  config.stream   = s;
+  cudaLaunchAttribute attribute{};
+  attribute.id               = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = segs;
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs    = &attribute;
+  config.numAttrs = clustered ? 1 : 0;
+  const auto kernel   = a.probabilities ? top_segments<T, true> : top_segments<T, false>;
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, a, segs, cols, clustered, keys, sums);
+  if (e != cudaSuccess) return e;
+  const bool join = segs > 1 && !clustered;
+  if (join) top_join<T><<<rows, kThreads, 0, s>>>(a, segs, keys, sums);
+  count_launches(join ? 2 : 1);
   return cudaGetLastError();
 }
 
@@ -858,7 +913,7 @@ cudaError_t run_top(const TopArgs& a, void* workspace, int n_sms, cudaStream_t s
 size_t top_workspace(int dtype, const TopArgs& a, int n_sms)
 {
   const int64_t segs = segments(a.n_rows, a.n_cols, n_sms);
-  if (segs <= 1) return 0;
+  if (segs <= 1 || a.n_cols <= kJoinCols) return 0;
   return a.n_rows * segs * (a.k * (dtype == kF64 ? sizeof(Key64) : sizeof(Key32)) + 2 * sizeof(double));
 }
 
