@@ -216,6 +216,14 @@ bool plain_rows(PyObject* o)
 }
 bool on(const Tensor& t, const Tensor& like) { return t.device() == like.device(); }
 
+// A teacher's numbers in 32 bits (scores of 16 or 64 bits are converted), constants to autograd.
+Tensor as_floats(const Tensor& x)
+{
+  if (x.scalar_type() == at::kFloat) return x;
+  at::AutoDispatchBelowADInplaceOrView below;
+  return x.to(at::kFloat);
+}
+
 // The teacher of one call.  values and logsumexp may be undefined.
 struct TeacherOf {
   Tensor values, index, logsumexp;
@@ -254,15 +262,17 @@ bool teacher_of(PyObject* values, PyObject* index, PyObject* lse, const Tensor& 
   if (values != Py_None) {
     if (!plain_rows(values)) return false;
     t.values = THPVariable_Unpack(values);
-    if (t.values.scalar_type() != at::kFloat || t.values.sizes() != t.index.sizes() || !on(t.values, like)) return false;
+    if (type_of(t.values) < 0 || t.values.sizes() != t.index.sizes() || !on(t.values, like)) return false;
+    t.values = as_floats(t.values);
   }
   if (lse != Py_None) {
     if (!THPVariable_Check(lse)) return false;
     t.logsumexp = THPVariable_Unpack(lse);
-    if (!t.logsumexp.is_cuda() || t.logsumexp.layout() != at::kStrided || t.logsumexp.scalar_type() != at::kFloat ||
+    if (!t.logsumexp.is_cuda() || t.logsumexp.layout() != at::kStrided || type_of(t.logsumexp) < 0 ||
         t.logsumexp.dim() != 1 || t.logsumexp.size(0) != n || (n > 1 && t.logsumexp.stride(0) != 1) ||
         at::isTensorSubclassLike(t.logsumexp) || !on(t.logsumexp, like))
       return false;
+    t.logsumexp = as_floats(t.logsumexp);
   }
   return true;
 }

@@ -468,3 +468,43 @@ def test_cross_entropy(monkeypatch, compiled, n, c):
             distill.cross_entropy(z, bad)
     with pytest.raises(ValueError, match="reduction"):
         distill.cross_entropy(z, target, reduction="max")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp64", "bf16", "fp16"])
+@pytest.mark.parametrize("compiled", [True, False])
+def test_teachers_of_other_types(monkeypatch, dtype, compiled):
+    """The scores that `top_scores` returns go into a loss as they are."""
+    from cuml_b200 import distill
+
+    if not compiled:
+        monkeypatch.setattr(distill, "_call", False)
+    t = torch.randn((40, 300), generator=gen(1), device="cuda").to(TYPES[dtype])
+    z = torch.randn((40, 300), generator=gen(2), device="cuda")
+    top = distill.top_scores(t, 9)
+    check_loss(z, top.values.float(), top.index, top.logsumexp.float(), 1.0, "mean")
+    for tail in ("renormalise", "bucket"):
+        given = distill.distillation_loss(z, top, tail=tail, reduction="none")
+        in_floats = distill.TopScores(top.values.float(), top.index, top.logsumexp.float())
+        assert torch.equal(given, distill.distillation_loss(z, in_floats, tail=tail, reduction="none"))
+
+
+@gpu
+def test_more_than_two_to_the_31_elements():
+    """The last rows of large arrays, and the last classes of a large layer, against the same rows alone."""
+    from cuml_b200 import distill
+
+    n, c = 66_000, 32_800
+    x = torch.randn((n, c), generator=gen(1), device="cuda", dtype=torch.bfloat16)
+    top = distill.top_scores(x, 7)
+    few = distill.top_scores(x[-900:].clone(), 7)
+    for a, b in zip(top, few):
+        assert torch.equal(a[-900:], b)
+    z = x.requires_grad_()
+    loss = distill.distillation_loss(z, top, reduction="none")
+    (g,) = torch.autograd.grad(loss, z, torch.ones_like(loss))
+    tail = x.detach()[-900:].clone().requires_grad_()
+    rows = distill.distillation_loss(tail, few, reduction="none")
+    assert torch.equal(loss[-900:], rows)
+    assert torch.equal(g[-900:], torch.autograd.grad(rows, tail, torch.ones_like(rows))[0])
+    assert (g[0] != 0).any()

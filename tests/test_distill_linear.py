@@ -252,3 +252,32 @@ def test_the_first_thing_that_autograds_thread_does():
 
     r = subprocess.run([sys.executable, "-c", _FIRST_BACKWARD], cwd=ROOT, capture_output=True, text=True)
     assert r.returncode == 0 and r.stdout.startswith("first 6.9"), r.stderr[-800:]
+
+
+@gpu
+def test_a_layer_of_more_than_two_to_the_31_weights():
+    """(4 x 1040 x 2,100,000.)  The logits' sums of 1040 terms are off by e_z = 2 u (1040 / 8 + 16) of the sum of their
+    terms' sizes, here below 60; the gradients as above."""
+    from cuml_b200 import distill
+
+    n, width, c = 4, 1040, 2_100_000
+    h = torch.randn((n, width), generator=gen(1), device="cuda").bfloat16().requires_grad_()
+    w = torch.randn((c, width), generator=gen(2), device="cuda", dtype=torch.bfloat16).mul_(2 / width ** 0.5).requires_grad_()
+    target = torch.tensor([c - 1, 5, c - 300, c // 2], device="cuda")
+    loss = distill.linear_cross_entropy(h, w, target, reduction="none")
+    dh, dw = torch.autograd.grad(loss, (h, w), torch.ones_like(loss))
+    distill.check_status()
+    with torch.no_grad():
+        z = torch.cat([h.double() @ part.double().t() for part in w.split(300_000)], 1)
+        rows, grad, _ = ref.loss(z, None, target[:, None])
+        e_z = adds(width) * 60
+        check_values(loss, rows, 4 * U, 3 * S + 2 * e_z, U)
+        half = HALF_STEP[torch.bfloat16]
+        e_d = grad.abs() * (half + 2 * S + 2 * e_z) + 1e-12
+        for at in (slice(0, 10), slice(c - 310, c)):
+            exact = grad[:, at].t() @ h.cpu().double()
+            check_values(dw[at], exact, 2 * U, (e_d[:, at].t() + adds(n) * grad[:, at].t().abs()) @ h.cpu().double().abs(), half)
+        exact = sum(grad[:, a:a + 300_000] @ w[a:a + 300_000].cpu().double() for a in range(0, c, 300_000))
+        allowed = sum((e_d[:, a:a + 300_000] + adds(c) * grad[:, a:a + 300_000].abs()) @ w[a:a + 300_000].cpu().double().abs()
+                      for a in range(0, c, 300_000))
+        check_values(dh, exact, 2 * U, allowed, half)
