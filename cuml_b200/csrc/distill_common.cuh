@@ -170,6 +170,89 @@ struct Stream {
   }
 };
 
+// ---- rows for one thread each, staged in shared memory ---------------------------------------
+constexpr int kTileRows = 128;  // and threads of a block
+
+// Rows an odd number of words apart fall into different banks.
+template <class T>
+struct TileShape {
+  int cols, pitch;
+  uint32_t inverse;  // i / cols = i * inverse / 2^32 for i < 128 x 512 (exact: i * cols < 2^32)
+  __host__ __device__ explicit TileShape(int n)
+      : cols(n), pitch(sizeof(T) >= 4 ? n | 1 : (n + 1) / 2 * 2 + ((n + 1) / 2 % 2 ? 0 : 2)), inverse(0xffffffffu / n + 1)
+  {
+  }
+  __host__ __device__ size_t bytes() const { return static_cast<size_t>(pitch) * kTileRows * sizeof(T); }
+  // Where element i of the rows one after the other lies in the tile.
+  __device__ __forceinline__ int at(uint32_t i) const { return i + __umulhi(i, inverse) * (pitch - cols); }
+};
+
+// Whether all rows of a tile lie one after the other from a 16-byte boundary on.
+template <class T>
+__device__ __forceinline__ bool without_gaps(const void* rows, int64_t stride, int cols)
+{
+  return stride == cols && (reinterpret_cast<uintptr_t>(rows) & 15) == 0 && cols > 1;
+}
+
+// Visits (row, column) of a tile of rows that are not one after the other.
+template <class F>
+__device__ __forceinline__ void visit_tile(int rows, int cols, F f)
+{
+  int r = threadIdx.x / cols, i = threadIdx.x % cols;
+  const int dr = kTileRows / cols, di = kTileRows % cols;
+  while (r < rows) {
+    f(r, i);
+    r += dr;
+    i += di;
+    if (i >= cols) {
+      i -= cols;
+      ++r;
+    }
+  }
+}
+
+// By all threads of a block, which wait for one another afterwards.
+template <class T>
+__device__ __forceinline__ void load_tile(T* tile, const TileShape<T>& shape, const T* from, int64_t stride, int rows, bool whole)
+{
+  constexpr int N = Piece<T>::N, U = 4;  // 16 bytes at a time, U of them in flight
+  if (whole) {
+    const int all = rows * shape.cols, pieces = all / N;
+    for (int p = threadIdx.x; p < pieces; p += U * kTileRows) {
+      Piece<T> v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (p + u * kTileRows < pieces) v[u] = load_piece(from + (p + u * kTileRows) * N);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (p + u * kTileRows >= pieces) break;
+#pragma unroll
+        for (int e = 0; e < N; ++e) tile[shape.at((p + u * kTileRows) * N + e)] = v[u].v[e];
+      }
+    }
+    for (int i = pieces * N + threadIdx.x; i < all; i += kTileRows) tile[shape.at(i)] = from[i];
+  } else {
+    visit_tile(rows, shape.cols, [&](int r, int i) { tile[r * shape.pitch + i] = from[r * stride + i]; });
+  }
+}
+template <class T>
+__device__ __forceinline__ void store_tile(T* to, int64_t stride, const T* tile, const TileShape<T>& shape, int rows, bool whole)
+{
+  constexpr int N = Piece<T>::N;
+  if (whole) {
+    const int all = rows * shape.cols, pieces = all / N;
+    for (int p = threadIdx.x; p < pieces; p += kTileRows) {
+      Piece<T> v;
+#pragma unroll
+      for (int e = 0; e < N; ++e) v.v[e] = tile[shape.at(p * N + e)];
+      *reinterpret_cast<uint4*>(to + p * N) = *reinterpret_cast<const uint4*>(&v);
+    }
+    for (int i = pieces * N + threadIdx.x; i < all; i += kTileRows) to[i] = tile[shape.at(i)];
+  } else {
+    visit_tile(rows, shape.cols, [&](int r, int i) { to[r * stride + i] = tile[r * shape.pitch + i]; });
+  }
+}
+
 // ---- the threads of one row: a warp or a block -----------------------------------------------
 template <int THREADS>
 __device__ __forceinline__ void sync_row()

@@ -11,7 +11,8 @@
 // dependent loads, votes and logarithms takes as long as reading some 32 KB.  Rows of up to kWarpCols
 // classes therefore belong to one warp altogether, and many warps hide it; longer ones to a block of eight
 // warps that read, while a ninth prepares the next row and a tenth finishes the last.  Where rows are few,
-// several blocks read parts of one and a warp joins their maxima and sums.
+// several blocks read parts of one and a warp joins their maxima and sums.  Many rows of a few classes belong to one
+// thread each, from a tile in shared memory.
 #include <cooperative_groups.h>
 
 #include "distill_common.cuh"
@@ -29,6 +30,12 @@ constexpr int kMostBits = 1 << 17;        // classes that a block marks (three r
 constexpr int kMostSegs = 64;
 constexpr int kInFlight = 8;              // pieces of a thread (the gradient of long rows: 4, as it writes as much)
 constexpr int kCluster  = 8;              // blocks that add up their losses without another kernel
+// Rows for one thread each: classes (the bits of one word), entries, and rows per SM from which on.  (1,000,000 x 10
+// fp32, k 3, rest as a class, loss and gradient: 1646 us with a warp per row, 113 this way; 292,366 x 13 bf16: 474
+// and 30.)
+constexpr int kTileCols  = 64;
+constexpr int kTileTop   = 16;
+constexpr int kTileLeast = 32;
 
 // Bits of the named classes: bit 32 stands for the first element on a 16-byte boundary.
 __host__ __device__ __forceinline__ size_t bit_bytes(int64_t cols) { return cols ? ((cols + 32) / 32 + 2) * 4 : 0; }
@@ -225,6 +232,157 @@ __global__ void __launch_bounds__(kThreads, 5) loss_narrow(LossArgs a, int segs,
   finish_block<kThreads>(sum, count, one_cluster, out, block_sums);
 }
 
+// A row per thread.  What is not named is what the word's bits leave.
+template <class T, bool REST>
+__global__ void __launch_bounds__(kTileRows) loss_tiles(LossArgs a, Reduced out, double2* block_sums)
+{
+  extern __shared__ __align__(16) char smem[];
+  T* tile         = reinterpret_cast<T*>(smem);
+  const Teacher t = a.teacher;
+  const int k = t.k, cols = static_cast<int>(a.n_cols);
+  const TileShape<T> shape(cols);
+  const float c = 1.4426950408889634f / a.temperature, ti = 1.f / a.temperature;
+  const double inv_t = 1.0 / a.temperature;
+  const bool whole   = without_gaps<T>(a.logits, a.row_stride, cols);
+  double sum = 0, count = 0;
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kTileRows; first < a.n_rows;
+       first += static_cast<int64_t>(gridDim.x) * kTileRows) {
+    const int rows = static_cast<int>(min(static_cast<int64_t>(kTileRows), a.n_rows - first));
+    __syncthreads();  // the last tile has been used
+    load_tile(tile, shape, static_cast<const T*>(a.logits) + first * a.row_stride, a.row_stride, rows, whole);
+    __syncthreads();
+    if (threadIdx.x >= rows) continue;
+    const T* x        = tile + threadIdx.x * shape.pitch;
+    const int64_t row = first + threadIdx.x;
+    // the teacher: classes, the largest score, classes named twice
+    float* p       = a.named.p + row * k;
+    int32_t* at    = a.named.at + row * k;
+    const float* v = t.values ? t.values + row * t.values_stride : nullptr;
+    uint64_t named = 0;
+    float top      = lowest<float>();
+    bool merged    = false;
+    for (int j = 0; j < k; ++j) {
+      const int64_t cls = teacher_index(t, row, j);
+      const bool is     = cls >= 0 && cls < cols && cls != t.ignore;
+      at[j]             = is ? static_cast<int>(cls) : -1;
+      if (!is) continue;
+      merged |= named >> cls & 1;
+      named |= 1ull << cls;
+      top = fmaxf(top, v ? v[j] : 0.f);
+    }
+    double log_norm;
+    float rest = 0.f, norm = 1.f;
+    bool counts;
+    if (REST) {
+      log_norm    = t.logsumexp[row];
+      counts      = !(log_norm == -INFINITY);
+      double mass = 0;
+      for (int j = 0; j < k; ++j) {
+        const double q = at[j] >= 0 && counts ? exp((v ? v[j] : 0.f) * inv_t - log_norm) : 0.0;
+        p[j]           = static_cast<float>(q);
+        mass += q;
+      }
+      const bool all = __popcll(named) >= cols;
+      rest           = all || 1.0 - mass < 0x1p-20 ? 0.f : static_cast<float>(1.0 - mass);
+    } else {
+      const float most = base_of(top);
+      float total      = 0.f;
+      for (int j = 0; j < k; ++j) {
+        const float e = at[j] >= 0 ? expf(((v ? v[j] : 0.f) - most) * ti) : 0.f;
+        p[j]          = e;
+        total += e;
+      }
+      log_norm = most * inv_t + log_sum(total);
+      counts   = !(total == 0.f);
+      norm     = counts ? 1.f / total : 1.f;
+    }
+    // the student
+    Stream<float> r;
+    float most = lowest<float>();
+    for (int i = 0; i < cols; ++i) most = fmaxf(most, widen(x[i]));
+    if (most > lowest<float>()) r.raise(most, c, 0.f);
+    float others = 0.f;
+    for (int i = 0; i < cols; ++i) {
+      const float e = power((widen(x[i]) - r.b) * c);
+      r.s += e;
+      if (REST && !(named >> i & 1)) others += e;
+    }
+    const double log_s = log_sum(r.s);
+    counts             = counts && !(r.s == 0.f);
+    double loss        = 0;
+    for (int j = 0; j < k; ++j) {
+      float q = p[j] * norm;
+      if (merged && at[j] >= 0) {  // the first entry of a class has the sum, the others are none
+        for (int i = j + 1; i < k; ++i)
+          if (at[i] == at[j]) {
+            q += p[i] * norm;
+            at[i] = -1;
+          }
+      }
+      p[j] = q;
+      if (at[j] < 0 || q == 0.f) continue;
+      const double log_p = merged ? log(static_cast<double>(q)) : (v ? v[j] : 0.f) * inv_t - log_norm;
+      loss += q * (log_p - ((static_cast<double>(widen(x[at[j]])) - r.m) * inv_t - log_s));
+    }
+    float factor = 1.f;
+    if (REST && rest != 0.f) {
+      loss += rest * (log_sum(rest) - (log_sum(others) - log_s));
+      factor = 1.f - rest / (others / r.s);
+    }
+    if (!counts) loss = 0;
+    loss *= static_cast<double>(a.temperature) * a.temperature;
+    a.row_loss[row]  = static_cast<float>(loss);
+    a.row_stats[row] = make_float4(r.m, 1.f / r.s, factor, counts ? 1.f : 0.f);
+    sum += loss;
+    count += counts;
+  }
+  finish_block<kTileRows>(sum, count, false, out, block_sums);
+}
+
+// Its gradient.
+template <class T>
+__global__ void __launch_bounds__(kTileRows) grad_tiles(LossGradArgs g)
+{
+  extern __shared__ __align__(16) char smem[];
+  T* tile           = reinterpret_cast<T*>(smem);
+  const LossArgs& a = g.fwd;
+  const int k = a.teacher.k, cols = static_cast<int>(a.n_cols);
+  const TileShape<T> shape(cols);
+  const float c     = 1.4426950408889634f / a.temperature;
+  const float scale = (g.factor ? *g.factor : 1.f) * a.temperature;
+  const bool whole_in = without_gaps<T>(a.logits, a.row_stride, cols), whole_out = without_gaps<T>(g.grad, g.grad_stride, cols);
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kTileRows; first < a.n_rows;
+       first += static_cast<int64_t>(gridDim.x) * kTileRows) {
+    const int rows = static_cast<int>(min(static_cast<int64_t>(kTileRows), a.n_rows - first));
+    __syncthreads();  // the last tile has been stored
+    load_tile(tile, shape, static_cast<const T*>(a.logits) + first * a.row_stride, a.row_stride, rows, whole_in);
+    __syncthreads();
+    if (threadIdx.x < rows) {
+      T* x              = tile + threadIdx.x * shape.pitch;
+      const int64_t row = first + threadIdx.x;
+      const float4 s    = a.row_stats[row];
+      const float up    = g.upstream[row * g.upstream_stride] * scale;
+      const bool counts = s.w != 0.f;
+      const float base  = base_of(s.x), f = s.y * up * s.z;
+      // the named classes' from their logits, which are then put over the others'
+      float named[kTileTop];
+#pragma unroll
+      for (int j = 0; j < kTileTop; ++j) {
+        const int at = j < k ? a.named.at[row * k + j] : -1;
+        named[j]     = at >= 0 ? (power((widen(x[at]) - base) * c) * s.y - a.named.p[row * k + j]) * up : 0.f;
+      }
+      for (int i = 0; i < cols; ++i) x[i] = narrow<T>(counts ? power((widen(x[i]) - base) * c) * f : 0.f);
+#pragma unroll
+      for (int j = 0; j < kTileTop; ++j) {
+        const int at = j < k && counts ? a.named.at[row * k + j] : -1;
+        if (at >= 0) x[at] = narrow<T>(named[j]);
+      }
+    }
+    __syncthreads();
+    store_tile(static_cast<T*>(g.grad) + first * g.grad_stride, g.grad_stride, tile, shape, rows, whole_out);
+  }
+}
+
 // A row per block: while eight warps read row i, one prepares row i + 1 and one finishes row i - 1.
 template <class T, bool REST>
 __global__ void __launch_bounds__(kWide, kWideRows) loss_wide(LossArgs a, size_t bits_room, bool one_cluster, Reduced out,
@@ -380,9 +538,23 @@ cudaError_t launch_rows(void (*kernel)(P...), int blocks, bool one_cluster, int 
   return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
 }
 
+bool by_tiles(const LossArgs& a, int n_sms)
+{
+  return a.n_cols <= kTileCols && a.teacher.k <= kTileTop && a.n_rows >= static_cast<int64_t>(kTileLeast) * n_sms;
+}
+
 template <class T, bool REST>
 cudaError_t run_loss(const LossArgs& a, const Reduced& out, void* workspace, int n_sms, cudaStream_t s)
 {
+  if (by_tiles(a, n_sms)) {
+    const int64_t need = (a.n_rows + kTileRows - 1) / kTileRows, most = 8ll * n_sms;
+    const int blocks   = static_cast<int>(need < most ? need : most);
+    double2* sums      = static_cast<double2*>(workspace);
+    loss_tiles<T, REST><<<blocks, kTileRows, TileShape<T>(static_cast<int>(a.n_cols)).bytes(), s>>>(a, out, sums);
+    if (out.reduction != 0) reduce_loss<<<1, kThreads, 0, s>>>(sums, blocks, out);
+    count_launches(out.reduction != 0 ? 2 : 1);
+    return cudaGetLastError();
+  }
   int segs           = segments(a.n_rows, a.n_cols, n_sms, REST);
   const int64_t cols = part_cols(a.n_cols, segs);
   segs               = segs == 1 ? 1 : static_cast<int>((a.n_cols + cols - 1) / cols);
@@ -428,6 +600,13 @@ template <class T>
 cudaError_t run_grad(const LossGradArgs& g, int n_sms, cudaStream_t s)
 {
   const LossArgs& a  = g.fwd;
+  if (by_tiles(a, n_sms)) {
+    const int64_t need = (a.n_rows + kTileRows - 1) / kTileRows, most = 16ll * n_sms;
+    grad_tiles<T><<<static_cast<unsigned>(need < most ? need : most), kTileRows,
+                    TileShape<T>(static_cast<int>(a.n_cols)).bytes(), s>>>(g);
+    count_launches(1);
+    return cudaGetLastError();
+  }
   const bool warp    = a.n_cols <= kWarpCols;
   const int per      = warp ? kThreads / 32 : 1;
   int segs           = warp ? 1 : segments(a.n_rows, a.n_cols, n_sms, false);

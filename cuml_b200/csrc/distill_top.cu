@@ -39,12 +39,10 @@ constexpr int kInFlight = 4;
 // Rows for one thread each: tiles of kTileRows.  A thread takes some 5 k instructions per score, a warp with a row
 // 20 per score and lane and 300 more: many short rows are a thread's (200,000 x 64 fp32, k 4: 155 us by
 // warps), few or long ones a warp's, since a thread's steps follow one another.
-constexpr int kTileRows  = 128;
 constexpr int kTileBytes = 512;  // of a row
 constexpr int kTileTop   = 32;   // largest k, and most classes where k is above 8
 constexpr int kTileSteps = 160;  // classes x (k + 1) that a thread takes however few rows there are
 constexpr int kTileLeast = 32;   // rows per SM from which on threads take the others
-constexpr int kTileFlight = 4;
 static_assert(kThreads >= kMostTop, "a group per entry");
 
 // ---- keys ----------------------------------------------------------------------------------
@@ -704,52 +702,18 @@ __global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
   extern __shared__ __align__(16) char smem[];
   T* tile       = reinterpret_cast<T*>(smem);
   const int c_n = static_cast<int>(a.n_cols);
-  // rows an odd number of words apart fall into different banks
-  const int pitch = sizeof(T) >= 4 ? c_n | 1 : (c_n + 1) / 2 * 2 + ((c_n + 1) / 2 % 2 ? 0 : 2);
-  const V c       = static_cast<V>(1.4426950408889634 * a.inv_temperature);
+  const TileShape<T> shape(c_n);
+  const V c        = static_cast<V>(1.4426950408889634 * a.inv_temperature);
   const bool plain = a.inv_temperature == 1.0;
-  const bool whole = a.row_stride == a.n_cols && (reinterpret_cast<uintptr_t>(a.scores) & 15) == 0 && c_n > 1;
-  // i / c_n = i * inverse / 2^32 for i < 128 x 512 (exact: i * c_n < 2^32)
-  const uint32_t inverse = 0xffffffffu / c_n + 1;
+  const bool whole = without_gaps<T>(a.scores, a.row_stride, c_n);
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * kTileRows; first < a.n_rows;
        first += static_cast<int64_t>(gridDim.x) * kTileRows) {
     const int rows = static_cast<int>(min(static_cast<int64_t>(kTileRows), a.n_rows - first));
-    const T* from  = static_cast<const T*>(a.scores) + first * a.row_stride;
     __syncthreads();  // the last tile has been used
-    if (whole) {
-      // rows without gaps: 16 bytes at a time, kTileFlight of them in flight
-      constexpr int N     = Piece<T>::N;
-      const int all       = rows * c_n, pieces = all / N, pad = pitch - c_n;
-      for (int p = threadIdx.x; p < pieces; p += kTileFlight * kTileRows) {
-        Piece<T> v[kTileFlight];
-#pragma unroll
-        for (int u = 0; u < kTileFlight; ++u)
-          if (p + u * kTileRows < pieces) v[u] = load_piece(from + (p + u * kTileRows) * N);
-#pragma unroll
-        for (int u = 0; u < kTileFlight; ++u) {
-          const uint32_t at = (p + u * kTileRows) * N;
-          if (p + u * kTileRows >= pieces) break;
-#pragma unroll
-          for (int e = 0; e < N; ++e) tile[at + e + __umulhi(at + e, inverse) * pad] = v[u].v[e];
-        }
-      }
-      for (int i = pieces * N + threadIdx.x; i < all; i += kTileRows) tile[i + __umulhi(i, inverse) * pad] = from[i];
-    } else {
-      int r = threadIdx.x / c_n, i = threadIdx.x % c_n;
-      const int dr = kTileRows / c_n, di = kTileRows % c_n;
-      while (r < rows) {
-        tile[r * pitch + i] = from[r * a.row_stride + i];
-        r += dr;
-        i += di;
-        if (i >= c_n) {
-          i -= c_n;
-          ++r;
-        }
-      }
-    }
+    load_tile(tile, shape, static_cast<const T*>(a.scores) + first * a.row_stride, a.row_stride, rows, whole);
     __syncthreads();
     if (threadIdx.x >= rows) continue;
-    const T* x = tile + threadIdx.x * pitch;
+    const T* x = tile + threadIdx.x * shape.pitch;
     // Sorted insertion without branches: of the entries that x exceeds the first becomes x, the others move down.
     V top[TOP], odd = V(0);
     int at[TOP];
@@ -830,7 +794,7 @@ int64_t part_cols(int64_t n_cols, int segs)
 template <class T, int TOP>
 cudaError_t run_tiles(const TopArgs& a, int n_sms, cudaStream_t s)
 {
-  const size_t bytes   = (a.n_cols + 3) * kTileRows * sizeof(T);
+  const size_t bytes   = TileShape<T>(static_cast<int>(a.n_cols)).bytes();
   const int64_t blocks = (a.n_rows + kTileRows - 1) / kTileRows, most = 16ll * n_sms;
   const auto kernel    = a.probabilities ? top_tiles<T, TOP, true> : top_tiles<T, TOP, false>;
   if (bytes > 48 * 1024) {

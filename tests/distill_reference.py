@@ -19,24 +19,22 @@ def top(scores, k, temperature=1.0, probabilities=False):
 def teacher(values, index, lse, n_cols, temperature, ignore=None):
     """(target probabilities (n, n_cols), which classes are named, rest (n,), rows that count)."""
     n, k = index.shape
-    p = torch.zeros((n, n_cols), dtype=torch.float64)
-    named = torch.zeros((n, n_cols), dtype=torch.bool)
+    index = index.long()
+    valid = (index >= 0) & (index < n_cols)
+    if ignore is not None:
+        valid &= index != ignore
+    v = torch.zeros((n, k), dtype=torch.float64) if values is None else values / temperature
+    v = v.masked_fill(~valid, NEG)
+    norm = torch.logsumexp(v, 1) if lse is None else lse.reshape(-1)
+    counts = norm != NEG
+    at = torch.where(valid, index, 0)
+    each = torch.where(valid & counts[:, None], (v - norm[:, None]).exp(), torch.zeros_like(v))
+    p = torch.zeros((n, n_cols), dtype=torch.float64).scatter_add_(1, at, each)
+    named = torch.zeros((n, n_cols), dtype=torch.float64).scatter_add_(1, at, valid.double()) > 0
     rest = torch.zeros(n, dtype=torch.float64)
-    counts = torch.zeros(n, dtype=torch.bool)
-    for i in range(n):
-        entries = [(int(c), 0.0 if values is None else float(values[i, j]) / temperature) for j, c in enumerate(index[i])
-                   if 0 <= int(c) < n_cols and int(c) != ignore]
-        v = torch.tensor([e[1] for e in entries], dtype=torch.float64)
-        norm = float(lse[i]) if lse is not None else float(torch.logsumexp(v, 0)) if len(entries) else NEG
-        counts[i] = norm != NEG
-        if not counts[i]:
-            continue
-        for (c, _), q in zip(entries, (v - norm).exp().tolist()):
-            p[i, c] += q
-            named[i, c] = True
-        if lse is not None and not named[i].all():
-            left = 1.0 - float(p[i].sum())
-            rest[i] = left if not left < 2.0 ** -20 else 0.0
+    if lse is not None:
+        left = 1.0 - p.sum(1)
+        rest = torch.where(counts & ~named.all(1) & ~(left < 2.0 ** -20), left, rest)
     return p, named, rest, counts
 
 

@@ -254,7 +254,8 @@ def check_loss(z, values, index, lse, temperature, reduction, upstream=None):
 
 
 LOSSES = [(1, 1, 1), (1, 2, 1), (64, 10, 3), (1003, 10, 10), (37, 33, 5), (130, 1001, 16), (9, 2048, 256), (9, 2049, 40),
-          (500, 3000, 8), (3, 50_001, 20), (2, 131_072, 64), (301, 9001, 2)]
+          (500, 3000, 8), (3, 50_001, 20), (2, 131_072, 64), (301, 9001, 2),
+          (9001, 2, 2), (5003, 13, 3), (6000, 64, 16), (5000, 64, 17), (5000, 65, 4)]
 
 
 @gpu
@@ -297,6 +298,9 @@ def test_masks_of_teacher_and_student(c, tail, dtype):
         lse[7] = torch.logsumexp(v[7], 0) + 0.3
     for reduction in ("mean", "none"):
         check_loss(z, v, i, lse if tail == "bucket" else None, 1.0, reduction)
+    if c == 40:  # as many rows as belong to a thread each, with sixteen entries
+        many = lambda x: x.repeat(700, *[1] * (x.ndim - 1))  # noqa: E731
+        check_loss(many(z), many(v[:, :16]), many(i[:, :16]), many(lse) if tail == "bucket" else None, 1.0, "mean")
 
 
 @gpu
