@@ -29,8 +29,10 @@ namespace {
 constexpr int kThreads  = 256;   // groups of a block: at least the largest k
 constexpr int kList     = 2048;  // candidates of a block
 constexpr int kWarpList = 320;   // candidates of a warp: at least the largest k
-constexpr int kWarpCols = 1024;  // longest rows of a warp (fp64: 512)
-constexpr int kFew      = 32;    // candidates that a warp places in one go
+constexpr int kWarpCols = 2048;  // longest rows of a warp (fp64: 1024)
+constexpr int kWarpTop  = 24;    // k up to which a warp finds its bound by its lanes' best alone, and the largest of
+                                 // rows above 1024 (30,000 x 2000: fp32, k 10 70 us, by blocks 258; bf16, k 100
+                                 // 414 and 367)
 constexpr int kCount    = 160;   // candidates of a block that are placed by counting; more are sorted
 constexpr int kCluster  = 8;     // blocks that share a row of up to kJoinCols and join their lists themselves
 constexpr int64_t kJoinCols = 1 << 17;  // (1 x 50,001, k 20: 13.8 us by two kernels, 10.7 this way, 14.2 by 16 blocks)
@@ -526,10 +528,13 @@ struct Ordered<double> {
 __device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint64_t max_of(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
+// Blocks of an SM whose lanes hold `bytes` of elements each.
+__host__ __device__ constexpr int warps_fit(size_t bytes) { return bytes <= 128 ? 4 : 2; }
+
 // A row per warp, in registers.  Short rows: every 32nd element is a lane's, S of them.  Longer ones: U pieces of
 // 16 bytes and at most one element from before the first or behind the last boundary per lane, and S is 0.
 template <class T, int U, int S, bool PROB>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 2 : 4) top_warps(TopArgs a)
+__global__ void __launch_bounds__(kThreads, warps_fit(U * 16 / sizeof(T) * sizeof(typename ValueOf<T>::type))) top_warps(TopArgs a)
 {
   using V = typename ValueOf<T>::type;
   using K = typename KeyOf<T>::type;
@@ -588,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 2 : 4) top_warps(To
     const bool nan = PROB ? dropped != dropped : s != s;
     // Few of many: a bound that at least k lanes' best reach, a ballot per bit.
     bool done = false;
-    if (k <= kFew - 8 && (S ? E > 2 : pieces >= kFew) && !nan) {
+    if (k <= kWarpTop && (S ? E > 2 : pieces >= 32) && !nan) {
       const O best = ordered(most);
       O tau        = 0;
       for (int bit = kBits - 1; bit >= 0; --bit) {
@@ -600,15 +605,19 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 2 : 4) top_warps(To
       }
       const V least = tau > ordered(lowest<V>()) ? from_ordered(tau) : lowest<V>();
       // the lane's hits, then its part of the list
-      uint64_t hits = 0;
+      constexpr int H = E < 64 ? E : 64;  // (a 65th is the odd one)
+      uint64_t hits   = 0;
+      bool last_hit   = false;
       if (least > lowest<V>()) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) hits |= v[e] >= least ? 1ull << e : 0ull;
+        for (int e = 0; e < H; ++e) hits |= v[e] >= least ? 1ull << e : 0ull;
+        if (E > H) last_hit = v[E - 1] >= least;
       } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) hits |= is_there(e) ? 1ull << e : 0ull;
+        for (int e = 0; e < H; ++e) hits |= is_there(e) ? 1ull << e : 0ull;
+        if (E > H) last_hit = is_there(E - 1);
       }
-      const int mine = __popcll(hits);
+      const int mine = __popcll(hits) + last_hit;
       int to         = mine;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -623,6 +632,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 2 : 4) top_warps(To
           const int at = place_of(__ffsll(hits) - 1);
           list[to++]   = K::of(widen(x[at]), static_cast<uint32_t>(at));
         }
+        if (last_hit) list[to] = K::of(v[E - 1], static_cast<uint32_t>(odd));
       }
     }
     if (!done) {
@@ -838,7 +848,8 @@ cudaError_t run_top(const TopArgs& a, void* workspace, int n_sms, cudaStream_t s
   if (a.n_cols <= 256) return run_warps<T, 0, 8>(a, n_sms, s);
   constexpr int kPieces = sizeof(T) == 8 ? 8 : sizeof(T);  // 512 elements
   if (a.n_cols <= 512) return run_warps<T, kPieces, 0>(a, n_sms, s);
-  if (a.n_cols <= kWarpCols && sizeof(T) < 8) return run_warps<T, 2 * kPieces, 0>(a, n_sms, s);
+  if (a.n_cols <= 1024) return run_warps<T, 2 * kPieces, 0>(a, n_sms, s);
+  if (a.n_cols <= kWarpCols && sizeof(T) < 8 && a.k <= kWarpTop) return run_warps<T, 4 * kPieces, 0>(a, n_sms, s);
   int segs             = segments(a.n_rows, a.n_cols, n_sms);
   const bool clustered = segs > 1 && a.n_cols <= kJoinCols;
   if (clustered) {

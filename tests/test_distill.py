@@ -139,7 +139,8 @@ def check_top(x, k, temperature=1.0, probabilities=False):
 
 
 SHAPES = [(1, 1, 1), (1, 2, 2), (3, 7, 7), (1000, 10, 3), (257, 33, 5), (5, 255, 64), (4, 1000, 256), (300, 1001, 17),
-          (2, 2049, 100), (3, 16_385, 256), (700, 5000, 8), (1, 50_001, 20), (2, 131_072, 128), (650, 20_000, 33)]
+          (2, 2049, 100), (3, 16_385, 256), (700, 5000, 8), (1, 50_001, 20), (2, 131_072, 128), (650, 20_000, 33),
+          (40, 513, 3), (40, 1024, 24), (40, 1025, 7), (40, 2048, 30), (9, 2047, 256)]
 
 
 @gpu
