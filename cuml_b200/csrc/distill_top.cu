@@ -853,7 +853,7 @@ cudaError_t run_top(const TopArgs& a, void* workspace, int n_sms, cudaStream_t s
   int segs             = segments(a.n_rows, a.n_cols, n_sms);
   const bool clustered = segs > 1 && a.n_cols <= kJoinCols;
   if (clustered) {
-    // (a part has more than 1024 elements: segs is at most one for 2048 of them)
+    // (a part has more than the largest k: rounded up, segs is less than one for 1024 elements)
     int power = 2;
     while (power < segs && power < kCluster) power *= 2;
     segs = power;

@@ -248,9 +248,11 @@ struct TeacherOf {
 bool teacher_of(PyObject* values, PyObject* index, PyObject* lse, const Tensor& like, TeacherOf& t)
 {
   const int64_t n = like.size(0);
-  if (values == Py_None && THPVariable_Check(index) && THPVariable_Unpack(index).dim() == 1) {
-    t.index = THPVariable_Unpack(index);  // one class per row
-    if (!t.index.is_cuda() || t.index.layout() != at::kStrided || at::isTensorSubclassLike(t.index)) return false;
+  if (values == Py_None) {  // one class per row
+    if (!THPVariable_Check(index)) return false;
+    t.index = THPVariable_Unpack(index);
+    if (t.index.dim() != 1 || !t.index.is_cuda() || t.index.layout() != at::kStrided || at::isTensorSubclassLike(t.index))
+      return false;
     t.index = t.index.unsqueeze(1);
   } else {
     if (!plain_rows(index)) return false;

@@ -280,8 +280,8 @@ def distillation_loss(logits, top, *, temperature: float = 1.0, tail: str = "ren
     reduction : 'mean' over the rows that count (0 where none does), 'sum', or 'none': (...), 0 for others.
 
     The loss is fp32, the gradient by the logits has their type."""
-    if reduction in _REDUCTIONS and tail in _TAILS and type(top) is TopScores and (tail != "bucket" or
-                                                                                   top.logsumexp is not None):
+    if (reduction in _REDUCTIONS and tail in _TAILS and type(top) is TopScores and top.values is not None
+            and (tail != "bucket" or top.logsumexp is not None)):
         loss = _loss(logits, top.values, top.index, top.logsumexp if tail == "bucket" else None, _temperature(temperature),
                      _REDUCTIONS[reduction], compiled_only=True)
         if loss is not None:
@@ -425,7 +425,7 @@ def linear_distillation_loss(hidden, weight, top, *, temperature: float = 1.0, r
     hidden : (..., width), weight : (n_classes, width), both bf16 or both fp16 (under autocast they are cast).
     top, temperature, reduction : as in `distillation_loss`; types and rounding as in
     `linear_cross_entropy`."""
-    if reduction in _REDUCTIONS and type(top) is TopScores:
+    if reduction in _REDUCTIONS and type(top) is TopScores and top.values is not None:
         loss = _linear(hidden, weight, top.values, top.index, _temperature(temperature), _NO_CLASS, _REDUCTIONS[reduction],
                        compiled_only=True)
         if loss is not None:

@@ -120,6 +120,25 @@ def test_python_refusals():
         distill.distillation_loss(torch.zeros(1, (1 << 20) + 1, device="cuda"), (v[:1], i[:1], v[:1, 0]), tail="bucket")
 
 
+@gpu
+@pytest.mark.parametrize("columns", [1, 2])
+def test_a_target_with_columns_is_refused(columns):
+    """One class per row is a target's whole shape, also where the columns could be read as a teacher's entries."""
+    from cuml_b200 import distill
+
+    z = torch.zeros(4, 8, device="cuda")
+    target = torch.zeros(4, columns, device="cuda", dtype=torch.int64)
+    with pytest.raises(ValueError, match="target must have shape"):
+        distill.cross_entropy(z, target)
+    with pytest.raises(ValueError, match="target must have shape"):
+        distill.linear_cross_entropy(z.bfloat16(), torch.zeros(5, 8, device="cuda", dtype=torch.bfloat16), target)
+    for index in (target, target[:, 0]):
+        with pytest.raises(TypeError, match="values"):
+            distill.distillation_loss(z, distill.TopScores(None, index, None))
+        with pytest.raises(TypeError, match="values"):
+            distill.linear_distillation_loss(z.bfloat16(), z.bfloat16(), distill.TopScores(None, index, None))
+
+
 # ---- best scores ---------------------------------------------------------------------------------------------
 def check_top(x, k, temperature=1.0, probabilities=False):
     from cuml_b200 import distill
