@@ -20,6 +20,7 @@
 // tiles (TMA, 128-byte swizzle, ring of 6 x 32 KB), warp 1 of the first CTA issues the products, the others
 // work on the finished tile while the next one is summed in the other half of TMEM.  All waits are
 // bounded: after two seconds a role gives up, sets the status word and leaves by the common exit.
+#include <cooperative_groups.h>
 #include <cuda.h>
 
 #include <algorithm>
@@ -57,6 +58,7 @@ constexpr float kHalfScale    = 16384.f;       // of d in fp16
 // own (4096 x 1024 x 50,001, seven pieces: 32 per row cost 290 us in the epilogue and 28 us in the kernel,
 // one per row nothing in the epilogue and 3.6 us per piece in the kernel).
 constexpr int kFewNamed = 4;
+constexpr int kScaleBlocks = 8;
 
 __device__ int g_status;
 
@@ -695,22 +697,31 @@ __global__ void __launch_bounds__(kThreads) linear_rows(LinearArgs a, const floa
 }
 
 // One upstream value per row of an fp16 layer: the rows' are brought below 1 by a power of two, which *scale takes
-// back, so that d stays in range.
-__global__ void __launch_bounds__(1024) grad_scales(LinearGradArgs g, float* scale, float* row_scale)
+// back, so that d stays in range.  By one cluster (one block took 280 us for 2^20 rows).
+__global__ void __cluster_dims__(kScaleBlocks, 1, 1) __launch_bounds__(1024) grad_scales(LinearGradArgs g, float* scale, float* row_scale)
 {
-  __shared__ float room[32];
+  namespace cg = cooperative_groups;
+  __shared__ float room[32], mine;
+  const int64_t from = blockIdx.x * 1024 + threadIdx.x;
   float most = 0.f;
-  for (int64_t i = threadIdx.x; i < g.fwd.n_rows; i += 1024) most = fmaxf(most, fabsf(g.upstream[i * g.upstream_stride]));
+#pragma unroll 4
+  for (int64_t i = from; i < g.fwd.n_rows; i += kScaleBlocks * 1024) most = fmaxf(most, fabsf(g.upstream[i * g.upstream_stride]));
   most = max_lanes(most);
   if (threadIdx.x % 32 == 0) room[threadIdx.x / 32] = most;
   __syncthreads();
-  most  = max_lanes(room[threadIdx.x % 32]);
+  most = max_lanes(room[threadIdx.x % 32]);
+  if (threadIdx.x == 0) mine = most;
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  for (int b = 0; b < kScaleBlocks; ++b) most = fmaxf(most, *cluster.map_shared_rank(&mine, b));
+  cluster.sync();  // the others' shared memory has been read
   int e = 0;
   if (most > 0.f && most < INFINITY) frexpf(most, &e);
   e                = max(-100, min(100, e));
   const float down = ldexpf(1.f, -e);
-  if (threadIdx.x == 0) *scale = ldexpf(1.f, e);
-  for (int64_t i = threadIdx.x; i < g.fwd.n_rows; i += 1024) row_scale[i] = g.upstream[i * g.upstream_stride] * down;
+  if (from == 0) *scale = ldexpf(1.f, e);
+#pragma unroll 4
+  for (int64_t i = from; i < g.fwd.n_rows; i += kScaleBlocks * 1024) row_scale[i] = g.upstream[i * g.upstream_stride] * down;
 }
 
 // d of the classes that the teacher names, in a piece of the classes.
@@ -940,7 +951,7 @@ cudaError_t run_linear(bool bf16, const LinearArgs& given, const Reduced& out, v
     linear_rows<T, 32><<<blocks, kThreads, bytes, s>>>(a, w.parts, tiles, out, sums, w.ticket);
   else
     linear_rows<T, kThreads><<<blocks, kThreads, bytes, s>>>(a, w.parts, tiles, out, sums, w.ticket);
-  count_launches(2);
+  count_launches(small ? 1 : 2);
   return cudaGetLastError();
 }
 
@@ -1017,7 +1028,7 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
   const bool per_row   = g.factor == nullptr;
   const bool scaled    = per_row && !bf16;  // (bf16 has the range of the upstream values itself)
   int launched         = scaled;
-  if (scaled) grad_scales<<<1, 1024, 0, s>>>(g, scale, row_scale);
+  if (scaled) grad_scales<<<kScaleBlocks, 1024, 0, s>>>(g, scale, row_scale);
   Work w{};
   w.bf16        = bf16;
   w.c           = 1.4426950408889634f / a.temperature;
