@@ -8,8 +8,8 @@
 //
 // Bound by memory: the forward pass reads the logits once (running maximum and sum), the backward pass
 // reads them again and writes as much.  What a teacher names in a row is the work of one warp, whose chain of
-// dependent loads, votes and logarithms takes as long as reading some 32 KB.  Rows of up to kWarpCols
-// classes therefore belong to one warp altogether, and many warps hide it; longer ones to a block of eight
+// dependent loads, votes and logarithms takes as long as reading some 32 KB.  Short rows
+// therefore belong to one warp altogether, and many warps hide it; longer ones to a block of eight
 // warps that read, while a ninth prepares the next row and a tenth finishes the last.  Where rows are few,
 // several blocks read parts of one and a warp joins their maxima and sums.  Many rows of a few classes belong to one
 // thread each, from a tile in shared memory.
@@ -24,7 +24,13 @@ namespace {
 constexpr int kThreads  = 256;
 constexpr int kWide     = kThreads + 64;  // eight warps that read, two for the teacher
 constexpr int kWideRows = 3;              // blocks of an SM (four with 4 pieces: 204 against 197 us, 4096 x 131,072)
-constexpr int kWarpCols = 2048;           // longest rows of one warp
+constexpr int kWarpCols = 2048;           // rows that belong to one warp
+// ... and where there are kWarpLeast of them per SM: longer ones whose logits take up to kWarpBytes, and in the
+// gradient, of 16 bits, which the instructions bound, up to kWarpLong.  (Loss and gradient by blocks and by warps, us:
+// 20,000 x 3000 bf16 101, 94 and 50, 46; 20,000 x 6000 bf16 135, 123 and 83, 97; 20,000 x 3000 fp32 121, 86 and 73, 97.)
+constexpr int kWarpLeast = 8;
+constexpr int kWarpBytes = 16384;
+constexpr int kWarpLong  = 8192;
 constexpr int kSegment  = 8192;           // fewest elements of a row that are worth a block of their own
 constexpr int kMostBits = 1 << 17;        // classes that a block marks (three rows of it: 48 KB)
 constexpr int kMostSegs = 64;
@@ -538,6 +544,10 @@ cudaError_t launch_rows(void (*kernel)(P...), int blocks, bool one_cluster, int 
   return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
 }
 
+bool by_warps(const LossArgs& a, int n_sms, bool longer)
+{
+  return a.n_cols <= kWarpCols || (longer && a.n_rows >= static_cast<int64_t>(kWarpLeast) * n_sms);
+}
 bool by_tiles(const LossArgs& a, int n_sms)
 {
   return a.n_cols <= kTileCols && a.teacher.k <= kTileTop && a.n_rows >= static_cast<int64_t>(kTileLeast) * n_sms;
@@ -558,7 +568,7 @@ cudaError_t run_loss(const LossArgs& a, const Reduced& out, void* workspace, int
   int segs           = segments(a.n_rows, a.n_cols, n_sms, REST);
   const int64_t cols = part_cols(a.n_cols, segs);
   segs               = segs == 1 ? 1 : static_cast<int>((a.n_cols + cols - 1) / cols);
-  const bool narrow  = a.n_cols <= kWarpCols || segs > 1;
+  const bool narrow  = segs > 1 || by_warps(a, n_sms, a.n_cols * sizeof(T) <= kWarpBytes);
   const int per      = narrow ? kThreads / 32 : 1;
   const int64_t need = (a.n_rows + per - 1) / per, most = (narrow ? 8ll : kWideRows) * n_sms;
   int blocks         = static_cast<int>(need < most ? need : most);
@@ -607,7 +617,7 @@ cudaError_t run_grad(const LossGradArgs& g, int n_sms, cudaStream_t s)
     count_launches(1);
     return cudaGetLastError();
   }
-  const bool warp    = a.n_cols <= kWarpCols;
+  const bool warp    = by_warps(a, n_sms, sizeof(T) == 2 && a.n_cols <= kWarpLong);
   const int per      = warp ? kThreads / 32 : 1;
   int segs           = warp ? 1 : segments(a.n_rows, a.n_cols, n_sms, false);
   const int64_t cols = part_cols(a.n_cols, segs);

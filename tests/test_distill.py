@@ -324,6 +324,20 @@ def test_masks_of_teacher_and_student(c, tail, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("n,c,k,dtype", [(1300, 2049, 40, "bf16"), (1300, 4096, 3, "fp32"), (1211, 4097, 9, "fp32"),
+                                         (1200, 8191, 16, "fp16"), (1200, 8193, 2, "bf16"), (1183, 6000, 5, "bf16")])
+@pytest.mark.parametrize("tail", ["renormalise", "bucket"])
+def test_many_rows_of_thousands_of_classes(n, c, k, dtype, tail):
+    """On both sides of where such rows belong to a warp each (at most 256 terms per lane); rows 3 elements apart."""
+    z, v, i, lse = make(n, c + 3, k, dtype, c, 2.0)
+    z, i = z[:, :c], i % c  # (some classes may be named twice)
+    lse = torch.logsumexp(v.double() / 2.0, 1).float() + 0.25
+    check_loss(z, v, i, lse if tail == "bucket" else None, 2.0, "mean")
+    up = torch.rand((n,), generator=gen(4), device="cuda")
+    check_loss(z, v, i, lse if tail == "bucket" else None, 2.0, "none", up)
+
+
+@gpu
 def test_rows_that_do_not_count_have_no_gradient_whatever_is_in_them():
     from cuml_b200 import distill
 
