@@ -10,7 +10,8 @@
 // again, from L1 or L2, dealt out anew to all threads.  Random rows leave little more than k candidates whatever
 // the row's length; each finds its place by counting the larger ones.  Where there are more than the list
 // holds, the k-th key itself is found bit by bit.  Shorter rows stay in the registers of a warp, which
-// finds its bound by votes on all of them.  Rows of a few classes are taken by one thread each, from a tile in
+// finds its bound by votes on all of them, and many rows of up to 16 KB are a
+// warp's that reads them twice.  Rows of a few classes are taken by one thread each, from a tile in
 // shared memory, which keeps its best sorted in registers.
 //
 // Bound by memory: one pass over the scores, which also takes the running maximum and sum of the
@@ -33,6 +34,11 @@ constexpr int kWarpCols = 2048;  // longest rows of a warp (fp64: 1024)
 constexpr int kWarpTop  = 24;    // k up to which a warp finds its bound by its lanes' best alone, and the largest of
                                  // rows above 1024 (30,000 x 2000: fp32, k 10 70 us, by blocks 258; bf16, k 100
                                  // 414 and 367)
+// Rows of a warp that its registers do not hold: bytes, and rows per SM from which on.  (By blocks and this way, us:
+// 30,000 x 3000 bf16, k 10, 268 and 104; 20,000 x 8192 bf16 189 and 107, fp32 equal; 20,000 x 2048 fp64 456 and 136;
+// 1184 x 4096 bf16 14.8 and 12.8, x 8192 14.7 and 16.8.)
+constexpr int kLongBytes = 16384;
+constexpr int kLongLeast = 8;
 constexpr int kCount    = 160;   // candidates of a block that are placed by counting; more are sorted
 constexpr int kCluster  = 8;     // blocks that share a row of up to kJoinCols and join their lists themselves
 constexpr int64_t kJoinCols = 1 << 17;  // (1 x 50,001, k 20: 13.8 us by two kernels, 10.7 this way, 14.2 by 16 blocks)
@@ -228,6 +234,24 @@ __device__ __forceinline__ void arrange(K* list, int got, int k, F put)
   }
 }
 
+// The first NaN among a thread's elements of a row, or ~0.
+template <class T>
+__device__ __forceinline__ uint32_t first_nan(const T* x, int64_t n, int tid, int threads)
+{
+  uint32_t first = ~0u;
+  visit_row<1>(
+    x, n, tid, threads,
+    [&](int64_t i, T e) {
+      if (widen(e) != widen(e)) first = min(first, static_cast<uint32_t>(i));
+    },
+    [&](int64_t i, const Piece<T>& p) {
+#pragma unroll
+      for (int e = 0; e < Piece<T>::N; ++e)
+        if (widen(p.v[e]) != widen(p.v[e])) first = min(first, static_cast<uint32_t>(i + e));
+    });
+  return first;
+}
+
 // A segment of a row per block.  segs == 1: the row's answer; else its k best keys and its sum, which the first
 // block of a cluster of segs blocks joins, or top_join does.
 template <class T, bool PROB>
@@ -282,17 +306,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
         for (int e = 0; e < N; ++e) sum.add(v[e], c, plain);
       });
     if (sum.s != sum.s) {  // a NaN, or infinities: the first NaN of the group is its best
-      uint32_t first = ~0u;
-      visit_row<1>(
-        x, n, tid, kThreads,
-        [&](int64_t i, T e) {
-          if (widen(e) != widen(e)) first = min(first, static_cast<uint32_t>(i));
-        },
-        [&](int64_t i, const Piece<T>& p) {
-#pragma unroll
-          for (int e = 0; e < N; ++e)
-            if (widen(p.v[e]) != widen(p.v[e])) first = min(first, static_cast<uint32_t>(i + e));
-        });
+      const uint32_t first = first_nan(x, n, tid, kThreads);
       if (first != ~0u) {
         top = static_cast<V>(NAN);
         at  = first;
@@ -702,6 +716,126 @@ __global__ void __launch_bounds__(kThreads, warps_fit(U * 16 / sizeof(T) * sizeo
   }
 }
 
+// A row per warp that its registers do not hold, of more than 32 x 32 elements; k <= kWarpTop.  Its lanes' best give the
+// bound, as above, and what reaches it is read again; where that is more than the list holds the k-th key is found
+// bit by bit as in top_segments.  (A bound by values alone took 5.7 ms where all but five of 4096 scores of 8192 rows
+// were -inf.)
+template <class T, bool PROB>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(TopArgs a)
+{
+  using V = typename ValueOf<T>::type;
+  using K = typename KeyOf<T>::type;
+  constexpr int N = Piece<T>::N, ROWS = kThreads / 32;
+  __shared__ K lists[ROWS][kWarpList];
+  __shared__ int counts[ROWS];
+  const int lane = threadIdx.x % 32, k = a.k;
+  K* list          = lists[threadIdx.x / 32];
+  int* found       = &counts[threadIdx.x / 32];
+  const V c        = static_cast<V>(1.4426950408889634 * a.inv_temperature);
+  const bool plain = a.inv_temperature == 1.0;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / 32; row < a.n_rows;
+       row += static_cast<int64_t>(gridDim.x) * ROWS) {
+    const T* x = static_cast<const T*>(a.scores) + row * a.row_stride;
+    // the lane's best score, the first element of the piece that holds it, and the sum
+    V best      = lowest<V>();
+    uint32_t at = ~0u;
+    Sum<V, PROB> sum;
+    visit_row<2 * kInFlight>(
+      x, a.n_cols, lane, 32,
+      [&](int64_t i, T e) {
+        const V v = widen(e);
+        if (v > best || at == ~0u) at = static_cast<uint32_t>(i);
+        best      = larger(best, v);
+        sum.reach(v, c);
+        sum.add(v, c, plain);
+      },
+      [&](int64_t i, const Piece<T>& p) {
+        V v[N], most;
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = widen(p.v[e]);
+        most = v[0];
+#pragma unroll
+        for (int e = 1; e < N; ++e) most = larger(most, v[e]);
+        if (most > best || at == ~0u) at = static_cast<uint32_t>(i);
+        best = larger(best, most);
+        sum.reach(most, c);
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum.add(v[e], c, plain);
+      });
+    double dropped = 0;
+    Running<V> all;
+    all.m = V(0);
+    if (PROB) {
+      dropped = sum_lanes(static_cast<double>(sum.s) + sum.dropped);
+    } else {
+      all.m = sum.first ? lowest<V>() : sum.r;
+      all.s = sum.s;
+      all.join_lanes(V(1));
+    }
+    if (sum.s != sum.s) {  // a NaN, or infinities
+      const uint32_t first = first_nan(x, a.n_cols, lane, 32);
+      if (first != ~0u) {
+        best = static_cast<V>(NAN);
+        at   = first;
+      }
+    }
+    // Puts what is above or equal into the list, as far as that goes; how many there are.
+    auto collect = [&](const K& bound, V least) {
+      __syncwarp();
+      if (lane == 0) *found = 0;
+      __syncwarp();
+      auto take = [&](int64_t i, T e) {
+        const K key = K::of(widen(e), static_cast<uint32_t>(i));
+        if (bound.above(key)) return;
+        const int to = atomicAdd(found, 1);
+        if (to < kWarpList) list[to] = key;
+      };
+      visit_row<kInFlight>(x, a.n_cols, lane, 32, take, [&](int64_t i, const Piece<T>& p) {
+        uint32_t some = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) some |= !(widen(p.v[e]) < least) ? 1u << e : 0u;
+        if (some == 0) return;
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (some >> e & 1) take(i + e, p.v[e]);
+      });
+      __syncwarp();
+      return *static_cast<volatile int*>(found);
+    };
+    // tau: a key that k lanes' best reach; the last element of its piece stands for a lane's best
+    const K mine = K::of(best, at + N - 1);
+    K tau        = K::none();
+    for (int bit = K::kBits - 1; bit >= 0; --bit) {
+      const K next   = tau.with(bit);
+      const int some = __popc(__ballot_sync(~0u, !next.above(mine)));
+      if (some < k) continue;
+      tau = next;
+      if (some <= k + 2) break;
+    }
+    int got = collect(tau, tau.value());
+    if (got > kWarpList) {
+      K bound = K::none();
+      for (int bit = K::kBits - 1; bit >= 0 && got > kWarpList; --bit) {
+        const K next   = bound.with(bit);
+        const int some = collect(next, next.value());
+        if (some < k) continue;
+        bound = next;
+        got   = some;
+      }
+    }
+    for (int i = lane; i < got; i += 32) {
+      const K key = list[i];
+      int place   = 0;
+#pragma unroll 4
+      for (int j = 0; j < got; ++j) place += list[j].above(key);
+      if (place >= k) continue;
+      write_top<T>(a, row, place, key);
+      if (place == 0) write_lse(a, row, all.m, all.s, dropped, key);
+    }
+    __syncwarp();
+  }
+}
+
 // A row per thread: n_cols x sizeof(T) <= kTileBytes, k <= TOP.
 template <class T, int TOP, bool PROB>
 __global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
@@ -850,6 +984,13 @@ cudaError_t run_top(const TopArgs& a, void* workspace, int n_sms, cudaStream_t s
   if (a.n_cols <= 512) return run_warps<T, kPieces, 0>(a, n_sms, s);
   if (a.n_cols <= 1024) return run_warps<T, 2 * kPieces, 0>(a, n_sms, s);
   if (a.n_cols <= kWarpCols && sizeof(T) < 8 && a.k <= kWarpTop) return run_warps<T, 4 * kPieces, 0>(a, n_sms, s);
+  if (bytes <= kLongBytes && a.k <= kWarpTop && a.n_rows >= static_cast<int64_t>(kLongLeast) * n_sms) {
+    const int64_t need = (a.n_rows + kThreads / 32 - 1) / (kThreads / 32), most = 16ll * n_sms;
+    const auto kernel  = a.probabilities ? top_long<T, true> : top_long<T, false>;
+    kernel<<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(a);
+    count_launches(1);
+    return cudaGetLastError();
+  }
   int segs             = segments(a.n_rows, a.n_cols, n_sms);
   const bool clustered = segs > 1 && a.n_cols <= kJoinCols;
   if (clustered) {

@@ -204,6 +204,34 @@ def test_top_of_hard_rows(n, c, k, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("c", [1025, 2049, 4001, 8192])
+@pytest.mark.parametrize("k", [1, 7, 24, 25])
+def test_top_of_many_rows_of_thousands_of_classes(c, k, dtype):
+    """As many rows as belong to a warp each, whose lanes' best give the bound: ordinary ones, ties, both zeros,
+    infinities, NaN, fewer scores than k above a mask, rows in order, and the best all in one lane's pieces."""
+    t = TYPES[dtype]
+    x = torch.randn((1200, c + 5), generator=gen(c + k), device="cuda").to(t)[:, 1:c + 1]  # (rows off the 16-byte boundaries)
+    x[10] = 0.0
+    x[10, 1::2] = -0.0
+    x[20] = float("-inf")
+    x[30, ::3] = torch.finfo(t).min
+    x[30, 5] = x[30, c - 1] = float("nan")
+    x[40] = torch.arange(c, device="cuda") / c
+    x[50] = torch.finfo(t).min
+    x[50, 7] = float("inf")
+    x[60, 3:] = float("-inf")
+    x[70, 3:] = torch.finfo(t).min
+    x[80] = -1.0
+    x[80, torch.arange(c, device="cuda") // (16 // t.itemsize) % 32 < 3] = 1.0
+    x[90] = float("nan")
+    x[100] = torch.where(torch.arange(c, device="cuda") % 32 < 16, (torch.arange(c, device="cuda") % 401) / 401.0, -1.0).to(t)
+    check_top(x, k)
+    x[20] = x[10]
+    check_top(torch.softmax(x.float().nan_to_num(0.0, 5.0, -5.0), 1).to(t), k, 2.0, probabilities=True)
+
+
+@gpu
 def test_top_where_the_candidates_overflow_their_list():
     """A row whose best 8 x 200 + 2000 scores lie in the groups of few threads: the k-th key is found by bits."""
     for dtype, per in ((torch.float32, 4), (torch.float64, 2), (torch.bfloat16, 8)):
