@@ -302,17 +302,25 @@ __global__ void __launch_bounds__(kTileRows) loss_tiles(LossArgs a, Reduced out,
       counts   = !(total == 0.f);
       norm     = counts ? 1.f / total : 1.f;
     }
-    // the student
-    Stream<float> r;
-    float most = lowest<float>();
-    for (int i = 0; i < cols; ++i) most = fmaxf(most, widen(x[i]));
-    if (most > lowest<float>()) r.raise(most, c, 0.f);
-    float others = 0.f;
+    // the student: maximum and sum; with REST of the others apart, which may lie far below the named ones
+    Running<float> r, others;
     for (int i = 0; i < cols; ++i) {
-      const float e = power((widen(x[i]) - r.b) * c);
-      r.s += e;
-      if (REST && !(named >> i & 1)) others += e;
+      const float v = widen(x[i]);
+      if (REST && !(named >> i & 1))
+        others.m = fmaxf(others.m, v);
+      else
+        r.m = fmaxf(r.m, v);
     }
+    const float base = base_of(r.m), base_others = base_of(others.m);
+    for (int i = 0; i < cols; ++i) {
+      const bool other = REST && !(named >> i & 1);
+      const float e    = power((widen(x[i]) - (other ? base_others : base)) * c);
+      if (other)
+        others.s += e;
+      else
+        r.s += e;
+    }
+    if (REST) r.join(others.m, others.s, c);
     const double log_s = log_sum(r.s);
     counts             = counts && !(r.s == 0.f);
     double loss        = 0;
@@ -332,8 +340,9 @@ __global__ void __launch_bounds__(kTileRows) loss_tiles(LossArgs a, Reduced out,
     }
     float factor = 1.f;
     if (REST && rest != 0.f) {
-      loss += rest * (log_sum(rest) - (log_sum(others) - log_s));
-      factor = 1.f - rest / (others / r.s);
+      const double log_rest = (static_cast<double>(others.m) - r.m) * inv_t + log_sum(others.s) - log_s;
+      loss += rest * (log_sum(rest) - log_rest);
+      factor = 1.f - rest / (others.s * power((others.m - base_of(r.m)) * c) / r.s);
     }
     if (!counts) loss = 0;
     loss *= static_cast<double>(a.temperature) * a.temperature;

@@ -1,0 +1,74 @@
+"""The distillation operators at the ends of their ranges, against 64 bits: low temperatures, logits far apart, teachers
+whose log-sum-exp is large, the largest scores; and what autograd offers beside a plain backward pass.
+
+u, S and the counting of roundings are those of test_distill.py."""
+import pytest
+import torch
+
+from tests.test_distill import S, TYPES, U, check_values, gen, gpu
+
+NEG = float("-inf")
+# rows, classes, entries: a thread per row, a warp per short row, parts of a row, a block per row, a warp per long row
+KERNELS = [(5000, 12, 4), (6000, 64, 16), (7, 12, 4), (300, 130, 20), (9, 3000, 8), (400, 3000, 8), (1300, 2500, 5),
+           (3, 50_001, 20)]
+
+
+def bucket(z, values, index, lse, temperature, least=0.0):
+    """(losses, gradients, allowed errors of both without the gradients' own rounding) with the rest as one more class, of
+    rows that all count and whose entries name no class twice; a rest below `least` is none.
+
+    With s the softmax over the classes that are not named, p_r what is left of 1 and P the sum of all of p,
+    d loss / d z_c = T (P q_c - p_c) for named classes and T (P q_c - p_r s_c) for the others.  Each logarithm is off
+    by S; q, p_r s and p by 2 S relative (of s and q: an exponent of up to 127, rounded twice, beside S)."""
+    z, v, lse = z.detach().cpu().double(), values.cpu().double() / temperature, lse.cpu().double()
+    index, (n, c) = index.cpu().long(), z.shape
+    inside = (index >= 0) & (index < c)
+    at = torch.where(inside, index, 0)
+    each = torch.where(inside, (v - lse[:, None]).exp(), torch.zeros_like(v))
+    p = torch.zeros((n, c), dtype=torch.float64).scatter_add_(1, at, each)
+    named = torch.zeros((n, c)).scatter_add_(1, at, inside.float()) > 0
+    rest = 1 - each.sum(1)
+    rest = torch.where((rest < least) | named.all(1), torch.zeros_like(rest), rest)
+    y = z / temperature
+    all_of, others = torch.logsumexp(y, 1), y.masked_fill(named, NEG)
+    left = torch.logsumexp(others, 1)
+    log_q = y - all_of[:, None]
+    loss = torch.where(p > 0, p * (p.log() - log_q), torch.zeros_like(p)).sum(1)
+    loss = loss + torch.where(rest > 0, rest * (rest.log() - (left - all_of)), torch.zeros_like(rest))
+    s = torch.where(rest[:, None] > 0, (others - left[:, None]).exp(), torch.zeros_like(p)).nan_to_num()
+    mass = (each.sum(1) + rest)[:, None]
+    grad = mass * log_q.exp() - p - rest[:, None] * s
+    size = mass * log_q.exp() + p + rest[:, None] * s
+    t2 = temperature ** 2
+    return loss * t2, grad * temperature, 3 * S * t2 + (loss * t2).abs() * 4 * U, 2 * S * size * temperature
+
+
+def apart(n, c, k, dtype, temperature, gap, seed=0):
+    """Logits whose named classes lie `gap` temperatures above the others (below them in every third row); a teacher that
+    leaves about a tenth."""
+    g = gen(seed + c)
+    order = torch.rand((n, c), generator=g, device="cuda").argsort(1)[:, :k]
+    z = torch.randn((n, c), generator=g, device="cuda")
+    sign = torch.where(torch.arange(n, device="cuda") % 3 == 1, -gap, gap)[:, None]
+    z = z.scatter_add_(1, order, sign.expand(n, k).to(z.dtype)) * temperature
+    v = torch.randn((n, k), generator=g, device="cuda") * temperature
+    return z.to(TYPES[dtype]), v, order.int(), torch.logsumexp(v.double() / temperature, 1).float() + 0.1
+
+
+# ---- the rest as one more class --------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("n,c,k", KERNELS)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("gap", [60.0, 90.0])
+def test_losses_of_named_classes_far_from_the_others(n, c, k, dtype, gap):
+    """The loss is finite and the same whichever kernel takes the row."""
+    from cuml_b200 import distill
+
+    for temperature in (1.0, 0.1, 0.01):
+        z, v, i, lse = apart(n, c, k, dtype, temperature, gap)
+        loss = distill.distillation_loss(z, (v, i, lse), temperature=temperature, tail="bucket", reduction="none")
+        rows, _, off, _ = bucket(z, v, i, lse, temperature)
+        check_values(loss, rows, 0.0, off, U)
+        few = distill.distillation_loss(z[:3], (v[:3], i[:3], lse[:3]), temperature=temperature, tail="bucket",
+                                        reduction="none")
+        check_values(loss[:3], few.cpu().double(), 0.0, 2 * off[:3], 2 * U)
