@@ -43,6 +43,14 @@ struct Teacher {
   int64_t ignore;          // an index that does not count (besides those outside the classes)
 };
 
+// In 64 bits: rounded to 32, 0.1 is off by 2^-26 of itself, and what is left of 1 by that part of a score.
+struct Temperature {
+  double t = 1.0, inverse = 1.0;
+  float c = 0.f;  // log2(e) / T
+  Temperature() = default;
+  explicit Temperature(double t) : t(t), inverse(1.0 / t), c(static_cast<float>(1.4426950408889634 / t)) {}
+};
+
 // What the teacher names in each row, kept for the gradient: (n_rows, k) each.
 struct Named {
   float* logit;  // of the class; not used by the loss on logits
@@ -55,7 +63,7 @@ struct LossArgs {
   const void* logits;
   int64_t n_rows, n_cols, row_stride;
   Teacher teacher;
-  float temperature;
+  Temperature temperature;
   float* row_loss;   // (n_rows)
   float4* row_stats; // (n_rows) max, 1 / sum, factor of the classes outside the teacher's, 1: the row counts
   Named named;
@@ -85,7 +93,7 @@ struct LinearArgs {
   const void* weight;  // (n_cols, width)
   int64_t n_rows, n_cols, width, hidden_stride, weight_stride;
   Teacher teacher;     // no logsumexp
-  float temperature;
+  Temperature temperature;
   float* row_loss;
   float4* row_stats;   // as in LossArgs; the factor is 1
   Named named;

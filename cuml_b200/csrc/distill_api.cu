@@ -202,7 +202,7 @@ int b2fil_distill_loss(int dtype, const void* logits, int64_t n_rows, int64_t n_
   a.n_rows      = n_rows;
   a.n_cols      = n_cols;
   a.row_stride  = row_stride;
-  a.temperature = static_cast<float>(temperature);
+  a.temperature = Temperature(temperature);
   a.row_loss    = row_loss;
   a.row_stats   = reinterpret_cast<float4*>(row_stats);
   a.named       = Named{nullptr, named_p, named_at};
@@ -234,7 +234,7 @@ int b2fil_distill_loss_grad(int dtype, const void* logits, int64_t n_rows, int64
   a.n_rows          = n_rows;
   a.n_cols          = n_cols;
   a.row_stride      = row_stride;
-  a.temperature     = static_cast<float>(temperature);
+  a.temperature     = Temperature(temperature);
   a.row_stats       = const_cast<float4*>(reinterpret_cast<const float4*>(row_stats));
   a.teacher.k       = k;
   a.named           = Named{nullptr, const_cast<float*>(named_p), const_cast<int32_t*>(named_at)};
@@ -295,7 +295,7 @@ int b2fil_linear_loss(int dtype, const void* hidden, int64_t hidden_stride, cons
   a.width         = width;
   a.hidden_stride = hidden_stride;
   a.weight_stride = weight_stride;
-  a.temperature   = static_cast<float>(temperature);
+  a.temperature   = Temperature(temperature);
   a.row_loss      = row_loss;
   a.row_stats     = reinterpret_cast<float4*>(row_stats);
   a.named         = Named{named_logit, named_p, named_at};
@@ -363,7 +363,7 @@ int b2fil_linear_loss_grad(int dtype, const void* hidden, int64_t hidden_stride,
   a.hidden_stride   = hidden_stride;
   a.weight_stride   = weight_stride;
   a.teacher.k       = k;
-  a.temperature     = static_cast<float>(temperature);
+  a.temperature     = Temperature(temperature);
   a.row_stats       = const_cast<float4*>(reinterpret_cast<const float4*>(row_stats));
   a.named           = Named{const_cast<float*>(named_logit), const_cast<float*>(named_p), const_cast<int32_t*>(named_at)};
   g.upstream        = upstream;

@@ -640,8 +640,8 @@ __global__ void __launch_bounds__(kThreads) linear_rows(LinearArgs a, const floa
   char* mine         = smem + slot * (entry_bytes(k) + static_cast<size_t>(k) * 4);
   const Entries e    = entries_at(mine, k);
   float* logit       = reinterpret_cast<float*>(e.at + k);
-  const float c      = 1.4426950408889634f / a.temperature;
-  const double inv_t = 1.0 / a.temperature;
+  const float c      = a.temperature.c;
+  const double inv_t = a.temperature.inverse;
   double sum = 0, count = 0;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + slot; row < a.n_rows;
        row += static_cast<int64_t>(gridDim.x) * ROWS) {
@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(kThreads) linear_rows(LinearArgs a, const floa
       const bool counts = t.counts && !(r.s == 0.f);
       double loss = named_loss(e, k, t, inv_t, r.m, log_sum(r.s), [&](int j, int) { return logit[j]; });
       if (!counts) loss = 0;
-      loss *= static_cast<double>(a.temperature) * a.temperature;
+      loss *= a.temperature.t * a.temperature.t;
       for (int j = lane; j < k; j += 32) {
         a.named.logit[row * k + j] = logit[j];
         a.named.p[row * k + j]     = e.p[j];
@@ -929,7 +929,7 @@ cudaError_t run_linear(bool bf16, const LinearArgs& given, const Reduced& out, v
   Work w{};
   w.products = 1;
   w.bf16     = bf16;
-  w.c        = 1.4426950408889634f / a.temperature;
+  w.c        = a.temperature.c;
   w.ticket   = reinterpret_cast<int*>(sums + 8 * n_sms);
   w.parts    = reinterpret_cast<float2*>(sums + 8 * n_sms + 1);
   const bool small = a.n_cols <= kFewClasses && a.n_rows * a.n_cols <= kSmallLogits / a.width;
@@ -1031,7 +1031,7 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
   if (scaled) grad_scales<<<kScaleBlocks, 1024, 0, s>>>(g, scale, row_scale);
   Work w{};
   w.bf16        = bf16;
-  w.c           = 1.4426950408889634f / a.temperature;
+  w.c           = a.temperature.c;
   w.stats       = a.row_stats;
   w.row_scale   = scaled ? row_scale : per_row ? g.upstream : nullptr;
   w.row_step    = scaled ? 1 : g.upstream_stride;
@@ -1040,7 +1040,7 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
   w.diff_scale  = d_scale;
   w.planes      = plan.planes;
   w.plane_rows  = static_cast<int>(plan.plane_rows);
-  w.scale       = Scale{scaled ? scale : per_row ? nullptr : g.upstream, g.factor, a.temperature / d_scale};
+  w.scale       = Scale{scaled ? scale : per_row ? nullptr : g.upstream, g.factor, static_cast<float>(a.temperature.t) / d_scale};
   w.named       = a.named;
   w.k           = a.teacher.k;
   w.ticket      = ticket;

@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kThreads) loss_parts(LossArgs a, int64_t seg_c
   uint32_t* bits      = reinterpret_cast<uint32_t*>(smem);
   const int64_t begin = blockIdx.x * seg_cols;
   const int64_t n     = min(seg_cols, a.n_cols - begin);
-  const float c       = 1.4426950408889634f / a.temperature;
+  const float c       = a.temperature.c;
   for (int64_t row = blockIdx.y; row < a.n_rows; row += gridDim.y) {
     const T* x = static_cast<const T*>(a.logits) + row * a.row_stride + begin;
     if (REST) {
@@ -158,7 +158,7 @@ __device__ __forceinline__ void finish_row(const LossArgs& a, int64_t row, const
     factor = 1.f - t.rest / (others.s * power((others.m - base_of(r.m)) * c) / r.s);
   }
   if (!counts) loss = 0;
-  loss *= static_cast<double>(a.temperature) * a.temperature;
+  loss *= a.temperature.t * a.temperature.t;
   for (int j = lane; j < k; j += 32) {
     a.named.p[row * k + j]  = e.p[j];
     a.named.at[row * k + j] = e.at[j];
@@ -209,8 +209,8 @@ __global__ void __launch_bounds__(kThreads, 5) loss_narrow(LossArgs a, int segs,
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, k = a.teacher.k;
   const Entries e    = entries_at(smem + warp * warp_room, k);
   uint32_t* bits     = reinterpret_cast<uint32_t*>(e.at + k);
-  const float c      = 1.4426950408889634f / a.temperature;
-  const double inv_t = 1.0 / a.temperature;
+  const float c      = a.temperature.c;
+  const double inv_t = a.temperature.inverse;
   double sum = 0, count = 0;
   if (REST && segs == 0) {
     for (int w = lane; w < bit_bytes(a.n_cols) / 4; w += 32) bits[w] = 0;
@@ -247,8 +247,8 @@ __global__ void __launch_bounds__(kTileRows) loss_tiles(LossArgs a, Reduced out,
   const Teacher t = a.teacher;
   const int k = t.k, cols = static_cast<int>(a.n_cols);
   const TileShape<T> shape(cols);
-  const float c = 1.4426950408889634f / a.temperature, ti = 1.f / a.temperature;
-  const double inv_t = 1.0 / a.temperature;
+  const float c = a.temperature.c, ti = static_cast<float>(a.temperature.inverse);
+  const double inv_t = a.temperature.inverse;
   const bool whole   = without_gaps<T>(a.logits, a.row_stride, cols);
   double sum = 0, count = 0;
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * kTileRows; first < a.n_rows;
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kTileRows) loss_tiles(LossArgs a, Reduced out,
       factor = 1.f - rest / (others.s * power((others.m - base_of(r.m)) * c) / r.s);
     }
     if (!counts) loss = 0;
-    loss *= static_cast<double>(a.temperature) * a.temperature;
+    loss *= a.temperature.t * a.temperature.t;
     a.row_loss[row]  = static_cast<float>(loss);
     a.row_stats[row] = make_float4(r.m, 1.f / r.s, factor, counts ? 1.f : 0.f);
     sum += loss;
@@ -363,8 +363,8 @@ __global__ void __launch_bounds__(kTileRows) grad_tiles(LossGradArgs g)
   const LossArgs& a = g.fwd;
   const int k = a.teacher.k, cols = static_cast<int>(a.n_cols);
   const TileShape<T> shape(cols);
-  const float c     = 1.4426950408889634f / a.temperature;
-  const float scale = (g.factor ? *g.factor : 1.f) * a.temperature;
+  const float c     = a.temperature.c;
+  const float scale = (g.factor ? *g.factor : 1.f) * static_cast<float>(a.temperature.t);
   const bool whole_in = without_gaps<T>(a.logits, a.row_stride, cols), whole_out = without_gaps<T>(g.grad, g.grad_stride, cols);
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * kTileRows; first < a.n_rows;
        first += static_cast<int64_t>(gridDim.x) * kTileRows) {
@@ -408,8 +408,8 @@ __global__ void __launch_bounds__(kWide, kWideRows) loss_wide(LossArgs a, size_t
   __shared__ float2 parts[2][W];
   __shared__ TeacherRow teachers[3];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, k = a.teacher.k;
-  const float c      = 1.4426950408889634f / a.temperature;
-  const double inv_t = 1.0 / a.temperature;
+  const float c      = a.temperature.c;
+  const double inv_t = a.temperature.inverse;
   auto entries       = [&](int i) { return entries_at(smem + 3 * bits_room + i * entry_bytes(k), k); };
   auto bits          = [&](int i) { return reinterpret_cast<uint32_t*>(smem + i * bits_room); };
   auto logits        = [&](int64_t row) { return static_cast<const T*>(a.logits) + row * a.row_stride; };
@@ -474,10 +474,10 @@ __global__ void __launch_bounds__(kThreads) loss_grad(LossGradArgs g, int64_t se
   constexpr int ROWS = kThreads / THREADS, N = Piece<T>::N;
   const LossArgs& a = g.fwd;
   const int slot = threadIdx.x / THREADS, tid = threadIdx.x % THREADS, k = a.teacher.k;
-  const float c       = 1.4426950408889634f / a.temperature;
+  const float c       = a.temperature.c;
   const int64_t begin = blockIdx.y * seg_cols;
   const int64_t n     = min(seg_cols, a.n_cols - begin);
-  const float scale   = (g.factor ? *g.factor : 1.f) * a.temperature;
+  const float scale   = (g.factor ? *g.factor : 1.f) * static_cast<float>(a.temperature.t);
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + slot; row < a.n_rows;
        row += static_cast<int64_t>(gridDim.x) * ROWS) {
     const T* x     = static_cast<const T*>(a.logits) + row * a.row_stride + begin;

@@ -59,7 +59,7 @@ def apart(n, c, k, dtype, temperature, gap, seed=0):
 @gpu
 @pytest.mark.parametrize("n,c,k", KERNELS)
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
-@pytest.mark.parametrize("gap", [60.0, 90.0])
+@pytest.mark.parametrize("gap", [60.0, 90.0, 1e4])
 def test_losses_of_named_classes_far_from_the_others(n, c, k, dtype, gap):
     """The loss is finite and the same whichever kernel takes the row."""
     from cuml_b200 import distill
