@@ -65,7 +65,9 @@ struct LossArgs {
   Teacher teacher;
   Temperature temperature;
   float* row_loss;   // (n_rows)
-  float4* row_stats; // (n_rows) max, 1 / sum, factor of the classes outside the teacher's, 1: the row counts
+  // (n_rows), for the gradient.  q of a class is 2^((z - x) c) y, d / T of one that is not named 2^((z - z_o) c) w (z_o:
+  // the third component); all 0 where the row does not count.
+  float4* row_stats;
   Named named;
 };
 // reduction: 0 none, 1 sum, 2 mean over the rows that count.
@@ -95,7 +97,7 @@ struct LinearArgs {
   Teacher teacher;     // no logsumexp
   Temperature temperature;
   float* row_loss;
-  float4* row_stats;   // as in LossArgs; the factor is 1
+  float4* row_stats;   // (n_rows) max, 1 / sum, 1, 1: the row counts
   Named named;
 };
 size_t linear_workspace(const LinearArgs& a, int n_sms);

@@ -3,7 +3,8 @@
 // With q = softmax(z / T), p the teacher's probabilities of the classes that it names and, where the rest
 // of its distribution is one more class, p_r and q_r what is left on either side:
 //   loss  = T^2 [ sum_named p (log p - log q) + p_r (log p_r - log q_r) ]
-//   dloss / dz_c = T (q_c - p_c) for named classes, T q_c (1 - p_r / q_r) for the others.
+//   dloss / dz_c = T (q_c - p_c) for named classes, T (q_r - p_r) s_c for the others, s the softmax over these:
+// T q_c (1 - p_r / q_r), whose parts leave the range where q_r does, though p_r s_c does not.
 // Softmax cross entropy is the case of one named class of probability 1 and T = 1.
 //
 // Bound by memory: the forward pass reads the logits once (running maximum and sum), the backward pass
@@ -151,11 +152,12 @@ __device__ __forceinline__ void finish_row(const LossArgs& a, int64_t row, const
   const double log_s = log_sum(r.s);
   const bool counts  = t.counts && !(r.s == 0.f);  // (no class has a finite logit: no softmax)
   double loss        = named_loss(e, k, t, inv_t, r.m, log_s, [&](int, int at) { return widen(x[at]); });
-  float factor       = 1.f;
+  float4 stats       = make_float4(r.m, 1.f / r.s, r.m, 1.f / r.s);
   if (REST && t.rest != 0.f) {
     const double log_rest = (static_cast<double>(others.m) - r.m) * inv_t + log_sum(others.s) - log_s;
     loss += t.rest * (log_sum(t.rest) - log_rest);
-    factor = 1.f - t.rest / (others.s * power((others.m - base_of(r.m)) * c) / r.s);
+    stats.z = others.m;
+    stats.w = (others.s * power((others.m - base_of(r.m)) * c) / r.s - t.rest) / others.s;
   }
   if (!counts) loss = 0;
   loss *= a.temperature.t * a.temperature.t;
@@ -165,7 +167,7 @@ __device__ __forceinline__ void finish_row(const LossArgs& a, int64_t row, const
   }
   if (lane == 0) {
     a.row_loss[row]  = static_cast<float>(loss);
-    a.row_stats[row] = make_float4(r.m, 1.f / r.s, factor, counts ? 1.f : 0.f);
+    a.row_stats[row] = counts ? stats : make_float4(0.f, 0.f, 0.f, 0.f);
     sum += loss;
     count += counts;
   }
@@ -338,16 +340,17 @@ __global__ void __launch_bounds__(kTileRows) loss_tiles(LossArgs a, Reduced out,
       const double log_p = merged ? log(static_cast<double>(q)) : (v ? v[j] : 0.f) * inv_t - log_norm;
       loss += q * (log_p - ((static_cast<double>(widen(x[at[j]])) - r.m) * inv_t - log_s));
     }
-    float factor = 1.f;
+    float4 stats = make_float4(r.m, 1.f / r.s, r.m, 1.f / r.s);
     if (REST && rest != 0.f) {
       const double log_rest = (static_cast<double>(others.m) - r.m) * inv_t + log_sum(others.s) - log_s;
       loss += rest * (log_sum(rest) - log_rest);
-      factor = 1.f - rest / (others.s * power((others.m - base_of(r.m)) * c) / r.s);
+      stats.z = others.m;
+      stats.w = (others.s * power((others.m - base_of(r.m)) * c) / r.s - rest) / others.s;
     }
     if (!counts) loss = 0;
     loss *= a.temperature.t * a.temperature.t;
     a.row_loss[row]  = static_cast<float>(loss);
-    a.row_stats[row] = make_float4(r.m, 1.f / r.s, factor, counts ? 1.f : 0.f);
+    a.row_stats[row] = counts ? stats : make_float4(0.f, 0.f, 0.f, 0.f);
     sum += loss;
     count += counts;
   }
@@ -377,8 +380,8 @@ __global__ void __launch_bounds__(kTileRows) grad_tiles(LossGradArgs g)
       const int64_t row = first + threadIdx.x;
       const float4 s    = a.row_stats[row];
       const float up    = g.upstream[row * g.upstream_stride] * scale;
-      const bool counts = s.w != 0.f;
-      const float base  = base_of(s.x), f = s.y * up * s.z;
+      const bool counts = s.y != 0.f;
+      const float base = base_of(s.x), base_others = base_of(s.z), f = s.w * up;
       // the named classes' from their logits, which are then put over the others'
       float named[kTileTop];
 #pragma unroll
@@ -386,7 +389,7 @@ __global__ void __launch_bounds__(kTileRows) grad_tiles(LossGradArgs g)
         const int at = j < k ? a.named.at[row * k + j] : -1;
         named[j]     = at >= 0 ? (power((widen(x[at]) - base) * c) * s.y - a.named.p[row * k + j]) * up : 0.f;
       }
-      for (int i = 0; i < cols; ++i) x[i] = narrow<T>(counts ? power((widen(x[i]) - base) * c) * f : 0.f);
+      for (int i = 0; i < cols; ++i) x[i] = narrow<T>(counts ? power((widen(x[i]) - base_others) * c) * f : 0.f);
 #pragma unroll
       for (int j = 0; j < kTileTop; ++j) {
         const int at = j < k && counts ? a.named.at[row * k + j] : -1;
@@ -484,15 +487,15 @@ __global__ void __launch_bounds__(kThreads) loss_grad(LossGradArgs g, int64_t se
     T* d           = static_cast<T*>(g.grad) + row * g.grad_stride + begin;
     const float4 s = a.row_stats[row];
     const float up = g.upstream[row * g.upstream_stride] * scale;
-    const bool counts = s.w != 0.f;
+    const bool counts = s.y != 0.f;
     // zero for rows that do not count, whatever their logits are
-    const float base = base_of(s.x), f = s.y * up * s.z;
-    auto one = [&](int64_t i, T v) { d[i] = narrow<T>(counts ? power((widen(v) - base) * c) * f : 0.f); };
+    const float base = base_of(s.x), base_others = base_of(s.z), f = s.w * up;
+    auto one = [&](int64_t i, T v) { d[i] = narrow<T>(counts ? power((widen(v) - base_others) * c) * f : 0.f); };
     if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0) {
       visit_row<THREADS == 32 ? kInFlight : kInFlight / 2>(x, n, tid, THREADS, one, [&](int64_t i, const Piece<T>& v) {
         Piece<T> w;
 #pragma unroll
-        for (int e = 0; e < N; ++e) w.v[e] = narrow<T>(counts ? power((widen(v.v[e]) - base) * c) * f : 0.f);
+        for (int e = 0; e < N; ++e) w.v[e] = narrow<T>(counts ? power((widen(v.v[e]) - base_others) * c) * f : 0.f);
         *reinterpret_cast<uint4*>(d + i) = *reinterpret_cast<const uint4*>(&w);
       });
     } else {

@@ -5,7 +5,7 @@ u, S and the counting of roundings are those of test_distill.py."""
 import pytest
 import torch
 
-from tests.test_distill import S, TYPES, U, check_values, gen, gpu
+from tests.test_distill import HALF_STEP, S, TINY, TYPES, U, check_values, gen, gpu
 
 NEG = float("-inf")
 # rows, classes, entries: a thread per row, a warp per short row, parts of a row, a block per row, a warp per long row
@@ -43,6 +43,26 @@ def bucket(z, values, index, lse, temperature, least=0.0):
     return loss * t2, grad * temperature, 3 * S * t2 + (loss * t2).abs() * 4 * U, 2 * S * size * temperature
 
 
+def check_bucket(z, values, index, lse, temperature, upstream=None, least=0.0, reduction="none"):
+    from cuml_b200 import distill
+
+    z = z.detach().requires_grad_()
+    loss = distill.distillation_loss(z, (values, index, lse), temperature=temperature, tail="bucket", reduction=reduction)
+    rows, grad, off, grad_off = bucket(z, values, index, lse, temperature, least)
+    factor = 1.0
+    if reduction == "mean":
+        factor = 1 / len(rows)
+        check_values(loss, rows.mean(), 4 * U, off.mean(), U)
+    else:
+        check_values(loss, rows, 0.0, off, U)
+    upstream = torch.ones_like(loss) if upstream is None else upstream
+    (got,) = torch.autograd.grad(loss, z, upstream)
+    up = upstream.detach().cpu().double().reshape(-1, 1) * factor
+    assert torch.isfinite(got.float()).all()
+    check_values(got, grad * up, 0.0, grad_off * up + TINY[z.dtype], HALF_STEP[z.dtype])
+    return loss
+
+
 def apart(n, c, k, dtype, temperature, gap, seed=0):
     """Logits whose named classes lie `gap` temperatures above the others (below them in every third row); a teacher that
     leaves about a tenth."""
@@ -72,3 +92,15 @@ def test_losses_of_named_classes_far_from_the_others(n, c, k, dtype, gap):
         few = distill.distillation_loss(z[:3], (v[:3], i[:3], lse[:3]), temperature=temperature, tail="bucket",
                                         reduction="none")
         check_values(loss[:3], few.cpu().double(), 0.0, 2 * off[:3], 2 * U)
+
+
+@gpu
+@pytest.mark.parametrize("n,c,k", KERNELS)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("gap", [9.0, 60.0, 90.0, 1e4])
+def test_gradients_of_named_classes_far_from_the_others(n, c, k, dtype, gap):
+    for temperature in (1.0, 0.1, 0.01):
+        z, v, i, lse = apart(n, c, k, dtype, temperature, gap)
+        check_bucket(z, v, i, lse, temperature)
+        check_bucket(z, v, i, lse, temperature, torch.tensor(65536.0 if dtype != "fp16" else 8.0 * n, device="cuda"),
+                     reduction="mean")
