@@ -65,8 +65,8 @@ struct LossArgs {
   Teacher teacher;
   Temperature temperature;
   float* row_loss;   // (n_rows)
-  // (n_rows), for the gradient.  q of a class is 2^((z - x) c) y, d / T of one that is not named 2^((z - z_o) c) w (z_o:
-  // the third component); all 0 where the row does not count.
+  // (n_rows), for the gradient.  q of a class times the sum of all of p is 2^((z - x) c) y, the gradient over T by a class
+  // that is not named 2^((z - z_o) c) w (z_o: the third component); all 0 where the row does not count.
   float4* row_stats;
   Named named;
 };

@@ -347,6 +347,7 @@ __device__ __forceinline__ Entries entries_at(void* base, int k)
 struct TeacherRow {
   double log_norm;
   float rest;    // probability of all classes that are not named
+  float mass;    // of all of p: 1, or less where the teacher gives some to no class of the student's
   bool counts;
   bool merged;   // a class was named twice: log p[j] is that of p[j]
 };
@@ -364,6 +365,8 @@ __device__ __forceinline__ TeacherRow read_teacher(const Teacher& t, int64_t row
   TeacherRow r;
   const int lane = threadIdx.x % 32, k = t.k;
   float top      = lowest<float>();
+  double mass    = 0;
+  r.mass         = 1.f;
   for (int j = lane; j < k; j += 32) {
     const int64_t c = teacher_index(t, row, j);
     const float v   = t.values ? t.values[row * t.values_stride + j] : 0.f;
@@ -377,7 +380,6 @@ __device__ __forceinline__ TeacherRow read_teacher(const Teacher& t, int64_t row
     // what is left of 1 is a difference: in 64 bits
     r.log_norm  = t.logsumexp[row];
     r.counts    = !(r.log_norm == -INFINITY);
-    double mass = 0;
     for (int j = lane; j < k; j += 32) {
       const double q = e.at[j] >= 0 && r.counts ? exp(e.v[j] * inv_t - r.log_norm) : 0.0;
       e.p[j]         = static_cast<float>(q);
@@ -435,7 +437,10 @@ __device__ __forceinline__ TeacherRow read_teacher(const Teacher& t, int64_t row
     }
     __syncwarp();
   }
-  if (REST && __reduce_add_sync(~0u, named) >= n_cols) r.rest = 0.f;  // no class is left
+  if (REST) {
+    if (__reduce_add_sync(~0u, named) >= n_cols) r.rest = 0.f;  // no class is left
+    if (r.rest == 0.f) r.mass = static_cast<float>(mass);
+  }
   return r;
 }
 

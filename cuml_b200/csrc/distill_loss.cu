@@ -4,7 +4,8 @@
 // of its distribution is one more class, p_r and q_r what is left on either side:
 //   loss  = T^2 [ sum_named p (log p - log q) + p_r (log p_r - log q_r) ]
 //   dloss / dz_c = T (q_c - p_c) for named classes, T (q_r - p_r) s_c for the others, s the softmax over these:
-// T q_c (1 - p_r / q_r), whose parts leave the range where q_r does, though p_r s_c does not.
+// T q_c (1 - p_r / q_r), whose parts leave the range where q_r does, though p_r s_c does not.  Where no class is left for
+// the rest, p adds up to P < 1, and q is P q in the gradient.
 // Softmax cross entropy is the case of one named class of probability 1 and T = 1.
 //
 // Bound by memory: the forward pass reads the logits once (running maximum and sum), the backward pass
@@ -152,7 +153,7 @@ __device__ __forceinline__ void finish_row(const LossArgs& a, int64_t row, const
   const double log_s = log_sum(r.s);
   const bool counts  = t.counts && !(r.s == 0.f);  // (no class has a finite logit: no softmax)
   double loss        = named_loss(e, k, t, inv_t, r.m, log_s, [&](int, int at) { return widen(x[at]); });
-  float4 stats       = make_float4(r.m, 1.f / r.s, r.m, 1.f / r.s);
+  float4 stats       = make_float4(r.m, t.mass / r.s, r.m, t.mass / r.s);
   if (REST && t.rest != 0.f) {
     const double log_rest = (static_cast<double>(others.m) - r.m) * inv_t + log_sum(others.s) - log_s;
     loss += t.rest * (log_sum(t.rest) - log_rest);
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(kTileRows) loss_tiles(LossArgs a, Reduced out,
       top = fmaxf(top, v ? v[j] : 0.f);
     }
     double log_norm;
-    float rest = 0.f, norm = 1.f;
+    float rest = 0.f, norm = 1.f, all_p = 1.f;
     bool counts;
     if (REST) {
       log_norm    = t.logsumexp[row];
@@ -292,6 +293,7 @@ __global__ void __launch_bounds__(kTileRows) loss_tiles(LossArgs a, Reduced out,
       }
       const bool all = __popcll(named) >= cols;
       rest           = all || 1.0 - mass < 0x1p-20 ? 0.f : static_cast<float>(1.0 - mass);
+      if (rest == 0.f) all_p = static_cast<float>(mass);
     } else {
       const float most = base_of(top);
       float total      = 0.f;
@@ -340,7 +342,7 @@ __global__ void __launch_bounds__(kTileRows) loss_tiles(LossArgs a, Reduced out,
       const double log_p = merged ? log(static_cast<double>(q)) : (v ? v[j] : 0.f) * inv_t - log_norm;
       loss += q * (log_p - ((static_cast<double>(widen(x[at[j]])) - r.m) * inv_t - log_s));
     }
-    float4 stats = make_float4(r.m, 1.f / r.s, r.m, 1.f / r.s);
+    float4 stats = make_float4(r.m, all_p / r.s, r.m, all_p / r.s);
     if (REST && rest != 0.f) {
       const double log_rest = (static_cast<double>(others.m) - r.m) * inv_t + log_sum(others.s) - log_s;
       loss += rest * (log_sum(rest) - log_rest);

@@ -104,3 +104,25 @@ def test_gradients_of_named_classes_far_from_the_others(n, c, k, dtype, gap):
         check_bucket(z, v, i, lse, temperature)
         check_bucket(z, v, i, lse, temperature, torch.tensor(65536.0 if dtype != "fp16" else 8.0 * n, device="cuda"),
                      reduction="mean")
+
+
+@gpu
+@pytest.mark.parametrize("n,c,k", [(5, 6, 6), (5000, 6, 8), (5000, 1, 3), (40, 200, 203), (3, 250, 256)])
+def test_a_teacher_of_more_classes_than_the_student(n, c, k):
+    """All of the student's classes are named, and a part of the teacher's mass is on none of them."""
+    from cuml_b200 import distill
+
+    g = gen(c)
+    z = torch.randn((n, c), generator=g, device="cuda") * 2
+    v = torch.randn((n, k), generator=g, device="cuda")
+    i = torch.rand((n, max(c, k)), generator=g, device="cuda").argsort(1)[:, :k].int()  # (k above c: some are outside)
+    for more in (0.0, 0.7):
+        lse = torch.logsumexp(v.double(), 1).float() + more
+        check_bucket(z, v, i, lse, 1.0, least=2.0 ** -20)
+    # the gradient is that of the loss that is returned: differences, off by 3 S / h and h^2 / 6 of the third derivative
+    h, x = 0.25, z[:1].detach().requires_grad_()
+    f = lambda x: distill.distillation_loss(x, (v[:1], i[:1], lse[:1]), tail="bucket", reduction="sum")  # noqa: E731
+    d = torch.zeros_like(x)
+    d[0, 0] = h
+    slope = (f(x.detach() + d) - f(x.detach() - d)) / (2 * h)
+    assert abs(slope.item() - torch.autograd.grad(f(x), x)[0][0, 0].item()) < h * h / 6 * 0.2 + 3 * S / h
