@@ -358,6 +358,10 @@ __device__ __forceinline__ int64_t teacher_index(const Teacher& t, int64_t row, 
                    : static_cast<int64_t>(static_cast<const int32_t*>(t.index)[row * t.index_stride + j]);
 }
 
+// What is left of 1 counts from here on: a log-sum-exp L in 32 bits is off by |L| 2^-24 at least and by few times that as it is
+// made, p by that part of itself.
+__device__ __forceinline__ double least_rest(double logsumexp) { return fmax(0x1p-20, fabs(logsumexp) * 0x1p-22); }
+
 // By one warp; e: shared memory.  REST: the teacher has a logsumexp.
 template <bool REST>
 __device__ __forceinline__ TeacherRow read_teacher(const Teacher& t, int64_t row, int64_t n_cols, double inv_t, const Entries& e)
@@ -386,8 +390,7 @@ __device__ __forceinline__ TeacherRow read_teacher(const Teacher& t, int64_t row
       mass += q;
     }
     mass = sum_lanes(mass);
-    // (a log-sum-exp in 32 bits leaves about 2^-20 where nothing is left)
-    r.rest = 1.0 - mass < 0x1p-20 ? 0.f : static_cast<float>(1.0 - mass);
+    r.rest = 1.0 - mass < least_rest(r.log_norm) ? 0.f : static_cast<float>(1.0 - mass);
   } else {
     const float most = base_of(max_lanes(top));
     const float ti   = static_cast<float>(inv_t);

@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kTileRows) loss_tiles(LossArgs a, Reduced out,
         mass += q;
       }
       const bool all = __popcll(named) >= cols;
-      rest           = all || 1.0 - mass < 0x1p-20 ? 0.f : static_cast<float>(1.0 - mass);
+      rest           = all || 1.0 - mass < least_rest(log_norm) ? 0.f : static_cast<float>(1.0 - mass);
       if (rest == 0.f) all_p = static_cast<float>(mass);
     } else {
       const float most = base_of(top);

@@ -277,6 +277,7 @@ def distillation_loss(logits, top, *, temperature: float = 1.0, tail: str = "ren
     tail : what becomes of the classes that the teacher does not name.  'renormalise': nothing, the named ones'
         probabilities are scaled to a sum of 1.  'bucket': together they are one more class on both sides;
         this takes the teacher's `logsumexp` over all its classes at the same temperature, and at most 2^20 classes.
+        Less than 2^-20, or 2^-22 of the log-sum-exp's size, counts as nothing: what 32 bits of that leave.
     reduction : 'mean' over the rows that count (0 where none does), 'sum', or 'none': (...), 0 for others.
 
     The loss is fp32, the gradient by the logits has their type."""

@@ -382,8 +382,9 @@ typedef struct b2fil_teacher {
   const void* index;       /* (n_rows, k) classes, int32 or int64                               */
   const float* logsumexp;  /* (n_rows) log sum exp(score / temperature) over ALL the teacher's classes:
                               the classes that are not named become one more, with what is left
-                              of 1 (less than 2^-20 counts as nothing).  NULL: the named classes'
-                              probabilities are scaled to a sum of 1                              */
+                              of 1 (less than 2^-20, or 2^-22 of the logsumexp's size, counts as
+                              nothing).  NULL: the named classes' probabilities are scaled to a
+                              sum of 1                                                            */
   int64_t values_stride;   /* elements between rows */
   int64_t index_stride;
   int64_t ignore;          /* class that does not count, e.g. -100 */

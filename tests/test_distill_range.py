@@ -126,3 +126,30 @@ def test_a_teacher_of_more_classes_than_the_student(n, c, k):
     d[0, 0] = h
     slope = (f(x.detach() + d) - f(x.detach() - d)) / (2 * h)
     assert abs(slope.item() - torch.autograd.grad(f(x), x)[0][0, 0].item()) < h * h / 6 * 0.2 + 3 * S / h
+
+
+@gpu
+@pytest.mark.parametrize("n,c,k", [(7, 40, 16), (5000, 40, 16), (300, 700, 100), (9, 3000, 40), (400, 3000, 40), (1300, 2500, 24)])
+@pytest.mark.parametrize("shift", [50.0, -100.0, 700.0])
+@pytest.mark.parametrize("dtype", ["fp32", "fp64"])
+def test_teachers_whose_logits_are_far_from_zero(n, c, k, shift, dtype):
+    """A 32-bit log-sum-exp of that size says 1 to some 2^-19 only; where the teacher names all that it has, and the student
+    masks the same classes, nothing is left, and the masked classes have no gradient."""
+    from cuml_b200 import distill
+
+    t = torch.randn((n, c), generator=gen(c), device="cuda").add_(shift).to(TYPES[dtype])
+    t[:, k:] = NEG
+    z = torch.randn((n, c), generator=gen(c + 1), device="cuda")
+    z[:, k:] = NEG
+    z = z.requires_grad_()
+    top = distill.top_scores(t, k)
+    loss = distill.distillation_loss(z, top, tail="bucket", reduction="none")
+    rows = distill.distillation_loss(z, top, reduction="none")
+    assert torch.isfinite(loss).all()
+    # p is off by the log-sum-exp's half step, 2^-24 of its size, and so is a loss whose logarithms are below 16
+    off = 6 * S + 16 * (abs(shift) + 16) * U
+    check_values(loss, rows.detach().cpu().double(), 4 * U, off, U)
+    (g,) = torch.autograd.grad(loss, z, torch.ones_like(loss))
+    (want,) = torch.autograd.grad(rows, z, torch.ones_like(rows))
+    assert (g[:, k:] == 0).all()
+    check_values(g, want.cpu().double(), 4 * S, 4 * S + 2 * (abs(shift) + 16) * U, U)
