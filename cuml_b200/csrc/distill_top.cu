@@ -149,9 +149,14 @@ __device__ __forceinline__ void write_top(const TopArgs& a, int64_t row, int j, 
   a.index[row * a.k + j]                   = static_cast<int32_t>(key.index());
 }
 
+// Scores over T of this size and above are more than 31, the logarithm of the longest row, apart or equal: the
+// log-sum-exp is the largest, to half a step (2^30: 64).
+template <class V>
+constexpr double kHuge = sizeof(V) == 4 ? 0x1p30 : 0x1p59;
+
 // The sum over a row: of 2^(x c - r), c = log2(e) / T, or of the probabilities' x^(1/T).  r is m c of a score m that
-// no score exceeds by more than kSlack powers of two; it stays finite for the lowest values, whose terms
-// may all be 0 then: such a row's log-sum-exp is its largest score.  Probabilities add up to nearly 1, whose
+// no score exceeds by more than kSlack powers of two, or -2 kHuge, below which terms are 0: the difference keeps what m c is
+// rounded by, which has to be an exponent of a number.  Probabilities add up to nearly 1, whose
 // logarithm is a difference: at T = 1 their sum keeps what each addition drops.
 template <class V, bool PROB>
 struct Sum {
@@ -160,11 +165,11 @@ struct Sum {
   __device__ __forceinline__ void reach(V most, V c)
   {
     if (PROB || !(most > limit)) return;
-    const V to = larger(larger(most, V(-1e36)) * c, V(-1e36));
+    const V to = larger(most * c, V(-2 * kHuge<V>));
     s          = first ? s : s * power(r - to);
     r          = to;
     first      = false;
-    limit      = larger(most, V(-1e36)) + V(kSlack) / c;
+    limit      = most + V(kSlack) / c;
   }
   __device__ __forceinline__ void add(V x, V c, bool plain)
   {
@@ -205,9 +210,9 @@ __device__ __forceinline__ void write_lse(const TopArgs& a, int64_t row, V m, V 
   else if (a.probabilities)
     r = log_of_sum(s, dropped);
   else
-    r = top == lowest<V>() || top == -lowest<V>() ? top
-        : s == V(0)                               ? static_cast<V>(top * a.inv_temperature)
-                                                  : static_cast<V>(m * 0.69314718055994530942 + log_of_terms(s));
+    r = top == lowest<V>() || top == -lowest<V>()        ? top
+        : fabs(top * a.inv_temperature) >= kHuge<V>      ? static_cast<V>(top * a.inv_temperature)
+                                                         : static_cast<V>(m * 0.69314718055994530942 + log_of_terms(s));
   static_cast<V*>(a.logsumexp)[row] = r;
 }
 

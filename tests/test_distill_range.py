@@ -5,7 +5,7 @@ u, S and the counting of roundings are those of test_distill.py."""
 import pytest
 import torch
 
-from tests.test_distill import HALF_STEP, S, TINY, TYPES, U, check_values, gen, gpu
+from tests.test_distill import HALF_STEP, S, TINY, TYPES, U, check_top, check_values, gen, gpu
 
 NEG = float("-inf")
 # rows, classes, entries: a thread per row, a warp per short row, parts of a row, a block per row, a warp per long row
@@ -153,3 +153,40 @@ def test_teachers_whose_logits_are_far_from_zero(n, c, k, shift, dtype):
     (want,) = torch.autograd.grad(rows, z, torch.ones_like(rows))
     assert (g[:, k:] == 0).all()
     check_values(g, want.cpu().double(), 4 * S, 4 * S + 2 * (abs(shift) + 16) * U, U)
+
+
+# ---- best scores -----------------------------------------------------------------------------------------------
+TOPS = [(1000, 10, 3), (5000, 60, 20), (9, 200, 40), (64, 1000, 9), (33, 2000, 30), (1300, 3000, 10), (2, 40_000, 100),
+        (1, 140_000, 20), (700, 5000, 30)]
+
+
+@gpu
+@pytest.mark.parametrize("n,c,k", TOPS)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scores_of_a_types_largest_value(n, c, k, dtype):
+    """The largest value times log2(e) is no number of the type."""
+    t = TYPES[dtype]
+    x = torch.randn((n, c), generator=gen(c), device="cuda").to(t)
+    x[0, c // 2] = torch.finfo(t).max
+    x[-1, ::2] = torch.finfo(t).max
+    x[n // 2] = torch.finfo(t).max * 0.75
+    check_top(x, k)
+    check_top(x, k, 4.0)
+
+
+@gpu
+@pytest.mark.parametrize("n,c,k", TOPS)
+@pytest.mark.parametrize("dtype", ["fp32", "fp64", "bf16"])
+@pytest.mark.parametrize("size", [1e7, 1e9, 3e10, 1e20, 1e36])
+def test_scores_far_from_zero(n, c, k, dtype, size):
+    """Scores of which one step is more than all exponents; masks of that size on whole rows, and on the first, the last and most
+    of the classes of rows."""
+    x = torch.randn((n, c), generator=gen(c), device="cuda")
+    x[n // 2] *= size
+    x[n - 1] = -size
+    x[0, :c // 2] = -size
+    if n > 2:
+        x[1, c // 2:] = -size
+        x[n - 2, torch.arange(c, device="cuda") % 256 > 3] = -size
+    check_top(x.to(TYPES[dtype]), k)
+    check_top(x.to(TYPES[dtype]), k, 2.0)
