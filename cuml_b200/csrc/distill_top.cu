@@ -154,33 +154,31 @@ __device__ __forceinline__ void write_top(const TopArgs& a, int64_t row, int j, 
 template <class V>
 constexpr double kHuge = sizeof(V) == 4 ? 0x1p30 : 0x1p59;
 
-// The sum over a row: of 2^(x c - r), c = log2(e) / T, or of the probabilities' x^(1/T).  r is m c of a score m that
-// no score exceeds by more than kSlack powers of two, or -2 kHuge, below which terms are 0: the difference keeps what m c is
+// The sum over a row: of 2^(x c - r), c = log2(e) / T, x the score or the probability's logarithm.  r is m c of an m that
+// no x exceeds by more than kSlack powers of two, or -2 kHuge, below which terms are 0: the difference keeps what m c is
 // rounded by, which has to be an exponent of a number.  Probabilities add up to nearly 1, whose
-// logarithm is a difference: at T = 1 their sum keeps what each addition drops.
+// logarithm is a difference: at T = 1 (`plain`) the sum is their own and keeps what each addition drops.
 template <class V, bool PROB>
 struct Sum {
   V r = V(0), s = V(0), limit = lowest<V>(), dropped = V(0);
   bool first = true;
-  __device__ __forceinline__ void reach(V most, V c)
+  __device__ __forceinline__ void reach(V most, V c, bool plain)  // most, limit: scores or probabilities themselves
   {
-    if (PROB || !(most > limit)) return;
-    const V to = larger(most * c, V(-2 * kHuge<V>));
+    if (plain || !(most > limit)) return;
+    const V to = larger((PROB ? log_of(most) : most) * c, V(-2 * kHuge<V>));
     s          = first ? s : s * power(r - to);
     r          = to;
     first      = false;
-    limit      = most + V(kSlack) / c;
+    limit      = PROB ? most * smaller(power(V(kSlack * 1.4426950408889634) / c), V(1e30)) : most + V(kSlack) / c;
   }
   __device__ __forceinline__ void add(V x, V c, bool plain)
   {
-    if (!PROB) {
-      s += power(fma(x, c, -r));
-    } else if (plain) {
+    if (plain) {
       const V t = s + x, b = t - s;
       dropped += (s - (t - b)) + (x - b);
       s = t;
     } else {
-      s += x == V(0) ? V(0) : power(log_of(x) * c);
+      s += power(fma(PROB ? log_of(x) : x, c, -r));
     }
   }
 };
@@ -203,16 +201,15 @@ template <class V, class K>
 __device__ __forceinline__ void write_lse(const TopArgs& a, int64_t row, V m, V s, double dropped, const K& best)
 {
   if (!a.logsumexp) return;
-  const V top = best.value();
-  V r;
-  if (top != top)
+  V top = best.value(), r;
+  if (a.probabilities) top = log_of(top);
+  if (top != top || top == lowest<V>() || top == -lowest<V>())
     r = top;
-  else if (a.probabilities)
+  else if (a.probabilities && a.inv_temperature == 1.0)
     r = log_of_sum(s, dropped);
   else
-    r = top == lowest<V>() || top == -lowest<V>()        ? top
-        : fabs(top * a.inv_temperature) >= kHuge<V>      ? static_cast<V>(top * a.inv_temperature)
-                                                         : static_cast<V>(m * 0.69314718055994530942 + log_of_terms(s));
+    r = fabs(top * a.inv_temperature) >= kHuge<V> ? static_cast<V>(top * a.inv_temperature)
+                                                  : static_cast<V>(m * 0.69314718055994530942 + log_of_terms(s));
   static_cast<V*>(a.logsumexp)[row] = r;
 }
 
@@ -278,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
   const int64_t n     = min(seg_cols, a.n_cols - begin);
   const int k         = static_cast<int>(min(static_cast<int64_t>(a.k), n));
   const V c           = static_cast<V>(1.4426950408889634 * a.inv_temperature);
-  const bool plain    = a.inv_temperature == 1.0;
+  const bool plain    = PROB && a.inv_temperature == 1.0;
   for (int64_t row = blockIdx.x / segs; row < a.n_rows; row += gridDim.x / segs) {
     const T* x       = static_cast<const T*>(a.scores) + row * a.row_stride + begin;
     const int lead   = lead_of(x, n);
@@ -294,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
         const V v = widen(e);
         if (v > top || at == ~0u) at = static_cast<uint32_t>(i);
         top = larger(top, v);
-        sum.reach(v, c);
+        sum.reach(v, c, plain);
         sum.add(v, c, plain);
       },
       [&](int64_t i, const Piece<T>& p) {
@@ -306,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
         for (int e = 1; e < N; ++e) most = larger(most, v[e]);
         if (most > top || at == ~0u) at = static_cast<uint32_t>(i);
         top = larger(top, most);
-        sum.reach(most, c);
+        sum.reach(most, c, plain);
 #pragma unroll
         for (int e = 0; e < N; ++e) sum.add(v[e], c, plain);
       });
@@ -324,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
     double dropped = 0;
     Running<V> all;
     all.m = V(0);
-    if (PROB) {
+    if (plain) {
       // (in 64 bits: see Sum)
       dropped = sum_row<kThreads>(static_cast<double>(sum.s) + sum.dropped, room);
     } else {
@@ -428,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
     for (int j = k + tid; j < a.k; j += kThreads) to[j] = K::none();
     if (tid == 0) {
       double* sum_to = clustered ? best_sum : sums + 2 * part;
-      sum_to[0]      = PROB ? dropped : static_cast<double>(all.s);
+      sum_to[0]      = plain ? dropped : static_cast<double>(all.s);
       sum_to[1]      = all.m;
     }
     if (clustered) {
@@ -454,12 +451,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
           Running<double> r;
           for (int i = 0; i < segs; ++i) {
             const double* from = cluster.map_shared_rank(best_sum, i);
-            if (PROB)
+            if (plain)
               r.s += from[0];
             else
               r.join(from[1], from[0], 1.0);
           }
-          write_lse(a, row, static_cast<V>(r.m), static_cast<V>(PROB ? 0.0 : r.s), PROB ? r.s : 0.0, key);
+          write_lse(a, row, static_cast<V>(r.m), static_cast<V>(plain ? 0.0 : r.s), plain ? r.s : 0.0, key);
         });
       }
       cluster.sync();  // the others' lists have been read
@@ -479,6 +476,7 @@ __global__ void __launch_bounds__(kThreads) top_join(TopArgs a, int segs, const 
   __shared__ K list[kList];
   __shared__ double room[64];
   __shared__ int found;
+  const bool plain = a.probabilities && a.inv_temperature == 1.0;
   for (int64_t row = blockIdx.x; row < a.n_rows; row += gridDim.x) {
     const K* from = keys + row * segs * a.k;
     const int all = segs * a.k, r_th = (a.k + segs - 1) / segs - 1;
@@ -520,16 +518,16 @@ __global__ void __launch_bounds__(kThreads) top_join(TopArgs a, int segs, const 
     Running<double> r;
     for (int i = threadIdx.x; i < segs; i += kThreads) {
       const double s = sums[2 * (row * segs + i)], m = sums[2 * (row * segs + i) + 1];
-      if (a.probabilities)
+      if (plain)
         r.s += s;
       else
         r.join(m, s, 1.0);
     }
-    if (a.probabilities)
+    if (plain)
       r.s = sum_row<kThreads>(r.s, room);
     else
       join_row<kThreads>(r, 1.0, room);
-    if (threadIdx.x == 0) write_lse(a, row, static_cast<V>(r.m), static_cast<V>(a.probabilities ? 0.0 : r.s), a.probabilities ? r.s : 0.0, list[0]);
+    if (threadIdx.x == 0) write_lse(a, row, static_cast<V>(r.m), static_cast<V>(plain ? 0.0 : r.s), plain ? r.s : 0.0, list[0]);
     __syncthreads();
   }
 }
@@ -563,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, warps_fit(U * 16 / sizeof(T) * sizeo
   const int lane = threadIdx.x % 32, n = static_cast<int>(a.n_cols), k = a.k;
   K* list          = lists[threadIdx.x / 32];
   const V c        = static_cast<V>(1.4426950408889634 * a.inv_temperature);
-  const bool plain = a.inv_temperature == 1.0;
+  const bool plain = PROB && a.inv_temperature == 1.0;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / 32; row < a.n_rows;
        row += static_cast<int64_t>(gridDim.x) * ROWS) {
     const T* x       = static_cast<const T*>(a.scores) + row * a.row_stride;
@@ -596,20 +594,20 @@ __global__ void __launch_bounds__(kThreads, warps_fit(U * 16 / sizeof(T) * sizeo
     for (int d = 16; d; d >>= 1) top = larger(top, __shfl_xor_sync(~0u, top, d));
     // the sum (what is not there is -inf and adds nothing to a sum of powers)
     Sum<V, PROB> sum;
-    sum.reach(top, c);
+    sum.reach(top, c, plain);
 #pragma unroll
     for (int e = 0; e < E; ++e)
       if (!PROB || is_there(e)) sum.add(v[e], c, plain);
     V s            = sum.s;
     double dropped = 0;
-    if (PROB) {
+    if (plain) {
       dropped = sum_lanes(static_cast<double>(sum.s) + sum.dropped);
       s       = V(0);
     } else {
       s = sum_lanes(s);
     }
     int got = 0;
-    const bool nan = PROB ? dropped != dropped : s != s;
+    const bool nan = plain ? dropped != dropped : s != s;
     // Few of many: a bound that at least k lanes' best reach, a ballot per bit.
     bool done = false;
     if (k <= kWarpTop && (S ? E > 2 : pieces >= 32) && !nan) {
@@ -737,7 +735,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(Top
   K* list          = lists[threadIdx.x / 32];
   int* found       = &counts[threadIdx.x / 32];
   const V c        = static_cast<V>(1.4426950408889634 * a.inv_temperature);
-  const bool plain = a.inv_temperature == 1.0;
+  const bool plain = PROB && a.inv_temperature == 1.0;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / 32; row < a.n_rows;
        row += static_cast<int64_t>(gridDim.x) * ROWS) {
     const T* x = static_cast<const T*>(a.scores) + row * a.row_stride;
@@ -751,7 +749,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(Top
         const V v = widen(e);
         if (v > best || at == ~0u) at = static_cast<uint32_t>(i);
         best      = larger(best, v);
-        sum.reach(v, c);
+        sum.reach(v, c, plain);
         sum.add(v, c, plain);
       },
       [&](int64_t i, const Piece<T>& p) {
@@ -763,14 +761,14 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(Top
         for (int e = 1; e < N; ++e) most = larger(most, v[e]);
         if (most > best || at == ~0u) at = static_cast<uint32_t>(i);
         best = larger(best, most);
-        sum.reach(most, c);
+        sum.reach(most, c, plain);
 #pragma unroll
         for (int e = 0; e < N; ++e) sum.add(v[e], c, plain);
       });
     double dropped = 0;
     Running<V> all;
     all.m = V(0);
-    if (PROB) {
+    if (plain) {
       dropped = sum_lanes(static_cast<double>(sum.s) + sum.dropped);
     } else {
       all.m = sum.first ? lowest<V>() : sum.r;
@@ -853,7 +851,7 @@ __global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
   const int c_n = static_cast<int>(a.n_cols);
   const TileShape<T> shape(c_n);
   const V c        = static_cast<V>(1.4426950408889634 * a.inv_temperature);
-  const bool plain = a.inv_temperature == 1.0;
+  const bool plain = PROB && a.inv_temperature == 1.0;
   const bool whole = without_gaps<T>(a.scores, a.row_stride, c_n);
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * kTileRows; first < a.n_rows;
        first += static_cast<int64_t>(gridDim.x) * kTileRows) {
@@ -911,7 +909,7 @@ __global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
       for (int j = 0; j < TOP; ++j) top[j] = from_ordered(key[j]);
     }
     Sum<V, PROB> sum;
-    sum.reach(top[0], c);
+    sum.reach(top[0], c, plain);
     for (int i = 0; i < c_n; ++i) sum.add(widen(x[i]), c, plain);
     const int64_t row = first + threadIdx.x;
     T* values         = static_cast<T*>(a.values) + row * a.k;

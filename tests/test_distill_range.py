@@ -163,6 +163,20 @@ TOPS = [(1000, 10, 3), (5000, 60, 20), (9, 200, 40), (64, 1000, 9), (33, 2000, 3
 @gpu
 @pytest.mark.parametrize("n,c,k", TOPS)
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [0.05, 0.2, 0.5, 1000.0])
+def test_probabilities_at_other_temperatures(n, c, k, dtype, temperature):
+    """x^(1/T) leaves the range of 32 bits, its logarithm does not.  (log x is off by 2 u of its size and the factor 1 / T by
+    u; flat rows, nearly flat ones, rows with zeros and with one sure class.)"""
+    x = torch.ones((n, c), device="cuda")
+    x[n // 3:] += torch.rand((n - n // 3, c), generator=gen(c), device="cuda")
+    x[n // 2:, ::3] = 0.0
+    x[-1, 1:] = 0.0
+    check_top((x / x.sum(1, keepdim=True)).to(TYPES[dtype]), k, temperature, probabilities=True)
+
+
+@gpu
+@pytest.mark.parametrize("n,c,k", TOPS)
+@pytest.mark.parametrize("dtype", TYPES)
 def test_scores_of_a_types_largest_value(n, c, k, dtype):
     """The largest value times log2(e) is no number of the type."""
     t = TYPES[dtype]
@@ -190,3 +204,18 @@ def test_scores_far_from_zero(n, c, k, dtype, size):
         x[n - 2, torch.arange(c, device="cuda") % 256 > 3] = -size
     check_top(x.to(TYPES[dtype]), k)
     check_top(x.to(TYPES[dtype]), k, 2.0)
+
+
+@gpu
+@pytest.mark.parametrize("c", [2, 10, 300, 2000, 40_000])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_the_sum_of_probabilities_keeps_what_additions_drop(c, dtype):
+    """At T = 1 log sum p is off by a few u whatever the number of classes: the sum's own rounding to 64 bits, the
+    logarithm's, 1 u each, and 2 u where the sum is nearly 1."""
+    from cuml_b200 import distill
+
+    x = torch.rand((600, c), generator=gen(c), device="cuda")
+    x = (x / x.sum(1, keepdim=True)).to(TYPES[dtype])
+    want = x.double().sum(1).log()
+    got = distill.top_scores(x, 2, probabilities=True).logsumexp.double()
+    assert ((got - want).abs() <= 4 * U * (want.abs() + 2.0 ** -6)).all()
