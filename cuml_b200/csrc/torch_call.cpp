@@ -293,6 +293,37 @@ bool options_of(PyObject* const* args, Options& o)
   return !PyErr_Occurred();
 }
 
+// What a node keeps of its inputs.
+struct Saved {
+  ag::SavedVariable variable;
+  at::ScalarType type;
+  int64_t rows, cols;
+  at::Device device = at::kCPU;
+  void set(const Tensor& x)
+  {
+    variable = ag::SavedVariable(x, false);
+    type     = x.scalar_type();
+    rows     = x.size(0);
+    cols     = x.size(1);
+    device   = x.device();
+  }
+  // Called outside of dispatch guards: hooks may compute it again, through autograd.
+  Tensor unpack()
+  {
+    Tensor x = variable.unpack();
+    TORCH_CHECK(x.layout() == at::kStrided && x.dim() == 2 && x.size(0) == rows && x.size(1) == cols &&
+                  x.scalar_type() == type && x.device() == device,
+                "a hook gave back another tensor than the distillation loss had saved");
+    return x;
+  }
+};
+// Rows one after the other: what hooks return may lie in another order.
+Tensor in_rows(const Tensor& x)
+{
+  const bool as_saved = (x.stride(1) == 1 || x.size(1) == 1) && (x.stride(0) >= x.size(1) || x.size(0) == 1);
+  return as_saved ? x : x.contiguous();
+}
+
 // What a node's gradient is by the loss: 32-bit values, and elements from one row's to the next.
 Tensor upstream_of(const Tensor& g, int64_t& stride)
 {
@@ -313,7 +344,7 @@ void no_second_derivative(Tensor& grad, const ag::variable_list& of)
 }
 
 struct LossNode : ag::Node {
-  ag::SavedVariable logits;
+  Saved logits;
   Tensor kept;
   Options o;
   int k;
@@ -323,11 +354,12 @@ struct LossNode : ag::Node {
   {
     TORCH_CHECK(!gone, "the distillation loss's graph has been freed: retain_graph=True keeps it");
     if (!grads[0].defined()) return {Tensor()};
-    Tensor x, grad;
+    const Tensor saved = logits.unpack();
+    Tensor grad;
     {
       at::AutoDispatchBelowADInplaceOrView below;
       at::NoGradGuard no_grad;
-      x = logits.unpack();
+      const Tensor x  = in_rows(saved);
       const int64_t n = x.size(0), c = x.size(1);
       grad = make({n, c}, x.scalar_type(), x);
       int64_t stride;
@@ -343,12 +375,12 @@ struct LossNode : ag::Node {
         raise_library_error(e);
       }
     }
-    no_second_derivative(grad, {grads[0], x});
+    no_second_derivative(grad, {grads[0], saved});
     return {grad};
   }
   void release_variables() override
   {
-    logits.reset_data();
+    logits.variable.reset_data();
     kept = Tensor();
     gone = true;
   }
@@ -393,10 +425,10 @@ PyObject* distill_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   if (at::GradMode::is_enabled() && x.requires_grad()) {
     auto node = std::shared_ptr<LossNode>(new LossNode(), ag::deleteNode);
     node->set_next_edges(ag::collect_next_edges(x));
-    node->logits = ag::SavedVariable(x, false);
-    node->kept   = std::move(kept);
-    node->o      = o;
-    node->k      = k;
+    node->logits.set(x);
+    node->kept = std::move(kept);
+    node->o    = o;
+    node->k    = k;
     ag::set_history(loss, node);
   }
   return THPVariable_Wrap(std::move(loss));
@@ -404,7 +436,7 @@ PyObject* distill_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs)
 }
 
 struct LinearNode : ag::Node {
-  ag::SavedVariable hidden, weight;
+  Saved hidden, weight;
   Tensor kept;
   Options o;
   int k;
@@ -414,12 +446,12 @@ struct LinearNode : ag::Node {
   {
     TORCH_CHECK(!gone, "the distillation loss's graph has been freed: retain_graph=True keeps it");
     if (!grads[0].defined()) return {Tensor(), Tensor()};
-    Tensor h, w, dh, dw;
+    const Tensor saved_h = hidden.unpack(), saved_w = weight.unpack();
+    Tensor dh, dw;
     {
       at::AutoDispatchBelowADInplaceOrView below;
       at::NoGradGuard no_grad;
-      h = hidden.unpack();
-      w = weight.unpack();
+      const Tensor h = in_rows(saved_h), w = in_rows(saved_w);
       const int64_t n = h.size(0), width = h.size(1), c = w.size(0);
       auto step = [&](const Tensor& x) { return x.size(0) == 1 ? width : x.stride(0); };
       const bool wants_h = task_should_compute_output(0), wants_w = task_should_compute_output(1);
@@ -443,14 +475,14 @@ struct LinearNode : ag::Node {
         raise_library_error(e);
       }
     }
-    no_second_derivative(dh, {grads[0], h, w});
-    no_second_derivative(dw, {grads[0], h, w});
+    no_second_derivative(dh, {grads[0], saved_h, saved_w});
+    no_second_derivative(dw, {grads[0], saved_h, saved_w});
     return {dh, dw};
   }
   void release_variables() override
   {
-    hidden.reset_data();
-    weight.reset_data();
+    hidden.variable.reset_data();
+    weight.variable.reset_data();
     kept = Tensor();
     gone = true;
   }
@@ -502,11 +534,11 @@ PyObject* linear_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   if (at::GradMode::is_enabled() && (h.requires_grad() || w.requires_grad())) {
     auto node = std::shared_ptr<LinearNode>(new LinearNode(), ag::deleteNode);
     node->set_next_edges(ag::collect_next_edges(h, w));
-    node->hidden = ag::SavedVariable(h, false);
-    node->weight = ag::SavedVariable(w, false);
-    node->kept   = std::move(kept);
-    node->o      = o;
-    node->k      = k;
+    node->hidden.set(h);
+    node->weight.set(w);
+    node->kept = std::move(kept);
+    node->o    = o;
+    node->k    = k;
     ag::set_history(loss, node);
   }
   return THPVariable_Wrap(std::move(loss));

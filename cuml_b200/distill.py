@@ -198,6 +198,13 @@ def _top(top, n, dev, tail):
     return _rows(values.float()), _rows(index), lse
 
 
+def _saved(x, like):
+    """A saved tensor as the kernels read it: hooks may have given back another one."""
+    if (x.shape, x.dtype, x.device) != like:
+        raise RuntimeError("a hook gave back another tensor than the distillation loss had saved")
+    return _rows(x.detach())
+
+
 def _upstream(g):
     """(fp32 gradient by the loss, elements from one row's to the next)."""
     g = g if g.dtype == torch.float32 else g.float()
@@ -229,6 +236,7 @@ class _Loss(torch.autograd.Function):
             named + 4 * n * k, loss.data_ptr(), factor if reduction else None, ws.data_ptr(), ws.numel(), dev.index,
             _stream(dev)))
         ctx.save_for_backward(logits)
+        ctx.like = (logits.shape, logits.dtype, logits.device)
         ctx.kept, ctx.options = kept, (temperature, reduction, k)
         return loss
 
@@ -238,7 +246,7 @@ class _Loss(torch.autograd.Function):
         (logits,) = ctx.saved_tensors
         temperature, reduction, k = ctx.options
         lib, kind, dev = _lib.load(), _TYPES[logits.dtype], logits.device
-        x = _rows(logits)
+        x = _saved(logits, ctx.like)
         n, n_cols = x.shape
         grad = torch.empty((n, n_cols), dtype=x.dtype, device=dev)
         g, stride = _upstream(g)
@@ -345,13 +353,14 @@ class _Linear(torch.autograd.Function):
             kind, *layer, C.byref(t.c), temperature, reduction, rows.data_ptr(), stats, named, named + 4 * n * k, named + 8 * n * k,
             loss.data_ptr(), factor if reduction else None, ws.data_ptr(), ws.numel(), dev.index, _stream(dev)))
         ctx.save_for_backward(hidden, weight)
+        ctx.like = [(x.shape, x.dtype, x.device) for x in (hidden, weight)]
         ctx.kept, ctx.options = kept, (temperature, reduction, k)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        hidden, weight = ctx.saved_tensors
+        hidden, weight = map(_saved, ctx.saved_tensors, ctx.like)
         temperature, reduction, k = ctx.options
         lib, kind, dev = _lib.load(), _TYPES[hidden.dtype], hidden.device
         (n, width), n_cols = hidden.shape, weight.shape[0]

@@ -219,3 +219,68 @@ def test_the_sum_of_probabilities_keeps_what_additions_drop(c, dtype):
     want = x.double().sum(1).log()
     got = distill.top_scores(x, 2, probabilities=True).logsumexp.double()
     assert ((got - want).abs() <= 4 * U * (want.abs() + 2.0 ** -6)).all()
+
+
+# ---- autograd --------------------------------------------------------------------------------------------------
+def students(dtype=torch.float32):
+    """(leaves, loss of them) of each operator."""
+    from cuml_b200 import distill
+
+    n, c, width = 24, 40, 32
+    z = torch.randn((n, c), generator=gen(1), device="cuda")
+    h = torch.randn((n, width), generator=gen(2), device="cuda").bfloat16()
+    w = torch.randn((c, width), generator=gen(3), device="cuda").bfloat16()
+    top = distill.top_scores(torch.randn((n, c), generator=gen(4), device="cuda"), 5)
+    target = torch.randint(0, c, (n,), generator=gen(5), device="cuda")
+    return [([z], lambda a: distill.distillation_loss(a * 2, top, tail="bucket")),
+            ([z], lambda a: distill.cross_entropy(a * 2, target)),
+            ([h, w], lambda a, b: distill.linear_distillation_loss(a * 2, b * 2, top)),
+            ([h, w], lambda a, b: distill.linear_cross_entropy(a * 2, b * 2, target, reduction="sum"))]
+
+
+@pytest.fixture(params=["compiled", "ctypes"])
+def path(request, monkeypatch):
+    from cuml_b200 import distill
+
+    if request.param == "ctypes":
+        monkeypatch.setattr(distill, "_call", False)
+    return request.param
+
+
+def fresh(leaves):
+    return [x.detach().clone().requires_grad_() for x in leaves]
+
+
+@gpu
+def test_under_an_activation_checkpoint(path):
+    """What is saved is computed again in the backward pass."""
+    from torch.utils.checkpoint import checkpoint
+
+    for leaves, f in students():
+        a = fresh(leaves)
+        want = torch.autograd.grad(f(*a), a)
+        for reentrant in (False, True):
+            b = fresh(leaves)
+            checkpoint(f, *b, use_reentrant=reentrant).backward()
+            assert all(torch.equal(x, y.grad) for x, y in zip(want, b))
+
+
+@gpu
+def test_under_hooks_that_move_what_is_saved(path):
+    """Saved on the host; and given back with its columns first."""
+    for leaves, f in students():
+        a = fresh(leaves)
+        want = torch.autograd.grad(f(*a), a)
+        columns = torch.autograd.graph.saved_tensors_hooks(
+            lambda x: x, lambda x: x.t().contiguous().t() if x.ndim == 2 else x)
+        for hooks in (torch.autograd.graph.save_on_cpu(), columns):
+            b = fresh(leaves)
+            with hooks:
+                loss = f(*b)
+            got = torch.autograd.grad(loss, b)
+            assert all(torch.equal(x, y) for x, y in zip(want, got))
+        for other in (lambda x: x[:5], lambda x: x.double(), lambda x: x.cpu()):
+            with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: other(x) if x.ndim == 2 else x):
+                loss = f(*fresh(leaves))
+            with pytest.raises(RuntimeError, match="hook"):
+                loss.backward()
