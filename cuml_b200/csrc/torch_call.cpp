@@ -214,6 +214,9 @@ bool plain_rows(PyObject* o)
          !t.is_conj() && (t.stride(1) == 1 || t.size(1) == 1) && (t.stride(0) >= t.size(1) || t.size(0) == 1) &&
          t.size(0) > 0 && t.size(1) > 0;
 }
+// Whether a student's tensor carries a forward-mode tangent: the ctypes path's autograd function refuses that, a
+// node of this file would leave it out.
+bool has_tangent(PyObject* o) { return THPVariable_Unpack(o)._fw_grad(/*level=*/0).defined(); }
 bool on(const Tensor& t, const Tensor& like) { return t.device() == like.device(); }
 
 // A teacher's numbers in 32 bits (scores of 16 or 64 bits are converted), constants to autograd.
@@ -394,7 +397,7 @@ PyObject* distill_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   if (nargs != 7) return PyErr_Format(PyExc_TypeError, "distill_loss takes 7 arguments");
   Options o;
   if (!options_of(args + 4, o)) return nullptr;
-  if (!library.loss || !plain_rows(args[0])) Py_RETURN_NONE;
+  if (!library.loss || !plain_rows(args[0]) || has_tangent(args[0])) Py_RETURN_NONE;
   const Tensor& x = THPVariable_Unpack(args[0]);
   const int type  = type_of(x);
   TeacherOf t;
@@ -496,7 +499,8 @@ PyObject* linear_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   if (nargs != 7) return PyErr_Format(PyExc_TypeError, "linear_loss takes 7 arguments");
   Options o;
   if (!options_of(args + 4, o)) return nullptr;
-  if (!library.linear || at::autocast::is_autocast_enabled(at::kCUDA) || !plain_rows(args[0]) || !plain_rows(args[1]))
+  if (!library.linear || at::autocast::is_autocast_enabled(at::kCUDA) || !plain_rows(args[0]) || !plain_rows(args[1]) ||
+      has_tangent(args[0]) || has_tangent(args[1]))
     Py_RETURN_NONE;
   const Tensor& h = THPVariable_Unpack(args[0]);
   const Tensor& w = THPVariable_Unpack(args[1]);

@@ -12,8 +12,8 @@ model), keep the `k` best classes of each row, and compute the loss of a student
 
 `ForestInference.predict_top`, `.teach` and `.distillation_loss` call them with a forest as the teacher.
 All tensors are CUDA tensors of one device; work is enqueued on torch's current stream of that device and
-nothing waits.  The losses have first derivatives by the logits, or by the layer's input and weight; the
-teacher's values are constants.  Calls and their gradients can be captured into CUDA graphs once they have run on
+nothing waits.  The losses have first derivatives by the logits, or by the layer's input and weight (backward mode
+only: second and forward-mode derivatives are errors); the teacher's values are constants.  Calls and their gradients can be captured into CUDA graphs once they have run on
 the device (as everywhere in torch, while no autograd graph of the same leaves from outside the capture is
 alive).  All computation happens in libb2fil.so.
 """

@@ -284,3 +284,16 @@ def test_under_hooks_that_move_what_is_saved(path):
                 loss = f(*fresh(leaves))
             with pytest.raises(RuntimeError, match="hook"):
                 loss.backward()
+
+
+@gpu
+def test_forward_mode_is_refused(path):
+    """There is no forward-mode derivative: an error, not a tangent that is left out."""
+    import torch.autograd.forward_ad as fw
+
+    for leaves, f in students():
+        for which in range(len(leaves)):
+            with fw.dual_level():
+                duals = [fw.make_dual(x, torch.ones_like(x)) if j == which else x for j, x in enumerate(leaves)]
+                with pytest.raises(NotImplementedError):
+                    f(*duals)
