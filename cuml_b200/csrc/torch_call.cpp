@@ -492,14 +492,15 @@ struct LinearNode : ag::Node {
   std::string name() const override { return "LinearDistillLossBackward"; }
 };
 
-// hidden, weight, values or None, index, temperature, ignored class, reduction
+// hidden, weight, values or None, index, temperature, ignored class, reduction, whether autocast has been heeded
 PyObject* linear_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs)
 {
   HANDLE_TH_ERRORS
-  if (nargs != 7) return PyErr_Format(PyExc_TypeError, "linear_loss takes 7 arguments");
+  if (nargs != 8) return PyErr_Format(PyExc_TypeError, "linear_loss takes 8 arguments");
   Options o;
-  if (!options_of(args + 4, o)) return nullptr;
-  if (!library.linear || at::autocast::is_autocast_enabled(at::kCUDA) || !plain_rows(args[0]) || !plain_rows(args[1]) ||
+  const int cast = PyObject_IsTrue(args[7]);
+  if (cast < 0 || !options_of(args + 4, o)) return nullptr;
+  if (!library.linear || (!cast && at::autocast::is_autocast_enabled(at::kCUDA)) || !plain_rows(args[0]) || !plain_rows(args[1]) ||
       has_tangent(args[0]) || has_tangent(args[1]))
     Py_RETURN_NONE;
   const Tensor& h = THPVariable_Unpack(args[0]);

@@ -266,13 +266,20 @@ def _kept(kept, n):
 _STUDENT = (torch.float32, torch.bfloat16, torch.float16)
 
 
+def _columns(index):
+    """Classes (n,) or (n, k) as (n, k)."""
+    return index.unsqueeze(1) if index.ndim == 1 else index
+
+
 def _loss(x, values, index, lse, temperature, reduction, ignore=_NO_CLASS, compiled_only=False):
     call = _native() if isinstance(x, torch.Tensor) and x.is_cuda else False
     if call:
         out = _answer(call.distill_loss(x, values, index, lse, temperature, ignore, reduction))
         if out is not None:
             return out
-    return None if compiled_only else _Loss.apply(x, values, index, lse, temperature, ignore, reduction)
+    if compiled_only:
+        return None
+    return _Loss.apply(x, values, _columns(index), lse, temperature, ignore, reduction)
 
 
 def distillation_loss(logits, top, *, temperature: float = 1.0, tail: str = "renormalise", reduction: str = "mean"):
@@ -326,13 +333,13 @@ def cross_entropy(logits, target, *, ignore_index: int = -100, reduction: str = 
 
 
 def _target(target, shape, dev):
-    """Classes of rows of that leading shape as (n, 1), checked."""
+    """Classes of rows of that leading shape as (n,), checked."""
     _cuda("target", target, (torch.int32, torch.int64))
     if target.shape != shape:
         raise ValueError(f"target must have shape {tuple(shape)}, got {tuple(target.shape)}")
     if target.device != dev:
         raise ValueError(f"target is on {target.device}, the student on {dev}")
-    return target.reshape(-1, 1)
+    return target.reshape(-1)
 
 
 class _Linear(torch.autograd.Function):
@@ -401,12 +408,15 @@ def _layer(hidden, weight):
 
 
 def _linear(hidden, weight, values, index, temperature, ignore, reduction, compiled_only=False):
+    # (compiled_only: the layer as the caller gave it, which autocast may have to cast)
     call = _native() if isinstance(hidden, torch.Tensor) and hidden.is_cuda else False
     if call:
-        out = _answer(call.linear_loss(hidden, weight, values, index, temperature, ignore, reduction))
+        out = _answer(call.linear_loss(hidden, weight, values, index, temperature, ignore, reduction, not compiled_only))
         if out is not None:
             return out
-    return None if compiled_only else _Linear.apply(hidden, weight, values, index, temperature, ignore, reduction)
+    if compiled_only:
+        return None
+    return _Linear.apply(hidden, weight, values, _columns(index), temperature, ignore, reduction)
 
 
 def linear_cross_entropy(hidden, weight, target, *, ignore_index: int = -100, reduction: str = "mean"):

@@ -297,3 +297,27 @@ def test_forward_mode_is_refused(path):
                 duals = [fw.make_dual(x, torch.ones_like(x)) if j == which else x for j, x in enumerate(leaves)]
                 with pytest.raises(NotImplementedError):
                     f(*duals)
+
+
+@gpu
+def test_the_compiled_path_takes_every_shape_and_autocast():
+    """(batch, position, class) logits with their targets, and layers that are cast: no slower than flat ones."""
+    from cuml_b200 import distill
+
+    assert distill._native()
+    z = torch.randn((4, 6, 50), generator=gen(1), device="cuda").requires_grad_()
+    target = torch.randint(0, 50, (4, 6), generator=gen(2), device="cuda")
+    for t in (target, target.int(), target.t().contiguous().t()):
+        loss = distill.cross_entropy(z, t)
+        assert loss.grad_fn.name() == "DistillLossBackward"
+        assert torch.equal(loss, distill.cross_entropy(z.detach().view(24, 50), target.reshape(24)))
+    h = torch.randn((4, 6, 32), generator=gen(3), device="cuda").requires_grad_()
+    w = torch.randn((50, 32), generator=gen(4), device="cuda").requires_grad_()
+    top = distill.top_scores(z.detach(), 5)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        losses = [distill.linear_cross_entropy(h, w, target), distill.linear_distillation_loss(h, w, top),
+                  distill.linear_cross_entropy(h[0], w, target[0])]
+    for loss in losses:
+        assert loss.grad_fn.name() == "LinearDistillLossBackward"
+        assert all(g.dtype == torch.float32 for g in torch.autograd.grad(loss, (h, w)))
+    assert torch.equal(losses[0], distill.linear_cross_entropy(h.bfloat16(), w.bfloat16(), target))
