@@ -19,7 +19,8 @@
 // one CTA alone with 128 x 256 would have to read 96 bytes per cycle from L2 where 64 pass.  Warp 0 brings the
 // tiles (TMA, 128-byte swizzle, ring of 6 x 32 KB), warp 1 of the first CTA issues the products, the others
 // work on the finished tile while the next one is summed in the other half of TMEM.  All waits are
-// bounded: after two seconds a role gives up, sets the status word and leaves by the common exit.
+// bounded: after two seconds a role gives up, sets the status word and leaves by the common exit.  Until the host has read
+// the word, losses and gradients are NaN: they may be incomplete.
 #include <cooperative_groups.h>
 #include <cuda.h>
 
@@ -61,6 +62,7 @@ constexpr int kFewNamed = 4;
 constexpr int kScaleBlocks = 8;
 
 __device__ int g_status;
+__device__ __forceinline__ bool incomplete() { return *static_cast<volatile int*>(&g_status) != 0; }
 
 // ---- PTX -------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t shared_of(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -205,11 +207,11 @@ struct Product {
   int add;
   void* out;    // times `scale`
 };
-// A factor, of what is there of a, b and t.
+// A factor, of what is there of a, b and t, of results that may be used.
 struct Scale {
   const float *a, *b;
   float t;
-  __device__ __forceinline__ float operator()() const { return (a ? *a : 1.f) * (b ? *b : 1.f) * t; }
+  __device__ __forceinline__ float operator()() const { return incomplete() ? NAN : (a ? *a : 1.f) * (b ? *b : 1.f) * t; }
 };
 struct Work {
   Product product[2];
@@ -642,6 +644,7 @@ __global__ void __launch_bounds__(kThreads) linear_rows(LinearArgs a, const floa
   float* logit       = reinterpret_cast<float*>(e.at + k);
   const float c      = a.temperature.c;
   const double inv_t = a.temperature.inverse;
+  const bool lost    = tiles > 0 && incomplete();
   double sum = 0, count = 0;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + slot; row < a.n_rows;
        row += static_cast<int64_t>(gridDim.x) * ROWS) {
@@ -663,6 +666,7 @@ __global__ void __launch_bounds__(kThreads) linear_rows(LinearArgs a, const floa
       const bool counts = t.counts && !(r.s == 0.f);
       double loss = named_loss(e, k, t, inv_t, r.m, log_sum(r.s), [&](int j, int) { return logit[j]; });
       if (!counts) loss = 0;
+      if (lost) loss = NAN;
       loss *= a.temperature.t * a.temperature.t;
       for (int j = lane; j < k; j += 32) {
         a.named.logit[row * k + j] = logit[j];

@@ -428,7 +428,9 @@ def linear_cross_entropy(hidden, weight, target, *, ignore_index: int = -100, re
     reduction : 'mean' over the rows that count (0 where none does), 'sum', or 'none': (...), 0 for others.
 
     The loss is fp32; products are summed in fp32.  The gradients have the layer's type; the
-    differences softmax - target are rounded to it before they are multiplied."""
+    differences softmax - target are rounded to it before they are multiplied (small layers: to two numbers of
+    it).  Waits inside the kernels are bounded; `check_status` tells whether one ran out, and until it has,
+    losses and gradients are NaN."""
     if reduction in _REDUCTIONS:
         loss = _linear(hidden, weight, None, target, 1.0, int(ignore_index), _REDUCTIONS[reduction], compiled_only=True)
         if loss is not None:
@@ -443,7 +445,7 @@ def linear_distillation_loss(hidden, weight, top, *, temperature: float = 1.0, r
     """`distillation_loss` (with tail='renormalise') of the logits `hidden @ weight.T`, without keeping them.
 
     hidden : (..., width), weight : (n_classes, width), both bf16 or both fp16 (under autocast they are cast).
-    top, temperature, reduction : as in `distillation_loss`; types and rounding as in
+    top, temperature, reduction : as in `distillation_loss`; types, rounding and waits as in
     `linear_cross_entropy`."""
     if reduction in _REDUCTIONS and type(top) is TopScores and top.values is not None:
         loss = _linear(hidden, weight, top.values, top.index, _temperature(temperature), _NO_CLASS, _REDUCTIONS[reduction],
@@ -458,7 +460,8 @@ def linear_distillation_loss(hidden, weight, top, *, temperature: float = 1.0, r
 
 def check_status(device=None) -> None:
     """Wait for all work on `device` and raise `B2FilError` (code -7) if a bounded wait inside a kernel of the
-    linear losses ran out since the last check."""
+    linear losses ran out since the last check.  The losses and gradients that follow such a wait are NaN until
+    then, as nothing in a stream-ordered call can raise; where a linear loss is NaN, ask here first."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     word = C.c_int32(0)
     index = torch.cuda.current_device() if device.index is None else device.index

@@ -429,7 +429,8 @@ class ForestInference:
         (n_classes, width) of its last linear layer, whose logits are then not kept (bf16 or fp16).
         k (at most n_classes are taken), temperature, tail, reduction : as in
         `cuml_b200.distill.distillation_loss`; tail='bucket' needs `logits`.  The loss has gradients by
-        the student's tensors."""
+        the student's tensors.  `check_status`, and with `hidden` `cuml_b200.distill.check_status`, tell
+        whether a bounded wait inside a kernel ran out."""
         from .. import distill
 
         linear = hidden is not None or weight is not None

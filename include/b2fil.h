@@ -443,8 +443,9 @@ int b2fil_linear_loss_grad(int dtype, const void* hidden, int64_t hidden_stride,
                            int64_t workspace_bytes, int device_id, void* cuda_stream);
 
 /* Waits for all work on device_id, reads the status word of the linear loss's kernels there and returns
- * B2FIL_ERR_TIMEOUT when a bounded wait inside one ran out (its outputs are then incomplete); the
- * word is cleared by the read. */
+ * B2FIL_ERR_TIMEOUT when a bounded wait inside one ran out; the word is cleared by the read.  That call's outputs may be
+ * incomplete, and from then until the word is read the linear losses on the device (of layers whose logits
+ * go through the tensor cores) and their gradients are NaN. */
 int b2fil_distill_status(int device_id, int32_t* status);
 
 /* Self test of that report: enqueues a kernel whose only work is a bounded wait that nothing ends. */

@@ -321,3 +321,33 @@ def test_the_compiled_path_takes_every_shape_and_autocast():
         assert loss.grad_fn.name() == "LinearDistillLossBackward"
         assert all(g.dtype == torch.float32 for g in torch.autograd.grad(loss, (h, w)))
     assert torch.equal(losses[0], distill.linear_cross_entropy(h.bfloat16(), w.bfloat16(), target))
+
+
+@gpu
+def test_a_wait_that_ran_out_is_seen_in_what_is_returned():
+    """Until `check_status` has reported it, the losses and gradients of a linear layer are NaN."""
+    from cuml_b200 import distill
+    from cuml_b200.fil import _lib
+
+    distill.check_status()
+    sizes = [(24, 40, 32), (300, 600, 64), (300, 20, 33)]
+    layers = [(torch.randn((n, w), generator=gen(1), device="cuda").bfloat16().requires_grad_(),
+               torch.randn((c, w), generator=gen(2), device="cuda").bfloat16().requires_grad_(),
+               torch.randint(0, c, (n,), generator=gen(3), device="cuda")) for n, c, w in sizes]
+
+    def everything():
+        out = []
+        for h, w, target in layers:
+            loss = distill.linear_cross_entropy(h, w, target)
+            out.append((loss, *torch.autograd.grad(loss, (h, w))))
+        return out
+
+    want = everything()
+    assert _lib.load().b2fil_distill_selftest_timeout(0, torch.cuda.current_stream().cuda_stream) == 0
+    for (_, c, _), (loss, *grads) in zip(sizes, everything()):
+        assert loss.isnan() or c <= 128  # (logits of few classes are dot products, which wait for nothing)
+        assert all(g.isnan().all() for g in grads)
+    with pytest.raises(_lib.B2FilError):
+        distill.check_status()
+    for a, b in zip(want, everything()):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
