@@ -281,6 +281,16 @@ __device__ __forceinline__ uint32_t two(float lo, float hi, bool bf16)
   return r;
 }
 
+// 2^x of a logit by the maximum, at most the sum of all of them (NaN stays).  The tensor cores' sums and those of the dot
+// products, of which the maximum or the named classes' logits may be, differ by some 1e-6 of their size: over a
+// temperature of that size or less, an exponent.
+__device__ __forceinline__ float power_within(float x, float sum)
+{
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(power(x)), "f"(sum));
+  return y;
+}
+
 // What rounding x to 16 bits leaves.
 __device__ __forceinline__ float left_of(float x, bool bf16)
 {
@@ -290,7 +300,7 @@ __device__ __forceinline__ float left_of(float x, bool bf16)
 // Part of a row (32 columns from `col` on) of a finished tile.  n: columns of the result.
 template <int KIND>
 __device__ __forceinline__ void take_columns(const Work& w, const Product& p, int split, int64_t row, int col, float (&x)[32],
-                                             Running<float>& r, float base, float factor)
+                                             Running<float>& r, float base, float sum, float factor)
 {
   if (KIND == kStats) {
     if (col + 32 > p.n) {
@@ -311,7 +321,7 @@ __device__ __forceinline__ void take_columns(const Work& w, const Product& p, in
   }
   if (KIND == kDiff) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) x[i] = col + i < p.n ? power((x[i] - base) * w.c) * factor : 0.f;
+    for (int i = 0; i < 32; ++i) x[i] = col + i < p.n ? power_within((x[i] - base) * w.c, sum) * factor : 0.f;
     if (factor == 0.f) {  // a row that does not count, whatever its logits are
 #pragma unroll
       for (int i = 0; i < 32; ++i) x[i] = 0.f;
@@ -534,10 +544,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
       const Product& p  = w.product[t.which];
       const int64_t row = static_cast<int64_t>(t.m) * kTile + rank * kHalf + quarter * 32 + lane;
       const bool in     = row < (KIND == kDiff ? w.plane_rows : p.m);
-      float base = 0.f, factor = 1.f;
+      float base = 0.f, sum = 1.f, factor = 1.f;
       if (KIND == kDiff && in) {  // (rows up to a plane's end are zeros: they meet zeros, but not as NaN)
         const float4 s = row < p.m ? w.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
         base           = base_of(s.x);
+        sum            = 1.f / s.y;
         factor         = s.w == 0.f ? 0.f : s.y * w.diff_scale * (w.row_scale ? w.row_scale[row * w.row_step] : 1.f);
       }
       if (KIND == kGrad && !p.sums) factor = w.scale();
@@ -550,7 +561,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
         if (KIND != kDiff && col >= p.n) break;
         float x[32];
         load_columns(tmem + half * kTile + c + (static_cast<uint32_t>(quarter * 32) << 16), x);
-        if (in) take_columns<KIND>(w, p, t.split, row, col, x, r, base, factor);
+        if (in) take_columns<KIND>(w, p, t.split, row, col, x, r, base, sum, factor);
         __syncwarp();
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -563,7 +574,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
           const int64_t e = row * w.k + j;
           const int at    = w.named.at[e] - w.first;
           if (at < low || at >= high) continue;
-          float d  = (power((w.named.logit[e] - base) * w.c) * inv - w.named.p[e]) * per;
+          float d  = (power_within((w.named.logit[e] - base) * w.c, sum) * inv - w.named.p[e]) * per;
           char* to = static_cast<char*>(w.diff) + (row * w.diff_stride + at) * 2;
           for (int plane = 0; plane < w.planes; ++plane, d = left_of(d, w.bf16), to += w.plane_rows * w.diff_stride * 2)
             *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(two(d, 0.f, w.bf16));
@@ -738,7 +749,7 @@ __global__ void __launch_bounds__(kThreads) named_diff(Work w, int64_t entries, 
     const int64_t row = i / w.k;
     const float4 s    = w.stats[row];
     if (s.w == 0.f) continue;
-    const float q = power((w.named.logit[i] - base_of(s.x)) * w.c) * s.y;
+    const float q = power_within((w.named.logit[i] - base_of(s.x)) * w.c, 1.f / s.y) * s.y;
     float d       = (q - w.named.p[i]) * w.diff_scale * (w.row_scale ? w.row_scale[row * w.row_step] : 1.f);
     for (int plane = 0; plane < w.planes; ++plane, d -= widen(narrow<T>(d)))
       static_cast<T*>(w.diff)[(plane * static_cast<int64_t>(w.plane_rows) + row) * w.diff_stride + at] = narrow<T>(d);

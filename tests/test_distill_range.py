@@ -351,3 +351,21 @@ def test_a_wait_that_ran_out_is_seen_in_what_is_returned():
         distill.check_status()
     for a, b in zip(want, everything()):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,width,c", [(64, 256, 1000), (64, 256, 100), (600, 1024, 2000)])
+def test_a_linear_layer_at_the_lowest_temperatures(n, width, c, dtype):
+    """Logits are off by some 1e-6 of their size, which at such temperatures decides between classes: the gradients are
+    those of one of the choices, never infinite."""
+    from cuml_b200 import distill
+
+    h = torch.randn((n, width), generator=gen(1), device="cuda").to(TYPES[dtype]).requires_grad_()
+    w = torch.randn((c, width), generator=gen(2), device="cuda").to(TYPES[dtype]).requires_grad_()
+    top = distill.top_scores(h.detach().float() @ w.detach().float().t(), 6)
+    for temperature in (1e-6, 1e-5, 1e-4):
+        loss = distill.linear_distillation_loss(h, w, top, temperature=temperature)
+        up = torch.tensor(1 / temperature, device="cuda")
+        grads = torch.autograd.grad(loss, (h, w), up)
+        assert torch.isfinite(loss) and all(torch.isfinite(g).all() for g in grads)
