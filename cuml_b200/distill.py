@@ -288,11 +288,13 @@ def distillation_loss(logits, top, *, temperature: float = 1.0, tail: str = "ren
     logits : (..., n_classes) fp32, bf16 or fp16; rows whose logits are all -inf do not count.
     top : `TopScores`, or (values, index[, logsumexp]) with values and index of shape (..., k), k <= 256.
         Entries whose class is outside [0, n_classes) do not count, a class that is named twice has the sum of its
-        probabilities; rows without an entry do not count.
+        probabilities; rows without an entry do not count (but with tail='bucket', see there).
     tail : what becomes of the classes that the teacher does not name.  'renormalise': nothing, the named ones'
         probabilities are scaled to a sum of 1.  'bucket': together they are one more class on both sides;
         this takes the teacher's `logsumexp` over all its classes at the same temperature, and at most 2^20 classes.
-        Less than 2^-20, or 2^-22 of the log-sum-exp's size, counts as nothing: what 32 bits of that leave.
+        Less than 2^-20, or 2^-22 of the log-sum-exp's size, counts as nothing: what 32 bits of that leave.  A row without an
+        entry has all of the teacher's mass there: it counts, with a loss of 0, unless its `logsumexp` is -inf (to be
+        given to rows of padding).
     reduction : 'mean' over the rows that count (0 where none does), 'sum', or 'none': (...), 0 for others.
 
     The loss is fp32, the gradient by the logits has their type."""

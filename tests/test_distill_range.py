@@ -155,6 +155,31 @@ def test_teachers_whose_logits_are_far_from_zero(n, c, k, shift, dtype):
     check_values(g, want.cpu().double(), 4 * S, 4 * S + 2 * (abs(shift) + 16) * U, U)
 
 
+@gpu
+@pytest.mark.parametrize("n,c", [(6, 12), (5000, 12), (6, 5000)])
+def test_rows_without_an_entry(n, c):
+    """They do not count where the named classes are scaled to 1.  With the rest as one more class all of a teacher's mass
+    may be there: such a row counts, with a loss of 0, unless its log-sum-exp is -inf."""
+    from cuml_b200 import distill
+
+    z = torch.randn((n, c), generator=gen(1), device="cuda")
+    v = torch.randn((n, 3), generator=gen(2), device="cuda")
+    i = torch.arange(3, device="cuda", dtype=torch.int32).repeat(n, 1)
+    lse = torch.logsumexp(v, 1) + 0.5
+    i[1::2] = -1
+    full = distill.distillation_loss(z, (v, i, lse), tail="bucket", reduction="none")
+    assert (full[1::2] == 0).all()
+    total = full.double().sum().item()
+    mean = distill.distillation_loss(z, (v, i, lse), tail="bucket")
+    assert abs(mean.item() - total / n) <= 4 * U * total
+    lse[1::2] = NEG
+    mean = distill.distillation_loss(z, (v, i, lse), tail="bucket")
+    assert abs(mean.item() - total / (n - n // 2)) <= 4 * U * total
+    rows = distill.distillation_loss(z, (v, i), reduction="none").double()
+    mean = distill.distillation_loss(z, (v, i))
+    assert (rows[1::2] == 0).all() and abs(mean.item() - rows.sum().item() / (n - n // 2)) <= 4 * U * rows.sum().item()
+
+
 # ---- best scores -----------------------------------------------------------------------------------------------
 TOPS = [(1000, 10, 3), (5000, 60, 20), (9, 200, 40), (64, 1000, 9), (33, 2000, 30), (1300, 3000, 10), (2, 40_000, 100),
         (1, 140_000, 20), (700, 5000, 30)]
