@@ -986,7 +986,9 @@ cudaError_t run_top(const TopArgs& a, void* workspace, int n_sms, cudaStream_t s
   constexpr int kPieces = sizeof(T) == 8 ? 8 : sizeof(T);  // 512 elements
   if (a.n_cols <= 512) return run_warps<T, kPieces, 0>(a, n_sms, s);
   if (a.n_cols <= 1024) return run_warps<T, 2 * kPieces, 0>(a, n_sms, s);
-  if (a.n_cols <= kWarpCols && sizeof(T) < 8 && a.k <= kWarpTop) return run_warps<T, 4 * kPieces, 0>(a, n_sms, s);
+  if constexpr (sizeof(T) < 8) {
+    if (a.n_cols <= kWarpCols && a.k <= kWarpTop) return run_warps<T, 4 * kPieces, 0>(a, n_sms, s);
+  }
   if (bytes <= kLongBytes && a.k <= kWarpTop && a.n_rows >= static_cast<int64_t>(kLongLeast) * n_sms) {
     const int64_t need = (a.n_rows + kThreads / 32 - 1) / (kThreads / 32), most = 16ll * n_sms;
     const auto kernel  = a.probabilities ? top_long<T, true> : top_long<T, false>;
