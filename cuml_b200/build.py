@@ -24,14 +24,6 @@ SOURCES = ["api.cu", "kernels.cu", "kernels_q_top6.cu", "kernels_q_plain6.cu", "
            "kernels_sparse_c.cu",
            "pack.cpp", "blocks.cpp",
            "distill_api.cu", "distill_top.cu", "distill_loss.cu", "distill_linear.cu"]
-HEADERS = ["each_tree.hpp", "forest.hpp", "host_pool.hpp", "kernels.hpp", "kernels_q.hpp", "device_common.cuh", "dense_q.cuh",
-           os.path.join("..", "..", "include", "b2fil.h"), "distill.hpp", "distill_common.cuh"]
-# sources that include none of the others' headers: they are compiled again for these alone
-OWN_HEADERS = {"distill_api.cu": ["distill.hpp", os.path.join("..", "..", "include", "b2fil.h")],
-               "distill_top.cu": ["distill.hpp", "distill_common.cuh"],
-               "distill_loss.cu": ["distill.hpp", "distill_common.cuh"],
-               "distill_linear.cu": ["distill.hpp", "distill_common.cuh"]}
-
 
 # Native call path for torch tensors: a CPython module compiled against the installed torch, whose
 # version is part of the file name (another torch needs another build).
@@ -71,15 +63,25 @@ def _newer(target: str, deps: list) -> bool:
     return all((not os.path.exists(d)) or os.path.getmtime(d) <= t for d in deps)
 
 
-def _object_deps(src: str) -> list:
-    """Files that an object is older than when it has to be compiled again."""
-    headers = OWN_HEADERS.get(src, [h for h in HEADERS if h != "distill_common.cuh"])
-    return [os.path.join(SRC, f) for f in [src] + headers] + [os.path.abspath(__file__)]
-
-
 def _lib_up_to_date() -> bool:
-    deps = [os.path.join(SRC, s) for s in SOURCES + HEADERS] + [os.path.abspath(__file__)]
-    return _newer(LIB, deps)
+    deps = [os.path.join(SRC, f) for f in os.listdir(SRC)] if os.path.isdir(SRC) else []
+    deps += [os.path.join(HERE, "..", "include", "b2fil.h"), os.path.abspath(__file__)]
+    return _newer(LIB, [f for f in deps if f != TORCH_SOURCE])
+
+
+def _read(path: str) -> str:
+    with open(path) as fh:
+        return fh.read()
+
+
+def _object_current(obj: str, recipe: str) -> bool:
+    """Whether an object was made by that command of that compiler and is newer than all files that it was made of (as the
+    compiler listed them)."""
+    try:
+        made_of = _read(obj + ".d").replace("\\\n", " ").split(":", 1)[1].split()
+        return _read(obj + ".recipe") == recipe and all(os.path.exists(f) for f in made_of) and _newer(obj, made_of)
+    except (OSError, IndexError):
+        return False
 
 
 def _torch_module_settled() -> bool:
@@ -137,24 +139,29 @@ def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(obj_dir, exist_ok=True)
     base = [_nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
             "-Xcompiler", "-fPIC,-Wall", "-Xptxas", "-v"]
+    version = subprocess.run([base[0], "--version"], stdout=subprocess.PIPE, text=True).stdout
     jobs, objects = [], []
     for src in SOURCES:
         obj = os.path.join(obj_dir, os.path.splitext(src)[0] + ".o")
         objects.append(obj)
-        if not force and _newer(obj, _object_deps(src)):
+        cmd = base + ["-MD", "-MF", obj + ".d", "-c", os.path.join(SRC, src), "-o", obj]
+        recipe = " ".join(cmd) + "\n" + version
+        if not force and _object_current(obj, recipe):
             continue
-        cmd = base + ["-c", os.path.join(SRC, src), "-o", obj]
+        if os.path.exists(obj + ".recipe"):
+            os.remove(obj + ".recipe")  # of an earlier build
         out = open(obj + ".log", "w+")  # a file, not a pipe: nothing blocks while others run
-        jobs.append((cmd, obj, subprocess.Popen(cmd, stdout=out, stderr=subprocess.STDOUT), out))
+        jobs.append((recipe, obj, subprocess.Popen(cmd, stdout=out, stderr=subprocess.STDOUT), out))
     log, failed = [], False
-    for cmd, obj, proc, out in jobs:
+    for recipe, obj, proc, out in jobs:
         proc.wait()
         out.seek(0)
-        log.append(" ".join(cmd) + "\n" + out.read())
+        log.append(recipe + out.read())
         out.close()
         failed |= proc.returncode != 0
-        if proc.returncode != 0 and os.path.exists(obj):
-            os.remove(obj)  # of an earlier build
+        if proc.returncode == 0:
+            with open(obj + ".recipe", "w") as fh:
+                fh.write(recipe)
     if not failed:
         cmd = [_nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", LIB]
         cmd += objects
