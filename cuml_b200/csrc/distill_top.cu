@@ -201,15 +201,16 @@ template <class V, class K>
 __device__ __forceinline__ void write_lse(const TopArgs& a, int64_t row, V m, V s, double dropped, const K& best)
 {
   if (!a.logsumexp) return;
-  V top = best.value(), r;
-  if (a.probabilities) top = log_of(top);
-  if (top != top || top == lowest<V>() || top == -lowest<V>())
-    r = top;
-  else if (a.probabilities && a.inv_temperature == 1.0)
-    r = log_of_sum(s, dropped);
-  else
-    r = fabs(top * a.inv_temperature) >= kHuge<V> ? static_cast<V>(top * a.inv_temperature)
-                                                  : static_cast<V>(m * 0.69314718055994530942 + log_of_terms(s));
+  const bool plain = a.probabilities && a.inv_temperature == 1.0;
+  V top = best.value(), r;  // (infinite, or NaN, of a score that is)
+  if (plain) {
+    r = top < V(INFINITY) ? log_of_sum(s, dropped) : top;
+  } else {
+    if (a.probabilities) top = log_of(top);
+    r = top != top || top == lowest<V>() || top == -lowest<V>() ? top
+        : fabs(top * a.inv_temperature) >= kHuge<V>             ? static_cast<V>(top * a.inv_temperature)
+                                                                : static_cast<V>(m * 0.69314718055994530942 + log_of_terms(s));
+  }
   static_cast<V*>(a.logsumexp)[row] = r;
 }
 
@@ -909,8 +910,12 @@ __global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
       for (int j = 0; j < TOP; ++j) top[j] = from_ordered(key[j]);
     }
     Sum<V, PROB> sum;
-    sum.reach(top[0], c, plain);
-    for (int i = 0; i < c_n; ++i) sum.add(widen(x[i]), c, plain);
+    if (plain) {
+      for (int i = 0; i < c_n; ++i) sum.add(widen(x[i]), c, true);
+    } else {
+      sum.reach(top[0], c, false);
+      for (int i = 0; i < c_n; ++i) sum.add(widen(x[i]), c, false);
+    }
     const int64_t row = first + threadIdx.x;
     T* values         = static_cast<T*>(a.values) + row * a.k;
     int32_t* index    = a.index + row * a.k;
