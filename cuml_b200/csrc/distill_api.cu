@@ -187,7 +187,8 @@ int b2fil_distill_loss(int dtype, const void* logits, int64_t n_rows, int64_t n_
   if (rc == B2FIL_OK) rc = check_temperature(temperature);
   if (rc != B2FIL_OK) return rc;
   if (reduction < B2FIL_REDUCE_NONE || reduction > B2FIL_REDUCE_MEAN) return invalid("unknown reduction");
-  if (reduction != B2FIL_REDUCE_NONE && (!loss || !factor)) return invalid("a reduced loss needs loss and factor");
+  if (reduction != B2FIL_REDUCE_NONE && (!loss || !factor || !aligned(loss, 4) || !aligned(factor, 4)))
+    return invalid("a reduced loss needs loss and factor, aligned to their elements");
   if (n_rows > 0 && (!logits || !row_loss || !row_stats || !named_p || !named_at)) return invalid("NULL buffer");
   if (!aligned(logits, type_bytes(dtype)) || !aligned(row_stats, 16) || !aligned(row_loss, 4) || !aligned(named_p, 4) ||
       !aligned(named_at, 4))
@@ -279,7 +280,8 @@ int b2fil_linear_loss(int dtype, const void* hidden, int64_t hidden_stride, cons
   if (rc != B2FIL_OK) return rc;
   if (a.teacher.logsumexp) return invalid("the loss of a linear layer takes no logsumexp of the teacher");
   if (reduction < B2FIL_REDUCE_NONE || reduction > B2FIL_REDUCE_MEAN) return invalid("unknown reduction");
-  if (reduction != B2FIL_REDUCE_NONE && (!loss || !factor)) return invalid("a reduced loss needs loss and factor");
+  if (reduction != B2FIL_REDUCE_NONE && (!loss || !factor || !aligned(loss, 4) || !aligned(factor, 4)))
+    return invalid("a reduced loss needs loss and factor, aligned to their elements");
   if (n_rows > 0 && (!row_loss || !row_stats || !named_logit || !named_p || !named_at)) return invalid("NULL buffer");
   if (!aligned(row_stats, 16) || !aligned(row_loss, 4) || !aligned(named_logit, 4) || !aligned(named_p, 4) || !aligned(named_at, 4))
     return invalid("a buffer is not aligned");

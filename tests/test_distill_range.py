@@ -59,7 +59,9 @@ def check_bucket(z, values, index, lse, temperature, upstream=None, least=0.0, r
     (got,) = torch.autograd.grad(loss, z, upstream)
     up = upstream.detach().cpu().double().reshape(-1, 1) * factor
     assert torch.isfinite(got.float()).all()
-    check_values(got, grad * up, 0.0, grad_off * up + TINY[z.dtype], HALF_STEP[z.dtype])
+    # (a power of less than 2^-126 is 0: q, s and p are each off by up to that, times what multiplies them, at most 1)
+    none = 3 * 2.0 ** -126 * temperature * up
+    check_values(got, grad * up, 0.0, grad_off * up + none + TINY[z.dtype], HALF_STEP[z.dtype])
     return loss
 
 
@@ -153,6 +155,44 @@ def test_teachers_whose_logits_are_far_from_zero(n, c, k, shift, dtype):
     (want,) = torch.autograd.grad(rows, z, torch.ones_like(rows))
     assert (g[:, k:] == 0).all()
     check_values(g, want.cpu().double(), 4 * S, 4 * S + 2 * (abs(shift) + 16) * U, U)
+
+
+def test_scalars_off_their_elements_are_refused(lib):
+    """(On the CPU: a kernel would write to an address that is none of a 32-bit number's.)"""
+    import ctypes as C
+
+    from cuml_b200.distill import CTeacher
+
+    teacher = CTeacher(64, 64, None, 2, 2, -100, 2, 0)
+    for loss, factor in ((66, 64), (64, 65), (None, 64), (64, None)):
+        for reduction in (1, 2):
+            assert lib.b2fil_distill_loss(2, 64, 4, 8, 8, C.byref(teacher), 1.0, reduction, 64, 64, 64, 64, loss, factor, None,
+                                          0, 0, None) == -1, (loss, factor)
+            assert lib.b2fil_linear_loss(2, 64, 16, 64, 16, 4, 10, 16, C.byref(teacher), 1.0, reduction, 64, 64, 64, 64, 64,
+                                         loss, factor, None, 0, 0, None) == -1, (loss, factor)
+        assert b"loss and factor" in lib.b2fil_last_error()
+
+
+@gpu
+@pytest.mark.parametrize("precision", ["single", "double"])
+@pytest.mark.parametrize("n", [60, 6000])
+def test_a_student_of_a_forest_at_a_low_temperature(precision, n):
+    """A forest's probabilities, whose powers leave the range of 32 bits, with the rest as one more class; what counts as
+    one is 2^-20, or 2^-22 of the log-sum-exp's size."""
+    from tests.helpers import random_rows
+    from tests.test_distill_forest import N_CLASSES, forest
+
+    fi = forest(precision)
+    X = torch.as_tensor(random_rows(4, n, 6), device="cuda")
+    z = torch.randn((n, N_CLASSES), generator=gen(1), device="cuda")
+    for temperature in (0.02, 0.1):
+        top = fi.teach(X, 4, temperature=temperature)
+        assert torch.isfinite(top.logsumexp).all()
+        least = (top.logsumexp.cpu().double().abs() * 2.0 ** -22).clamp(min=2.0 ** -20)
+        check_bucket(z, top.values.float(), top.index, top.logsumexp.float(), temperature, least=least)
+        loss = fi.distillation_loss(X, z, k=4, temperature=temperature, tail="bucket", reduction="none")
+        rows = bucket(z, top.values.float(), top.index, top.logsumexp.float(), temperature, least)[0]
+        check_values(loss, rows, 4 * U, 3 * S * temperature ** 2, U)
 
 
 @gpu
