@@ -3,8 +3,8 @@
 //   forward   z tile by tile on the tensor cores; of a tile only each row's maximum and sum of
 //             exp((z - max) / T) are kept, then joined per row with the logits of the classes that the
 //             teacher names (dot products of their own: k per row)
-//   backward  piece by piece of the classes: z again, d = q - p to a buffer of 16-bit values that
-//             stays in L2, then dH += d W and dW = d^T H from it
+//   backward  piece by piece of the classes: z again, d = q - p to a buffer of 16-bit values (up to
+//             256 MB, twice the L2), then dH += d W and dW = d^T H from it
 //
 // Bound by the tensor cores: 8 N D V operations for a training step, of which the second z (2 N D V) is the
 // price of not keeping it; kept in 16 bits it would be written once and read twice, and its rounding would

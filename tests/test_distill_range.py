@@ -65,6 +65,26 @@ def check_bucket(z, values, index, lse, temperature, upstream=None, least=0.0, r
     return loss
 
 
+@pytest.mark.parametrize("temperature", [1.0, 0.1])
+@pytest.mark.parametrize("c,k,more", [(9, 3, 0.4), (9, 3, 0.0), (6, 6, 0.0), (6, 8, 0.7)])
+def test_the_oracles_gradient_is_that_of_its_loss(c, k, more, temperature):
+    """Central differences of the 64-bit loss, h = 2^-10 T: off by h^2 / 6 of the third derivative, below 4 / T,
+    and by 2^-52 of losses below 100 over h (3e-10)."""
+    g = gen(c, "cpu")
+    z = torch.randn((4, c), generator=g, dtype=torch.float64) * temperature
+    z[1, :k // 2] += 30 * temperature
+    v = torch.randn((4, k), generator=g, dtype=torch.float64) * temperature
+    i = torch.stack([torch.randperm(max(c, k), generator=g)[:k] for _ in range(4)])
+    lse = torch.logsumexp(v / temperature, 1) + more
+    loss = lambda x: bucket(x, v, i, lse, temperature, least=1e-9)[0]  # noqa: E731
+    grad, h = bucket(z, v, i, lse, temperature, least=1e-9)[1], 2.0 ** -10 * temperature
+    for j in range(c):
+        d = torch.zeros_like(z)
+        d[:, j] = h
+        slope = (loss(z + d) - loss(z - d)) / (2 * h)
+        assert ((slope - grad[:, j]).abs() <= 2.0 ** -20 / 6 * temperature * 4 + 1e-9).all()
+
+
 def apart(n, c, k, dtype, temperature, gap, seed=0):
     """Logits whose named classes lie `gap` temperatures above the others (below them in every third row); a teacher that
     leaves about a tenth."""
