@@ -346,7 +346,7 @@ __device__ __forceinline__ Entries entries_at(void* base, int k)
 // log p[j] = v[j] / T - log_norm is taken in 64 bits, as it nearly cancels with the student's logarithm.
 struct TeacherRow {
   double log_norm;
-  float rest;    // probability of all classes that are not named
+  double rest;   // probability of all classes that are not named: where it is nearly 1 what matters is how nearly
   float mass;    // of all of p: 1, or less where the teacher gives some to no class of the student's
   bool counts;
   bool merged;   // a class was named twice: log p[j] is that of p[j]
@@ -390,7 +390,7 @@ __device__ __forceinline__ TeacherRow read_teacher(const Teacher& t, int64_t row
       mass += q;
     }
     mass = sum_lanes(mass);
-    r.rest = 1.0 - mass < least_rest(r.log_norm) ? 0.f : static_cast<float>(1.0 - mass);
+    r.rest = 1.0 - mass < least_rest(r.log_norm) ? 0.0 : 1.0 - mass;
   } else {
     const float most = base_of(max_lanes(top));
     const float ti   = static_cast<float>(inv_t);
@@ -403,7 +403,7 @@ __device__ __forceinline__ TeacherRow read_teacher(const Teacher& t, int64_t row
     sum        = sum_lanes(sum);
     r.log_norm = most * inv_t + log_sum(sum);
     r.counts   = !(sum == 0.f);
-    r.rest     = 0.f;
+    r.rest     = 0.0;
     if (r.counts)
       for (int j = lane; j < k; j += 32) e.p[j] = e.p[j] / sum;
   }
@@ -441,8 +441,8 @@ __device__ __forceinline__ TeacherRow read_teacher(const Teacher& t, int64_t row
     __syncwarp();
   }
   if (REST) {
-    if (__reduce_add_sync(~0u, named) >= n_cols) r.rest = 0.f;  // no class is left
-    if (r.rest == 0.f) r.mass = static_cast<float>(mass);
+    if (__reduce_add_sync(~0u, named) >= n_cols) r.rest = 0.0;  // no class is left
+    if (r.rest == 0.0) r.mass = static_cast<float>(mass);
   }
   return r;
 }

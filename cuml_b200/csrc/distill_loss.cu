@@ -43,7 +43,9 @@ constexpr int kCluster  = 8;              // blocks that add up their losses wit
 // and 30.)
 constexpr int kTileCols  = 64;
 constexpr int kTileTop   = 16;
-constexpr int kTileLeast = 32;
+constexpr int kTileLeast  = 32;
+constexpr int kTileBlocks = 8;  // of an SM, all there at once (292,366 x 13 bf16, rest as a class: 26.8 us, 28.8 with the seven that
+                                // 72 registers allow)
 
 // Bits of the named classes: bit 32 stands for the first element on a 16-byte boundary.
 __host__ __device__ __forceinline__ size_t bit_bytes(int64_t cols) { return cols ? ((cols + 32) / 32 + 2) * 4 : 0; }
@@ -136,6 +138,26 @@ __global__ void __launch_bounds__(kThreads) loss_parts(LossArgs a, int64_t seg_c
   }
 }
 
+// The named and the other classes of a row together.  With d the logarithm of their sums' ratio, log q_r = -log(1 + e^d) and
+// q_r - p_r = (1 - p_r) - (1 - q_r): where both rests are nearly 1 the loss is a difference of small numbers, which keep their
+// relative exactness.
+struct Split {
+  double log_s;      // of all, relative to m
+  double log_rest;   // log q_r
+  float difference;  // q_r - p_r
+};
+__device__ __forceinline__ Split split(const Running<float>& named, const Running<float>& others, float m, double inv_t, double rest)
+{
+  const double a = (static_cast<double>(named.m) - m) * inv_t + log_sum(named.s);
+  const double b = (static_cast<double>(others.m) - m) * inv_t + log_sum(others.s);
+  const double d = a - b;
+  const float e = expf(-fabsf(static_cast<float>(d))), more = log1pf(e), less = e / (1.f + e);
+  const bool few = d <= 0;  // less of the student is on the named classes
+  return {(few ? b : a) + more, (few ? 0.0 : -d) - more, few ? static_cast<float>(1.0 - rest) - less : less - static_cast<float>(rest)};
+}
+// log p_r: where p_r is small it is off by 2^-24 / p_r, and weighs with p_r.
+__device__ __forceinline__ float log_of_rest(double rest) { return log1pf(-static_cast<float>(1.0 - rest)); }
+
 // A row's loss, by one warp.  r: maximum and sum of the logits (REST: of those that are not named).
 template <class T, bool REST>
 __device__ __forceinline__ void finish_row(const LossArgs& a, int64_t row, const T* x, const Entries& e, const TeacherRow& t,
@@ -143,22 +165,23 @@ __device__ __forceinline__ void finish_row(const LossArgs& a, int64_t row, const
 {
   const int lane = threadIdx.x % 32, k = a.teacher.k;
   const Running<float> others = r;
+  Split both;
   if (REST) {
     Running<float> mine;
     for (int j = lane; j < k; j += 32)
       if (e.at[j] >= 0) mine.take(widen(x[e.at[j]]), c);
     mine.join_lanes(c);
     r.join(mine.m, mine.s, c);
+    both = split(mine, others, r.m, inv_t, t.rest);
   }
-  const double log_s = log_sum(r.s);
+  const double log_s = REST ? both.log_s : log_sum(r.s);
   const bool counts  = t.counts && !(r.s == 0.f);  // (no class has a finite logit: no softmax)
   double loss        = named_loss(e, k, t, inv_t, r.m, log_s, [&](int, int at) { return widen(x[at]); });
   float4 stats       = make_float4(r.m, t.mass / r.s, r.m, t.mass / r.s);
-  if (REST && t.rest != 0.f) {
-    const double log_rest = (static_cast<double>(others.m) - r.m) * inv_t + log_sum(others.s) - log_s;
-    loss += t.rest * (log_sum(t.rest) - log_rest);
+  if (REST && t.rest != 0.0) {
+    loss += t.rest * (log_of_rest(t.rest) - both.log_rest);
     stats.z = others.m;
-    stats.w = (others.s * power((others.m - base_of(r.m)) * c) / r.s - t.rest) / others.s;
+    stats.w = both.difference / others.s;
   }
   if (!counts) loss = 0;
   loss *= a.temperature.t * a.temperature.t;
@@ -243,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 5) loss_narrow(LossArgs a, int segs,
 
 // A row per thread.  What is not named is what the word's bits leave.
 template <class T, bool REST>
-__global__ void __launch_bounds__(kTileRows) loss_tiles(LossArgs a, Reduced out, double2* block_sums)
+__global__ void __launch_bounds__(kTileRows, kTileBlocks) loss_tiles(LossArgs a, Reduced out, double2* block_sums)
 {
   extern __shared__ __align__(16) char smem[];
   T* tile         = reinterpret_cast<T*>(smem);
@@ -280,7 +303,8 @@ __global__ void __launch_bounds__(kTileRows) loss_tiles(LossArgs a, Reduced out,
       top = fmaxf(top, v ? v[j] : 0.f);
     }
     double log_norm;
-    float rest = 0.f, norm = 1.f, all_p = 1.f;
+    double rest = 0.0;
+    float norm = 1.f, all_p = 1.f;
     bool counts;
     if (REST) {
       log_norm    = t.logsumexp[row];
@@ -292,8 +316,8 @@ __global__ void __launch_bounds__(kTileRows) loss_tiles(LossArgs a, Reduced out,
         mass += q;
       }
       const bool all = __popcll(named) >= cols;
-      rest           = all || 1.0 - mass < least_rest(log_norm) ? 0.f : static_cast<float>(1.0 - mass);
-      if (rest == 0.f) all_p = static_cast<float>(mass);
+      rest           = all || 1.0 - mass < least_rest(log_norm) ? 0.0 : 1.0 - mass;
+      if (rest == 0.0) all_p = static_cast<float>(mass);
     } else {
       const float most = base_of(top);
       float total      = 0.f;
@@ -306,26 +330,32 @@ __global__ void __launch_bounds__(kTileRows) loss_tiles(LossArgs a, Reduced out,
       counts   = !(total == 0.f);
       norm     = counts ? 1.f / total : 1.f;
     }
-    // the student: maximum and sum; with REST of the others apart, which may lie far below the named ones
+    // the student: maximum and sum, with REST of the others apart
     Running<float> r, others;
+    for (int i = 0; i < cols; ++i) r.m = fmaxf(r.m, widen(x[i]));
+    const float base = base_of(r.m);
     for (int i = 0; i < cols; ++i) {
-      const float v = widen(x[i]);
+      const float e = power((widen(x[i]) - base) * c);
       if (REST && !(named >> i & 1))
-        others.m = fmaxf(others.m, v);
-      else
-        r.m = fmaxf(r.m, v);
-    }
-    const float base = base_of(r.m), base_others = base_of(others.m);
-    for (int i = 0; i < cols; ++i) {
-      const bool other = REST && !(named >> i & 1);
-      const float e    = power((widen(x[i]) - (other ? base_others : base)) * c);
-      if (other)
         others.s += e;
       else
         r.s += e;
     }
-    if (REST) r.join(others.m, others.s, c);
-    const double log_s = log_sum(r.s);
+    Split both;
+    if (REST) {
+      const Running<float> mine = r;
+      r.s += others.s;
+      others.m = r.m;
+      if (others.s < 0x1p-60f) {  // far below the named ones (or none): relative to their own maximum, the terms leave the range
+        others = Running<float>();
+        for (int i = 0; i < cols; ++i)
+          if (!(named >> i & 1)) others.m = fmaxf(others.m, widen(x[i]));
+        for (int i = 0; i < cols; ++i)
+          if (!(named >> i & 1)) others.s += power((widen(x[i]) - base_of(others.m)) * c);
+      }
+      both = split(mine, others, r.m, inv_t, rest);
+    }
+    const double log_s = REST ? both.log_s : log_sum(r.s);
     counts             = counts && !(r.s == 0.f);
     double loss        = 0;
     for (int j = 0; j < k; ++j) {
@@ -343,11 +373,10 @@ __global__ void __launch_bounds__(kTileRows) loss_tiles(LossArgs a, Reduced out,
       loss += q * (log_p - ((static_cast<double>(widen(x[at[j]])) - r.m) * inv_t - log_s));
     }
     float4 stats = make_float4(r.m, all_p / r.s, r.m, all_p / r.s);
-    if (REST && rest != 0.f) {
-      const double log_rest = (static_cast<double>(others.m) - r.m) * inv_t + log_sum(others.s) - log_s;
-      loss += rest * (log_sum(rest) - log_rest);
+    if (REST && rest != 0.0) {
+      loss += rest * (log_of_rest(rest) - both.log_rest);
       stats.z = others.m;
-      stats.w = (others.s * power((others.m - base_of(r.m)) * c) / r.s - rest) / others.s;
+      stats.w = both.difference / others.s;
     }
     if (!counts) loss = 0;
     loss *= a.temperature.t * a.temperature.t;
@@ -571,7 +600,7 @@ template <class T, bool REST>
 cudaError_t run_loss(const LossArgs& a, const Reduced& out, void* workspace, int n_sms, cudaStream_t s)
 {
   if (by_tiles(a, n_sms)) {
-    const int64_t need = (a.n_rows + kTileRows - 1) / kTileRows, most = 8ll * n_sms;
+    const int64_t need = (a.n_rows + kTileRows - 1) / kTileRows, most = static_cast<int64_t>(kTileBlocks) * n_sms;
     const int blocks   = static_cast<int>(need < most ? need : most);
     double2* sums      = static_cast<double2*>(workspace);
     loss_tiles<T, REST><<<blocks, kTileRows, TileShape<T>(static_cast<int>(a.n_cols)).bytes(), s>>>(a, out, sums);

@@ -129,6 +129,30 @@ def test_gradients_of_named_classes_far_from_the_others(n, c, k, dtype, gap):
 
 
 @gpu
+@pytest.mark.parametrize("n,c,k", [(5000, 12, 4), (6000, 64, 16), (7, 12, 4), (300, 130, 20), (133, 3000, 8), (400, 3000, 8),
+                                   (1300, 2500, 5), (133, 60_000, 10)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("less", [3.0, 7.0])
+def test_rests_of_nearly_one(n, c, k, dtype, less):
+    """Few classes named of many, as at high temperatures: the loss is a difference of numbers near 1.  With M the named classes'
+    probabilities of both sides together, what the sums are off by (64 additions of a thread, 20 of threads, 16 u of a term) weighs with M,
+    and each p, and each logarithm of 1 - M, is off by 2 u of itself."""
+    from cuml_b200 import distill
+
+    for temperature in (1.0, 4.0):
+        z, v, i, _ = apart(n, c, k, dtype, temperature, 0.0)
+        z = z.float().scatter_add_(1, i.long(), torch.full_like(v, -less * temperature)).to(z.dtype)
+        lse = torch.logsumexp(v.double() / temperature, 1).float() + less
+        loss = distill.distillation_loss(z, (v, i, lse), temperature=temperature, tail="bucket", reduction="none")
+        rows = bucket(z, v, i, lse, temperature)[0]
+        p = (v.double() / temperature - lse.double()[:, None]).exp()
+        log_q = torch.log_softmax(z.double() / temperature, 1).gather(1, i.long())
+        m = p.sum(1) + log_q.exp().sum(1)
+        off = 100 * U * m + 2 * U * (p * (p.log() - log_q).abs()).sum(1) + 4 * U * m
+        check_values(loss, rows, 0.0, (off * temperature ** 2).cpu(), U)
+
+
+@gpu
 @pytest.mark.parametrize("n,c,k", [(5, 6, 6), (5000, 6, 8), (5000, 1, 3), (40, 200, 203), (3, 250, 256)])
 def test_a_teacher_of_more_classes_than_the_student(n, c, k):
     """All of the student's classes are named, and a part of the teacher's mass is on none of them."""
