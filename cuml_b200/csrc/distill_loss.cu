@@ -39,8 +39,8 @@ constexpr int kMostSegs = 64;
 constexpr int kInFlight = 8;              // pieces of a thread (the gradient of long rows: 4, as it writes as much)
 constexpr int kCluster  = 8;              // blocks that add up their losses without another kernel
 // Rows for one thread each: classes (the bits of one word), entries, and rows per SM from which on.  (1,000,000 x 10
-// fp32, k 3, rest as a class, loss and gradient: 1646 us with a warp per row, 113 this way; 292,366 x 13 bf16: 474
-// and 30.)
+// fp32, k 3, rest as a class, loss and gradient: 1646 us with a warp per row, 100 this way; 292,366 x 13 bf16: 474
+// and 37.)
 constexpr int kTileCols  = 64;
 constexpr int kTileTop   = 16;
 constexpr int kTileLeast  = 32;
