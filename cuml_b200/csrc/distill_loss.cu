@@ -346,7 +346,9 @@ __global__ void __launch_bounds__(kTileRows, kTileBlocks) loss_tiles(LossArgs a,
       const Running<float> mine = r;
       r.s += others.s;
       others.m = r.m;
-      if (others.s < 0x1p-60f) {  // far below the named ones (or none): relative to their own maximum, the terms leave the range
+      // far below the named ones (or none): relative to their own maximum, or the gradient's terms leave the range (2^-126) at more
+      // than 2^-96 of the largest
+      if (others.s < 0x1p-30f) {
         others = Running<float>();
         for (int i = 0; i < cols; ++i)
           if (!(named >> i & 1)) others.m = fmaxf(others.m, widen(x[i]));
