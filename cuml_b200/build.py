@@ -23,7 +23,8 @@ SOURCES = ["api.cu", "kernels.cu", "kernels_q_top6.cu", "kernels_q_plain6.cu", "
            "kernels_q_leafg.cu", "kernels_q_vec.cu", "kernels_q_top_vec.cu", "kernels_q_top_out.cu",
            "kernels_sparse_c.cu",
            "pack.cpp", "blocks.cpp",
-           "distill_api.cu", "distill_top.cu", "distill_loss.cu", "distill_linear.cu"]
+           "distill_api.cu", "distill_top.cu", "distill_loss.cu", "distill_linear.cu", "score_logits.cu",
+           "gradients.cu"]
 
 # Native call path for torch tensors: a CPython module compiled against the installed torch, whose
 # version is part of the file name (another torch needs another build).

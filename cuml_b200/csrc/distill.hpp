@@ -114,6 +114,81 @@ struct LinearGradArgs {
 size_t linear_grad_workspace(const LinearGradArgs& g, int n_sms);
 cudaError_t launch_linear_grad(int dtype, const LinearGradArgs& g, void* workspace, int n_sms, cudaStream_t s);
 
+// ---- scores of given classes (score_logits.cu, distill_linear.cu) -----------------------------
+struct Target {
+  const void* index;  // (n_rows) int32 or int64, `stride` elements apart; null: none is given
+  int64_t stride, ignore;
+  bool index64;
+};
+struct Scores {
+  float* log_prob;  // (n_rows), or null
+  float* entropy;   // (n_rows)
+  float4* kept;     // (n_rows) for the gradient: m, 1 / s (0: the row does not count), -u / s, class
+};
+// Gradients by a row's two scores, `*_stride` elements from one row's to the next; either may be null.
+struct ScoreUpstream {
+  const float *log_prob, *entropy;
+  int64_t log_prob_stride, entropy_stride;
+};
+
+struct ScoreArgs {
+  const void* logits;  // (n_rows, n_cols), row_stride elements between rows
+  int64_t n_rows, n_cols, row_stride;
+  Target target;
+  Temperature temperature;
+  Scores out;
+  int k;               // best classes of each row, 0: none
+  float* top;          // (n_rows, k) their log probabilities
+  int32_t* top_index;  // (n_rows, k)
+};
+size_t score_workspace(int dtype, const ScoreArgs& a, int n_sms);
+cudaError_t launch_score(int dtype, const ScoreArgs& a, void* workspace, int n_sms, cudaStream_t s);
+
+struct ScoreGradArgs {
+  ScoreArgs fwd;  // logits, sizes, temperature and what was kept
+  ScoreUpstream upstream;
+  void* grad;     // (n_rows, n_cols), grad_stride elements between rows
+  int64_t grad_stride;
+};
+cudaError_t launch_score_grad(int dtype, const ScoreGradArgs& g, int n_sms, cudaStream_t s);
+
+// The same of a linear layer's output (distill_linear.cu); `layer`: hidden, weight, sizes, strides and temperature.
+struct LinearScoreArgs {
+  LinearArgs layer;
+  Target target;
+  Scores out;
+};
+size_t linear_score_workspace(const LinearScoreArgs& a, int n_sms);
+cudaError_t launch_linear_score(int dtype, const LinearScoreArgs& a, void* workspace, int n_sms, cudaStream_t s);
+
+struct LinearScoreGradArgs {
+  LinearScoreArgs fwd;
+  ScoreUpstream upstream;
+  void* grad_hidden;  // (n_rows, width) contiguous, or null
+  void* grad_weight;  // (n_cols, width) contiguous, or null
+};
+size_t linear_score_grad_workspace(const LinearScoreGradArgs& g, int n_sms);
+cudaError_t launch_linear_score_grad(int dtype, const LinearScoreGradArgs& g, void* workspace, int n_sms, cudaStream_t s);
+
+// ---- norm of many tensors, and clipping (gradients.cu) ----------------------------------------
+// `rows` rows of `cols` elements; strides in elements.
+struct Gradient {
+  const void* from;
+  void* to;  // may be `from`; null: not scaled
+  int64_t rows, cols, from_row, from_col, to_row, to_col;
+  int from_type, to_type;
+};
+struct ClipArgs {
+  const Gradient* gradients;  // host memory
+  int64_t n;
+  int kind;     // 0: largest size, 1: sum of the sizes, 2: root of the sum of the squares
+  bool scales;  // else only the norm
+  double most;
+  float* norm;
+};
+size_t clip_workspace(const ClipArgs& a, int n_sms);
+cudaError_t launch_clip(const ClipArgs& a, void* workspace, int n_sms, cudaStream_t s);
+
 // Waits for the current device, reads its status word and clears it: not 0 where a bounded wait ran out.
 cudaError_t linear_status(int* status);
 // A kernel whose only work is such a wait, which nothing ends and which gives up after a millisecond.

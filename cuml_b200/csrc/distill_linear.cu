@@ -26,7 +26,7 @@
 
 #include <algorithm>
 
-#include "distill_common.cuh"
+#include "score_common.cuh"
 
 namespace b2fil {
 namespace distill {
@@ -192,7 +192,10 @@ __device__ __forceinline__ uint32_t instruction(bool bf16, bool a_outer, bool b_
 }
 
 // ---- products --------------------------------------------------------------------------------
-enum Result { kStats, kDiff, kGrad };
+enum Result { kStats, kDiff, kGrad, kScoreStats, kScoreDiff };
+// of either loss or score
+__host__ __device__ constexpr bool is_stats(int kind) { return kind == kStats || kind == kScoreStats; }
+__host__ __device__ constexpr bool is_diff(int kind) { return kind == kDiff || kind == kScoreDiff; }
 
 // out (m x n) = A (m x depth) B (n x depth)^T.  *_outer: the matrix lies with its depth outermost.
 struct Product {
@@ -231,6 +234,12 @@ struct Work {
   int planes, plane_rows;
   Named named;
   int k, first;
+  // scores: kScoreStats, kScoreDiff
+  Target target;
+  float4* score_parts;    // as `parts`, with the sum of the exponents
+  float* target_logit;
+  ScoreUpstream upstream;
+  const float* down;      // a factor of the upstream values, or null
   Scale scale;            // kGrad
   int* ticket;            // kStats: set to 0 for linear_rows; kDiff: for the next kernel, which takes its tiles by it
 };
@@ -298,11 +307,13 @@ __device__ __forceinline__ float left_of(float x, bool bf16)
 }
 
 // Part of a row (32 columns from `col` on) of a finished tile.  n: columns of the result.
+// at: the given class (kScoreStats), -1: none.
 template <int KIND>
 __device__ __forceinline__ void take_columns(const Work& w, const Product& p, int split, int64_t row, int col, float (&x)[32],
-                                             Running<float>& r, float base, float sum, float factor)
+                                             Running<float>& r, Scored& score, const RowGrad& of_score, int at, float base, float sum,
+                                             float factor)
 {
-  if (KIND == kStats) {
+  if (is_stats(KIND)) {
     if (col + 32 > p.n) {
 #pragma unroll
       for (int i = 0; i < 32; ++i)
@@ -311,6 +322,26 @@ __device__ __forceinline__ void take_columns(const Work& w, const Product& p, in
     float most = x[0];
 #pragma unroll
     for (int i = 1; i < 32; ++i) most = fmaxf(most, x[i]);
+    if (KIND == kScoreStats) {
+      if (most > score.m) score.move(most, w.c);
+      const float b = base_of(score.m);
+      float s[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float a = at_least((x[i] - b) * w.c, kLeast), e = power(a);
+        s[i & 3] += e;
+        u[i & 3] = fmaf(e, a, u[i & 3]);
+      }
+      score.s += (s[0] + s[1]) + (s[2] + s[3]);
+      score.u += (u[0] + u[1]) + (u[2] + u[3]);
+      if (at >= col && at < col + 32) {
+        float z = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) z += at - col == i ? x[i] : 0.f;
+        w.target_logit[row] = z;
+      }
+      return;
+    }
     if (most > r.m) r.raise(most, w.c);
     const float b = base_of(r.m);
     float s[4]    = {0.f, 0.f, 0.f, 0.f};
@@ -319,9 +350,21 @@ __device__ __forceinline__ void take_columns(const Work& w, const Product& p, in
     r.s += (s[0] + s[1]) + (s[2] + s[3]);
     return;
   }
-  if (KIND == kDiff) {
+  if (is_diff(KIND)) {
+    if (KIND == kScoreDiff) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) x[i] = col + i < p.n ? power_within((x[i] - base) * w.c, sum) * factor : 0.f;
+      for (int i = 0; i < 32; ++i) {
+        const float a = at_least((x[i] - of_score.base) * w.c, kLeast);
+        x[i]          = col + i < p.n ? power_within(a, sum) * fmaf(of_score.B, a, of_score.A) : 0.f;
+      }
+      if (of_score.at >= col && of_score.at < col + 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[i] += of_score.at - col == i ? of_score.add : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) x[i] = col + i < p.n ? power_within((x[i] - base) * w.c, sum) * factor : 0.f;
+    }
     if (factor == 0.f) {  // a row that does not count, whatever its logits are
 #pragma unroll
       for (int i = 0; i < 32; ++i) x[i] = 0.f;
@@ -543,8 +586,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
     for (int i = cluster; ok && tile_of(w, i, t); ok = next_tile(i)) {
       const Product& p  = w.product[t.which];
       const int64_t row = static_cast<int64_t>(t.m) * kTile + rank * kHalf + quarter * 32 + lane;
-      const bool in     = row < (KIND == kDiff ? w.plane_rows : p.m);
+      const bool in     = row < (is_diff(KIND) ? w.plane_rows : p.m);
       float base = 0.f, sum = 1.f, factor = 1.f;
+      RowGrad of_score{};
+      int at = -1;
+      if (KIND == kScoreStats && in) at = target_of(w.target, row, p.n);
+      if (KIND == kScoreDiff && in) {
+        const float4 s = row < p.m ? w.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+        if (s.y != 0.f) {
+          const ScoreUpstream& up = w.upstream;
+          const float f = w.diff_scale * (w.down ? *w.down : 1.f);
+          of_score = row_grad(s, up.log_prob ? up.log_prob[row * up.log_prob_stride] * f : 0.f,
+                              up.entropy ? up.entropy[row * up.entropy_stride] * f : 0.f);
+          of_score.at = of_score.at < 0 ? -1 : of_score.at - w.first;
+          sum = 1.f / s.y;
+        } else {
+          factor = 0.f;
+        }
+      }
       if (KIND == kDiff && in) {  // (rows up to a plane's end are zeros: they meet zeros, but not as NaN)
         const float4 s = row < p.m ? w.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
         base           = base_of(s.x);
@@ -555,13 +614,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
       if (!warp_wait(done + 8 * half, turn, &gave_up)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       Running<float> r;
+      Scored score;
 #pragma unroll 1
       for (int c = from; c < from + kTile / 2; c += 32) {
         const int col = t.n * kTile + c;
-        if (KIND != kDiff && col >= p.n) break;
+        if (!is_diff(KIND) && col >= p.n) break;
         float x[32];
         load_columns(tmem + half * kTile + c + (static_cast<uint32_t>(quarter * 32) << 16), x);
-        if (in) take_columns<KIND>(w, p, t.split, row, col, x, r, base, sum, factor);
+        if (in) take_columns<KIND>(w, p, t.split, row, col, x, r, score, of_score, at, base, sum, factor);
         __syncwarp();
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -581,6 +641,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
         }
       }
       if (KIND == kStats && in) w.parts[(row * p.n_tiles + t.n) * 2 + (from != 0)] = make_float2(r.m, r.s);
+      if (KIND == kScoreStats && in)
+        w.score_parts[(row * p.n_tiles + t.n) * 2 + (from != 0)] = make_float4(score.m, score.s, score.u, 0.f);
       half ^= 1;
       turn ^= half == 0;
     }
@@ -711,6 +773,28 @@ __global__ void __launch_bounds__(kThreads) linear_rows(LinearArgs a, const floa
   if (threadIdx.x == 0) write_reduced(out, total);
 }
 
+// Scores of a row from those of its tiles, by a warp.
+__global__ void __launch_bounds__(kThreads) linear_scores(LinearScoreArgs a, const float4* parts, const float* target_logit, int tiles)
+{
+  constexpr int ROWS = kThreads / 32;
+  const int lane  = threadIdx.x % 32;
+  const float c   = a.layer.temperature.c;
+  const bool lost = incomplete();
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / 32; row < a.layer.n_rows;
+       row += static_cast<int64_t>(gridDim.x) * ROWS) {
+    Scored r;
+    for (int i = lane; i < tiles; i += 32) {
+      const float4 p = parts[row * tiles + i];
+      r.join(p.x, p.y, p.z, c);
+    }
+    r.join_lanes(c);
+    if (lost) r.s = NAN;
+    if (lane > 0) continue;
+    const int at = target_of(a.target, row, a.layer.n_cols);
+    finish_score(a.out, row, r, a.layer.temperature.inverse, at, at >= 0 ? target_logit[row] : 0.f);
+  }
+}
+
 // One upstream value per row of an fp16 layer: the rows' are brought below 1 by a power of two, which *scale takes
 // back, so that d stays in range.  By one cluster (one block took 280 us for 2^20 rows).
 __global__ void __cluster_dims__(kScaleBlocks, 1, 1) __launch_bounds__(1024) grad_scales(LinearGradArgs g, float* scale, float* row_scale)
@@ -737,6 +821,37 @@ __global__ void __cluster_dims__(kScaleBlocks, 1, 1) __launch_bounds__(1024) gra
   if (from == 0) *scale = ldexpf(1.f, e);
 #pragma unroll 4
   for (int64_t i = from; i < g.fwd.n_rows; i += kScaleBlocks * 1024) row_scale[i] = g.upstream[i * g.upstream_stride] * down;
+}
+
+// The same for the gradients by a row's two scores: a difference is at most |g| + 6 |h| (of a class of probability q, |log q + H| q <=
+// q (1 - q) log n_cols + 1).  scale[1] is what brings them below 1.
+__global__ void __cluster_dims__(kScaleBlocks, 1, 1) __launch_bounds__(1024) score_scales(ScoreUpstream up, const float4* kept, int64_t n_rows, float* scale)
+{
+  namespace cg = cooperative_groups;
+  __shared__ float room[32], mine;
+  const int64_t from = blockIdx.x * 1024 + threadIdx.x;
+  float most = 0.f;
+#pragma unroll 4
+  for (int64_t i = from; i < n_rows; i += kScaleBlocks * 1024) {
+    const float g = up.log_prob ? fabsf(up.log_prob[i * up.log_prob_stride]) : 0.f, h = up.entropy ? fabsf(up.entropy[i * up.entropy_stride]) : 0.f;
+    if (kept[i].y != 0.f) most = fmaxf(most, fmaf(8.f, h, g));
+  }
+  most = max_lanes(most);
+  if (threadIdx.x % 32 == 0) room[threadIdx.x / 32] = most;
+  __syncthreads();
+  most = max_lanes(room[threadIdx.x % 32]);
+  if (threadIdx.x == 0) mine = most;
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  for (int b = 0; b < kScaleBlocks; ++b) most = fmaxf(most, *cluster.map_shared_rank(&mine, b));
+  cluster.sync();  // the others' shared memory has been read
+  int e = 0;
+  if (most > 0.f && most < INFINITY) frexpf(most, &e);
+  e = max(-100, min(100, e));
+  if (from == 0) {
+    scale[0] = ldexpf(1.f, e);
+    scale[1] = ldexpf(1.f, -e);
+  }
 }
 
 // d of the classes that the teacher names, in a piece of the classes.
@@ -1023,8 +1138,35 @@ cudaError_t finish(const float* sums, int splits, int64_t rows, int64_t pitch, i
   return cudaGetLastError();
 }
 
+// Scores of a layer's output.
 template <class T>
-cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace, int n_sms, cudaStream_t s)
+cudaError_t run_linear_score(bool bf16, const LinearScoreArgs& given, void* workspace, int n_sms, cudaStream_t s)
+{
+  if (given.layer.n_rows == 0) return cudaSuccess;
+  LinearArgs a  = given.layer;
+  char* at      = static_cast<char*>(workspace);
+  cudaError_t e = give_layer<T>(a, layer_of(given.layer), at, n_sms, s);
+  if (e != cudaSuccess) return e;
+  Work w{};
+  w.products = 1;
+  w.bf16     = bf16;
+  w.c        = a.temperature.c;
+  w.ticket   = reinterpret_cast<int*>(at);  // not used
+  w.target   = given.target;
+  w.target_logit = reinterpret_cast<float*>(at += 256);
+  w.score_parts  = reinterpret_cast<float4*>(at + padded(a.n_rows * 4));
+  if (!logits_product(w.product[0], bf16, a, 0, a.n_cols)) return cudaErrorInvalidValue;
+  if ((e = run_products<kScoreStats>(w, n_sms, s)) != cudaSuccess) return e;
+  const int64_t need = (a.n_rows + kThreads / 32 - 1) / (kThreads / 32), most = 8ll * n_sms;
+  linear_scores<<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(given, w.score_parts, w.target_logit,
+                                                                                     2 * w.product[0].n_tiles);
+  count_launches(2);
+  return cudaGetLastError();
+}
+
+// score: of the scores, not of a loss; g.fwd then has the layer, the temperature and, as row_stats, what was kept.
+template <class T>
+cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, const ScoreUpstream* score, void* workspace, int n_sms, cudaStream_t s)
 {
   LinearArgs a        = g.fwd;
   const int64_t width = a.width;  // of the gradients' rows
@@ -1043,7 +1185,10 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
   const bool per_row   = g.factor == nullptr;
   const bool scaled    = per_row && !bf16;  // (bf16 has the range of the upstream values itself)
   int launched         = scaled;
-  if (scaled) grad_scales<<<kScaleBlocks, 1024, 0, s>>>(g, scale, row_scale);
+  if (scaled && score)
+    score_scales<<<kScaleBlocks, 1024, 0, s>>>(*score, a.row_stats, a.n_rows, scale);
+  else if (scaled)
+    grad_scales<<<kScaleBlocks, 1024, 0, s>>>(g, scale, row_scale);
   Work w{};
   w.bf16        = bf16;
   w.c           = a.temperature.c;
@@ -1055,7 +1200,12 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
   w.diff_scale  = d_scale;
   w.planes      = plan.planes;
   w.plane_rows  = static_cast<int>(plan.plane_rows);
-  w.scale       = Scale{scaled ? scale : per_row ? nullptr : g.upstream, g.factor, static_cast<float>(a.temperature.t) / d_scale};
+  w.scale       = Scale{scaled ? scale : per_row ? nullptr : g.upstream, g.factor,
+                        static_cast<float>(score ? a.temperature.inverse : a.temperature.t) / d_scale};
+  if (score) {
+    w.upstream = *score;
+    w.down     = scaled ? scale + 1 : nullptr;
+  }
   w.named       = a.named;
   w.k           = a.teacher.k;
   w.ticket      = ticket;
@@ -1064,7 +1214,8 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, void* workspace,
     w.products = 1;
     w.first    = static_cast<int>(first);
     if (!logits_product(w.product[0], bf16, a, first, n)) return cudaErrorInvalidValue;
-    if ((e = run_products<kDiff>(w, n_sms, s)) != cudaSuccess) return e;
+    e = score ? run_products<kScoreDiff>(w, n_sms, s) : run_products<kDiff>(w, n_sms, s);
+    if (e != cudaSuccess) return e;
     if (w.k > kFewNamed) {
       const int64_t entries = a.n_rows * w.k, need = (entries + kThreads - 1) / kThreads;
       named_diff<T><<<static_cast<unsigned>(need < 8 * n_sms ? need : 8 * n_sms), kThreads, 0, s>>>(w, entries, static_cast<int>(n));
@@ -1156,8 +1307,41 @@ cudaError_t launch_linear(int dtype, const LinearArgs& a, const Reduced& out, vo
 
 cudaError_t launch_linear_grad(int dtype, const LinearGradArgs& g, void* workspace, int n_sms, cudaStream_t s)
 {
-  return dtype == kBF16 ? run_linear_grad<__nv_bfloat16>(true, g, workspace, n_sms, s)
-                        : run_linear_grad<__half>(false, g, workspace, n_sms, s);
+  return dtype == kBF16 ? run_linear_grad<__nv_bfloat16>(true, g, nullptr, workspace, n_sms, s)
+                        : run_linear_grad<__half>(false, g, nullptr, workspace, n_sms, s);
+}
+
+size_t linear_score_workspace(const LinearScoreArgs& a, int)
+{
+  const LinearArgs& l = a.layer;
+  return layer_of(l).bytes + 256 + padded(l.n_rows * 4) + l.n_rows * static_cast<size_t>(2 * tiles_of(l.n_cols)) * sizeof(float4);
+}
+
+cudaError_t launch_linear_score(int dtype, const LinearScoreArgs& a, void* workspace, int n_sms, cudaStream_t s)
+{
+  return dtype == kBF16 ? run_linear_score<__nv_bfloat16>(true, a, workspace, n_sms, s)
+                        : run_linear_score<__half>(false, a, workspace, n_sms, s);
+}
+
+namespace {
+LinearGradArgs grad_of(const LinearScoreGradArgs& g)
+{
+  LinearGradArgs r{};
+  r.fwd           = g.fwd.layer;
+  r.fwd.row_stats = g.fwd.out.kept;
+  r.fwd.teacher.k = 0;
+  r.grad_hidden   = g.grad_hidden;
+  r.grad_weight   = g.grad_weight;
+  return r;
+}
+}  // namespace
+
+size_t linear_score_grad_workspace(const LinearScoreGradArgs& g, int n_sms) { return linear_grad_workspace(grad_of(g), n_sms); }
+
+cudaError_t launch_linear_score_grad(int dtype, const LinearScoreGradArgs& g, void* workspace, int n_sms, cudaStream_t s)
+{
+  return dtype == kBF16 ? run_linear_grad<__nv_bfloat16>(true, grad_of(g), &g.upstream, workspace, n_sms, s)
+                        : run_linear_grad<__half>(false, grad_of(g), &g.upstream, workspace, n_sms, s);
 }
 
 cudaError_t linear_status(int* status)

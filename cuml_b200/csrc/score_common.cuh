@@ -1,0 +1,179 @@
+// What the scoring kernels share: a softmax's maximum, sum and mean exponent in one pass, and what follows from them for
+// a row.
+//
+// With a reference m, a_c = (z_c - m) log2(e) / T, s = sum 2^a and u = sum 2^a a:
+//   log q_c = ln2 a_c - ln s,   entropy H = -sum q log q = ln s - ln2 u / s
+//   d log q_t / dz_c = (1(c = t) - q_c) / T,   dH / dz_c = -q_c (log q_c + H) / T = -q_c ln2 (a_c - u / s) / T
+#pragma once
+
+#include "distill_common.cuh"
+
+namespace b2fil {
+namespace distill {
+
+constexpr float kLn2 = 0.69314718055994530942f;
+
+// Exponents below this are as good as any: 2^a is 0, and so is 2^a a, which -inf would make NaN.
+constexpr float kLeast = -256.f;
+
+// (NaN stays, unlike in fmaxf)
+__device__ __forceinline__ float at_least(float x, float least)
+{
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(least));
+  return y;
+}
+
+// m is the largest value, or one that none exceeds by more than kSlack powers of two (Stream).
+struct Scored {
+  float m = lowest<float>(), s = 0.f, u = 0.f;
+
+  __device__ __forceinline__ void move(float to, float c)  // s and u relative to `to`, which is finite or +inf
+  {
+    const float a = at_least((m - to) * c, kLeast), f = power(a);
+    u = fmaf(s, a, u) * f;
+    s = s * f;
+    m = to;
+  }
+  __device__ __forceinline__ void add(float x, float base, float c)
+  {
+    const float a = at_least((x - base) * c, kLeast), p = power(a);
+    s += p;
+    u = fmaf(p, a, u);
+  }
+  __device__ __forceinline__ void join(float m2, float s2, float u2, float c)
+  {
+    const float to = fmaxf(m, m2);
+    if (to == lowest<float>()) {
+      s += s2;  // 0, or NaN
+      return;
+    }
+    Scored o;
+    o.m = m2;
+    o.s = s2;
+    o.u = u2;
+    o.move(to, c);
+    move(to, c);
+    s += o.s;
+    u += o.u;
+  }
+  __device__ __forceinline__ void join_lanes(float c)
+  {
+    const float to = max_lanes(m);
+    if (to != lowest<float>()) move(to, c);
+    s = sum_lanes(s);
+    u = sum_lanes(u);
+  }
+};
+
+// The same for a stream of pieces: `limit` is m + slack.
+struct ScoredStream : Scored {
+  float base = 0.f, limit = lowest<float>();
+  __device__ __forceinline__ void reach(float most, float c, float slack)
+  {
+    if (!(most > limit)) return;
+    move(most, c);
+    base  = most;
+    limit = most + slack;
+  }
+  template <int N>
+  __device__ __forceinline__ void take(const float (&x)[N], float c, float slack)
+  {
+    float most = x[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) most = fmaxf(most, x[e]);
+    reach(most, c, slack);
+#pragma unroll
+    for (int e = 0; e < N; ++e) add(x[e], base, c);
+  }
+};
+
+// All threads of the row get the joined value; `room`: shared, 3 floats per warp.
+template <int THREADS>
+__device__ __forceinline__ void join_scored(Scored& r, float c, float* room)
+{
+  r.join_lanes(c);
+  if (THREADS == 32) return;
+  constexpr int W = THREADS / 32;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  __syncthreads();
+  if (lane == 0) {
+    room[3 * warp]     = r.m;
+    room[3 * warp + 1] = r.s;
+    room[3 * warp + 2] = r.u;
+  }
+  __syncthreads();
+  r = Scored();
+  if (lane < W) {
+    r.m = room[3 * lane];
+    r.s = room[3 * lane + 1];
+    r.u = room[3 * lane + 2];
+  }
+  r.join_lanes(c);
+}
+
+// What is kept of a row for its gradient: m, 1 / s (0: the row does not count), -u / s and the class.
+__device__ __forceinline__ float4 kept_row(float m, float inverse, float mean, int at)
+{
+  return make_float4(m, inverse, mean, __int_as_float(at));
+}
+
+// The given class of a row, -1: none, -2: the row does not count.
+__device__ __forceinline__ int target_of(const Target& t, int64_t row, int64_t n_cols)
+{
+  if (!t.index) return -1;
+  const int64_t i = t.index64 ? static_cast<const int64_t*>(t.index)[row * t.stride]
+                              : static_cast<int64_t>(static_cast<const int32_t*>(t.index)[row * t.stride]);
+  return i >= 0 && i < n_cols && i != t.ignore ? static_cast<int>(i) : -2;
+}
+
+// Scores of a row, by one thread.  logit: of class `at`.  The difference of logits and the logarithm are joined in 64 bits; neither
+// a logarithm of a probability above 0 nor an entropy below it leaves by their roundings.
+struct RowScore {
+  double log_s;
+  bool counts;
+};
+__device__ __forceinline__ RowScore finish_score(const Scores& out, int64_t row, const Scored& r, double inv_t, int at, float logit)
+{
+  RowScore o;
+  o.log_s  = log_sum(r.s);
+  o.counts = at != -2 && !(r.s == 0.f);  // (no finite logit: no softmax)
+  const float mean = -r.u / r.s;
+  double log_prob  = (static_cast<double>(logit) - r.m) * inv_t - o.log_s;
+  double entropy   = o.log_s + mean * 0.69314718055994530942;
+  if (log_prob > 0) log_prob = 0;
+  if (entropy < 0) entropy = 0;
+  if (r.s != r.s) log_prob = NAN;
+  if (out.log_prob) out.log_prob[row] = o.counts ? static_cast<float>(log_prob) : 0.f;
+  out.entropy[row] = o.counts ? static_cast<float>(entropy) : 0.f;
+  out.kept[row]    = o.counts ? kept_row(r.m, 1.f / r.s, mean, at) : kept_row(0.f, 0.f, 0.f, -1);
+  return o;
+}
+
+// The gradient by the logits of a row: of class c it is 2^a (A + B a), and `add` more for the given one.
+struct RowGrad {
+  float base, A, B, add;
+  int at;
+  bool counts;
+  __device__ __forceinline__ float operator()(float z, float c) const
+  {
+    const float a = at_least((z - base) * c, kLeast);
+    return power(a) * fmaf(B, a, A);
+  }
+};
+// g, h: gradients by the row's log probability and entropy, times 1 / T (and a scale).
+__device__ __forceinline__ RowGrad row_grad(const float4& kept, float g, float h)
+{
+  RowGrad r;
+  r.base   = base_of(kept.x);
+  r.at     = __float_as_int(kept.w);
+  r.counts = kept.y != 0.f;
+  if (r.at < 0) g = 0.f;
+  r.add = g;
+  r.B   = -kept.y * kLn2 * h;
+  r.A   = fmaf(r.B, kept.z, -kept.y * g);
+  return r;
+}
+
+}  // namespace distill
+}  // namespace b2fil

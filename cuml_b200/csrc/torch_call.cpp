@@ -175,6 +175,15 @@ struct Library {
   decltype(&b2fil_linear_loss) linear;
   decltype(&b2fil_linear_loss_grad_workspace) linear_grad_workspace;
   decltype(&b2fil_linear_loss_grad) linear_grad;
+  decltype(&b2fil_log_probs_workspace) score_workspace;
+  decltype(&b2fil_log_probs) score;
+  decltype(&b2fil_log_probs_grad) score_grad;
+  decltype(&b2fil_linear_log_probs_workspace) linear_score_workspace;
+  decltype(&b2fil_linear_log_probs) linear_score;
+  decltype(&b2fil_linear_log_probs_grad_workspace) linear_score_grad_workspace;
+  decltype(&b2fil_linear_log_probs_grad) linear_score_grad;
+  decltype(&b2fil_clip_gradients_workspace) clip_workspace;
+  decltype(&b2fil_clip_gradients) clip;
 } library;
 
 struct LibraryError {
@@ -587,12 +596,338 @@ PyObject* top_scores(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   END_HANDLE_TH_ERRORS
 }
 
+// ---- scores ----------------------------------------------------------------------------------
+// One class per row, or none.  False: not what the library takes as it is.
+bool target_of(PyObject* o, const Tensor& like, int64_t ignore, Tensor& index, b2fil_target& t)
+{
+  t        = b2fil_target{};
+  t.ignore = ignore;
+  if (o == Py_None) return true;
+  if (!THPVariable_Check(o)) return false;
+  index = THPVariable_Unpack(o);
+  if (index.dim() != 1 || !index.is_cuda() || index.layout() != at::kStrided || at::isTensorSubclassLike(index) ||
+      (index.scalar_type() != at::kInt && index.scalar_type() != at::kLong) || index.size(0) != like.size(0) || !on(index, like))
+    return false;
+  t.index   = index.const_data_ptr();
+  t.stride  = index.stride(0);
+  t.index64 = index.scalar_type() == at::kLong;
+  return true;
+}
+
+// A node's gradients by the rows' log probabilities and entropies, which may not be there.
+struct Upstreams {
+  Tensor log_prob, entropy;
+  int64_t log_prob_stride = 0, entropy_stride = 0;
+  Upstreams(const Tensor& g, const Tensor& h)
+  {
+    if (g.defined()) log_prob = upstream_of(g, log_prob_stride);
+    if (h.defined()) entropy = upstream_of(h, entropy_stride);
+  }
+  static const float* at(const Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
+};
+constexpr const char* kFreed = "the scores' graph has been freed: retain_graph=True keeps it";
+
+// Outputs: log probability (where a target is given), entropy.
+struct ScoreNode : ag::Node {
+  Saved logits;
+  Tensor kept;
+  double temperature;
+  bool has_target, gone = false;
+
+  ag::variable_list apply(ag::variable_list&& grads) override
+  {
+    TORCH_CHECK(!gone, kFreed);
+    const Tensor g = has_target ? grads[0] : Tensor(), h = grads[has_target];
+    if (!g.defined() && !h.defined()) return {Tensor()};
+    const Tensor saved = logits.unpack();
+    Tensor grad;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      at::NoGradGuard no_grad;
+      const Tensor x  = in_rows(saved);
+      const int64_t n = x.size(0), c = x.size(1);
+      grad = make({n, c}, x.scalar_type(), x);
+      const Upstreams up(g, h);
+      const int device = x.get_device();
+      try {
+        ok(library.score_grad(type_of(x), x.const_data_ptr(), n, c, x.stride(0), temperature, kept.const_data_ptr<float>(),
+                              Upstreams::at(up.log_prob), up.log_prob_stride, Upstreams::at(up.entropy), up.entropy_stride,
+                              grad.mutable_data_ptr(), c, device, stream_of(device)));
+      } catch (const LibraryError& e) {
+        raise_library_error(e);
+      }
+    }
+    no_second_derivative(grad, {g, h, saved});
+    return {grad};
+  }
+  void release_variables() override
+  {
+    logits.variable.reset_data();
+    kept = Tensor();
+    gone = true;
+  }
+  std::string name() const override { return "LogProbsBackward"; }
+};
+
+struct LinearScoreNode : ag::Node {
+  Saved hidden, weight;
+  Tensor kept;
+  double temperature;
+  bool has_target, gone = false;
+
+  ag::variable_list apply(ag::variable_list&& grads) override
+  {
+    TORCH_CHECK(!gone, kFreed);
+    const Tensor g = has_target ? grads[0] : Tensor(), h_up = grads[has_target];
+    if (!g.defined() && !h_up.defined()) return {Tensor(), Tensor()};
+    const Tensor saved_h = hidden.unpack(), saved_w = weight.unpack();
+    Tensor dh, dw;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      at::NoGradGuard no_grad;
+      const Tensor h = in_rows(saved_h), w = in_rows(saved_w);
+      const int64_t n = h.size(0), width = h.size(1), c = w.size(0);
+      auto step = [&](const Tensor& x) { return x.size(0) == 1 ? width : x.stride(0); };
+      const bool wants_h = task_should_compute_output(0), wants_w = task_should_compute_output(1);
+      if (wants_h) dh = make({n, width}, h.scalar_type(), h);
+      if (wants_w) dw = make({c, width}, h.scalar_type(), h);
+      const Upstreams up(g, h_up);
+      const int device = h.get_device(), type = type_of(h);
+      try {
+        const int64_t room = ok(library.linear_score_grad_workspace(type, h.const_data_ptr(), step(h), w.const_data_ptr(), step(w),
+                                                                     n, c, width, wants_h, wants_w, device));
+        const Tensor work  = make({room}, at::kByte, h);
+        ok(library.linear_score_grad(type, h.const_data_ptr(), step(h), w.const_data_ptr(), step(w), n, c, width, temperature,
+                                     kept.const_data_ptr<float>(), Upstreams::at(up.log_prob), up.log_prob_stride,
+                                     Upstreams::at(up.entropy), up.entropy_stride, wants_h ? dh.mutable_data_ptr() : nullptr,
+                                     wants_w ? dw.mutable_data_ptr() : nullptr, work.mutable_data_ptr(), room, device,
+                                     stream_of(device)));
+      } catch (const LibraryError& e) {
+        raise_library_error(e);
+      }
+    }
+    no_second_derivative(dh, {g, h_up, saved_h, saved_w});
+    no_second_derivative(dw, {g, h_up, saved_h, saved_w});
+    return {dh, dw};
+  }
+  void release_variables() override
+  {
+    hidden.variable.reset_data();
+    weight.variable.reset_data();
+    kept = Tensor();
+    gone = true;
+  }
+  std::string name() const override { return "LinearLogProbsBackward"; }
+};
+
+// The log probabilities (None without a target), the entropies and two more, as a tuple of `n`.
+PyObject* pack_scores(Tensor log_prob, Tensor entropy, Tensor top, Tensor index, int n)
+{
+  PyObject* out[4] = {THPVariable_Wrap(std::move(log_prob)), THPVariable_Wrap(std::move(entropy)), nullptr, nullptr};
+  for (int i = 2; i < n; ++i) out[i] = THPVariable_Wrap(i == 2 ? std::move(top) : std::move(index));  // (undefined: None)
+  PyObject* r = nullptr;
+  if (out[0] && out[1] && (n < 3 || (out[2] && out[3])))
+    r = n == 2 ? PyTuple_Pack(2, out[0], out[1]) : PyTuple_Pack(4, out[0], out[1], out[2], out[3]);
+  for (PyObject* x : out) Py_XDECREF(x);
+  return r;
+}
+// Room for a row's scores in `kept`: what the gradient needs comes first.
+Tensor score_room(int64_t n, int64_t more, const Tensor& like) { return make({4 * n + more}, at::kFloat, like); }
+
+// logits, target or None, temperature, k, ignored class -> (log_prob or None, entropy, best log probabilities, their classes)
+PyObject* log_probs(PyObject*, PyObject* const* args, Py_ssize_t nargs)
+{
+  HANDLE_TH_ERRORS
+  if (nargs != 5) return PyErr_Format(PyExc_TypeError, "log_probs takes 5 arguments");
+  const double temperature = PyFloat_AsDouble(args[2]);
+  const int64_t k = PyLong_AsLongLong(args[3]), ignore = PyLong_AsLongLong(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!library.score || !plain_rows(args[0]) || has_tangent(args[0])) Py_RETURN_NONE;
+  const Tensor& x = THPVariable_Unpack(args[0]);
+  const int type  = type_of(x);
+  Tensor index;
+  b2fil_target t;
+  if (type < 0 || type == B2FIL_TYPE_F64 || k < 0 || k > x.size(1) || k > B2FIL_MOST_TOP || !target_of(args[1], x, ignore, index, t))
+    Py_RETURN_NONE;
+  const bool has_target = t.index != nullptr;
+  const int64_t n = x.size(0), c = x.size(1);
+  Tensor kept, log_prob, entropy, top, classes;
+  try {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const int device   = x.get_device();
+    const int64_t room = ok(library.score_workspace(type, n, c, static_cast<int>(k), device));
+    const int64_t work_at = (4 * n + 63) / 64 * 64;
+    kept    = score_room(n, work_at - 4 * n + room / 4, x);
+    entropy = make({n}, at::kFloat, x);
+    if (has_target) log_prob = make({n}, at::kFloat, x);
+    if (k) {
+      top     = make({n, k}, at::kFloat, x);
+      classes = make({n, k}, at::kInt, x);
+    }
+    float* at = kept.mutable_data_ptr<float>();
+    ok(library.score(type, x.const_data_ptr(), n, c, x.stride(0), &t, temperature, static_cast<int>(k),
+                     has_target ? log_prob.mutable_data_ptr<float>() : nullptr, entropy.mutable_data_ptr<float>(), at,
+                     k ? top.mutable_data_ptr<float>() : nullptr, k ? classes.mutable_data_ptr<int>() : nullptr, at + work_at, room,
+                     device, stream_of(device)));
+  } catch (const LibraryError& e) {
+    return PyLong_FromLong(e.code);
+  }
+  if (at::GradMode::is_enabled() && x.requires_grad()) {
+    auto node = std::shared_ptr<ScoreNode>(new ScoreNode(), ag::deleteNode);
+    node->set_next_edges(ag::collect_next_edges(x));
+    node->logits.set(x);
+    node->kept        = std::move(kept);
+    node->temperature = temperature;
+    node->has_target  = has_target;
+    if (has_target) ag::set_history(log_prob, node);
+    ag::set_history(entropy, node);
+  }
+  return pack_scores(std::move(log_prob), std::move(entropy), std::move(top), std::move(classes), 4);
+  END_HANDLE_TH_ERRORS
+}
+
+// hidden, weight, target or None, temperature, ignored class, whether autocast has been heeded -> (log_prob or None, entropy)
+PyObject* linear_log_probs(PyObject*, PyObject* const* args, Py_ssize_t nargs)
+{
+  HANDLE_TH_ERRORS
+  if (nargs != 6) return PyErr_Format(PyExc_TypeError, "linear_log_probs takes 6 arguments");
+  const double temperature = PyFloat_AsDouble(args[3]);
+  const int64_t ignore     = PyLong_AsLongLong(args[4]);
+  const int cast           = PyObject_IsTrue(args[5]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!library.linear_score || (!cast && at::autocast::is_autocast_enabled(at::kCUDA)) || !plain_rows(args[0]) ||
+      !plain_rows(args[1]) || has_tangent(args[0]) || has_tangent(args[1]))
+    Py_RETURN_NONE;
+  const Tensor& h = THPVariable_Unpack(args[0]);
+  const Tensor& w = THPVariable_Unpack(args[1]);
+  const int type  = type_of(h);
+  const int64_t n = h.size(0), width = h.size(1), c = w.size(0);
+  auto step = [&](const Tensor& x) { return x.size(0) == 1 ? width : x.stride(0); };
+  Tensor index;
+  b2fil_target t;
+  if ((type != B2FIL_TYPE_BF16 && type != B2FIL_TYPE_F16) || w.scalar_type() != h.scalar_type() || !on(w, h) ||
+      w.size(1) != width || !target_of(args[2], h, ignore, index, t))
+    Py_RETURN_NONE;
+  const bool has_target = t.index != nullptr;
+  Tensor kept, log_prob, entropy;
+  try {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const int device   = h.get_device();
+    const int64_t room = ok(library.linear_score_workspace(type, h.const_data_ptr(), step(h), w.const_data_ptr(), step(w), n, c,
+                                                            width, device));
+    const Tensor work  = make({room}, at::kByte, h);
+    kept    = score_room(n, 0, h);
+    entropy = make({n}, at::kFloat, h);
+    if (has_target) log_prob = make({n}, at::kFloat, h);
+    ok(library.linear_score(type, h.const_data_ptr(), step(h), w.const_data_ptr(), step(w), n, c, width, &t, temperature,
+                            has_target ? log_prob.mutable_data_ptr<float>() : nullptr, entropy.mutable_data_ptr<float>(),
+                            kept.mutable_data_ptr<float>(), work.mutable_data_ptr(), room, device, stream_of(device)));
+  } catch (const LibraryError& e) {
+    return PyLong_FromLong(e.code);
+  }
+  if (at::GradMode::is_enabled() && (h.requires_grad() || w.requires_grad())) {
+    auto node = std::shared_ptr<LinearScoreNode>(new LinearScoreNode(), ag::deleteNode);
+    node->set_next_edges(ag::collect_next_edges(h, w));
+    node->hidden.set(h);
+    node->weight.set(w);
+    node->kept        = std::move(kept);
+    node->temperature = temperature;
+    node->has_target  = has_target;
+    if (has_target) ag::set_history(log_prob, node);
+    ag::set_history(entropy, node);
+  }
+  return pack_scores(std::move(log_prob), std::move(entropy), Tensor(), Tensor(), 2);
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- gradients -------------------------------------------------------------------------------
+// A gradient (or what takes it) whose elements lie one after the other in some order.
+bool dense(const Tensor& t, const Tensor& like)
+{
+  const int type = type_of(t);
+  return t.is_cuda() && t.layout() == at::kStrided && !at::isTensorSubclassLike(t) && !t.is_neg() && !t.is_conj() &&
+         (type == B2FIL_TYPE_F32 || type == B2FIL_TYPE_BF16 || type == B2FIL_TYPE_F16) && on(t, like) &&
+         t.is_non_overlapping_and_dense();
+}
+
+// gradients, out (lists; out may be None), largest norm, kind of norm, whether to scale -> norm
+PyObject* clip_gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs)
+{
+  HANDLE_TH_ERRORS
+  if (nargs != 5) return PyErr_Format(PyExc_TypeError, "clip_gradients takes 5 arguments");
+  const double most = PyFloat_AsDouble(args[2]);
+  const int kind    = static_cast<int>(PyLong_AsLong(args[3]));
+  const int scales  = PyObject_IsTrue(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  const bool apart = args[1] != Py_None;
+  if (!library.clip || !PyList_Check(args[0]) || (apart && (!PyList_Check(args[1]) || PyList_GET_SIZE(args[0]) != PyList_GET_SIZE(args[1]))))
+    Py_RETURN_NONE;
+  std::vector<b2fil_gradient> entries;
+  std::vector<Tensor> written;
+  Tensor first;
+  const Py_ssize_t size = PyList_GET_SIZE(args[0]);
+  entries.reserve(size);
+  written.reserve(size);
+  for (Py_ssize_t i = 0; i < size; ++i) {
+    PyObject* o = PyList_GET_ITEM(args[0], i);
+    if (o == Py_None) continue;
+    if (!THPVariable_Check(o)) Py_RETURN_NONE;
+    Tensor x = THPVariable_Unpack(o);
+    if (at::isTensorSubclassLike(x)) Py_RETURN_NONE;
+    if (x.requires_grad() && x.is_leaf()) x = x.grad();
+    if (!x.defined()) continue;
+    if (!first.defined()) first = x;
+    if (!dense(x, first)) Py_RETURN_NONE;
+    Tensor to = x;
+    if (apart) {
+      PyObject* p = PyList_GET_ITEM(args[1], i);
+      if (!THPVariable_Check(p)) Py_RETURN_NONE;
+      to = THPVariable_Unpack(p);
+      if (!dense(to, first) || to.sizes() != x.sizes() || to.strides() != x.strides() || to.requires_grad()) Py_RETURN_NONE;
+    }
+    b2fil_gradient g{};
+    g.from      = x.const_data_ptr();
+    g.to        = const_cast<void*>(to.const_data_ptr());
+    g.rows      = 1;
+    g.cols      = x.numel();
+    g.from_col  = g.to_col = 1;
+    g.from_type = type_of(x);
+    g.to_type   = type_of(to);
+    g.tensor    = static_cast<int32_t>(i);
+    entries.push_back(g);
+    if (scales) written.push_back(std::move(to));
+  }
+  if (!first.defined()) Py_RETURN_NONE;
+  Tensor norm;
+  try {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const int device   = first.get_device();
+    const int64_t n    = static_cast<int64_t>(entries.size());
+    const int64_t room = ok(library.clip_workspace(entries.data(), n, device));
+    const Tensor work  = make({room}, at::kByte, first);
+    norm               = make({}, at::kFloat, first);
+    ok(library.clip(entries.data(), n, kind, scales, most, norm.mutable_data_ptr<float>(), work.mutable_data_ptr(), room, device,
+                    stream_of(device)));
+  } catch (const LibraryError& e) {
+    return PyLong_FromLong(e.code);
+  }
+  for (const Tensor& x : written)
+    if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+  return THPVariable_Wrap(std::move(norm));
+  END_HANDLE_TH_ERRORS
+}
+
 // Addresses of the library's entry points, in the order of `Library`.
 PyObject* bind(PyObject*, PyObject* args)
 {
-  unsigned long long a[10];
-  if (!PyArg_ParseTuple(args, "KKKKKKKKKK", a, a + 1, a + 2, a + 3, a + 4, a + 5, a + 6, a + 7, a + 8, a + 9)) return nullptr;
-  static_assert(sizeof(Library) == 10 * sizeof(void*), "one address each");
+  constexpr int N = 19;
+  static_assert(sizeof(Library) == N * sizeof(void*), "one address each");
+  unsigned long long a[N];
+  if (PyTuple_GET_SIZE(args) != N) return PyErr_Format(PyExc_TypeError, "bind takes %d addresses", N);
+  for (int i = 0; i < N; ++i) {
+    a[i] = PyLong_AsUnsignedLongLong(PyTuple_GET_ITEM(args, i));
+    if (PyErr_Occurred()) return nullptr;
+  }
   Library l;
   auto put = [](auto& f, unsigned long long at) { f = reinterpret_cast<std::decay_t<decltype(f)>>(static_cast<uintptr_t>(at)); };
   put(l.last_error, a[0]);
@@ -605,6 +940,15 @@ PyObject* bind(PyObject*, PyObject* args)
   put(l.linear, a[7]);
   put(l.linear_grad_workspace, a[8]);
   put(l.linear_grad, a[9]);
+  put(l.score_workspace, a[10]);
+  put(l.score, a[11]);
+  put(l.score_grad, a[12]);
+  put(l.linear_score_workspace, a[13]);
+  put(l.linear_score, a[14]);
+  put(l.linear_score_grad_workspace, a[15]);
+  put(l.linear_score_grad, a[16]);
+  put(l.clip_workspace, a[17]);
+  put(l.clip, a[18]);
   library = l;
   Py_RETURN_NONE;
 }
@@ -614,6 +958,9 @@ PyMethodDef module_methods[] = {
   {"top_scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(top_scores)), METH_FASTCALL, nullptr},
   {"distill_loss", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(distill_loss)), METH_FASTCALL, nullptr},
   {"linear_loss", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_loss)), METH_FASTCALL, nullptr},
+  {"log_probs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(log_probs)), METH_FASTCALL, nullptr},
+  {"linear_log_probs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_log_probs)), METH_FASTCALL, nullptr},
+  {"clip_gradients", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(clip_gradients)), METH_FASTCALL, nullptr},
   {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "b2fil_torch",

@@ -10,6 +10,13 @@ model), keep the `k` best classes of each row, and compute the loss of a student
     linear_cross_entropy       softmax cross entropy from the last linear layer, logits not kept
     linear_distillation_loss   distillation_loss from the last linear layer, logits not kept
 
+score its (or any classifier's) answers, with gradients, and take care of the gradients of a step:
+
+    log_probs                  log probability of each row's given class, its entropy, its best alternatives
+    linear_log_probs           the first two from the last linear layer, logits not kept
+    gradient_norm              the norm of all gradients together
+    clip_gradients             gradients scaled down to a largest norm
+
 `ForestInference.predict_top`, `.teach` and `.distillation_loss` call them with a forest as the teacher.
 All tensors are CUDA tensors of one device; work is enqueued on torch's current stream of that device and
 nothing waits.  The losses have first derivatives by the logits, or by the layer's input and weight (backward mode
@@ -20,6 +27,7 @@ alive).  All computation happens in libb2fil.so.
 from __future__ import annotations
 
 import ctypes as C
+import math
 import warnings
 from typing import NamedTuple, Optional
 
@@ -49,6 +57,25 @@ class CTeacher(C.Structure):
                 ("k", C.c_int32), ("index64", C.c_int32)]
 
 
+class LogProbs(NamedTuple):
+    """Scores of each row (see `log_probs`); `log_prob` is None without a target, `top` without alternatives."""
+    log_prob: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top: Optional[TopScores]
+
+
+class CTarget(C.Structure):
+    """`b2fil_target`."""
+    _fields_ = [("index", C.c_void_p), ("stride", C.c_int64), ("ignore", C.c_int64), ("index64", C.c_int32)]
+
+
+class CGradient(C.Structure):
+    """`b2fil_gradient`."""
+    _fields_ = [("from_", C.c_void_p), ("to", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64),
+                ("from_row", C.c_int64), ("from_col", C.c_int64), ("to_row", C.c_int64), ("to_col", C.c_int64),
+                ("from_type", C.c_int32), ("to_type", C.c_int32), ("tensor", C.c_int32)]
+
+
 _call = None  # the compiled call path; False: not available
 
 
@@ -67,7 +94,9 @@ def _native():
         module.bind(*(C.cast(getattr(lib, "b2fil_" + name), C.c_void_p).value for name in (
             "last_error", "top_scores_workspace", "top_scores", "distill_loss_workspace", "distill_loss",
             "distill_loss_grad", "linear_loss_workspace", "linear_loss", "linear_loss_grad_workspace",
-            "linear_loss_grad")))
+            "linear_loss_grad", "log_probs_workspace", "log_probs", "log_probs_grad", "linear_log_probs_workspace",
+            "linear_log_probs", "linear_log_probs_grad_workspace", "linear_log_probs_grad", "clip_gradients_workspace",
+            "clip_gradients")))
         _call = module
     return _call
 
@@ -458,6 +487,274 @@ def linear_distillation_loss(hidden, weight, top, *, temperature: float = 1.0, r
     values, index, _ = _top(top, hidden.shape[0], hidden.device, "renormalise")
     loss = _linear(hidden, weight, values, index, _temperature(temperature), _NO_CLASS, _reduction(reduction))
     return loss.view(shape) if reduction == "none" and len(shape) != 1 else loss
+
+
+class _Scores(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, target, temperature, k, ignore):
+        lib, kind, dev = _lib.load(), _TYPES[logits.dtype], logits.device
+        x = _rows(logits)
+        n, n_cols = x.shape
+        ws = _workspace(lib.b2fil_log_probs_workspace(kind, n, n_cols, k, dev.index), dev)
+        log_prob, entropy, kept = _scores(n, target, dev)
+        top = torch.empty((n, k), dtype=torch.float32, device=dev) if k else None
+        index = torch.empty((n, k), dtype=torch.int32, device=dev) if k else None
+        _lib.check(lib.b2fil_log_probs(
+            kind, x.data_ptr(), n, n_cols, x.stride(0), C.byref(_c_target(target, ignore)), temperature, k, _at(log_prob),
+            entropy.data_ptr(), kept.data_ptr(), _at(top), _at(index), ws.data_ptr(), ws.numel(), dev.index, _stream(dev)))
+        ctx.save_for_backward(logits)
+        ctx.like = (logits.shape, logits.dtype, logits.device)
+        ctx.kept, ctx.temperature = kept, temperature
+        ctx.set_materialize_grads(False)
+        if k:
+            ctx.mark_non_differentiable(top, index)
+        return log_prob, entropy, top, index
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, of_log_prob, of_entropy, *_):
+        (logits,) = ctx.saved_tensors
+        lib, kind, dev = _lib.load(), _TYPES[logits.dtype], logits.device
+        x = _saved(logits, ctx.like)
+        n, n_cols = x.shape
+        grad = torch.empty((n, n_cols), dtype=x.dtype, device=dev)
+        g, g_stride, h, h_stride = _both(of_log_prob, of_entropy)
+        _lib.check(lib.b2fil_log_probs_grad(
+            kind, x.data_ptr(), n, n_cols, x.stride(0), ctx.temperature, ctx.kept.data_ptr(), _at(g), g_stride, _at(h),
+            h_stride, grad.data_ptr(), n_cols, dev.index, _stream(dev)))
+        return grad, None, None, None, None
+
+
+class _LinearScores(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, target, temperature, ignore):
+        lib, kind, dev = _lib.load(), _TYPES[hidden.dtype], hidden.device
+        (n, width), n_cols = hidden.shape, weight.shape[0]
+        layer = (hidden.data_ptr(), _step(hidden), weight.data_ptr(), _step(weight), n, n_cols, width)
+        ws = _workspace(lib.b2fil_linear_log_probs_workspace(kind, *layer, dev.index), dev)
+        log_prob, entropy, kept = _scores(n, target, dev)
+        _lib.check(lib.b2fil_linear_log_probs(
+            kind, *layer, C.byref(_c_target(target, ignore)), temperature, _at(log_prob), entropy.data_ptr(),
+            kept.data_ptr(), ws.data_ptr(), ws.numel(), dev.index, _stream(dev)))
+        ctx.save_for_backward(hidden, weight)
+        ctx.like = [(x.shape, x.dtype, x.device) for x in (hidden, weight)]
+        ctx.kept, ctx.temperature = kept, temperature
+        ctx.set_materialize_grads(False)
+        return log_prob, entropy
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, of_log_prob, of_entropy):
+        hidden, weight = map(_saved, ctx.saved_tensors, ctx.like)
+        lib, kind, dev = _lib.load(), _TYPES[hidden.dtype], hidden.device
+        (n, width), n_cols = hidden.shape, weight.shape[0]
+        of_hidden, of_weight = ctx.needs_input_grad[:2]
+        dh = torch.empty((n, width), dtype=hidden.dtype, device=dev) if of_hidden else None
+        dw = torch.empty((n_cols, width), dtype=hidden.dtype, device=dev) if of_weight else None
+        layer = (hidden.data_ptr(), _step(hidden), weight.data_ptr(), _step(weight), n, n_cols, width)
+        ws = _workspace(lib.b2fil_linear_log_probs_grad_workspace(kind, *layer, of_hidden, of_weight, dev.index), dev)
+        g, g_stride, h, h_stride = _both(of_log_prob, of_entropy)
+        _lib.check(lib.b2fil_linear_log_probs_grad(
+            kind, *layer, ctx.temperature, ctx.kept.data_ptr(), _at(g), g_stride, _at(h), h_stride, _at(dh), _at(dw),
+            ws.data_ptr(), ws.numel(), dev.index, _stream(dev)))
+        return dh, dw, None, None, None
+
+
+def _at(x):
+    return None if x is None else x.data_ptr()
+
+
+def _scores(n, target, dev):
+    """(log_prob or None, entropy, what is kept for the gradient)."""
+    new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)  # noqa: E731
+    return new(n) if target is not None else None, new(n), new(n, 4)
+
+
+def _c_target(target, ignore):
+    if target is None:
+        return CTarget(None, 0, ignore, 0)
+    return CTarget(target.data_ptr(), target.stride(0), ignore, target.dtype == torch.int64)
+
+
+def _both(of_log_prob, of_entropy):
+    """Gradients by the two scores in fp32 and their strides; None: not used."""
+    out = []
+    for g in (of_log_prob, of_entropy):
+        out += (None, 0) if g is None else _upstream(g)
+    return out
+
+
+def log_probs(logits, target=None, *, temperature: float = 1.0, top: int = 0, ignore_index: int = -100) -> LogProbs:
+    """Scores of each row of `logits` (..., n_classes), fp32, bf16 or fp16, with q = softmax(logits / temperature).
+
+    target : (...) int32 or int64, the given classes, or None.  Rows whose target is `ignore_index` or outside
+        [0, n_classes) do not count; nor do rows whose logits are all -inf.
+    top : also the `top` most probable classes, at most min(n_classes, 256).
+
+    Returns `LogProbs`, fp32: `log_prob` (...), log q of the target; `entropy` (...), -sum q log q; `top`, a
+    `TopScores` of log q in descending order, equal logits in the order of their classes, without a
+    logsumexp.  Rows that do not count have the scores 0, and alternatives of log q 0 and class -1 (which a distillation
+    loss does not count); their logits may be anything, their gradient is 0.  `log_prob` and `entropy` have first
+    derivatives by the logits, the alternatives are constants."""
+    temperature, ignore, k = _temperature(temperature), int(ignore_index), int(top)
+    call = _native() if isinstance(logits, torch.Tensor) and logits.is_cuda else False
+    if call and (out := _answer(call.log_probs(logits, target, temperature, k, ignore))) is not None:
+        return LogProbs(out[0], out[1], TopScores(out[2], out[3], None) if k else None)
+    _cuda("logits", logits, _STUDENT)
+    if logits.ndim < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must have shape (..., n_classes), got {tuple(logits.shape)}")
+    shape, n_cols = logits.shape[:-1], logits.shape[-1]
+    if not 0 <= k <= min(n_cols, MOST_TOP):
+        raise ValueError(f"top must be between 0 and min(n_classes, {MOST_TOP}) = {min(n_cols, MOST_TOP)}, got {k}")
+    if target is not None:
+        target = _target(target, shape, logits.device)
+    x = logits if logits.ndim == 2 else logits.reshape(-1, n_cols)
+    log_prob, entropy, values, index = _Scores.apply(x, target, temperature, k, ignore)
+    if len(shape) != 1:
+        log_prob, entropy = (s if s is None else s.view(shape) for s in (log_prob, entropy))
+        values, index = (s if s is None else s.view(*shape, k) for s in (values, index))
+    return LogProbs(log_prob, entropy, TopScores(values, index, None) if k else None)
+
+
+def linear_log_probs(hidden, weight, target=None, *, temperature: float = 1.0, ignore_index: int = -100) -> LogProbs:
+    """`log_probs` (without alternatives) of the logits `hidden @ weight.T`, without keeping them.
+
+    hidden : (..., width), weight : (n_classes, width), both bf16 or both fp16 (under autocast they are cast).
+    target, temperature, ignore_index : as in `log_probs`; the hidden values of rows that do not count must be finite
+        all the same (they take part in weight's gradient with zeros).
+
+    Types, rounding and waits as in `linear_cross_entropy`."""
+    temperature, ignore = _temperature(temperature), int(ignore_index)
+    call = _native() if isinstance(hidden, torch.Tensor) and hidden.is_cuda else False
+    if call and (out := _answer(call.linear_log_probs(hidden, weight, target, temperature, ignore, False))) is not None:
+        return LogProbs(*out, None)
+    hidden, weight, shape = _layer(hidden, weight)
+    if target is not None:
+        target = _target(target, shape, hidden.device)
+    out = _answer(call.linear_log_probs(hidden, weight, target, temperature, ignore, True)) if call else None
+    if out is None:
+        out = _LinearScores.apply(hidden, weight, target, temperature, ignore)
+    if len(shape) != 1:
+        out = [s if s is None else s.view(shape) for s in out]
+    return LogProbs(*out, None)
+
+
+_NORMS = {2.0: 2, 1.0: 1, math.inf: 0}
+
+
+def _dims(x, out):
+    """Dimensions of `x` (and of `out`, of the same shape) as (size, stride, stride of out), the largest stride first,
+    neighbours that are one in both joined."""
+    dims = sorted(((n, s, t) for n, s, t in zip(x.shape, x.stride(), out.stride()) if n != 1),
+                  key=lambda d: (-d[1], -d[2]))
+    joined = []
+    for n, s, t in dims:
+        if joined and joined[-1][1] == n * s and joined[-1][2] == n * t:
+            joined[-1] = (joined[-1][0] * n, s, t)
+        else:
+            joined.append((n, s, t))
+    return joined
+
+
+def _entries(number, x, out):
+    """`b2fil_gradient`s of one tensor: rows and columns, one entry per index of what dimensions are left."""
+    if x.numel() == 0:
+        return []
+    types = _TYPES[x.dtype], _TYPES[out.dtype]
+    *outer, (rows, from_row, to_row), (cols, from_col, to_col) = [(1, 0, 0)] * 2 + _dims(x, out)
+    places = [(x.data_ptr(), out.data_ptr())]
+    for n, s, t in outer:
+        places = [(a + i * s * x.element_size(), b + i * t * out.element_size()) for a, b in places for i in range(n)]
+    return [CGradient(a, b, rows, cols, from_row, from_col, to_row, to_col, *types, number) for a, b in places]
+
+
+def _overlaps_itself(x):
+    span = 1
+    for n, s, _ in reversed(_dims(x, x)):
+        if s < span and x.numel():
+            return True
+        span += (n - 1) * s
+    return False
+
+
+def _clip(gradients, most, norm_type, out, scales):
+    try:
+        kind = _NORMS[float(norm_type)]
+    except (KeyError, TypeError, ValueError):
+        raise ValueError(f"norm_type must be 2, 1 or inf, got {norm_type!r}") from None
+    if isinstance(gradients, torch.Tensor):
+        raise TypeError("gradients must be a list of tensors, not a tensor")
+    gradients = list(gradients)
+    if isinstance(out, torch.Tensor):
+        raise TypeError("out must be a list of tensors, not a tensor")
+    out = None if out is None else list(out)
+    if out is not None and len(out) != len(gradients):
+        raise ValueError(f"out has {len(out)} tensors, there are {len(gradients)} gradients")
+    call = _native() if torch.cuda.is_available() else False
+    if call and (norm := _answer(call.clip_gradients(gradients, out, most, kind, scales))) is not None:
+        return norm
+    pairs = []
+    for i, x in enumerate(gradients):
+        if isinstance(x, torch.Tensor) and x.is_leaf and x.requires_grad:
+            x = x.grad
+        if x is None:
+            continue
+        _cuda("a gradient", x, _STUDENT)
+        to = x if out is None else out[i]
+        if out is not None:
+            _cuda("a tensor of out", to, _STUDENT)
+            if to.shape != x.shape:
+                raise ValueError(f"a gradient and its out differ in shape: {tuple(x.shape)}, {tuple(to.shape)}")
+            if to.requires_grad:
+                raise ValueError("a tensor of out requires grad")
+        if x.layout != torch.strided or to.layout != torch.strided:
+            raise ValueError("gradients must be strided tensors")
+        if scales and _overlaps_itself(to):
+            raise ValueError("the elements of a scaled gradient overlap in memory")
+        pairs.append((x.detach(), to.detach() if to is not x else None))
+    dev = pairs[0][0].device if pairs else torch.device("cuda", torch.cuda.current_device())
+    for x, to in pairs:
+        if x.device != dev or (to is not None and to.device != dev):
+            raise ValueError(f"gradients are on {dev} and on {x.device if x.device != dev else to.device}")
+    entries = [e for i, (x, to) in enumerate(pairs) for e in _entries(i, x, x if to is None else to)]
+    array = (CGradient * len(entries))(*entries)
+    lib = _lib.load()
+    ws = _workspace(lib.b2fil_clip_gradients_workspace(array, len(entries), dev.index), dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    _lib.check(lib.b2fil_clip_gradients(array, len(entries), kind, scales, most, norm.data_ptr(), ws.data_ptr(), ws.numel(),
+                                        dev.index, _stream(dev)))
+    if scales:
+        for x, to in pairs:
+            written = x if to is None else to
+            if not written.is_inference():
+                torch.autograd.graph.increment_version(written)
+    return norm
+
+
+def gradient_norm(gradients, *, norm_type: float = 2.0) -> torch.Tensor:
+    """The norm of all `gradients` together, a fp32 tensor without dimensions: the root of the sum of their squares
+    (`norm_type` 2), the sum of their sizes (1) or the largest of these (inf).
+
+    gradients : tensors of any shapes and strides on one device, fp32, bf16 or fp16; a parameter (a leaf that requires grad)
+        stands for its `.grad`; None is left out.  Without any the norm is 0.
+
+    Sums are taken in 64 bits where 32 would overflow or lose the small ones; no result depends on an order."""
+    return _clip(gradients, 0.0, norm_type, None, False)
+
+
+def clip_gradients(gradients, max_norm: float, *, norm_type: float = 2.0, out=None) -> torch.Tensor:
+    """Scale `gradients` by min(1, max_norm / norm), in place, and return their norm before that (`gradient_norm`).
+
+    out : a tensor for each gradient, of its shape and of any of the types, which takes the scaled one instead (where a gradient
+        is None: anything).
+
+    Each element is multiplied in 32 bits and rounded once.  Where the norm is not finite, the gradients stay as they
+    are: nothing waits for the norm, its caller sees it.  Tensors that are written may not overlap with others of the call;
+    autograd sees that they have been written, and no more."""
+    most = float(max_norm)
+    if not most >= 0:
+        raise ValueError(f"max_norm must be 0 or more, got {max_norm}")
+    return _clip(gradients, most, norm_type, out, True)
 
 
 def check_status(device=None) -> None:

@@ -105,6 +105,25 @@ def load() -> C.CDLL:
     lib.b2fil_linear_loss_grad.restype = i32
     lib.b2fil_linear_loss_grad.argtypes = [i32, vp, i64, vp, i64, i64, i64, i64, i32, f64, vp, vp, vp, vp, vp, i64, vp,
                                            vp, vp, vp, i64, i32, vp]
+    lib.b2fil_log_probs_workspace.restype = i64
+    lib.b2fil_log_probs_workspace.argtypes = [i32, i64, i64, i32, i32]
+    lib.b2fil_log_probs.restype = i32
+    lib.b2fil_log_probs.argtypes = [i32, vp, i64, i64, i64, vp, f64, i32, vp, vp, vp, vp, vp, vp, i64, i32, vp]
+    lib.b2fil_log_probs_grad.restype = i32
+    lib.b2fil_log_probs_grad.argtypes = [i32, vp, i64, i64, i64, f64, vp, vp, i64, vp, i64, vp, i64, i32, vp]
+    lib.b2fil_linear_log_probs_workspace.restype = i64
+    lib.b2fil_linear_log_probs_workspace.argtypes = [i32, vp, i64, vp, i64, i64, i64, i64, i32]
+    lib.b2fil_linear_log_probs.restype = i32
+    lib.b2fil_linear_log_probs.argtypes = [i32, vp, i64, vp, i64, i64, i64, i64, vp, f64, vp, vp, vp, vp, i64, i32, vp]
+    lib.b2fil_linear_log_probs_grad_workspace.restype = i64
+    lib.b2fil_linear_log_probs_grad_workspace.argtypes = [i32, vp, i64, vp, i64, i64, i64, i64, i32, i32, i32]
+    lib.b2fil_linear_log_probs_grad.restype = i32
+    lib.b2fil_linear_log_probs_grad.argtypes = [i32, vp, i64, vp, i64, i64, i64, i64, f64, vp, vp, i64, vp, i64, vp, vp, vp,
+                                                i64, i32, vp]
+    lib.b2fil_clip_gradients_workspace.restype = i64
+    lib.b2fil_clip_gradients_workspace.argtypes = [vp, i64, i32]
+    lib.b2fil_clip_gradients.restype = i32
+    lib.b2fil_clip_gradients.argtypes = [vp, i64, i32, i32, f64, vp, vp, i64, i32, vp]
     lib.b2fil_distill_status.restype = i32
     lib.b2fil_distill_status.argtypes = [i32, C.POINTER(C.c_int32)]
     lib.b2fil_distill_selftest_timeout.restype = i32

@@ -442,6 +442,75 @@ int b2fil_linear_loss_grad(int dtype, const void* hidden, int64_t hidden_stride,
                            void* grad_hidden, void* grad_weight, void* workspace,
                            int64_t workspace_bytes, int device_id, void* cuda_stream);
 
+/* The given class of each row, `stride` elements apart.  A row whose class is outside [0, n_cols) or equals
+ * `ignore` does not count.  index NULL: no class is given, all rows count. */
+typedef struct b2fil_target {
+  const void* index; /* (n_rows) int32 or int64 */
+  int64_t stride;
+  int64_t ignore;    /* class that does not count, e.g. -100 */
+  int32_t index64;   /* 1: int64 classes */
+} b2fil_target;
+
+/* Scores of rows of logits (fp32, bf16 or fp16) with q = softmax(logits / temperature): the given class's log q to log_prob
+ * (n_rows), NULL without a target; the entropy -sum q log q to entropy (n_rows); what the gradient needs to kept
+ * (n_rows, 4), 16-byte aligned.  With k > 0 the k largest logits' log q to top (n_rows, k), in the order of
+ * b2fil_top_scores, and their classes to top_index (n_rows, k); k <= min(n_cols, B2FIL_MOST_TOP).  Rows that do not
+ * count, or without a logit above -inf, have the scores 0, best classes of log q 0 and class -1. */
+int64_t b2fil_log_probs_workspace(int dtype, int64_t n_rows, int64_t n_cols, int k, int device_id);
+int b2fil_log_probs(int dtype, const void* logits, int64_t n_rows, int64_t n_cols, int64_t row_stride,
+                    const b2fil_target* target, double temperature, int k, float* log_prob, float* entropy, float* kept,
+                    float* top, int32_t* top_index, void* workspace, int64_t workspace_bytes, int device_id,
+                    void* cuda_stream);
+
+/* The gradient of those scores by the logits to grad (n_rows, n_cols), grad_stride elements between rows.
+ * of_log_prob, of_entropy: the gradients by the rows' scores, each a stride apart (0: one value); either may be NULL. */
+int b2fil_log_probs_grad(int dtype, const void* logits, int64_t n_rows, int64_t n_cols, int64_t row_stride,
+                         double temperature, const float* kept, const float* of_log_prob, int64_t of_log_prob_stride,
+                         const float* of_entropy, int64_t of_entropy_stride, void* grad, int64_t grad_stride,
+                         int device_id, void* cuda_stream);
+
+/* The same scores (k = 0) of logits = hidden * weight^T that are not kept; layer, types and limits as in
+ * b2fil_linear_loss, whose status word they share. */
+int64_t b2fil_linear_log_probs_workspace(int dtype, const void* hidden, int64_t hidden_stride, const void* weight,
+                                         int64_t weight_stride, int64_t n_rows, int64_t n_cols, int64_t width,
+                                         int device_id);
+int b2fil_linear_log_probs(int dtype, const void* hidden, int64_t hidden_stride, const void* weight,
+                           int64_t weight_stride, int64_t n_rows, int64_t n_cols, int64_t width,
+                           const b2fil_target* target, double temperature, float* log_prob, float* entropy, float* kept,
+                           void* workspace, int64_t workspace_bytes, int device_id, void* cuda_stream);
+
+/* Their gradients by hidden and weight, as in b2fil_linear_loss_grad. */
+int64_t b2fil_linear_log_probs_grad_workspace(int dtype, const void* hidden, int64_t hidden_stride, const void* weight,
+                                              int64_t weight_stride, int64_t n_rows, int64_t n_cols, int64_t width,
+                                              int wants_hidden, int wants_weight, int device_id);
+int b2fil_linear_log_probs_grad(int dtype, const void* hidden, int64_t hidden_stride, const void* weight,
+                                int64_t weight_stride, int64_t n_rows, int64_t n_cols, int64_t width,
+                                double temperature, const float* kept, const float* of_log_prob,
+                                int64_t of_log_prob_stride, const float* of_entropy, int64_t of_entropy_stride,
+                                void* grad_hidden, void* grad_weight, void* workspace, int64_t workspace_bytes,
+                                int device_id, void* cuda_stream);
+
+/* One of many gradients: `rows` rows of `cols` elements at `from`, strides in elements. */
+typedef struct b2fil_gradient {
+  const void* from;
+  void* to;          /* the scaled ones: `from` itself (same strides and type), memory of its own, or NULL */
+  int64_t rows, cols, from_row, from_col, to_row, to_col;
+  int32_t from_type, to_type; /* B2FIL_TYPE_F32, _BF16 or _F16 */
+  int32_t tensor;    /* entries of one number are parts of one tensor and known not to overlap */
+} b2fil_gradient;
+
+#define B2FIL_NORM_LARGEST 0 /* max |x| */
+#define B2FIL_NORM_SUM 1     /* sum |x| */
+#define B2FIL_NORM_SQUARES 2 /* (sum x^2)^1/2 */
+
+/* The norm of n gradients (an array in host memory) together to norm[0], and with scales = 1 each times
+ * min(1, most / norm), rounded once, to its `to`; times 1 where the norm is not finite.  What is written overlaps nothing
+ * else but its own `from`, which is then the same (checked, between the address ranges of different tensors, where rows of one
+ * stride may lie side by side).  Strides and most are 0 or more. */
+int64_t b2fil_clip_gradients_workspace(const b2fil_gradient* gradients, int64_t n, int device_id);
+int b2fil_clip_gradients(const b2fil_gradient* gradients, int64_t n, int norm_kind, int scales, double most, float* norm,
+                         void* workspace, int64_t workspace_bytes, int device_id, void* cuda_stream);
+
 /* Waits for all work on device_id, reads the status word of the linear loss's kernels there and returns
  * B2FIL_ERR_TIMEOUT when a bounded wait inside one ran out; the word is cleared by the read.  That call's outputs may be
  * incomplete, and from then until the word is read the linear losses on the device (of layers whose logits
