@@ -19,9 +19,13 @@
 // their first and last element stand for its own above and below.
 // Where rows are few, several blocks share one: up to eight as a cluster, whose first block joins the lists over
 // distributed shared memory; of longer rows a second kernel does.
+//
+// The same kernels give a row's scores (score_common.cuh) with its best classes, of which the log probabilities are then
+// written: kScored.  (A pass of its own for the scores: 4096 x 32,768 bf16, k 8, 138 us
+// instead of 83; 1 x 50,001 fp32, k 20, 23.5 instead of 10.3; 1,000,003 x 10 fp32, k 3, 467 instead of 33.)
 #include <cooperative_groups.h>
 
-#include "distill_common.cuh"
+#include "score_common.cuh"
 
 namespace b2fil {
 namespace distill {
@@ -138,6 +142,53 @@ __device__ __forceinline__ float log_of(float x) { return logf(x); }
 template <>
 __device__ __forceinline__ double log_of(double x) { return log(x); }
 
+enum { kScores = 0, kProbabilities = 1, kScored = 2 };  // what a kernel is given, and whether it scores
+
+// Best classes with a row's scores: values and logsumexp are not used.
+struct ScoredTopArgs : TopArgs {
+  Target target;
+  Temperature temperature;
+  Scores out;
+  float* top;
+};
+template <int MODE>
+using ArgsOf = std::conditional_t<MODE == kScored, ScoredTopArgs, TopArgs>;
+
+// Exponents' factor log2(e) / T, as the gradient takes it.
+template <class V, class A>
+__device__ __forceinline__ V factor_of(const A& a)
+{
+  if constexpr (std::is_same_v<A, ScoredTopArgs>)
+    return a.temperature.c;
+  else
+    return static_cast<V>(1.4426950408889634 * a.inv_temperature);
+}
+
+// Entry j of a scored row: m and log s, as in finish_score.
+template <class K>
+__device__ __forceinline__ void write_scored(const ScoredTopArgs& a, int64_t row, int j, const K& key, float m, const RowScore& score)
+{
+  const double x = (static_cast<double>(key.value()) - m) * a.temperature.inverse - score.log_s;
+  a.top[row * a.k + j]   = !score.counts ? 0.f : static_cast<float>(x > 0 ? 0 : x);
+  a.index[row * a.k + j] = score.counts ? static_cast<int32_t>(key.index()) : -1;
+}
+// A row that does not count, by `threads` threads.
+__device__ __forceinline__ void write_uncounted(const ScoredTopArgs& a, int64_t row, int tid, int threads)
+{
+  if (tid == 0) finish_score(a.out, row, Scored(), a.temperature.inverse, -2, 0.f);
+  for (int j = tid; j < a.k; j += threads) {
+    a.top[row * a.k + j]   = 0.f;
+    a.index[row * a.k + j] = -1;
+  }
+}
+// Scores of a row: written by one thread, known to all that call.
+template <class T>
+__device__ __forceinline__ RowScore score_row(const ScoredTopArgs& a, int64_t row, const T* x, const Scored& r, int at, bool writes)
+{
+  if (writes) return finish_score(a.out, row, r, a.temperature.inverse, at, at >= 0 ? widen(x[at]) : 0.f);
+  return {log_sum(r.s), at != -2 && !(r.s == 0.f)};
+}
+
 // Writes entry j of a row.
 template <class T, class K>
 __device__ __forceinline__ void write_top(const TopArgs& a, int64_t row, int j, const K& key)
@@ -182,6 +233,22 @@ struct Sum {
     }
   }
 };
+
+// The same with what scores need.
+struct ScoredSum : ScoredStream {
+  float slack;
+  __device__ __forceinline__ explicit ScoredSum(float c) : slack(kSlack / c) {}
+  __device__ __forceinline__ void reach(float most, float c, bool) { ScoredStream::reach(most, c, slack); }
+  __device__ __forceinline__ void add(float x, float c, bool) { Scored::add(x, base, c); }
+};
+template <class V, int MODE>
+__device__ __forceinline__ auto new_sum(V c)
+{
+  if constexpr (MODE == kScored)
+    return ScoredSum(c);
+  else
+    return Sum<V, MODE == kProbabilities>();
+}
 
 // The logarithm of s + dropped, which may be nearly 1: of its 32-bit part, and what that leaves.
 __device__ __forceinline__ float log_of_sum(float s, double dropped)
@@ -257,16 +324,19 @@ __device__ __forceinline__ uint32_t first_nan(const T* x, int64_t n, int tid, in
 
 // A segment of a row per block.  segs == 1: the row's answer; else its k best keys and its sum, which the first
 // block of a cluster of segs blocks joins, or top_join does.
-template <class T, bool PROB>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments(TopArgs a, int segs, int64_t seg_cols,
+template <class T, int MODE>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments(ArgsOf<MODE> a, int segs, int64_t seg_cols,
                                                                                  bool clustered,
                                                                                  typename KeyOf<T>::type* keys, double* sums)
 {
   using V = typename ValueOf<T>::type;
   using K = typename KeyOf<T>::type;
-  constexpr int N = Piece<T>::N;
+  constexpr int N     = Piece<T>::N;
+  constexpr bool PROB = MODE == kProbabilities;
   __shared__ K list[kList], best[kMostTop], shared_tau;
-  __shared__ double best_sum[2];
+  __shared__ double best_sum[3];
+  __shared__ float joined_m;
+  __shared__ RowScore joined_score;
   __shared__ int16_t groups[kThreads];
   __shared__ int found, chosen;
   __shared__ double room[64];
@@ -275,15 +345,23 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
   const int64_t begin = seg * seg_cols;
   const int64_t n     = min(seg_cols, a.n_cols - begin);
   const int k         = static_cast<int>(min(static_cast<int64_t>(a.k), n));
-  const V c           = static_cast<V>(1.4426950408889634 * a.inv_temperature);
+  const V c           = factor_of<V>(a);
   const bool plain    = PROB && a.inv_temperature == 1.0;
   for (int64_t row = blockIdx.x / segs; row < a.n_rows; row += gridDim.x / segs) {
     const T* x       = static_cast<const T*>(a.scores) + row * a.row_stride + begin;
     const int lead   = lead_of(x, n);
     const int pieces = static_cast<int>((n - lead) / N);
     const T* body    = x + lead;
+    int given        = -1;
+    if constexpr (MODE == kScored) {
+      given = target_of(a.target, row, a.n_cols);
+      if (given == -2) {  // (for all blocks of a cluster)
+        if (seg == 0) write_uncounted(a, row, tid, kThreads);
+        continue;
+      }
+    }
     // the thread's best score, the first element of the piece that holds it, and the sum
-    Sum<V, PROB> sum;
+    auto sum    = new_sum<V, MODE>(c);
     V top       = lowest<V>();
     uint32_t at = ~0u;  // none yet
     visit_row<kInFlight>(
@@ -322,7 +400,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
     double dropped = 0;
     Running<V> all;
     all.m = V(0);
-    if (plain) {
+    if constexpr (MODE == kScored) {
+      join_scored<kThreads>(sum, c, reinterpret_cast<float*>(room));
+    } else if (plain) {
       // (in 64 bits: see Sum)
       dropped = sum_row<kThreads>(static_cast<double>(sum.s) + sum.dropped, room);
     } else {
@@ -415,8 +495,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
     const int64_t part = row * segs + seg;
     if (segs == 1) {
       arrange(list, got, k, [&](int place, const K& key) {
-        write_top<T>(a, row, place, key);
-        if (place == 0) write_lse(a, row, all.m, all.s, dropped, key);
+        if constexpr (MODE == kScored) {
+          write_scored(a, row, place, key, sum.m, score_row(a, row, x, sum, given, place == 0));
+        } else {
+          write_top<T>(a, row, place, key);
+          if (place == 0) write_lse(a, row, all.m, all.s, dropped, key);
+        }
       });
       __syncthreads();
       continue;
@@ -425,9 +509,15 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
     arrange(list, got, k, [&](int place, const K& key) { to[place] = key; });
     for (int j = k + tid; j < a.k; j += kThreads) to[j] = K::none();
     if (tid == 0) {
-      double* sum_to = clustered ? best_sum : sums + 2 * part;
-      sum_to[0]      = plain ? dropped : static_cast<double>(all.s);
-      sum_to[1]      = all.m;
+      double* sum_to = clustered ? best_sum : sums + 3 * part;
+      if constexpr (MODE == kScored) {
+        sum_to[0] = sum.s;
+        sum_to[1] = sum.m;
+        sum_to[2] = sum.u;
+      } else {
+        sum_to[0] = plain ? dropped : static_cast<double>(all.s);
+        sum_to[1] = all.m;
+      }
     }
     if (clustered) {
       // With r = k / segs rounded up, at least k keys reach the least of the lists' r-th keys.
@@ -445,8 +535,28 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
           const K key = *cluster.map_shared_rank(best + i % a.k, i / a.k);
           if (!least.above(key)) list[atomicAdd(&found, 1)] = key;
         }
+        if constexpr (MODE == kScored) {
+          if (tid < 32) {
+            Scored r;
+            if (tid < segs) {
+              const double* from = cluster.map_shared_rank(best_sum, tid);
+              r.s = static_cast<float>(from[0]);
+              r.m = static_cast<float>(from[1]);
+              r.u = static_cast<float>(from[2]);
+            }
+            r.join_lanes(c);
+            if (tid == 0) {
+              joined_m     = r.m;
+              joined_score = score_row(a, row, x, r, given, true);  // (the first block's part begins with the row)
+            }
+          }
+        }
         __syncthreads();
         arrange(list, found, a.k, [&](int place, const K& key) {
+          if constexpr (MODE == kScored) {
+            write_scored(a, row, place, key, joined_m, joined_score);
+            return;
+          } else {
           write_top<T>(a, row, place, key);
           if (place > 0) return;
           Running<double> r;
@@ -458,6 +568,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
               r.join(from[1], from[0], 1.0);
           }
           write_lse(a, row, static_cast<V>(r.m), static_cast<V>(plain ? 0.0 : r.s), plain ? r.s : 0.0, key);
+          }
         });
       }
       cluster.sync();  // the others' lists have been read
@@ -468,8 +579,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
 
 // Joins the segments' sorted lists of a row.  With r = k / segs rounded up, at least k keys reach the least of the
 // lists' r-th keys: these alone are sorted, where they fit; else as many as fit with the best so far.
-template <class T>
-__global__ void __launch_bounds__(kThreads) top_join(TopArgs a, int segs, const typename KeyOf<T>::type* keys,
+template <class T, int MODE>
+__global__ void __launch_bounds__(kThreads) top_join(ArgsOf<MODE> a, int segs, const typename KeyOf<T>::type* keys,
                                                      const double* sums)
 {
   using V = typename ValueOf<T>::type;
@@ -479,6 +590,11 @@ __global__ void __launch_bounds__(kThreads) top_join(TopArgs a, int segs, const 
   __shared__ int found;
   const bool plain = a.probabilities && a.inv_temperature == 1.0;
   for (int64_t row = blockIdx.x; row < a.n_rows; row += gridDim.x) {
+    int given = -1;
+    if constexpr (MODE == kScored) {
+      given = target_of(a.target, row, a.n_cols);
+      if (given == -2) continue;  // (written already)
+    }
     const K* from = keys + row * segs * a.k;
     const int all = segs * a.k, r_th = (a.k + segs - 1) / segs - 1;
     if (threadIdx.x == 0) found = 0;
@@ -515,10 +631,23 @@ __global__ void __launch_bounds__(kThreads) top_join(TopArgs a, int segs, const 
         have = min(a.k, have + more);
       }
     }
+    if constexpr (MODE == kScored) {
+      const float c = factor_of<V>(a);
+      Scored r;
+      for (int i = threadIdx.x; i < segs; i += kThreads) {
+        const double* part = sums + 3 * (row * segs + i);
+        r.join(static_cast<float>(part[1]), static_cast<float>(part[0]), static_cast<float>(part[2]), c);
+      }
+      join_scored<kThreads>(r, c, reinterpret_cast<float*>(room));
+      const T* x           = static_cast<const T*>(a.scores) + row * a.row_stride;
+      const RowScore score = score_row(a, row, x, r, given, threadIdx.x == 0);
+      for (int j = threadIdx.x; j < a.k; j += kThreads) write_scored(a, row, j, list[j], r.m, score);
+      __syncthreads();
+    } else {
     for (int j = threadIdx.x; j < a.k; j += kThreads) write_top<T>(a, row, j, list[j]);
     Running<double> r;
     for (int i = threadIdx.x; i < segs; i += kThreads) {
-      const double s = sums[2 * (row * segs + i)], m = sums[2 * (row * segs + i) + 1];
+      const double s = sums[3 * (row * segs + i)], m = sums[3 * (row * segs + i) + 1];
       if (plain)
         r.s += s;
       else
@@ -530,6 +659,7 @@ __global__ void __launch_bounds__(kThreads) top_join(TopArgs a, int segs, const 
       join_row<kThreads>(r, 1.0, room);
     if (threadIdx.x == 0) write_lse(a, row, static_cast<V>(r.m), static_cast<V>(plain ? 0.0 : r.s), plain ? r.s : 0.0, list[0]);
     __syncthreads();
+    }
   }
 }
 
@@ -551,21 +681,30 @@ __host__ __device__ constexpr int warps_fit(size_t bytes) { return bytes <= 128 
 
 // A row per warp, in registers.  Short rows: every 32nd element is a lane's, S of them.  Longer ones: U pieces of
 // 16 bytes and at most one element from before the first or behind the last boundary per lane, and S is 0.
-template <class T, int U, int S, bool PROB>
-__global__ void __launch_bounds__(kThreads, warps_fit(U * 16 / sizeof(T) * sizeof(typename ValueOf<T>::type))) top_warps(TopArgs a)
+template <class T, int U, int S, int MODE>
+__global__ void __launch_bounds__(kThreads, warps_fit(U * 16 / sizeof(T) * sizeof(typename ValueOf<T>::type))) top_warps(ArgsOf<MODE> a)
 {
   using V = typename ValueOf<T>::type;
   using K = typename KeyOf<T>::type;
   using O = typename Ordered<V>::type;
   constexpr int N = Piece<T>::N, E = S ? S : U * N + 1, ROWS = kThreads / 32, kBits = sizeof(O) * 8;
+  constexpr bool PROB = MODE == kProbabilities;
   __shared__ K lists[ROWS][kWarpList];
   const int lane = threadIdx.x % 32, n = static_cast<int>(a.n_cols), k = a.k;
   K* list          = lists[threadIdx.x / 32];
-  const V c        = static_cast<V>(1.4426950408889634 * a.inv_temperature);
+  const V c        = factor_of<V>(a);
   const bool plain = PROB && a.inv_temperature == 1.0;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / 32; row < a.n_rows;
        row += static_cast<int64_t>(gridDim.x) * ROWS) {
     const T* x       = static_cast<const T*>(a.scores) + row * a.row_stride;
+    int given        = -1;
+    if constexpr (MODE == kScored) {
+      given = target_of(a.target, row, a.n_cols);
+      if (given == -2) {
+        write_uncounted(a, row, lane, 32);
+        continue;
+      }
+    }
     const int lead   = S ? 0 : lead_of(x, n), pieces = S ? 0 : (n - lead) / N;
     // the odd element: the first lanes' before, the last lanes' behind the pieces
     const int behind = lead + pieces * N + 31 - lane;
@@ -594,14 +733,17 @@ __global__ void __launch_bounds__(kThreads, warps_fit(U * 16 / sizeof(T) * sizeo
 #pragma unroll
     for (int d = 16; d; d >>= 1) top = larger(top, __shfl_xor_sync(~0u, top, d));
     // the sum (what is not there is -inf and adds nothing to a sum of powers)
-    Sum<V, PROB> sum;
+    auto sum = new_sum<V, MODE>(c);
     sum.reach(top, c, plain);
 #pragma unroll
     for (int e = 0; e < E; ++e)
       if (!PROB || is_there(e)) sum.add(v[e], c, plain);
     V s            = sum.s;
     double dropped = 0;
-    if (plain) {
+    if constexpr (MODE == kScored) {
+      s = sum.s = sum_lanes(sum.s);
+      sum.u     = sum_lanes(sum.u);
+    } else if (plain) {
       dropped = sum_lanes(static_cast<double>(sum.s) + sum.dropped);
       s       = V(0);
     } else {
@@ -713,8 +855,12 @@ __global__ void __launch_bounds__(kThreads, warps_fit(U * 16 / sizeof(T) * sizeo
 #pragma unroll 4
       for (int j = 0; j < got; ++j) place += list[j].above(key);
       if (place >= k) continue;
-      write_top<T>(a, row, place, key);
-      if (place == 0) write_lse(a, row, sum.r, s, dropped, key);
+      if constexpr (MODE == kScored) {
+        write_scored(a, row, place, key, sum.m, score_row(a, row, x, sum, given, place == 0));
+      } else {
+        write_top<T>(a, row, place, key);
+        if (place == 0) write_lse(a, row, sum.r, s, dropped, key);
+      }
     }
     __syncwarp();
   }
@@ -724,26 +870,35 @@ __global__ void __launch_bounds__(kThreads, warps_fit(U * 16 / sizeof(T) * sizeo
 // bound, as above, and what reaches it is read again; where that is more than the list holds the k-th key is found
 // bit by bit as in top_segments.  (A bound by values alone took 5.7 ms where all but five of 4096 scores of 8192 rows
 // were -inf.)
-template <class T, bool PROB>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(TopArgs a)
+template <class T, int MODE>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(ArgsOf<MODE> a)
 {
   using V = typename ValueOf<T>::type;
   using K = typename KeyOf<T>::type;
   constexpr int N = Piece<T>::N, ROWS = kThreads / 32;
+  constexpr bool PROB = MODE == kProbabilities;
   __shared__ K lists[ROWS][kWarpList];
   __shared__ int counts[ROWS];
   const int lane = threadIdx.x % 32, k = a.k;
   K* list          = lists[threadIdx.x / 32];
   int* found       = &counts[threadIdx.x / 32];
-  const V c        = static_cast<V>(1.4426950408889634 * a.inv_temperature);
+  const V c        = factor_of<V>(a);
   const bool plain = PROB && a.inv_temperature == 1.0;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / 32; row < a.n_rows;
        row += static_cast<int64_t>(gridDim.x) * ROWS) {
     const T* x = static_cast<const T*>(a.scores) + row * a.row_stride;
+    int given  = -1;
+    if constexpr (MODE == kScored) {
+      given = target_of(a.target, row, a.n_cols);
+      if (given == -2) {
+        write_uncounted(a, row, lane, 32);
+        continue;
+      }
+    }
     // the lane's best score, the first element of the piece that holds it, and the sum
     V best      = lowest<V>();
     uint32_t at = ~0u;
-    Sum<V, PROB> sum;
+    auto sum    = new_sum<V, MODE>(c);
     visit_row<2 * kInFlight>(
       x, a.n_cols, lane, 32,
       [&](int64_t i, T e) {
@@ -769,7 +924,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(Top
     double dropped = 0;
     Running<V> all;
     all.m = V(0);
-    if (plain) {
+    Scored scored;  // (the lane's own sum is asked for NaN below)
+    if constexpr (MODE == kScored) {
+      scored = sum;
+      scored.join_lanes(c);
+    } else if (plain) {
       dropped = sum_lanes(static_cast<double>(sum.s) + sum.dropped);
     } else {
       all.m = sum.first ? lowest<V>() : sum.r;
@@ -833,17 +992,22 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(Top
 #pragma unroll 4
       for (int j = 0; j < got; ++j) place += list[j].above(key);
       if (place >= k) continue;
-      write_top<T>(a, row, place, key);
-      if (place == 0) write_lse(a, row, all.m, all.s, dropped, key);
+      if constexpr (MODE == kScored) {
+        write_scored(a, row, place, key, scored.m, score_row(a, row, x, scored, given, place == 0));
+      } else {
+        write_top<T>(a, row, place, key);
+        if (place == 0) write_lse(a, row, all.m, all.s, dropped, key);
+      }
     }
     __syncwarp();
   }
 }
 
 // A row per thread: n_cols x sizeof(T) <= kTileBytes, k <= TOP.
-template <class T, int TOP, bool PROB>
-__global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
+template <class T, int TOP, int MODE>
+__global__ void __launch_bounds__(kTileRows) top_tiles(ArgsOf<MODE> a)
 {
+  constexpr bool PROB = MODE == kProbabilities;
   using V = typename ValueOf<T>::type;
   using K = typename KeyOf<T>::type;
   using O = typename Ordered<V>::type;
@@ -851,7 +1015,7 @@ __global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
   T* tile       = reinterpret_cast<T*>(smem);
   const int c_n = static_cast<int>(a.n_cols);
   const TileShape<T> shape(c_n);
-  const V c        = static_cast<V>(1.4426950408889634 * a.inv_temperature);
+  const V c        = factor_of<V>(a);
   const bool plain = PROB && a.inv_temperature == 1.0;
   const bool whole = without_gaps<T>(a.scores, a.row_stride, c_n);
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * kTileRows; first < a.n_rows;
@@ -909,7 +1073,7 @@ __global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
 #pragma unroll
       for (int j = 0; j < TOP; ++j) top[j] = from_ordered(key[j]);
     }
-    Sum<V, PROB> sum;
+    auto sum = new_sum<V, MODE>(c);
     if (plain) {
       for (int i = 0; i < c_n; ++i) sum.add(widen(x[i]), c, true);
     } else {
@@ -917,6 +1081,13 @@ __global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
       for (int i = 0; i < c_n; ++i) sum.add(widen(x[i]), c, false);
     }
     const int64_t row = first + threadIdx.x;
+    if constexpr (MODE == kScored) {
+      const int given      = target_of(a.target, row, a.n_cols);
+      const RowScore score = score_row(a, row, x, sum, given, true);
+#pragma unroll
+      for (int j = 0; j < TOP; ++j)
+        if (j < a.k) write_scored(a, row, j, K::of(top[j], static_cast<uint32_t>(at[j])), sum.m, score);
+    } else {
     T* values         = static_cast<T*>(a.values) + row * a.k;
     int32_t* index    = a.index + row * a.k;
 #pragma unroll
@@ -926,6 +1097,7 @@ __global__ void __launch_bounds__(kTileRows) top_tiles(TopArgs a)
       index[j]  = at[j];
     }
     write_lse(a, row, sum.r, sum.s, static_cast<double>(sum.dropped), K::of(top[0], 0u));
+    }
   }
 }
 
@@ -943,12 +1115,24 @@ int64_t part_cols(int64_t n_cols, int segs)
   return segs == 1 ? n_cols : ((n_cols + segs - 1) / segs + 63) / 64 * 64;
 }
 
-template <class T, int TOP>
-cudaError_t run_tiles(const TopArgs& a, int n_sms, cudaStream_t s)
+// `a`'s kernel of the three modes.
+template <class A, class K>
+auto kernel_of(const A& a, K scores, K probabilities)
+{
+  return a.probabilities ? probabilities : scores;
+}
+
+template <class T, int TOP, class A>
+cudaError_t run_tiles(const A& a, int n_sms, cudaStream_t s)
 {
   const size_t bytes   = TileShape<T>(static_cast<int>(a.n_cols)).bytes();
   const int64_t blocks = (a.n_rows + kTileRows - 1) / kTileRows, most = 16ll * n_sms;
-  const auto kernel    = a.probabilities ? top_tiles<T, TOP, true> : top_tiles<T, TOP, false>;
+  const auto kernel    = [&] {
+    if constexpr (std::is_same_v<A, ScoredTopArgs>)
+      return top_tiles<T, TOP, kScored>;
+    else
+      return kernel_of(a, top_tiles<T, TOP, kScores>, top_tiles<T, TOP, kProbabilities>);
+  }();
   if (bytes > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
     if (e != cudaSuccess) return e;
@@ -958,19 +1142,25 @@ cudaError_t run_tiles(const TopArgs& a, int n_sms, cudaStream_t s)
   return cudaGetLastError();
 }
 
-template <class T, int U, int S>
-cudaError_t run_warps(const TopArgs& a, int n_sms, cudaStream_t s)
+template <class T, int U, int S, class A>
+cudaError_t run_warps(const A& a, int n_sms, cudaStream_t s)
 {
   const int64_t need = (a.n_rows + kThreads / 32 - 1) / (kThreads / 32), most = 16ll * n_sms;
-  const auto kernel  = a.probabilities ? top_warps<T, U, S, true> : top_warps<T, U, S, false>;
+  const auto kernel  = [&] {
+    if constexpr (std::is_same_v<A, ScoredTopArgs>)
+      return top_warps<T, U, S, kScored>;
+    else
+      return kernel_of(a, top_warps<T, U, S, kScores>, top_warps<T, U, S, kProbabilities>);
+  }();
   kernel<<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(a);
   count_launches(1);
   return cudaGetLastError();
 }
 
-template <class T>
-cudaError_t run_top(const TopArgs& a, void* workspace, int n_sms, cudaStream_t s)
+template <class T, class A>
+cudaError_t run_top(const A& a, void* workspace, int n_sms, cudaStream_t s)
 {
+  constexpr bool kIsScored = std::is_same_v<A, ScoredTopArgs>;
   using K = typename KeyOf<T>::type;
   const int64_t bytes = a.n_cols * static_cast<int64_t>(sizeof(T));
   if (a.n_cols <= kTileTop && a.k > 8 && a.n_rows >= kTileLeast * n_sms)
@@ -996,7 +1186,12 @@ cudaError_t run_top(const TopArgs& a, void* workspace, int n_sms, cudaStream_t s
   }
   if (bytes <= kLongBytes && a.k <= kWarpTop && a.n_rows >= static_cast<int64_t>(kLongLeast) * n_sms) {
     const int64_t need = (a.n_rows + kThreads / 32 - 1) / (kThreads / 32), most = 16ll * n_sms;
-    const auto kernel  = a.probabilities ? top_long<T, true> : top_long<T, false>;
+    const auto kernel  = [&] {
+      if constexpr (kIsScored)
+        return top_long<T, kScored>;
+      else
+        return kernel_of(a, top_long<T, kScores>, top_long<T, kProbabilities>);
+    }();
     kernel<<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(a);
     count_launches(1);
     return cudaGetLastError();
@@ -1012,7 +1207,7 @@ cudaError_t run_top(const TopArgs& a, void* workspace, int n_sms, cudaStream_t s
   int64_t cols = part_cols(a.n_cols, segs);
   if (!clustered) segs = static_cast<int>((a.n_cols + cols - 1) / cols);
   double* sums       = static_cast<double*>(workspace);
-  K* keys            = reinterpret_cast<K*>(sums + (segs > 1 ? 2 * a.n_rows * segs : 0));
+  K* keys            = reinterpret_cast<K*>(sums + (segs > 1 ? 3 * a.n_rows * segs : 0));
   const int64_t most = 16ll * n_sms;
   const unsigned rows = static_cast<unsigned>(a.n_rows < most ? a.n_rows : most);
   cudaLaunchConfig_t config{};
@@ -1025,11 +1220,16 @@ cudaError_t run_top(const TopArgs& a, void* workspace, int n_sms, cudaStream_t s
   attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
   config.attrs    = &attribute;
   config.numAttrs = clustered ? 1 : 0;
-  const auto kernel   = a.probabilities ? top_segments<T, true> : top_segments<T, false>;
+  const auto kernel   = [&] {
+    if constexpr (kIsScored)
+      return top_segments<T, kScored>;
+    else
+      return kernel_of(a, top_segments<T, kScores>, top_segments<T, kProbabilities>);
+  }();
   const cudaError_t e = cudaLaunchKernelEx(&config, kernel, a, segs, cols, clustered, keys, sums);
   if (e != cudaSuccess) return e;
   const bool join = segs > 1 && !clustered;
-  if (join) top_join<T><<<rows, kThreads, 0, s>>>(a, segs, keys, sums);
+  if (join) top_join<T, kIsScored ? kScored : kScores><<<rows, kThreads, 0, s>>>(a, segs, keys, sums);
   count_launches(join ? 2 : 1);
   return cudaGetLastError();
 }
@@ -1040,7 +1240,7 @@ size_t top_workspace(int dtype, const TopArgs& a, int n_sms)
 {
   const int64_t segs = segments(a.n_rows, a.n_cols, n_sms);
   if (segs <= 1 || a.n_cols <= kJoinCols) return 0;
-  return a.n_rows * segs * (a.k * (dtype == kF64 ? sizeof(Key64) : sizeof(Key32)) + 2 * sizeof(double));
+  return a.n_rows * segs * (a.k * (dtype == kF64 ? sizeof(Key64) : sizeof(Key32)) + 3 * sizeof(double));
 }
 
 cudaError_t launch_top(int dtype, const TopArgs& a, void* workspace, int n_sms, cudaStream_t s)
@@ -1048,6 +1248,27 @@ cudaError_t launch_top(int dtype, const TopArgs& a, void* workspace, int n_sms, 
   switch (dtype) {
     case kF32: return run_top<float>(a, workspace, n_sms, s);
     case kF64: return run_top<double>(a, workspace, n_sms, s);
+    case kBF16: return run_top<__nv_bfloat16>(a, workspace, n_sms, s);
+    case kF16: return run_top<__half>(a, workspace, n_sms, s);
+  }
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_scored_top(int dtype, const ScoreArgs& g, void* workspace, int n_sms, cudaStream_t s)
+{
+  ScoredTopArgs a{};
+  a.scores      = g.logits;
+  a.n_rows      = g.n_rows;
+  a.n_cols      = g.n_cols;
+  a.row_stride  = g.row_stride;
+  a.k           = g.k;
+  a.index       = g.top_index;
+  a.target      = g.target;
+  a.temperature = g.temperature;
+  a.out         = g.out;
+  a.top         = g.top;
+  switch (dtype) {
+    case kF32: return run_top<float>(a, workspace, n_sms, s);
     case kBF16: return run_top<__nv_bfloat16>(a, workspace, n_sms, s);
     case kF16: return run_top<__half>(a, workspace, n_sms, s);
   }

@@ -14,6 +14,10 @@ constexpr int kWarpCols = 2048;  // rows that belong to one warp
 constexpr int kSegment  = 8192;  // fewest elements of a row that are worth a block of their own
 constexpr int kMostSegs = 64;
 constexpr int kInFlight = 4;     // pieces of a thread
+// Rows for one thread each: classes, and rows per SM from which on.
+constexpr int kTileCols   = 64;
+constexpr int kTileLeast  = 32;
+constexpr int kTileBlocks = 8;   // of an SM
 
 // n elements of a row by `threads` threads.
 template <class T>
@@ -80,20 +84,61 @@ __global__ void __launch_bounds__(kThreads) score_rows(ScoreArgs a, int segs, co
   }
 }
 
-// Log probabilities of the best classes from their logits (of the logits' type, in `values`).
+// A row per thread, from a tile in shared memory.
 template <class T>
-__global__ void __launch_bounds__(kThreads) score_top(ScoreArgs a, const T* values)
+__global__ void __launch_bounds__(kTileRows, kTileBlocks) score_tiles(ScoreArgs a)
 {
-  const int64_t all = a.n_rows * a.k;
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < all; i += gridDim.x * static_cast<int64_t>(kThreads)) {
-    const float4 kept = a.out.kept[i / a.k];
-    if (kept.y == 0.f) {
-      a.top[i]       = 0.f;
-      a.top_index[i] = -1;
-    } else {
-      const double x = (static_cast<double>(widen(values[i])) - kept.x) * a.temperature.inverse + log_sum(kept.y);
-      a.top[i]       = static_cast<float>(x > 0 ? 0 : x);
+  extern __shared__ __align__(16) char smem[];
+  T* tile        = reinterpret_cast<T*>(smem);
+  const int cols = static_cast<int>(a.n_cols);
+  const TileShape<T> shape(cols);
+  const float c    = a.temperature.c;
+  const bool whole = without_gaps<T>(a.logits, a.row_stride, cols);
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kTileRows; first < a.n_rows;
+       first += static_cast<int64_t>(gridDim.x) * kTileRows) {
+    const int rows = static_cast<int>(min(static_cast<int64_t>(kTileRows), a.n_rows - first));
+    __syncthreads();  // the last tile has been used
+    load_tile(tile, shape, static_cast<const T*>(a.logits) + first * a.row_stride, a.row_stride, rows, whole);
+    __syncthreads();
+    if (threadIdx.x >= rows) continue;
+    const T* x        = tile + threadIdx.x * shape.pitch;
+    const int64_t row = first + threadIdx.x;
+    const int at      = target_of(a.target, row, cols);
+    Scored r;
+    for (int i = 0; i < cols; ++i) r.m = fmaxf(r.m, widen(x[i]));
+    const float base = base_of(r.m);
+    for (int i = 0; i < cols; ++i) r.add(widen(x[i]), base, c);
+    finish_score(a.out, row, r, a.temperature.inverse, at, at >= 0 ? widen(x[at]) : 0.f);
+  }
+}
+
+// Its gradient.
+template <class T>
+__global__ void __launch_bounds__(kTileRows, kTileBlocks) grad_tiles(ScoreGradArgs g)
+{
+  extern __shared__ __align__(16) char smem[];
+  T* tile            = reinterpret_cast<T*>(smem);
+  const ScoreArgs& a = g.fwd;
+  const int cols     = static_cast<int>(a.n_cols);
+  const TileShape<T> shape(cols);
+  const float c       = a.temperature.c, inv_t = static_cast<float>(a.temperature.inverse);
+  const bool whole_in = without_gaps<T>(a.logits, a.row_stride, cols), whole_out = without_gaps<T>(g.grad, g.grad_stride, cols);
+  const ScoreUpstream& up = g.upstream;
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kTileRows; first < a.n_rows;
+       first += static_cast<int64_t>(gridDim.x) * kTileRows) {
+    const int rows = static_cast<int>(min(static_cast<int64_t>(kTileRows), a.n_rows - first));
+    __syncthreads();  // the last tile has been stored
+    load_tile(tile, shape, static_cast<const T*>(a.logits) + first * a.row_stride, a.row_stride, rows, whole_in);
+    __syncthreads();
+    if (threadIdx.x < rows) {
+      T* x              = tile + threadIdx.x * shape.pitch;
+      const int64_t row = first + threadIdx.x;
+      const RowGrad r   = row_grad(a.out.kept[row], up.log_prob ? up.log_prob[row * up.log_prob_stride] * inv_t : 0.f,
+                                   up.entropy ? up.entropy[row * up.entropy_stride] * inv_t : 0.f);
+      for (int i = 0; i < cols; ++i) x[i] = narrow<T>(r.counts ? r(widen(x[i]), c) + (i == r.at ? r.add : 0.f) : 0.f);
     }
+    __syncthreads();
+    store_tile(static_cast<T*>(g.grad) + first * g.grad_stride, g.grad_stride, tile, shape, rows, whole_out);
   }
 }
 
@@ -166,22 +211,27 @@ int64_t part_cols(int64_t n_cols, int segs)
 {
   return segs == 1 ? n_cols : ((n_cols + segs - 1) / segs + 63) / 64 * 64;
 }
-size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
-size_t bytes_of(int dtype) { return dtype == kF32 ? 4 : 2; }
 unsigned blocks_of(int64_t need, int64_t most) { return static_cast<unsigned>(need < most ? need : most); }
 
-template <class T>
-cudaError_t run_score(int dtype, const ScoreArgs& a, void* workspace, int n_sms, cudaStream_t s)
+bool by_tiles(const ScoreArgs& a, int n_sms) { return a.n_cols <= kTileCols && a.n_rows >= static_cast<int64_t>(kTileLeast) * n_sms; }
+template <class T, class A>
+cudaError_t run_tiles(void (*kernel)(A), const A& args, const ScoreArgs& a, int n_sms, cudaStream_t s)
 {
+  const unsigned blocks = blocks_of((a.n_rows + kTileRows - 1) / kTileRows, static_cast<int64_t>(kTileBlocks) * n_sms);
+  kernel<<<blocks, kTileRows, TileShape<T>(static_cast<int>(a.n_cols)).bytes(), s>>>(args);
+  count_launches(1);
+  return cudaGetLastError();
+}
+
+template <class T>
+cudaError_t run_score(const ScoreArgs& a, void* workspace, int n_sms, cudaStream_t s)
+{
+  if (by_tiles(a, n_sms)) return run_tiles<T>(score_tiles<T>, a, a, n_sms, s);
   int segs           = segments(a.n_rows, a.n_cols, n_sms);
   const int64_t cols = part_cols(a.n_cols, segs);
   segs               = segs == 1 ? 1 : static_cast<int>((a.n_cols + cols - 1) / cols);
-  char* at           = static_cast<char*>(workspace);
-  float4* parts      = reinterpret_cast<float4*>(at);
-  if (segs > 1) {
-    score_parts<T><<<dim3(segs, blocks_of(a.n_rows, 65535)), kThreads, 0, s>>>(a, cols, parts);
-    at += padded(a.n_rows * segs * sizeof(float4));
-  }
+  float4* parts      = static_cast<float4*>(workspace);
+  if (segs > 1) score_parts<T><<<dim3(segs, blocks_of(a.n_rows, 65535)), kThreads, 0, s>>>(a, cols, parts);
   const bool warp    = segs > 1 || a.n_cols <= kWarpCols;
   const int per      = warp ? kThreads / 32 : 1;
   const unsigned blocks = blocks_of((a.n_rows + per - 1) / per, 8ll * n_sms);
@@ -190,13 +240,6 @@ cudaError_t run_score(int dtype, const ScoreArgs& a, void* workspace, int n_sms,
   else
     score_rows<T, kThreads><<<blocks, kThreads, 0, s>>>(a, 0, parts);
   count_launches(segs > 1 ? 2 : 1);
-  cudaError_t e = cudaGetLastError();
-  if (a.k == 0 || e != cudaSuccess) return e;
-  const TopArgs t{a.logits, a.n_rows, a.n_cols, a.row_stride, a.k, false, a.temperature.inverse, at, a.top_index, nullptr};
-  at += padded(static_cast<size_t>(a.n_rows) * a.k * sizeof(T));
-  if ((e = launch_top(dtype, t, at, n_sms, s)) != cudaSuccess) return e;
-  score_top<T><<<blocks_of((a.n_rows * a.k + kThreads - 1) / kThreads, 8ll * n_sms), kThreads, 0, s>>>(a, static_cast<const T*>(t.values));
-  count_launches(1);
   return cudaGetLastError();
 }
 
@@ -204,6 +247,7 @@ template <class T>
 cudaError_t run_grad(const ScoreGradArgs& g, int n_sms, cudaStream_t s)
 {
   const ScoreArgs& a = g.fwd;
+  if (by_tiles(a, n_sms)) return run_tiles<T>(grad_tiles<T>, g, a, n_sms, s);
   const bool warp    = a.n_cols <= kWarpCols;
   const int per      = warp ? kThreads / 32 : 1;
   int segs           = warp ? 1 : segments(a.n_rows, a.n_cols, n_sms);
@@ -222,24 +266,24 @@ cudaError_t run_grad(const ScoreGradArgs& g, int n_sms, cudaStream_t s)
 
 size_t score_workspace(int dtype, const ScoreArgs& a, int n_sms)
 {
-  const int segs = segments(a.n_rows, a.n_cols, n_sms);
-  size_t bytes   = segs > 1 ? padded(a.n_rows * segs * sizeof(float4)) : 0;
   if (a.k > 0) {
     TopArgs t{};
     t.n_rows = a.n_rows;
     t.n_cols = a.n_cols;
     t.k      = a.k;
-    bytes += padded(static_cast<size_t>(a.n_rows) * a.k * bytes_of(dtype)) + top_workspace(dtype, t, n_sms);
+    return top_workspace(dtype, t, n_sms);
   }
-  return bytes;
+  const int segs = segments(a.n_rows, a.n_cols, n_sms);
+  return segs > 1 ? a.n_rows * segs * sizeof(float4) : 0;
 }
 
 cudaError_t launch_score(int dtype, const ScoreArgs& a, void* workspace, int n_sms, cudaStream_t s)
 {
+  if (a.k > 0) return launch_scored_top(dtype, a, workspace, n_sms, s);
   switch (dtype) {
-    case kF32: return run_score<float>(dtype, a, workspace, n_sms, s);
-    case kBF16: return run_score<__nv_bfloat16>(dtype, a, workspace, n_sms, s);
-    case kF16: return run_score<__half>(dtype, a, workspace, n_sms, s);
+    case kF32: return run_score<float>(a, workspace, n_sms, s);
+    case kBF16: return run_score<__nv_bfloat16>(a, workspace, n_sms, s);
+    case kF16: return run_score<__half>(a, workspace, n_sms, s);
   }
   return cudaErrorInvalidValue;
 }
