@@ -235,6 +235,7 @@ struct Sum {
 };
 
 // The same with what scores need.
+// (of rows in registers, whose maximum is known)
 struct ScoredSum : ScoredStream {
   float slack;
   __device__ __forceinline__ explicit ScoredSum(float c) : slack(kSlack / c) {}
@@ -248,6 +249,46 @@ __device__ __forceinline__ auto new_sum(V c)
     return ScoredSum(c);
   else
     return Sum<V, MODE == kProbabilities>();
+}
+// ... and of a row that is read once.
+template <class T, int MODE>
+struct StreamOf {
+  using type = Sum<typename ValueOf<T>::type, MODE == kProbabilities>;
+};
+template <class T>
+struct StreamOf<T, kScored> {
+  using type = PairedStream<T>;
+};
+template <class V, bool PROB>
+__device__ __forceinline__ bool is_nan(const Sum<V, PROB>& sum) { return sum.s != sum.s; }
+template <class T>
+__device__ __forceinline__ bool is_nan(const PairedStream<T>& sum)
+{
+  float lo, hi;
+  split_pair(sum.s, lo, hi);
+  return lo != lo || hi != hi;
+}
+// A row again whose logits are not ordinary ones; joined.
+template <class T, int THREADS>
+__device__ __noinline__ Scored score_any(const T* x, int64_t n, int tid, float c, float* room)
+{
+  constexpr int N = Piece<T>::N;
+  ScoredStream r;
+  const float slack = kSlack / c;
+  visit_row<kInFlight>(
+    x, n, tid, THREADS,
+    [&](int64_t, T e) {
+      const float one[1] = {widen(e)};
+      r.take(one, c, slack);
+    },
+    [&](int64_t, const Piece<T>& p) {
+      float v[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = widen(p.v[e]);
+      r.take(v, c, slack);
+    });
+  join_scored<THREADS>(r, c, room);
+  return r;
 }
 
 // The logarithm of s + dropped, which may be nearly 1: of its 32-bit part, and what that leaves.
@@ -361,7 +402,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
       }
     }
     // the thread's best score, the first element of the piece that holds it, and the sum
-    auto sum    = new_sum<V, MODE>(c);
+    typename StreamOf<T, MODE>::type sum;
+    const V slack = static_cast<V>(kSlack) / c;
     V top       = lowest<V>();
     uint32_t at = ~0u;  // none yet
     visit_row<kInFlight>(
@@ -370,10 +412,21 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
         const V v = widen(e);
         if (v > top || at == ~0u) at = static_cast<uint32_t>(i);
         top = larger(top, v);
-        sum.reach(v, c, plain);
-        sum.add(v, c, plain);
+        if constexpr (MODE == kScored) {
+          sum.take(v, c, slack);
+        } else {
+          sum.reach(v, c, plain);
+          sum.add(v, c, plain);
+        }
       },
       [&](int64_t i, const Piece<T>& p) {
+        if constexpr (MODE == kScored) {
+          const V most = largest_of(p);
+          if (most > top || at == ~0u) at = static_cast<uint32_t>(i);
+          top = larger(top, most);
+          sum.take(p, most, c, slack);
+          return;
+        }
         V v[N], most;
 #pragma unroll
         for (int e = 0; e < N; ++e) v[e] = widen(p.v[e]);
@@ -382,11 +435,13 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
         for (int e = 1; e < N; ++e) most = larger(most, v[e]);
         if (most > top || at == ~0u) at = static_cast<uint32_t>(i);
         top = larger(top, most);
-        sum.reach(most, c, plain);
+        if constexpr (MODE != kScored) {
+          sum.reach(most, c, plain);
 #pragma unroll
-        for (int e = 0; e < N; ++e) sum.add(v[e], c, plain);
+          for (int e = 0; e < N; ++e) sum.add(v[e], c, plain);
+        }
       });
-    if (sum.s != sum.s) {  // a NaN, or infinities: the first NaN of the group is its best
+    if (is_nan(sum)) {  // a NaN, or infinities: the first NaN of the group is its best
       const uint32_t first = first_nan(x, n, tid, kThreads);
       if (first != ~0u) {
         top = static_cast<V>(NAN);
@@ -400,8 +455,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
     double dropped = 0;
     Running<V> all;
     all.m = V(0);
+    Scored scored;
     if constexpr (MODE == kScored) {
-      join_scored<kThreads>(sum, c, reinterpret_cast<float*>(room));
+      scored = sum.scored(c);
+      join_scored<kThreads>(scored, c, reinterpret_cast<float*>(room));
+      if (!sum.usable(scored.m, c)) scored = score_any<T, kThreads>(x, n, tid, c, reinterpret_cast<float*>(room));
     } else if (plain) {
       // (in 64 bits: see Sum)
       dropped = sum_row<kThreads>(static_cast<double>(sum.s) + sum.dropped, room);
@@ -496,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
     if (segs == 1) {
       arrange(list, got, k, [&](int place, const K& key) {
         if constexpr (MODE == kScored) {
-          write_scored(a, row, place, key, sum.m, score_row(a, row, x, sum, given, place == 0));
+          write_scored(a, row, place, key, scored.m, score_row(a, row, x, scored, given, place == 0));
         } else {
           write_top<T>(a, row, place, key);
           if (place == 0) write_lse(a, row, all.m, all.s, dropped, key);
@@ -511,9 +569,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
     if (tid == 0) {
       double* sum_to = clustered ? best_sum : sums + 3 * part;
       if constexpr (MODE == kScored) {
-        sum_to[0] = sum.s;
-        sum_to[1] = sum.m;
-        sum_to[2] = sum.u;
+        sum_to[0] = scored.s;
+        sum_to[1] = scored.m;
+        sum_to[2] = scored.u;
       } else {
         sum_to[0] = plain ? dropped : static_cast<double>(all.s);
         sum_to[1] = all.m;
@@ -898,17 +956,29 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(Arg
     // the lane's best score, the first element of the piece that holds it, and the sum
     V best      = lowest<V>();
     uint32_t at = ~0u;
-    auto sum    = new_sum<V, MODE>(c);
+    typename StreamOf<T, MODE>::type sum;
+    const V slack = static_cast<V>(kSlack) / c;
     visit_row<2 * kInFlight>(
       x, a.n_cols, lane, 32,
       [&](int64_t i, T e) {
         const V v = widen(e);
         if (v > best || at == ~0u) at = static_cast<uint32_t>(i);
         best      = larger(best, v);
-        sum.reach(v, c, plain);
-        sum.add(v, c, plain);
+        if constexpr (MODE == kScored) {
+          sum.take(v, c, slack);
+        } else {
+          sum.reach(v, c, plain);
+          sum.add(v, c, plain);
+        }
       },
       [&](int64_t i, const Piece<T>& p) {
+        if constexpr (MODE == kScored) {
+          const V most = largest_of(p);
+          if (most > best || at == ~0u) at = static_cast<uint32_t>(i);
+          best = larger(best, most);
+          sum.take(p, most, c, slack);
+          return;
+        }
         V v[N], most;
 #pragma unroll
         for (int e = 0; e < N; ++e) v[e] = widen(p.v[e]);
@@ -917,17 +987,20 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(Arg
         for (int e = 1; e < N; ++e) most = larger(most, v[e]);
         if (most > best || at == ~0u) at = static_cast<uint32_t>(i);
         best = larger(best, most);
-        sum.reach(most, c, plain);
+        if constexpr (MODE != kScored) {
+          sum.reach(most, c, plain);
 #pragma unroll
-        for (int e = 0; e < N; ++e) sum.add(v[e], c, plain);
+          for (int e = 0; e < N; ++e) sum.add(v[e], c, plain);
+        }
       });
     double dropped = 0;
     Running<V> all;
     all.m = V(0);
-    Scored scored;  // (the lane's own sum is asked for NaN below)
+    Scored scored;
     if constexpr (MODE == kScored) {
-      scored = sum;
+      scored = sum.scored(c);
       scored.join_lanes(c);
+      if (!sum.usable(scored.m, c)) scored = score_any<T, 32>(x, a.n_cols, lane, c, nullptr);
     } else if (plain) {
       dropped = sum_lanes(static_cast<double>(sum.s) + sum.dropped);
     } else {
@@ -935,7 +1008,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(Arg
       all.s = sum.s;
       all.join_lanes(V(1));
     }
-    if (sum.s != sum.s) {  // a NaN, or infinities
+    if (is_nan(sum)) {  // a NaN, or infinities
       const uint32_t first = first_nan(x, a.n_cols, lane, 32);
       if (first != ~0u) {
         best = static_cast<V>(NAN);

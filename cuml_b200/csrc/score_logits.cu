@@ -19,15 +19,27 @@ constexpr int kTileCols   = 64;
 constexpr int kTileLeast  = 32;
 constexpr int kTileBlocks = 8;   // of an SM
 
-// n elements of a row by `threads` threads.
-template <class T>
-__device__ __forceinline__ Scored visit_scores(const T* row, int64_t n, int tid, int threads, float c)
+// n elements of a row by THREADS threads, joined for all of them.
+template <class T, int THREADS>
+__device__ __forceinline__ Scored visit_ordinary(const T* row, int64_t n, int tid, float c, float* room)
+{
+  PairedStream<T> r;
+  const float slack = kSlack / c;
+  visit_row<kInFlight>(
+    row, n, tid, THREADS, [&](int64_t, T x) { r.take(widen(x), c, slack); },
+    [&](int64_t, const Piece<T>& v) { r.take(v, largest_of(v), c, slack); });
+  Scored o = r.scored(c);
+  join_scored<THREADS>(o, c, room);
+  return o;
+}
+template <class T, int THREADS>
+__device__ __noinline__ Scored visit_any(const T* row, int64_t n, int tid, float c, float* room)
 {
   constexpr int N = Piece<T>::N;
   ScoredStream r;
   const float slack = kSlack / c;
   visit_row<kInFlight>(
-    row, n, tid, threads,
+    row, n, tid, THREADS,
     [&](int64_t, T x) {
       const float one[1] = {widen(x)};
       r.take(one, c, slack);
@@ -38,7 +50,14 @@ __device__ __forceinline__ Scored visit_scores(const T* row, int64_t n, int tid,
       for (int e = 0; e < N; ++e) x[e] = widen(v.v[e]);
       r.take(x, c, slack);
     });
+  join_scored<THREADS>(r, c, room);
   return r;
+}
+template <class T, int THREADS>
+__device__ __forceinline__ Scored visit_scores(const T* row, int64_t n, int tid, float c, float* room)
+{
+  const Scored r = visit_ordinary<T, THREADS>(row, n, tid, c, room);
+  return PairedStream<T>::usable(r.m, c) ? r : visit_any<T, THREADS>(row, n, tid, c, room);
 }
 
 // One part of a row per block: (row, segment) -> its m, s and u.
@@ -51,8 +70,7 @@ __global__ void __launch_bounds__(kThreads) score_parts(ScoreArgs a, int64_t seg
   const float c       = a.temperature.c;
   for (int64_t row = blockIdx.y; row < a.n_rows; row += gridDim.y) {
     const T* x = static_cast<const T*>(a.logits) + row * a.row_stride + begin;
-    Scored r   = visit_scores(x, n, threadIdx.x, kThreads, c);
-    join_scored<kThreads>(r, c, room);
+    const Scored r = visit_scores<T, kThreads>(x, n, threadIdx.x, c, room);
     if (threadIdx.x == 0) parts[row * gridDim.x + blockIdx.x] = make_float4(r.m, r.s, r.u, 0.f);
   }
 }
@@ -76,10 +94,10 @@ __global__ void __launch_bounds__(kThreads) score_rows(ScoreArgs a, int segs, co
         const float4 p = parts[row * segs + i];
         r.join(p.x, p.y, p.z, c);
       }
+      join_scored<THREADS>(r, c, room);
     } else {
-      r = visit_scores(x, a.n_cols, tid, THREADS, c);
+      r = visit_scores<T, THREADS>(x, a.n_cols, tid, c, room);
     }
-    join_scored<THREADS>(r, c, room);
     if (tid == 0) finish_score(a.out, row, r, a.temperature.inverse, at, at >= 0 ? widen(x[at]) : 0.f);
   }
 }

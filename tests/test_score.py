@@ -310,6 +310,33 @@ def test_logits_far_apart_and_far_from_zero(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TRAINED)
+@pytest.mark.parametrize("k", [0, 3])
+def test_logits_that_the_paired_sums_do_not_take(dtype, k):
+    """Rows below and around the border of what counts as ordinary, masked parts of a row beside ordinary ones, and very high and low
+    temperatures, by which a mask of the type's lowest value may count."""
+    border = 30_000.0 if dtype == "fp16" else 1e29
+    for n, c in ((6, 3000), (6, 20_000), (1200, 2500)):
+        z, t = logits(n, c, dtype, scale=1.0), targets(n, c)
+        lowest = torch.finfo(z.dtype).min
+        low = z.float()
+        low[0] = -border + low[0] * border / 1000
+        low[1, : c // 2] = -border * 0.999
+        low[1, c // 2:] = -border * 1.001
+        low[2, : c - 50] = lowest
+        low[3] = lowest if dtype == "fp16" else -2 * border
+        low[4, : c // 2] = float("-inf")
+        low[4, c // 2:] = -border * 1.5
+        t[:5] = c - 1
+        z = low.to(z.dtype)
+        g, h = upstreams(n)
+        for temperature in (1.0, 50.0, 1e4, 1e6, 1e-3):
+            if temperature == 1e-3 and dtype == "fp16":
+                continue  # (gradients beyond 65504)
+            check(z, t, temperature, k, g, h)
+
+
+@gpu
 @pytest.mark.parametrize("compiled", [True, False])
 def test_strides_and_shapes(monkeypatch, compiled):
     from cuml_b200 import distill
