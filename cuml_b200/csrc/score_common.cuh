@@ -59,7 +59,8 @@ struct Scored {
   }
   __device__ __forceinline__ void join_lanes(float c)
   {
-    const float to = max_lanes(m);
+    float to;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(to) : "f"(m));
     if (to != lowest<float>()) move(to, c);
     s = sum_lanes(s);
     u = sum_lanes(u);
@@ -87,6 +88,51 @@ struct ScoredStream : Scored {
     for (int e = 0; e < N; ++e) add(x[e], base, c);
   }
 };
+
+// A piece's 16 bytes and back, as the language allows it.  (Elements written through another type's pointer were left out of
+// later stores.)
+template <class T>
+__device__ __forceinline__ uint4 words_of(const Piece<T>& p)
+{
+  uint4 w;
+  memcpy(&w, &p, 16);
+  return w;
+}
+template <class T>
+__device__ __forceinline__ Piece<T> piece_of(const uint4& w)
+{
+  Piece<T> p;
+  memcpy(&p, &w, 16);
+  return p;
+}
+
+// visit_row whose last pieces are in flight together, too, and the elements before and behind them with the first: ends(i, x, k, y) for those that
+// a thread has, i or k below 0 where it has none.  A row of a warp may be no more than that.
+template <int U, class T, class Ends, class Many>
+__device__ __forceinline__ void visit_all(const T* row, int n, int tid, int threads, Ends ends, Many many)
+{
+  constexpr int N  = Piece<T>::N;
+  const int lead   = lead_of(row, n);
+  const int pieces = (n - lead) / N;
+  const T* body    = row + lead;
+  const int at     = lead + pieces * N + tid;
+  T before = T(), behind = T();
+  if (tid < lead) before = row[tid];
+  if (at < n) behind = row[at];
+  for (int first = 0; first < pieces; first += U * threads) {  // (the same rounds for all threads: none goes two ways)
+    const int left  = pieces - first - tid;
+    const bool full = left + tid >= U * threads;
+    const T* from   = body + static_cast<int64_t>(first + tid) * N;
+    Piece<T> r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (full || u * threads < left) r[u] = piece_of<T>(__ldg(reinterpret_cast<const uint4*>(from + u * threads * N)));
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (full || u * threads < left) many(lead + (first + tid + u * threads) * N, r[u]);
+  }
+  if (tid < lead || at < n) ends(tid < lead ? tid : -1, before, at < n ? at : -1, behind);
+}
 
 // ---- two numbers at a time ---------------------------------------------------------------------
 __device__ __forceinline__ uint64_t pair_of(float lo, float hi)
@@ -119,25 +165,60 @@ struct Ordinary<__half> {
   static constexpr float kFloor = -65504.f, kAbove = -30000.f;
 };
 
+__device__ __forceinline__ float2 halves_of(uint32_t w)
+{
+  __half2 h;
+  memcpy(&h, &w, 4);
+  return __half22float2(h);
+}
+
+// A piece's numbers.
+__device__ __forceinline__ void numbers_of(const Piece<float>& p, float (&x)[4])
+{
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = p.v[i];
+}
+__device__ __forceinline__ void numbers_of(const Piece<__nv_bfloat16>& p, float (&x)[8])
+{
+  const uint4 all     = words_of(p);
+  const uint32_t w[4] = {all.x, all.y, all.z, all.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i]     = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void numbers_of(const Piece<__half>& p, float (&x)[8])
+{
+  const uint4 all     = words_of(p);
+  const uint32_t w[4] = {all.x, all.y, all.z, all.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = halves_of(w[i]);
+    x[2 * i]       = f.x;
+    x[2 * i + 1]   = f.y;
+  }
+}
+
 // 16 bytes of logits: the largest (NaN left out), and all of them, at least kFloor, in pairs.
 __device__ __forceinline__ float largest_of(const Piece<float>& p) { return fmaxf(fmaxf(p.v[0], p.v[1]), fmaxf(p.v[2], p.v[3])); }
 __device__ __forceinline__ float largest_of(const Piece<__nv_bfloat16>& p)
 {
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(&p);
+  const uint4 w = words_of(p);
   uint32_t a, b;
-  asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(w[0]), "r"(w[1]));
-  asm("max.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(w[2]), "r"(w[3]));
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(w.x), "r"(w.y));
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(w.z), "r"(w.w));
   asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
   return fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u));
 }
 __device__ __forceinline__ float largest_of(const Piece<__half>& p)
 {
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(&p);
+  const uint4 w = words_of(p);
   uint32_t a, b;
-  asm("max.f16x2 %0, %1, %2;" : "=r"(a) : "r"(w[0]), "r"(w[1]));
-  asm("max.f16x2 %0, %1, %2;" : "=r"(b) : "r"(w[2]), "r"(w[3]));
+  asm("max.f16x2 %0, %1, %2;" : "=r"(a) : "r"(w.x), "r"(w.y));
+  asm("max.f16x2 %0, %1, %2;" : "=r"(b) : "r"(w.z), "r"(w.w));
   asm("max.f16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
+  const float2 f = halves_of(a);
   return fmaxf(f.x, f.y);
 }
 template <class F>
@@ -150,7 +231,8 @@ __device__ __forceinline__ void each_pair(const Piece<float>& p, F f)
 template <class F>
 __device__ __forceinline__ void each_pair(const Piece<__nv_bfloat16>& p, F f)
 {
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(&p);
+  const uint4 all     = words_of(p);
+  const uint32_t w[4] = {all.x, all.y, all.z, all.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t x;
@@ -161,12 +243,13 @@ __device__ __forceinline__ void each_pair(const Piece<__nv_bfloat16>& p, F f)
 template <class F>
 __device__ __forceinline__ void each_pair(const Piece<__half>& p, F f)
 {
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(&p);
+  const uint4 all     = words_of(p);
+  const uint32_t w[4] = {all.x, all.y, all.z, all.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t x;
     asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(x) : "r"(w[i]), "r"(0xfbfffbffu));  // -65504
-    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&x));
+    const float2 v = halves_of(x);
     f(pair_of(v.x, v.y));
   }
 }
@@ -205,11 +288,12 @@ struct PairedStream {
     const uint64_t cc = pair_of(c, c), minus_r = pair_of(-r, -r);
     each_pair(p, [&](uint64_t z) { add(z, cc, minus_r); });
   }
-  __device__ __forceinline__ void take(float z, float c, float slack)
+  __device__ __forceinline__ void take(float z, float c, float slack) { take(z, Ordinary<T>::kFloor, c, slack); }
+  __device__ __forceinline__ void take(float z, float y, float c, float slack)
   {
-    reach(z, c, slack);
+    reach(fmaxf(z, y), c, slack);
     constexpr float kFloor = Ordinary<T>::kFloor;
-    add(pair_of(at_least(z, kFloor), kFloor), pair_of(c, c), pair_of(-r, -r));
+    add(pair_of(at_least(z, kFloor), at_least(y, kFloor)), pair_of(c, c), pair_of(-r, -r));
   }
   // relative to 2^(m c)
   __device__ __forceinline__ Scored scored(float c) const
@@ -307,6 +391,23 @@ struct RowGrad {
     return power(a) * fmaf(B, a, A);
   }
 };
+// The same of a piece; none for classes.
+template <class T>
+__device__ __forceinline__ void grads_of(const RowGrad& r, const Piece<T>& z, float c, float (&y)[Piece<T>::N])
+{
+  const uint64_t minus_base = pair_of(-r.base, -r.base), cc = pair_of(c, c), AA = pair_of(r.A, r.A), BB = pair_of(r.B, r.B);
+  float x[Piece<T>::N];
+  numbers_of(z, x);
+#pragma unroll
+  for (int e = 0; e < Piece<T>::N; e += 2) {
+    const uint64_t far = fma_pairs(add_pairs(pair_of(x[e], x[e + 1]), minus_base), cc, 0);
+    float lo, hi;
+    split_pair(far, lo, hi);
+    lo = at_least(lo, kLeast);
+    hi = at_least(hi, kLeast);
+    split_pair(fma_pairs(pair_of(power(lo), power(hi)), fma_pairs(BB, pair_of(lo, hi), AA), 0), y[e], y[e + 1]);
+  }
+}
 // g, h: gradients by the row's log probability and entropy, times 1 / T (and a scale).
 __device__ __forceinline__ RowGrad row_grad(const float4& kept, float g, float h)
 {

@@ -14,24 +14,41 @@ constexpr int kWarpCols = 2048;  // rows that belong to one warp
 constexpr int kSegment  = 8192;  // fewest elements of a row that are worth a block of their own
 constexpr int kMostSegs = 64;
 constexpr int kInFlight = 4;     // pieces of a thread
+// Blocks of an SM, all there at once: of rows by blocks, rows by warps and gradients.  (4096 x 131,072 bf16, 164 us at memory's
+// rate: the reading alone takes 186 us with four, 172 with five.)  Their rows lie next to one another at any time (60,000 x 1001 bf16,
+// both passes: 42 and 58 us; 50 and 64 where each had rows of its own).
+constexpr int kRowBlocks  = 5;
+constexpr int kWarpBlocks = 4;
+constexpr int kGradBlocks = 4;
+// Bytes of a row that is worth a block's start.  (Gradient of 4096 x 131,072 bf16: 319 us, 345 with ten blocks of an SM that take several;
+// 4096 x 8192 fp32: 38 us with a block for each row, 32 so.)
+constexpr int64_t kLongRow = 1 << 16;
+// Where there are kWarpLeast rows per SM, a warp takes longer ones, too: whose logits take up to kWarpBytes, and in the
+// gradient, of 16 bits, up to kWarpLong.  (20,000 x 3000 bf16, both passes: 96 and 66 us by blocks, 34 and 43 so.)
+constexpr int kWarpLeast = 8;
+constexpr int kWarpBytes = 16384;
+constexpr int kWarpLong  = 8192;
 // Rows for one thread each: classes, and rows per SM from which on.
 constexpr int kTileCols   = 64;
 constexpr int kTileLeast  = 32;
 constexpr int kTileBlocks = 8;   // of an SM
 
-// n elements of a row by THREADS threads, joined for all of them.
-template <class T, int THREADS>
-__device__ __forceinline__ Scored visit_ordinary(const T* row, int64_t n, int tid, float c, float* room)
+// n elements of a row by `threads` threads; the thread's part.
+template <class T>
+__device__ __forceinline__ Scored visit_ordinary(const T* row, int n, int tid, int threads, float c)
 {
   PairedStream<T> r;
   const float slack = kSlack / c;
-  visit_row<kInFlight>(
-    row, n, tid, THREADS, [&](int64_t, T x) { r.take(widen(x), c, slack); },
-    [&](int64_t, const Piece<T>& v) { r.take(v, largest_of(v), c, slack); });
-  Scored o = r.scored(c);
-  join_scored<THREADS>(o, c, room);
-  return o;
+  visit_all<kInFlight>(
+    row, n, tid, threads,
+    [&](int i, T x, int k, T y) {
+      constexpr float kFloor = Ordinary<T>::kFloor;
+      r.take(i < 0 ? kFloor : widen(x), k < 0 ? kFloor : widen(y), c, slack);
+    },
+    [&](int, const Piece<T>& v) { r.take(v, largest_of(v), c, slack); });
+  return r.scored(c);
 }
+// The same of any logits, joined for all threads.
 template <class T, int THREADS>
 __device__ __noinline__ Scored visit_any(const T* row, int64_t n, int tid, float c, float* room)
 {
@@ -53,12 +70,6 @@ __device__ __noinline__ Scored visit_any(const T* row, int64_t n, int tid, float
   join_scored<THREADS>(r, c, room);
   return r;
 }
-template <class T, int THREADS>
-__device__ __forceinline__ Scored visit_scores(const T* row, int64_t n, int tid, float c, float* room)
-{
-  const Scored r = visit_ordinary<T, THREADS>(row, n, tid, c, room);
-  return PairedStream<T>::usable(r.m, c) ? r : visit_any<T, THREADS>(row, n, tid, c, room);
-}
 
 // One part of a row per block: (row, segment) -> its m, s and u.
 template <class T>
@@ -66,39 +77,82 @@ __global__ void __launch_bounds__(kThreads) score_parts(ScoreArgs a, int64_t seg
 {
   __shared__ float room[3 * kThreads / 32];
   const int64_t begin = blockIdx.x * seg_cols;
-  const int64_t n     = min(seg_cols, a.n_cols - begin);
+  const int n         = static_cast<int>(min(seg_cols, a.n_cols - begin));
   const float c       = a.temperature.c;
   for (int64_t row = blockIdx.y; row < a.n_rows; row += gridDim.y) {
     const T* x = static_cast<const T*>(a.logits) + row * a.row_stride + begin;
-    const Scored r = visit_scores<T, kThreads>(x, n, threadIdx.x, c, room);
+    Scored r   = visit_ordinary(x, n, threadIdx.x, kThreads, c);
+    join_scored<kThreads>(r, c, room);
+    if (!PairedStream<T>::usable(r.m, c)) r = visit_any<T, kThreads>(x, n, threadIdx.x, c, room);
     if (threadIdx.x == 0) parts[row * gridDim.x + blockIdx.x] = make_float4(r.m, r.s, r.u, 0.f);
   }
 }
-
-// A row by THREADS threads.  segs > 0: its parts are joined (by a warp).
-template <class T, int THREADS>
-__global__ void __launch_bounds__(kThreads) score_rows(ScoreArgs a, int segs, const float4* parts)
+// ... and a row's scores from them, by a warp.
+template <class T>
+__global__ void __launch_bounds__(kThreads) score_join(ScoreArgs a, int segs, const float4* parts)
 {
-  constexpr int ROWS = kThreads / THREADS;
-  __shared__ float room[3 * kThreads / 32];
-  const int slot = threadIdx.x / THREADS, tid = threadIdx.x % THREADS;
-  const float c = a.temperature.c;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + slot; row < a.n_rows;
-       row += static_cast<int64_t>(gridDim.x) * ROWS) {
-    const T* x   = static_cast<const T*>(a.logits) + row * a.row_stride;
-    const int at = target_of(a.target, row, a.n_cols);
+  constexpr int ROWS = kThreads / 32;
+  const int lane = threadIdx.x % 32;
+  const float c  = a.temperature.c;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / 32; row < a.n_rows; row += static_cast<int64_t>(gridDim.x) * ROWS) {
+    const int at      = target_of(a.target, row, a.n_cols);
+    const float given = at >= 0 ? widen(static_cast<const T*>(a.logits)[row * a.row_stride + at]) : 0.f;
     Scored r;
-    if (at == -2) {  // not read
-    } else if (segs > 0) {
-      for (int i = tid; i < segs; i += THREADS) {
-        const float4 p = parts[row * segs + i];
-        r.join(p.x, p.y, p.z, c);
-      }
-      join_scored<THREADS>(r, c, room);
-    } else {
-      r = visit_scores<T, THREADS>(x, a.n_cols, tid, c, room);
+    for (int i = lane; i < segs; i += 32) {
+      const float4 p = parts[row * segs + i];
+      r.join(p.x, p.y, p.z, c);
     }
-    if (tid == 0) finish_score(a.out, row, r, a.temperature.inverse, at, at >= 0 ? widen(x[at]) : 0.f);
+    r.join_lanes(c);
+    if (lane == 0) finish_score(a.out, row, r, a.temperature.inverse, at, given);
+  }
+}
+
+// Rows by THREADS threads.  What a row takes besides its logits is done for 32 of them at a time, a lane each: the given
+// classes before, the scores behind.  The warps of a block go through the rows on their own.
+template <class T, int THREADS>
+__global__ void __launch_bounds__(kThreads, THREADS == 32 ? kWarpBlocks : kRowBlocks) score_rows(ScoreArgs a)
+{
+  constexpr int ROWS = kThreads / THREADS, W = THREADS / 32;
+  __shared__ float room[3 * W];
+  __shared__ float parts[W > 1 ? 32 * W * 3 : 1];
+  const int tid = threadIdx.x % THREADS, lane = threadIdx.x % 32, warp = tid / 32;
+  const float c      = a.temperature.c;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS;
+  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / THREADS; row0 < a.n_rows; row0 += 32 * step) {
+    const int count = static_cast<int>(min(static_cast<int64_t>(32), (a.n_rows - row0 + step - 1) / step));
+    auto logits     = [&](int j) { return static_cast<const T*>(a.logits) + (row0 + j * step) * a.row_stride; };
+    const int at    = lane < count ? target_of(a.target, row0 + lane * step, a.n_cols) : -2;
+    Scored mine;  // of the lane's row
+    for (int j = 0; j < count; ++j) {
+      if (__shfl_sync(~0u, at, j) == -2) continue;  // not read
+      Scored r = visit_ordinary(logits(j), static_cast<int>(a.n_cols), tid, THREADS, c);
+      r.join_lanes(c);
+      if (W == 1) {
+        if (lane == j) mine = r;
+      } else if (lane == 0) {
+        float* p = parts + (j * W + warp) * 3;
+        p[0]     = r.m;
+        p[1]     = r.s;
+        p[2]     = r.u;
+      }
+    }
+    if (W > 1) {
+      __syncthreads();
+      if (at != -2) {
+        for (int w = 0; w < W; ++w) {
+          const float* p = parts + (lane * W + w) * 3;
+          mine.join(p[0], p[1], p[2], c);
+        }
+      }
+    }
+    for (unsigned again = __ballot_sync(~0u, at != -2 && !PairedStream<T>::usable(mine.m, c)); again; again &= again - 1) {
+      const int j    = __ffs(again) - 1;
+      const Scored r = visit_any<T, THREADS>(logits(j), a.n_cols, tid, c, room);
+      if (lane == j) mine = r;
+    }
+    if (lane < count && warp == 0)
+      finish_score(a.out, row0 + lane * step, mine, a.temperature.inverse, at, at >= 0 ? widen(logits(lane)[at]) : 0.f);
+    if (W > 1) __syncthreads();  // `parts` has been read
   }
 }
 
@@ -172,45 +226,64 @@ __device__ __forceinline__ void zero_row(T* row, int64_t n, int tid, int threads
   if (end + tid < n) row[end + tid] = narrow<T>(0.f);
 }
 
-// Gradient of a part of a row by THREADS threads; blockIdx.y: the part.
+// Gradient of a part (blockIdx.y) of rows by THREADS threads.  Rows' factors are made by a lane each, 32 at a time.
 template <class T, int THREADS>
-__global__ void __launch_bounds__(kThreads) score_grad(ScoreGradArgs g, int64_t seg_cols)
+__global__ void __launch_bounds__(kThreads, kGradBlocks) score_grad(ScoreGradArgs g, int64_t seg_cols)
 {
   constexpr int ROWS = kThreads / THREADS, N = Piece<T>::N;
   const ScoreArgs& a = g.fwd;
-  const int slot = threadIdx.x / THREADS, tid = threadIdx.x % THREADS;
+  const int tid = threadIdx.x % THREADS, lane = threadIdx.x % 32;
   const float c       = a.temperature.c, inv_t = static_cast<float>(a.temperature.inverse);
   const int64_t begin = blockIdx.y * seg_cols;
-  const int64_t n     = min(seg_cols, a.n_cols - begin);
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + slot; row < a.n_rows;
-       row += static_cast<int64_t>(gridDim.x) * ROWS) {
-    const T* x = static_cast<const T*>(a.logits) + row * a.row_stride + begin;
-    T* d       = static_cast<T*>(g.grad) + row * g.grad_stride + begin;
-    const ScoreUpstream& up = g.upstream;
-    const RowGrad r  = row_grad(a.out.kept[row], up.log_prob ? up.log_prob[row * up.log_prob_stride] * inv_t : 0.f,
-                                up.entropy ? up.entropy[row * up.entropy_stride] * inv_t : 0.f);
-    const int64_t at = r.at < 0 ? -1 : r.at - begin;
-    if (!r.counts) {
-      zero_row(d, n, tid, THREADS);
-      continue;
+  const int n         = static_cast<int>(min(seg_cols, a.n_cols - begin));
+  const int64_t step  = static_cast<int64_t>(gridDim.x) * ROWS;
+  const ScoreUpstream& up = g.upstream;
+  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / THREADS; row0 < a.n_rows; row0 += 32 * step) {
+    const int count = static_cast<int>(min(static_cast<int64_t>(32), (a.n_rows - row0 + step - 1) / step));
+    RowGrad mine{};
+    if (lane < count) {
+      const int64_t row = row0 + lane * step;
+      mine = row_grad(a.out.kept[row], up.log_prob ? up.log_prob[row * up.log_prob_stride] * inv_t : 0.f,
+                      up.entropy ? up.entropy[row * up.entropy_stride] * inv_t : 0.f);
+      if (!mine.counts) mine.at = -2;
     }
-    auto one = [&](int64_t i, T v) { d[i] = narrow<T>(r(widen(v), c) + (i == at ? r.add : 0.f)); };
-    if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0) {
-      visit_row<kInFlight>(x, n, tid, THREADS, one, [&](int64_t i, const Piece<T>& v) {
-        float y[N];
+    for (int j = 0; j < count; ++j) {
+      const T* x = static_cast<const T*>(a.logits) + (row0 + j * step) * a.row_stride + begin;
+      T* d       = static_cast<T*>(g.grad) + (row0 + j * step) * g.grad_stride + begin;
+      RowGrad r;
+      r.at = __shfl_sync(~0u, mine.at, j);
+      if (r.at == -2) {
+        zero_row(d, n, tid, THREADS);
+        continue;
+      }
+      r.base = __shfl_sync(~0u, mine.base, j);
+      r.A    = __shfl_sync(~0u, mine.A, j);
+      r.B    = __shfl_sync(~0u, mine.B, j);
+      r.add  = __shfl_sync(~0u, mine.add, j);
+      const int at = r.at >= begin && r.at - begin < n ? static_cast<int>(r.at - begin) : -1;
+      auto one     = [&](int i, T v) { d[i] = narrow<T>(r(widen(v), c) + (i == at ? r.add : 0.f)); };
+      if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0) {
+        visit_all<kInFlight>(
+          x, n, tid, THREADS,
+          [&](int i, T v, int k, T w) {
+            if (i >= 0) one(i, v);
+            if (k >= 0) one(k, w);
+          },
+          [&](int i, const Piece<T>& v) {
+            float y[N];
+            grads_of(r, v, c, y);
+            if (static_cast<unsigned>(at - i) < N) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) y[e] = r(widen(v.v[e]), c);
-        if (at >= i && at < i + N) {
+              for (int e = 0; e < N; ++e) y[e] += at - i == e ? r.add : 0.f;
+            }
+            Piece<T> w;
 #pragma unroll
-          for (int e = 0; e < N; ++e) y[e] += at - i == e ? r.add : 0.f;
-        }
-        Piece<T> w;
-#pragma unroll
-        for (int e = 0; e < N; ++e) w.v[e] = narrow<T>(y[e]);
-        *reinterpret_cast<uint4*>(d + i) = *reinterpret_cast<const uint4*>(&w);
-      });
-    } else {
-      for (int64_t i = tid; i < n; i += THREADS) one(i, x[i]);
+            for (int e = 0; e < N; ++e) w.v[e] = narrow<T>(y[e]);
+            *reinterpret_cast<uint4*>(d + i) = words_of(w);
+          });
+      } else {
+        for (int i = tid; i < n; i += THREADS) one(i, x[i]);
+      }
     }
   }
 }
@@ -231,6 +304,16 @@ int64_t part_cols(int64_t n_cols, int segs)
 }
 unsigned blocks_of(int64_t need, int64_t most) { return static_cast<unsigned>(need < most ? need : most); }
 
+bool by_warps(const ScoreArgs& a, int n_sms, bool longer)
+{
+  return a.n_cols <= kWarpCols || (longer && a.n_rows >= static_cast<int64_t>(kWarpLeast) * n_sms);
+}
+// Blocks of a launch: a block for each long row, else as many as are there at once.
+unsigned row_blocks(const ScoreArgs& a, bool warp, int element, int64_t at_once)
+{
+  if (warp) return blocks_of((a.n_rows + kThreads / 32 - 1) / (kThreads / 32), at_once);
+  return blocks_of(a.n_rows, a.n_cols * element >= kLongRow ? 1 << 30 : at_once);
+}
 bool by_tiles(const ScoreArgs& a, int n_sms) { return a.n_cols <= kTileCols && a.n_rows >= static_cast<int64_t>(kTileLeast) * n_sms; }
 template <class T, class A>
 cudaError_t run_tiles(void (*kernel)(A), const A& args, const ScoreArgs& a, int n_sms, cudaStream_t s)
@@ -248,16 +331,18 @@ cudaError_t run_score(const ScoreArgs& a, void* workspace, int n_sms, cudaStream
   int segs           = segments(a.n_rows, a.n_cols, n_sms);
   const int64_t cols = part_cols(a.n_cols, segs);
   segs               = segs == 1 ? 1 : static_cast<int>((a.n_cols + cols - 1) / cols);
-  float4* parts      = static_cast<float4*>(workspace);
-  if (segs > 1) score_parts<T><<<dim3(segs, blocks_of(a.n_rows, 65535)), kThreads, 0, s>>>(a, cols, parts);
-  const bool warp    = segs > 1 || a.n_cols <= kWarpCols;
-  const int per      = warp ? kThreads / 32 : 1;
-  const unsigned blocks = blocks_of((a.n_rows + per - 1) / per, 8ll * n_sms);
-  if (warp)
-    score_rows<T, 32><<<blocks, kThreads, 0, s>>>(a, segs > 1 ? segs : 0, parts);
+  if (segs > 1) {
+    float4* parts = static_cast<float4*>(workspace);
+    score_parts<T><<<dim3(segs, blocks_of(a.n_rows, 65535)), kThreads, 0, s>>>(a, cols, parts);
+    score_join<T><<<blocks_of((a.n_rows + kThreads / 32 - 1) / (kThreads / 32), 8ll * n_sms), kThreads, 0, s>>>(a, segs, parts);
+    count_launches(2);
+    return cudaGetLastError();
+  }
+  if (by_warps(a, n_sms, a.n_cols * sizeof(T) <= kWarpBytes))
+    score_rows<T, 32><<<row_blocks(a, true, sizeof(T), kWarpBlocks * n_sms), kThreads, 0, s>>>(a);
   else
-    score_rows<T, kThreads><<<blocks, kThreads, 0, s>>>(a, 0, parts);
-  count_launches(segs > 1 ? 2 : 1);
+    score_rows<T, kThreads><<<row_blocks(a, false, sizeof(T), kRowBlocks * n_sms), kThreads, 0, s>>>(a);
+  count_launches(1);
   return cudaGetLastError();
 }
 
@@ -266,16 +351,15 @@ cudaError_t run_grad(const ScoreGradArgs& g, int n_sms, cudaStream_t s)
 {
   const ScoreArgs& a = g.fwd;
   if (by_tiles(a, n_sms)) return run_tiles<T>(grad_tiles<T>, g, a, n_sms, s);
-  const bool warp    = a.n_cols <= kWarpCols;
-  const int per      = warp ? kThreads / 32 : 1;
+  const bool warp    = by_warps(a, n_sms, sizeof(T) == 2 && a.n_cols <= kWarpLong);
+  const unsigned rows = row_blocks(a, warp, sizeof(T), kGradBlocks * n_sms);
   int segs           = warp ? 1 : segments(a.n_rows, a.n_cols, n_sms);
   const int64_t cols = part_cols(a.n_cols, segs);
   segs               = segs == 1 ? 1 : static_cast<int>((a.n_cols + cols - 1) / cols);
-  const unsigned blocks = blocks_of((a.n_rows + per - 1) / per, 8ll * n_sms);
   if (warp)
-    score_grad<T, 32><<<blocks, kThreads, 0, s>>>(g, cols);
+    score_grad<T, 32><<<rows, kThreads, 0, s>>>(g, cols);
   else
-    score_grad<T, kThreads><<<dim3(blocks, segs), kThreads, 0, s>>>(g, cols);
+    score_grad<T, kThreads><<<dim3(rows, segs), kThreads, 0, s>>>(g, cols);
   count_launches(1);
   return cudaGetLastError();
 }
