@@ -60,6 +60,9 @@ constexpr float kHalfScale    = 16384.f;       // of d in fp16
 // one per row nothing in the epilogue and 3.6 us per piece in the kernel).
 constexpr int kFewNamed = 4;
 constexpr int kScaleBlocks = 8;
+// Stages whose sums stay in TMEM before the epilogue adds them up, where the logits themselves are the answer (kScoreStats): the tensor
+// cores cut each addition short, which over 2048 terms takes 1.5e-6 off a logit, and its log q and entropy with it.
+constexpr int kSumStages = 8;
 
 __device__ int g_status;
 __device__ __forceinline__ bool incomplete() { return *static_cast<volatile int*>(&g_status) != 0; }
@@ -335,10 +338,11 @@ __device__ __forceinline__ void take_columns(const Work& w, const Product& p, in
       score.s += (s[0] + s[1]) + (s[2] + s[3]);
       score.u += (u[0] + u[1]) + (u[2] + u[3]);
       if (at >= col && at < col + 32) {
-        float z = 0.f;
+        // (as a choice in C++ it is an index, for which all of x would be put into memory)
 #pragma unroll
-        for (int i = 0; i < 32; ++i) z += at - col == i ? x[i] : 0.f;
-        w.target_logit[row] = z;
+        for (int i = 0; i < 32; ++i)
+          asm volatile("{\n.reg .pred p;\nsetp.eq.s32 p, %0, %1;\n@p st.global.f32 [%2], %3;\n}" ::"r"(at - col), "r"(i),
+                       "l"(w.target_logit + row), "f"(x[i]) : "memory");
       }
       return;
     }
@@ -535,7 +539,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      int first = t.begin;  // of the sum
       for (int k = t.begin; k < t.end; ++k) {
+        if (KIND == kScoreStats && k == first + kSumStages) {
+          first = k;
+          half ^= 1;
+          turn ^= half == 0;
+          if (!warp_wait(freed + 8 * half, turn ^ 1, &gave_up)) {
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
         if (!warp_wait(full + 8 * stage, phase, &gave_up)) {
           ok = false;
           break;
@@ -545,9 +560,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
         if (elected()) {
 #pragma unroll
           for (int j = 0; j < kDepth / 16; ++j)
-            mma(tmem + half * kTile, a + j * step_a, b + j * step_b, idesc, k > t.begin || j > 0);
+            mma(tmem + half * kTile, a + j * step_a, b + j * step_b, idesc, k > first || j > 0);
           commit(empty + 8 * stage);
-          if (k + 1 == t.end) commit(done + 8 * half);
+          if (k + 1 == t.end || (KIND == kScoreStats && k + 1 == first + kSumStages)) commit(done + 8 * half);
         }
         __syncwarp();
         if (++stage == kStages) {
@@ -611,6 +626,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
         factor         = s.w == 0.f ? 0.f : s.y * w.diff_scale * (w.row_scale ? w.row_scale[row * w.row_step] : 1.f);
       }
       if (KIND == kGrad && !p.sums) factor = w.scale();
+      if constexpr (KIND == kScoreStats) {
+        static_assert(kTile / 2 == 4 * 32, "four arrays of 32");
+        float z0[32], z1[32], z2[32], z3[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) z0[i] = z1[i] = z2[i] = z3[i] = 0.f;
+        auto add = [&](int c, float(&z)[32]) {
+          float x[32];
+          load_columns(tmem + half * kTile + from + 32 * c + (static_cast<uint32_t>(quarter * 32) << 16), x);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) z[i] += x[i];
+        };
+        for (int k = t.begin; ok && k < t.end; k += kSumStages) {
+          if (!warp_wait(done + 8 * half, turn, &gave_up)) {
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          add(0, z0);
+          add(1, z1);
+          add(2, z2);
+          add(3, z3);
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) bar_arrive_cluster(freed0 + 8 * half);
+          half ^= 1;
+          turn ^= half == 0;
+        }
+        if (!ok) break;
+        if (in) {
+          Running<float> unused;
+          Scored score;
+          const int col = t.n * kTile + from;
+          if (col < p.n) take_columns<KIND>(w, p, t.split, row, col, z0, unused, score, of_score, at, base, sum, factor);
+          if (col + 32 < p.n) take_columns<KIND>(w, p, t.split, row, col + 32, z1, unused, score, of_score, at, base, sum, factor);
+          if (col + 64 < p.n) take_columns<KIND>(w, p, t.split, row, col + 64, z2, unused, score, of_score, at, base, sum, factor);
+          if (col + 96 < p.n) take_columns<KIND>(w, p, t.split, row, col + 96, z3, unused, score, of_score, at, base, sum, factor);
+          w.score_parts[(row * p.n_tiles + t.n) * 2 + (from != 0)] = make_float4(score.m, score.s, score.u, 0.f);
+        }
+        __syncwarp();
+        continue;
+      }
       if (!warp_wait(done + 8 * half, turn, &gave_up)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       Running<float> r;
@@ -641,8 +697,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
         }
       }
       if (KIND == kStats && in) w.parts[(row * p.n_tiles + t.n) * 2 + (from != 0)] = make_float2(r.m, r.s);
-      if (KIND == kScoreStats && in)
-        w.score_parts[(row * p.n_tiles + t.n) * 2 + (from != 0)] = make_float4(score.m, score.s, score.u, 0.f);
       half ^= 1;
       turn ^= half == 0;
     }
