@@ -941,32 +941,30 @@ __global__ void __launch_bounds__(kThreads) finish_sums(const float* sums, int s
   }
 }
 
-// The same for rows of `width` of `pitch` columns: four results per thread, which may be in two rows (or more).
+// The same for rows of `width` of `pitch` columns, a warp for each.  (Four results per thread, which may be in two rows: 1999 x
+// 1001 x 50,001 took 84 us, this way 38.)
 template <class T>
 __global__ void __launch_bounds__(kThreads) finish_rows(const float* sums, int splits, int64_t rows, int pitch, int width,
                                                         Scale scale, T* out)
 {
-  const float f     = scale();
-  const int64_t all = rows * width;
-  for (int64_t i = 4 * (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x); i < all; i += 4 * gridDim.x * static_cast<int64_t>(kThreads)) {
-    int64_t r = i / width;
-    int c     = static_cast<int>(i - r * width);
-    T v[4];
+  constexpr int ROWS = kThreads / 32, U = 4;
+  const float f  = scale();
+  const int lane = threadIdx.x % 32;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / 32; r < rows; r += static_cast<int64_t>(gridDim.x) * ROWS) {
+    const float* from = sums + r * pitch;
+    T* to             = out + r * width;
+    for (int c = lane; c < width; c += 32 * U) {
+      float x[U];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float x = 0.f;
-      if (i + j < all)
-        for (int s = 0; s < splits; ++s) x += sums[(s * rows + r) * pitch + c];
-      v[j] = narrow<T>(x * f);
-      if (++c == width) {
-        c = 0;
-        ++r;
+      for (int u = 0; u < U; ++u) x[u] = c + 32 * u < width ? 0.f + __ldg(from + c + 32 * u) : 0.f;
+      for (int s = 1; s < splits; ++s) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (c + 32 * u < width) x[u] += __ldg(from + s * rows * pitch + c + 32 * u);
       }
-    }
-    if (i + 3 < all) {
-      *reinterpret_cast<uint2*>(out + i) = *reinterpret_cast<const uint2*>(v);
-    } else {
-      for (int j = 0; i + j < all; ++j) out[i + j] = v[j];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c + 32 * u < width) to[c + 32 * u] = narrow<T>(x[u] * f);
     }
   }
 }
@@ -977,9 +975,14 @@ __global__ void __launch_bounds__(kThreads) pad_rows(const T* from, int64_t stri
 {
   const int per     = pitch / 8;
   const int64_t all = rows * per;
+  const bool whole  = (reinterpret_cast<uintptr_t>(from) & 15) == 0 && stride % 8 == 0;  // pieces lie on 16 bytes
   for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < all; i += gridDim.x * static_cast<int64_t>(kThreads)) {
     const int64_t r = i / per;
     const int c     = static_cast<int>(i - r * per) * 8;
+    if (whole && c + 8 <= width) {
+      *reinterpret_cast<uint4*>(to + i * 8) = __ldg(reinterpret_cast<const uint4*>(from + r * stride + c));
+      continue;
+    }
     Piece<T> v;
 #pragma unroll
     for (int j = 0; j < 8; ++j) v.v[j] = c + j < width ? from[r * stride + c + j] : narrow<T>(0.f);
@@ -1043,19 +1046,25 @@ cudaError_t run_products(const Work& w, int n_sms, cudaStream_t s)
 // The kernels read 16 bytes at a time, rows that start on them and end with whole pieces.  Others are copied, with
 // zeros behind each row, which change no product; so are large ones off the 32-byte sectors, which are read a
 // quarter slower (4096 x 1032 x 16,384, loss and gradient: 501 us, with 1040 or 1024 columns 380).
+// Scores are copied for that from kCopyRows rows on, and to whole 128-byte lines.  (Kernels of scores and gradients as they are and
+// copied, us: 1999 x 712 x 50,001 545 and 605, 4096 x 1032 x 16,384 491 and 509, 8192 x 1032 x 16,384 943 and 919, 8192 x 2040 x 16,000
+// 1605 and 1545.  Lines or sectors, 1999 x 1001 x 50,001: 580 and 610 in the products.)
+constexpr int64_t kCopyRows = 6000;
 struct Layer {
   bool copied;
   int64_t width;         // of a row as the kernels read it
   int64_t bytes;         // of the copies
 };
 int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
-Layer layer_of(const LinearArgs& a)
+Layer layer_of(const LinearArgs& a, bool scores)
 {
   Layer l;
   l.copied = a.width % 8 || a.hidden_stride % 8 || a.weight_stride % 8 || reinterpret_cast<uintptr_t>(a.hidden) % 16 ||
              reinterpret_cast<uintptr_t>(a.weight) % 16 ||
-             ((a.width % 16 || a.hidden_stride % 16 || a.weight_stride % 16) && a.n_rows * a.n_cols >= (1ll << 36) / a.width);
-  l.width = l.copied ? (a.width + 15) / 16 * 16 : a.width;
+             ((a.width % 16 || a.hidden_stride % 16 || a.weight_stride % 16) && a.n_rows * a.n_cols >= (1ll << 36) / a.width &&
+              (!scores || a.n_rows >= kCopyRows));
+  const int64_t line = scores && a.width > 256 ? 64 : 16;
+  l.width = l.copied ? (a.width + line - 1) / line * line : a.width;
   l.bytes = l.copied ? padded(a.n_rows * l.width * 2) + padded(a.n_cols * l.width * 2) : 0;
   return l;
 }
@@ -1107,7 +1116,7 @@ cudaError_t run_linear(bool bf16, const LinearArgs& given, const Reduced& out, v
     return cudaGetLastError();
   }
   char* at      = static_cast<char*>(workspace);
-  cudaError_t e = give_layer<T>(a, layer_of(given), at, n_sms, s);
+  cudaError_t e = give_layer<T>(a, layer_of(given, false), at, n_sms, s);
   if (e != cudaSuccess) return e;
   double2* sums = reinterpret_cast<double2*>(at);
   Work w{};
@@ -1185,7 +1194,7 @@ cudaError_t finish(const float* sums, int splits, int64_t rows, int64_t pitch, i
     const int64_t need = (n / 4 + kThreads - 1) / kThreads;
     finish_sums<T><<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(sums, splits, n, scale, static_cast<T*>(out));
   } else {
-    const int64_t need = (n / 4 + kThreads) / kThreads;
+    const int64_t need = (rows + kThreads / 32 - 1) / (kThreads / 32);
     finish_rows<T><<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(
       sums, splits, rows, static_cast<int>(pitch), static_cast<int>(width), scale, static_cast<T*>(out));
   }
@@ -1199,7 +1208,7 @@ cudaError_t run_linear_score(bool bf16, const LinearScoreArgs& given, void* work
   if (given.layer.n_rows == 0) return cudaSuccess;
   LinearArgs a  = given.layer;
   char* at      = static_cast<char*>(workspace);
-  cudaError_t e = give_layer<T>(a, layer_of(given.layer), at, n_sms, s);
+  cudaError_t e = give_layer<T>(a, layer_of(given.layer, true), at, n_sms, s);
   if (e != cudaSuccess) return e;
   Work w{};
   w.products = 1;
@@ -1224,7 +1233,7 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, const ScoreUpstr
 {
   LinearArgs a        = g.fwd;
   const int64_t width = a.width;  // of the gradients' rows
-  const Layer layer   = layer_of(a);
+  const Layer layer   = layer_of(a, score != nullptr);
   const Plan plan     = plan_of(g, layer, n_sms);
   char* at            = static_cast<char*>(workspace);
   cudaError_t e       = give_layer<T>(a, layer, at, n_sms, s);
@@ -1339,19 +1348,23 @@ cudaError_t run_linear_grad(bool bf16, const LinearGradArgs& g, const ScoreUpstr
 
 size_t linear_workspace(const LinearArgs& a, int n_sms)
 {
-  return layer_of(a).bytes + (8 * n_sms + 1) * sizeof(double2) +
+  return layer_of(a, false).bytes + (8 * n_sms + 1) * sizeof(double2) +
          a.n_rows * static_cast<size_t>(2 * tiles_of(a.n_cols)) * sizeof(float2);
 }
 
-size_t linear_grad_workspace(const LinearGradArgs& g, int n_sms)
+namespace {
+size_t grad_workspace(const LinearGradArgs& g, bool scores, int n_sms)
 {
   const LinearArgs& a = g.fwd;
-  const Layer l       = layer_of(a);
+  const Layer l       = layer_of(a, scores);
   const Plan p        = plan_of(g, l, n_sms);
   return l.bytes + 256 + padded(a.n_rows * 4) + padded(p.planes * p.plane_rows * p.cols * 2) +
          (p.sums_hidden ? p.splits_hidden * a.n_rows * l.width * sizeof(float) : 0) +
          (p.sums_weight ? p.splits_weight * p.cols * l.width * sizeof(float) : 0);
 }
+}  // namespace
+
+size_t linear_grad_workspace(const LinearGradArgs& g, int n_sms) { return grad_workspace(g, false, n_sms); }
 
 cudaError_t launch_linear(int dtype, const LinearArgs& a, const Reduced& out, void* workspace, int n_sms, cudaStream_t s)
 {
@@ -1368,7 +1381,7 @@ cudaError_t launch_linear_grad(int dtype, const LinearGradArgs& g, void* workspa
 size_t linear_score_workspace(const LinearScoreArgs& a, int)
 {
   const LinearArgs& l = a.layer;
-  return layer_of(l).bytes + 256 + padded(l.n_rows * 4) + l.n_rows * static_cast<size_t>(2 * tiles_of(l.n_cols)) * sizeof(float4);
+  return layer_of(l, true).bytes + 256 + padded(l.n_rows * 4) + l.n_rows * static_cast<size_t>(2 * tiles_of(l.n_cols)) * sizeof(float4);
 }
 
 cudaError_t launch_linear_score(int dtype, const LinearScoreArgs& a, void* workspace, int n_sms, cudaStream_t s)
@@ -1390,7 +1403,7 @@ LinearGradArgs grad_of(const LinearScoreGradArgs& g)
 }
 }  // namespace
 
-size_t linear_score_grad_workspace(const LinearScoreGradArgs& g, int n_sms) { return linear_grad_workspace(grad_of(g), n_sms); }
+size_t linear_score_grad_workspace(const LinearScoreGradArgs& g, int n_sms) { return grad_workspace(grad_of(g), true, n_sms); }
 
 cudaError_t launch_linear_score_grad(int dtype, const LinearScoreGradArgs& g, void* workspace, int n_sms, cudaStream_t s)
 {
