@@ -141,7 +141,8 @@ struct ScoreArgs {
   float* top;          // (n_rows, k) their log probabilities
   int32_t* top_index;  // (n_rows, k)
 };
-// Scores with the best classes in one pass (distill_top.cu; workspace as for launch_top).
+// Scores with the best classes in one pass (distill_top.cu).
+size_t scored_top_workspace(int dtype, const ScoreArgs& a, int n_sms);
 cudaError_t launch_scored_top(int dtype, const ScoreArgs& a, void* workspace, int n_sms, cudaStream_t s);
 size_t score_workspace(int dtype, const ScoreArgs& a, int n_sms);
 cudaError_t launch_score(int dtype, const ScoreArgs& a, void* workspace, int n_sms, cudaStream_t s);

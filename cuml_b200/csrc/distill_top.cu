@@ -25,6 +25,8 @@
 // instead of 83; 1 x 50,001 fp32, k 20, 23.5 instead of 10.3; 1,000,003 x 10 fp32, k 3, 467 instead of 33.)
 #include <cooperative_groups.h>
 
+#include <algorithm>
+
 #include "score_common.cuh"
 
 namespace b2fil {
@@ -43,6 +45,10 @@ constexpr int kWarpTop  = 24;    // k up to which a warp finds its bound by its 
 // 1184 x 4096 bf16 14.8 and 12.8, x 8192 14.7 and 16.8.)
 constexpr int kLongBytes = 16384;
 constexpr int kLongLeast = 8;
+// Bytes of scored rows that a warp takes by groups, from kLongLeast rows per SM on, and twice that from twice as many on.  (By blocks and
+// this way, us: 20,000 x 3000 bf16 196 and 53, 4096 x 4096 fp32 43 and 23, 4096 x 8192 fp32 53 and 39, 4096 x 16,384 bf16 54 and 41, x
+// 32,768 78 and 75, 1300 x 16,384 22 and 26, x 8192 18 and 16.)
+constexpr int64_t kGroupBytes = 16384;
 constexpr int kCount    = 160;   // candidates of a block that are placed by counting; more are sorted
 constexpr int kCluster  = 8;     // blocks that share a row of up to kJoinCols and join their lists themselves
 constexpr int64_t kJoinCols = 1 << 17;  // (1 x 50,001, k 20: 13.8 us by two kernels, 10.7 this way, 14.2 by 16 blocks)
@@ -173,13 +179,17 @@ __device__ __forceinline__ void write_scored(const ScoredTopArgs& a, int64_t row
   a.index[row * a.k + j] = score.counts ? static_cast<int32_t>(key.index()) : -1;
 }
 // A row that does not count, by `threads` threads.
-__device__ __forceinline__ void write_uncounted(const ScoredTopArgs& a, int64_t row, int tid, int threads)
+__device__ __forceinline__ void write_uncounted_top(const ScoredTopArgs& a, int64_t row, int tid, int threads)
 {
-  if (tid == 0) finish_score(a.out, row, Scored(), a.temperature.inverse, -2, 0.f);
   for (int j = tid; j < a.k; j += threads) {
     a.top[row * a.k + j]   = 0.f;
     a.index[row * a.k + j] = -1;
   }
+}
+__device__ __forceinline__ void write_uncounted(const ScoredTopArgs& a, int64_t row, int tid, int threads)
+{
+  if (tid == 0) finish_score(a.out, row, Scored(), a.temperature.inverse, -2, 0.f);
+  write_uncounted_top(a, row, tid, threads);
 }
 // Scores of a row: written by one thread, known to all that call.
 template <class T>
@@ -929,7 +939,7 @@ __global__ void __launch_bounds__(kThreads, warps_fit(U * 16 / sizeof(T) * sizeo
 // bit by bit as in top_segments.  (A bound by values alone took 5.7 ms where all but five of 4096 scores of 8192 rows
 // were -inf.)
 template <class T, int MODE>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(ArgsOf<MODE> a)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(TopArgs a)
 {
   using V = typename ValueOf<T>::type;
   using K = typename KeyOf<T>::type;
@@ -945,40 +955,20 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(Arg
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / 32; row < a.n_rows;
        row += static_cast<int64_t>(gridDim.x) * ROWS) {
     const T* x = static_cast<const T*>(a.scores) + row * a.row_stride;
-    int given  = -1;
-    if constexpr (MODE == kScored) {
-      given = target_of(a.target, row, a.n_cols);
-      if (given == -2) {
-        write_uncounted(a, row, lane, 32);
-        continue;
-      }
-    }
     // the lane's best score, the first element of the piece that holds it, and the sum
     V best      = lowest<V>();
     uint32_t at = ~0u;
-    typename StreamOf<T, MODE>::type sum;
-    const V slack = static_cast<V>(kSlack) / c;
+    auto sum    = new_sum<V, MODE>(c);
     visit_row<2 * kInFlight>(
       x, a.n_cols, lane, 32,
       [&](int64_t i, T e) {
         const V v = widen(e);
         if (v > best || at == ~0u) at = static_cast<uint32_t>(i);
         best      = larger(best, v);
-        if constexpr (MODE == kScored) {
-          sum.take(v, c, slack);
-        } else {
-          sum.reach(v, c, plain);
-          sum.add(v, c, plain);
-        }
+        sum.reach(v, c, plain);
+        sum.add(v, c, plain);
       },
       [&](int64_t i, const Piece<T>& p) {
-        if constexpr (MODE == kScored) {
-          const V most = largest_of(p);
-          if (most > best || at == ~0u) at = static_cast<uint32_t>(i);
-          best = larger(best, most);
-          sum.take(p, most, c, slack);
-          return;
-        }
         V v[N], most;
 #pragma unroll
         for (int e = 0; e < N; ++e) v[e] = widen(p.v[e]);
@@ -987,21 +977,14 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(Arg
         for (int e = 1; e < N; ++e) most = larger(most, v[e]);
         if (most > best || at == ~0u) at = static_cast<uint32_t>(i);
         best = larger(best, most);
-        if constexpr (MODE != kScored) {
-          sum.reach(most, c, plain);
+        sum.reach(most, c, plain);
 #pragma unroll
-          for (int e = 0; e < N; ++e) sum.add(v[e], c, plain);
-        }
+        for (int e = 0; e < N; ++e) sum.add(v[e], c, plain);
       });
     double dropped = 0;
     Running<V> all;
     all.m = V(0);
-    Scored scored;
-    if constexpr (MODE == kScored) {
-      scored = sum.scored(c);
-      scored.join_lanes(c);
-      if (!sum.usable(scored.m, c)) scored = score_any<T, 32>(x, a.n_cols, lane, c, nullptr);
-    } else if (plain) {
+    if (plain) {
       dropped = sum_lanes(static_cast<double>(sum.s) + sum.dropped);
     } else {
       all.m = sum.first ? lowest<V>() : sum.r;
@@ -1065,14 +1048,175 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(Arg
 #pragma unroll 4
       for (int j = 0; j < got; ++j) place += list[j].above(key);
       if (place >= k) continue;
-      if constexpr (MODE == kScored) {
-        write_scored(a, row, place, key, scored.m, score_row(a, row, x, scored, given, place == 0));
-      } else {
-        write_top<T>(a, row, place, key);
-        if (place == 0) write_lse(a, row, all.m, all.s, dropped, key);
-      }
+      write_top<T>(a, row, place, key);
+      if (place == 0) write_lse(a, row, all.m, all.s, dropped, key);
     }
     __syncwarp();
+  }
+}
+
+// The best classes of a scored row from the largest of kBestGroups groups of its pieces, kGroups of a lane: group g of lane l is
+// l + 32 g.  By a warp; k <= kWarpTop.  A value tau that k of them reach is found by votes, and only the groups that reach it
+// are read again.  Where that is more than the list holds, what is above tau is taken, and of its equals (a mask, for
+// instance) the first of the row.
+constexpr int kBestGroups = 256, kGroups = kBestGroups / 32;
+struct GroupRoom {
+  Key32 list[kWarpList];
+  uint8_t chosen[kBestGroups];
+  int count;
+};
+template <class T, class F>
+__device__ __forceinline__ void best_of_groups(const T* x, int n, int k, const float (&best)[kGroups], bool nan, GroupRoom& room, F put)
+{
+  constexpr int N = Piece<T>::N, R = kBestGroups;
+  using K = Key32;
+  const int lane       = threadIdx.x % 32;
+  const unsigned below = (1u << lane) - 1;
+  const int lead = lead_of(x, n), pieces = (n - lead) / N, behind = lead + pieces * N + lane;
+  // the elements before the first and behind the last boundary are looked at whatever they are
+  const float before = lane < lead ? widen(x[lane]) : 0.f, after = behind < n ? widen(x[behind]) : 0.f;
+  uint32_t o[kGroups], tau = 0;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) o[g] = ordered(best[g]);
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t next = tau | 1u << bit;
+    int some            = 0;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) some += o[g] >= next;
+    some = __reduce_add_sync(~0u, some);
+    if (some < k) continue;
+    tau = next;
+    if (some <= k + kMore) break;
+  }
+  int reached_by = 0;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    const unsigned all = __ballot_sync(~0u, o[g] >= tau);
+    if (o[g] >= tau) room.chosen[reached_by + __popc(all & below)] = static_cast<uint8_t>(g * 32 + lane);
+    reached_by += __popc(all);
+  }
+  __syncwarp();
+  // Puts those of the reached groups, or of the whole row, whose keys are `bound` or above into the list; how many there are, or
+  // that there are more than it holds.
+  auto collect = [&](const K& bound, bool whole) {
+    volatile int* count = &room.count;
+    __syncwarp();
+    if (lane == 0) *count = 0;
+    __syncwarp();
+    auto take = [&](int i, float v) {
+      const K key = K::of(v, static_cast<uint32_t>(i));
+      if (bound.above(key)) return;
+      const int to = atomicAdd(&room.count, 1);
+      if (to < kWarpList) room.list[to] = key;
+    };
+    const float least = bound.value();  // (NaN is not below)
+    const int rounds = (pieces + R - 1) / R, all = whole ? pieces : reached_by * rounds;
+    for (int i = lane; i - lane < all; i += 32) {
+      if (__any_sync(~0u, *count > kWarpList)) break;
+      const int p = i >= all ? pieces : whole ? i : room.chosen[i / rounds] + i % rounds * R;
+      if (p >= pieces) continue;
+      float v[N];
+      numbers_of(piece_of<T>(__ldg(reinterpret_cast<const uint4*>(x + lead + static_cast<int64_t>(p) * N))), v);
+      uint32_t some = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e) some |= !(v[e] < least) ? 1u << e : 0u;
+      for (; some; some &= some - 1) {
+        const int e = lead + p * N + __ffs(some) - 1;
+        take(e, widen(x[e]));
+      }
+    }
+    if (lane < lead) take(lane, before);
+    if (behind < n) take(behind, after);
+    __syncwarp();
+    return *count;
+  };
+  int got = nan ? kWarpList + 1 : collect(K{static_cast<uint64_t>(tau) << 32}, false);
+  if (got > kWarpList && !nan) {
+    got = tau == ~0u ? 0 : collect(K{static_cast<uint64_t>(tau + 1) << 32}, false);
+    // equals of tau, in the order of their classes
+    for (int first = 0; first < n && got < k; first += 32) {
+      const int i        = first + lane;
+      const bool is      = i < n && ordered(widen(x[i])) == tau;
+      const unsigned all = __ballot_sync(~0u, is);
+      if (is) room.list[got + __popc(all & below)] = K::of(widen(x[i]), static_cast<uint32_t>(i));
+      got += __popc(all);
+    }
+    __syncwarp();
+  }
+  if (got > kWarpList) {  // NaN, or many above tau in few groups: the k-th key bit by bit
+    K bound = K::none();
+    for (int bit = K::kBits - 1; bit >= 0 && got > kWarpList; --bit) {
+      const K next   = bound.with(bit);
+      const int some = collect(next, true);
+      if (some < k) continue;
+      bound = next;
+      got   = some;
+    }
+  }
+  for (int i = lane; i < got; i += 32) {
+    const K key = room.list[i];
+    int place   = 0;
+#pragma unroll 4
+    for (int j = 0; j < got; ++j) place += room.list[j].above(key);
+    if (place < k) put(place, key);
+  }
+  __syncwarp();
+}
+
+// A scored row per warp, of more than kWarpCols elements.
+constexpr int kGroupThreads = 128;  // (small blocks: few rows are spread evenly over the SMs)
+constexpr int kGroupBlocks  = 8;    // of an SM, all there at once
+template <class T>
+__global__ void __launch_bounds__(kGroupThreads, kGroupBlocks) top_groups(ScoredTopArgs a)
+{
+  constexpr int N = Piece<T>::N, ROWS = kGroupThreads / 32, U = kInFlight, R = kBestGroups;
+  __shared__ GroupRoom rooms[ROWS];
+  const int lane = threadIdx.x % 32, n = static_cast<int>(a.n_cols);
+  const float c  = a.temperature.c, slack = kSlack / c;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / 32; row < a.n_rows;
+       row += static_cast<int64_t>(gridDim.x) * ROWS) {
+    const T* x      = static_cast<const T*>(a.scores) + row * a.row_stride;
+    const int given = target_of(a.target, row, a.n_cols);
+    if (given == -2) {
+      write_uncounted(a, row, lane, 32);
+      continue;
+    }
+    const int lead = lead_of(x, n), pieces = (n - lead) / N, behind = lead + pieces * N + lane;
+    const T* body  = x + lead;
+    PairedStream<T> sum;
+    float best[kGroups];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) best[g] = lowest<float>();
+    for (int first = lane; first - lane < pieces; first += R) {
+      const bool full = first - lane + R <= pieces;
+#pragma unroll
+      for (int h = 0; h < kGroups; h += U) {
+        Piece<T> r[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (full || first + (h + u) * 32 < pieces)
+            r[u] = piece_of<T>(__ldg(reinterpret_cast<const uint4*>(body + static_cast<int64_t>(first + (h + u) * 32) * N)));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (!full && first + (h + u) * 32 >= pieces) continue;
+          const float most = largest_of(r[u]);
+          best[h + u]      = fmaxf(best[h + u], most);
+          sum.take(r[u], most, c, slack);
+        }
+      }
+    }
+    sum.take(lane < lead ? widen(x[lane]) : lowest<float>(), behind < n ? widen(x[behind]) : lowest<float>(), c, slack);
+    const bool nan = __any_sync(~0u, is_nan(sum));  // (or an infinite one)
+    Scored scored  = sum.scored(c);
+    scored.join_lanes(c);
+    if (!sum.usable(scored.m, c)) scored = score_any<T, 32>(x, a.n_cols, lane, c, nullptr);
+    if (scored.s == 0.f) {
+      write_uncounted(a, row, lane, 32);
+      continue;
+    }
+    best_of_groups(x, n, a.k, best, nan, rooms[threadIdx.x / 32], [&](int place, const Key32& key) {
+      write_scored(a, row, place, key, scored.m, score_row(a, row, x, scored, given, place == 0));
+    });
   }
 }
 
@@ -1230,6 +1374,13 @@ cudaError_t run_warps(const A& a, int n_sms, cudaStream_t s)
   return cudaGetLastError();
 }
 
+// Scored rows by a warp each.
+bool by_groups(int64_t n_rows, int64_t n_cols, int k, int element, int n_sms)
+{
+  const int64_t bytes = n_cols * element, per = n_rows / n_sms;
+  return n_cols > kWarpCols && k <= kWarpTop && ((bytes <= kGroupBytes && per >= kLongLeast) || (bytes <= 2 * kGroupBytes && per >= 2 * kLongLeast));
+}
+
 template <class T, class A>
 cudaError_t run_top(const A& a, void* workspace, int n_sms, cudaStream_t s)
 {
@@ -1257,14 +1408,16 @@ cudaError_t run_top(const A& a, void* workspace, int n_sms, cudaStream_t s)
   if constexpr (sizeof(T) < 8) {
     if (a.n_cols <= kWarpCols && a.k <= kWarpTop) return run_warps<T, 4 * kPieces, 0>(a, n_sms, s);
   }
-  if (bytes <= kLongBytes && a.k <= kWarpTop && a.n_rows >= static_cast<int64_t>(kLongLeast) * n_sms) {
+  if constexpr (kIsScored) {
+    const int64_t blocks = std::min<int64_t>((a.n_rows + kGroupThreads / 32 - 1) / (kGroupThreads / 32), kGroupBlocks * n_sms);
+    if (by_groups(a.n_rows, a.n_cols, a.k, sizeof(T), n_sms)) {
+      top_groups<T><<<static_cast<unsigned>(blocks), kGroupThreads, 0, s>>>(a);
+      count_launches(1);
+      return cudaGetLastError();
+    }
+  } else if (bytes <= kLongBytes && a.k <= kWarpTop && a.n_rows >= static_cast<int64_t>(kLongLeast) * n_sms) {
     const int64_t need = (a.n_rows + kThreads / 32 - 1) / (kThreads / 32), most = 16ll * n_sms;
-    const auto kernel  = [&] {
-      if constexpr (kIsScored)
-        return top_long<T, kScored>;
-      else
-        return kernel_of(a, top_long<T, kScores>, top_long<T, kProbabilities>);
-    }();
+    const auto kernel  = kernel_of(a, top_long<T, kScores>, top_long<T, kProbabilities>);
     kernel<<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(a);
     count_launches(1);
     return cudaGetLastError();
@@ -1325,6 +1478,16 @@ cudaError_t launch_top(int dtype, const TopArgs& a, void* workspace, int n_sms, 
     case kF16: return run_top<__half>(a, workspace, n_sms, s);
   }
   return cudaErrorInvalidValue;
+}
+
+size_t scored_top_workspace(int dtype, const ScoreArgs& a, int n_sms)
+{
+  if (by_groups(a.n_rows, a.n_cols, a.k, dtype == kF32 ? 4 : 2, n_sms)) return 0;
+  TopArgs t{};
+  t.n_rows = a.n_rows;
+  t.n_cols = a.n_cols;
+  t.k      = a.k;
+  return top_workspace(dtype, t, n_sms);
 }
 
 cudaError_t launch_scored_top(int dtype, const ScoreArgs& g, void* workspace, int n_sms, cudaStream_t s)

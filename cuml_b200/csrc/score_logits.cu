@@ -20,9 +20,12 @@ constexpr int kInFlight = 4;     // pieces of a thread
 constexpr int kRowBlocks  = 5;
 constexpr int kWarpBlocks = 4;
 constexpr int kGradBlocks = 4;
-// Bytes of a row that is worth a block's start.  (Gradient of 4096 x 131,072 bf16: 319 us, 345 with ten blocks of an SM that take several;
-// 4096 x 8192 fp32: 38 us with a block for each row, 32 so.)
-constexpr int64_t kLongRow = 1 << 16;
+// Bytes of a row that is worth a block's start, and of one of the gradient's.  (us with a block for each row and with those that are there
+// at once taking several: 4096 x 131,072 bf16 184 and 191, gradient 319 and 345; x 32,768 66 and 58, gradient 78 and 83; 4096 x 8192
+// fp32 38 and 32.  Copies to shared memory ahead of the sums, the next row's among them, made the warps of a block drift apart:
+// 191 and 66.)
+constexpr int64_t kLongRow     = 1 << 17;
+constexpr int64_t kLongGradRow = 1 << 16;
 // Where there are kWarpLeast rows per SM, a warp takes longer ones, too: whose logits take up to kWarpBytes, and in the
 // gradient, of 16 bits, up to kWarpLong.  (20,000 x 3000 bf16, both passes: 96 and 66 us by blocks, 34 and 43 so.)
 constexpr int kWarpLeast = 8;
@@ -309,10 +312,10 @@ bool by_warps(const ScoreArgs& a, int n_sms, bool longer)
   return a.n_cols <= kWarpCols || (longer && a.n_rows >= static_cast<int64_t>(kWarpLeast) * n_sms);
 }
 // Blocks of a launch: a block for each long row, else as many as are there at once.
-unsigned row_blocks(const ScoreArgs& a, bool warp, int element, int64_t at_once)
+unsigned row_blocks(const ScoreArgs& a, bool warp, int element, int64_t at_once, int64_t long_row)
 {
   if (warp) return blocks_of((a.n_rows + kThreads / 32 - 1) / (kThreads / 32), at_once);
-  return blocks_of(a.n_rows, a.n_cols * element >= kLongRow ? 1 << 30 : at_once);
+  return blocks_of(a.n_rows, a.n_cols * element >= long_row ? 1 << 30 : at_once);
 }
 bool by_tiles(const ScoreArgs& a, int n_sms) { return a.n_cols <= kTileCols && a.n_rows >= static_cast<int64_t>(kTileLeast) * n_sms; }
 template <class T, class A>
@@ -339,9 +342,9 @@ cudaError_t run_score(const ScoreArgs& a, void* workspace, int n_sms, cudaStream
     return cudaGetLastError();
   }
   if (by_warps(a, n_sms, a.n_cols * sizeof(T) <= kWarpBytes))
-    score_rows<T, 32><<<row_blocks(a, true, sizeof(T), kWarpBlocks * n_sms), kThreads, 0, s>>>(a);
+    score_rows<T, 32><<<row_blocks(a, true, sizeof(T), kWarpBlocks * n_sms, kLongRow), kThreads, 0, s>>>(a);
   else
-    score_rows<T, kThreads><<<row_blocks(a, false, sizeof(T), kRowBlocks * n_sms), kThreads, 0, s>>>(a);
+    score_rows<T, kThreads><<<row_blocks(a, false, sizeof(T), kRowBlocks * n_sms, kLongRow), kThreads, 0, s>>>(a);
   count_launches(1);
   return cudaGetLastError();
 }
@@ -352,7 +355,7 @@ cudaError_t run_grad(const ScoreGradArgs& g, int n_sms, cudaStream_t s)
   const ScoreArgs& a = g.fwd;
   if (by_tiles(a, n_sms)) return run_tiles<T>(grad_tiles<T>, g, a, n_sms, s);
   const bool warp    = by_warps(a, n_sms, sizeof(T) == 2 && a.n_cols <= kWarpLong);
-  const unsigned rows = row_blocks(a, warp, sizeof(T), kGradBlocks * n_sms);
+  const unsigned rows = row_blocks(a, warp, sizeof(T), kGradBlocks * n_sms, kLongGradRow);
   int segs           = warp ? 1 : segments(a.n_rows, a.n_cols, n_sms);
   const int64_t cols = part_cols(a.n_cols, segs);
   segs               = segs == 1 ? 1 : static_cast<int>((a.n_cols + cols - 1) / cols);
@@ -369,11 +372,7 @@ cudaError_t run_grad(const ScoreGradArgs& g, int n_sms, cudaStream_t s)
 size_t score_workspace(int dtype, const ScoreArgs& a, int n_sms)
 {
   if (a.k > 0) {
-    TopArgs t{};
-    t.n_rows = a.n_rows;
-    t.n_cols = a.n_cols;
-    t.k      = a.k;
-    return top_workspace(dtype, t, n_sms);
+    return scored_top_workspace(dtype, a, n_sms);
   }
   const int segs = segments(a.n_rows, a.n_cols, n_sms);
   return segs > 1 ? a.n_rows * segs * sizeof(float4) : 0;
