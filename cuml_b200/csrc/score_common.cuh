@@ -65,6 +65,24 @@ struct Scored {
     s = sum_lanes(s);
     u = sum_lanes(u);
   }
+  // The same for every LANES lanes of a warp.
+  template <int LANES>
+  __device__ __forceinline__ void join_some(float c)
+  {
+    if (LANES == 32) {
+      join_lanes(c);
+      return;
+    }
+    float to = m;
+#pragma unroll
+    for (int d = LANES / 2; d; d >>= 1) to = fmaxf(to, __shfl_xor_sync(~0u, to, d));
+    if (to != lowest<float>()) move(to, c);
+#pragma unroll
+    for (int d = LANES / 2; d; d >>= 1) {
+      s += __shfl_xor_sync(~0u, s, d);
+      u += __shfl_xor_sync(~0u, u, d);
+    }
+  }
 };
 
 // The same for a stream of pieces: `limit` is m + slack.

@@ -11,6 +11,10 @@ namespace {
 
 constexpr int kThreads  = 256;
 constexpr int kWarpCols = 2048;  // rows that belong to one warp
+// ... or, up to kSubCols, to eight lanes of one.  (Both passes, us, by warps and by eight lanes: 200,000 x 100 fp32 59, 53 and 28, 27; 100,000 x
+// 200 bf16 33, 31 and 19, 18; 60,000 x 500 bf16 31, 29 and 24, 20; x 1000 equal.)
+constexpr int kSubCols    = 512;
+constexpr int kSubThreads = 8;
 constexpr int kSegment  = 8192;  // fewest elements of a row that are worth a block of their own
 constexpr int kMostSegs = 64;
 constexpr int kInFlight = 4;     // pieces of a thread
@@ -110,52 +114,102 @@ __global__ void __launch_bounds__(kThreads) score_join(ScoreArgs a, int segs, co
   }
 }
 
-// Rows by THREADS threads.  What a row takes besides its logits is done for 32 of them at a time, a lane each: the given
+// Rows by a block each.  What a row takes besides its logits is done for 32 of them at a time, a lane each: the given
 // classes before, the scores behind.  The warps of a block go through the rows on their own.
-template <class T, int THREADS>
-__global__ void __launch_bounds__(kThreads, THREADS == 32 ? kWarpBlocks : kRowBlocks) score_rows(ScoreArgs a)
+template <class T>
+__global__ void __launch_bounds__(kThreads, kRowBlocks) score_blocks(ScoreArgs a)
 {
-  constexpr int ROWS = kThreads / THREADS, W = THREADS / 32;
+  constexpr int W = kThreads / 32;
   __shared__ float room[3 * W];
-  __shared__ float parts[W > 1 ? 32 * W * 3 : 1];
-  const int tid = threadIdx.x % THREADS, lane = threadIdx.x % 32, warp = tid / 32;
+  __shared__ float parts[32 * W * 3];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const float c      = a.temperature.c;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS;
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / THREADS; row0 < a.n_rows; row0 += 32 * step) {
+  const int64_t step = gridDim.x;
+  for (int64_t row0 = blockIdx.x; row0 < a.n_rows; row0 += 32 * step) {
     const int count = static_cast<int>(min(static_cast<int64_t>(32), (a.n_rows - row0 + step - 1) / step));
     auto logits     = [&](int j) { return static_cast<const T*>(a.logits) + (row0 + j * step) * a.row_stride; };
     const int at    = lane < count ? target_of(a.target, row0 + lane * step, a.n_cols) : -2;
-    Scored mine;  // of the lane's row
     for (int j = 0; j < count; ++j) {
       if (__shfl_sync(~0u, at, j) == -2) continue;  // not read
-      Scored r = visit_ordinary(logits(j), static_cast<int>(a.n_cols), tid, THREADS, c);
+      Scored r = visit_ordinary(logits(j), static_cast<int>(a.n_cols), threadIdx.x, kThreads, c);
       r.join_lanes(c);
-      if (W == 1) {
-        if (lane == j) mine = r;
-      } else if (lane == 0) {
+      if (lane == 0) {
         float* p = parts + (j * W + warp) * 3;
         p[0]     = r.m;
         p[1]     = r.s;
         p[2]     = r.u;
       }
     }
-    if (W > 1) {
-      __syncthreads();
-      if (at != -2) {
-        for (int w = 0; w < W; ++w) {
-          const float* p = parts + (lane * W + w) * 3;
-          mine.join(p[0], p[1], p[2], c);
-        }
+    __syncthreads();
+    Scored mine;  // of the lane's row
+    if (at != -2) {
+      for (int w = 0; w < W; ++w) {
+        const float* p = parts + (lane * W + w) * 3;
+        mine.join(p[0], p[1], p[2], c);
       }
     }
     for (unsigned again = __ballot_sync(~0u, at != -2 && !PairedStream<T>::usable(mine.m, c)); again; again &= again - 1) {
       const int j    = __ffs(again) - 1;
-      const Scored r = visit_any<T, THREADS>(logits(j), a.n_cols, tid, c, room);
+      const Scored r = visit_any<T, kThreads>(logits(j), a.n_cols, threadIdx.x, c, room);
       if (lane == j) mine = r;
     }
     if (lane < count && warp == 0)
       finish_score(a.out, row0 + lane * step, mine, a.temperature.inverse, at, at >= 0 ? widen(logits(lane)[at]) : 0.f);
-    if (W > 1) __syncthreads();  // `parts` has been read
+    __syncthreads();  // `parts` has been read
+  }
+}
+
+// The rows of a warp, which takes 32 / THREADS of them at a time, or of a block: those that are read at a time lie next to one
+// another.  row(j): the j-th of 32.
+template <int THREADS>
+struct RowOrder {
+  static constexpr int kAtOnce = THREADS < 32 ? 32 / THREADS : 1;
+  static constexpr int kPer    = THREADS > 32 ? 1 : kThreads / 32;
+  int64_t slot = static_cast<int64_t>(blockIdx.x) * kPer + (THREADS > 32 ? 0 : threadIdx.x / 32);
+  static __device__ __forceinline__ int64_t slots() { return static_cast<int64_t>(gridDim.x) * kPer; }
+  __device__ __forceinline__ int64_t row(int j) const { return (slot + j / kAtOnce * slots()) * kAtOnce + j % kAtOnce; }
+  __device__ __forceinline__ void next() { slot += 32 / kAtOnce * slots(); }
+};
+
+// The same by a warp, or eight lanes, each.
+template <class T, int THREADS>
+__global__ void __launch_bounds__(kThreads, kWarpBlocks) score_rows(ScoreArgs a)
+{
+  const int tid = threadIdx.x % THREADS, lane = threadIdx.x % 32;
+  const float c = a.temperature.c;
+  using Order   = RowOrder<THREADS>;
+  constexpr int kAtOnce = Order::kAtOnce;
+  for (Order rows; rows.row(0) < a.n_rows; rows.next()) {
+    auto logits  = [&](int j) { return static_cast<const T*>(a.logits) + rows.row(j) * a.row_stride; };
+    const int at = rows.row(lane) < a.n_rows ? target_of(a.target, rows.row(lane), a.n_cols) : -2;
+    Scored mine;  // of the lane's row
+    for (int first = 0; first < 32 && rows.row(first) < a.n_rows; first += kAtOnce) {
+      const int j       = first + (kAtOnce > 1 ? lane / THREADS : 0);
+      const bool counts = __shfl_sync(~0u, at, j) != -2;  // (else not read)
+      if (kAtOnce == 1 && !counts) continue;
+      Scored r = visit_ordinary(logits(j), counts ? static_cast<int>(a.n_cols) : 0, tid, THREADS, c);
+      __syncwarp();
+      r.join_some<THREADS>(c);
+      if (kAtOnce == 1) {
+        if (lane == j) mine = r;
+        continue;
+      }
+      // to the lanes whose rows they are
+      const int from = lane % kAtOnce * THREADS;
+      const float m = __shfl_sync(~0u, r.m, from), s = __shfl_sync(~0u, r.s, from), u = __shfl_sync(~0u, r.u, from);
+      if (lane - lane % kAtOnce == first) {
+        mine.m = m;
+        mine.s = s;
+        mine.u = u;
+      }
+    }
+    for (unsigned again = __ballot_sync(~0u, at != -2 && !PairedStream<T>::usable(mine.m, c)); again; again &= again - 1) {
+      const int j    = __ffs(again) - 1;
+      const Scored r = visit_any<T, 32>(logits(j), a.n_cols, lane, c, nullptr);
+      if (lane == j) mine = r;
+    }
+    if (rows.row(lane) < a.n_rows)
+      finish_score(a.out, rows.row(lane), mine, a.temperature.inverse, at, at >= 0 ? widen(logits(lane)[at]) : 0.f);
   }
 }
 
@@ -233,36 +287,38 @@ __device__ __forceinline__ void zero_row(T* row, int64_t n, int tid, int threads
 template <class T, int THREADS>
 __global__ void __launch_bounds__(kThreads, kGradBlocks) score_grad(ScoreGradArgs g, int64_t seg_cols)
 {
-  constexpr int ROWS = kThreads / THREADS, N = Piece<T>::N;
+  constexpr int N    = Piece<T>::N;
   const ScoreArgs& a = g.fwd;
   const int tid = threadIdx.x % THREADS, lane = threadIdx.x % 32;
+  using Order   = RowOrder<THREADS>;
+  constexpr int kAtOnce = Order::kAtOnce;
   const float c       = a.temperature.c, inv_t = static_cast<float>(a.temperature.inverse);
   const int64_t begin = blockIdx.y * seg_cols;
   const int n         = static_cast<int>(min(seg_cols, a.n_cols - begin));
-  const int64_t step  = static_cast<int64_t>(gridDim.x) * ROWS;
   const ScoreUpstream& up = g.upstream;
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / THREADS; row0 < a.n_rows; row0 += 32 * step) {
-    const int count = static_cast<int>(min(static_cast<int64_t>(32), (a.n_rows - row0 + step - 1) / step));
+  for (Order rows; rows.row(0) < a.n_rows; rows.next()) {
     RowGrad mine{};
-    if (lane < count) {
-      const int64_t row = row0 + lane * step;
+    if (rows.row(lane) < a.n_rows) {
+      const int64_t row = rows.row(lane);
       mine = row_grad(a.out.kept[row], up.log_prob ? up.log_prob[row * up.log_prob_stride] * inv_t : 0.f,
                       up.entropy ? up.entropy[row * up.entropy_stride] * inv_t : 0.f);
       if (!mine.counts) mine.at = -2;
     }
-    for (int j = 0; j < count; ++j) {
-      const T* x = static_cast<const T*>(a.logits) + (row0 + j * step) * a.row_stride + begin;
-      T* d       = static_cast<T*>(g.grad) + (row0 + j * step) * g.grad_stride + begin;
+    for (int first = 0; first < 32 && rows.row(first) < a.n_rows; first += kAtOnce) {
+      const int j = first + (kAtOnce > 1 ? lane / THREADS : 0);
       RowGrad r;
-      r.at = __shfl_sync(~0u, mine.at, j);
-      if (r.at == -2) {
-        zero_row(d, n, tid, THREADS);
-        continue;
-      }
+      r.at   = __shfl_sync(~0u, mine.at, j);
       r.base = __shfl_sync(~0u, mine.base, j);
       r.A    = __shfl_sync(~0u, mine.A, j);
       r.B    = __shfl_sync(~0u, mine.B, j);
       r.add  = __shfl_sync(~0u, mine.add, j);
+      if (kAtOnce > 1 && rows.row(j) >= a.n_rows) continue;
+      const T* x = static_cast<const T*>(a.logits) + rows.row(j) * a.row_stride + begin;
+      T* d       = static_cast<T*>(g.grad) + rows.row(j) * g.grad_stride + begin;
+      if (r.at == -2) {
+        zero_row(d, n, tid, THREADS);
+        continue;
+      }
       const int at = r.at >= begin && r.at - begin < n ? static_cast<int>(r.at - begin) : -1;
       auto one     = [&](int i, T v) { d[i] = narrow<T>(r(widen(v), c) + (i == at ? r.add : 0.f)); };
       if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0) {
@@ -314,7 +370,8 @@ bool by_warps(const ScoreArgs& a, int n_sms, bool longer)
 // Blocks of a launch: a block for each long row, else as many as are there at once.
 unsigned row_blocks(const ScoreArgs& a, bool warp, int element, int64_t at_once, int64_t long_row)
 {
-  if (warp) return blocks_of((a.n_rows + kThreads / 32 - 1) / (kThreads / 32), at_once);
+  const int per = kThreads / (a.n_cols <= kSubCols ? kSubThreads : 32);
+  if (warp) return blocks_of((a.n_rows + per - 1) / per, at_once);
   return blocks_of(a.n_rows, a.n_cols * element >= long_row ? 1 << 30 : at_once);
 }
 bool by_tiles(const ScoreArgs& a, int n_sms) { return a.n_cols <= kTileCols && a.n_rows >= static_cast<int64_t>(kTileLeast) * n_sms; }
@@ -341,10 +398,12 @@ cudaError_t run_score(const ScoreArgs& a, void* workspace, int n_sms, cudaStream
     count_launches(2);
     return cudaGetLastError();
   }
-  if (by_warps(a, n_sms, a.n_cols * sizeof(T) <= kWarpBytes))
+  if (a.n_cols <= kSubCols)
+    score_rows<T, kSubThreads><<<row_blocks(a, true, sizeof(T), kWarpBlocks * n_sms, kLongRow), kThreads, 0, s>>>(a);
+  else if (by_warps(a, n_sms, a.n_cols * sizeof(T) <= kWarpBytes))
     score_rows<T, 32><<<row_blocks(a, true, sizeof(T), kWarpBlocks * n_sms, kLongRow), kThreads, 0, s>>>(a);
   else
-    score_rows<T, kThreads><<<row_blocks(a, false, sizeof(T), kRowBlocks * n_sms, kLongRow), kThreads, 0, s>>>(a);
+    score_blocks<T><<<row_blocks(a, false, sizeof(T), kRowBlocks * n_sms, kLongRow), kThreads, 0, s>>>(a);
   count_launches(1);
   return cudaGetLastError();
 }
@@ -359,7 +418,9 @@ cudaError_t run_grad(const ScoreGradArgs& g, int n_sms, cudaStream_t s)
   int segs           = warp ? 1 : segments(a.n_rows, a.n_cols, n_sms);
   const int64_t cols = part_cols(a.n_cols, segs);
   segs               = segs == 1 ? 1 : static_cast<int>((a.n_cols + cols - 1) / cols);
-  if (warp)
+  if (a.n_cols <= kSubCols)
+    score_grad<T, kSubThreads><<<rows, kThreads, 0, s>>>(g, cols);
+  else if (warp)
     score_grad<T, 32><<<rows, kThreads, 0, s>>>(g, cols);
   else
     score_grad<T, kThreads><<<dim3(rows, segs), kThreads, 0, s>>>(g, cols);
