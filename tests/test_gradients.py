@@ -249,6 +249,11 @@ def test_not_finite_and_out_of_the_usual_range(kind):
             norm = float(norm_of(tensors, kind))
             if norm < 3e38:
                 check_clip(tensors, norm / 2, kind)
+    # a norm that 32 bits do not hold is infinite to its caller, and changes nothing
+    large = [torch.full((1000,), 3e38, device="cuda") for _ in range(2)]
+    norm = distill.clip_gradients(large, 1.0, norm_type=kind)
+    if kind != math.inf:
+        assert norm == float("inf") and all((x == 3e38).all() for x in large)
     mixed = made([(5000,), (5000,)], ["fp32"], 2, 1.0)
     mixed[0].mul_(1e-25)
     mixed[1][::2] = 1e20
@@ -319,6 +324,39 @@ def test_captured_and_replayed():
             want = distill.clip_gradients(values, 0.001)
             assert torch.equal(norm, want) and all(torch.equal(x, y) for x, y in zip(held, values))
         del graph
+
+
+@gpu
+def test_more_strided_tensors_than_a_launch_takes():
+    """600 columns of a matrix, between flat tensors, and a view of five dimensions none of which are neighbours."""
+    base = made([(700, 601), (40_000,), (6, 5, 8, 9, 4)], MADE, 8)
+    odd = base[2][::2, ::3, 1::3, 2::4, :3]
+    parts = [base[0][:, i] for i in range(600)] + [base[1], odd]
+    kept = base[0][:, 600].clone()
+    check_clip(parts, float(norm_of(parts, 2.0)) / 2, 2.0)
+    assert torch.equal(base[0][:, 600], kept)
+
+
+@gpu
+def test_without_the_compiled_call_path(monkeypatch):
+    """The same numbers through ctypes."""
+    from cuml_b200 import distill
+
+    def everything():
+        out = []
+        for name, shapes in SHAPES.items():
+            for kind in KINDS:
+                x = made(shapes, MADE)
+                to = [torch.zeros_like(t, dtype=torch.bfloat16) for t in x]
+                out += [distill.gradient_norm(x, norm_type=kind), distill.clip_gradients(x, 0.01, norm_type=kind, out=to), *to]
+                out += [distill.clip_gradients(x, 0.01, norm_type=kind), *x]
+        return out
+
+    assert distill._native()
+    compiled = everything()
+    monkeypatch.setattr(distill, "_call", False)
+    for x, y in zip(compiled, everything()):
+        assert x.dtype == y.dtype and torch.equal(x, y)
 
 
 @gpu

@@ -636,6 +636,37 @@ def test_autograd_rules(monkeypatch, compiled):
 
 
 @gpu
+@pytest.mark.parametrize("compiled", [True, False])
+def test_saved_tensors_under_hooks_and_checkpoints(monkeypatch, compiled):
+    from torch.utils.checkpoint import checkpoint
+
+    from cuml_b200 import distill
+
+    if not compiled:
+        monkeypatch.setattr(distill, "_call", False)
+    z, t = logits(20, 300, "fp32").requires_grad_(), targets(20, 300)
+    h, w = (x.requires_grad_() for x in layer(20, 64, 300, "bf16"))
+
+    def step(z, h, w):
+        a, b = distill.log_probs(z, t, top=2), distill.linear_log_probs(h, w, t)
+        return a.log_prob.sum() + 2 * a.entropy.sum() + 3 * b.log_prob.sum() + 4 * b.entropy.sum()
+
+    want = torch.autograd.grad(step(z, h, w), (z, h, w))
+    pack, unpack = (lambda x: x.t().contiguous().cpu()), (lambda x: x.cuda().t())  # (given back in another order of rows)
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        loss = step(z, h, w)
+    for a, b in zip(torch.autograd.grad(loss, (z, h, w)), want):
+        assert torch.equal(a, b)
+    loss = checkpoint(step, z, h, w, use_reentrant=False)
+    for a, b in zip(torch.autograd.grad(loss, (z, h, w)), want):
+        assert torch.equal(a, b)
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: x[:1] if x.dim() == 2 else x):
+        loss = step(z, h, w)
+    with pytest.raises(RuntimeError, match="hook gave back another tensor"):
+        torch.autograd.grad(loss, (z, h, w))
+
+
+@gpu
 def test_captured_and_replayed():
     """A captured step runs again on other values of its inputs."""
     from cuml_b200 import distill
