@@ -61,8 +61,10 @@ constexpr float kHalfScale    = 16384.f;       // of d in fp16
 constexpr int kFewNamed = 4;
 constexpr int kScaleBlocks = 8;
 // Stages whose sums stay in TMEM before the epilogue adds them up, where the logits themselves are the answer (kScoreStats): the tensor
-// cores cut each addition short, which over 2048 terms takes 1.5e-6 off a logit, and its log q and entropy with it.
-constexpr int kSumStages = 8;
+// cores cut each addition short, which over 2048 terms takes 1.5e-6 off a logit, and its log q and entropy with it.  (2-norm of log q's
+// error over log q's, 4096 x 2048 x 2 fp16: 2.3e-6 in one sum, 8.4e-7 this way, 6.0e-7 with 8, 6.8e-7 by sums of 32 bits without tensor
+// cores.  4096 x 2048 x 16,384: 150 us with one sum and this way, 163 with 8, which the epilogue does not clear in time.)
+constexpr int kSumStages = 12;
 
 __device__ int g_status;
 __device__ __forceinline__ bool incomplete() { return *static_cast<volatile int*>(&g_status) != 0; }
@@ -323,20 +325,34 @@ __device__ __forceinline__ void take_columns(const Work& w, const Product& p, in
         if (col + i >= p.n) x[i] = lowest<float>();
     }
     float most = x[0];
-#pragma unroll
-    for (int i = 1; i < 32; ++i) most = fmaxf(most, x[i]);
     if (KIND == kScoreStats) {
-      if (most > score.m) score.move(most, w.c);
-      const float b = base_of(score.m);
-      float s[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+      float other = x[16];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const float a = at_least((x[i] - b) * w.c, kLeast), e = power(a);
-        s[i & 3] += e;
-        u[i & 3] = fmaf(e, a, u[i & 3]);
+      for (int i = 1; i < 16; ++i) {
+        most  = fmaxf(most, x[i]);
+        other = fmaxf(other, x[16 + i]);
       }
-      score.s += (s[0] + s[1]) + (s[2] + s[3]);
-      score.u += (u[0] + u[1]) + (u[2] + u[3]);
+      most = fmaxf(most, other);
+      // (two at a time: the epilogue has to end before the tensor cores are two sums ahead)
+      if (most > score.m) score.move(most, w.c);
+      const float b           = base_of(score.m);
+      const uint64_t minus_b = pair_of(-b, -b), cc = pair_of(w.c, w.c);
+      uint64_t s[2] = {0, 0}, u[2] = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        float lo, hi;
+        split_pair(fma_pairs(add_pairs(pair_of(x[i], x[i + 1]), minus_b), cc, 0), lo, hi);
+        const uint64_t a = pair_of(at_least(lo, kLeast), at_least(hi, kLeast));
+        split_pair(a, lo, hi);
+        const uint64_t e = pair_of(power(lo), power(hi));
+        s[i / 2 & 1] = add_pairs(s[i / 2 & 1], e);
+        u[i / 2 & 1] = fma_pairs(e, a, u[i / 2 & 1]);
+      }
+      float lo, hi;
+      split_pair(add_pairs(s[0], s[1]), lo, hi);
+      score.s += lo + hi;
+      split_pair(add_pairs(u[0], u[1]), lo, hi);
+      score.u += lo + hi;
       if (at >= col && at < col + 32) {
         // (as a choice in C++ it is an index, for which all of x would be put into memory)
 #pragma unroll
@@ -346,6 +362,8 @@ __device__ __forceinline__ void take_columns(const Work& w, const Product& p, in
       }
       return;
     }
+#pragma unroll
+    for (int i = 1; i < 32; ++i) most = fmaxf(most, x[i]);
     if (most > r.m) r.raise(most, w.c);
     const float b = base_of(r.m);
     float s[4]    = {0.f, 0.f, 0.f, 0.f};
@@ -635,7 +653,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
           float x[32];
           load_columns(tmem + half * kTile + from + 32 * c + (static_cast<uint32_t>(quarter * 32) << 16), x);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) z[i] += x[i];
+          for (int i = 0; i < 32; i += 2) split_pair(add_pairs(pair_of(z[i], z[i + 1]), pair_of(x[i], x[i + 1])), z[i], z[i + 1]);
         };
         for (int k = t.begin; ok && k < t.end; k += kSumStages) {
           if (!warp_wait(done + 8 * half, turn, &gave_up)) {
