@@ -867,6 +867,32 @@ __global__ void __launch_bounds__(kThreads) linear_scores(LinearScoreArgs a, con
   }
 }
 
+// The same of few classes and little to multiply, by THREADS threads: the logits are dot products, as in linear_rows.  (5 x 416 x 27 fp16:
+// with the tensor cores' sums the scores' errors are 1e-6 of them; 256 classes take a block as long as those kernels.)
+template <class T, int THREADS>
+__global__ void __launch_bounds__(kThreads) linear_scores_few(LinearScoreArgs a)
+{
+  constexpr int ROWS = kThreads / THREADS, WARPS = THREADS / 32;
+  __shared__ float joins[3 * kThreads / 32], given[ROWS];
+  const int slot = threadIdx.x / THREADS, tid = threadIdx.x % THREADS;
+  const LinearArgs& l = a.layer;
+  const float c       = l.temperature.c;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + slot; row < l.n_rows; row += static_cast<int64_t>(gridDim.x) * ROWS) {
+    const int at = target_of(a.target, row, l.n_cols);
+    Scored r;
+    dots<T, WARPS>(l, static_cast<const T*>(l.hidden) + row * l.hidden_stride, static_cast<int>(l.n_cols), tid / 32, [](int j) { return j; },
+                   [&](int j, float z) {
+                     if (z > r.m) r.move(z, c);
+                     r.add(z, base_of(r.m), c);
+                     if (j == at) given[slot] = z;
+                   });
+    join_scored<THREADS>(r, c, joins);
+    sync_row<THREADS>();  // `given` has been written
+    if (tid == 0) finish_score(a.out, row, r, l.temperature.inverse, at, at >= 0 ? given[slot] : 0.f);
+    sync_row<THREADS>();
+  }
+}
+
 // One upstream value per row of an fp16 layer: the rows' are brought below 1 by a power of two, which *scale takes
 // back, so that d stays in range.  By one cluster (one block took 280 us for 2^20 rows).
 __global__ void __cluster_dims__(kScaleBlocks, 1, 1) __launch_bounds__(1024) grad_scales(LinearGradArgs g, float* scale, float* row_scale)
@@ -1233,6 +1259,19 @@ cudaError_t run_linear_score(bool bf16, const LinearScoreArgs& given, void* work
   w.bf16     = bf16;
   w.c        = a.temperature.c;
   w.ticket   = reinterpret_cast<int*>(at);  // not used
+  if (a.n_cols <= 2 * kFewClasses && a.n_rows * a.n_cols <= kSmallLogits / a.width) {
+    LinearScoreArgs few = given;
+    few.layer           = a;
+    const bool warp     = a.n_cols <= 8 || a.n_rows >= 8 * n_sms;  // (a block has four classes for each warp at a time)
+    const int per       = warp ? kThreads / 32 : 1;
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((a.n_rows + per - 1) / per, 8ll * n_sms));
+    if (warp)
+      linear_scores_few<T, 32><<<blocks, kThreads, 0, s>>>(few);
+    else
+      linear_scores_few<T, kThreads><<<blocks, kThreads, 0, s>>>(few);
+    count_launches(1);
+    return cudaGetLastError();
+  }
   w.target   = given.target;
   w.target_logit = reinterpret_cast<float*>(at += 256);
   w.score_parts  = reinterpret_cast<float4*>(at + padded(a.n_rows * 4));

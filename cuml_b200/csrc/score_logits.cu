@@ -35,7 +35,8 @@ constexpr int64_t kLongGradRow = 1 << 16;
 constexpr int kWarpLeast = 8;
 constexpr int kWarpBytes = 16384;
 constexpr int kWarpLong  = 8192;
-// Rows for one thread each: classes, and rows per SM from which on.
+// Rows for one thread each: classes, and rows per SM from which on.  (Both passes, us, by eight lanes and by threads: 1,000,003 x 10 fp32 92,
+// 83 and 24, 26; 200,000 x 33 fp32 25, 19 and 14, 16; 200,000 x 64 fp32 23, 21 and 21, 25.)
 constexpr int kTileCols   = 64;
 constexpr int kTileLeast  = 32;
 constexpr int kTileBlocks = 8;   // of an SM

@@ -1,4 +1,4 @@
-"""Distillation: a teacher's best scores, and losses that train a small network on them.
+"""Distillation: a teacher's best scores, losses that train a small network on them, and scores of its answers.
 
 A large forest can be compressed into a small network by training that on the forest's answers.
 These operators take a teacher's scores over classes (a forest's probabilities, or the logits of any other
@@ -10,7 +10,7 @@ model), keep the `k` best classes of each row, and compute the loss of a student
     linear_cross_entropy       softmax cross entropy from the last linear layer, logits not kept
     linear_distillation_loss   distillation_loss from the last linear layer, logits not kept
 
-score its (or any classifier's) answers, with gradients, and take care of the gradients of a step:
+Others score a student's (or any classifier's) answers, with gradients, and clip the gradients of a step:
 
     log_probs                  log probability of each row's given class, its entropy, its best alternatives
     linear_log_probs           the first two from the last linear layer, logits not kept
@@ -19,10 +19,10 @@ score its (or any classifier's) answers, with gradients, and take care of the gr
 
 `ForestInference.predict_top`, `.teach` and `.distillation_loss` call them with a forest as the teacher.
 All tensors are CUDA tensors of one device; work is enqueued on torch's current stream of that device and
-nothing waits.  The losses have first derivatives by the logits, or by the layer's input and weight (backward mode
-only: second and forward-mode derivatives are errors); the teacher's values are constants.  Calls and their gradients can be captured into CUDA graphs once they have run on
-the device (as everywhere in torch, while no autograd graph of the same leaves from outside the capture is
-alive).  All computation happens in libb2fil.so.
+nothing waits.  Losses and scores have first derivatives by the logits, or by the layer's input and weight (backward mode
+only: second and forward-mode derivatives are errors); the teacher's values are constants.  Calls and their
+gradients can be captured into CUDA graphs once they have run on the device (as everywhere in torch, while no
+autograd graph of the same leaves from outside the capture is alive).  All computation happens in libb2fil.so.
 """
 from __future__ import annotations
 
@@ -759,8 +759,8 @@ def clip_gradients(gradients, max_norm: float, *, norm_type: float = 2.0, out=No
 
 def check_status(device=None) -> None:
     """Wait for all work on `device` and raise `B2FilError` (code -7) if a bounded wait inside a kernel of the
-    linear losses ran out since the last check.  The losses and gradients that follow such a wait are NaN until
-    then, as nothing in a stream-ordered call can raise; where a linear loss is NaN, ask here first."""
+    linear losses and scores ran out since the last check.  Losses, scores and gradients that follow such a wait are NaN
+    until then, as nothing in a stream-ordered call can raise; where a linear loss is NaN, ask here first."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     word = C.c_int32(0)
     index = torch.cuda.current_device() if device.index is None else device.index

@@ -511,9 +511,9 @@ int64_t b2fil_clip_gradients_workspace(const b2fil_gradient* gradients, int64_t 
 int b2fil_clip_gradients(const b2fil_gradient* gradients, int64_t n, int norm_kind, int scales, double most, float* norm,
                          void* workspace, int64_t workspace_bytes, int device_id, void* cuda_stream);
 
-/* Waits for all work on device_id, reads the status word of the linear loss's kernels there and returns
+/* Waits for all work on device_id, reads the status word of the linear losses' and scores' kernels there and returns
  * B2FIL_ERR_TIMEOUT when a bounded wait inside one ran out; the word is cleared by the read.  That call's outputs may be
- * incomplete, and from then until the word is read the linear losses on the device (of layers whose logits
+ * incomplete, and from then until the word is read the linear losses and scores on the device (of layers whose logits
  * go through the tensor cores) and their gradients are NaN. */
 int b2fil_distill_status(int device_id, int32_t* status);
 
