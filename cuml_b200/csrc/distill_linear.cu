@@ -305,6 +305,14 @@ __device__ __forceinline__ float power_within(float x, float sum)
   return y;
 }
 
+// The same of an exponent that is a factor, too.
+__device__ __forceinline__ float at_most(float x, float most)
+{
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(most));
+  return y;
+}
+
 // What rounding x to 16 bits leaves.
 __device__ __forceinline__ float left_of(float x, bool bf16)
 {
@@ -312,7 +320,8 @@ __device__ __forceinline__ float left_of(float x, bool bf16)
 }
 
 // Part of a row (32 columns from `col` on) of a finished tile.  n: columns of the result.
-// at: the given class (kScoreStats), -1: none.
+// at: the given class (kScoreStats), -1: none.  sum: the row's (kDiff), or its logarithm to base 2 (kScoreDiff), which bounds a score's
+// powers and the exponents that they are multiplied with alike.
 template <int KIND>
 __device__ __forceinline__ void take_columns(const Work& w, const Product& p, int split, int64_t row, int col, float (&x)[32],
                                              Running<float>& r, Scored& score, const RowGrad& of_score, int at, float base, float sum,
@@ -376,8 +385,8 @@ __device__ __forceinline__ void take_columns(const Work& w, const Product& p, in
     if (KIND == kScoreDiff) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        const float a = at_least((x[i] - of_score.base) * w.c, kLeast);
-        x[i]          = col + i < p.n ? power_within(a, sum) * fmaf(of_score.B, a, of_score.A) : 0.f;
+        const float a = at_most(at_least((x[i] - of_score.base) * w.c, kLeast), sum);
+        x[i]          = col + i < p.n ? power(a) * fmaf(of_score.B, a, of_score.A) : 0.f;
       }
       if (of_score.at >= col && of_score.at < col + 32) {
 #pragma unroll
@@ -632,7 +641,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1) 
           of_score = row_grad(s, up.log_prob ? up.log_prob[row * up.log_prob_stride] * f : 0.f,
                               up.entropy ? up.entropy[row * up.entropy_stride] * f : 0.f);
           of_score.at = of_score.at < 0 ? -1 : of_score.at - w.first;
-          sum = 1.f / s.y;
+          sum = -log2f(s.y);
         } else {
           factor = 0.f;
         }
@@ -922,7 +931,8 @@ __global__ void __cluster_dims__(kScaleBlocks, 1, 1) __launch_bounds__(1024) gra
 }
 
 // The same for the gradients by a row's two scores: a difference is at most |g| + 6 |h| (of a class of probability q, |log q + H| q <=
-// q (1 - q) log n_cols + 1).  scale[1] is what brings them below 1.
+// q (1 - q) log n_cols + 1), and where a low temperature makes a class's logit that of the whole row (power_within) |g| + |h| log n_cols,
+// which is less than three times |g| + 8 |h|: kHalfScale leaves four.  scale[1] is what brings |g| + 8 |h| below 1.
 __global__ void __cluster_dims__(kScaleBlocks, 1, 1) __launch_bounds__(1024) score_scales(ScoreUpstream up, const float4* kept, int64_t n_rows, float* scale)
 {
   namespace cg = cooperative_groups;

@@ -1,0 +1,32 @@
+"""Scores and clipping at the ends of their ranges: low temperatures, many sums per tile, shared memory of tensors."""
+import math
+
+import pytest
+import torch
+
+from tests.test_distill import HALF_STEP, TYPES, gen
+from tests.test_score import wide
+
+gpu = pytest.mark.gpu
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,width,c", [(64, 2048, 300), (64, 2048, 200), (64, 2048, 2000), (500, 1024, 1000), (3, 520, 20)])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_entropy_of_a_layer_at_the_lowest_temperature(n, width, c, dtype, sign):
+    """The logits' roundings over T are exponents of tens there, so a class of many that are equal may seem to have all of the row in the
+    backward pass.  Whatever q <= 1 is taken for it, its difference is h q (log q + H) / T with q |log q| <= 1 / e and H <= log n_classes:
+    at most |h| log n_classes / T, which bounds both gradients (and rounding takes at most half a step more, of the differences
+    and of the sums)."""
+    from cuml_b200 import distill
+
+    t, temperature, up = TYPES[dtype], 1e-6, 1e-8
+    h = (torch.rand((n, width), generator=gen(1), device="cuda") + 0.5).to(t).requires_grad_()
+    w = ((torch.rand((1, width), generator=gen(2), device="cuda") + 0.5) * (sign / 8)).to(t).repeat(c, 1).requires_grad_()
+    got = distill.linear_log_probs(h, w, temperature=temperature)
+    dh, dw = torch.autograd.grad(got.entropy, (h, w), torch.full((n,), up, device="cuda"))
+    each = up / temperature * math.log(c) * (1 + 4 * HALF_STEP[t])
+    assert (wide(dh).abs() <= each * wide(w).abs().sum(0)).all()
+    assert (wide(dw).abs() <= each * wide(h).abs().sum(0)).all()
+    distill.check_status()
