@@ -886,8 +886,9 @@ PyObject* clip_gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs)
       if (!dense(to, first) || to.sizes() != x.sizes() || to.strides() != x.strides() || to.requires_grad()) Py_RETURN_NONE;
     }
     b2fil_gradient g{};
+    // (a tensor that is written first gets memory of its own where it shares some)
+    g.to        = scales ? to.mutable_data_ptr() : const_cast<void*>(to.const_data_ptr());
     g.from      = x.const_data_ptr();
-    g.to        = const_cast<void*>(to.const_data_ptr());
     g.rows      = 1;
     g.cols      = x.numel();
     g.from_col  = g.to_col = 1;

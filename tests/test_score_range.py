@@ -30,3 +30,27 @@ def test_entropy_of_a_layer_at_the_lowest_temperature(n, width, c, dtype, sign):
     assert (wide(dh).abs() <= each * wide(w).abs().sum(0)).all()
     assert (wide(dw).abs() <= each * wide(h).abs().sum(0)).all()
     distill.check_status()
+
+
+@gpu
+@pytest.mark.parametrize("compiled", [True, False])
+def test_tensors_that_share_memory_until_one_is_written(monkeypatch, compiled):
+    """A clone that is made when it is written (copy on write) is made before it is clipped, or taken as `out`: what it was made from stays.
+    Measuring a norm makes none."""
+    from cuml_b200 import distill
+
+    if not compiled:
+        monkeypatch.setattr(distill, "_call", False)
+    for n in (1000, 300_000):
+        source = torch.full((n,), 2.0, device="cuda")
+        x, y = torch._lazy_clone(source), torch._lazy_clone(source)
+        norm = distill.clip_gradients([x], 1.0)
+        assert (source == 2).all() and (y == 2).all() and torch.allclose(x, source / norm)
+        kept = torch.full((n,), 5.0, device="cuda")
+        out = torch._lazy_clone(kept)
+        distill.clip_gradients([source], 1.0, out=[out])
+        assert (kept == 5).all() and (source == 2).all() and torch.equal(out, x)
+        z = torch._lazy_clone(source)
+        assert torch.equal(distill.gradient_norm([z, y]), distill.gradient_norm([source, source]))
+        if compiled:
+            assert torch._C._is_cow_tensor(z)
