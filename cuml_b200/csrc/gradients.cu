@@ -136,8 +136,15 @@ __device__ __forceinline__ double join_block(double x, double* room)
   return x;
 }
 
+// 16 bytes: of memory that this launch does not write, or of any.
+template <bool READ_ONLY>
+__device__ __forceinline__ uint4 load_words(const uint4* from)
+{
+  return READ_ONLY ? __ldg(from) : *from;
+}
+
 // (a function of its own, called once per tensor of a chunk: inlined for all types it spilled registers)
-template <class T, int KIND>
+template <class T, int KIND, bool READ_ONLY>
 __device__ __noinline__ Norm<KIND> norm_row(const T* x, int n)
 {
   constexpr int N  = Piece<T>::N;
@@ -156,14 +163,14 @@ __device__ __noinline__ Norm<KIND> norm_row(const T* x, int n)
   for (; p + (kInFlight - 1) * kThreads < pieces; p += kInFlight * kThreads) {
     uint4 w[kInFlight];
 #pragma unroll
-    for (int u = 0; u < kInFlight; ++u) w[u] = __ldg(from + p + u * kThreads);
+    for (int u = 0; u < kInFlight; ++u) w[u] = load_words<READ_ONLY>(from + p + u * kThreads);
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) take(w[u]);
   }
   if (p < pieces) {  // (at most kInFlight - 1, in flight together)
     uint4 w[kInFlight - 1];
 #pragma unroll
-    for (int u = 0; u < kInFlight - 1; ++u) w[u] = p + u * kThreads < pieces ? __ldg(from + p + u * kThreads) : make_uint4(0, 0, 0, 0);
+    for (int u = 0; u < kInFlight - 1; ++u) w[u] = p + u * kThreads < pieces ? load_words<READ_ONLY>(from + p + u * kThreads) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int u = 0; u < kInFlight - 1; ++u)
       if (p + u * kThreads < pieces) take(w[u]);
@@ -186,8 +193,8 @@ __device__ __forceinline__ void put_element(void* to, int type, int64_t i, float
     static_cast<__half*>(to)[i] = narrow<__half>(x);
 }
 
-// The norm's part of a block's chunks.
-template <int KIND, int N, bool STRIDED>
+// The norm's part of a block's chunks.  READ_ONLY: this launch does not write the tensors.
+template <int KIND, bool READ_ONLY, int N, bool STRIDED>
 __device__ __forceinline__ void norm_chunks(const Batch<N, STRIDED>& b, Norm<KIND>& r)
 {
   const int chunks = chunks_of(b);
@@ -203,11 +210,11 @@ __device__ __forceinline__ void norm_chunks(const Batch<N, STRIDED>& b, Norm<KIN
           r.take(one);
         }
       } else if (type == kF32) {
-        r.take(norm_row<float, KIND>(static_cast<const float*>(from) + begin, n));
+        r.take(norm_row<float, KIND, READ_ONLY>(static_cast<const float*>(from) + begin, n));
       } else if (type == kBF16) {
-        r.take(norm_row<__nv_bfloat16, KIND>(static_cast<const __nv_bfloat16*>(from) + begin, n));
+        r.take(norm_row<__nv_bfloat16, KIND, READ_ONLY>(static_cast<const __nv_bfloat16*>(from) + begin, n));
       } else {
-        r.take(norm_row<__half, KIND>(static_cast<const __half*>(from) + begin, n));
+        r.take(norm_row<__half, KIND, READ_ONLY>(static_cast<const __half*>(from) + begin, n));
       }
     });
 }
@@ -317,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_parts(const __grid_con
 {
   __shared__ double room[kThreads / 32];
   Norm<KIND> r;
-  norm_chunks(b, r);
+  norm_chunks<KIND, true>(b, r);
   const double all = join_block<KIND>(r.value(), room);
   if (threadIdx.x == 0) sums[blockIdx.x] = all;
 }
@@ -344,7 +351,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) cli
   namespace cg = cooperative_groups;
   __shared__ double room[kThreads / 32], mine;
   Norm<KIND> r;
-  norm_chunks(b, r);
+  norm_chunks<KIND, false>(b, r);
   double all = join_block<KIND>(r.value(), room);
   if (threadIdx.x == 0) mine = all;
   cg::cluster_group cluster = cg::this_cluster();

@@ -54,3 +54,40 @@ def test_tensors_that_share_memory_until_one_is_written(monkeypatch, compiled):
         assert torch.equal(distill.gradient_norm([z, y]), distill.gradient_norm([source, source]))
         if compiled:
             assert torch._C._is_cow_tensor(z)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("kind", [2.0, 1.0, math.inf])
+def test_few_gradients_clipped_by_one_launch_after_the_other(dtype, kind):
+    """A launch reads what the launch before has written, and what it writes itself only after all of it has been read.  Halved each time, so
+    that nothing is rounded: powers of two that fp16 holds, 50,000 of them and few, on and off the 16-byte boundaries."""
+    from cuml_b200 import distill
+
+    for n in (7, 3001, 50_000):
+        flat = torch.zeros(n + 11, dtype=TYPES[dtype], device="cuda")
+        parts = list(flat[3:3 + n].split((n + 2) // 3))
+        start = [2.0 ** torch.randint(0, 6, x.shape, generator=gen(n), device="cuda") for x in parts]
+
+        def clip():
+            for x, y in zip(parts, start):
+                x.copy_(y)
+            return [distill.clip_gradients(parts, m, norm_type=kind) for m in limits]
+
+        size = torch.cat(start).double()
+        norm = float(size.max() if kind == math.inf else size.sum() if kind == 1.0 else size.square().sum().sqrt())
+        limits = [norm / 2 ** i for i in range(1, 6)]
+        clip()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            norms = clip()
+        for _ in range(3):
+            graph.replay()
+            for i, got in enumerate(norms):
+                assert abs(got.item() - norm / 2 ** i) <= 12 * (i + 1) * 2.0 ** -24 * norm / 2 ** i
+            for x, y in zip(parts, start):
+                # (a factor is off by 12 steps of fp32 at most, an element by half a step of its type for each of the five)
+                assert ((wide(x) * 32 - wide(y)).abs() <= wide(y) * 5 * (12 * 2.0 ** -24 + HALF_STEP[x.dtype])).all()
+            assert not flat[:3].any() and not flat[3 + n:].any()
+        del graph
