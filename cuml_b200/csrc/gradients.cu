@@ -100,8 +100,14 @@ struct Norm {
     float s = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) s = KIND == kSum ? s + fabsf(x[e]) : fmaf(x[e], x[e], s);
-    // (squares of numbers below 2^-50 or so lose bits, those above 2^60 may overflow; all zero is neither)
+    // (squares of numbers below 2^-50 or so lose bits, those above 2^60 may overflow; zeros do neither)
     if (KIND == kSquares ? !(s > 0x1p-90f && s < 0x1p120f) : !(s < 0x1p120f)) {
+      if (KIND == kSquares) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) bits |= __float_as_uint(x[e]);
+        if ((bits & 0x7fffffffu) == 0) return;
+      }
       double d = 0;
 #pragma unroll
       for (int e = 0; e < E; ++e) d += KIND == kSum ? fabs(static_cast<double>(x[e])) : static_cast<double>(x[e]) * x[e];

@@ -91,3 +91,24 @@ def test_few_gradients_clipped_by_one_launch_after_the_other(dtype, kind):
                 assert ((wide(x) * 32 - wide(y)).abs() <= wide(y) * 5 * (12 * 2.0 ** -24 + HALF_STEP[x.dtype])).all()
             assert not flat[:3].any() and not flat[3 + n:].any()
         del graph
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_norm_of_mostly_zero_gradients(dtype):
+    """Zeros of both signs are left out at once; what is so small that its square is zero in 32 bits is not.  (9 u of the norm, as in
+    test_gradients.py, and for norms below 2^-126, which are multiples of 2^-149 in fp32, half of that: 2^-150.)"""
+    from cuml_b200 import distill
+
+    for size in (1.0, 1e-30, 2.0 ** -133):
+        for n in (5, 4099, 100_003):
+            x = torch.zeros(n, dtype=TYPES[dtype], device="cuda")
+            x[1::3] = -0.0
+            assert distill.gradient_norm([x]) == 0
+            x[:: 997] = size
+            x[n - 1] = -3 * size
+            want = float(wide(x).square().sum().sqrt())
+            assert abs(distill.gradient_norm([x]).item() - want) <= 9 * 2.0 ** -24 * want + 2.0 ** -150
+            assert distill.gradient_norm([x], norm_type=math.inf) == wide(x).abs().max()
+            x[n // 2] = float("nan")
+            assert distill.gradient_norm([x]).isnan()
