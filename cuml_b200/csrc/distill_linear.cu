@@ -995,30 +995,33 @@ __global__ void __launch_bounds__(kThreads) finish_sums(const float* sums, int s
   }
 }
 
-// The same for rows of `width` of `pitch` columns, a warp for each.  (Four results per thread, which may be in two rows: 1999 x
-// 1001 x 50,001 took 84 us, this way 38.)
-template <class T>
+// The same for rows of `width` of `pitch` columns, LANES threads for each; a row's parts (blockIdx.y) are of LANES x 4 columns.  (us of
+// both gradients' by four results per thread in order, by a warp per row and with the lanes that finish takes: 200,000 x 12 x 300 18, 35
+// and 15; 200,000 x 20 x 300 22, 36 and 18; 200,000 x 50 x 300 40, 37 and 23; 300 x 20 x 50,001 12, 16 and 12; 300 x 1001 x 50,001 152, 88
+// and 69.)
+template <class T, int LANES, int UNROLL>
 __global__ void __launch_bounds__(kThreads) finish_rows(const float* sums, int splits, int64_t rows, int pitch, int width,
                                                         Scale scale, T* out)
 {
-  constexpr int ROWS = kThreads / 32, U = 4;
+  constexpr int ROWS = kThreads / LANES, U = 4;
   const float f  = scale();
-  const int lane = threadIdx.x % 32;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / 32; r < rows; r += static_cast<int64_t>(gridDim.x) * ROWS) {
+  const int lane = threadIdx.x % LANES;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / LANES; r < rows; r += static_cast<int64_t>(gridDim.x) * ROWS) {
     const float* from = sums + r * pitch;
     T* to             = out + r * width;
-    for (int c = lane; c < width; c += 32 * U) {
+    for (int c = blockIdx.y * (LANES * U) + lane; c < width; c += gridDim.y * (LANES * U)) {
       float x[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) x[u] = c + 32 * u < width ? 0.f + __ldg(from + c + 32 * u) : 0.f;
+      for (int u = 0; u < U; ++u) x[u] = c + LANES * u < width ? 0.f + __ldg(from + c + LANES * u) : 0.f;
+#pragma unroll UNROLL
       for (int s = 1; s < splits; ++s) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (c + 32 * u < width) x[u] += __ldg(from + s * rows * pitch + c + 32 * u);
+          if (c + LANES * u < width) x[u] += __ldg(from + s * rows * pitch + c + LANES * u);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (c + 32 * u < width) to[c + 32 * u] = narrow<T>(x[u] * f);
+        if (c + LANES * u < width) to[c + LANES * u] = narrow<T>(x[u] * f);
     }
   }
 }
@@ -1248,9 +1251,17 @@ cudaError_t finish(const float* sums, int splits, int64_t rows, int64_t pitch, i
     const int64_t need = (n / 4 + kThreads - 1) / kThreads;
     finish_sums<T><<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(sums, splits, n, scale, static_cast<T*>(out));
   } else {
-    const int64_t need = (rows + kThreads / 32 - 1) / (kThreads / 32);
-    finish_rows<T><<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(
-      sums, splits, rows, static_cast<int>(pitch), static_cast<int>(width), scale, static_cast<T*>(out));
+    // Few lanes for narrow rows; of many sums, which few rows have, eight at a time (300 x 20, sixteen sums: 8.0 us with four, 6.0).
+    const bool many    = splits > 2;
+    const int lanes    = width <= 16 ? 4 : width <= 32 ? 8 : width <= 64 || many ? 16 : 32;
+    const int64_t need = (rows + kThreads / lanes - 1) / (kThreads / lanes), parts = (width + 4 * lanes - 1) / (4 * lanes);
+    const unsigned x   = static_cast<unsigned>(std::min(need, most));
+    const dim3 grid(x, static_cast<unsigned>(std::max<int64_t>(1, std::min(parts, most / x))));
+    const auto kernel  = lanes == 4    ? (many ? finish_rows<T, 4, 8> : finish_rows<T, 4, 1>)
+                         : lanes == 8  ? (many ? finish_rows<T, 8, 8> : finish_rows<T, 8, 1>)
+                         : lanes == 16 ? (many ? finish_rows<T, 16, 8> : finish_rows<T, 16, 1>)
+                                       : finish_rows<T, 32, 1>;
+    kernel<<<grid, kThreads, 0, s>>>(sums, splits, rows, static_cast<int>(pitch), static_cast<int>(width), scale, static_cast<T*>(out));
   }
   return cudaGetLastError();
 }

@@ -112,3 +112,29 @@ def test_norm_of_mostly_zero_gradients(dtype):
             assert distill.gradient_norm([x], norm_type=math.inf) == wide(x).abs().max()
             x[n // 2] = float("nan")
             assert distill.gradient_norm([x]).isnan()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,width,c", [(7000, 3, 40), (7000, 12, 300), (3000, 17, 5000), (6000, 20, 300), (300, 20, 9000), (2000, 29, 300),
+                                       (257, 33, 300), (5000, 50, 515), (300, 100, 9001), (300, 1001, 20_011), (1500, 250, 700)])
+def test_gradients_of_odd_widths_are_those_of_wider_rows_of_zeros(n, width, c, dtype):
+    """Rows that are no whole pieces of 16 bytes are copied with zeros behind them.  Those zeros given by the caller take part in the same
+    products and sums, so what comes out for the other columns is the same, bit for bit."""
+    from cuml_b200 import distill
+
+    t, line = TYPES[dtype], 16
+    h, w = (torch.randn(s, generator=gen(width + s[0]), device="cuda").to(t) for s in ((n, width), (c, width)))
+    pad = (width + line - 1) // line * line - width
+    target = torch.randint(0, c, (n,), generator=gen(c), device="cuda")
+    up = torch.randn(n, generator=gen(9), device="cuda")
+
+    def grads(h, w):
+        h, w = h.detach().requires_grad_(), w.detach().requires_grad_()
+        return torch.autograd.grad(distill.linear_cross_entropy(h, w, target, reduction="none"), (h, w), up)
+
+    odd = grads(h, w)
+    wide_rows = grads(*(torch.nn.functional.pad(x, (0, pad)) for x in (h, w)))
+    for a, b in zip(odd, wide_rows):
+        assert torch.equal(a, b[:, :width])
+        assert not b[:, width:].any()
