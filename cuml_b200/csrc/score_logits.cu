@@ -2,7 +2,8 @@
 // logits.  The formulas are in score_common.cuh.
 //
 // Bound by memory: the forward pass reads the logits once (maximum, sum and mean exponent in one pass), the backward
-// pass reads them again and writes as much; rows that do not count are not read.
+// pass reads them again and writes as much.  Rows that do not count are not read, but where a thread has a row: a tile of rows is copied
+// to shared memory as a whole.
 #include "score_common.cuh"
 
 namespace b2fil {
@@ -79,7 +80,9 @@ __device__ __noinline__ Scored visit_any(const T* row, int64_t n, int tid, float
   return r;
 }
 
-// One part of a row per block: (row, segment) -> its m, s and u.
+// One part of a row per block: (row, segment) -> its m, s and u, nothing for rows that do not count.  (Asking for the class first costs a
+// row's 0.5 us, of which the join gives back 0.3: 100 x 131,072 fp32, both kernels: 21.3 us with and 22.0 without reading such rows,
+// where half of them are that 21.3 and 13.4.)
 template <class T>
 __global__ void __launch_bounds__(kThreads) score_parts(ScoreArgs a, int64_t seg_cols, float4* parts)
 {
@@ -88,6 +91,7 @@ __global__ void __launch_bounds__(kThreads) score_parts(ScoreArgs a, int64_t seg
   const int n         = static_cast<int>(min(seg_cols, a.n_cols - begin));
   const float c       = a.temperature.c;
   for (int64_t row = blockIdx.y; row < a.n_rows; row += gridDim.y) {
+    if (target_of(a.target, row, a.n_cols) == -2) continue;  // not read
     const T* x = static_cast<const T*>(a.logits) + row * a.row_stride + begin;
     Scored r   = visit_ordinary(x, n, threadIdx.x, kThreads, c);
     join_scored<kThreads>(r, c, room);
@@ -106,7 +110,7 @@ __global__ void __launch_bounds__(kThreads) score_join(ScoreArgs a, int segs, co
     const int at      = target_of(a.target, row, a.n_cols);
     const float given = at >= 0 ? widen(static_cast<const T*>(a.logits)[row * a.row_stride + at]) : 0.f;
     Scored r;
-    for (int i = lane; i < segs; i += 32) {
+    for (int i = lane; i < segs && at != -2; i += 32) {
       const float4 p = parts[row * segs + i];
       r.join(p.x, p.y, p.z, c);
     }

@@ -138,3 +138,30 @@ def test_gradients_of_odd_widths_are_those_of_wider_rows_of_zeros(n, width, c, d
     for a, b in zip(odd, wide_rows):
         assert torch.equal(a, b[:, :width])
         assert not b[:, width:].any()
+
+
+@gpu
+@pytest.mark.parametrize("n,c", [(4, 10), (6000, 10), (6000, 50), (200_000, 40), (400, 600), (1300, 4000), (400, 20_000), (20, 50_000),
+                                 (400, 3000)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_rows_that_do_not_count_may_hold_anything(n, c, dtype):
+    """Scores alone, with and without gradients: NaN and infinities of such rows reach no other row's, and nothing kept of the memory."""
+    from cuml_b200 import distill
+
+    z, t = torch.randn((n, c), generator=gen(c), device="cuda").to(TYPES[dtype]), torch.randint(0, c, (n,), generator=gen(n), device="cuda")
+    t[1::3] = -100
+    counts = t >= 0
+    plain, odd = z.clone(), z.clone()
+    plain[~counts] = 0.5
+    odd[1::3, ::2] = float("nan")
+    odd[1::3, 1::2] = float("inf")
+    odd[4::6] = float("-inf")
+    up = torch.randn((2, n), generator=gen(3), device="cuda")
+    out = []
+    for x in (plain, odd):
+        torch.empty((1 << 26,), device="cuda").fill_(float("nan"))  # (what a workspace is made from)
+        x.requires_grad_()
+        got = distill.log_probs(x, t)
+        out.append((got.log_prob, got.entropy, *torch.autograd.grad((got.log_prob, got.entropy), x, (up[0], up[1]))))
+    for a, b in zip(*out):
+        assert torch.equal(a, b) and (b[~counts] == 0).all()
