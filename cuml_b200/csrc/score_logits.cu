@@ -4,6 +4,8 @@
 // Bound by memory: the forward pass reads the logits once (maximum, sum and mean exponent in one pass), the backward
 // pass reads them again and writes as much.  Rows that do not count are not read, but where a thread has a row: a tile of rows is copied
 // to shared memory as a whole.
+#include <algorithm>
+
 #include "score_common.cuh"
 
 namespace b2fil {
@@ -32,14 +34,22 @@ constexpr int kGradBlocks = 4;
 constexpr int64_t kLongRow     = 1 << 17;
 constexpr int64_t kLongGradRow = 1 << 16;
 // Where there are kWarpLeast rows per SM, a warp takes longer ones, too: whose logits take up to kWarpBytes, and in the
-// gradient, of 16 bits, up to kWarpLong.  (20,000 x 3000 bf16, both passes: 96 and 66 us by blocks, 34 and 43 so.)
+// gradient, of 16 bits, up to kWarpLong.  (20,000 x 3000 bf16, both passes: 96 and 66 us by blocks, 34 and 43 so; the gradient of fp32: 72 and
+// 77, 1200 x 3000 5.4 and 6.9, 4096 x 3000 15.1 and 13.8.)
 constexpr int kWarpLeast = 8;
 constexpr int kWarpBytes = 16384;
 constexpr int kWarpLong  = 8192;
-// Rows for one thread each: classes, and rows per SM from which on.  (Both passes, us, by eight lanes and by threads: 1,000,003 x 10 fp32 92,
-// 83 and 24, 26; 200,000 x 33 fp32 25, 19 and 14, 16; 200,000 x 64 fp32 23, 21 and 21, 25.)
-constexpr int kTileCols   = 64;
-constexpr int kTileLeast  = 32;
+// Rows for one thread each: rows per SM from which on, and per SM and class, classes, bytes of a row; and of the gradient's, which writes the tile
+// back, too.  A tile takes a time of its own by its classes, however few tiles there are.  (us of each pass by eight lanes and by threads:
+// 1,000,000 x 10 fp32 93, 78 and 24, 25, x 48 95, 90 and 60, 85, x 64 94, 94 and 95, 147; 200,000 x 56 fp32 23, 19 and 19, 22, bf16 22, 18
+// and 14, 19; 120,000 x 64 fp32 14, 12 and 17, 19; 40,000 x 33 fp32 8.6, 5.5 and 6.5, 6.8, x 64 7.7, 5.4 and 8.5, 9.4; 20,000 x 10 bf16 5.9,
+// 4.5 and 4.1, 3.7, x 48 5.5, 4.1 and 5.5, 6.7; 5000 x 10 fp32 4.1, 3.1 and 4.0, 3.7, x 64 4.1, 3.0 and 7.0, 7.8.)
+constexpr int kTileLeast    = 32;
+constexpr int kTilePer      = 4;
+constexpr int kTileCols     = 64;
+constexpr int kTileBytes    = 224;
+constexpr int kTileGradPer  = 12;
+constexpr int kTileGradCols = 48;
 constexpr int kTileBlocks = 8;   // of an SM
 
 // n elements of a row by `threads` threads; the thread's part.
@@ -379,7 +389,14 @@ unsigned row_blocks(const ScoreArgs& a, bool warp, int element, int64_t at_once,
   if (warp) return blocks_of((a.n_rows + per - 1) / per, at_once);
   return blocks_of(a.n_rows, a.n_cols * element >= long_row ? 1 << 30 : at_once);
 }
-bool by_tiles(const ScoreArgs& a, int n_sms) { return a.n_cols <= kTileCols && a.n_rows >= static_cast<int64_t>(kTileLeast) * n_sms; }
+bool by_tiles(const ScoreArgs& a, int element, int n_sms)
+{
+  return a.n_cols <= kTileCols && a.n_cols * element <= kTileBytes && a.n_rows >= std::max<int64_t>(kTileLeast, kTilePer * a.n_cols) * n_sms;
+}
+bool grad_by_tiles(const ScoreArgs& a, int n_sms)
+{
+  return a.n_cols <= kTileGradCols && a.n_rows >= std::max<int64_t>(kTileLeast, kTileGradPer * a.n_cols) * n_sms;
+}
 template <class T, class A>
 cudaError_t run_tiles(void (*kernel)(A), const A& args, const ScoreArgs& a, int n_sms, cudaStream_t s)
 {
@@ -392,7 +409,7 @@ cudaError_t run_tiles(void (*kernel)(A), const A& args, const ScoreArgs& a, int 
 template <class T>
 cudaError_t run_score(const ScoreArgs& a, void* workspace, int n_sms, cudaStream_t s)
 {
-  if (by_tiles(a, n_sms)) return run_tiles<T>(score_tiles<T>, a, a, n_sms, s);
+  if (by_tiles(a, sizeof(T), n_sms)) return run_tiles<T>(score_tiles<T>, a, a, n_sms, s);
   int segs           = segments(a.n_rows, a.n_cols, n_sms);
   const int64_t cols = part_cols(a.n_cols, segs);
   segs               = segs == 1 ? 1 : static_cast<int>((a.n_cols + cols - 1) / cols);
@@ -417,7 +434,7 @@ template <class T>
 cudaError_t run_grad(const ScoreGradArgs& g, int n_sms, cudaStream_t s)
 {
   const ScoreArgs& a = g.fwd;
-  if (by_tiles(a, n_sms)) return run_tiles<T>(grad_tiles<T>, g, a, n_sms, s);
+  if (grad_by_tiles(a, n_sms)) return run_tiles<T>(grad_tiles<T>, g, a, n_sms, s);
   const bool warp    = by_warps(a, n_sms, sizeof(T) == 2 && a.n_cols <= kWarpLong);
   const unsigned rows = row_blocks(a, warp, sizeof(T), kGradBlocks * n_sms, kLongGradRow);
   int segs           = warp ? 1 : segments(a.n_rows, a.n_cols, n_sms);

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests.test_distill import HALF_STEP, TYPES, gen
-from tests.test_score import wide
+from tests.test_score import check, logits, targets, upstreams, wide
 
 gpu = pytest.mark.gpu
 
@@ -165,3 +165,16 @@ def test_rows_that_do_not_count_may_hold_anything(n, c, dtype):
         out.append((got.log_prob, got.entropy, *torch.autograd.grad((got.log_prob, got.entropy), x, (up[0], up[1]))))
     for a, b in zip(*out):
         assert torch.equal(a, b) and (b[~counts] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("n,c", [(9000, 13), (9000, 16), (7200, 3), (24_000, 40), (24_000, 14), (90_000, 47), (90_000, 49), (90_000, 60),
+                                 (60_000, 33)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_rows_of_few_classes_by_threads_in_one_pass_and_by_lanes_in_the_other(n, c, dtype):
+    z, t = logits(n, c, dtype), targets(n, c)
+    t[::11] = -100
+    z[5] = float("-inf")
+    g, h = upstreams(n)
+    check(z, t, 1.5, 0, g, h)
+    check(torch.nn.functional.pad(z, (1, 2))[:, 1:c + 1], t, 1.5, 0, g, h)
