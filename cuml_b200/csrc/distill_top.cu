@@ -278,29 +278,6 @@ __device__ __forceinline__ bool is_nan(const PairedStream<T>& sum)
   split_pair(sum.s, lo, hi);
   return lo != lo || hi != hi;
 }
-// A row again whose logits are not ordinary ones; joined.
-template <class T, int THREADS>
-__device__ __noinline__ Scored score_any(const T* x, int64_t n, int tid, float c, float* room)
-{
-  constexpr int N = Piece<T>::N;
-  ScoredStream r;
-  const float slack = kSlack / c;
-  visit_row<kInFlight>(
-    x, n, tid, THREADS,
-    [&](int64_t, T e) {
-      const float one[1] = {widen(e)};
-      r.take(one, c, slack);
-    },
-    [&](int64_t, const Piece<T>& p) {
-      float v[N];
-#pragma unroll
-      for (int e = 0; e < N; ++e) v[e] = widen(p.v[e]);
-      r.take(v, c, slack);
-    });
-  join_scored<THREADS>(r, c, room);
-  return r;
-}
-
 // The logarithm of s + dropped, which may be nearly 1: of its 32-bit part, and what that leaves.
 __device__ __forceinline__ float log_of_sum(float s, double dropped)
 {
@@ -469,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
     if constexpr (MODE == kScored) {
       scored = sum.scored(c);
       join_scored<kThreads>(scored, c, reinterpret_cast<float*>(room));
-      if (!sum.usable(scored.m, c)) scored = score_any<T, kThreads>(x, n, tid, c, reinterpret_cast<float*>(room));
+      if (!sum.usable(scored.m, c)) scored = visit_any<T, kThreads, kInFlight>(x, n, tid, c, reinterpret_cast<float*>(room));
     } else if (plain) {
       // (in 64 bits: see Sum)
       dropped = sum_row<kThreads>(static_cast<double>(sum.s) + sum.dropped, room);
@@ -625,17 +602,17 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 5) top_segments
             write_scored(a, row, place, key, joined_m, joined_score);
             return;
           } else {
-          write_top<T>(a, row, place, key);
-          if (place > 0) return;
-          Running<double> r;
-          for (int i = 0; i < segs; ++i) {
-            const double* from = cluster.map_shared_rank(best_sum, i);
-            if (plain)
-              r.s += from[0];
-            else
-              r.join(from[1], from[0], 1.0);
-          }
-          write_lse(a, row, static_cast<V>(r.m), static_cast<V>(plain ? 0.0 : r.s), plain ? r.s : 0.0, key);
+            write_top<T>(a, row, place, key);
+            if (place > 0) return;
+            Running<double> r;
+            for (int i = 0; i < segs; ++i) {
+              const double* from = cluster.map_shared_rank(best_sum, i);
+              if (plain)
+                r.s += from[0];
+              else
+                r.join(from[1], from[0], 1.0);
+            }
+            write_lse(a, row, static_cast<V>(r.m), static_cast<V>(plain ? 0.0 : r.s), plain ? r.s : 0.0, key);
           }
         });
       }
@@ -712,21 +689,21 @@ __global__ void __launch_bounds__(kThreads) top_join(ArgsOf<MODE> a, int segs, c
       for (int j = threadIdx.x; j < a.k; j += kThreads) write_scored(a, row, j, list[j], r.m, score);
       __syncthreads();
     } else {
-    for (int j = threadIdx.x; j < a.k; j += kThreads) write_top<T>(a, row, j, list[j]);
-    Running<double> r;
-    for (int i = threadIdx.x; i < segs; i += kThreads) {
-      const double s = sums[3 * (row * segs + i)], m = sums[3 * (row * segs + i) + 1];
+      for (int j = threadIdx.x; j < a.k; j += kThreads) write_top<T>(a, row, j, list[j]);
+      Running<double> r;
+      for (int i = threadIdx.x; i < segs; i += kThreads) {
+        const double s = sums[3 * (row * segs + i)], m = sums[3 * (row * segs + i) + 1];
+        if (plain)
+          r.s += s;
+        else
+          r.join(m, s, 1.0);
+      }
       if (plain)
-        r.s += s;
+        r.s = sum_row<kThreads>(r.s, room);
       else
-        r.join(m, s, 1.0);
-    }
-    if (plain)
-      r.s = sum_row<kThreads>(r.s, room);
-    else
-      join_row<kThreads>(r, 1.0, room);
-    if (threadIdx.x == 0) write_lse(a, row, static_cast<V>(r.m), static_cast<V>(plain ? 0.0 : r.s), plain ? r.s : 0.0, list[0]);
-    __syncthreads();
+        join_row<kThreads>(r, 1.0, room);
+      if (threadIdx.x == 0) write_lse(a, row, static_cast<V>(r.m), static_cast<V>(plain ? 0.0 : r.s), plain ? r.s : 0.0, list[0]);
+      __syncthreads();
     }
   }
 }
@@ -938,13 +915,12 @@ __global__ void __launch_bounds__(kThreads, warps_fit(U * 16 / sizeof(T) * sizeo
 // bound, as above, and what reaches it is read again; where that is more than the list holds the k-th key is found
 // bit by bit as in top_segments.  (A bound by values alone took 5.7 ms where all but five of 4096 scores of 8192 rows
 // were -inf.)
-template <class T, int MODE>
+template <class T, bool PROB>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(TopArgs a)
 {
   using V = typename ValueOf<T>::type;
   using K = typename KeyOf<T>::type;
   constexpr int N = Piece<T>::N, ROWS = kThreads / 32;
-  constexpr bool PROB = MODE == kProbabilities;
   __shared__ K lists[ROWS][kWarpList];
   __shared__ int counts[ROWS];
   const int lane = threadIdx.x % 32, k = a.k;
@@ -958,7 +934,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(Top
     // the lane's best score, the first element of the piece that holds it, and the sum
     V best      = lowest<V>();
     uint32_t at = ~0u;
-    auto sum    = new_sum<V, MODE>(c);
+    Sum<V, PROB> sum;
     visit_row<2 * kInFlight>(
       x, a.n_cols, lane, 32,
       [&](int64_t i, T e) {
@@ -991,7 +967,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 3 : 4) top_long(Top
       all.s = sum.s;
       all.join_lanes(V(1));
     }
-    if (is_nan(sum)) {  // a NaN, or infinities
+    if (sum.s != sum.s) {  // a NaN, or infinities
       const uint32_t first = first_nan(x, a.n_cols, lane, 32);
       if (first != ~0u) {
         best = static_cast<V>(NAN);
@@ -1209,7 +1185,7 @@ __global__ void __launch_bounds__(kGroupThreads, kGroupBlocks) top_groups(Scored
     const bool nan = __any_sync(~0u, is_nan(sum));  // (or an infinite one)
     Scored scored  = sum.scored(c);
     scored.join_lanes(c);
-    if (!sum.usable(scored.m, c)) scored = score_any<T, 32>(x, a.n_cols, lane, c, nullptr);
+    if (!sum.usable(scored.m, c)) scored = visit_any<T, 32, kInFlight>(x, a.n_cols, lane, c, nullptr);
     if (scored.s == 0.f) {
       write_uncounted(a, row, lane, 32);
       continue;
@@ -1305,15 +1281,15 @@ __global__ void __launch_bounds__(kTileRows) top_tiles(ArgsOf<MODE> a)
       for (int j = 0; j < TOP; ++j)
         if (j < a.k) write_scored(a, row, j, K::of(top[j], static_cast<uint32_t>(at[j])), sum.m, score);
     } else {
-    T* values         = static_cast<T*>(a.values) + row * a.k;
-    int32_t* index    = a.index + row * a.k;
+      T* values         = static_cast<T*>(a.values) + row * a.k;
+      int32_t* index    = a.index + row * a.k;
 #pragma unroll
-    for (int j = 0; j < TOP; ++j) {
-      if (j >= a.k) break;
-      values[j] = narrow<T>(PROB ? log_of(top[j]) : top[j]);
-      index[j]  = at[j];
-    }
-    write_lse(a, row, sum.r, sum.s, static_cast<double>(sum.dropped), K::of(top[0], 0u));
+      for (int j = 0; j < TOP; ++j) {
+        if (j >= a.k) break;
+        values[j] = narrow<T>(PROB ? log_of(top[j]) : top[j]);
+        index[j]  = at[j];
+      }
+      write_lse(a, row, sum.r, sum.s, static_cast<double>(sum.dropped), K::of(top[0], 0u));
     }
   }
 }
@@ -1417,7 +1393,7 @@ cudaError_t run_top(const A& a, void* workspace, int n_sms, cudaStream_t s)
     }
   } else if (bytes <= kLongBytes && a.k <= kWarpTop && a.n_rows >= static_cast<int64_t>(kLongLeast) * n_sms) {
     const int64_t need = (a.n_rows + kThreads / 32 - 1) / (kThreads / 32), most = 16ll * n_sms;
-    const auto kernel  = kernel_of(a, top_long<T, kScores>, top_long<T, kProbabilities>);
+    const auto kernel  = kernel_of(a, top_long<T, false>, top_long<T, true>);
     kernel<<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(a);
     count_launches(1);
     return cudaGetLastError();

@@ -360,6 +360,29 @@ __device__ __forceinline__ void join_scored(Scored& r, float c, float* room)
   r.join_lanes(c);
 }
 
+// A row of any logits by THREADS threads, joined for all of them; U pieces of a thread are in flight.
+template <class T, int THREADS, int U>
+__device__ __noinline__ Scored visit_any(const T* row, int64_t n, int tid, float c, float* room)
+{
+  constexpr int N = Piece<T>::N;
+  ScoredStream r;
+  const float slack = kSlack / c;
+  visit_row<U>(
+    row, n, tid, THREADS,
+    [&](int64_t, T x) {
+      const float one[1] = {widen(x)};
+      r.take(one, c, slack);
+    },
+    [&](int64_t, const Piece<T>& v) {
+      float x[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[e] = widen(v.v[e]);
+      r.take(x, c, slack);
+    });
+  join_scored<THREADS>(r, c, room);
+  return r;
+}
+
 // What is kept of a row for its gradient: m, 1 / s (0: the row does not count), -u / s and the class.
 __device__ __forceinline__ float4 kept_row(float m, float inverse, float mean, int at)
 {

@@ -67,29 +67,6 @@ __device__ __forceinline__ Scored visit_ordinary(const T* row, int n, int tid, i
     [&](int, const Piece<T>& v) { r.take(v, largest_of(v), c, slack); });
   return r.scored(c);
 }
-// The same of any logits, joined for all threads.
-template <class T, int THREADS>
-__device__ __noinline__ Scored visit_any(const T* row, int64_t n, int tid, float c, float* room)
-{
-  constexpr int N = Piece<T>::N;
-  ScoredStream r;
-  const float slack = kSlack / c;
-  visit_row<kInFlight>(
-    row, n, tid, THREADS,
-    [&](int64_t, T x) {
-      const float one[1] = {widen(x)};
-      r.take(one, c, slack);
-    },
-    [&](int64_t, const Piece<T>& v) {
-      float x[N];
-#pragma unroll
-      for (int e = 0; e < N; ++e) x[e] = widen(v.v[e]);
-      r.take(x, c, slack);
-    });
-  join_scored<THREADS>(r, c, room);
-  return r;
-}
-
 // One part of a row per block: (row, segment) -> its m, s and u, nothing for rows that do not count.  (Asking for the class first costs a
 // row's 0.5 us, of which the join gives back 0.3: 100 x 131,072 fp32, both kernels: 21.3 us with and 22.0 without reading such rows,
 // where half of them are that 21.3 and 13.4.)
@@ -105,7 +82,7 @@ __global__ void __launch_bounds__(kThreads) score_parts(ScoreArgs a, int64_t seg
     const T* x = static_cast<const T*>(a.logits) + row * a.row_stride + begin;
     Scored r   = visit_ordinary(x, n, threadIdx.x, kThreads, c);
     join_scored<kThreads>(r, c, room);
-    if (!PairedStream<T>::usable(r.m, c)) r = visit_any<T, kThreads>(x, n, threadIdx.x, c, room);
+    if (!PairedStream<T>::usable(r.m, c)) r = visit_any<T, kThreads, kInFlight>(x, n, threadIdx.x, c, room);
     if (threadIdx.x == 0) parts[row * gridDim.x + blockIdx.x] = make_float4(r.m, r.s, r.u, 0.f);
   }
 }
@@ -165,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, kRowBlocks) score_blocks(ScoreArgs a
     }
     for (unsigned again = __ballot_sync(~0u, at != -2 && !PairedStream<T>::usable(mine.m, c)); again; again &= again - 1) {
       const int j    = __ffs(again) - 1;
-      const Scored r = visit_any<T, kThreads>(logits(j), a.n_cols, threadIdx.x, c, room);
+      const Scored r = visit_any<T, kThreads, kInFlight>(logits(j), a.n_cols, threadIdx.x, c, room);
       if (lane == j) mine = r;
     }
     if (lane < count && warp == 0)
@@ -220,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, kWarpBlocks) score_rows(ScoreArgs a)
     }
     for (unsigned again = __ballot_sync(~0u, at != -2 && !PairedStream<T>::usable(mine.m, c)); again; again &= again - 1) {
       const int j    = __ffs(again) - 1;
-      const Scored r = visit_any<T, 32>(logits(j), a.n_cols, lane, c, nullptr);
+      const Scored r = visit_any<T, 32, kInFlight>(logits(j), a.n_cols, lane, c, nullptr);
       if (lane == j) mine = r;
     }
     if (rows.row(lane) < a.n_rows)
