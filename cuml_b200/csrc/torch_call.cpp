@@ -263,7 +263,8 @@ bool teacher_of(PyObject* values, PyObject* index, PyObject* lse, const Tensor& 
   if (values == Py_None) {  // one class per row
     if (!THPVariable_Check(index)) return false;
     t.index = THPVariable_Unpack(index);
-    if (t.index.dim() != 1 || !t.index.is_cuda() || t.index.layout() != at::kStrided || at::isTensorSubclassLike(t.index))
+    if (t.index.dim() != 1 || !t.index.is_cuda() || t.index.layout() != at::kStrided || at::isTensorSubclassLike(t.index) ||
+        t.index.is_neg())
       return false;
     t.index = t.index.unsqueeze(1);
   } else {
@@ -284,7 +285,7 @@ bool teacher_of(PyObject* values, PyObject* index, PyObject* lse, const Tensor& 
     t.logsumexp = THPVariable_Unpack(lse);
     if (!t.logsumexp.is_cuda() || t.logsumexp.layout() != at::kStrided || type_of(t.logsumexp) < 0 ||
         t.logsumexp.dim() != 1 || t.logsumexp.size(0) != n || (n > 1 && t.logsumexp.stride(0) != 1) ||
-        at::isTensorSubclassLike(t.logsumexp) || !on(t.logsumexp, like))
+        at::isTensorSubclassLike(t.logsumexp) || t.logsumexp.is_neg() || !on(t.logsumexp, like))
       return false;
     t.logsumexp = as_floats(t.logsumexp);
   }
@@ -330,17 +331,20 @@ struct Saved {
   }
 };
 // Rows one after the other: what hooks return may lie in another order.
-Tensor in_rows(const Tensor& x)
+Tensor in_rows(const Tensor& given)
 {
+  const Tensor x = given.resolve_neg();
   const bool as_saved = (x.stride(1) == 1 || x.size(1) == 1) && (x.stride(0) >= x.size(1) || x.size(0) == 1);
   return as_saved ? x : x.contiguous();
 }
 
-// What a node's gradient is by the loss: 32-bit values, and elements from one row's to the next.
+// What a node's gradient is by the loss: 32-bit values, and elements from one row's to the next.  (The gradient of a part of a
+// conjugate may be a view whose numbers are the negatives of those in memory.)
 Tensor upstream_of(const Tensor& g, int64_t& stride)
 {
-  stride = g.dim() ? g.stride(0) : 0;
-  return g.scalar_type() == at::kFloat ? g : g.to(at::kFloat);
+  const Tensor x = g.scalar_type() == at::kFloat ? g.resolve_neg() : g.to(at::kFloat);
+  stride         = x.dim() ? x.stride(0) : 0;
+  return x;
 }
 [[noreturn]] void raise_library_error(const LibraryError& e)
 {
@@ -605,7 +609,7 @@ bool target_of(PyObject* o, const Tensor& like, int64_t ignore, Tensor& index, b
   if (o == Py_None) return true;
   if (!THPVariable_Check(o)) return false;
   index = THPVariable_Unpack(o);
-  if (index.dim() != 1 || !index.is_cuda() || index.layout() != at::kStrided || at::isTensorSubclassLike(index) ||
+  if (index.dim() != 1 || !index.is_cuda() || index.layout() != at::kStrided || at::isTensorSubclassLike(index) || index.is_neg() ||
       (index.scalar_type() != at::kInt && index.scalar_type() != at::kLong) || index.size(0) != like.size(0) || !on(index, like))
     return false;
   t.index   = index.const_data_ptr();

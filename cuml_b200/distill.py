@@ -120,7 +120,8 @@ def _cuda(name, x, dtypes, ndim=None):
 
 
 def _rows(x):
-    """`x` with unit stride within its rows and rows that do not overlap."""
+    """`x` with unit stride within its rows and rows that do not overlap, its numbers as they lie in memory."""
+    x = x.resolve_neg()
     if x.stride(1) != 1 and x.shape[1] > 1 or x.stride(0) < x.shape[1] and x.shape[0] > 1:
         x = x.contiguous()
     return x
@@ -218,7 +219,7 @@ def _top(top, n, dev, tail):
         _cuda("the teacher's logsumexp", lse, _TYPES)
         if lse.numel() != n:
             raise ValueError(f"the teacher's logsumexp has {lse.numel()} rows, the student {n}")
-        lse = lse.detach().reshape(-1).float().contiguous()
+        lse = lse.detach().reshape(-1).float().resolve_neg().contiguous()
     else:
         lse = None
     for t in (values, index, lse):
@@ -236,7 +237,7 @@ def _saved(x, like):
 
 def _upstream(g):
     """(fp32 gradient by the loss, elements from one row's to the next)."""
-    g = g if g.dtype == torch.float32 else g.float()
+    g = g.resolve_neg() if g.dtype == torch.float32 else g.float()  # (the gradient of a part of a conjugate may be a negative view)
     return g, (g.stride(0) if g.ndim else 0)
 
 
@@ -370,7 +371,7 @@ def _target(target, shape, dev):
         raise ValueError(f"target must have shape {tuple(shape)}, got {tuple(target.shape)}")
     if target.device != dev:
         raise ValueError(f"target is on {target.device}, the student on {dev}")
-    return target.reshape(-1)
+    return target.reshape(-1).resolve_neg()
 
 
 class _Linear(torch.autograd.Function):
@@ -707,6 +708,9 @@ def _clip(gradients, most, norm_type, out, scales):
                 raise ValueError(f"a gradient and its out differ in shape: {tuple(x.shape)}, {tuple(to.shape)}")
             if to.requires_grad:
                 raise ValueError("a tensor of out requires grad")
+            if to.is_neg():
+                raise ValueError("a tensor of out is a negative view")
+            x = x.resolve_neg()
         if x.layout != torch.strided or to.layout != torch.strided:
             raise ValueError("gradients must be strided tensors")
         if scales and _overlaps_itself(to):

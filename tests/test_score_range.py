@@ -230,3 +230,60 @@ def test_sums_of_a_layer_are_not_cut_short_over_their_whole_length(dtype, border
     want = scores_of_layer(h, w, t)[0]
     off = wide(got) - want
     assert float(off.norm() / want.norm()) < border
+
+
+@gpu
+@pytest.mark.parametrize("compiled", [True, False])
+def test_views_of_the_negatives_of_what_lies_in_memory(monkeypatch, compiled):
+    """Gradients that come from a part of a conjugate, and inputs that are such views, have the other sign than their memory."""
+    from cuml_b200 import distill
+
+    if not compiled:
+        monkeypatch.setattr(distill, "_call", False)
+    n, c = 40, 300
+    z, t = logits(n, c, "fp32"), targets(n, c)
+    h, w = layer(n, 64, c, "bf16")
+    a, b = upstreams(n)
+    teacher = distill.log_probs(logits(n, c, "fp32", 3), top=5).top
+    both = [(distill.log_probs, (z,), (t,)), (distill.linear_log_probs, (h, w), (t,))]
+    one = [(distill.cross_entropy, (z,), (t,)), (distill.distillation_loss, (z,), (teacher,)), (distill.linear_cross_entropy, (h, w), (t,)),
+           (distill.linear_distillation_loss, (h, w), (teacher,))]
+    for f, leaves, rest in both + one:
+        leaves = [x.detach().requires_grad_() for x in leaves]
+
+        def run(*args):
+            out = f(*args) if f in (distill.log_probs, distill.linear_log_probs) else (f(*args, reduction="none"),)
+            return out[0], out[1] if len(out) > 1 else out[0] * 0
+
+        x, y = run(*leaves, *rest)
+        want = torch.autograd.grad((x, y), leaves, (a, b))
+        x, y = run(*leaves, *rest)
+        seen = []
+        x.register_hook(lambda g: seen.append(g.is_neg()))
+        y.register_hook(lambda g: seen.append(g.is_neg()))
+        got = torch.autograd.grad(torch.complex(x, y).conj().mul(torch.complex(a, b)).real.sum(), leaves)
+        assert any(seen) and all(torch.equal(p, q) for p, q in zip(want, got))
+        negative = [torch._neg_view(-p.detach()).requires_grad_() for p in leaves]
+        flipped = [torch._neg_view(-p) if isinstance(p, torch.Tensor) else
+                   type(p)(*(q if q is None else torch._neg_view(-q) for q in p)) for p in rest]
+        x2, y2 = run(*negative, *flipped)
+        assert torch.equal(x, x2) and torch.equal(y, y2)
+        for p, q in zip(want, torch.autograd.grad((x2, y2), negative, (torch._neg_view(-a), torch._neg_view(-b)))):
+            assert torch.equal(p, q)
+    assert torch.equal(distill.top_scores(z, 3).values, distill.top_scores(torch._neg_view(-z), 3).values)
+    tail = distill.top_scores(z, 3)
+    odd = distill.TopScores(tail.values, tail.index, torch._neg_view(-tail.logsumexp))
+    other = logits(n, c, "fp32", 4)
+    assert torch.equal(*(distill.distillation_loss(other, x, tail="bucket") for x in (tail, odd)))
+    # gradients
+    x = torch._neg_view(-z)
+    norm = distill.gradient_norm([z])
+    assert torch.equal(distill.gradient_norm([x]), norm)
+    plain, out = z.clone(), torch.empty_like(z)
+    distill.clip_gradients([plain], 1.0)
+    distill.clip_gradients([x], 1.0, out=[out])
+    assert torch.equal(out, plain)
+    distill.clip_gradients([x], 1.0)
+    assert x.is_neg() and torch.equal(x, plain)
+    with pytest.raises(ValueError, match="negative view"):
+        distill.clip_gradients([z], 1.0, out=[torch._neg_view(torch.empty_like(z))])
