@@ -22,7 +22,7 @@
 //
 // The same kernels give a row's scores (score_common.cuh) with its best classes, of which the log probabilities are then
 // written: kScored.  (With a pass of its own for the scores 4096 x 32,768 bf16, k 8, took
-// 138 us, now 72; 1 x 50,001 fp32, k 20, 23.5 and 10.3; 1,000,003 x 10 fp32, k 3, 467 and 33.)
+// 138 us, now 74; 1 x 50,001 fp32, k 20, 23.5 and 10.3; 1,000,003 x 10 fp32, k 3, 467 and 33.)
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -45,10 +45,13 @@ constexpr int kWarpTop  = 24;    // k up to which a warp finds its bound by its 
 // 1184 x 4096 bf16 14.8 and 12.8, x 8192 14.7 and 16.8.)
 constexpr int kLongBytes = 16384;
 constexpr int kLongLeast = 8;
-// Bytes of scored rows that a warp takes by groups, from kLongLeast rows per SM on, and twice that from twice as many on.  (By blocks and
-// this way, us: 20,000 x 3000 bf16 196 and 53, 4096 x 4096 fp32 43 and 23, 4096 x 8192 fp32 53 and 39, 4096 x 16,384 bf16 54 and 41, x
-// 32,768 78 and 75, 1300 x 16,384 22 and 26, x 8192 18 and 16.)
+// Bytes of scored rows that a warp takes by groups where there are kLongLeast rows per SM, as many times that as there are more of them, and at
+// most kGroupMost.  (us of a call, k 8, by blocks and this way: 20,000 x 3000 bf16 204 and 53, 4096 x 4096 fp32 44 and 23, 4096 x 16,384 bf16 57
+// and 43, x 20,001 72 and 55, x 32,768 82 and 85 (one after the other 74 and 68; k 24 88 and 98), 8192 x 32,768 156 and 147, x 50,001 217 and
+// 213, k 24 242 and 257, 8192 x 12,000 fp32 145 and 100, 20,000 x 40,000 bf16 465 and 377, 1300 x 16,384 22 and 26, x 8192 17 and 16, 2600 x
+// 32,768 59 and 66.)
 constexpr int64_t kGroupBytes = 16384;
+constexpr int64_t kGroupMost  = 6 * kGroupBytes;
 constexpr int kCount    = 160;   // candidates of a block that are placed by counting; more are sorted
 constexpr int kCluster  = 8;     // blocks that share a row of up to kJoinCols and join their lists themselves
 constexpr int64_t kJoinCols = 1 << 17;  // (1 x 50,001, k 20: 13.8 us by two kernels, 10.7 this way, 14.2 by 16 blocks)
@@ -1353,8 +1356,8 @@ cudaError_t run_warps(const A& a, int n_sms, cudaStream_t s)
 // Scored rows by a warp each.
 bool by_groups(int64_t n_rows, int64_t n_cols, int k, int element, int n_sms)
 {
-  const int64_t bytes = n_cols * element, per = n_rows / n_sms;
-  return n_cols > kWarpCols && k <= kWarpTop && ((bytes <= kGroupBytes && per >= kLongLeast) || (bytes <= 2 * kGroupBytes && per >= 2 * kLongLeast));
+  const int64_t per = n_rows / n_sms, most = std::min(kGroupBytes * per / kLongLeast, kGroupMost);
+  return n_cols > kWarpCols && k <= kWarpTop && per >= kLongLeast && n_cols * element <= most;
 }
 
 template <class T, class A>

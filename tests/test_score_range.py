@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+from tests import score_reference as ref
 from tests.test_distill import HALF_STEP, S, TYPES, U, check_values, gen
 from tests.test_score import adds, check, entropy_error, layer, logits, targets, upstreams, wide
 
@@ -287,3 +288,34 @@ def test_views_of_the_negatives_of_what_lies_in_memory(monkeypatch, compiled):
     assert x.is_neg() and torch.equal(x, plain)
     with pytest.raises(ValueError, match="negative view"):
         distill.clip_gradients([z], 1.0, out=[torch._neg_view(torch.empty_like(z))])
+
+
+@gpu
+@pytest.mark.parametrize("n,c,dtype", [(2500, 16_500, "bf16"), (3000, 20_001, "bf16"), (2500, 8200, "fp32"), (5000, 16_500, "fp32"),
+                                       (10_000, 33_001, "fp16")])
+@pytest.mark.parametrize("k", [1, 8, 24])
+def test_best_of_many_long_rows(n, c, dtype, k):
+    """As many rows as let a warp take long ones: the same rows few at a time, which are shared by blocks, and some against 64 bits.  The
+    largest logit is many times there, at the row's ends among them."""
+    from cuml_b200 import distill
+
+    z, t = logits(n, c, dtype), targets(n, c)
+    z[::7, ::97] = 11.0
+    z[3::7, -2:] = z[3::7, :1] = 12.5
+    z[5::50, 40:] = float("-inf")
+    t[::9] = -100
+    got = distill.log_probs(z, t, top=k)
+    for first in (0, n // 3, n - 250):
+        rows = slice(first, first + 250)
+        few = distill.log_probs(z[rows].clone(), t[rows].clone(), top=k)
+        assert torch.equal(got.top.index[rows], few.top.index)
+        check_values(got.log_prob[rows], wide(few.log_prob), 8 * U, 2 * S, 2 * U)
+        check_values(got.entropy[rows], wide(few.entropy), 8 * U, 2 * entropy_error(c), 2 * U)
+        check_values(got.top.values[rows], wide(few.top.values), 8 * U, 2 * S, 2 * U)
+    some = torch.arange(0, n, n // 30, device="cuda")
+    log_prob, entropy, log_q, _, counts = ref.scores(z[some], t[some])
+    values, index = ref.top(z[some], k, counts, log_q)
+    assert torch.equal(got.top.index[some].cpu(), index)
+    check_values(got.top.values[some], values, 4 * U, S, U)
+    check_values(got.log_prob[some], log_prob, 4 * U, S, U)
+    check_values(got.entropy[some], entropy, 4 * U, entropy_error(c), U)
