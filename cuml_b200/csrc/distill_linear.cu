@@ -62,8 +62,8 @@ constexpr int kFewNamed = 4;
 constexpr int kScaleBlocks = 8;
 // Stages whose sums stay in TMEM before the epilogue adds them up, where the logits themselves are the answer (kScoreStats): the tensor
 // cores cut each addition short, which over 2048 terms takes 1.5e-6 off a logit, and its log q and entropy with it.  (2-norm of log q's
-// error over log q's, 4096 x 2048 x 2 fp16: 2.3e-6 in one sum, 8.4e-7 this way, 6.0e-7 with 8, 6.8e-7 by sums of 32 bits without tensor
-// cores.  4096 x 2048 x 16,384: 150 us with one sum and this way, 163 with 8, which the epilogue does not clear in time.)
+// error over log q's, 4096 x 2048 x 2 fp16 through them: 2.3e-6 in one sum, 8.4e-7 this way, 6.0e-7 with 8, 6.8e-7 by sums of 32 bits
+// without tensor cores; where all products have one sign, x 300: 1.1e-5 in one sum, 3.8e-6 this way.  4096 x 2048 x 16,384: 150 us with one sum and this way, 163 with 8, which the epilogue does not clear in time.)
 constexpr int kSumStages = 12;
 
 __device__ int g_status;

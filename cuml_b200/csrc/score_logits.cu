@@ -23,7 +23,7 @@ constexpr int kMostSegs = 64;
 constexpr int kInFlight = 4;     // pieces of a thread
 // Blocks of an SM, all there at once: of rows by blocks, rows by warps and gradients.  (4096 x 131,072 bf16, 164 us at memory's
 // rate: the reading alone takes 186 us with four, 172 with five.)  Their rows lie next to one another at any time (60,000 x 1001 bf16,
-// both passes: 42 and 58 us; 50 and 64 where each had rows of its own).
+// both passes: 41 and 44 us; 72 and 73 where a warp has 32 rows in a row).
 constexpr int kRowBlocks  = 5;
 constexpr int kWarpBlocks = 4;
 constexpr int kGradBlocks = 4;

@@ -333,7 +333,7 @@ struct Saved {
 // Rows one after the other: what hooks return may lie in another order.
 Tensor in_rows(const Tensor& given)
 {
-  const Tensor x = given.resolve_neg();
+  const Tensor x = given.is_neg() ? given.resolve_neg() : given;  // (the call by itself would cost 0.5 us of a step)
   const bool as_saved = (x.stride(1) == 1 || x.size(1) == 1) && (x.stride(0) >= x.size(1) || x.size(0) == 1);
   return as_saved ? x : x.contiguous();
 }
@@ -342,7 +342,7 @@ Tensor in_rows(const Tensor& given)
 // conjugate may be a view whose numbers are the negatives of those in memory.)
 Tensor upstream_of(const Tensor& g, int64_t& stride)
 {
-  const Tensor x = g.scalar_type() == at::kFloat ? g.resolve_neg() : g.to(at::kFloat);
+  const Tensor x = g.scalar_type() != at::kFloat ? g.to(at::kFloat) : g.is_neg() ? g.resolve_neg() : g;
   stride         = x.dim() ? x.stride(0) : 0;
   return x;
 }
