@@ -747,7 +747,8 @@ def gradient_norm(gradients, *, norm_type: float = 2.0) -> torch.Tensor:
 
 
 def clip_gradients(gradients, max_norm: float, *, norm_type: float = 2.0, out=None) -> torch.Tensor:
-    """Scale `gradients` by min(1, max_norm / norm), in place, and return their norm before that (`gradient_norm`).
+    """Scale `gradients` by min(1, max_norm / norm), in place, and return their norm before that (`gradient_norm`, but for its
+    last bit where `out` lies in another order and sums are taken in parts that go by both).
 
     out : a tensor for each gradient, of its shape and of any of the types, which takes the scaled one instead (where a gradient
         is None: anything).
