@@ -63,7 +63,8 @@ constexpr int kScaleBlocks = 8;
 // Stages whose sums stay in TMEM before the epilogue adds them up, where the logits themselves are the answer (kScoreStats): the tensor
 // cores cut each addition short, which over 2048 terms takes 1.5e-6 off a logit, and its log q and entropy with it.  (2-norm of log q's
 // error over log q's, 4096 x 2048 x 2 fp16 through them: 2.3e-6 in one sum, 8.4e-7 this way, 6.0e-7 with 8, 6.8e-7 by sums of 32 bits
-// without tensor cores; where all products have one sign, x 300: 1.1e-5 in one sum, 3.8e-6 this way.  4096 x 2048 x 16,384: 150 us with one sum and this way, 163 with 8, which the epilogue does not clear in time.)
+// without tensor cores; where all products have one sign, x 300: 1.1e-5 in one sum, 3.8e-6 this way.  4096 x 2048 x 16,384: 150 us with one
+// sum and this way, 163 with 8, which the epilogue does not clear in time.)
 constexpr int kSumStages = 12;
 
 __device__ int g_status;
@@ -931,7 +932,7 @@ __global__ void __cluster_dims__(kScaleBlocks, 1, 1) __launch_bounds__(1024) gra
 }
 
 // The same for the gradients by a row's two scores: a difference is at most |g| + 6 |h| (of a class of probability q, |log q + H| q <=
-// q (1 - q) log n_cols + 1), and where a low temperature makes a class's logit that of the whole row (power_within) |g| + |h| log n_cols,
+// q (1 - q) log n_cols + 1), and where a low temperature gives a class all of its row (at_most) |g| + |h| log n_cols,
 // which is less than three times |g| + 8 |h|: kHalfScale leaves four.  scale[1] is what brings |g| + 8 |h| below 1.
 __global__ void __cluster_dims__(kScaleBlocks, 1, 1) __launch_bounds__(1024) score_scales(ScoreUpstream up, const float4* kept, int64_t n_rows, float* scale)
 {
